@@ -59,7 +59,8 @@ enum fa_error {
     FA_ERR_LAUNCH = 5,       /* kernel launch failed (cudaGetLastError) */
     FA_ERR_PLAN_SIZE = 6,    /* plan buffer too small / missing for FA_MODE1_DOC, or workspace of a split forward */
     FA_ERR_NO_DRIVER = 7,    /* cuTensorMapEncodeTiled could not be resolved */
-    FA_ERR_SCRATCH_LIMIT = 8 /* fa_fwd_static_plan: the plan does not fit in FA_STATIC_PLAN_BYTES */
+    FA_ERR_SCRATCH_LIMIT = 8, /* fa_fwd_static_plan: the plan does not fit in FA_STATIC_PLAN_BYTES */
+    FA_ERR_SCORES = 9        /* fa_scores: softcap neither 0 nor within 1e-6 .. 1e6, or a prefix without a causal mask */
 };
 
 typedef struct fa_problem {
@@ -161,6 +162,28 @@ int fa_bwd_dq(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const
 int fa_bwd(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
            const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk,
            const fa_tensor* dv, const void* plan, int32_t* status, void* stream);
+
+/* attention_scored: what is done to a scaled score s_ij = sm_scale q_i . k_j before the softmax (no counterpart in the reference):
+ *   x_ij = softcap * tanh(s_ij / softcap) - slopes[h] * |i + gap - j|,   gap = max(0, N - M);
+ * and, with a causal mask, prefix[b] leading keys that it leaves visible to every query of sequence b (values are taken into [0, N]; the
+ * ids' rule holds for those keys as for the others). softcap 0, slopes NULL, prefix NULL: without that part. There are no gradients for
+ * the three. */
+typedef struct fa_scores {
+    float softcap;         /* 0, or 1e-6 .. 1e6 */
+    const float* slopes;   /* [H], device */
+    const int32_t* prefix; /* [B], device; needs p->causal */
+} fa_scores;
+
+/* fa_plan_build, fa_fwd_split (splits = 1: fa_fwd) and fa_bwd of a call with such scores: the same arguments and rules. The plan of a call
+ * with ids must have been built with the same prefix; without ids fa_plan_build's will do. With M <= 64 and no ids the heads of a group share
+ * tiles and fa_fwd_splits says into how many runs the keys are best cut, as for fa_fwd_split. */
+int fa_plan_build_scored(const fa_problem* p, const fa_scores* scores, const fa_ids* eq, const fa_ids* ek, void* plan, size_t plan_bytes,
+                         int32_t* status, void* stream);
+int fa_fwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
+                  float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+int fa_bwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
+                  const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv,
+                  const void* plan, int32_t* status, void* stream);
 
 /* Debug: materialise the kernels' decisions. keep is [B, id_heads, M, N] bytes (1 = unmasked),
  * produced by the same device predicate the attention kernels use; tile_class is

@@ -1,0 +1,284 @@
+"""attention_scored against the plain computation in 64 bits, element by element within bounds derived from the roundings (scored_reference.py)."""
+import itertools
+
+import pytest
+import torch
+
+from scored_reference import attention_64
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _inputs(B, H, Hk, M, N, D, dtype, seed, std=1.5, layout="bhld"):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def tensor(h, n, s):
+        x = torch.randn((B, h, n, D) if layout == "bhld" else (B, n, h, D), generator=gen, device="cuda") * s
+        return (x if layout == "bhld" else x.transpose(1, 2)).to(dtype)
+
+    return tensor(H, M, std), tensor(Hk, N, std), tensor(Hk, N, 1.0), tensor(H, M, 1.0)
+
+
+def _slopes(H, kind):
+    if kind is None:
+        return None
+    if kind == "series":
+        return torch.tensor([2.0 ** (-8 * (h + 1) / H) for h in range(H)], device="cuda")
+    if kind == "mixed":  # zero, negative and steep ones
+        return torch.tensor([(0.0, -0.01, 3.0, 0.2)[h % 4] for h in range(H)], device="cuda")
+    return torch.full((H,), float(kind), device="cuda")
+
+
+def _docs(B, H, L, seed, per_head=False):
+    gen = torch.Generator().manual_seed(seed)
+    rows = []
+    for _ in range(B * (H if per_head else 1)):
+        cuts = torch.sort(torch.randint(1, max(2, L), (3,), generator=gen)).values
+        ids = -1 - torch.searchsorted(cuts, torch.arange(L), right=True)
+        ids[torch.rand(L, generator=gen) < 0.03] = 5
+        rows.append(ids)
+    ids = torch.stack(rows).reshape(B, -1, L).cuda()
+    return ids.expand(B, H, L)
+
+
+def _check(got, want, what):
+    value, bound = want
+    off = (got.double() - value).abs()
+    assert torch.isfinite(got).all(), what
+    worst = (off / bound).max().item()
+    assert worst <= 1, f"{what}: {worst:.2f} times its bound, at most {off.max().item():.3g} off"
+
+
+def _run(fb, q, k, v, do, causal, eq=None, ek=None, cap=None, slopes=None, prefix=None, sm_scale=None):
+    a, b, c = (x.detach().requires_grad_() for x in (q, k, v))
+    o = fb.attention_scored(a, b, c, causal, sm_scale, eq, ek, 0 if eq is None else 1, softcap=cap, slopes=slopes, prefix=prefix)
+    grads = torch.autograd.grad(o, (a, b, c), do)
+    with torch.no_grad():
+        assert torch.equal(o, fb.attention_scored(q, k, v, causal, sm_scale, eq, ek, 0 if eq is None else 1, softcap=cap, slopes=slopes, prefix=prefix))
+    fb.check_status()
+    return dict(zip(("o", "dq", "dk", "dv"), (o.detach(), *grads)))
+
+
+def _compare(q, k, v, do, causal, **kw):
+    import flash_b200 as fb
+    got = _run(fb, q, k, v, do, causal, **kw)
+    want = attention_64(q, k, v, do, causal, kw.get("sm_scale"), kw.get("eq"), kw.get("ek"), kw.get("cap"), kw.get("slopes"), kw.get("prefix"))
+    for name in ("o", "dq", "dk", "dv"):
+        _check(got[name], want[name], name)
+    return got, want
+
+
+# (B, H, Hk, M, N, D): one token, tiles that end inside, more keys than queries, grouped heads, few queries (packed heads, runs of keys)
+SHAPES = [(1, 1, 1, 1, 1, 64), (2, 2, 1, 129, 129, 128), (1, 4, 2, 200, 333, 64), (2, 8, 2, 1, 700, 128), (1, 4, 1, 30, 2500, 64), (1, 3, 1, 100, 1300, 128),
+          (1, 2, 2, 257, 300, 32), (2, 4, 4, 96, 96, 16), (1, 2, 1, 640, 640, 128)]
+CHANGES = [dict(cap=20.0), dict(slopes="series"), dict(cap=5.0, slopes="mixed")]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("change", CHANGES, ids=["cap", "bias", "both"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_shapes(shape, change, causal, dtype):
+    B, H, Hk, M, N, D = shape
+    q, k, v, do = _inputs(*shape, dtype, 7)
+    _compare(q, k, v, do, causal, cap=change.get("cap"), slopes=_slopes(H, change.get("slopes")))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("prefix,kind", [((0, 300), torch.int32), ((-5, 1000), torch.int32), ((130, 1 << 40), torch.int64), ((1, 127), torch.int64)])
+@pytest.mark.parametrize("D,M,N", [(64, 300, 300), (128, 140, 420), (32, 5, 300)])
+def test_prefix(D, M, N, prefix, kind, dtype):
+    q, k, v, do = _inputs(2, 4, 2, M, N, D, dtype, 8)
+    p = torch.tensor(prefix, dtype=kind, device="cuda")
+    _compare(q, k, v, do, True, prefix=p)
+    _compare(q, k, v, do, True, prefix=p, cap=10.0, slopes=_slopes(4, "mixed"))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("per_head", [False, True])
+@pytest.mark.parametrize("causal,prefix", [(True, None), (False, None), (True, (90, 300))])
+def test_documents(causal, prefix, per_head, dtype):
+    B, H, Hk, L, D = 2, 4, 2, 390, 64
+    q, k, v, do = _inputs(B, H, Hk, L, L, D, dtype, 9)
+    ids = _docs(B, H, L, 10, per_head)
+    prefix = None if prefix is None else torch.tensor(prefix, dtype=torch.int32, device="cuda")
+    for cap, slopes in ((15.0, None), (None, "series"), (6.0, "mixed")):
+        _compare(q, k, v, do, causal, eq=ids, ek=ids, cap=cap, slopes=_slopes(H, slopes), prefix=prefix)
+
+
+def test_documents_over_many_blocks():
+    """The plan of long id rows, built by three kernels, and queries of scattered documents without a causal mask."""
+    B, H, L, D = 1, 2, 4700, 64
+    q, k, v, do = _inputs(B, H, 1, L, L, D, BF16, 11)
+    ids = _docs(B, H, L, 12)
+    _compare(q, k, v, do, True, eq=ids, ek=ids, cap=20.0, slopes=_slopes(H, "series"), prefix=torch.tensor([1500], dtype=torch.int32, device="cuda"))
+    scattered = ids[:, :1, torch.randperm(L, device="cuda")].expand(B, H, L)
+    _compare(q, k, v, do, False, eq=scattered, ek=ids, cap=20.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_without_a_key(causal, dtype):
+    import flash_b200 as fb
+    q, k, v, do = _inputs(2, 2, 2, 260, 260, 64, dtype, 13)
+    eq = torch.full((2, 1, 260), -1, device="cuda")
+    ek = torch.full((2, 1, 260), -1, device="cuda")
+    eq[0, 0, 100:180] = -9  # nobody's
+    ek[1] = -2              # a whole sequence without keys
+    eq, ek = eq.expand(2, 2, 260), ek.expand(2, 2, 260)
+    got, want = _compare(q, k, v, do, causal, eq=eq, ek=ek, cap=10.0, slopes=_slopes(2, "series"))
+    empty = ~want["keep"].any(-1)[:, 0]
+    assert empty[0, 100:180].all() and empty[1].all()
+    for b in range(2):
+        assert (got["o"][b][:, empty[b]] == 0).all() and (got["dq"][b][:, empty[b]] == 0).all()
+    assert (got["dk"][1] == 0).all() and (got["dv"][1] == 0).all()
+
+
+@pytest.mark.parametrize("cap", [1e-6, 0.5, 1.0, 300.0, 1e6])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_caps_of_every_size(cap, dtype):
+    """Scores on both sides of the cap, within one call: both forms of the tanh, also next to each other."""
+    q, k, v, do = _inputs(1, 2, 2, 200, 200, 64, dtype, 14)
+    q[:, :, 50:60] *= 8
+    q[:, :, 100:150] *= 0.01
+    _compare(q, k, v, do, True, cap=cap)
+
+
+def test_scores_that_are_not_finite_in_the_type_of_the_inputs():
+    """fp16 products beyond 65504, capped."""
+    q, k, v, do = _inputs(1, 2, 2, 150, 150, 64, FP16, 15, std=60.0)
+    _compare(q, k, v, do, True, cap=30.0)
+
+
+def test_strides_and_scale():
+    q, k, v, do = _inputs(2, 4, 2, 190, 190, 64, BF16, 16, layout="blhd")
+    _compare(q, k, v, do, True, cap=8.0, slopes=_slopes(4, "series"), sm_scale=0.3)
+    wide = torch.randn(2, 190, 4, 3, 67, device="cuda", dtype=BF16)[..., 1:65]  # nothing that a tensor map takes
+    a, b, c = (wide[:, :, :, i].transpose(1, 2) for i in range(3))
+    _compare(a, b, c, do[:, :, :, torch.arange(64, device="cuda").flip(0)].transpose(2, 3).contiguous().transpose(2, 3), True, cap=8.0)
+    slopes = torch.rand(8, device="cuda")[::2]
+    prefix = torch.tensor([[7, 0], [100, 0]], dtype=torch.int32, device="cuda")[:, 0]
+    _compare(q, k, v, do, True, slopes=slopes, prefix=prefix)
+    _compare(q, k, v, do[:, :, :1].expand(2, 4, 190, 64), True, slopes=slopes)  # a broadcast gradient
+
+
+def test_without_changes_it_is_attention():
+    import flash_b200 as fb
+    q, k, v, do = _inputs(1, 4, 2, 300, 300, 64, BF16, 17)
+    for softcap in (None, 0, 0.0):
+        assert torch.equal(fb.attention_scored(q, k, v, True, softcap=softcap), fb.attention(q, k, v, True))
+    # nothing but zeros in the changes: the same function by the other instances
+    zero = fb.attention_scored(q, k, v, True, slopes=torch.zeros(4, device="cuda"), prefix=torch.zeros(1, dtype=torch.int32, device="cuda"))
+    want = attention_64(q, k, v, do, True, None, None, None, None, None, None)
+    _check(zero, want["o"], "o")
+
+
+def test_gradients_against_differences():
+    """A directional derivative of sum(o * do) by central differences of the fp32 kernels' forward. With a step of h the difference is off by h^2 / 6 of
+    the third derivative and by the forward's rounding over h: with h = 2^-6 some 1e-3 and 1e-4 of the derivative's size here; 5e-3 is asked for."""
+    import flash_b200 as fb
+    q, k, v, do = _inputs(1, 2, 1, 70, 90, 32, FP32, 18, std=0.7)
+    kw = dict(cap=2.0, slopes=_slopes(2, "series"), prefix=torch.tensor([40], dtype=torch.int32, device="cuda"))
+    got = _run(fb, q, k, v, do, True, **kw)
+    for i, name in enumerate(("dq", "dk", "dv")):
+        x = [q, k, v]
+        way = got[name] / got[name].norm()  # the steepest one
+        h = 2.0 ** -6
+        ends = []
+        for sign in (1, -1):
+            y = list(x)
+            y[i] = x[i] + sign * h * way
+            ends.append((fb.attention_scored(*y, True, softcap=2.0, slopes=kw["slopes"], prefix=kw["prefix"]).double() * do.double()).sum())
+        assert abs((ends[0] - ends[1]) / (2 * h) / got[name].double().norm() - 1) < 5e-3, name
+
+
+def test_captured_forward_and_backward_on_new_values():
+    import flash_b200 as fb
+    q, k, v, do = _inputs(2, 4, 2, 300, 300, 128, BF16, 19)
+    ids = _docs(2, 4, 300, 20)
+    slopes, prefix = _slopes(4, "series"), torch.tensor([20, 200], dtype=torch.int32, device="cuda")
+    call = dict(eq=ids, ek=ids, cap=10.0, slopes=slopes, prefix=prefix)
+    _run(fb, q, k, v, do, True, **call)
+    a, b, c = (x.detach().clone().requires_grad_() for x in (q, k, v))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        o = fb.attention_scored(a, b, c, True, None, ids, ids, 1, softcap=10.0, slopes=slopes, prefix=prefix)
+        grads = torch.autograd.grad(o, (a, b, c), do)
+    q2, k2, v2, do2 = _inputs(2, 4, 2, 300, 300, 128, BF16, 21)
+    with torch.no_grad():
+        for x, y in ((a, q2), (b, k2), (c, v2)):
+            x.copy_(y)
+    do.copy_(do2)
+    prefix.copy_(torch.tensor([150, 3]))
+    slopes.mul_(0.5)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    want = _run(fb, q2, k2, v2, do2, True, **call)
+    for got, name in zip((o, *grads), ("o", "dq", "dk", "dv")):
+        assert torch.equal(got, want[name]), name
+
+
+def test_two_streams_at_once():
+    import flash_b200 as fb
+    sets = [_inputs(1, 8, 8, 900, 900, 64, BF16, 30 + i) for i in range(2)]
+    want = [_run(fb, *s, True, cap=10.0 + i) for i, s in enumerate(sets)]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for i, (s, st) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(st):
+                a, b, c = (x.detach().requires_grad_() for x in s[:3])
+                o = fb.attention_scored(a, b, c, True, softcap=10.0 + i)
+                got.append((i, (o.detach(), *torch.autograd.grad(o, (a, b, c), s[3]))))
+    torch.cuda.synchronize()
+    for i, outs in got:
+        for x, name in zip(outs, ("o", "dq", "dk", "dv")):
+            assert torch.equal(x, want[i][name])
+
+
+def test_tiles_skipped_or_not_give_the_same(monkeypatch):
+    """The environment's switches walk every tile and evaluate every mask entry by entry."""
+    import flash_b200 as fb
+    q, k, v, do = _inputs(1, 2, 1, 520, 520, 64, BF16, 22)
+    ids = _docs(1, 2, 520, 23)
+    kw = dict(eq=ids, ek=ids, cap=10.0, slopes=_slopes(2, "series"), prefix=torch.tensor([140], dtype=torch.int32, device="cuda"))
+    want = _run(fb, q, k, v, do, True, **kw)
+    monkeypatch.setenv("FA_B200_ALL_PARTIAL", "1")
+    for name, x in _run(fb, q, k, v, do, True, **kw).items():
+        assert torch.equal(x, want[name]), name
+    monkeypatch.setenv("FA_B200_NO_SKIP", "1")
+    exact = attention_64(q, k, v, do, True, None, ids, ids, 10.0, kw["slopes"], kw["prefix"])
+    for name, x in _run(fb, q, k, v, do, True, **kw).items():
+        _check(x, exact[name], name)
+
+
+def test_refusals():
+    import flash_b200 as fb
+    q, k, v, _ = _inputs(2, 4, 2, 32, 32, 64, BF16, 24)
+    for bad in (-1.0, 1e-7, 2e6, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="softcap"):
+            fb.attention_scored(q, k, v, True, softcap=bad)
+    for bad in (torch.ones(2, device="cuda"), torch.ones(4, device="cuda", dtype=torch.float64), torch.ones(4), [1.0] * 4,
+                torch.ones(4, device="cuda", requires_grad=True)):
+        with pytest.raises(ValueError):
+            fb.attention_scored(q, k, v, True, slopes=bad)
+    for bad in (torch.ones(2), torch.ones(2, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda"), 5):
+        with pytest.raises(ValueError):
+            fb.attention_scored(q, k, v, True, prefix=bad)
+    with pytest.raises(ValueError, match="causal"):
+        fb.attention_scored(q, k, v, False, prefix=torch.ones(2, dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError, match="dtype"):
+        fb.attention_scored(q, k.half(), v, True, softcap=5.0)
+    with pytest.raises(AssertionError):
+        fb.attention_scored(q, k[:, :, :8], v[:, :, :8], True, softcap=5.0)
+    with pytest.raises(AssertionError):
+        fb.attention_scored(q, k, v, True, eq=torch.zeros(2, 4, 32, device="cuda", dtype=torch.int64), softcap=5.0)
+    a = q.detach().requires_grad_()
+    g, = torch.autograd.grad(fb.attention_scored(a, k, v, True, softcap=5.0).sum(), a, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()

@@ -8,7 +8,7 @@
 
 namespace fa {
 cudaError_t launch_plan_build(const void*, const int64_t*, int, const void*, const int64_t*, int, int32_t*,
-                              const PlanLayout&, int, int, int*, cudaStream_t);
+                              const PlanLayout&, int, int, const int32_t*, int*, cudaStream_t);
 cudaError_t launch_plan_clear(int32_t*, int, cudaStream_t);
 cudaError_t launch_debug_mask(const MaskArgs&, uint8_t*, uint8_t*, cudaStream_t);
 cudaError_t launch_fwd(int, bool, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
@@ -166,7 +166,20 @@ int debug_flags() {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-int make_mask(fa::MaskArgs* m, const fa_problem* p, const void* plan) {
+// null: a call of attention() itself
+int check_scores(const fa_problem* p, const fa_scores* sc) {
+    if (!sc) return FA_OK;
+    if (sc->softcap != 0.f && !(sc->softcap >= 1e-6f && sc->softcap <= 1e6f)) return FA_ERR_SCORES;
+    if (sc->prefix && !p->causal) return FA_ERR_SCORES;
+    if (reinterpret_cast<uintptr_t>(sc->slopes) % 4 != 0 || reinterpret_cast<uintptr_t>(sc->prefix) % 4 != 0) return FA_ERR_ALIGNMENT;
+    return FA_OK;
+}
+
+fa::ScoreArgs score_args(const fa_problem* p, const fa_scores* sc) {
+    return sc ? fa::make_score_args(sc->softcap, sc->slopes, sc->prefix != nullptr, p->sm_scale) : fa::ScoreArgs{};
+}
+
+int make_mask(fa::MaskArgs* m, const fa_problem* p, const void* plan, const fa_scores* sc = nullptr) {
     if (p->mode == FA_MODE1_DOC && !plan) return FA_ERR_PLAN_SIZE;
     if (!aligned16(plan)) return FA_ERR_ALIGNMENT;  // the kernels read it with 16-byte and bulk loads
     m->plan = (p->mode == FA_MODE1_DOC) ? static_cast<const int32_t*>(plan) : nullptr;
@@ -181,6 +194,7 @@ int make_mask(fa::MaskArgs* m, const fa_problem* p, const void* plan) {
     m->causal = p->causal ? 1 : 0;
     m->mode = p->mode;
     m->debug = debug_flags();
+    m->prefix = sc ? sc->prefix : nullptr;
     return FA_OK;
 }
 
@@ -269,7 +283,7 @@ size_t fwd_workspace_bytes(const fa_problem* p, int ns) {
 // fp32 inputs: which = 0 forward, 1 delta, 2 dK / dV, 3 dQ; absent tensors are null
 int run_f32(int which, const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
             const fa_tensor* d_o, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv, float* lse, float* delta,
-            const void* plan, void* stream, bool overlap = false) {
+            const void* plan, void* stream, const fa_scores* sc, bool overlap = false) {
     int rc;
     fa::F32Params fp{};
     const struct { const fa_tensor* t; fa::F32Tensor* dst; int H, L; } all[8] = {
@@ -282,7 +296,8 @@ int run_f32(int which, const fa_problem* p, const fa_tensor* q, const fa_tensor*
     }
     fa_problem pm = *p;
     if (which == 1) pm.mode = FA_MODE0_NOPE;  // the row sums do not depend on the mask (and take no plan)
-    if ((rc = make_mask(&fp.mask, &pm, plan))) return rc;
+    if ((rc = make_mask(&fp.mask, &pm, plan, sc))) return rc;
+    fp.score = score_args(p, sc);
     fp.lse = lse;
     fp.delta = delta;
     fp.B = p->B; fp.H = p->H; fp.Hk = p->Hk; fp.G = p->H / p->Hk;
@@ -292,22 +307,150 @@ int run_f32(int which, const fa_problem* p, const fa_tensor* q, const fa_tensor*
     return fa::launch_f32(which, p->D, fp, overlap, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
-int run_bwd_dq(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* d_o,
+int run_plan_build(const fa_problem* p, const fa_scores* sc, const fa_ids* eq, const fa_ids* ek, void* plan, size_t plan_bytes,
+                   int32_t* status, void* stream) {
+    int rc = check_problem(p);
+    if (!rc) rc = check_scores(p, sc);
+    if (rc) return rc;
+    if (p->mode != FA_MODE1_DOC) {  // no mask data: the plan is the work counters, cleared here
+        if (!plan) return FA_OK;
+        if (reinterpret_cast<uintptr_t>(plan) % 16 != 0) return FA_ERR_ALIGNMENT;
+        if (plan_bytes < kCtrWords * sizeof(int32_t)) return FA_ERR_PLAN_SIZE;
+        return fa::launch_plan_clear(static_cast<int32_t*>(plan), int(kCtrWords), static_cast<cudaStream_t>(stream)) == cudaSuccess
+                   ? FA_OK : FA_ERR_LAUNCH;
+    }
+    if (!eq || !ek || !eq->ptr || !ek->ptr || !plan || !status) return FA_ERR_BAD_ARG;
+    if ((eq->dtype != FA_ID_INT32 && eq->dtype != FA_ID_INT64) || (ek->dtype != FA_ID_INT32 && ek->dtype != FA_ID_INT64))
+        return FA_ERR_BAD_ARG;
+    if (reinterpret_cast<uintptr_t>(plan) % 16 != 0) return FA_ERR_ALIGNMENT;
+    fa::PlanLayout L(p->B, p->id_heads, p->M, p->N);
+    if (plan_bytes < size_t(L.total) * sizeof(int32_t)) return FA_ERR_PLAN_SIZE;
+    const int gap = p->N > p->M ? p->N - p->M : 0;
+    const cudaError_t e = fa::launch_plan_build(eq->ptr, eq->stride, eq->dtype == FA_ID_INT64, ek->ptr, ek->stride,
+                                                ek->dtype == FA_ID_INT64, static_cast<int32_t*>(plan), L, gap,
+                                                p->causal ? 1 : 0, sc ? sc->prefix : nullptr, status, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+int run_fwd(const fa_problem* p, const fa_scores* sc, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
+            float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+    int rc = check_problem(p);
+    if (rc) return rc;
+    if ((rc = check_scores(p, sc))) return rc;
+    if (!lse || !status || splits < 1) return FA_ERR_BAD_ARG;
+    if (!aligned16(lse)) return FA_ERR_ALIGNMENT;
+    if (splits > 1) {
+        if (p->mode != FA_MODE0_NOPE || p->dtype == FA_FP32 || splits > fa::cdiv(p->N, fa::kBlk)) return FA_ERR_UNSUPPORTED;
+        if (!workspace || workspace_bytes < fwd_workspace_bytes(p, splits)) return FA_ERR_PLAN_SIZE;
+        if (!aligned16(workspace)) return FA_ERR_ALIGNMENT;
+    }
+    if (p->dtype == FA_FP32) return run_f32(0, p, q, k, v, o, nullptr, nullptr, nullptr, nullptr, lse, nullptr, plan, stream, sc);
+    if ((rc = check_tensor(q, p->B, p->H, p->M))) return rc;
+    if ((rc = check_tensor(k, p->B, p->Hk, p->N))) return rc;
+    if ((rc = check_tensor(v, p->B, p->Hk, p->N))) return rc;
+    if ((rc = check_tensor(o, p->B, p->H, p->M))) return rc;
+    fa::FwdParams fp;
+    if ((rc = make_mask(&fp.mask, p, plan, sc))) return rc;
+    fp.score = score_args(p, sc);
+    fp.G = p->H / p->Hk;
+    fp.pack = fwd_pack(p);
+    fp.ns = splits;
+    const int box_rows = fp.pack > 1 ? p->M : fa::kBlk;
+    fp.rows = box_rows * fp.pack;
+    const bool grouped = fp.pack > 1 || fp.ns > 1;
+    CUtensorMap tq, tk, tv, to;
+    if ((rc = grouped ? make_map_grouped(&tq, q, p, box_rows, fp.pack) : make_map(&tq, q, p->dtype, p->B, p->H, p->M, p->D))) return rc;
+    if ((rc = make_map(&tk, k, p->dtype, p->B, p->Hk, p->N, p->D))) return rc;
+    if ((rc = make_map(&tv, v, p->dtype, p->B, p->Hk, p->N, p->D))) return rc;
+    if ((rc = grouped ? make_map_grouped(&to, o, p, box_rows, fp.pack) : make_map(&to, o, p->dtype, p->B, p->H, p->M, p->D))) return rc;
+    const int sms = sm_count();
+    if (sms <= 0) return FA_ERR_LAUNCH;
+    fp.lse = lse;
+    fp.H = p->H;
+    fp.B = p->B;
+    fp.gh = head_group(p, p->Hk * fa::cdiv(fp.G, fp.pack) * p->B);
+    fp.by_length = (p->mode == FA_MODE1_DOC && int64_t(fa::cdiv(p->M, fa::kBlk) * p->H * p->B) < 32 * int64_t(sms)) ? 1 : 0;
+    fp.scale_log2 = p->sm_scale * kLog2e;
+    fp.status = status;
+    fp.wait_limit = wait_limit_clocks();
+    const int64_t rows = int64_t(p->B) * p->H * p->M;
+    const int dk = p->D > 64 ? 128 : 64;
+    fp.part_o = static_cast<float*>(workspace);
+    fp.part_lse = splits > 1 ? fp.part_o + rows * splits * dk : nullptr;
+    cudaError_t e = fa::launch_fwd(p->D, p->dtype == FA_BF16, tq, tk, tv, to, fp, sms, static_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess && splits > 1) {
+        fa::CombineParams cp{fp.part_o, fp.part_lse, out_view(o), lse, p->B, p->H, p->M, p->D, dk, splits, fa::pad128(p->M), status};
+        e = fa::launch_fwd_combine(p->dtype == FA_BF16, cp, static_cast<cudaStream_t>(stream));
+    }
+    return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+int run_bwd_dkdv(const fa_problem* p, const fa_scores* sc, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v,
+                const fa_tensor* d_o, const float* lse, const float* delta, const fa_tensor* dk, const fa_tensor* dv,
+                const void* plan, int32_t* status, void* stream) {
+    int rc = check_problem(p);
+    if (rc) return rc;
+    if ((rc = check_scores(p, sc))) return rc;
+    if (!lse || !delta || !status) return FA_ERR_BAD_ARG;
+    if (!aligned16(lse) || !aligned16(delta)) return FA_ERR_ALIGNMENT;  // read with bulk copies
+    if (p->dtype == FA_FP32)
+        return run_f32(2, p, q, k, v, nullptr, d_o, nullptr, dk, dv, const_cast<float*>(lse), const_cast<float*>(delta), plan, stream, sc);
+    if ((rc = check_tensor(q, p->B, p->H, p->M))) return rc;
+    if ((rc = check_tensor(d_o, p->B, p->H, p->M))) return rc;
+    if ((rc = check_tensor(k, p->B, p->Hk, p->N))) return rc;
+    if ((rc = check_tensor(v, p->B, p->Hk, p->N))) return rc;
+    if ((rc = check_tensor(dk, p->B, p->Hk, p->N))) return rc;
+    if ((rc = check_tensor(dv, p->B, p->Hk, p->N))) return rc;
+    fa::DkdvParams kp;
+    if ((rc = make_mask(&kp.mask, p, plan, sc))) return rc;
+    kp.score = score_args(p, sc);
+    CUtensorMap tq, tk, tv, tdo;
+    if ((rc = make_map(&tq, q, p->dtype, p->B, p->H, p->M, p->D))) return rc;
+    if ((rc = make_map(&tdo, d_o, p->dtype, p->B, p->H, p->M, p->D))) return rc;
+    if ((rc = make_map(&tk, k, p->dtype, p->B, p->Hk, p->N, p->D))) return rc;
+    if ((rc = make_map(&tv, v, p->dtype, p->B, p->Hk, p->N, p->D))) return rc;
+    CUtensorMap tdk, tdv;
+    if ((rc = make_map(&tdk, dk, p->dtype, p->B, p->Hk, p->N, p->D))) return rc;
+    if ((rc = make_map(&tdv, dv, p->dtype, p->B, p->Hk, p->N, p->D))) return rc;
+    const int sms = sm_count();
+    if (sms <= 0) return FA_ERR_LAUNCH;
+    kp.lse = lse;
+    kp.delta = delta;
+    kp.B = p->B;
+    kp.H = p->H;
+    kp.Hk = p->Hk;
+    kp.G = p->H / p->Hk;
+    kp.ksteps = p->D / 16;
+    kp.gh = head_group(p, p->Hk * p->B);
+    kp.by_length = (p->mode == FA_MODE1_DOC && int64_t(fa::cdiv(p->N, fa::kBlk) * p->Hk * p->B) < 32 * int64_t(sms)) ? 1 : 0;
+    kp.scale_log2 = p->sm_scale * kLog2e;
+    kp.sm_scale = p->sm_scale;
+    kp.status = status;
+    kp.wait_limit = wait_limit_clocks();
+    const cudaError_t e =
+        fa::launch_bwd_dkdv(p->D, p->dtype == FA_BF16, tq, tk, tv, tdo, tdk, tdv, kp, sms,
+                            static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+int run_bwd_dq(const fa_problem* p, const fa_scores* sc, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* d_o,
               const float* lse, const float* delta, const fa_tensor* dq, const void* plan, int32_t* status,
                bool overlap, void* stream) {
     int rc = check_problem(p);
     if (rc) return rc;
+    if ((rc = check_scores(p, sc))) return rc;
     if (!lse || !delta || !status) return FA_ERR_BAD_ARG;
     if (!aligned16(lse) || !aligned16(delta)) return FA_ERR_ALIGNMENT;  // read with bulk copies
     if (p->dtype == FA_FP32)
-        return run_f32(3, p, q, k, v, nullptr, d_o, dq, nullptr, nullptr, const_cast<float*>(lse), const_cast<float*>(delta), plan, stream, overlap);
+        return run_f32(3, p, q, k, v, nullptr, d_o, dq, nullptr, nullptr, const_cast<float*>(lse), const_cast<float*>(delta), plan, stream, sc, overlap);
     if ((rc = check_tensor(q, p->B, p->H, p->M))) return rc;
     if ((rc = check_tensor(d_o, p->B, p->H, p->M))) return rc;
     if ((rc = check_tensor(dq, p->B, p->H, p->M))) return rc;
     if ((rc = check_tensor(k, p->B, p->Hk, p->N))) return rc;
     if ((rc = check_tensor(v, p->B, p->Hk, p->N))) return rc;
     fa::DqParams qp;
-    if ((rc = make_mask(&qp.mask, p, plan))) return rc;
+    if ((rc = make_mask(&qp.mask, p, plan, sc))) return rc;
+    qp.score = score_args(p, sc);
     CUtensorMap tq, tk, tv, tdo;
     if ((rc = make_map(&tq, q, p->dtype, p->B, p->H, p->M, p->D))) return rc;
     if ((rc = make_map(&tdo, d_o, p->dtype, p->B, p->H, p->M, p->D))) return rc;
@@ -370,6 +513,7 @@ const char* fa_error_string(int code) {
         case FA_ERR_PLAN_SIZE: return "mask plan or workspace missing or too small";
         case FA_ERR_NO_DRIVER: return "CUDA driver entry point cuTensorMapEncodeTiled not available";
         case FA_ERR_SCRATCH_LIMIT: return "mask plan larger than the library's built-in FA_STATIC_PLAN_BYTES array";
+        case FA_ERR_SCORES: return "scores refused (softcap must be 0 or from 1e-6 to 1e6, a prefix needs a causal mask)";
         default: return "unknown error";
     }
 }
@@ -407,26 +551,12 @@ int fa_plan_optional(const fa_problem* p, int32_t backward) {
 
 int fa_plan_build(const fa_problem* p, const fa_ids* eq, const fa_ids* ek, void* plan, size_t plan_bytes,
                   int32_t* status, void* stream) {
-    const int rc = check_problem(p);
-    if (rc) return rc;
-    if (p->mode != FA_MODE1_DOC) {  // no mask data: the plan is the work counters, cleared here
-        if (!plan) return FA_OK;
-        if (reinterpret_cast<uintptr_t>(plan) % 16 != 0) return FA_ERR_ALIGNMENT;
-        if (plan_bytes < kCtrWords * sizeof(int32_t)) return FA_ERR_PLAN_SIZE;
-        return fa::launch_plan_clear(static_cast<int32_t*>(plan), int(kCtrWords), static_cast<cudaStream_t>(stream)) == cudaSuccess
-                   ? FA_OK : FA_ERR_LAUNCH;
-    }
-    if (!eq || !ek || !eq->ptr || !ek->ptr || !plan || !status) return FA_ERR_BAD_ARG;
-    if ((eq->dtype != FA_ID_INT32 && eq->dtype != FA_ID_INT64) || (ek->dtype != FA_ID_INT32 && ek->dtype != FA_ID_INT64))
-        return FA_ERR_BAD_ARG;
-    if (reinterpret_cast<uintptr_t>(plan) % 16 != 0) return FA_ERR_ALIGNMENT;
-    fa::PlanLayout L(p->B, p->id_heads, p->M, p->N);
-    if (plan_bytes < size_t(L.total) * sizeof(int32_t)) return FA_ERR_PLAN_SIZE;
-    const int gap = p->N > p->M ? p->N - p->M : 0;
-    const cudaError_t e = fa::launch_plan_build(eq->ptr, eq->stride, eq->dtype == FA_ID_INT64, ek->ptr, ek->stride,
-                                                ek->dtype == FA_ID_INT64, static_cast<int32_t*>(plan), L, gap,
-                                                p->causal ? 1 : 0, status, static_cast<cudaStream_t>(stream));
-    return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+    return run_plan_build(p, nullptr, eq, ek, plan, plan_bytes, status, stream);
+}
+
+int fa_plan_build_scored(const fa_problem* p, const fa_scores* scores, const fa_ids* eq, const fa_ids* ek, void* plan, size_t plan_bytes,
+                         int32_t* status, void* stream) {
+    return scores ? run_plan_build(p, scores, eq, ek, plan, plan_bytes, status, stream) : FA_ERR_BAD_ARG;
 }
 
 int fa_fwd_splits(const fa_problem* p) {
@@ -451,53 +581,12 @@ int fa_fwd(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa
 int fa_fwd_split(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
                  float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status,
                  void* stream) {
-    int rc = check_problem(p);
-    if (rc) return rc;
-    if (!lse || !status || splits < 1) return FA_ERR_BAD_ARG;
-    if (!aligned16(lse)) return FA_ERR_ALIGNMENT;
-    if (splits > 1) {
-        if (p->mode != FA_MODE0_NOPE || p->dtype == FA_FP32 || splits > fa::cdiv(p->N, fa::kBlk)) return FA_ERR_UNSUPPORTED;
-        if (!workspace || workspace_bytes < fwd_workspace_bytes(p, splits)) return FA_ERR_PLAN_SIZE;
-        if (!aligned16(workspace)) return FA_ERR_ALIGNMENT;
-    }
-    if (p->dtype == FA_FP32) return run_f32(0, p, q, k, v, o, nullptr, nullptr, nullptr, nullptr, lse, nullptr, plan, stream);
-    if ((rc = check_tensor(q, p->B, p->H, p->M))) return rc;
-    if ((rc = check_tensor(k, p->B, p->Hk, p->N))) return rc;
-    if ((rc = check_tensor(v, p->B, p->Hk, p->N))) return rc;
-    if ((rc = check_tensor(o, p->B, p->H, p->M))) return rc;
-    fa::FwdParams fp;
-    if ((rc = make_mask(&fp.mask, p, plan))) return rc;
-    fp.G = p->H / p->Hk;
-    fp.pack = fwd_pack(p);
-    fp.ns = splits;
-    const int box_rows = fp.pack > 1 ? p->M : fa::kBlk;
-    fp.rows = box_rows * fp.pack;
-    const bool grouped = fp.pack > 1 || fp.ns > 1;
-    CUtensorMap tq, tk, tv, to;
-    if ((rc = grouped ? make_map_grouped(&tq, q, p, box_rows, fp.pack) : make_map(&tq, q, p->dtype, p->B, p->H, p->M, p->D))) return rc;
-    if ((rc = make_map(&tk, k, p->dtype, p->B, p->Hk, p->N, p->D))) return rc;
-    if ((rc = make_map(&tv, v, p->dtype, p->B, p->Hk, p->N, p->D))) return rc;
-    if ((rc = grouped ? make_map_grouped(&to, o, p, box_rows, fp.pack) : make_map(&to, o, p->dtype, p->B, p->H, p->M, p->D))) return rc;
-    const int sms = sm_count();
-    if (sms <= 0) return FA_ERR_LAUNCH;
-    fp.lse = lse;
-    fp.H = p->H;
-    fp.B = p->B;
-    fp.gh = head_group(p, p->Hk * fa::cdiv(fp.G, fp.pack) * p->B);
-    fp.by_length = (p->mode == FA_MODE1_DOC && int64_t(fa::cdiv(p->M, fa::kBlk) * p->H * p->B) < 32 * int64_t(sms)) ? 1 : 0;
-    fp.scale_log2 = p->sm_scale * kLog2e;
-    fp.status = status;
-    fp.wait_limit = wait_limit_clocks();
-    const int64_t rows = int64_t(p->B) * p->H * p->M;
-    const int dk = p->D > 64 ? 128 : 64;
-    fp.part_o = static_cast<float*>(workspace);
-    fp.part_lse = splits > 1 ? fp.part_o + rows * splits * dk : nullptr;
-    cudaError_t e = fa::launch_fwd(p->D, p->dtype == FA_BF16, tq, tk, tv, to, fp, sms, static_cast<cudaStream_t>(stream));
-    if (e == cudaSuccess && splits > 1) {
-        fa::CombineParams cp{fp.part_o, fp.part_lse, out_view(o), lse, p->B, p->H, p->M, p->D, dk, splits, fa::pad128(p->M), status};
-        e = fa::launch_fwd_combine(p->dtype == FA_BF16, cp, static_cast<cudaStream_t>(stream));
-    }
-    return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+    return run_fwd(p, nullptr, q, k, v, o, lse, plan, splits, workspace, workspace_bytes, status, stream);
+}
+
+int fa_fwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
+                  float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+    return scores ? run_fwd(p, scores, q, k, v, o, lse, plan, splits, workspace, workspace_bytes, status, stream) : FA_ERR_BAD_ARG;
 }
 
 int fa_bwd_delta(const fa_problem* p, const fa_tensor* o, const fa_tensor* d_o, float* delta, void* stream) {
@@ -506,7 +595,7 @@ int fa_bwd_delta(const fa_problem* p, const fa_tensor* o, const fa_tensor* d_o, 
     if (!delta) return FA_ERR_BAD_ARG;
     if (!aligned16(delta)) return FA_ERR_ALIGNMENT;
     if (p->dtype == FA_FP32)
-        return run_f32(1, p, nullptr, nullptr, nullptr, o, d_o, nullptr, nullptr, nullptr, nullptr, delta, nullptr, stream);
+        return run_f32(1, p, nullptr, nullptr, nullptr, o, d_o, nullptr, nullptr, nullptr, nullptr, delta, nullptr, stream, nullptr);
     if ((rc = check_tensor(o, p->B, p->H, p->M))) return rc;
     if ((rc = check_tensor(d_o, p->B, p->H, p->M))) return rc;
     fa::DeltaParams dp;
@@ -523,53 +612,13 @@ int fa_bwd_delta(const fa_problem* p, const fa_tensor* o, const fa_tensor* d_o, 
 int fa_bwd_dkdv(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v,
                 const fa_tensor* d_o, const float* lse, const float* delta, const fa_tensor* dk, const fa_tensor* dv,
                 const void* plan, int32_t* status, void* stream) {
-    int rc = check_problem(p);
-    if (rc) return rc;
-    if (!lse || !delta || !status) return FA_ERR_BAD_ARG;
-    if (!aligned16(lse) || !aligned16(delta)) return FA_ERR_ALIGNMENT;  // read with bulk copies
-    if (p->dtype == FA_FP32)
-        return run_f32(2, p, q, k, v, nullptr, d_o, nullptr, dk, dv, const_cast<float*>(lse), const_cast<float*>(delta), plan, stream);
-    if ((rc = check_tensor(q, p->B, p->H, p->M))) return rc;
-    if ((rc = check_tensor(d_o, p->B, p->H, p->M))) return rc;
-    if ((rc = check_tensor(k, p->B, p->Hk, p->N))) return rc;
-    if ((rc = check_tensor(v, p->B, p->Hk, p->N))) return rc;
-    if ((rc = check_tensor(dk, p->B, p->Hk, p->N))) return rc;
-    if ((rc = check_tensor(dv, p->B, p->Hk, p->N))) return rc;
-    fa::DkdvParams kp;
-    if ((rc = make_mask(&kp.mask, p, plan))) return rc;
-    CUtensorMap tq, tk, tv, tdo;
-    if ((rc = make_map(&tq, q, p->dtype, p->B, p->H, p->M, p->D))) return rc;
-    if ((rc = make_map(&tdo, d_o, p->dtype, p->B, p->H, p->M, p->D))) return rc;
-    if ((rc = make_map(&tk, k, p->dtype, p->B, p->Hk, p->N, p->D))) return rc;
-    if ((rc = make_map(&tv, v, p->dtype, p->B, p->Hk, p->N, p->D))) return rc;
-    CUtensorMap tdk, tdv;
-    if ((rc = make_map(&tdk, dk, p->dtype, p->B, p->Hk, p->N, p->D))) return rc;
-    if ((rc = make_map(&tdv, dv, p->dtype, p->B, p->Hk, p->N, p->D))) return rc;
-    const int sms = sm_count();
-    if (sms <= 0) return FA_ERR_LAUNCH;
-    kp.lse = lse;
-    kp.delta = delta;
-    kp.B = p->B;
-    kp.H = p->H;
-    kp.Hk = p->Hk;
-    kp.G = p->H / p->Hk;
-    kp.ksteps = p->D / 16;
-    kp.gh = head_group(p, p->Hk * p->B);
-    kp.by_length = (p->mode == FA_MODE1_DOC && int64_t(fa::cdiv(p->N, fa::kBlk) * p->Hk * p->B) < 32 * int64_t(sms)) ? 1 : 0;
-    kp.scale_log2 = p->sm_scale * kLog2e;
-    kp.sm_scale = p->sm_scale;
-    kp.status = status;
-    kp.wait_limit = wait_limit_clocks();
-    const cudaError_t e =
-        fa::launch_bwd_dkdv(p->D, p->dtype == FA_BF16, tq, tk, tv, tdo, tdk, tdv, kp, sms,
-                            static_cast<cudaStream_t>(stream));
-    return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+    return run_bwd_dkdv(p, nullptr, q, k, v, d_o, lse, delta, dk, dv, plan, status, stream);
 }
 
 int fa_bwd_dq(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* d_o,
               const float* lse, const float* delta, const fa_tensor* dq, const void* plan, int32_t* status,
               void* stream) {
-    return run_bwd_dq(p, q, k, v, d_o, lse, delta, dq, plan, status, false, stream);
+    return run_bwd_dq(p, nullptr, q, k, v, d_o, lse, delta, dq, plan, status, false, stream);
 }
 
 int fa_bwd(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
@@ -577,7 +626,19 @@ int fa_bwd(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa
            const void* plan, int32_t* status, void* stream) {
     int rc = fa_bwd_delta(p, o, d_o, delta, stream);
     if (!rc) rc = fa_bwd_dkdv(p, q, k, v, d_o, lse, delta, dk, dv, plan, status, stream);
-    if (!rc) rc = run_bwd_dq(p, q, k, v, d_o, lse, delta, dq, plan, status, true, stream);
+    if (!rc) rc = run_bwd_dq(p, nullptr, q, k, v, d_o, lse, delta, dq, plan, status, true, stream);
+    return rc;
+}
+
+int fa_bwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
+                  const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv,
+                  const void* plan, int32_t* status, void* stream) {
+    if (!scores) return FA_ERR_BAD_ARG;
+    int rc = check_problem(p);
+    if (!rc) rc = check_scores(p, scores);
+    if (!rc) rc = fa_bwd_delta(p, o, d_o, delta, stream);
+    if (!rc) rc = run_bwd_dkdv(p, scores, q, k, v, d_o, lse, delta, dk, dv, plan, status, stream);
+    if (!rc) rc = run_bwd_dq(p, scores, q, k, v, d_o, lse, delta, dq, plan, status, true, stream);
     return rc;
 }
 

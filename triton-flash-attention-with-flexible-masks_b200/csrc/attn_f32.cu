@@ -195,6 +195,22 @@ __device__ __forceinline__ void put_p(float* P, int x, const float (&w)[kRW][2])
     for (int c = 0; c < 2; ++c) *reinterpret_cast<float4*>(P + (x + 32 * c) * kRW) = make_float4(w[0][c], w[1][c], w[2][c], w[3][c]);
 }
 
+// The score of a product s for query i and key j of a head with this slope, and the derivative of the capped one (scores.cuh; natural logarithm)
+template <bool SCORED>
+__device__ __forceinline__ float score_f32(const F32Params& p, float s, float slope, int i, int j, float& factor) {
+    float y = s * p.scale;
+    factor = 1.f;
+    if (!SCORED) return y;
+    if (p.score.cap > 0.f) {
+        const float t = tanhf(s * p.score.k);
+        y = p.score.cap * t;
+        factor = 1.f - t * t;
+    }
+    return y - slope * fabsf(float(i + p.mask.gap - j));
+}
+template <bool SCORED>
+__device__ __forceinline__ float slope_of(const F32Params& p, int h) { return SCORED && p.score.slopes ? p.score.slopes[h] : 0.f; }
+
 __device__ __forceinline__ float warp_max(float x) {
     float y;
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
@@ -207,11 +223,11 @@ __device__ __forceinline__ float warp_sum(float x) {
 }
 
 // visited[o] for every 128-block o of the other side; the caller synchronises
-template <int R>
+template <int R, bool SCORED>
 __device__ __forceinline__ void find_visited(uint8_t* visited, const MaskArgs& mk, int b, int he, bool rows_are_queries, int own) {
     const int n = rows_are_queries ? mk.L.nK : mk.L.nQ;
     for (int o = threadIdx.x; o < n; o += threads(R))
-        visited[o] = (classify_from_plan(mk, b, he, rows_are_queries ? own : o, rows_are_queries ? o : own) & TILE_VISIT) != 0;
+        visited[o] = (classify_from_plan<SCORED>(mk, b, he, rows_are_queries ? own : o, rows_are_queries ? o : own) & TILE_VISIT) != 0;
 }
 // first column >= c (a multiple of kC) of a visited block, or end
 __device__ __forceinline__ int next_tile(const uint8_t* visited, int c, int end) {
@@ -229,7 +245,7 @@ __device__ __forceinline__ int code_k(const MaskArgs& mk, int b, int he, int j) 
 // ---------------------------------------------------------------------------------------------
 // forward: grid (H, B, ceil(M / R))
 // ---------------------------------------------------------------------------------------------
-template <int D, int R>
+template <int D, int R, bool SCORED>
 __global__ void __launch_bounds__(threads(R), R == 32 && D <= 32 ? 4 : 0) f32_fwd_kernel(const F32Params p) {
     using S = F32Smem<D, R>;
     extern __shared__ __align__(16) float sm[];
@@ -249,20 +265,22 @@ __global__ void __launch_bounds__(threads(R), R == 32 && D <= 32 ? 4 : 0) f32_fw
     const float* vbase = p.v.ptr + int64_t(b) * p.v.sb + int64_t(hk) * p.v.sh;
     const bool kvec = rows_aligned(kbase, p.k.sl), vvec = rows_aligned(vbase, p.v.sl);
     const int32_t* kcodes = mk.mode == 1 ? mk.plan + mk.L.off_kc + (int64_t(b) * mk.He + he) * mk.L.Npad : nullptr;
-    const int end = mk.causal ? min(mk.N, i0 + R + mk.gap) : mk.N;  // keys beyond the last row's causal bound
+    const int front = front_keys<SCORED>(mk, b);
+    const float slope = slope_of<SCORED>(p, h);
+    const int end = mk.causal ? min(mk.N, max(i0 + R + mk.gap, front)) : mk.N;  // keys beyond the last row's causal bound
     // In a block of 32 rows those beyond the first half's: the values there stay out of its P V, for a product with a P of 0 may be NaN.
     // What a NaN or an infinity reaches then does not go by the size of the blocks, which goes by what a sequence is batched with. us, forward and
     // forward with backward, products over the whole tile | over what the half sees: 4 x 8 heads x 1024 x 64 causal 179, 726 | 177, 712, not causal
     // 324, 1342 | 324, 1329; 4 x 8 x 1024 x 128 causal 363, 1462 | 359, 1466; 8 x 16 x 512 x 32 causal 121, 496 | 119, 488, not causal 205, 855 | 208, 859
     // (four blocks of head dims up to 32 share an SM only while a thread has 64 registers: 211 with three).
-    const int end_half = mk.causal && r0 < 16 ? i0 + 16 + mk.gap : mk.N + kC;
+    const int end_half = mk.causal && r0 < 16 ? max(i0 + 16 + mk.gap, front) : mk.N + kC;
     auto fetch = [&](int j0, int st) {
         load_tile<D, kC, R>(KVs + st * 2 * S::cols, kbase, p.k.sl, kvec, j0, end);
         load_tile<D, kC, R>(KVs + (st * 2 + 1) * S::cols, vbase, p.v.sl, vvec, j0, end);
         if (kcodes && threadIdx.x < kC) cp_async4(smem_u32(codes + st * kC + threadIdx.x), kcodes + j0 + threadIdx.x, true);
     };
     load_tile<D, R, R>(Qs, qbase, p.q.sl, rows_aligned(qbase, p.q.sl), i0, mk.M);
-    find_visited<R>(visited, mk, b, he, true, i0 / kBlk);
+    find_visited<R, SCORED>(visited, mk, b, he, true, i0 / kBlk);
     float m[kRW], l[kRW];
     F32Acc<D> acc;
     acc.clear();
@@ -293,8 +311,9 @@ __global__ void __launch_bounds__(threads(R), R == 32 && D <= 32 ? 4 : 0) f32_fw
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int j = j0 + x + 32 * c;
-                const bool keep = keep_entry(i, j, qc[r], kcodes ? codes[st * kC + x + 32 * c] : 0, mk.N, mk.gap, mk.causal, mk.mode);
-                s[r][c] = keep ? s[r][c] * p.scale : -INFINITY;
+                const bool keep = keep_entry(i, j, qc[r], kcodes ? codes[st * kC + x + 32 * c] : 0, mk.N, mk.gap, mk.causal, mk.mode, front);
+                float factor;
+                s[r][c] = keep ? score_f32<SCORED>(p, s[r][c], slope, i, j, factor) : -INFINITY;
                 mx = fmaxf(mx, s[r][c]);
             }
             const float mn = fmaxf(m[r], warp_max(mx));
@@ -349,7 +368,7 @@ __global__ void __launch_bounds__(128) f32_delta_kernel(const F32Params p) {
 // ---------------------------------------------------------------------------------------------
 // dQ: grid (H, B, ceil(M / R)). rows = queries, columns = keys
 // ---------------------------------------------------------------------------------------------
-template <int D, int R>
+template <int D, int R, bool SCORED>
 __global__ void __launch_bounds__(threads(R)) f32_bwd_dq_kernel(const F32Params p) {
     using S = F32Smem<D, R>;
     extern __shared__ __align__(16) float sm[];
@@ -370,8 +389,10 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dq_kernel(const F32Params 
     const float* vbase = p.v.ptr + int64_t(b) * p.v.sb + int64_t(hk) * p.v.sh;
     const bool kvec = rows_aligned(kbase, p.k.sl), vvec = rows_aligned(vbase, p.v.sl);
     const int32_t* kcodes = mk.mode == 1 ? mk.plan + mk.L.off_kc + (int64_t(b) * mk.He + he) * mk.L.Npad : nullptr;
-    const int end = mk.causal ? min(mk.N, i0 + R + mk.gap) : mk.N;  // keys beyond the last row's causal bound
-    const int end_half = mk.causal && r0 < 16 ? i0 + 16 + mk.gap : mk.N + kC;  // (see the forward)
+    const int front = front_keys<SCORED>(mk, b);
+    const float slope = slope_of<SCORED>(p, h);
+    const int end = mk.causal ? min(mk.N, max(i0 + R + mk.gap, front)) : mk.N;  // keys beyond the last row's causal bound
+    const int end_half = mk.causal && r0 < 16 ? max(i0 + 16 + mk.gap, front) : mk.N + kC;  // (see the forward)
     auto fetch = [&](int j0, int st) {
         load_tile<D, kC, R>(KVs + st * 2 * S::cols, kbase, p.k.sl, kvec, j0, end);
         load_tile<D, kC, R>(KVs + (st * 2 + 1) * S::cols, vbase, p.v.sl, vvec, j0, end);
@@ -379,7 +400,7 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dq_kernel(const F32Params 
     };
     load_tile<D, R, R>(Qs, qbase, p.q.sl, rows_aligned(qbase, p.q.sl), i0, mk.M);
     load_tile<D, R, R>(dOs, dobase, p.d_o.sl, rows_aligned(dobase, p.d_o.sl), i0, mk.M);
-    find_visited<R>(visited, mk, b, he, true, i0 / kBlk);
+    find_visited<R, SCORED>(visited, mk, b, he, true, i0 / kBlk);
     F32Acc<D> acc;
     acc.clear();
     float lse[kRW], dl[kRW];
@@ -412,9 +433,10 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dq_kernel(const F32Params 
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int j = j0 + x + 32 * c;
-                const bool keep = (i < mk.M) && keep_entry(i, j, qc[r], kcodes ? codes[st * kC + x + 32 * c] : 0, mk.N, mk.gap, mk.causal, mk.mode);
-                const float pe = keep ? expf(s[r][c] * p.scale - lse[r]) : 0.f;  // a kept entry has a finite lse
-                dp[r][c] = keep ? pe * (dp[r][c] - dl[r]) : 0.f;  // dS (flash_triton.py:301)
+                const bool keep = (i < mk.M) && keep_entry(i, j, qc[r], kcodes ? codes[st * kC + x + 32 * c] : 0, mk.N, mk.gap, mk.causal, mk.mode, front);
+                float factor;
+                const float pe = keep ? expf(score_f32<SCORED>(p, s[r][c], slope, i, j, factor) - lse[r]) : 0.f;  // a kept entry has a finite lse
+                dp[r][c] = keep ? pe * (dp[r][c] - dl[r]) * factor : 0.f;  // dS (flash_triton.py:301)
             }
         }
         put_p(Ps, x, dp);
@@ -440,7 +462,7 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dq_kernel(const F32Params 
 // dK, dV: grid (Hk, B, ceil(N / R)). rows = keys, columns = queries; the query heads of the group
 // are walked one after the other, so the group sum (flash_triton.py:635-637) needs no second pass
 // ---------------------------------------------------------------------------------------------
-template <int D, int R>
+template <int D, int R, bool SCORED>
 __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Params p) {
     using S = F32Smem<D, R>;
     extern __shared__ __align__(16) float sm[];
@@ -463,11 +485,13 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
     dk.clear();
     dv.clear();
     // first query row that can see key j0 under the causal mask (flash_triton.py:214-218)
-    const int first = mk.causal ? max(0, j0 - mk.gap) : 0;
-    const int first_half = mk.causal && r0 >= 16 ? j0 + 16 - mk.gap : 0;  // the same for the second half of 32 keys (see the forward)
+    const int front = front_keys<SCORED>(mk, b);
+    const int first = mk.causal && j0 >= front ? max(0, j0 - mk.gap) : 0;
+    const int first_half = mk.causal && r0 >= 16 && j0 + 16 >= front ? j0 + 16 - mk.gap : 0;  // the same for the second half of 32 keys (see the forward)
     for (int g = 0; g < p.G; ++g) {
         const int h = hk * p.G + g;
         const int he = (mk.He == 1) ? 0 : h;
+        const float slope = slope_of<SCORED>(p, h);
         const float* qbase = p.q.ptr + int64_t(b) * p.q.sb + int64_t(h) * p.q.sh;
         const float* dobase = p.d_o.ptr + int64_t(b) * p.d_o.sb + int64_t(h) * p.d_o.sh;
         const bool qvec = rows_aligned(qbase, p.q.sl), dovec = rows_aligned(dobase, p.d_o.sl);
@@ -486,7 +510,7 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
             // A head without a visible tile has passed no barrier since its next_tile: without this one a fast warp
             // would rewrite the table while a slow one reads it, and the two would take different numbers of tiles.
             if (g > 0) __syncthreads();
-            find_visited<R>(visited, mk, b, he, false, j0 / kBlk);
+            find_visited<R, SCORED>(visited, mk, b, he, false, j0 / kBlk);
         }
         int kc[kRW];
 #pragma unroll
@@ -514,10 +538,11 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
                 const float lse = vec[kC + x + 32 * c], dl = vec[2 * kC + x + 32 * c];
 #pragma unroll
                 for (int r = 0; r < kRW; ++r) {
-                    const bool keep = (i < mk.M) && keep_entry(i, j0 + r0 + r, qc, kc[r], mk.N, mk.gap, mk.causal, mk.mode);
-                    const float pe = keep ? expf(s[r][c] * p.scale - lse) : 0.f;
+                    const bool keep = (i < mk.M) && keep_entry(i, j0 + r0 + r, qc, kc[r], mk.N, mk.gap, mk.causal, mk.mode, front);
+                    float factor;
+                    const float pe = keep ? expf(score_f32<SCORED>(p, s[r][c], slope, i, j0 + r0 + r, factor) - lse) : 0.f;
                     s[r][c] = pe;
-                    dp[r][c] = keep ? pe * (dp[r][c] - dl) : 0.f;
+                    dp[r][c] = keep ? pe * (dp[r][c] - dl) * factor : 0.f;
                 }
             }
             put_p(Ps, x, s);
@@ -548,7 +573,7 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
 }
 
 // ---------------------------------------------------------------------------------------------
-template <int D, int R>
+template <int D, int R, bool SCORED>
 static cudaError_t launch_f32_t(int which, const F32Params& p, bool overlap, cudaStream_t stream) {
     using S = F32Smem<D, R>;
     const MaskArgs& mk = p.mask;
@@ -563,9 +588,9 @@ static cudaError_t launch_f32_t(int which, const F32Params& p, bool overlap, cud
         kern<<<grid, threads(R), smem, stream>>>(p);
         return cudaGetLastError();
     };
-    if (which == 0) return run(f32_fwd_kernel<D, R>, S::fwd_bytes, mk.M, p.H);
-    if (which == 2) return run(f32_bwd_dkdv_kernel<D, R>, S::bwd_bytes, mk.N, p.Hk);
-    return run(f32_bwd_dq_kernel<D, R>, S::bwd_bytes, mk.M, p.H);
+    if (which == 0) return run(f32_fwd_kernel<D, R, SCORED>, S::fwd_bytes, mk.M, p.H);
+    if (which == 2) return run(f32_bwd_dkdv_kernel<D, R, SCORED>, S::bwd_bytes, mk.N, p.Hk);
+    return run(f32_bwd_dq_kernel<D, R, SCORED>, S::bwd_bytes, mk.M, p.H);
 }
 
 // Blocks of 16 rows while those of 32 fit on the GPU all at once (`slots`): they have a chain of as many tiles but half the work, and the
@@ -582,7 +607,8 @@ static cudaError_t launch_f32_rows(int which, const F32Params& p, bool overlap, 
     constexpr int room = 232448 / ((S::fwd_bytes) + kStatic), per_sm = room < 4 ? room : 4;
     const int64_t rows = int64_t(cdiv(mk.M, 32)) * p.H * p.B, cols = int64_t(cdiv(mk.N, 32)) * p.Hk * p.B, slots = int64_t(per_sm) * sms;
     const bool small = which == 0 ? rows <= slots : 10 * (rows + cols) <= 13 * slots;
-    return small ? launch_f32_t<D, 16>(which, p, overlap, stream) : launch_f32_t<D, 32>(which, p, overlap, stream);
+    if (p.score.on) return small ? launch_f32_t<D, 16, true>(which, p, overlap, stream) : launch_f32_t<D, 32, true>(which, p, overlap, stream);
+    return small ? launch_f32_t<D, 16, false>(which, p, overlap, stream) : launch_f32_t<D, 32, false>(which, p, overlap, stream);
 }
 
 // which: 0 forward, 1 delta, 2 dK / dV, 3 dQ. overlap: the launch directly before this one in the stream is the dK/dV

@@ -31,6 +31,7 @@
 // power cap), other documents than above, us, that "sixteen" | now: 2 x 32 / 8 x 3001 261 | 264, 4 x 16 x 4096 x 128 in documents 186 | 185, 32 x 32768 x 128
 // in 64 documents 588 | 572, 8 x 8 x 1024 x 8192 x 64 143 | 129, 16 x 8 x 577 x 32 47.4 | 45.4, 4 x 12 x 1000 x 64 in documents 33.1 | 32.7, 4 x 16 x 4096 x 64
 // causal 309 | 309.
+#include <type_traits>
 #include "common.cuh"
 #include "params.cuh"
 
@@ -71,12 +72,13 @@ enum : uint32_t { KC_SKIP = 0u, KC_PLAIN = 1u, KC_DOC = 2u, KC_DOCMANY = 3u };
 
 // Flags of tile (qb, kb) for all query heads of one kv head at once. When the heads disagree
 // (ids given per head) the id check is forced, entry by entry, which is always exact.
+template <bool SCORED>
 __device__ __forceinline__ uint32_t classify_group(const MaskArgs& mk, int b, int hk, int G, int qb, int kb) {
-    if (mk.He == 1 || G == 1) return classify_from_plan(mk, b, mk.He == 1 ? 0 : hk * G, qb, kb);
+    if (mk.He == 1 || G == 1) return classify_from_plan<SCORED>(mk, b, mk.He == 1 ? 0 : hk * G, qb, kb);
     uint32_t f = 0;
     bool all = true;
     for (int g = 0; g < G; ++g) {
-        const uint32_t fg = classify_from_plan(mk, b, hk * G + g, qb, kb);
+        const uint32_t fg = classify_from_plan<SCORED>(mk, b, hk * G + g, qb, kb);
         if (fg & TILE_VISIT) f |= fg; else all = false;
     }
     if (f && !all) f |= TILE_DOC;
@@ -110,7 +112,8 @@ struct Walk {
     }
 };
 
-template <int D, bool BF16>
+// SCORED: as in the forward; with a cap dS takes the factor 1 - tanh^2, which P is multiplied by once it has been packed for dV.
+template <int D, bool BF16, bool SCORED = false>
 __global__ void __launch_bounds__(kDkdvThreads, 1)
 bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -252,7 +255,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     const int ng = (mk.He == 1) ? 1 : G;
                     for (int g = 0; g < ng; ++g) {
                         int l, h2;
-                        q_range(mk, b, mk.He == 1 ? 0 : hk * G + g, kb, l, h2);
+                        q_range<SCORED>(mk, b, mk.He == 1 ? 0 : hk * G + g, kb, l, h2);
                         if (h2 > l) { lo = min(lo, l); hi = max(hi, h2); }
                     }
                     if (hi == 0) lo = 0;
@@ -266,7 +269,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     for (int e = 0; e < 4; ++e) {
                         const int c = 4 * i + e;
                         if (c >= n) break;
-                        const uint32_t f = classify_group(mk, b, hk, G, lo + c, kb);
+                        const uint32_t f = classify_group<SCORED>(mk, b, hk, G, lo + c, kb);
                         uint32_t code = KC_SKIP;
                         if (f & TILE_VISIT) code = !(f & TILE_DOC) ? KC_PLAIN : (f & TILE_QMANY) ? KC_DOCMANY : KC_DOC;
                         cnt += (code != KC_SKIP);
@@ -284,6 +287,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     info[s * 8 + 4] = kb;
                     info[s * 8 + 5] = hk;
                     info[s * 8 + 6] = b;
+                    if constexpr (SCORED) info[s * 8 + 7] = front_keys<true>(mk, b);
                     mbar_arrive(BAR(B_ITEMFULL + s));
                 }
             }
@@ -501,12 +505,13 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             int cg = 0, cc = -1;
             uint32_t code = KC_SKIP;
             int kc = 0, kc_g = -1;  // this key's code for the current query head
+            const int front = SCORED ? info[s * 8 + 7] : 0;
             const float* const delta0 = p.delta + (int64_t(b) * p.H + hk * G) * mk.L.Mpad + cbase + 2 * (lane & 3);
             for (int it = 0; it < NIT && ok; ++it) {
                 wk.next(cg, cc, code);
                 const bool fl_doc = code >= KC_DOC, many = code == KC_DOCMANY;
                 const int qb0 = (lo + cc) * kBlk;
-                const bool fl_range = (mk.causal && (k0 + kBlk > mk.N || k1 - 1 > qb0 + mk.gap)) || (qb0 + kBlk > mk.M);
+                const bool fl_range = (mk.causal && (k0 + kBlk > mk.N || (k1 - 1 > qb0 + mk.gap && (!SCORED || k1 > front)))) || (qb0 + kBlk > mk.M);
                 const int q0 = qb0 + cbase;  // first query row of this warp's columns
                 const int gi = gt + it;
                 // the rows' LSE came with Q, which S^T has been computed from; their delta is asked for here
@@ -529,7 +534,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         keep = codes_equal(qcs, qc, kc, many) | __ballot_sync(0xffffffffu, qc >= 0);
                     }
                     if (fl_range) {
-                        const int cmin = mk.causal ? (j - mk.gap) - q0 : 0, cmax = mk.M - q0;
+                        const int cmin = mk.causal && (!SCORED || j >= front) ? (j - mk.gap) - q0 : 0, cmax = mk.M - q0;
                         keep &= first_bits(cmax) & ~first_bits(cmin);
                     }
                 }
@@ -545,9 +550,46 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 float* pr = reinterpret_cast<float*>(sr);  // [2 halves of 16 keys][4 chunks of 8 queries][2 keys][2 queries]
                 // P^T = exp2(S^T*c - LSE) on packed pairs, 0 where masked. A fully masked row has LSE = -inf and only
                 // occurs in flagged tiles.
+                uint32_t pk[16];
                 if (flagged && !__any_sync(0xffffffffu, keep != 0u)) {
 #pragma unroll
                     for (int x = 0; x < 32; ++x) pr[x] = 0.f;
+                    if constexpr (SCORED) {
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) pk[x] = 0u;
+                    }
+                } else if constexpr (SCORED) {
+                    const float slope = p.score.slopes ? p.score.slopes[hk * G + cg] * kScoreLog2e : 0.f;
+                    const Bias bias(slope, mk.causal && front == 0, qb0 + mk.gap - (k0 + kBlk - 1), qb0 + kBlk - 1 + mk.gap - k0);
+                    const bool capped = p.score.cap > 0.f, beyond = capped && any_beyond<32>(pr, p.score.most);
+                    const float d = float(q0 + 2 * (lane & 3) + mk.gap - (k0 + 32 * (warp & 3) + (lane >> 2))), sd = bias.s * d;
+                    uint32_t bits[4];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) bits[y] = __shfl_sync(0xffffffffu, keep, 8 * y + (lane >> 2)) >> (2 * (lane & 3));
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const float2 l2 = *reinterpret_cast<const float2*>(vlse + 8 * n);
+                        const uint64_t nl2 = pack_f2(-l2.x, -l2.y);
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            float* x = pr + 16 * (y >> 1) + 4 * n + 2 * (y & 1);
+                            uint64_t v = pack_f2(x[0], x[1]), f = pack_f2(1.f, 1.f);
+                            if (capped) {
+                                v = cap_pair(v, p.score, beyond);
+                                f = cap_slope(v, p.score);
+                                v = add_f2(v, nl2);
+                            } else {
+                                v = fma_f2(v, pack_f2(c, c), nl2);
+                            }
+                            if (bias.s != 0.f) v = add_f2(v, bias.pair(d, sd, float(8 * n - 8 * y), 1.f));
+                            float x0, x1;
+                            unpack_f2(v, x0, x1);
+                            x0 = (bits[y] & (1u << (8 * n))) ? fast_exp2(x0) : 0.f;
+                            x1 = (bits[y] & (2u << (8 * n))) ? fast_exp2(x1) : 0.f;
+                            pk[8 * (y >> 1) + 2 * n + (y & 1)] = pack2<BF16>(x0, x1);
+                            unpack_f2(mul_f2(pack_f2(x0, x1), f), x[0], x[1]);
+                        }
+                    }
                 } else {
                     const uint64_t c2 = pack_f2(c, c);
 #pragma unroll
@@ -578,9 +620,10 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     }
                 }
                 // P^T (input dtype) takes the place of its scores
-                uint32_t pk[16];
+                if constexpr (!SCORED) {
 #pragma unroll
-                for (int x = 0; x < 16; ++x) pk[x] = pack2<BF16>(pr[2 * x], pr[2 * x + 1]);
+                    for (int x = 0; x < 16; ++x) pk[x] = pack2<BF16>(pr[2 * x], pr[2 * x + 1]);
+                }
                 tmem_st_frag16(tS, pk);
                 tmem_st_frag16(tS + kHalfLanes, pk + 8);
                 tc_wait_st();
@@ -699,11 +742,11 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     }
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool SCORED>
 static cudaError_t launch_dkdv_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                                  const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
                                  const DkdvParams& p, int num_sms, cudaStream_t stream) {
-    auto kern = bwd_dkdv_kernel<D, BF16>;
+    auto kern = bwd_dkdv_kernel<D, BF16, SCORED>;
     constexpr int smem = DkdvSmem<D>::total;
     static SmemAllowed allowed;
     cudaError_t e = allow_smem(kern, smem, allowed);
@@ -717,10 +760,15 @@ static cudaError_t launch_dkdv_t(const CUtensorMap& tq, const CUtensorMap& tk, c
 cudaError_t launch_bwd_dkdv(int D, bool bf16, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                             const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
                             const DkdvParams& p, int num_sms, cudaStream_t stream) {
-    if (D == 128) return bf16 ? launch_dkdv_t<128, true>(tq, tk, tv, tdo, tdk, tdv, p, num_sms, stream)
-                              : launch_dkdv_t<128, false>(tq, tk, tv, tdo, tdk, tdv, p, num_sms, stream);
-    return bf16 ? launch_dkdv_t<64, true>(tq, tk, tv, tdo, tdk, tdv, p, num_sms, stream)
-                : launch_dkdv_t<64, false>(tq, tk, tv, tdo, tdk, tdv, p, num_sms, stream);
+    auto pick = [&](auto d, auto scored) {
+        constexpr int kD = decltype(d)::value;
+        constexpr bool kScored = decltype(scored)::value;
+        return bf16 ? launch_dkdv_t<kD, true, kScored>(tq, tk, tv, tdo, tdk, tdv, p, num_sms, stream)
+                    : launch_dkdv_t<kD, false, kScored>(tq, tk, tv, tdo, tdk, tdv, p, num_sms, stream);
+    };
+    using std::integral_constant;
+    if (D == 128) return p.score.on ? pick(integral_constant<int, 128>{}, std::true_type{}) : pick(integral_constant<int, 128>{}, std::false_type{});
+    return p.score.on ? pick(integral_constant<int, 64>{}, std::true_type{}) : pick(integral_constant<int, 64>{}, std::false_type{});
 }
 
 }  // namespace fa

@@ -64,7 +64,8 @@ struct DqWalk {
     }
 };
 
-template <int D, int NW, bool BF16>
+// SCORED: as in the forward; with a cap dS takes the factor 1 - tanh^2.
+template <int D, int NW, bool BF16, bool SCORED = false>
 __global__ void __launch_bounds__(DqSmem<D, NW>::THREADS, 1)
 bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
               const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -184,7 +185,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                 decode(j, qb, h, b);
                 const int he = (mk.He == 1) ? 0 : h;
                 int lo, hi;
-                kv_range(mk, b, he, qb, lo, hi);
+                kv_range<SCORED>(mk, b, he, qb, lo, hi);
                 int n = hi - lo;
                 if (n > kListCap) n = kListCap;  // the host refuses problems that could exceed the cap
                 uint8_t* fl = smem + S::off_flags + s * S::FLAGS;
@@ -194,7 +195,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                     for (int e = 0; e < 4; ++e) {
                         const int c = 4 * i + e;
                         if (c >= n) break;
-                        const uint32_t f = classify_from_plan(mk, b, he, qb, lo + c);
+                        const uint32_t f = classify_from_plan<SCORED>(mk, b, he, qb, lo + c);
                         uint32_t code = QC_SKIP;
                         if (f & TILE_VISIT) code = !(f & TILE_DOC) ? QC_PLAIN : (f & TILE_KMANY) ? QC_DOCMANY : QC_DOC;
                         cnt += (code != QC_SKIP);
@@ -212,6 +213,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                     info[s * 8 + 4] = qb;
                     info[s * 8 + 5] = h;
                     info[s * 8 + 6] = b;
+                    if constexpr (SCORED) info[s * 8 + 7] = front_keys<true>(mk, b);
                     mbar_arrive(BAR(B_ITEMFULL + s));
                 }
             }
@@ -411,6 +413,8 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             const int he = (mk.He == 1) ? 0 : h;
             const DqWalk wk = walk_of(s, n);
             const int row = qb * kBlk + r;
+            const int front = SCORED ? info[s * 8 + 7] : 0;
+            const float slope = SCORED && p.score.slopes ? p.score.slopes[h] * kScoreLog2e : 0.f;
             const int q0 = qb * kBlk;
             const int64_t bh_ids = int64_t(b) * mk.He + he;
             const int qc = (mk.mode == 1) ? mk.plan[mk.L.off_qc + bh_ids * mk.L.Mpad + row] : 0;
@@ -430,7 +434,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                 const bool fl_doc = code >= QC_DOC, many = code == QC_DOCMANY;
                 const int kb0 = (lo + cc) * kBlk;
                 const int kb1 = min(kb0 + kBlk, mk.N);
-                const bool fl_bound = (kb0 + kBlk > mk.N) || (mk.causal && kb1 - 1 > q0 + mk.gap);
+                const bool fl_bound = (kb0 + kBlk > mk.N) || (mk.causal && kb1 - 1 > q0 + mk.gap && (!SCORED || kb1 > front));
                 const int k0 = kb0 + cbase;  // first key column of this thread
                 const uint32_t tS = tmem + lane_base + uint32_t(gi & 1) * 128u + uint32_t(cbase);
                 // keep(x) = (x <= lim) & (qc >= 0 | kc[x] == qc) as 32-bit masks, worked out before the scores are there
@@ -452,7 +456,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                     }
                     if (fl_bound) {
                         int jmax = mk.N - 1;
-                        if (mk.causal) jmax = min(jmax, row + mk.gap);
+                        if (mk.causal) jmax = min(jmax, SCORED ? max(row + mk.gap, front - 1) : row + mk.gap);
 #pragma unroll
                         for (int q = 0; q < NC / 32; ++q) keep[q] &= first_bits(jmax + 1 - k0 - 32 * q);
                     }
@@ -473,6 +477,30 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                     if (flagged && !__any_sync(0xffffffffu, keep[q] != 0u)) {
 #pragma unroll
                         for (int x = 0; x < 32; ++x) pr[32 * q + x] = 0.f;
+                        continue;
+                    }
+                    if constexpr (SCORED) {
+                        const Bias bias(slope, mk.causal && front == 0, q0 + mk.gap - (kb0 + kBlk - 1), q0 + kBlk - 1 + mk.gap - kb0);
+                        const bool capped = p.score.cap > 0.f, beyond = capped && any_beyond<32>(pr + 32 * q, p.score.most);
+                        const float d = float(row + mk.gap - k0 - 32 * q), sd = bias.s * d;
+#pragma unroll
+                        for (int x = 0; x < 32; x += 2) {
+                            float* y = pr + 32 * q + x;
+                            uint64_t v = pack_f2(y[0], y[1]), f = pack_f2(1.f, 1.f);
+                            if (capped) {
+                                v = cap_pair(v, p.score, beyond);
+                                f = cap_slope(v, p.score);
+                                v = add_f2(v, nl2);
+                            } else {
+                                v = fma_f2(v, c2, nl2);
+                            }
+                            if (bias.s != 0.f) v = add_f2(v, bias.pair(d, sd, float(-x), -1.f));
+                            float x0, x1;
+                            unpack_f2(v, x0, x1);
+                            x0 = (keep[q] & (1u << x)) ? fast_exp2(x0) : 0.f;
+                            x1 = (keep[q] & (2u << x)) ? fast_exp2(x1) : 0.f;
+                            unpack_f2(mul_f2(pack_f2(x0, x1), f), y[0], y[1]);
+                        }
                         continue;
                     }
 #pragma unroll
@@ -586,11 +614,11 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     if (tid == 0) wait_prerequisites();
 }
 
-template <int D, int NW, bool BF16>
+template <int D, int NW, bool BF16, bool SCORED>
 static cudaError_t launch_dq_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                                const CUtensorMap& tdo, const CUtensorMap& tdq, const DqParams& p, int num_sms,
                                bool overlap, cudaStream_t stream) {
-    auto kern = bwd_dq_kernel<D, NW, BF16>;
+    auto kern = bwd_dq_kernel<D, NW, BF16, SCORED>;
     constexpr int smem = DqSmem<D, NW>::total;
     static SmemAllowed allowed;
     cudaError_t e = allow_smem(kern, smem, allowed);
@@ -615,8 +643,11 @@ cudaError_t launch_bwd_dq(int D, bool bf16, const CUtensorMap& tq, const CUtenso
                           cudaStream_t stream) {
     auto pick = [&](auto d, auto nw) {
         constexpr int kD = decltype(d)::value, kWarps = decltype(nw)::value;
-        return bf16 ? launch_dq_t<kD, kWarps, true>(tq, tk, tv, tdo, tdq, p, num_sms, overlap, stream)
-                    : launch_dq_t<kD, kWarps, false>(tq, tk, tv, tdo, tdq, p, num_sms, overlap, stream);
+        if (p.score.on)
+            return bf16 ? launch_dq_t<kD, kWarps, true, true>(tq, tk, tv, tdo, tdq, p, num_sms, overlap, stream)
+                        : launch_dq_t<kD, kWarps, false, true>(tq, tk, tv, tdo, tdq, p, num_sms, overlap, stream);
+        return bf16 ? launch_dq_t<kD, kWarps, true, false>(tq, tk, tv, tdo, tdq, p, num_sms, overlap, stream)
+                    : launch_dq_t<kD, kWarps, false, false>(tq, tk, tv, tdo, tdq, p, num_sms, overlap, stream);
     };
     using std::integral_constant;
     if (D == 128) return pick(integral_constant<int, 128>{}, integral_constant<int, 8>{});

@@ -75,7 +75,17 @@ struct MaskArgs {
     int M, N, gap, causal, mode;
     int He;               // 1 or H
     int debug;            // DBG_* bits (0 in normal use)
+    const int32_t* prefix;  // [B], or null: with a causal mask, so many leading keys are visible to every query (the ids' rule holds for them too).
+                            // Looked at by the instances for attention_scored alone (kPrefix below)
 };
+
+// Leading keys that the causal mask leaves visible to every query of sequence b.
+template <bool kPrefix>
+__device__ __forceinline__ int front_keys(const MaskArgs& a, int b) {
+    if (!kPrefix || !a.causal || !a.prefix) return 0;
+    const int n = a.prefix[b];
+    return n < 0 ? 0 : n > a.N ? a.N : n;
+}
 
 // Debug switches that change which tiles are visited and how they are evaluated, never the result:
 // they exist to show that skipping tiles and the per-chunk shortcuts are exact.
@@ -102,8 +112,9 @@ enum : uint32_t {
 
 // Classification of tile (qb, kb) from the block statistics. Conservative: a tile is skipped
 // only when every entry is masked, and declared free of a check only when every entry passes it.
+// front: leading keys that the causal mask does not hide.
 __host__ __device__ inline uint32_t classify_tile(int qb, int kb, int M, int N, int gap, int causal,
-                                                  int mode, int qmin, int qmax, int kmin, int kmax) {
+                                                  int mode, int qmin, int qmax, int kmin, int kmax, int front = 0) {
     const int q0 = qb * kBlk, k0 = kb * kBlk;
     const int q1 = (q0 + kBlk < M) ? q0 + kBlk : M;  // exclusive
     const int k1 = (k0 + kBlk < N) ? k0 + kBlk : N;
@@ -111,8 +122,8 @@ __host__ __device__ inline uint32_t classify_tile(int qb, int kb, int M, int N, 
     if (k0 + kBlk > N) f |= TILE_BOUND;
     if (q0 + kBlk > M) f |= TILE_QTAIL;
     if (causal) {
-        if (k0 > q1 - 1 + gap) return 0;
-        if (k1 - 1 > q0 + gap) f |= TILE_BOUND;
+        if (k0 > q1 - 1 + gap && k0 >= front) return 0;
+        if (k1 - 1 > q0 + gap && k1 > front) f |= TILE_BOUND;
     }
     if (mode == 1) {
         if (qmax < 0 && (kmax < qmin || kmin > qmax)) return 0;
@@ -124,7 +135,9 @@ __host__ __device__ inline uint32_t classify_tile(int qb, int kb, int M, int N, 
 }
 
 // All loads are issued together: they are on the way of a kernel's first tile. Bits that a caller does not look at cost none.
+template <bool kPrefix = false>
 __device__ __forceinline__ uint32_t classify_from_plan(const MaskArgs& a, int b, int he, int qb, int kb) {
+    const int front = front_keys<kPrefix>(a, b);
     int qmin = 0, qmax = 0, kmin = 0, kmax = 0, qf = 0, kf = 0;
     if (a.mode == 1) {
         const int64_t bh = int64_t(b) * a.He + he;
@@ -135,10 +148,10 @@ __device__ __forceinline__ uint32_t classify_from_plan(const MaskArgs& a, int b,
         qf = a.plan[a.L.off_qflags + bh * a.L.nQ + qb];
         kf = a.plan[a.L.off_kflags + bh * a.L.nK + kb];
     }
-    uint32_t f = classify_tile(qb, kb, a.M, a.N, a.gap, a.causal, a.mode, qmin, qmax, kmin, kmax);
+    uint32_t f = classify_tile(qb, kb, a.M, a.N, a.gap, a.causal, a.mode, qmin, qmax, kmin, kmax, front);
     if (a.debug) {
         if ((a.debug & DBG_NO_SKIP) && f == 0 && a.mode == 1) {
-            f = classify_tile(qb, kb, a.M, a.N, a.gap, a.causal, 0, 0, 0, 0, 0);  // the bounds alone
+            f = classify_tile(qb, kb, a.M, a.N, a.gap, a.causal, 0, 0, 0, 0, 0, front);  // the bounds alone
             if (f) f |= TILE_DOC;                                                // the ids mask every entry
         }
         if ((a.debug & DBG_ALL_PARTIAL) && f) return f | TILE_BOUND | (a.mode == 1 ? TILE_DOC : 0u);
@@ -151,6 +164,7 @@ __device__ __forceinline__ uint32_t classify_from_plan(const MaskArgs& a, int b,
 }
 
 // Key-block range [lo, hi) a query block has to walk.
+template <bool kPrefix = false>
 __device__ __forceinline__ void kv_range(const MaskArgs& a, int b, int he, int qb, int& lo, int& hi) {
     if (a.mode == 1 && !(a.debug & DBG_NO_SKIP)) {
         const int64_t bh = int64_t(b) * a.He + he;
@@ -162,10 +176,12 @@ __device__ __forceinline__ void kv_range(const MaskArgs& a, int b, int he, int q
         if (a.causal) {
             const int q1 = min(qb * kBlk + kBlk, a.M);
             hi = min(a.L.nK, (q1 - 1 + a.gap) / kBlk + 1);
+            if (kPrefix) hi = max(hi, cdiv(front_keys<kPrefix>(a, b), kBlk));
         }
     }
 }
 // Query-block range [lo, hi) a key block has to walk.
+template <bool kPrefix = false>
 __device__ __forceinline__ void q_range(const MaskArgs& a, int b, int he, int kb, int& lo, int& hi) {
     if (a.mode == 1 && !(a.debug & DBG_NO_SKIP)) {
         const int64_t bh = int64_t(b) * a.He + he;
@@ -176,7 +192,7 @@ __device__ __forceinline__ void q_range(const MaskArgs& a, int b, int he, int kb
         hi = a.L.nQ;
         if (a.causal) {
             const int first = kb * kBlk - a.gap;  // first query row that sees key k0
-            lo = first > 0 ? first / kBlk : 0;
+            lo = first > 0 && kb * kBlk >= front_keys<kPrefix>(a, b) ? first / kBlk : 0;
             if (lo > hi) lo = hi;
         }
     }
@@ -185,9 +201,9 @@ __device__ __forceinline__ void q_range(const MaskArgs& a, int b, int he, int kb
 // The per-entry predicate on codes. Identical to the reference's rule on the original ids:
 // qc >= 0 <=> eq >= 0; for eq < 0, qc == eq and kc == ek whenever ek is a negative int32,
 // and kc == 0 != qc otherwise.
-__device__ __forceinline__ bool keep_entry(int i, int j, int qc, int kc, int N, int gap, int causal, int mode) {
+__device__ __forceinline__ bool keep_entry(int i, int j, int qc, int kc, int N, int gap, int causal, int mode, int front = 0) {
     bool keep = j < N;
-    if (causal) keep = keep && (gap + i >= j);
+    if (causal) keep = keep && (gap + i >= j || j < front);
     if (mode == 1) keep = keep && ((qc >= 0) || (qc == kc));
     return keep;
 }

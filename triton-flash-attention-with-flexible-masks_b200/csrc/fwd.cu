@@ -98,7 +98,8 @@ static_assert(FwdSmem<128>::total > 116736 && FwdSmem<64>::total > 116736, "shar
 //    and their log-sum-exp go to the workspace, and fwd_combine_kernel merges them.
 // Such calls are bound by reading K and V (16 tokens of 32 / 8 heads of 128 against 4500 keys: 295 MB, 45 us at the
 // copy rate; 127 us with a tile per head, 55 us packed) or, with few heads, by the longest item's chain of tiles.
-template <int D, bool BF16, bool SHORT>
+// SCORED: the scores pass through score_row (scores.cuh) and are in the log2 domain from there on; the causal mask leaves a prefix visible.
+template <int D, bool BF16, bool SHORT, bool SCORED = false>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
            const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const FwdParams p) {
@@ -148,7 +149,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         int4 qc;
     };
     auto classify = [&](const Item& it, int i) {
-        return i < it.n ? classify_from_plan(mk, it.b, (mk.He == 1) ? 0 : it.h, it.qb, it.lo + i) & (TILE_VISIT | TILE_BOUND | TILE_DOC | TILE_KMONO | TILE_KMANY) : 0u;
+        return i < it.n ? classify_from_plan<SCORED>(mk, it.b, (mk.He == 1) ? 0 : it.h, it.qb, it.lo + i) & (TILE_VISIT | TILE_BOUND | TILE_DOC | TILE_KMONO | TILE_KMANY) : 0u;
     };
     auto prepare = [&](int j) {
         Item it;
@@ -156,7 +157,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         decode(SHORT ? j / ns : j, it.qb, it.h, it.b);
         const int he = (mk.He == 1) ? 0 : it.h;
         int lo, hi;
-        kv_range(mk, it.b, he, it.qb, lo, hi);
+        kv_range<SCORED>(mk, it.b, he, it.qb, lo, hi);
         int n = hi - lo;
         if constexpr (SHORT) {  // no ids: every tile of the range is visited
             const int first = int(int64_t(n) * sp / ns);
@@ -305,6 +306,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     info[s * 8 + 4] = item.qb;
                     info[s * 8 + 5] = item.h;
                     info[s * 8 + 6] = item.b;
+                    if constexpr (SCORED) info[s * 8 + 7] = front_keys<true>(mk, item.b);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(BAR(B_ITEMFULL + s));
@@ -472,7 +474,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         setmaxnreg_dec<kFwdEpilogueRegs>();
         const int r = tid & 127;
         const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
-        const float c = p.scale_log2;
+        const float c = SCORED ? 1.f : p.scale_log2;
         bool alive = !aborted;
         int G = 0;           // tiles of all earlier items
         int n0 = 0, n1 = 0;  // items in which the chains of group 0 and 1 had tiles
@@ -604,7 +606,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         const int w = warp >> 2;  // group
         const int r = tid & 127;  // row inside the block
         const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
-        const float c = p.scale_log2;
+        const float c = SCORED ? 1.f : p.scale_log2;
         const uint32_t tO = tmem + lane_base + uint32_t(S::tmem_o + w * D);
         bool alive = !aborted;
         if (SHORT && S::POWN) {  // P of the rows without a query
@@ -631,6 +633,13 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
             const bool active = !SHORT || __any_sync(0xffffffffu, valid);  // does this warp hold a query at all?
             const int qc = reinterpret_cast<const int*>(smem + S::off_qc)[s * kBlk + r];
             const int t0 = (G ^ w) & 1;  // this group's first tile of the item
+            int front = 0;       // SCORED: of the item's sequence and this row's head
+            float slope = 0.f;
+            if constexpr (SCORED) {
+                front = info[s * 8 + 7];
+                const int h = info[s * 8 + 5], own = SHORT ? min((h % nG) * p.pack + g_row, p.G - 1) + h / nG * p.G : h;
+                if (p.score.slopes) slope = p.score.slopes[int64_t(own)] * kScoreLog2e;
+            }
             float m_run = -INFINITY, l_run = 0.f;
 
             for (int t = t0; t < T && alive; t += 2) {
@@ -662,6 +671,12 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     mbar_arrive_warp(BAR(B_SFREE + w), lane);  // the next tile's scores may overwrite these
                 }
                 float* sc = reinterpret_cast<float*>(sr);
+                if constexpr (SCORED) {
+                    const int first = SHORT ? 0 : qb * kBlk, last = SHORT ? mk.M - 1 : qb * kBlk + kBlk - 1;  // rows of the tile, and perhaps more
+                    const Bias bias(slope, mk.causal && front == 0, first + mk.gap - (k0 + kBlk - 1), last + mk.gap - k0);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) score_row(sc + 32 * q, p.score, bias, p.scale_log2, row + mk.gap - k0 - 32 * q);
+                }
 
                 if (fl & (TILE_BOUND | TILE_DOC)) {
                     // keep(x) = (x <= lim) & (qc >= 0 | kc[x] == qc) as 32-bit masks, one select per entry behind them. The ids' part is worked
@@ -672,7 +687,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     int lim = kBlk - 1;
                     if (fl & TILE_BOUND) {
                         int jmax = mk.N - 1;
-                        if (mk.causal) jmax = min(jmax, row + mk.gap);
+                        if (mk.causal) jmax = min(jmax, SCORED ? max(row + mk.gap, front - 1) : row + mk.gap);
                         lim = jmax - k0;
                     }
                     // (the key codes completed on K's barrier, before the S MMA whose result was just read)
@@ -876,10 +891,10 @@ cudaError_t launch_fwd_combine(bool bf16, const CombineParams& p, cudaStream_t s
 }
 
 // ---- host launcher (called from api.cu) -------------------------------------------------
-template <int D, bool BF16, bool SHORT>
+template <int D, bool BF16, bool SHORT, bool SCORED>
 static cudaError_t launch_fwd_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                                 const CUtensorMap& to, const FwdParams& p, int num_sms, cudaStream_t stream) {
-    auto kern = fwd_kernel<D, BF16, SHORT>;
+    auto kern = fwd_kernel<D, BF16, SHORT, SCORED>;
     constexpr int smem = FwdSmem<D>::total;
     static SmemAllowed allowed;
     cudaError_t e = allow_smem(kern, smem, allowed);
@@ -896,8 +911,11 @@ cudaError_t launch_fwd(int D, bool bf16, const CUtensorMap& tq, const CUtensorMa
     auto pick = [&](auto d, auto shrt) {
         constexpr int kD = decltype(d)::value;
         constexpr bool kShort = decltype(shrt)::value;
-        return bf16 ? launch_fwd_t<kD, true, kShort>(tq, tk, tv, to, p, num_sms, stream)
-                    : launch_fwd_t<kD, false, kShort>(tq, tk, tv, to, p, num_sms, stream);
+        if (p.score.on)
+            return bf16 ? launch_fwd_t<kD, true, kShort, true>(tq, tk, tv, to, p, num_sms, stream)
+                        : launch_fwd_t<kD, false, kShort, true>(tq, tk, tv, to, p, num_sms, stream);
+        return bf16 ? launch_fwd_t<kD, true, kShort, false>(tq, tk, tv, to, p, num_sms, stream)
+                    : launch_fwd_t<kD, false, kShort, false>(tq, tk, tv, to, p, num_sms, stream);
     };
     using std::integral_constant;
     const bool shrt = p.pack > 1 || p.ns > 1;

@@ -106,13 +106,14 @@ __global__ void __launch_bounds__(128) plan_codes_kernel(IdsView eq, IdsView ek,
 
 // grid (nQ + nK, He, B), 128 threads: visit range of one query block over key blocks, or of
 // one key block over query blocks.
-__global__ void __launch_bounds__(128) plan_ranges_kernel(int32_t* plan, PlanLayout L, int gap, int causal) {
+__global__ void __launch_bounds__(128) plan_ranges_kernel(int32_t* plan, PlanLayout L, int gap, int causal, const int32_t* prefix) {
     __shared__ int scratch[4];
     follow_stream();
     const int he = blockIdx.y, b = blockIdx.z;
     const int64_t bh = int64_t(b) * L.He + he;
     const bool is_q = int(blockIdx.x) < L.nQ;
     const int blk = is_q ? blockIdx.x : blockIdx.x - L.nQ;
+    const int front = causal && prefix ? prefix[b] : 0;
     const int32_t* qmin = plan + L.off_qmin + bh * L.nQ;
     const int32_t* qmax = plan + L.off_qmax + bh * L.nQ;
     const int32_t* kmin = plan + L.off_kmin + bh * L.nK;
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(128) plan_ranges_kernel(int32_t* plan, PlanLay
     int lo = 0x7fffffff, hi = 0;
     for (int o = threadIdx.x; o < n_other; o += blockDim.x) {
         const int qb = is_q ? blk : o, kb = is_q ? o : blk;
-        const uint32_t f = classify_tile(qb, kb, L.M, L.N, gap, causal, 1, qmin[qb], qmax[qb], kmin[kb], kmax[kb]);
+        const uint32_t f = classify_tile(qb, kb, L.M, L.N, gap, causal, 1, qmin[qb], qmax[qb], kmin[kb], kmax[kb], front);
         if (f & TILE_VISIT) {
             lo = min(lo, o);
             hi = max(hi, o + 1);
@@ -182,12 +183,12 @@ __device__ __forceinline__ int warp_min(int v) { return __reduce_min_sync(0xffff
 __device__ __forceinline__ int warp_max(int v) { return __reduce_max_sync(0xffffffffu, v); }
 
 __global__ void __launch_bounds__(1024) plan_small_kernel(IdsView eq, IdsView ek, int32_t* plan, PlanLayout L, int gap, int causal,
-                                                          int* status) {
+                                                          const int32_t* prefix, int* status) {
     __shared__ int smin[kSmallBlocks], smax[kSmallBlocks], len[kSmallBlocks];  // query blocks, then key blocks
     follow_stream();
     const int he = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t bh = int64_t(b) * L.He + he;
-    const int n = L.nQ + L.nK;
+    const int n = L.nQ + L.nK, front = causal && prefix ? prefix[b] : 0;
     if (he == 0 && b == 0 && threadIdx.x < 128) plan[L.off_ctr + threadIdx.x] = 0;
     for (int i = warp; i < n; i += 32) {
         const bool is_q = i < L.nQ;
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(1024) plan_small_kernel(IdsView eq, IdsView ek
         int lo = 0x7fffffff, hi = 0;
         for (int o = lane; o < n_other; o += 32) {
             const int qb = is_q ? blk : o, kb = is_q ? o : blk;
-            const uint32_t f = classify_tile(qb, kb, L.M, L.N, gap, causal, 1, smin[qb], smax[qb], smin[L.nQ + kb], smax[L.nQ + kb]);
+            const uint32_t f = classify_tile(qb, kb, L.M, L.N, gap, causal, 1, smin[qb], smax[qb], smin[L.nQ + kb], smax[L.nQ + kb], front);
             if (f & TILE_VISIT) {
                 lo = min(lo, o);
                 hi = max(hi, o + 1);
@@ -317,15 +318,15 @@ __global__ void plan_clear_kernel(int32_t* ctr) {
 // ---- host launchers (called from api.cu) ------------------------------------------------
 cudaError_t launch_plan_build(const void* eq_ptr, const int64_t* eq_stride, int eq64, const void* ek_ptr,
                               const int64_t* ek_stride, int ek64, int32_t* plan, const PlanLayout& L, int gap,
-                              int causal, int* status, cudaStream_t stream) {
+                              int causal, const int32_t* prefix, int* status, cudaStream_t stream) {
     IdsView q{eq_ptr, eq_stride[0], eq_stride[1], eq_stride[2], eq64};
     IdsView k{ek_ptr, ek_stride[0], ek_stride[1], ek_stride[2], ek64};
     if (L.nQ + L.nK <= kSmallBlocks) {
-        return launch_overlapping(plan_small_kernel, dim3(L.He, L.B), 1024, 0, stream, q, k, plan, L, gap, causal, status);
+        return launch_overlapping(plan_small_kernel, dim3(L.He, L.B), 1024, 0, stream, q, k, plan, L, gap, causal, prefix, status);
     }
     dim3 grid(L.nQ + L.nK, L.He, L.B);
     cudaError_t e = launch_overlapping(plan_codes_kernel, grid, 128, 0, stream, q, k, plan, L, status);
-    if (e == cudaSuccess) e = launch_overlapping(plan_ranges_kernel, grid, 128, 0, stream, plan, L, gap, causal);
+    if (e == cudaSuccess) e = launch_overlapping(plan_ranges_kernel, grid, 128, 0, stream, plan, L, gap, causal, prefix);
     if (e == cudaSuccess) e = launch_overlapping(plan_order_kernel, dim3(2, L.He, L.B), 1024, 0, stream, plan, L);
     return e;
 }

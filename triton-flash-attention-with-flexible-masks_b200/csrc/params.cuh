@@ -2,6 +2,7 @@
 #pragma once
 #include <atomic>
 #include "common.cuh"
+#include "scores.cuh"
 
 namespace fa {
 
@@ -25,6 +26,7 @@ struct FwdParams {
     int ns;           // runs an item's tiles are cut into; 1: none
     float* part_o;    // [ns, B, H, M, 64 or 128] normalised rows of each run (ns > 1)
     float* part_lse;  // [B, H, M, ns]
+    ScoreArgs score;  // the instances for attention_scored
 };
 
 struct CombineParams {
@@ -58,6 +60,7 @@ struct DkdvParams {
     float scale_log2, sm_scale;
     int* status;
     long long wait_limit;  // SM clocks a bounded wait may last
+    ScoreArgs score;       // the instances for attention_scored
 };
 
 struct DqParams {
@@ -71,6 +74,7 @@ struct DqParams {
     float scale_log2, sm_scale;
     int* status;
     long long wait_limit;  // SM clocks a bounded wait may last
+    ScoreArgs score;       // the instances for attention_scored
 };
 
 // fp32 kernels (attn_f32.cu): plain pointers and element strides, no tensor maps
@@ -86,6 +90,7 @@ struct F32Params {
     MaskArgs mask;
     int B, H, Hk, G;
     float scale;
+    ScoreArgs score;  // the instances for attention_scored: cap and slopes
 };
 
 // A number for the current CUDA context that no other context of the process ever has, or 0 (api.cu).

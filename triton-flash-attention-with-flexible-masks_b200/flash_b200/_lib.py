@@ -17,7 +17,7 @@ EXPORTS = (
     "fa_version", "fa_error_string", "fa_padded_rows", "fa_plan_bytes", "fa_plan_build", "fa_fwd",
     "fa_bwd_delta", "fa_bwd_dkdv", "fa_bwd_dq", "fa_debug_mask", "fa_classify_tile", "fa_fwd_static_plan",
     "fa_debug_wait_timeout", "fa_group_rows", "fa_permute_rows", "fa_fwd_splits", "fa_fwd_workspace_bytes", "fa_fwd_split",
-    "fa_plan_optional", "fa_bwd",
+    "fa_plan_optional", "fa_bwd", "fa_plan_build_scored", "fa_fwd_scored", "fa_bwd_scored",
 )
 
 
@@ -36,6 +36,10 @@ class Tensor(ctypes.Structure):
 
 class Ids(ctypes.Structure):
     _fields_ = [("ptr", ctypes.c_void_p), ("stride", ctypes.c_int64 * 3), ("dtype", ctypes.c_int32)]
+
+
+class Scores(ctypes.Structure):
+    _fields_ = [("softcap", ctypes.c_float), ("slopes", ctypes.c_void_p), ("prefix", ctypes.c_void_p)]
 
 
 _lib = None
@@ -80,6 +84,13 @@ def load():
     lib.fa_bwd_dkdv.argtypes = [P, T, T, T, T, vp, vp, T, T, vp, vp, vp]
     lib.fa_bwd_dq.restype = i32
     lib.fa_bwd_dq.argtypes = [P, T, T, T, T, vp, vp, T, vp, vp, vp]
+    S, size = ctypes.POINTER(Scores), ctypes.c_size_t
+    lib.fa_plan_build_scored.restype = i32
+    lib.fa_plan_build_scored.argtypes = [P, S, I, I, vp, size, vp, vp]
+    lib.fa_fwd_scored.restype = i32
+    lib.fa_fwd_scored.argtypes = [P, S, T, T, T, T, vp, vp, ctypes.c_int32, vp, size, vp, vp]
+    lib.fa_bwd_scored.restype = i32
+    lib.fa_bwd_scored.argtypes = [P, S, T, T, T, T, T, vp, vp, T, T, T, vp, vp, vp]
     lib.fa_debug_mask.restype = i32
     lib.fa_debug_mask.argtypes = [P, vp, vp, vp, vp]
     lib.fa_fwd_static_plan.restype = i32
