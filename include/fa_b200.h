@@ -60,7 +60,8 @@ enum fa_error {
     FA_ERR_PLAN_SIZE = 6,    /* plan buffer too small / missing for FA_MODE1_DOC, or workspace of a split forward */
     FA_ERR_NO_DRIVER = 7,    /* cuTensorMapEncodeTiled could not be resolved */
     FA_ERR_SCRATCH_LIMIT = 8, /* fa_fwd_static_plan: the plan does not fit in FA_STATIC_PLAN_BYTES */
-    FA_ERR_SCORES = 9        /* fa_scores: softcap neither 0 nor within 1e-6 .. 1e6, or a prefix without a causal mask */
+    FA_ERR_SCORES = 9,       /* fa_scores: softcap neither 0 nor within 1e-6 .. 1e6, or a prefix without a causal mask */
+    FA_ERR_PAGED = 10        /* fa_paged_cache: page size not a power of two from 8 on, or sizes beyond what the kernels count */
 };
 
 typedef struct fa_problem {
@@ -185,6 +186,45 @@ int fa_bwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor*
                   const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv,
                   const void* plan, int32_t* status, void* stream);
 
+/* A cache of keys and values in pages, for serving (no counterpart in the reference). k and v are [pages, page_size, Hk, D], 16-bit, with 16-byte
+ * aligned bases, last stride 1 and other strides multiples of 8 elements. Sequence b's tokens lie, page_size at a time, in the pages
+ * table[b * table_stride + i], i = 0 .. ; lens[b] is how many tokens it has. table and lens are device memory, read when the kernels run.
+ * Entries of the table behind a sequence's last page are not read. page_size: a power of two, at least 8; table_pages * page_size <= 2^22.
+ *
+ * New tokens: rows [T, heads, D]. starts [B + 1], non-decreasing: sequence b has the rows from starts[b] to starts[b + 1]; they are its last
+ * ones, at the positions lens[b] - n .. lens[b] - 1, so that lens counts them. starts NULL: T == B and every sequence has one new token.
+ * Rows before starts[0] and from starts[B] on belong to no sequence. A page number outside [0, pages) or a length outside
+ * [0, table_pages * page_size] sets status 201 or 202; nothing outside the tensors is read or written, the results of that sequence are
+ * undefined, and later calls run. */
+typedef struct fa_paged_cache {
+    int32_t B, Hk, D, dtype;          /* sequences; kv heads; head dim 16, 32, 64 or 128; FA_BF16 or FA_FP16 */
+    int32_t pages, page_size, table_pages; /* table_pages: entries of a sequence's row of the table */
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* lens;
+    void* k;
+    void* v;
+    int64_t k_stride[3], v_stride[3]; /* elements: page, slot, head */
+} fa_paged_cache;
+
+typedef struct fa_rows {
+    void* ptr;
+    int64_t stride[2]; /* elements: token, head */
+} fa_rows;
+
+/* Copies new tokens' k and v, [T, Hk, D], to their places in the pages. Rows of no sequence, and new tokens in front of position 0 (more new
+ * ones than lens says there are), are left out. Two tokens at one place (a page that two sequences name): either's values may stay. */
+int fa_paged_append(const fa_paged_cache* cache, int32_t T, const int32_t* starts, const fa_rows* k, const fa_rows* v, int32_t* status, void* stream);
+
+/* o[t] = softmax(scores of row t with the keys it sees) V, for new tokens q [T, H, D] whose own keys are in the cache already. A token at position p
+ * sees the keys j <= p and, with scores->prefix, j < prefix[b], of its sequence (scores may be NULL; i + gap in fa_scores is the position). H / Hk at most 128. A row that sees no key gets zeros. Rows of no
+ * sequence are set to 0 where `fill` is not 0 and else left as they are. o may not overlap q or the cache. Two kernels; `workspace`: 16-byte
+ * aligned, at least fa_paged_workspace_bytes, which goes by the head dim and the current device alone; free again when the launches are done.
+ * How the work is cut depends on all lengths of the batch, so the last bits of a sequence's result can differ with what it is batched with. */
+int fa_paged_workspace_bytes(const fa_paged_cache* cache, size_t* bytes);
+int fa_paged_fwd(const fa_paged_cache* cache, int32_t T, int32_t H, const int32_t* starts, float sm_scale, const fa_scores* scores, const fa_rows* q,
+                 const fa_rows* o, int32_t fill, void* workspace, size_t bytes, int32_t* status, void* stream);
+
 /* Debug: materialise the kernels' decisions. keep is [B, id_heads, M, N] bytes (1 = unmasked),
  * produced by the same device predicate the attention kernels use; tile_class is
  * [B, id_heads, ceil(M/128), ceil(N/128)] bytes: bit0 visited, bit1 bound/causal check,
@@ -246,6 +286,13 @@ int fa_debug_wait_timeout(int32_t* status, int64_t limit_clocks, int32_t role, v
  * (no counterpart in the reference, which never skips a tile). */
 uint32_t fa_classify_tile(int32_t M, int32_t N, int32_t causal, int32_t mode, int32_t qb, int32_t kb,
                           int32_t qmin, int32_t qmax, int32_t kmin, int32_t kmax);
+
+/* Host-only helper, no GPU involved: how fa_paged_fwd cuts a batch among `most_workers` blocks, by the kernels' own code; lens, starts and prefix are
+ * host memory here. Writes up to most_rows rows of 8 and returns how many there are, or -1: (worker, sequence, kv head, tile of queries, first key tile,
+ * last + 1, key tiles of the item, slot of the workspace or -1 for a whole item) for each piece, and (-1, sequence, kv head, tile of queries, 0, 0, 0, slot) for each
+ * piece that the second kernel merges. Exposed so that the cutting can be tested on a CPU. */
+int fa_debug_paged_pieces(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t capacity, const int32_t* lens, const int32_t* starts, const int32_t* prefix,
+                          int32_t most_workers, int32_t* rows, int32_t most_rows);
 
 #ifdef __cplusplus
 }

@@ -4,6 +4,7 @@
 #include <mutex>
 #include "../../include/fa_b200.h"
 #include "common.cuh"
+#include "host_shared.cuh"
 #include "params.cuh"
 
 namespace fa {
@@ -23,13 +24,6 @@ cudaError_t launch_bwd_dq(int, bool, const CUtensorMap&, const CUtensorMap&, con
 
 // fp32 path (attn_f32.cu)
 cudaError_t launch_f32(int which, int D, const F32Params& p, bool overlap, int sms, cudaStream_t stream);
-}  // namespace fa
-
-namespace {
-
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 // The driver entry point is resolved through the runtime so that the library has no link-time
 // dependency on libcuda (it must load, and list its symbols, on a machine without a driver).
@@ -45,6 +39,44 @@ EncodeFn encode_fn() {
     });
     return fn;
 }
+
+// Limit of one bounded wait inside the kernels, in SM clocks: FA_B200_WAIT_LIMIT_CLOCKS if set to a
+// number >= 10000 when the library is first used, else the built-in default.
+long long wait_limit_clocks() {
+    constexpr long long kMost = 1LL << 50;  // a week; a wait for a whole item multiplies it by the item's tiles
+    static const long long v = [] {
+        const char* e = getenv("FA_B200_WAIT_LIMIT_CLOCKS");
+        if (e) {
+            const long long x = atoll(e);
+            if (x >= 10000) return x < kMost ? x : kMost;
+        }
+        return fa::kWaitLimitClocks;
+    }();
+    return v;
+}
+
+int sm_count() {
+    static std::mutex mu;
+    static int cached[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+    std::lock_guard<std::mutex> lock(mu);
+    if (cached[dev] == 0) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return -1;
+        cached[dev] = n;
+    }
+    return cached[dev];
+}
+}  // namespace fa
+
+namespace {
+
+using fa::encode_fn;
+using fa::EncodeFn;
+using fa::sm_count;
+using fa::wait_limit_clocks;
+
 
 using ContextIdFn = CUresult (*)(CUcontext, unsigned long long*);
 
@@ -202,20 +234,6 @@ fa::OutTensor out_view(const fa_tensor* t) { return fa::OutTensor{t->ptr, t->str
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Limit of one bounded wait inside the kernels, in SM clocks: FA_B200_WAIT_LIMIT_CLOCKS if set to a
-// number >= 10000 when the library is first used, else the built-in default.
-long long wait_limit_clocks() {
-    constexpr long long kMost = 1LL << 50;  // a week; a wait for a whole item multiplies it by the item's tiles
-    static const long long v = [] {
-        const char* e = getenv("FA_B200_WAIT_LIMIT_CLOCKS");
-        if (e) {
-            const long long x = atoll(e);
-            if (x >= 10000) return x < kMost ? x : kMost;
-        }
-        return fa::kWaitLimitClocks;
-    }();
-    return v;
-}
 
 // Number of SMs of the current device (persistent kernels launch one CTA per SM); cached per device.
 // Heads per scheduling group of the persistent kernels (see their `decode`): as many heads as
@@ -235,19 +253,6 @@ int head_group(const fa_problem* p, int heads_total) {
     return gh < heads_total ? gh : heads_total;
 }
 
-int sm_count() {
-    static std::mutex mu;
-    static int cached[64] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
-    std::lock_guard<std::mutex> lock(mu);
-    if (cached[dev] == 0) {
-        int n = 0;
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return -1;
-        cached[dev] = n;
-    }
-    return cached[dev];
-}
 
 // Runs into which the forward cuts each item's key tiles, for calls without ids that have fewer items than the GPU
 // has SMs. A round of items is taken to cost its tiles plus 4 tile times of fill, drain and epilogue, the second
@@ -514,6 +519,8 @@ const char* fa_error_string(int code) {
         case FA_ERR_NO_DRIVER: return "CUDA driver entry point cuTensorMapEncodeTiled not available";
         case FA_ERR_SCRATCH_LIMIT: return "mask plan larger than the library's built-in FA_STATIC_PLAN_BYTES array";
         case FA_ERR_SCORES: return "scores refused (softcap must be 0 or from 1e-6 to 1e6, a prefix needs a causal mask)";
+        case FA_ERR_PAGED:
+            return "paged cache refused (page size a power of two from 8 on, at most 4194304 tokens per sequence and call, 65535 sequences, 1024 kv heads)";
         default: return "unknown error";
     }
 }

@@ -1,0 +1,674 @@
+// Attention of new tokens over a paged cache: O = softmax(scores) V for a ragged batch of new tokens [T, H, D], whose sequences' keys and values
+// lie in pages [pages, page size, Hk, D] that a table names. A token at position p of its sequence sees the keys up to p (and a prefix); what lies
+// in the pages behind a sequence's length is never part of a result. The score of a pair is that of the forward kernel, with the changes of
+// scores.cuh.
+//
+// The forward kernel's structure (fwd.cu): two chains of key tiles with a maximum, a sum and an accumulator each, an epilogue group that merges them
+// while the chains are in the next item, K and V rings that run across items, S and P V issued by a warp each. What differs:
+//  - all heads of a kv head's group share a tile of queries, row = token * G + head of the group, so that K and V are read once for the group: one decoded
+//    token of 32 / 8 heads reads its keys once instead of four times;
+//  - a tile of 128 keys is 128 / page size boxes, one a page, which land one behind the other in the tile (a page of 8 rows is one
+//    swizzle atom); the producer's lanes read the page numbers of the next tile while this one is under way;
+//  - P of a masked entry is 0, but 0 times a NaN that an earlier user left in the page is not: rows of V behind the sequence's end are
+//    zeroed in shared memory by the warp that issues P V, before it does;
+//  - each block works on one stretch of a line of all items (paged_plan.cuh); a piece of an item that was cut leaves normalised fp32 rows and
+//    their log-sum-exp to paged_combine_kernel.
+#include <type_traits>
+#include "common.cuh"
+#include "paged_plan.cuh"
+#include "params.cuh"
+
+namespace fa {
+
+template <int D>
+struct PagedSmem {
+    static constexpr int NS = (D == 128) ? 2 : 4;  // depth of the K ring and of the V ring
+    static constexpr int NQ = 2;                   // item slots
+    // TMEM columns as in the forward kernel
+    static constexpr bool POWN = D == 128;
+    static constexpr int NP = POWN ? 2 : 3;
+    static constexpr int tmem_o = POWN ? 256 : 384;
+    static __device__ int tmem_s(int g) { return POWN ? 0 : g % 3 * 128; }
+    static __device__ int tmem_p(int g) { return POWN ? 128 + (g & 1) * 64 : g % 3 * 128; }
+    static constexpr int TILE = kBlk * D * 2;
+    static constexpr int BOX = kBlk * 64 * 2;
+    static constexpr int NBOX = D / 64;
+    static constexpr int off_q = 0;  // NQ Q tiles
+    static constexpr int off_k = NQ * TILE;
+    static constexpr int off_v = off_k + NS * TILE;
+    static constexpr int off_ml = off_v + NS * TILE;             // float [NQ][2 groups][m, l][128]
+    static constexpr int off_info = off_ml + NQ * 4 * kBlk * 4;  // int32 [NQ][16]: see I_*
+    static constexpr int off_plan = off_info + NQ * 64;
+    static constexpr int off_bar = off_plan + int(sizeof(PagedPlan));
+    // item_full[NQ] item_empty[NQ] q_full[NQ] q_empty[NQ] ml_full[NQ] k_full[NS] k_empty[NS] v_full[NS] v_empty[NS]
+    // s_full[4] s_free[2] p_full[NP] pv_done[NP] o_full[2] o_free[2]
+    static constexpr int n_bar = 5 * NQ + 4 * NS + 6 + 2 * NP + 4;
+    static constexpr int off_misc = off_bar + n_bar * 8;  // tmem slot, abort flag
+    static constexpr int total = off_misc + 16;
+    static_assert(off_plan % 8 == 0 && off_bar % 8 == 0, "alignment");
+};
+static_assert(PagedSmem<128>::total <= 232448 && PagedSmem<64>::total <= 232448, "shared memory budget");
+static_assert(PagedSmem<128>::total > 116736 && PagedSmem<64>::total > 116736, "shares an SM");
+
+// What an item's slot says: number of its key tiles, the first one, whether there is an item (1, or -1: no more), kv head, first row of its tokens in
+// q and out, how many of them, position of the first one, the sequence's length, its prefix, the sequence, slot of the workspace (-1: straight to out)
+enum : int { I_TILES = 0, I_LO, I_MORE, I_HEAD, I_ROW, I_TOKENS, I_POS, I_LEN, I_FRONT, I_SEQ, I_PART };
+
+template <int D, bool BF16, bool SCORED>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const PagedParams p) {
+    using S = PagedSmem<D>;
+    constexpr int NS = S::NS, NQ = S::NQ, NP = S::NP;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t sbase = smem_u32(smem);
+    const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
+
+    volatile int* misc = reinterpret_cast<volatile int*>(smem + S::off_misc);  // [0] tmem, [1] abort
+    volatile int* info = reinterpret_cast<volatile int*>(smem + S::off_info);
+    PagedPlan& plan = *reinterpret_cast<PagedPlan*>(smem + S::off_plan);
+    const uint32_t bar0 = sbase + S::off_bar;
+    auto BAR = [&](int i) { return bar0 + 8u * uint32_t(i); };
+    constexpr int B_ITEMFULL = 0, B_ITEMEMPTY = NQ, B_QFULL = 2 * NQ, B_QEMPTY = 3 * NQ, B_MLFULL = 4 * NQ, B_KFULL = 5 * NQ,
+                  B_KEMPTY = B_KFULL + NS, B_VFULL = B_KEMPTY + NS, B_VEMPTY = B_VFULL + NS, B_SFULL = B_VEMPTY + NS,
+                  B_SFREE = B_SFULL + 4, B_PFULL = B_SFREE + 2, B_PVDONE = B_PFULL + NP, B_OFULL = B_PVDONE + NP, B_OFREE = B_OFULL + 2;
+    static_assert(B_OFREE + 2 == S::n_bar, "barriers");
+    Abort ab{misc + 1, p.status, p.wait_limit};
+
+    if (tid == 0) {
+        for (int s = 0; s < NQ; ++s) {
+            mbar_init(BAR(B_ITEMFULL + s), 1);
+            mbar_init(BAR(B_ITEMEMPTY + s), 15);  // producer, two MMA issuers, eight softmax warps, four epilogue warps
+            mbar_init(BAR(B_QFULL + s), 1);
+            mbar_init(BAR(B_QEMPTY + s), 1);
+            mbar_init(BAR(B_MLFULL + s), 8);
+        }
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(BAR(B_KFULL + s), 1);
+            mbar_init(BAR(B_KEMPTY + s), 1);
+            mbar_init(BAR(B_VFULL + s), 1);
+            mbar_init(BAR(B_VEMPTY + s), 1);
+        }
+        for (int s = 0; s < 4; ++s) mbar_init(BAR(B_SFULL + s), 1);
+        for (int s = 0; s < NP; ++s) {
+            mbar_init(BAR(B_PFULL + s), 4);  // here and below: one arrival a warp
+            mbar_init(BAR(B_PVDONE + s), 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(BAR(B_SFREE + s), 4);
+            mbar_init(BAR(B_OFULL + s), 1);
+            mbar_init(BAR(B_OFREE + s), 4);
+        }
+        fence_mbar_init();
+    }
+    // Rows without a query are multiplied all the same: as zeros, until another item's rows have been there
+    for (int i = tid; i < NQ * S::TILE / 16; i += kFwdThreads) reinterpret_cast<uint4*>(smem + S::off_q)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async();
+    wait_prerequisites();
+    if (warp == 13) {
+        take_tensor_memory(sbase + S::off_misc);
+    }
+    if (tid == 0) misc[1] = (status_is_fatal(*reinterpret_cast<volatile int*>(p.status)) || (sbase & 1023u) != 0) ? 1 : 0;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    launch_dependents();
+    const uint32_t tmem = uint32_t(misc[0]);
+    const bool aborted = misc[1] != 0;
+    uint16_t* const out = static_cast<uint16_t*>(p.out);
+    if (aborted) {
+        // an earlier launch ran into a time-out that the host has not yet cleared: the whole of the output becomes NaN, shared out by rows of a head
+        for (int64_t i = blockIdx.x; i < int64_t(p.T) * p.H; i += gridDim.x)
+            for (int d = tid; d < p.D; d += kFwdThreads) out[i / p.H * p.out_t + i % p.H * p.out_h + d] = 0xffffu;
+    } else {
+        paged_plan<kFwdThreads>(p, plan, int(gridDim.x));
+    }
+    const int worker = int(blockIdx.x);
+    const bool idle = aborted || worker >= plan.workers;
+
+    auto sQ = [&](int s) { return sbase + S::off_q + uint32_t(s) * S::TILE; };
+    auto sK = [&](int s) { return sbase + S::off_k + uint32_t(s) * S::TILE; };
+    auto sV = [&](int s) { return sbase + S::off_v + uint32_t(s) * S::TILE; };
+    if (warp >= 12) {
+        setmaxnreg_dec<kFwdServiceRegs>();
+        if (aborted) {
+        } else if (warp == 14) {
+            // ------------------------------ item scheduler ------------------------------
+            bool ok = true;
+            int k = 0;
+            if (!idle) {
+                paged_stretch(p, plan, worker, [&](const PagedWalk& walk, int, int lo, int hi, int part) {
+                    const int s = k % NQ, use = k / NQ;
+                    if (use > 0) ok = mbar_wait_warp(BAR(B_ITEMEMPTY + s), (use - 1) & 1, ab, ST_WAIT_TIMEOUT + 11);
+                    if (!ok) return false;
+                    if (lane == 0) {
+                        volatile int* it = info + 16 * s;
+                        it[I_TILES] = hi - lo;
+                        it[I_LO] = lo;
+                        it[I_MORE] = 1;
+                        it[I_HEAD] = walk.hk;
+                        it[I_ROW] = walk.s.start + walk.tile * p.tokens;
+                        it[I_TOKENS] = min(p.tokens, walk.s.n - walk.tile * p.tokens);
+                        it[I_POS] = walk.s.base + walk.tile * p.tokens;
+                        it[I_LEN] = walk.s.len;
+                        it[I_FRONT] = walk.s.front;
+                        it[I_SEQ] = walk.b;
+                        it[I_PART] = part;
+                        mbar_arrive(BAR(B_ITEMFULL + s));
+                    }
+                    __syncwarp();
+                    ++k;
+                    return true;
+                });
+            }
+            if (ok) {  // end marker
+                const int s = k % NQ, use = k / NQ;
+                if (use > 0) ok = mbar_wait_warp(BAR(B_ITEMEMPTY + s), (use - 1) & 1, ab, ST_WAIT_TIMEOUT + 11);
+                if (ok && lane == 0) {
+                    info[16 * s + I_MORE] = -1;
+                    mbar_arrive(BAR(B_ITEMFULL + s));
+                }
+            }
+        } else if (warp == 12) {
+            // ------------------------------ TMA producer ------------------------------
+            // Two walks over the block's tiles, as in the forward kernel: K (with its item's Q), up to kAhead tiles ahead of V.
+            tma_prefetch_desc(&tmQ);
+            tma_prefetch_desc(&tmK);
+            tma_prefetch_desc(&tmV);
+            constexpr int kAhead = 3;
+            const int rows = p.page < kBlk ? p.page : kBlk;  // of a box
+            const int boxes = kBlk / rows;                   // of a tile, 16 at most
+            bool ok = true, last = false;
+            int kk = -1, kt = 0, kT = 0, gk = 0, klo = 0, khk = 0, klen = 0, kseq = 0;
+            int vk = -1, vt = 0, vT = 0, gv = 0, vlo = 0, vhk = 0, vlen = 0, vseq = 0;
+            // Lane i: the page that box i of the tile comes from, or -1 behind the sequence's end.
+            auto pages_of = [&](int seq, int tile, int len) {
+                const int at = tile * kBlk + lane * rows;
+                if (lane >= boxes || at >= len) return -1;
+                const int page = p.table[int64_t(seq) * p.table_stride + (at >> p.log2_page)];
+                if (uint32_t(page) >= uint32_t(p.n_pages)) {
+                    atomicCAS(p.status, 0, ST_PAGED_PAGE);
+                    return p.n_pages;  // beyond the tensor: zeros
+                }
+                return page;
+            };
+            auto load = [&](const CUtensorMap* m, uint32_t dst, uint32_t bar, int pages, int tile, int hk, int len) {
+                const int left = len - tile * kBlk, n = left >= kBlk ? boxes : cdiv(left, rows);
+                mbar_expect_tx_elect(bar, uint32_t(n * rows) * 128u * S::NBOX);
+                const int row = p.page > kBlk ? tile * kBlk & (p.page - 1) : 0;
+                for (int i = 0; i < n; ++i) {
+                    const int page = __shfl_sync(0xffffffffu, pages, i);
+#pragma unroll
+                    for (int x = 0; x < S::NBOX; ++x)
+                        tma_load_4d_elect(dst + uint32_t(x) * S::BOX + uint32_t(i * rows) * 128u, m, bar, x * 64, hk, row, page);
+                }
+            };
+            int kpages = -1, vpages = -1;  // of the next tile of each walk
+            while (ok) {
+                while (vt == vT && vk < kk) {  // the V walk goes on to the next item
+                    if (vk >= 0 && lane == 0) mbar_arrive(BAR(B_ITEMEMPTY + vk % NQ));
+                    ++vk;
+                    volatile int* it = info + 16 * (vk % NQ);
+                    vt = 0;
+                    vT = uniform(it[I_TILES]);
+                    vlo = uniform(it[I_LO]);
+                    vhk = uniform(it[I_HEAD]);
+                    vlen = uniform(it[I_LEN]);
+                    vseq = uniform(it[I_SEQ]);
+                    if (vT > 0) vpages = pages_of(vseq, vlo, vlen);
+                }
+                if (last && gv == gk) break;
+                bool do_k = !last && gk - gv < kAhead;
+                if (do_k && kt == kT) {  // the next item: the rows of the one that had its slot must have left
+                    const int s = (kk + 1) % NQ, use = (kk + 1) / NQ;
+                    if (gv < gk && !(mbar_test_warp(BAR(B_ITEMFULL + s), use & 1) &&
+                                     (use == 0 || mbar_test_warp(BAR(B_QEMPTY + s), (use - 1) & 1)))) {
+                        do_k = false;
+                    } else {
+                        ok = mbar_wait_warp(BAR(B_ITEMFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 12);
+                        if (!ok) break;
+                        volatile int* it = info + 16 * s;
+                        if (uniform(it[I_MORE]) < 0) {
+                            last = true;
+                            continue;
+                        }
+                        if (use > 0) ok = mbar_wait_warp(BAR(B_QEMPTY + s), (use - 1) & 1, ab, ST_WAIT_TIMEOUT + 13);
+                        if (!ok) break;
+                        ++kk;
+                        kt = 0;
+                        kT = uniform(it[I_TILES]);
+                        klo = uniform(it[I_LO]);
+                        khk = uniform(it[I_HEAD]);
+                        klen = uniform(it[I_LEN]);
+                        kseq = uniform(it[I_SEQ]);
+                        const int row = uniform(it[I_ROW]);
+                        if (kT > 0) kpages = pages_of(kseq, klo, klen);
+                        mbar_expect_tx_elect(BAR(B_QFULL + s), uint32_t(p.tokens * p.G) * 128u * S::NBOX);
+                        for (int x = 0; x < S::NBOX; ++x)
+                            tma_load_4d_elect(sQ(s) + x * S::BOX, &tmQ, BAR(B_QFULL + s), x * 64, 0, khk, row);
+                        continue;  // (an item may have no tiles)
+                    }
+                }
+                if (do_k) {
+                    const int st = gk % NS, ug = gk / NS, pages = kpages;
+                    if (kt + 1 < kT) kpages = pages_of(kseq, klo + kt + 1, klen);
+                    if (ug > 0) ok = mbar_wait_warp(BAR(B_KEMPTY + st), (ug - 1) & 1, ab, ST_WAIT_TIMEOUT + 1);
+                    if (!ok) break;
+                    load(&tmK, sK(st), BAR(B_KFULL + st), pages, klo + kt, khk, klen);
+                    ++kt;
+                    ++gk;
+                } else {
+                    const int st = gv % NS, ug = gv / NS, pages = vpages;
+                    if (vt + 1 < vT) vpages = pages_of(vseq, vlo + vt + 1, vlen);
+                    if (ug > 0) ok = mbar_wait_warp(BAR(B_VEMPTY + st), (ug - 1) & 1, ab, ST_WAIT_TIMEOUT + 2);
+                    if (!ok) break;
+                    load(&tmV, sV(st), BAR(B_VFULL + st), pages, vlo + vt, vhk, vlen);
+                    ++vt;
+                    ++gv;
+                }
+            }
+        } else {
+            // ------------------------------ MMA issuers ------------------------------
+            //   warp 13: P*V(g) when P(g) is there; warp 15: S(g) when its buffer is free
+            const uint32_t utmem = uniform(int(tmem));
+            constexpr uint32_t idesc_s = make_idesc(BF16, 128, 128, false, false);
+            constexpr uint32_t idesc_pv = make_idesc(BF16, 128, D, false, true);
+            constexpr uint64_t desc_v = desc_mn_major(S::BOX);
+            bool ok = true;
+            int G = 0;           // tiles of all earlier items
+            int n0 = 0, n1 = 0;  // items in which the chains had tiles
+            for (int k = 0;; ++k) {
+                const int s = k % NQ, use = k / NQ;
+                ok = mbar_wait_warp(BAR(B_ITEMFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 12);
+                if (!ok) break;
+                const int T = uniform(info[16 * s + I_TILES]), lo = uniform(info[16 * s + I_LO]), len = uniform(info[16 * s + I_LEN]);
+                if (uniform(info[16 * s + I_MORE]) < 0) break;
+                if (warp == 15) {
+                    if (T > 0) ok = mbar_wait_warp(BAR(B_QFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 3);
+                    for (int g = G; g < G + T && ok; ++g) {
+                        const int st = g % NS;
+                        ok = mbar_wait_warp(BAR(B_KFULL + st), (g / NS) & 1, ab, ST_WAIT_TIMEOUT + 4);
+                        // the buffer: its scores have been read, or the P that took their place
+                        if (S::POWN && ok && g > 0) ok = mbar_wait_warp(BAR(B_SFREE + ((g - 1) & 1)), ((g - 1) >> 1) & 1, ab, ST_WAIT_TIMEOUT + 15);
+                        if (!S::POWN && ok && g >= NP) ok = mbar_wait_warp(BAR(B_PVDONE + g % NP), (g / NP - 1) & 1, ab, ST_WAIT_TIMEOUT + 15);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t tS = utmem + uint32_t(S::tmem_s(g)), q_tile = sQ(s), k_tile = sK(st);
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            const uint32_t off = uint32_t(kk >> 2) * S::BOX + uint32_t(kk & 3) * 32u;
+                            umma_ss(tS, smem_desc_at(kDescKMajor, q_tile + off), smem_desc_at(kDescKMajor, k_tile + off), idesc_s, kk > 0);
+                        }
+                        umma_commit(BAR(B_KEMPTY + st));
+                        umma_commit(BAR(B_SFULL + (g & 3)));
+                    }
+                } else {
+                    for (int t = 0; t < T; ++t) {
+                        const int g = G + t, st = g % NS, w = g & 1;
+                        const uint32_t tO = utmem + uint32_t(S::tmem_o + w * D), tP = utmem + uint32_t(S::tmem_p(g)), v_tile = sV(st);
+                        ok = mbar_wait_warp(BAR(B_VFULL + st), (g / NS) & 1, ab, ST_WAIT_TIMEOUT + 5);
+                        const int real = len - (lo + t) * kBlk;
+                        if (ok && real < kBlk) {  // rows behind the end: what was in the page, or in the stage
+#pragma unroll
+                            for (int x = 0; x < S::NBOX; ++x) {
+                                uint8_t* box = smem + S::off_v + st * S::TILE + x * S::BOX;
+                                for (int i = real * 8 + lane; i < kBlk * 8; i += 32) reinterpret_cast<uint4*>(box)[i] = make_uint4(0, 0, 0, 0);
+                            }
+                            fence_proxy_async();
+                            __syncwarp();
+                        }
+                        // The first P*V of a chain in an item overwrites its O: the epilogue of the last item that used it must have
+                        // read it. (o_full and o_free count the items in which the chain had tiles, on both sides.)
+                        const int n = w ? n1 : n0;
+                        if (ok && t < 2 && n > 0) ok = mbar_wait_warp(BAR(B_OFREE + w), (n - 1) & 1, ab, ST_WAIT_TIMEOUT + 14);
+                        if (ok) ok = mbar_wait_warp(BAR(B_PFULL + g % NP), (g / NP) & 1, ab, ST_WAIT_TIMEOUT + 6);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk)
+                            umma_ts(tO, tP + uint32_t(kk) * 8u, smem_desc_at(desc_v, v_tile + uint32_t(kk) * 2048u), idesc_pv,
+                                    (t > 1 || kk > 0) ? 1u : 0u);
+                        umma_commit(BAR(B_VEMPTY + st));
+                        umma_commit(BAR(B_PVDONE + g % NP));
+                        if (t + 2 >= T) {  // the chain's last tile
+                            umma_commit(BAR(B_OFULL + w));
+                            if (w) ++n1; else ++n0;
+                        }
+                    }
+                }
+                if (!ok) break;
+                G += T;
+                if (lane == 0) mbar_arrive(BAR(B_ITEMEMPTY + s));
+                __syncwarp();
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 8) {
+        // ------------------------------ epilogue group ------------------------------
+        setmaxnreg_dec<kFwdEpilogueRegs>();
+        const int r = tid & 127;
+        const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
+        const float c = SCORED ? 1.f : p.scale_log2;
+        const int tok = r / p.G, g_row = r - tok * p.G;
+        bool alive = !aborted;
+        if (alive && p.fill && p.starts) {
+            // rows in front of the first sequence and behind the last one
+            const int front = min(max(p.starts[0], 0), p.T), behind = max(min(p.starts[p.B], p.T), front);
+            const int rows = front + p.T - behind;
+            for (int64_t i = int64_t(blockIdx.x) * 4 + (warp & 3); i < int64_t(rows) * p.H; i += int64_t(gridDim.x) * 4) {
+                const int t = int(i / p.H), h = int(i % p.H);
+                for (int d = lane; d < p.D; d += 32) out[int64_t(t < front ? t : t - front + behind) * p.out_t + h * p.out_h + d] = 0;
+            }
+        }
+        int G = 0;           // tiles of all earlier items
+        int n0 = 0, n1 = 0;  // items in which the chains of group 0 and 1 had tiles
+        for (int k = 0; alive; ++k) {
+            const int s = k % NQ, use = k / NQ;
+            alive = mbar_wait_warp(BAR(B_ITEMFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 12);
+            if (!alive) break;
+            volatile int* it = info + 16 * s;
+            const int T = it[I_TILES], part = it[I_PART], hk = it[I_HEAD], row = it[I_ROW] + tok;
+            if (it[I_MORE] < 0) break;
+            const bool valid = tok < it[I_TOKENS];
+            // the only wait here that lasts as long as an item: it allows each of the tiles what another wait may last
+            const Abort item{ab.flag, ab.status, ab.limit * (T + 1)};
+            alive = mbar_wait_warp(BAR(B_MLFULL + s), use & 1, item, ST_WAIT_TIMEOUT + 16);
+            // an item without tiles: nobody has waited for its Q load yet, and its slot is about to be given away
+            if (alive && T == 0) alive = mbar_wait_warp(BAR(B_QFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 17);
+            const int we = G & 1;  // the chain that had the item's even tiles: index 0 below, 1 the other one
+            const int i0 = we ? n1 : n0, i1 = we ? n0 : n1;
+            if (alive && T > 0) alive = mbar_wait_warp(BAR(B_OFULL + we), i0 & 1, ab, ST_WAIT_TIMEOUT + 9);
+            if (alive && T > 1) alive = mbar_wait_warp(BAR(B_OFULL + (we ^ 1)), i1 & 1, ab, ST_WAIT_TIMEOUT + 9);
+            if (!alive) break;
+            tc_fence_after();
+            const float* ml = reinterpret_cast<const float*>(smem + S::off_ml) + s * (4 * kBlk);  // [2 groups][m, l][128]
+            const int even = we * (2 * kBlk), odd = 2 * kBlk - even;
+            const float m0 = ml[even + r], l0 = ml[even + kBlk + r], m1 = ml[odd + r], l1 = ml[odd + kBlk + r];
+            // Q has been read (every S of the item is complete) and so have m and l
+            if (warp == 8 && lane == 0) mbar_arrive(BAR(B_QEMPTY + s));
+            const float mt = fmaxf(m0, m1);
+            const float a0 = (m0 == -INFINITY) ? 0.f : fast_exp2((m0 - mt) * c);
+            const float a1 = (m1 == -INFINITY) ? 0.f : fast_exp2((m1 - mt) * c);
+            const float lt = l0 * a0 + l1 * a1;
+            const float inv = (lt > 0.f) ? 1.0f / lt : 0.f;
+            const float f0 = a0 * inv, f1 = a1 * inv;
+            // a chain in which the row had no key takes no part, whatever the values behind its mask are
+            const bool use0 = (T > 0) && (f0 != 0.f), use1 = (T > 1) && (f1 != 0.f);
+            const bool store = valid && misc[1] == 0;
+            if (part >= 0 && store)  // (a piece that went NaN says so: -inf would pass for a piece without keys)
+                p.part_lse[int64_t(part) * kBlk + r] = lt > 0.f ? fmaf(mt, c, log2f(lt)) : lt == lt ? -INFINITY : lt;
+            float* const rows_of_part = p.part_o + (int64_t(part) * kBlk + r) * D;
+            uint16_t* const row_out = out + int64_t(row) * p.out_t + int64_t(hk * p.G + g_row) * p.out_h;
+            const uint32_t tO0 = tmem + lane_base + uint32_t(S::tmem_o + we * D), tO1 = tmem + lane_base + uint32_t(S::tmem_o + (we ^ 1) * D);
+#pragma unroll 1
+            for (int q = 0; q < D / 16; ++q) {
+                uint32_t x0[16], x1[16];
+                // tcgen05.ld is warp-collective: always executed, the values are ignored when unused
+                tmem_ld16(tO0 + uint32_t(q) * 16u, x0);
+                tmem_ld16(tO1 + uint32_t(q) * 16u, x1);
+                tc_wait_ld();
+                if (q == D / 16 - 1) {  // O has been read: the MMA issuers may start another item's P*V
+                    tc_fence_before();
+                    if (T > 0) mbar_arrive_warp(BAR(B_OFREE + we), lane);
+                    if (T > 1) mbar_arrive_warp(BAR(B_OFREE + (we ^ 1)), lane);
+                }
+#pragma unroll
+                for (int y = 0; y < 16; ++y) {
+                    float v = 0.f;
+                    if (use0) v = __uint_as_float(x0[y]) * f0;
+                    if (use1) v = fmaf(__uint_as_float(x1[y]), f1, v);
+                    x0[y] = __float_as_uint(v);
+                }
+                if (store && 16 * q < p.D) {
+                    if (part >= 0) {
+#pragma unroll
+                        for (int y = 0; y < 4; ++y)
+                            *reinterpret_cast<uint4*>(rows_of_part + 16 * q + 4 * y) = make_uint4(x0[4 * y], x0[4 * y + 1], x0[4 * y + 2], x0[4 * y + 3]);
+                    } else {
+                        auto two = [&](int y) { return pack2<BF16>(__uint_as_float(x0[y]), __uint_as_float(x0[y + 1])); };
+                        uint4* dst = reinterpret_cast<uint4*>(row_out + 16 * q);
+                        dst[0] = make_uint4(two(0), two(2), two(4), two(6));
+                        dst[1] = make_uint4(two(8), two(10), two(12), two(14));
+                    }
+                }
+            }
+            G += T;
+            n0 += (we ? T > 1 : T > 0) ? 1 : 0;
+            n1 += (we ? T > 0 : T > 1) ? 1 : 0;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(BAR(B_ITEMEMPTY + s));
+        }
+    } else {
+        setmaxnreg_inc<kFwdSoftmaxRegs>();
+        // ------------------------------ softmax groups ------------------------------
+        const int w = warp >> 2;  // group
+        const int r = tid & 127;  // row inside the tile
+        const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
+        const float c = SCORED ? 1.f : p.scale_log2;
+        const uint32_t tO = tmem + lane_base + uint32_t(S::tmem_o + w * D);
+        const int tok = r / p.G, g_row = r - tok * p.G;
+        bool alive = !aborted;
+        int G = 0;  // tiles of all earlier items
+        for (int k = 0; alive; ++k) {
+            const int s = k % NQ, use = k / NQ;
+            alive = mbar_wait_warp(BAR(B_ITEMFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 12);
+            if (!alive) break;
+            volatile int* it = info + 16 * s;
+            const int T = it[I_TILES], lo = it[I_LO];
+            if (it[I_MORE] < 0) break;
+            const int pos0 = it[I_POS], len = it[I_LEN], front = it[I_FRONT];
+            const bool valid = tok < it[I_TOKENS];
+            const bool active = __any_sync(0xffffffffu, valid);  // does this warp hold a query at all?
+            const int pos = pos0 + tok;
+            const int last = min(max(pos, front - 1), len - 1);                // the last key that this row sees
+            const int all_see = min(max(pos0, front - 1), len - 1);            // and that all rows of the tile see
+            float slope = 0.f;
+            if constexpr (SCORED) {
+                if (p.score.slopes) slope = p.score.slopes[int64_t(it[I_HEAD]) * p.G + g_row] * kScoreLog2e;
+            }
+            const int t0 = (G ^ w) & 1;  // this group's first tile of the item
+            float m_run = -INFINITY, l_run = 0.f;
+
+            for (int t = t0; t < T && alive; t += 2) {
+                const int k0 = (lo + t) * kBlk;
+                const int g = G + t;
+                const uint32_t tS = tmem + lane_base + uint32_t(S::tmem_s(g)), tP = tmem + lane_base + uint32_t(S::tmem_p(g));
+                // P*V of the group's tile before: it has read its P and added to O
+                auto pv_before = [&] { return g < 2 || mbar_wait_warp(BAR(B_PVDONE + (g - 2) % NP), ((g - 2) / NP) & 1, ab, ST_WAIT_TIMEOUT + 8); };
+                alive = mbar_wait_warp(BAR(B_SFULL + (g & 3)), (g >> 2) & 1, ab, ST_WAIT_TIMEOUT + 7);
+                if (!alive) break;
+                tc_fence_after();
+                if (!active) {  // no row of this warp is a query: its lanes of P and O are never stored
+                    if (S::POWN) {
+                        mbar_arrive_warp(BAR(B_SFREE + w), lane);
+                        alive = pv_before();
+                        if (!alive) break;
+                    }
+                    mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
+                    continue;
+                }
+                uint32_t sr[128];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) tmem_ld32(tS + uint32_t(q) * 32u, sr + q * 32);
+                tc_wait_ld();
+                if (S::POWN) {
+                    tc_fence_before();
+                    mbar_arrive_warp(BAR(B_SFREE + w), lane);  // the next tile's scores may overwrite these
+                }
+                float* sc = reinterpret_cast<float*>(sr);
+                if constexpr (SCORED) {
+                    const Bias bias(slope, front == 0, pos0 - (k0 + kBlk - 1), pos0 + kBlk - 1 - k0);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) score_row(sc + 32 * q, p.score, bias, p.scale_log2, pos - k0 - 32 * q);
+                }
+                if (k0 + kBlk - 1 > all_see) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const uint32_t keep = first_bits(last - k0 + 1 - 32 * q);
+                        if (__any_sync(0xffffffffu, keep != ~0u)) {
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) sc[32 * q + x] = (keep & (1u << x)) ? sc[32 * q + x] : -INFINITY;
+                        }
+                    }
+                }
+                float mxa[8];
+#pragma unroll
+                for (int a = 0; a < 8; ++a) mxa[a] = max3(sc[a], sc[8 + a], sc[16 + a]);
+#pragma unroll
+                for (int x = 24; x < 120; x += 16) {
+#pragma unroll
+                    for (int a = 0; a < 8; ++a) mxa[a] = max3(mxa[a], sc[x + a], sc[x + 8 + a]);
+                }
+#pragma unroll
+                for (int a = 0; a < 8; ++a) mxa[a] = fmaxf(mxa[a], sc[120 + a]);
+                const float mx = fmaxf(max3(mxa[0], mxa[1], mxa[2]), max3(max3(mxa[3], mxa[4], mxa[5]), mxa[6], mxa[7]));
+                float m_new = fmaxf(m_run, mx);
+                // lazy rescale: keep the old reference point while the new maximum is within 2^8 of it
+                const bool need = (m_new - m_run) * c > 8.0f;
+                if (!need) m_new = m_run;
+                if (S::POWN) {  // this tile's P overwrites that one's
+                    alive = pv_before();
+                    if (!alive) break;
+                    tc_fence_after();
+                }
+                if (__any_sync(0xffffffffu, need)) {
+                    const float alpha = need ? fast_exp2((m_run - m_new) * c) : 1.0f;
+                    l_run *= alpha;
+                    if (t > t0) {
+                        if (!S::POWN) {
+                            alive = pv_before();
+                            if (!alive) break;
+                            tc_fence_after();
+                        }
+#pragma unroll 1
+                        for (int q = 0; q < D / 16; ++q) {
+                            uint32_t orr[16];
+                            tmem_ld16(tO + uint32_t(q) * 16u, orr);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int x = 0; x < 16; ++x) orr[x] = __float_as_uint(__uint_as_float(orr[x]) * alpha);
+                            tmem_st16(tO + uint32_t(q) * 16u, orr);
+                        }
+                        tc_wait_st();
+                    }
+                }
+                m_run = m_new;
+                const float mneg = (m_run == -INFINITY) ? 0.f : -m_run * c;
+                // exp2(s*c - m*c) on packed pairs
+                const uint64_t c2 = pack_f2(c, c), mneg2 = pack_f2(mneg, mneg);
+                uint64_t lacc0 = pack_f2(0.f, 0.f), lacc1 = lacc0;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const uint64_t x2 = fma_f2(pack_f2(sc[32 * q + 2 * x], sc[32 * q + 2 * x + 1]), c2, mneg2);
+                        float x0, x1;
+                        unpack_f2(x2, x0, x1);
+                        const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+                        if (x & 1) lacc1 = add_f2(lacc1, pack_f2(p0, p1)); else lacc0 = add_f2(lacc0, pack_f2(p0, p1));
+                        pk[x] = pack2<BF16>(p0, p1);
+                    }
+                    tmem_st16(tP + uint32_t(q) * 16u, pk);
+                }
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
+                {
+                    float a0, a1, b0, b1;
+                    unpack_f2(lacc0, a0, a1);
+                    unpack_f2(lacc1, b0, b1);
+                    l_run += (a0 + a1) + (b0 + b1);
+                }
+            }
+            if (!alive) break;
+            float* ml = reinterpret_cast<float*>(smem + S::off_ml) + s * (4 * kBlk) + w * (2 * kBlk) + r;
+            ml[0] = m_run;
+            ml[kBlk] = l_run;
+            mbar_arrive_warp(BAR(B_MLFULL + s), lane);
+            G += T;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(BAR(B_ITEMEMPTY + s));
+        }
+    }
+
+    // ------------------------------ tear-down ------------------------------
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 13) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Merges the pieces of the items that a cut went through: O = sum_s w_s O_s with w_s = 2^(lse_s - lse). Block w looks after the item
+// that the cut before worker w goes through first. A piece whose lse is NaN or +inf makes the row its own, as in fwd_combine_kernel. All
+// sums in fp32, in the order of the pieces. One warp per row, lane l owns columns l, l + 32, ...
+template <bool BF16>
+__global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p, int most_workers) {
+    __shared__ PagedPlan plan;
+    // The lengths were complete before the attention kernel let this one begin, so that the plan need not wait for that kernel.
+    paged_plan<256>(p, plan, most_workers);
+    wait_prerequisites();
+    launch_dependents();
+    const int w = int(blockIdx.x), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    PagedWalk walk;
+    if (!paged_first_cut(p, plan, w, walk) || status_is_fatal(*reinterpret_cast<volatile int*>(p.status))) return;
+    int pieces = 0;
+    paged_pieces(p, plan, w, walk, [&](int) { ++pieces; });
+    if (pieces < 2) return;  // one piece that has all tiles has gone straight to the output
+    const int Dk = p.D > 64 ? 128 : 64;
+    const int tokens = min(p.tokens, walk.s.n - walk.tile * p.tokens);
+    for (int r = warp; r < tokens * p.G; r += 8) {
+        const int tok = r / p.G, g = r - tok * p.G;
+        float top = -INFINITY, total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+        bool spoilt = false;
+        paged_pieces(p, plan, w, walk, [&](int slot) {
+            const float lse = p.part_lse[int64_t(slot) * kBlk + r];
+            spoilt |= !(lse < INFINITY);
+            top = fmaxf(top, lse);
+        });
+        if (top != -INFINITY || spoilt)
+            paged_pieces(p, plan, w, walk, [&](int slot) {
+                const int64_t at = int64_t(slot) * kBlk + r;
+                const float lse = p.part_lse[at], wgt = !spoilt ? fast_exp2(lse - top) : lse < INFINITY ? 0.f : 1.f;
+                if (wgt == 0.f) return;
+                total += wgt;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (lane + 32 * i < p.D) acc[i] = fmaf(wgt, p.part_o[at * Dk + lane + 32 * i], acc[i]);
+            });
+        const float inv = total > 0.f ? 1.f / total : 0.f;
+        uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(walk.s.start + walk.tile * p.tokens + tok) * p.out_t + int64_t(walk.hk * p.G + g) * p.out_h;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + 32 * i < p.D) out[lane + 32 * i] = uint16_t(pack2<BF16>(acc[i] * inv, 0.f));
+    }
+}
+
+// ---- host launchers (called from paged.cu) ----------------------------------------------
+template <int D, bool BF16, bool SCORED>
+static cudaError_t launch_paged_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {
+    auto kern = paged_fwd_kernel<D, BF16, SCORED>;
+    constexpr int smem = PagedSmem<D>::total;
+    static SmemAllowed allowed;
+    cudaError_t e = allow_smem(kern, smem, allowed);
+    if (e != cudaSuccess) return e;
+    e = launch_overlapping(kern, dim3(workers), kFwdThreads, smem, stream, tq, tk, tv, p);
+    if (e != cudaSuccess) return e;
+    return launch_overlapping(paged_combine_kernel<BF16>, dim3(workers), 256, 0, stream, p, workers);
+}
+
+cudaError_t launch_paged_fwd(bool bf16, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {
+    auto pick = [&](auto d, auto scored) {
+        constexpr int kD = decltype(d)::value;
+        constexpr bool kScored = decltype(scored)::value;
+        return bf16 ? launch_paged_t<kD, true, kScored>(tq, tk, tv, p, workers, stream) : launch_paged_t<kD, false, kScored>(tq, tk, tv, p, workers, stream);
+    };
+    using std::integral_constant;
+    const bool scored = p.score.cap > 0.f || p.score.slopes;
+    if (p.D == 128) return scored ? pick(integral_constant<int, 128>{}, std::true_type{}) : pick(integral_constant<int, 128>{}, std::false_type{});
+    return scored ? pick(integral_constant<int, 64>{}, std::true_type{}) : pick(integral_constant<int, 64>{}, std::false_type{});
+}
+
+}  // namespace fa

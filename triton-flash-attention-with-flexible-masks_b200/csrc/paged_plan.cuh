@@ -1,0 +1,266 @@
+// How the attention over a paged cache is shared out, worked out by every block for itself from the lengths in device memory (the host does not
+// know them, and a captured call has to follow them).
+//
+// An item is a tile of queries (tokens_per_tile new tokens of a sequence, all heads of a kv head's group) of one kv head. Its weight is the
+// number of keys that its last token sees, and a constant for what an item costs besides its tiles. The items, in the order sequence, kv head,
+// tile, lie behind one another on a line of length `total`, and worker w of n gets the stretch [w total / n, (w + 1) total / n) of it: equal work
+// whatever the lengths, with at most n - 1 cuts. An item that a cut goes through is computed in pieces, whose fp32 rows the second kernel merges.
+// Where whole items, one a worker, are done as soon, nothing is cut (`keyed` false: all weights are 1).
+#pragma once
+#include "common.cuh"
+#include "params.cuh"
+
+namespace fa {
+
+constexpr int kPagedGroups = 1024;   // entries of the table of sums: a sequence each, or several
+constexpr int kPagedItemCost = 256;  // of an item, in keys
+constexpr int kPagedPieceKeys = 512; // a worker's stretch is at least this long
+constexpr int kPagedMergeTiles = 6;  // of the second kernel, in tiles of 128 keys
+
+struct PagedPlan {
+    long long total;
+    int workers;
+    int keyed;
+    int group;  // sequences an entry of `sums`
+    int pad;
+    long long warp_sums[32], warp_items[32];
+    int warp_max[32];
+    long long sums[kPagedGroups + 1];  // of what lies before an entry's sequences
+};
+
+__host__ __device__ __forceinline__ int paged_clamp(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
+
+// One sequence of the batch. Every number is taken into its range: whatever the caller's tensors hold, nothing outside of them is touched.
+struct PagedSeq {
+    int start, n;  // first row and number of new tokens
+    int len;       // cached tokens, the new ones among them
+    int base;      // position of the first new one (below 0: those see nothing)
+    int front;     // leading keys that all see
+    int tiles;     // of queries
+};
+
+__host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
+    PagedSeq s;
+    int end;
+    if (p.starts) {
+        s.start = paged_clamp(p.starts[b], 0, p.T);
+        end = paged_clamp(p.starts[b + 1], s.start, p.T);
+    } else {
+        s.start = b;
+        end = b + 1;
+    }
+    s.n = end - s.start;
+    s.len = paged_clamp(p.lens[b], 0, p.capacity);
+    s.base = s.len - s.n;
+    s.front = p.prefix ? paged_clamp(p.prefix[b], 0, s.len) : 0;
+    s.tiles = cdiv(s.n, p.tokens);
+    return s;
+}
+
+// Keys that tile i's last token sees.
+__host__ __device__ __forceinline__ int paged_keys(const PagedParams& p, const PagedSeq& s, int i) {
+    const long long end = s.base + (long long)(i + 1) * p.tokens;
+    const int seen = end < s.len ? int(end) : s.len;
+    return seen > s.front ? seen : s.front;
+}
+
+// The weights of the first m tiles of one head together.
+__host__ __device__ __forceinline__ long long paged_weight(const PagedParams& p, const PagedSeq& s, int m, bool keyed) {
+    if (!keyed) return m;
+    // the tiles but the last end at base + (i + 1) tokens < len; those below `front` see that many keys
+    const int inner = m < s.tiles ? m : s.tiles - 1;
+    long long sum = (long long)m * kPagedItemCost;
+    if (inner > 0) {
+        const long long ahead = (long long)s.front - s.base;
+        const long long fewer = ahead > 0 ? (ahead + p.tokens - 1) / p.tokens - 1 : 0, below = fewer < inner ? fewer : inner;
+        const long long rest = inner - below;
+        sum += below * s.front + rest * s.base + (long long)p.tokens * (rest * (below + 1) + rest * (rest - 1) / 2);
+    }
+    return m == s.tiles && m > 0 ? sum + s.len : sum;
+}
+
+// Weights of all items together, their number and the longest sequence's length, to the plan's numbers.
+__host__ __device__ __forceinline__ void paged_share_out(PagedPlan& plan, long long weight, long long items, int longest, int most_workers) {
+    long long workers = weight / (kPagedPieceKeys + kPagedItemCost);
+    workers = workers < 1 ? 1 : workers > most_workers ? most_workers : workers;
+    plan.keyed = items > most_workers || cdiv(longest, kBlk) > weight / workers / kBlk + kPagedMergeTiles;
+    plan.workers = int(plan.keyed ? workers : items);
+    plan.total = plan.keyed ? weight : items;
+}
+
+// All threads of the block (a multiple of 32, at most 1024, that divides 2 * kPagedGroups). Ends with a barrier.
+template <int kThreads>
+__device__ __forceinline__ void paged_plan(const PagedParams& p, PagedPlan& plan, int most_workers) {
+    constexpr int kOwn = kPagedGroups / kThreads, kWarps = kThreads / 32;
+    static_assert(kOwn * kThreads == kPagedGroups && kOwn >= 1, "groups of a thread");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = cdiv(p.B, kPagedGroups), first = threadIdx.x * kOwn;
+    long long weight[kOwn], items[kOwn], w = 0, n = 0;
+    int longest = 0;
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) {
+        weight[o] = items[o] = 0;
+        for (int b = (first + o) * group; b < min(p.B, (first + o + 1) * group); ++b) {
+            const PagedSeq s = paged_seq(p, b);
+            if (p.lens[b] > p.capacity || p.lens[b] < 0) atomicCAS(p.status, 0, ST_PAGED_LENGTH);
+            weight[o] += p.Hk * paged_weight(p, s, s.tiles, true);
+            items[o] += (long long)p.Hk * s.tiles;
+            if (s.tiles > 0) longest = max(longest, s.len);
+        }
+        w += weight[o];
+        n += items[o];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        w += __shfl_xor_sync(0xffffffffu, w, o);
+        n += __shfl_xor_sync(0xffffffffu, n, o);
+        longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+    }
+    if (lane == 0) {
+        plan.warp_sums[warp] = w;
+        plan.warp_items[warp] = n;
+        plan.warp_max[warp] = longest;
+    }
+    __syncthreads();
+    w = n = 0;
+    longest = 0;
+    for (int i = 0; i < kWarps; ++i) {
+        w += plan.warp_sums[i];
+        n += plan.warp_items[i];
+        longest = max(longest, plan.warp_max[i]);
+    }
+    PagedPlan own;
+    paged_share_out(own, w, n, longest, most_workers);
+    const bool keyed = own.keyed;
+    long long mine = 0;
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) mine += keyed ? weight[o] : items[o];
+    long long before = mine;  // an inclusive sum over the warp, then the warps before
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += x;
+    }
+    __syncthreads();  // (the sums above have been read)
+    if (lane == 31) plan.warp_sums[warp] = before;
+    __syncthreads();
+    before -= mine;
+    for (int i = 0; i < warp; ++i) before += plan.warp_sums[i];
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) {
+        plan.sums[first + o] = before;
+        before += keyed ? weight[o] : items[o];
+    }
+    if (threadIdx.x == 0) {
+        plan.total = plan.sums[kPagedGroups] = own.total;
+        plan.workers = own.workers;
+        plan.keyed = own.keyed;
+        plan.group = group;
+    }
+    __syncthreads();
+}
+
+// Where worker w's stretch begins.
+__host__ __device__ __forceinline__ long long paged_cut(const PagedPlan& plan, int w) {
+    // total < 2^49 (see api.cu) and w <= 2^14
+    return plan.total * w / plan.workers;
+}
+
+// A walk over the items from a point of the line on.
+struct PagedWalk {
+    PagedSeq s;
+    int b, hk, tile;
+    long long at;  // where the item begins
+
+    // The item that covers x, 0 <= x < total.
+    __host__ __device__ __forceinline__ void find(const PagedParams& p, const PagedPlan& plan, long long x) {
+        int lo = 0, hi = kPagedGroups;  // sums[lo] <= x < sums[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (plan.sums[mid] <= x) lo = mid; else hi = mid;
+        }
+        long long rem = x - plan.sums[lo];
+        b = lo * plan.group;
+        long long head;
+        for (;; ++b) {
+            if (b >= p.B) {  // (somebody writes the lengths while the kernel reads them)
+                s = PagedSeq{};
+                hk = tile = 0;
+                at = x;
+                return;
+            }
+            s = paged_seq(p, b);
+            head = paged_weight(p, s, s.tiles, plan.keyed);
+            if (rem < head * p.Hk) break;
+            rem -= head * p.Hk;
+        }
+        hk = int(rem / head);
+        rem -= hk * head;
+        int t0 = 0, t1 = s.tiles;  // weight(t0) <= rem < weight(t1)
+        while (t1 - t0 > 1) {
+            const int mid = (t0 + t1) >> 1;
+            if (paged_weight(p, s, mid, plan.keyed) <= rem) t0 = mid; else t1 = mid;
+        }
+        tile = t0;
+        at = x - rem + paged_weight(p, s, t0, plan.keyed);
+    }
+    __host__ __device__ __forceinline__ long long end(const PagedParams& p, const PagedPlan& plan) const {
+        return at + (plan.keyed ? paged_keys(p, s, tile) + kPagedItemCost : 1);
+    }
+    // The next item; there is one.
+    __host__ __device__ __forceinline__ void next(const PagedParams& p, const PagedPlan& plan) {
+        at = end(p, plan);
+        if (++tile < s.tiles) return;
+        tile = 0;
+        if (++hk < p.Hk) return;
+        hk = 0;
+        do s = ++b < p.B ? paged_seq(p, b) : PagedSeq{}; while (s.tiles == 0 && b < p.B);
+    }
+    __host__ __device__ __forceinline__ int key_tiles(const PagedParams& p) const { return cdiv(paged_keys(p, s, tile), kBlk); }
+    // The item's key tile at point x of the line: the pieces on both sides of a cut at x meet there.
+    __host__ __device__ __forceinline__ int key_tile_at(const PagedParams& p, const PagedPlan& plan, long long x) const {
+        const int n = key_tiles(p);
+        if (x <= at) return 0;
+        if (x >= end(p, plan)) return n;
+        const long long t = (x - at - kPagedItemCost) / kBlk;
+        return t < 0 ? 0 : t > n ? n : int(t);
+    }
+};
+
+// The pieces of worker w's stretch, in their order: emit(walk, key tiles of the item, first and last + 1 of the piece, slot of the workspace or -1 for a
+// piece that is the whole item) until one says false. A piece without tiles is left out, but for the one that begins an item without any,
+// whose rows are zeros.
+template <class Emit>
+__host__ __device__ __forceinline__ void paged_stretch(const PagedParams& p, const PagedPlan& plan, int w, Emit emit) {
+    const long long x0 = paged_cut(plan, w), x1 = paged_cut(plan, w + 1);
+    PagedWalk walk;
+    walk.find(p, plan, x0);
+    for (long long from = x0;;) {
+        const int n = walk.key_tiles(p), lo = walk.key_tile_at(p, plan, from), hi = walk.key_tile_at(p, plan, x1);
+        if (walk.s.tiles > 0 && (hi > lo || (n == 0 && from <= walk.at)) && !emit(walk, n, lo, hi, hi - lo == n ? -1 : 2 * w + (lo == 0 ? 1 : 0))) return;
+        if (walk.end(p, plan) >= x1 || walk.b >= p.B) return;
+        walk.next(p, plan);
+        from = walk.at;
+    }
+}
+
+// Does the cut before worker w go through an item, as the first one that does? `walk` is at that item then.
+__host__ __device__ __forceinline__ bool paged_first_cut(const PagedParams& p, const PagedPlan& plan, int w, PagedWalk& walk) {
+    if (w <= 0 || w >= plan.workers) return false;
+    const long long x = paged_cut(plan, w);
+    walk.find(p, plan, x);
+    return walk.s.tiles > 0 && walk.at < x && (w == 1 || walk.at >= paged_cut(plan, w - 1));
+}
+
+// The pieces of the item at `walk`, which the cut before worker w goes through first: each(slot) in their order.
+template <class Each>
+__host__ __device__ __forceinline__ void paged_pieces(const PagedParams& p, const PagedPlan& plan, int w, const PagedWalk& walk, Each each) {
+    const int n = walk.key_tiles(p);
+    for (int v = w, lo = 0; lo < n; ++v) {
+        const int hi = v < plan.workers ? walk.key_tile_at(p, plan, paged_cut(plan, v)) : n;
+        if (hi > lo) each(2 * (v - 1) + (lo == 0 ? 1 : 0));
+        lo = hi;
+    }
+}
+
+}  // namespace fa

@@ -93,6 +93,28 @@ struct F32Params {
     ScoreArgs score;  // the instances for attention_scored: cap and slopes
 };
 
+// Attention over a paged cache (paged_fwd.cu), and the tokens' way into it (paged_append.cu)
+struct PagedParams {
+    const int32_t* table;   // [B, pages of a sequence]
+    int64_t table_stride;
+    const int32_t* lens;    // [B] cached tokens, the new ones among them
+    const int32_t* starts;  // [B + 1] first row of each sequence; null: one token each
+    const int32_t* prefix;  // [B], or null: leading keys that all tokens of a sequence see
+    void* out;              // [T, H, D]
+    int64_t out_t, out_h;   // element strides
+    float* part_o;          // [2 * workers, 128, 64 or 128] fp32 rows of the pieces
+    float* part_lse;        // [2 * workers, 128]
+    int B, T, H, Hk, G, D;
+    int tokens;             // of a tile: 128 / G
+    int page, log2_page, n_pages;
+    int capacity;           // tokens that the table has room for
+    int fill;               // rows of no sequence are set to 0
+    float scale_log2;
+    int* status;
+    long long wait_limit;
+    ScoreArgs score;
+};
+
 // A number for the current CUDA context that no other context of the process ever has, or 0 (api.cu).
 uint64_t context_number();
 

@@ -17,6 +17,8 @@ enum : int {
     ST_OK = 0,
     ST_WAIT_TIMEOUT = 100,     // + role id (see the kernels): a bounded mbarrier wait ran out
     ST_ID_RANGE = 200,         // a negative query id does not fit in int32
+    ST_PAGED_PAGE = 201,       // a page number of a paged cache is not one
+    ST_PAGED_LENGTH = 202,     // a sequence's length is negative or beyond its row of the page table
 };
 // A time-out leaves the device in an unknown state: every later launch refuses to compute until the
 // host has read and cleared the word. An id out of range only concerns the call that passed it.
@@ -214,6 +216,12 @@ __device__ __forceinline__ void tmem_relinquish() {
 __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
                  : "memory");
+}
+// All columns, by one warp; their address goes to `smem_dst`. Between the kernel's wait for the one before it and the barrier behind
+// which it lets the next one begin (see launch_dependents below).
+__device__ __forceinline__ void take_tensor_memory(uint32_t smem_dst) {
+    tmem_alloc(smem_dst, 512);
+    tmem_relinquish();
 }
 __device__ __forceinline__ void tc_fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

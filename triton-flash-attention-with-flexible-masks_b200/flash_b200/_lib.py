@@ -17,7 +17,8 @@ EXPORTS = (
     "fa_version", "fa_error_string", "fa_padded_rows", "fa_plan_bytes", "fa_plan_build", "fa_fwd",
     "fa_bwd_delta", "fa_bwd_dkdv", "fa_bwd_dq", "fa_debug_mask", "fa_classify_tile", "fa_fwd_static_plan",
     "fa_debug_wait_timeout", "fa_group_rows", "fa_permute_rows", "fa_fwd_splits", "fa_fwd_workspace_bytes", "fa_fwd_split",
-    "fa_plan_optional", "fa_bwd", "fa_plan_build_scored", "fa_fwd_scored", "fa_bwd_scored",
+    "fa_plan_optional", "fa_bwd", "fa_plan_build_scored", "fa_fwd_scored", "fa_bwd_scored", "fa_paged_append",
+    "fa_paged_workspace_bytes", "fa_paged_fwd", "fa_debug_paged_pieces",
 )
 
 
@@ -40,6 +41,16 @@ class Ids(ctypes.Structure):
 
 class Scores(ctypes.Structure):
     _fields_ = [("softcap", ctypes.c_float), ("slopes", ctypes.c_void_p), ("prefix", ctypes.c_void_p)]
+
+
+class PagedCache(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "Hk", "D", "dtype", "pages", "page_size", "table_pages")] + [
+        ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("lens", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3)]
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [("ptr", ctypes.c_void_p), ("stride", ctypes.c_int64 * 2)]
 
 
 _lib = None
@@ -91,6 +102,15 @@ def load():
     lib.fa_fwd_scored.argtypes = [P, S, T, T, T, T, vp, vp, ctypes.c_int32, vp, size, vp, vp]
     lib.fa_bwd_scored.restype = i32
     lib.fa_bwd_scored.argtypes = [P, S, T, T, T, T, T, vp, vp, T, T, T, vp, vp, vp]
+    C, R = ctypes.POINTER(PagedCache), ctypes.POINTER(Rows)
+    lib.fa_paged_append.restype = i32
+    lib.fa_paged_append.argtypes = [C, ctypes.c_int32, vp, R, R, vp, vp]
+    lib.fa_paged_workspace_bytes.restype = i32
+    lib.fa_paged_workspace_bytes.argtypes = [C, ctypes.POINTER(size)]
+    lib.fa_paged_fwd.restype = i32
+    lib.fa_paged_fwd.argtypes = [C, ctypes.c_int32, ctypes.c_int32, vp, ctypes.c_float, S, R, R, ctypes.c_int32, vp, size, vp, vp]
+    lib.fa_debug_paged_pieces.restype = i32
+    lib.fa_debug_paged_pieces.argtypes = [ctypes.c_int32] * 5 + [vp] * 3 + [ctypes.c_int32, vp, ctypes.c_int32]
     lib.fa_debug_mask.restype = i32
     lib.fa_debug_mask.argtypes = [P, vp, vp, vp, vp]
     lib.fa_fwd_static_plan.restype = i32

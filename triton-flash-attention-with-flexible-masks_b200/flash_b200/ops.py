@@ -110,6 +110,10 @@ def check_status(device=None):
                                    "results of that call are invalid")
             if code == 200:
                 raise RuntimeError("flash_b200: a negative query id does not fit in int32")
+            if code == 201:
+                raise RuntimeError("flash_b200: a page table names a page that the cache does not have")
+            if code == 202:
+                raise RuntimeError("flash_b200: a length of a paged cache is negative or beyond its row of the page table")
             raise RuntimeError(f"flash_b200: kernel status {code}")
 
 
