@@ -607,7 +607,7 @@ static cudaError_t launch_f32_rows(int which, const F32Params& p, bool overlap, 
     constexpr int room = 232448 / ((S::fwd_bytes) + kStatic), per_sm = room < 4 ? room : 4;
     const int64_t rows = int64_t(cdiv(mk.M, 32)) * p.H * p.B, cols = int64_t(cdiv(mk.N, 32)) * p.Hk * p.B, slots = int64_t(per_sm) * sms;
     const bool small = which == 0 ? rows <= slots : 10 * (rows + cols) <= 13 * slots;
-    if (p.score.on) return small ? launch_f32_t<D, 16, true>(which, p, overlap, stream) : launch_f32_t<D, 32, true>(which, p, overlap, stream);
+    if (p.score.kind != SCORE_PLAIN) return small ? launch_f32_t<D, 16, true>(which, p, overlap, stream) : launch_f32_t<D, 32, true>(which, p, overlap, stream);
     return small ? launch_f32_t<D, 16, false>(which, p, overlap, stream) : launch_f32_t<D, 32, false>(which, p, overlap, stream);
 }
 

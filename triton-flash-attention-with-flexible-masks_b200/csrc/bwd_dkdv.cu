@@ -112,14 +112,15 @@ struct Walk {
     }
 };
 
-// SCORED: as in the forward; with a cap dS takes the factor 1 - tanh^2, which P is multiplied by once it has been packed for dV.
-template <int D, bool BF16, bool SCORED = false>
+// KIND: as in the forward; with a cap dS takes the factor 1 - tanh^2, which P is multiplied by once it has been packed for dV.
+template <int D, bool BF16, int KIND = SCORE_PLAIN>
 __global__ void __launch_bounds__(kDkdvThreads, 1)
 bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
                 const __grid_constant__ CUtensorMap tmdK, const __grid_constant__ CUtensorMap tmdV,
                 const DkdvParams p) {
     using S = DkdvSmem<D>;
+    constexpr bool SCORED = KIND != SCORE_PLAIN;
     constexpr int NQ = S::NQ, NDO = S::NDO;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -561,35 +562,54 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 } else if constexpr (SCORED) {
                     const float slope = p.score.slopes ? p.score.slopes[hk * G + cg] * kScoreLog2e : 0.f;
                     const Bias bias(slope, mk.causal && front == 0, qb0 + mk.gap - (k0 + kBlk - 1), qb0 + kBlk - 1 + mk.gap - k0);
-                    const bool capped = p.score.cap > 0.f, beyond = capped && any_beyond<32>(pr, p.score.most);
-                    const float d = float(q0 + 2 * (lane & 3) + mk.gap - (k0 + 32 * (warp & 3) + (lane >> 2))), sd = bias.s * d;
+                    const bool beyond = KIND == SCORE_CAPPED && any_beyond<32>(pr, p.score.most);
+                    const float d = float(q0 + 2 * (lane & 3) + mk.gap - (k0 + 32 * (warp & 3) + (lane >> 2)));
                     uint32_t bits[4];
 #pragma unroll
                     for (int y = 0; y < 4; ++y) bits[y] = __shfl_sync(0xffffffffu, keep, 8 * y + (lane >> 2)) >> (2 * (lane & 3));
+                    // y is exponent + lse from here on to the place where P is made
+                    auto walk = [&](auto capped) {
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const float2 l2 = *reinterpret_cast<const float2*>(vlse + 8 * n);
-                        const uint64_t nl2 = pack_f2(-l2.x, -l2.y);
+                        for (int n = 0; n < 4; ++n) {
+                            const float2 l2 = *reinterpret_cast<const float2*>(vlse + 8 * n);
+                            uint64_t b2 = pack_f2(fmaf(bias.line, d + float(8 * n), -l2.x), fmaf(bias.line, d + float(8 * n + 1), -l2.y));
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            float* x = pr + 16 * (y >> 1) + 4 * n + 2 * (y & 1);
-                            uint64_t v = pack_f2(x[0], x[1]), f = pack_f2(1.f, 1.f);
-                            if (capped) {
-                                v = cap_pair(v, p.score, beyond);
-                                f = cap_slope(v, p.score);
-                                v = add_f2(v, nl2);
-                            } else {
-                                v = fma_f2(v, pack_f2(c, c), nl2);
+                            for (int y = 0; y < 4; ++y) {
+                                float* x = pr + 16 * (y >> 1) + 4 * n + 2 * (y & 1);
+                                const uint64_t s2 = pack_f2(x[0], x[1]);
+                                uint64_t v, f = 0;
+                                if constexpr (KIND == SCORE_CAPPED) {
+                                    v = capped(s2);
+                                    f = cap_slope(v, p.score);
+                                    v = add_f2(v, b2);
+                                } else {
+                                    v = fma_f2(s2, pack_f2(c, c), b2);
+                                }
+                                if (y < 3) b2 = add_f2(b2, pack_f2(-8.f * bias.line, -8.f * bias.line));
+                                float x0, x1;
+                                unpack_f2(v, x0, x1);
+                                if (bias.both) {
+                                    x0 = fmaf(bias.s, fabsf(d + float(8 * n - 8 * y)), x0);
+                                    x1 = fmaf(bias.s, fabsf(d + float(8 * n - 8 * y + 1)), x1);
+                                }
+                                x0 = fast_exp2(x0);
+                                x1 = fast_exp2(x1);
+                                if (flagged) {
+                                    x0 = (bits[y] & (1u << (8 * n))) ? x0 : 0.f;
+                                    x1 = (bits[y] & (2u << (8 * n))) ? x1 : 0.f;
+                                }
+                                pk[8 * (y >> 1) + 2 * n + (y & 1)] = pack2<BF16>(x0, x1);
+                                if constexpr (KIND == SCORE_CAPPED) {
+                                    unpack_f2(mul_f2(pack_f2(x0, x1), f), x[0], x[1]);
+                                } else {
+                                    x[0] = x0;
+                                    x[1] = x1;
+                                }
                             }
-                            if (bias.s != 0.f) v = add_f2(v, bias.pair(d, sd, float(8 * n - 8 * y), 1.f));
-                            float x0, x1;
-                            unpack_f2(v, x0, x1);
-                            x0 = (bits[y] & (1u << (8 * n))) ? fast_exp2(x0) : 0.f;
-                            x1 = (bits[y] & (2u << (8 * n))) ? fast_exp2(x1) : 0.f;
-                            pk[8 * (y >> 1) + 2 * n + (y & 1)] = pack2<BF16>(x0, x1);
-                            unpack_f2(mul_f2(pack_f2(x0, x1), f), x[0], x[1]);
                         }
-                    }
+                    };
+                    if (beyond) walk([&](uint64_t s2) { return cap_pair(s2, p.score, true); });
+                    else walk([&](uint64_t s2) { return cap_pair(s2, p.score, false); });
                 } else {
                     const uint64_t c2 = pack_f2(c, c);
 #pragma unroll
@@ -742,11 +762,11 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     }
 }
 
-template <int D, bool BF16, bool SCORED>
+template <int D, bool BF16, int KIND>
 static cudaError_t launch_dkdv_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                                  const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
                                  const DkdvParams& p, int num_sms, cudaStream_t stream) {
-    auto kern = bwd_dkdv_kernel<D, BF16, SCORED>;
+    auto kern = bwd_dkdv_kernel<D, BF16, KIND>;
     constexpr int smem = DkdvSmem<D>::total;
     static SmemAllowed allowed;
     cudaError_t e = allow_smem(kern, smem, allowed);
@@ -760,15 +780,18 @@ static cudaError_t launch_dkdv_t(const CUtensorMap& tq, const CUtensorMap& tk, c
 cudaError_t launch_bwd_dkdv(int D, bool bf16, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                             const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
                             const DkdvParams& p, int num_sms, cudaStream_t stream) {
-    auto pick = [&](auto d, auto scored) {
-        constexpr int kD = decltype(d)::value;
-        constexpr bool kScored = decltype(scored)::value;
-        return bf16 ? launch_dkdv_t<kD, true, kScored>(tq, tk, tv, tdo, tdk, tdv, p, num_sms, stream)
-                    : launch_dkdv_t<kD, false, kScored>(tq, tk, tv, tdo, tdk, tdv, p, num_sms, stream);
+    auto pick = [&](auto d, auto kind) {
+        constexpr int kD = decltype(d)::value, kKind = decltype(kind)::value;
+        return bf16 ? launch_dkdv_t<kD, true, kKind>(tq, tk, tv, tdo, tdk, tdv, p, num_sms, stream)
+                    : launch_dkdv_t<kD, false, kKind>(tq, tk, tv, tdo, tdk, tdv, p, num_sms, stream);
     };
     using std::integral_constant;
-    if (D == 128) return p.score.on ? pick(integral_constant<int, 128>{}, std::true_type{}) : pick(integral_constant<int, 128>{}, std::false_type{});
-    return p.score.on ? pick(integral_constant<int, 64>{}, std::true_type{}) : pick(integral_constant<int, 64>{}, std::false_type{});
+    auto of = [&](auto d) {
+        if (p.score.kind == SCORE_CAPPED) return pick(d, integral_constant<int, SCORE_CAPPED>{});
+        if (p.score.kind == SCORE_BIAS) return pick(d, integral_constant<int, SCORE_BIAS>{});
+        return pick(d, integral_constant<int, SCORE_PLAIN>{});
+    };
+    return D == 128 ? of(integral_constant<int, 128>{}) : of(integral_constant<int, 64>{});
 }
 
 }  // namespace fa

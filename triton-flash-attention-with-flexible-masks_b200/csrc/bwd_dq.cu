@@ -64,13 +64,14 @@ struct DqWalk {
     }
 };
 
-// SCORED: as in the forward; with a cap dS takes the factor 1 - tanh^2.
-template <int D, int NW, bool BF16, bool SCORED = false>
+// KIND: as in the forward; with a cap dS takes the factor 1 - tanh^2.
+template <int D, int NW, bool BF16, int KIND = SCORE_PLAIN>
 __global__ void __launch_bounds__(DqSmem<D, NW>::THREADS, 1)
 bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
               const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
               const __grid_constant__ CUtensorMap tmdQ, const DqParams p) {
     using S = DqSmem<D, NW>;
+    constexpr bool SCORED = KIND != SCORE_PLAIN;
     constexpr int NSK = S::NSK, NC = S::COLS;
     constexpr bool kOne = D == 128;  // one warp issues all MMAs
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -481,26 +482,45 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                     }
                     if constexpr (SCORED) {
                         const Bias bias(slope, mk.causal && front == 0, q0 + mk.gap - (kb0 + kBlk - 1), q0 + kBlk - 1 + mk.gap - kb0);
-                        const bool capped = p.score.cap > 0.f, beyond = capped && any_beyond<32>(pr + 32 * q, p.score.most);
-                        const float d = float(row + mk.gap - k0 - 32 * q), sd = bias.s * d;
+                        const bool beyond = KIND == SCORE_CAPPED && any_beyond<32>(pr + 32 * q, p.score.most);
+                        const float d = float(row + mk.gap - k0 - 32 * q);
+                        auto walk = [&](auto capped) {
+                            uint64_t b2 = pack_f2(fmaf(bias.line, d, -lse), fmaf(bias.line, d - 1.f, -lse));
 #pragma unroll
-                        for (int x = 0; x < 32; x += 2) {
-                            float* y = pr + 32 * q + x;
-                            uint64_t v = pack_f2(y[0], y[1]), f = pack_f2(1.f, 1.f);
-                            if (capped) {
-                                v = cap_pair(v, p.score, beyond);
-                                f = cap_slope(v, p.score);
-                                v = add_f2(v, nl2);
-                            } else {
-                                v = fma_f2(v, c2, nl2);
+                            for (int x = 0; x < 32; x += 2) {
+                                float* y = pr + 32 * q + x;
+                                const uint64_t s2 = pack_f2(y[0], y[1]);
+                                uint64_t v, f = 0;
+                                if constexpr (KIND == SCORE_CAPPED) {
+                                    v = capped(s2);
+                                    f = cap_slope(v, p.score);
+                                    v = add_f2(v, b2);
+                                } else {
+                                    v = fma_f2(s2, c2, b2);
+                                }
+                                if (x < 30) b2 = add_f2(b2, pack_f2(-2.f * bias.line, -2.f * bias.line));
+                                float x0, x1;
+                                unpack_f2(v, x0, x1);
+                                if (bias.both) {
+                                    x0 = fmaf(bias.s, fabsf(d - float(x)), x0);
+                                    x1 = fmaf(bias.s, fabsf(d - float(x + 1)), x1);
+                                }
+                                x0 = fast_exp2(x0);
+                                x1 = fast_exp2(x1);
+                                if (flagged) {
+                                    x0 = (keep[q] & (1u << x)) ? x0 : 0.f;
+                                    x1 = (keep[q] & (2u << x)) ? x1 : 0.f;
+                                }
+                                if constexpr (KIND == SCORE_CAPPED) {
+                                    unpack_f2(mul_f2(pack_f2(x0, x1), f), y[0], y[1]);
+                                } else {
+                                    y[0] = x0;
+                                    y[1] = x1;
+                                }
                             }
-                            if (bias.s != 0.f) v = add_f2(v, bias.pair(d, sd, float(-x), -1.f));
-                            float x0, x1;
-                            unpack_f2(v, x0, x1);
-                            x0 = (keep[q] & (1u << x)) ? fast_exp2(x0) : 0.f;
-                            x1 = (keep[q] & (2u << x)) ? fast_exp2(x1) : 0.f;
-                            unpack_f2(mul_f2(pack_f2(x0, x1), f), y[0], y[1]);
-                        }
+                        };
+                        if (beyond) walk([&](uint64_t s2) { return cap_pair(s2, p.score, true); });
+                        else walk([&](uint64_t s2) { return cap_pair(s2, p.score, false); });
                         continue;
                     }
 #pragma unroll
@@ -614,11 +634,11 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     if (tid == 0) wait_prerequisites();
 }
 
-template <int D, int NW, bool BF16, bool SCORED>
+template <int D, int NW, bool BF16, int KIND>
 static cudaError_t launch_dq_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                                const CUtensorMap& tdo, const CUtensorMap& tdq, const DqParams& p, int num_sms,
                                bool overlap, cudaStream_t stream) {
-    auto kern = bwd_dq_kernel<D, NW, BF16, SCORED>;
+    auto kern = bwd_dq_kernel<D, NW, BF16, KIND>;
     constexpr int smem = DqSmem<D, NW>::total;
     static SmemAllowed allowed;
     cudaError_t e = allow_smem(kern, smem, allowed);
@@ -643,11 +663,15 @@ cudaError_t launch_bwd_dq(int D, bool bf16, const CUtensorMap& tq, const CUtenso
                           cudaStream_t stream) {
     auto pick = [&](auto d, auto nw) {
         constexpr int kD = decltype(d)::value, kWarps = decltype(nw)::value;
-        if (p.score.on)
-            return bf16 ? launch_dq_t<kD, kWarps, true, true>(tq, tk, tv, tdo, tdq, p, num_sms, overlap, stream)
-                        : launch_dq_t<kD, kWarps, false, true>(tq, tk, tv, tdo, tdq, p, num_sms, overlap, stream);
-        return bf16 ? launch_dq_t<kD, kWarps, true, false>(tq, tk, tv, tdo, tdq, p, num_sms, overlap, stream)
-                    : launch_dq_t<kD, kWarps, false, false>(tq, tk, tv, tdo, tdq, p, num_sms, overlap, stream);
+        auto of = [&](auto kind) {
+            constexpr int kKind = decltype(kind)::value;
+            return bf16 ? launch_dq_t<kD, kWarps, true, kKind>(tq, tk, tv, tdo, tdq, p, num_sms, overlap, stream)
+                        : launch_dq_t<kD, kWarps, false, kKind>(tq, tk, tv, tdo, tdq, p, num_sms, overlap, stream);
+        };
+        using std::integral_constant;
+        if (p.score.kind == SCORE_CAPPED) return of(integral_constant<int, SCORE_CAPPED>{});
+        if (p.score.kind == SCORE_BIAS) return of(integral_constant<int, SCORE_BIAS>{});
+        return of(integral_constant<int, SCORE_PLAIN>{});
     };
     using std::integral_constant;
     if (D == 128) return pick(integral_constant<int, 128>{}, integral_constant<int, 8>{});

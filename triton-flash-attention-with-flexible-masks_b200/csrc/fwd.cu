@@ -98,12 +98,13 @@ static_assert(FwdSmem<128>::total > 116736 && FwdSmem<64>::total > 116736, "shar
 //    and their log-sum-exp go to the workspace, and fwd_combine_kernel merges them.
 // Such calls are bound by reading K and V (16 tokens of 32 / 8 heads of 128 against 4500 keys: 295 MB, 45 us at the
 // copy rate; 127 us with a tile per head, 55 us packed) or, with few heads, by the longest item's chain of tiles.
-// SCORED: the scores pass through score_row (scores.cuh) and are in the log2 domain from there on; the causal mask leaves a prefix visible.
-template <int D, bool BF16, bool SHORT, bool SCORED = false>
+// KIND: other than SCORE_PLAIN, the scores pass through score_row (scores.cuh) and are in the log2 domain from there on, and the causal mask may leave a prefix visible.
+template <int D, bool BF16, bool SHORT, int KIND = SCORE_PLAIN>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
            const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const FwdParams p) {
     using S = FwdSmem<D>;
+    constexpr bool SCORED = KIND != SCORE_PLAIN;
     constexpr int NS = S::NS, NQ = S::NQ, NP = S::NP;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -674,8 +675,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                 if constexpr (SCORED) {
                     const int first = SHORT ? 0 : qb * kBlk, last = SHORT ? mk.M - 1 : qb * kBlk + kBlk - 1;  // rows of the tile, and perhaps more
                     const Bias bias(slope, mk.causal && front == 0, first + mk.gap - (k0 + kBlk - 1), last + mk.gap - k0);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) score_row(sc + 32 * q, p.score, bias, p.scale_log2, row + mk.gap - k0 - 32 * q);
+                    score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, row + mk.gap - k0, valid);
                 }
 
                 if (fl & (TILE_BOUND | TILE_DOC)) {
@@ -891,10 +891,10 @@ cudaError_t launch_fwd_combine(bool bf16, const CombineParams& p, cudaStream_t s
 }
 
 // ---- host launcher (called from api.cu) -------------------------------------------------
-template <int D, bool BF16, bool SHORT, bool SCORED>
+template <int D, bool BF16, bool SHORT, int KIND>
 static cudaError_t launch_fwd_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                                 const CUtensorMap& to, const FwdParams& p, int num_sms, cudaStream_t stream) {
-    auto kern = fwd_kernel<D, BF16, SHORT, SCORED>;
+    auto kern = fwd_kernel<D, BF16, SHORT, KIND>;
     constexpr int smem = FwdSmem<D>::total;
     static SmemAllowed allowed;
     cudaError_t e = allow_smem(kern, smem, allowed);
@@ -911,11 +911,15 @@ cudaError_t launch_fwd(int D, bool bf16, const CUtensorMap& tq, const CUtensorMa
     auto pick = [&](auto d, auto shrt) {
         constexpr int kD = decltype(d)::value;
         constexpr bool kShort = decltype(shrt)::value;
-        if (p.score.on)
-            return bf16 ? launch_fwd_t<kD, true, kShort, true>(tq, tk, tv, to, p, num_sms, stream)
-                        : launch_fwd_t<kD, false, kShort, true>(tq, tk, tv, to, p, num_sms, stream);
-        return bf16 ? launch_fwd_t<kD, true, kShort, false>(tq, tk, tv, to, p, num_sms, stream)
-                    : launch_fwd_t<kD, false, kShort, false>(tq, tk, tv, to, p, num_sms, stream);
+        auto of = [&](auto kind) {
+            constexpr int kKind = decltype(kind)::value;
+            return bf16 ? launch_fwd_t<kD, true, kShort, kKind>(tq, tk, tv, to, p, num_sms, stream)
+                        : launch_fwd_t<kD, false, kShort, kKind>(tq, tk, tv, to, p, num_sms, stream);
+        };
+        using std::integral_constant;
+        if (p.score.kind == SCORE_CAPPED) return of(integral_constant<int, SCORE_CAPPED>{});
+        if (p.score.kind == SCORE_BIAS) return of(integral_constant<int, SCORE_BIAS>{});
+        return of(integral_constant<int, SCORE_PLAIN>{});
     };
     using std::integral_constant;
     const bool shrt = p.pack > 1 || p.ns > 1;

@@ -9,8 +9,9 @@
 //    token of 32 / 8 heads reads its keys once instead of four times;
 //  - a tile of 128 keys is 128 / page size boxes, one a page, which land one behind the other in the tile (a page of 8 rows is one
 //    swizzle atom); the producer's lanes read the page numbers of the next tile while this one is under way;
-//  - P of a masked entry is 0, but 0 times a NaN that an earlier user left in the page is not: rows of V behind the sequence's end are
-//    zeroed in shared memory by the warp that issues P V, before it does;
+//  - P of a masked entry is 0, but 0 times a NaN that an earlier user left in the page is not: rows of K and V behind the sequence's end are
+//    zeroed in shared memory by the warp that issues the product, before it does (of K, for what a masked score is must not tell the other rows
+//    which form of the cap to take);
 //  - each block works on one stretch of a line of all items (paged_plan.cuh); a piece of an item that was cut leaves normalised fp32 rows and
 //    their log-sum-exp to paged_combine_kernel.
 #include <type_traits>
@@ -54,11 +55,12 @@ static_assert(PagedSmem<128>::total > 116736 && PagedSmem<64>::total > 116736, "
 // q and out, how many of them, position of the first one, the sequence's length, its prefix, the sequence, slot of the workspace (-1: straight to out)
 enum : int { I_TILES = 0, I_LO, I_MORE, I_HEAD, I_ROW, I_TOKENS, I_POS, I_LEN, I_FRONT, I_SEQ, I_PART };
 
-template <int D, bool BF16, bool SCORED>
+template <int D, bool BF16, int KIND>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const PagedParams p) {
     using S = PagedSmem<D>;
+    constexpr bool SCORED = KIND != SCORE_PLAIN;
     constexpr int NS = S::NS, NQ = S::NQ, NP = S::NP;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -274,6 +276,15 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             constexpr uint32_t idesc_s = make_idesc(BF16, 128, 128, false, false);
             constexpr uint32_t idesc_pv = make_idesc(BF16, 128, D, false, true);
             constexpr uint64_t desc_v = desc_mn_major(S::BOX);
+            // Rows behind the sequence's end hold what was in the page, or in the stage.
+            auto zero_behind = [&](int tile, int real) {
+                if (real >= kBlk) return;
+#pragma unroll
+                for (int x = 0; x < S::NBOX; ++x)
+                    for (int i = real * 8 + lane; i < kBlk * 8; i += 32) reinterpret_cast<uint4*>(smem + tile + x * S::BOX)[i] = make_uint4(0, 0, 0, 0);
+                fence_proxy_async();
+                __syncwarp();
+            };
             bool ok = true;
             int G = 0;           // tiles of all earlier items
             int n0 = 0, n1 = 0;  // items in which the chains had tiles
@@ -292,6 +303,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         if (S::POWN && ok && g > 0) ok = mbar_wait_warp(BAR(B_SFREE + ((g - 1) & 1)), ((g - 1) >> 1) & 1, ab, ST_WAIT_TIMEOUT + 15);
                         if (!S::POWN && ok && g >= NP) ok = mbar_wait_warp(BAR(B_PVDONE + g % NP), (g / NP - 1) & 1, ab, ST_WAIT_TIMEOUT + 15);
                         if (!ok) break;
+                        zero_behind(S::off_k + st * S::TILE, len - (lo + g - G) * kBlk);
                         tc_fence_after();
                         const uint32_t tS = utmem + uint32_t(S::tmem_s(g)), q_tile = sQ(s), k_tile = sK(st);
 #pragma unroll
@@ -307,16 +319,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         const int g = G + t, st = g % NS, w = g & 1;
                         const uint32_t tO = utmem + uint32_t(S::tmem_o + w * D), tP = utmem + uint32_t(S::tmem_p(g)), v_tile = sV(st);
                         ok = mbar_wait_warp(BAR(B_VFULL + st), (g / NS) & 1, ab, ST_WAIT_TIMEOUT + 5);
-                        const int real = len - (lo + t) * kBlk;
-                        if (ok && real < kBlk) {  // rows behind the end: what was in the page, or in the stage
-#pragma unroll
-                            for (int x = 0; x < S::NBOX; ++x) {
-                                uint8_t* box = smem + S::off_v + st * S::TILE + x * S::BOX;
-                                for (int i = real * 8 + lane; i < kBlk * 8; i += 32) reinterpret_cast<uint4*>(box)[i] = make_uint4(0, 0, 0, 0);
-                            }
-                            fence_proxy_async();
-                            __syncwarp();
-                        }
+                        if (ok) zero_behind(S::off_v + st * S::TILE, len - (lo + t) * kBlk);
                         // The first P*V of a chain in an item overwrites its O: the epilogue of the last item that used it must have
                         // read it. (o_full and o_free count the items in which the chain had tiles, on both sides.)
                         const int n = w ? n1 : n0;
@@ -498,8 +501,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 float* sc = reinterpret_cast<float*>(sr);
                 if constexpr (SCORED) {
                     const Bias bias(slope, front == 0, pos0 - (k0 + kBlk - 1), pos0 + kBlk - 1 - k0);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) score_row(sc + 32 * q, p.score, bias, p.scale_log2, pos - k0 - 32 * q);
+                    score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, pos - k0, valid);
                 }
                 if (k0 + kBlk - 1 > all_see) {
 #pragma unroll
@@ -647,9 +649,9 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p,
 }
 
 // ---- host launchers (called from paged.cu) ----------------------------------------------
-template <int D, bool BF16, bool SCORED>
+template <int D, bool BF16, int KIND>
 static cudaError_t launch_paged_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {
-    auto kern = paged_fwd_kernel<D, BF16, SCORED>;
+    auto kern = paged_fwd_kernel<D, BF16, KIND>;
     constexpr int smem = PagedSmem<D>::total;
     static SmemAllowed allowed;
     cudaError_t e = allow_smem(kern, smem, allowed);
@@ -660,15 +662,17 @@ static cudaError_t launch_paged_t(const CUtensorMap& tq, const CUtensorMap& tk, 
 }
 
 cudaError_t launch_paged_fwd(bool bf16, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {
-    auto pick = [&](auto d, auto scored) {
-        constexpr int kD = decltype(d)::value;
-        constexpr bool kScored = decltype(scored)::value;
-        return bf16 ? launch_paged_t<kD, true, kScored>(tq, tk, tv, p, workers, stream) : launch_paged_t<kD, false, kScored>(tq, tk, tv, p, workers, stream);
+    auto pick = [&](auto d, auto kind) {
+        constexpr int kD = decltype(d)::value, kKind = decltype(kind)::value;
+        return bf16 ? launch_paged_t<kD, true, kKind>(tq, tk, tv, p, workers, stream) : launch_paged_t<kD, false, kKind>(tq, tk, tv, p, workers, stream);
     };
     using std::integral_constant;
-    const bool scored = p.score.cap > 0.f || p.score.slopes;
-    if (p.D == 128) return scored ? pick(integral_constant<int, 128>{}, std::true_type{}) : pick(integral_constant<int, 128>{}, std::false_type{});
-    return scored ? pick(integral_constant<int, 64>{}, std::true_type{}) : pick(integral_constant<int, 64>{}, std::false_type{});
+    auto of = [&](auto d) {
+        if (p.score.kind == SCORE_CAPPED) return pick(d, integral_constant<int, SCORE_CAPPED>{});
+        if (p.score.kind == SCORE_BIAS && p.score.slopes) return pick(d, integral_constant<int, SCORE_BIAS>{});
+        return pick(d, integral_constant<int, SCORE_PLAIN>{});  // (a prefix alone is part of the mask)
+    };
+    return p.D == 128 ? of(integral_constant<int, 128>{}) : of(integral_constant<int, 64>{});
 }
 
 }  // namespace fa

@@ -1,47 +1,64 @@
 // What attention_scored does to a score between Q K^T and the softmax, in the log2 domain that the tensor-core kernels work in:
 //   y_ij = log2(e) * (cap * tanh(s_ij * sm_scale / cap) - slope_h * |i + gap - j|)
-// without a cap y = log2(e) * (s * sm_scale - ...). The gradient through the cap is the factor 1 - tanh^2 = 1 - (y before the bias / A)^2,
-// A = cap * log2(e).
+// without a cap y = log2(e) * (s * sm_scale - ...). The gradient through the cap is the factor 1 - tanh^2 = 1 - (y before the bias / a)^2,
+// a = cap * log2(e).
 //
-// tanh: where a warp's scores are all at most `cap` (after the scale), x * (an even polynomial of x), fitted by interpolation of
-// tanh(x) / x over x^2 in [0, 1] at Chebyshev's points; relative error 7.3e-7. That is eight packed FMAs for two scores and no
-// special-function unit, which the exponentials keep busy. Elsewhere 1 - 2 / (1 + e^2x), whose absolute error of some 2^-23 is relative to a
-// tanh of at least 0.76 in one of them. Close to 0 the second form would lose the small scores of a large cap.
+// The capped score is s * (an even polynomial of s) where all of a warp's are at most 0.75 cap: tanh(x) / x over x^2 in [0, 0.5625] by interpolation at
+// Chebyshev's points, relative error 7.1e-7, with a and sm_scale / cap multiplied into its coefficients. That is six packed FMAs for two
+// scores and nothing of the special-function unit, which the exponentials keep busy. Elsewhere it is a - 2 a / (1 + 2^(2 log2(e) x)), whose absolute error
+// is some 2^-22 of a; close to 0 that form would lose the small scores of a large cap.
 #pragma once
 #include "common.cuh"
 
 namespace fa {
 
+// Instances of the attention kernels
+enum : int {
+    SCORE_PLAIN = 0,   // attention
+    SCORE_BIAS = 1,    // a bias, a prefix, or both (a bias of 0 costs one packed addition for two scores)
+    SCORE_CAPPED = 2,  // the same and a cap
+};
+
+constexpr int kTanhTerms = 5;
+
 struct ScoreArgs {
     const float* slopes;  // [H], null: none
     float cap;            // 0: none
-    int on;               // any of cap, slopes and the mask's prefix is given
+    int kind;             // SCORE_*
+    float poly[kTanhTerms];  // capped score = s (poly[0] + poly[1] s^2 + ...) up to |s| = most
+    float most;
+    float k2e;            // 2 log2(e) sm_scale / cap
     float k;              // sm_scale / cap
-    float k2e;            // 2 log2(e) k
-    float a;              // cap log2(e)
-    float inv_a;
-    float most;           // |s| up to which tanh is the polynomial: 1 / k
+    float a, inv_a;       // cap log2(e)
 };
 
 constexpr float kScoreLog2e = 1.4426950408889634f;
 
 inline ScoreArgs make_score_args(float cap, const float* slopes, bool prefix, float sm_scale) {
+    constexpr double kTanh[kTanhTerms] = {0.999999424, -0.333281921, 0.132584621, -0.0500416086, 0.0129166518};
+    // largest x at which the term of x^(2i) is below 2e-7 of the sum
+    constexpr double kWithout[kTanhTerms] = {0.0, 7.7e-4, 0.035, 0.126, 0.25};
     ScoreArgs s{};
     s.slopes = slopes;
     s.cap = cap;
-    s.on = cap > 0.f || slopes || prefix;
+    s.kind = cap > 0.f ? SCORE_CAPPED : slopes || prefix ? SCORE_BIAS : SCORE_PLAIN;
     if (cap > 0.f) {
-        s.k = sm_scale / cap;
-        s.k2e = 2.f * kScoreLog2e * s.k;
-        s.a = cap * kScoreLog2e;
-        s.inv_a = 1.f / s.a;
-        s.most = 1.f / s.k;
+        const double a = double(cap) * 1.4426950408889634, k = double(sm_scale) / cap;
+        double power = a * k, most = 0.75;
+        for (int i = 0; i < kTanhTerms; ++i, power *= k * k) {
+            const double c = kTanh[i] * power, size = c < 0 ? -c : c;
+            // a coefficient that fp32 cannot hold is left out, with the scores that need it
+            if (i > 0 && !(size > 1e-37 && size < 1e37)) most = most < kWithout[i] ? most : kWithout[i];
+            else s.poly[i] = float(c);
+        }
+        s.most = float(most / k < 1e38 ? most / k : 1e38);
+        s.k = float(k < 1e37 ? k : 1e37);
+        s.k2e = float(2.885390081777927 * k < 1e38 ? 2.885390081777927 * k : 1e38);
+        s.a = float(a);
+        s.inv_a = float(1.0 / a);
     }
     return s;
 }
-
-// tanh(x) = x (c0 + c1 x^2 + ... + c5 x^10) for |x| <= 1
-__device__ constexpr float kTanhPoly[6] = {0.999999395f, -0.333289514f, 0.132807206f, -0.0515859884f, 0.0167208552f, -0.00305822904f};
 
 __device__ __forceinline__ float fast_rcp(float x) {
     float y;
@@ -49,31 +66,32 @@ __device__ __forceinline__ float fast_rcp(float x) {
     return y;
 }
 
-// Does any of a warp's scores (N a thread) ask for the second form?
+// Does any of a warp's scores (N a thread) lie beyond the polynomial?
 template <int N>
 __device__ __forceinline__ bool any_beyond(const float* v, float most) {
-    float m0 = 0.f, m1 = 0.f;
+    float m[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int x = 0; x < N; x += 4) {
-        m0 = max3(m0, fabsf(v[x]), fabsf(v[x + 1]));
-        m1 = max3(m1, fabsf(v[x + 2]), fabsf(v[x + 3]));
+    for (int x = 0; x < N; x += 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = max3(m[i], fabsf(v[x + 2 * i]), fabsf(v[x + 2 * i + 1]));
     }
-    return __any_sync(0xffffffffu, fmaxf(m0, m1) > most);
+    return __any_sync(0xffffffffu, fmaxf(max3(m[0], m[1], m[2]), m[3]) > most);
 }
 
-// log2(e) cap tanh(s sm_scale / cap) of two scores
-__device__ __forceinline__ uint64_t cap_small(uint64_t s2, const ScoreArgs& a) {
-    const uint64_t x2 = mul_f2(s2, pack_f2(a.k, a.k)), u2 = mul_f2(x2, x2);
-    uint64_t t = pack_f2(kTanhPoly[5], kTanhPoly[5]);
+// poly[0] + poly[1] s^2 + ... of two scores
+__device__ __forceinline__ uint64_t cap_poly(uint64_t s2, const ScoreArgs& a) {
+    const uint64_t u2 = mul_f2(s2, s2);
+    uint64_t t = pack_f2(a.poly[kTanhTerms - 1], a.poly[kTanhTerms - 1]);
 #pragma unroll
-    for (int i = 4; i >= 0; --i) t = fma_f2(t, u2, pack_f2(kTanhPoly[i], kTanhPoly[i]));
-    return mul_f2(mul_f2(x2, pack_f2(a.a, a.a)), t);
+    for (int i = kTanhTerms - 2; i >= 0; --i) t = fma_f2(t, u2, pack_f2(a.poly[i], a.poly[i]));
+    return t;
 }
+// the capped score, whatever its size
 __device__ __forceinline__ float cap_any(float s, const ScoreArgs& a) {
     return fmaf(-2.f * a.a, fast_rcp(1.f + fast_exp2(s * a.k2e)), a.a);
 }
 __device__ __forceinline__ uint64_t cap_pair(uint64_t s2, const ScoreArgs& a, bool beyond) {
-    if (!beyond) return cap_small(s2, a);
+    if (!beyond) return mul_f2(s2, cap_poly(s2, a));
     float s0, s1;
     unpack_f2(s2, s0, s1);
     return pack_f2(cap_any(s0, a), cap_any(s1, a));
@@ -89,38 +107,44 @@ __device__ __forceinline__ uint64_t cap_slope(uint64_t y2, const ScoreArgs& a) {
 // The bias of the entries of one tile. The distance i + gap - j of an entry that the masks keep has one sign over most tiles (with a causal
 // mask and no prefix over all): there the bias is linear in it, elsewhere the distance's size is taken.
 struct Bias {
-    float s;    // -log2(e) slope, or +: of tiles whose keys all lie ahead; 0: no bias
-    bool both;  // both signs occur
+    float s;     // -log2(e) slope, or +: of tiles whose keys all lie ahead; 0: no bias
+    float line;  // the same where the bias is linear, 0 where both signs occur
+    bool both;
     // least and most: distances of the tile's corners. slope: log2(e) times the head's
     __device__ __forceinline__ Bias(float slope, bool never_ahead, int least, int most) {
         both = slope != 0.f && !never_ahead && least < 0 && most > 0;
         s = !never_ahead && !both && least < 0 ? slope : -slope;
-    }
-    // of distances d + x and d + x + step (x and step known to the compiler); sd = s * d
-    __device__ __forceinline__ uint64_t pair(float d, float sd, float x, float step) const {
-        if (both) return pack_f2(s * fabsf(d + x), s * fabsf(d + (x + step)));
-        return pack_f2(fmaf(s, x, sd), fmaf(s, x + step, sd));
+        line = both ? 0.f : s;
     }
 };
 
-// 32 neighbouring scores of one row, in place, to the log2 domain; d: distance of the first one
-__device__ __forceinline__ void score_row(float* v, const ScoreArgs& a, const Bias& bias, float c, int dist) {
-    const float d = float(dist), sd = bias.s * d;
-    if (a.cap > 0.f) {
-        if (!any_beyond<32>(v, a.most)) {
+// N neighbouring scores of one row (a multiple of 32), in place, to the log2 domain; dist: distance of the first one. real: the row is a
+// query's (what lies in other rows of the tile must not tell the warp which form of the tanh to take, and so the last bits).
+template <int KIND, int N>
+__device__ __forceinline__ void score_row(float* v, const ScoreArgs& a, const Bias& bias, float c, int dist, bool real) {
+    const uint64_t step2 = pack_f2(-2.f * bias.line, -2.f * bias.line);
+    auto each = [&](auto score) {  // score(two scores, their bias)
 #pragma unroll
-            for (int x = 0; x < 32; x += 2) unpack_f2(cap_small(pack_f2(v[x], v[x + 1]), a), v[x], v[x + 1]);
-        } else {
+        for (int q = 0; q < N; q += 32) {
+            const float d = float(dist - q);
+            uint64_t b2 = pack_f2(bias.line * d, bias.line * (d - 1.f));
 #pragma unroll
-            for (int x = 0; x < 32; ++x) v[x] = cap_any(v[x], a);
+            for (int x = q; x < q + 32; x += 2) {
+                unpack_f2(score(pack_f2(v[x], v[x + 1]), b2), v[x], v[x + 1]);
+                if (x + 2 < q + 32) b2 = add_f2(b2, step2);
+            }
         }
+    };
+    if constexpr (KIND == SCORE_CAPPED) {
+        if (!any_beyond<N>(v, real ? a.most : INFINITY)) each([&](uint64_t s2, uint64_t b2) { return fma_f2(s2, cap_poly(s2, a), b2); });
+        else each([&](uint64_t s2, uint64_t b2) { return add_f2(cap_pair(s2, a, true), b2); });
     } else {
-#pragma unroll
-        for (int x = 0; x < 32; x += 2) unpack_f2(mul_f2(pack_f2(v[x], v[x + 1]), pack_f2(c, c)), v[x], v[x + 1]);
+        each([&](uint64_t s2, uint64_t b2) { return fma_f2(s2, pack_f2(c, c), b2); });
     }
-    if (bias.s != 0.f) {
+    if (bias.both) {
+        const float d = float(dist);
 #pragma unroll
-        for (int x = 0; x < 32; x += 2) unpack_f2(add_f2(pack_f2(v[x], v[x + 1]), bias.pair(d, sd, float(-x), -1.f)), v[x], v[x + 1]);
+        for (int x = 0; x < N; ++x) v[x] = fmaf(bias.s, fabsf(d - float(x)), v[x]);
     }
 }
 
