@@ -363,3 +363,23 @@ def test_refusals():
     with torch.no_grad():
         fb.paged_attention(**{**good, "q": asks})
     fb.check_status()
+
+
+def test_inference_mode_and_both_ways_through_the_host(monkeypatch):
+    """Tensors made in inference mode have no version counters. The same bits by the native host call and by the Python one."""
+    import flash_b200 as fb
+    from flash_b200 import ops
+    with torch.inference_mode():
+        cache = Cache([100, 30], 2, 64, 16, BF16, 20)
+        k, v, q = (torch.randn(2, h, 64, device="cuda").to(BF16) for h in (2, 2, 4))
+        results = []
+        for profile in (None, []):
+            monkeypatch.setattr(ops, "PROFILE", profile)
+            cache.fill()
+            fb.paged_append(k, v, cache.k_pages, cache.v_pages, cache.table, cache.kv_lens)
+            out = torch.empty_like(q)
+            fb.paged_attention(q, cache.k_pages, cache.v_pages, cache.table, cache.kv_lens, out=out)
+            results.append((cache.k_pages.clone(), cache.v_pages.clone(), out, fb.paged_attention(q, cache.k_pages, cache.v_pages, cache.table, cache.kv_lens)))
+        for a, b in zip(*results):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+        assert torch.equal(results[0][2], results[0][3])

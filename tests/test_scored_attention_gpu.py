@@ -282,3 +282,32 @@ def test_refusals():
     g, = torch.autograd.grad(fb.attention_scored(a, k, v, True, softcap=5.0).sum(), a, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_both_ways_through_the_host_give_the_same(monkeypatch):
+    """The native host call and its autograd node, and the ones in Python: a call that the kernels do not take as it is, and hooks on saved tensors, go that way."""
+    import flash_b200 as fb
+    from flash_b200 import ops
+    q, k, v, do = _inputs(2, 4, 2, 260, 260, 64, BF16, 40)
+    ids, slopes, prefix = _docs(2, 4, 260, 41), _slopes(4, "series"), torch.tensor([100, 9], dtype=torch.int32, device="cuda")
+    for kw in (dict(cap=9.0), dict(slopes=slopes, prefix=prefix), dict(cap=9.0, eq=ids, ek=ids, prefix=prefix)):
+        want = _run(fb, q, k, v, do, True, **kw)
+        with monkeypatch.context() as m:
+            m.setattr(ops, "PROFILE", [])
+            other = _run(fb, q, k, v, do, True, **kw)
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: x):
+            hooked = _run(fb, q, k, v, do, True, **kw)
+        for name in want:
+            assert torch.equal(want[name], other[name]) and torch.equal(want[name], hooked[name]), name
+
+
+def test_saved_tensors_that_change_are_noticed():
+    import flash_b200 as fb
+    q, k, v, do = _inputs(1, 4, 4, 40, 40, 64, BF16, 42)
+    for victim in ("slopes", "prefix"):
+        kw = dict(slopes=_slopes(4, "series"), prefix=torch.tensor([10], dtype=torch.int32, device="cuda"))
+        a = q.detach().requires_grad_()
+        o = fb.attention_scored(a, k, v, True, **kw)
+        kw[victim].add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            o.backward(do)

@@ -92,13 +92,18 @@ fa_ids id_view(const Tensor& t) {
 }
 
 // The plan of a call: its memory and the launches that fill it. eq and ek, if any, are int32 or int64 tensors [B, H, M] and [B, H, N].
-Tensor build_plan(const fa_problem& p, const Tensor* eq, const Tensor* ek, const Tensor& status) {
+// scores: of attention_scored, else null (here and below).
+Tensor build_plan(const fa_problem& p, const Tensor* eq, const Tensor* ek, const Tensor& status, const fa_scores* scores = nullptr) {
     size_t bytes = 0;
     check(fa_plan_bytes(&p, &bytes), "fa_plan_bytes");
     Tensor plan = at::empty({int64_t(bytes / 4)}, status.options());
     const fa_ids q = eq ? id_view(*eq) : fa_ids{}, k = ek ? id_view(*ek) : fa_ids{};
-    check(fa_plan_build(&p, eq ? &q : nullptr, ek ? &k : nullptr, plan.data_ptr(), bytes, status.data_ptr<int>(), current_stream(status)),
-          "fa_plan_build");
+    if (scores)
+        check(fa_plan_build_scored(&p, scores, eq ? &q : nullptr, ek ? &k : nullptr, plan.data_ptr(), bytes, status.data_ptr<int>(), current_stream(status)),
+              "fa_plan_build_scored");
+    else
+        check(fa_plan_build(&p, eq ? &q : nullptr, ek ? &k : nullptr, plan.data_ptr(), bytes, status.data_ptr<int>(), current_stream(status)),
+              "fa_plan_build");
     return plan;
 }
 
@@ -115,7 +120,7 @@ struct Outputs {
 
 // The forward's allocations and launches for a problem that `regular` has filled.
 Outputs launch_forward(const fa_problem& p, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& plan, int key_runs,
-                       const Tensor& status, const std::optional<Tensor>& out) {
+                       const Tensor& status, const std::optional<Tensor>& out, const fa_scores* scores = nullptr) {
     Outputs r;
     r.o = out ? *out : at::empty_like(q);
     if (!taken_as_is(r.o)) r.o = at::empty(q.sizes(), q.options());
@@ -129,22 +134,35 @@ Outputs launch_forward(const fa_problem& p, const Tensor& q, const Tensor& k, co
         work = at::empty({int64_t(bytes / 4)}, f32);
     }
     const fa_tensor tq = view(q), tk = view(k), tv = view(v), to = view(r.o);
-    check(fa_fwd_split(&p, &tq, &tk, &tv, &to, r.lse.data_ptr<float>(), plan.defined() ? plan.data_ptr() : nullptr, r.splits,
-                       work.defined() ? work.data_ptr() : nullptr, bytes, status.data_ptr<int>(), current_stream(q)),
-          "fa_fwd_split");
+    void* const plan_ptr = plan.defined() ? plan.data_ptr() : nullptr;
+    void* const work_ptr = work.defined() ? work.data_ptr() : nullptr;
+    if (scores)
+        check(fa_fwd_scored(&p, scores, &tq, &tk, &tv, &to, r.lse.data_ptr<float>(), plan_ptr, r.splits, work_ptr, bytes, status.data_ptr<int>(),
+                            current_stream(q)),
+              "fa_fwd_scored");
+    else
+        check(fa_fwd_split(&p, &tq, &tk, &tv, &to, r.lse.data_ptr<float>(), plan_ptr, r.splits, work_ptr, bytes, status.data_ptr<int>(), current_stream(q)),
+              "fa_fwd_split");
     return r;
 }
 
 // dq, dk, dv. q, k, v, o, lse and the problem are those of a forward, d_o is like q.
 std::array<Tensor, 3> launch_backward(const fa_problem& p, const Tensor& d_o, const Tensor& q, const Tensor& k, const Tensor& v,
-                                      const Tensor& o, const Tensor& lse, const Tensor& plan, const Tensor& status) {
+                                      const Tensor& o, const Tensor& lse, const Tensor& plan, const Tensor& status,
+                                      const fa_scores* scores = nullptr) {
     Tensor delta = at::empty_like(lse);
     Tensor dk = at::empty({p.B, p.Hk, p.N, p.D}, k.options()), dv = at::empty({p.B, p.Hk, p.N, p.D}, v.options());
     Tensor dq = at::empty(q.sizes(), q.options());
     const fa_tensor tq = view(q), tk = view(k), tv = view(v), to = view(o), tdo = view(d_o), tdq = view(dq), tdk = view(dk), tdv = view(dv);
-    check(fa_bwd(&p, &tq, &tk, &tv, &to, &tdo, lse.data_ptr<float>(), delta.data_ptr<float>(), &tdq, &tdk, &tdv,
-                 plan.defined() ? plan.data_ptr() : nullptr, status.data_ptr<int>(), current_stream(q)),
-          "fa_bwd");
+    void* const plan_ptr = plan.defined() ? plan.data_ptr() : nullptr;
+    if (scores)
+        check(fa_bwd_scored(&p, scores, &tq, &tk, &tv, &to, &tdo, lse.data_ptr<float>(), delta.data_ptr<float>(), &tdq, &tdk, &tdv, plan_ptr,
+                            status.data_ptr<int>(), current_stream(q)),
+              "fa_bwd_scored");
+    else
+        check(fa_bwd(&p, &tq, &tk, &tv, &to, &tdo, lse.data_ptr<float>(), delta.data_ptr<float>(), &tdq, &tdk, &tdv, plan_ptr, status.data_ptr<int>(),
+                     current_stream(q)),
+              "fa_bwd");
     return {std::move(dq), std::move(dk), std::move(dv)};
 }
 
@@ -271,6 +289,189 @@ py::object attend(const Tensor& q, const Tensor& k, const Tensor& v, bool causal
     return py::cast(FlashAttention::launch(q, k, v, call, plan).o);
 }
 
+// What attention_scored changes: as scored.py has checked it, or None.
+bool scores_of(double softcap, const std::optional<Tensor>& slopes, const std::optional<Tensor>& prefix, const Tensor& q, int64_t H, int64_t B, fa_scores& s) {
+    if (!(softcap == 0.0 || (softcap >= 1e-6 && softcap <= 1e6))) return false;
+    auto vector = [&](const Tensor& t, at::ScalarType type, int64_t n) {
+        return t.is_cuda() && t.layout() == at::kStrided && t.dim() == 1 && t.size(0) == n && t.scalar_type() == type && t.is_contiguous() && !t.is_neg() &&
+               t.device() == q.device() && !t.requires_grad();
+    };
+    if ((slopes && !vector(*slopes, at::kFloat, H)) || (prefix && !vector(*prefix, at::kInt, B))) return false;
+    s = fa_scores{float(softcap), slopes ? slopes->const_data_ptr<float>() : nullptr, prefix ? prefix->const_data_ptr<int>() : nullptr};
+    return true;
+}
+
+// The autograd node of a regular call of attention_scored, as scored.ScoredAttention.
+struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
+    struct Scores {
+        fa_scores s;
+        const std::optional<Tensor>&slopes, &prefix;
+    };
+
+    static Outputs launch(const Tensor& q, const Tensor& k, const Tensor& v, const Call& c, const fa_scores& s, Tensor& plan) {
+        py::gil_scoped_release free;
+        if (c.eq || !fa_plan_optional(&c.p, c.needs_grad)) plan = build_plan(c.p, c.eq, c.ek, c.status, &s);
+        Outputs r = launch_forward(c.p, q, k, v, plan, 0, c.status, std::nullopt, &s);
+        n_launched += (plan.defined() ? c.plan_kernels : 0) + (r.splits > 1 ? 2 : 1);
+        return r;
+    }
+
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Call& c, const Scores& sc) {
+        Tensor plan;
+        Outputs r = launch(q, k, v, c, sc.s, plan);
+        torch::autograd::variable_list saved{q, k, v, r.o, r.lse};
+        if (sc.slopes) saved.push_back(*sc.slopes);
+        if (sc.prefix) saved.push_back(*sc.prefix);
+        ctx->save_for_backward(std::move(saved));
+        auto& data = ctx->saved_data;
+        data["plan"] = plan;
+        data["status"] = c.status;
+        data["causal"] = int64_t(c.p.causal);
+        data["mode"] = int64_t(c.p.mode);
+        data["id_heads"] = int64_t(c.p.id_heads);
+        data["scale"] = c.sm_scale;
+        data["softcap"] = double(sc.s.softcap);
+        data["slopes"] = sc.slopes.has_value();
+        return r.o;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &q = saved[0], &k = saved[1], &v = saved[2];
+        const c10::cuda::CUDAGuard device(q.device());
+        auto& data = ctx->saved_data;
+        fa_problem p;
+        TORCH_CHECK(regular(q, k, v, true, data["causal"].toInt() != 0, data["scale"].toDouble(), int(data["mode"].toInt()),
+                            int(data["id_heads"].toInt()), p),
+                    "flash_b200: the saved q, k, v are not plain [bs, H, L, D] CUDA tensors of matching shapes");
+        size_t at = 5;
+        const bool slopes = data["slopes"].toBool();
+        fa_scores s{float(data["softcap"].toDouble()), nullptr, nullptr};
+        if (slopes) s.slopes = saved[at++].const_data_ptr<float>();
+        if (saved.size() > at) s.prefix = saved[at].const_data_ptr<int>();
+        Tensor d_o = grads[0];
+        if (d_o.scalar_type() != q.scalar_type()) d_o = d_o.to(q.scalar_type());
+        d_o = d_o.resolve_neg();
+        TORCH_CHECK(like_query(d_o, q), "flash_b200: the gradient is not a plain [bs, H, M, D] CUDA tensor");
+        if (!taken_as_is(d_o)) d_o = d_o.contiguous();  // (ops.maybe_contiguous)
+        auto g = launch_backward(p, d_o, q, k, v, saved[3], saved[4], data["plan"].toTensor(), data["status"].toTensor(), &s);
+        n_launched += 3;
+        return {std::move(g[0]), std::move(g[1]), std::move(g[2]), Tensor(), Tensor()};
+    }
+};
+
+// The whole of a regular call of attention_scored, its gradients included; None: scored.py takes it another way.
+py::object attend_scored(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, std::optional<double> scale, const std::optional<Tensor>& eq,
+                         const std::optional<Tensor>& ek, int64_t mode, double softcap, const std::optional<Tensor>& slopes,
+                         const std::optional<Tensor>& prefix, const Tensor& status) {
+    fa_problem p;
+    const double sm_scale = scale ? *scale : 1.0 / std::sqrt(double(q.dim() == 4 ? q.size(3) : 1));
+    if (eq.has_value() != ek.has_value() || mode != (eq ? FA_MODE1_DOC : FA_MODE0_NOPE) || (prefix && !causal)) return py::none();
+    if (!regular(q, k, v, false, causal, sm_scale, int(mode), 1, p)) return py::none();
+    if (eq) {
+        if (eq->device() != q.device() || ek->device() != q.device()) return py::none();
+        p.id_heads = int(id_heads(*eq, *ek, p.B, p.H, p.M, p.N));
+        if (p.id_heads == 0) return py::none();
+    }
+    fa_scores s;
+    if (!scores_of(softcap, slopes, prefix, q, p.H, p.B, s)) return py::none();
+    const bool needs_grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+    if (needs_grad && at::SavedTensorDefaultHooks::get_hooks()) return py::none();
+    const int plan_kernels = !eq || (p.M + 127) / 128 + (p.N + 127) / 128 <= FA_PLAN_ONE_KERNEL_BLOCKS ? 1 : 3;
+    const Call call{p, sm_scale, eq ? &*eq : nullptr, ek ? &*ek : nullptr, status, needs_grad, plan_kernels};
+    if (needs_grad) return py::cast(ScoredAttention::apply(q, k, v, call, ScoredAttention::Scores{s, slopes, prefix}));
+    Tensor plan;
+    return py::cast(ScoredAttention::launch(q, k, v, call, s, plan).o);
+}
+
+// ---- paged cache (paged.py). A call that is not a regular one on the current device is declined, and paged.py copies, raises or does nothing.
+bool rows_as_is(const Tensor& t, int dim) {
+    if (!t.is_cuda() || t.layout() != at::kStrided || t.dim() != dim || t.is_neg() || t.stride(dim - 1) != 1 || t.numel() == 0 ||
+        reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 != 0)
+        return false;
+    for (int i = 0; i < dim - 1; ++i)
+        if (t.size(i) > 1 && (t.stride(i) <= 0 || t.stride(i) % 8 != 0)) return false;
+    return !(at::GradMode::is_enabled() && t.requires_grad());
+}
+
+bool cache_of(const Tensor& rows, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens, const std::optional<Tensor>& starts,
+              fa_paged_cache& c) {
+    if (!rows_as_is(rows, 3) || !rows_as_is(k_pages, 4) || !rows_as_is(v_pages, 4) || rows.get_device() != c10::cuda::current_device()) return false;
+    const int dt = dtype_of(rows);
+    if ((dt != FA_BF16 && dt != FA_FP16) || k_pages.scalar_type() != rows.scalar_type() || v_pages.scalar_type() != rows.scalar_type()) return false;
+    auto ints = [&](const Tensor& t, int dim) {
+        return t.is_cuda() && t.layout() == at::kStrided && t.scalar_type() == at::kInt && t.dim() == dim && t.device() == rows.device() && !t.is_neg();
+    };
+    if (k_pages.device() != rows.device() || v_pages.device() != rows.device() || v_pages.sizes() != k_pages.sizes()) return false;
+    if (!ints(table, 2) || !ints(lens, 1) || (starts && !ints(*starts, 1))) return false;
+    const int64_t B = table.size(0), T = rows.size(0), page = k_pages.size(1), D = rows.size(2);
+    if (B < 1 || B > 65535 || table.size(1) < 1 || table.stride(1) != 1 || (B > 1 && table.stride(0) < table.size(1)) || lens.size(0) != B ||
+        !lens.is_contiguous() || T > INT32_MAX || k_pages.size(0) > INT32_MAX || page > (1 << 22) || k_pages.size(2) > 1024)
+        return false;
+    if (starts ? starts->size(0) != B + 1 || !starts->is_contiguous() : T != B) return false;
+    if (page < 8 || (page & (page - 1)) != 0 || table.size(1) * page > (1 << 22) || k_pages.size(3) != D || (D != 16 && D != 32 && D != 64 && D != 128)) return false;
+    c = fa_paged_cache{int(B), int(k_pages.size(2)), int(D), dt, int(k_pages.size(0)), int(page), int(table.size(1)), table.const_data_ptr<int>(), table.stride(0),
+                       lens.const_data_ptr<int>(), k_pages.data_ptr(), v_pages.data_ptr(), {k_pages.stride(0), k_pages.stride(1), k_pages.stride(2)},
+                       {v_pages.stride(0), v_pages.stride(1), v_pages.stride(2)}};
+    return true;
+}
+
+fa_rows rows_view(const Tensor& t) { return fa_rows{t.data_ptr(), {t.stride(0), t.stride(1)}}; }
+
+void bump(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+bool paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens,
+                  const std::optional<Tensor>& starts, const Tensor& status) {
+    fa_paged_cache c;
+    if (!cache_of(k, k_pages, v_pages, table, lens, starts, c) || !rows_as_is(v, 3) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() ||
+        v.device() != k.device() || k.size(1) != c.Hk)
+        return false;
+    {
+        py::gil_scoped_release free;
+        const fa_rows rk = rows_view(k), rv = rows_view(v);
+        check(fa_paged_append(&c, int(k.size(0)), starts ? starts->const_data_ptr<int>() : nullptr, &rk, &rv, status.data_ptr<int>(), current_stream(k)),
+              "fa_paged_append");
+        ++n_launched;
+    }
+    bump(k_pages);
+    bump(v_pages);
+    return true;
+}
+
+py::object paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens,
+                           const std::optional<Tensor>& starts, std::optional<double> scale, double softcap, const std::optional<Tensor>& slopes,
+                           const std::optional<Tensor>& prefix, const std::optional<Tensor>& out, const Tensor& status) {
+    fa_paged_cache c;
+    fa_scores s;
+    if (!cache_of(q, k_pages, v_pages, table, lens, starts, c)) return py::none();
+    const int64_t H = q.size(1);
+    const double sm_scale = scale ? *scale : 1.0 / std::sqrt(double(c.D));
+    if (H % c.Hk != 0 || H / c.Hk > 128 || !(sm_scale > 0) || !std::isfinite(sm_scale) || !scores_of(softcap, slopes, prefix, q, H, c.B, s)) return py::none();
+    if (out) {
+        if (!rows_as_is(*out, 3) || out->sizes() != q.sizes() || out->scalar_type() != q.scalar_type() || out->device() != q.device() || out->requires_grad())
+            return py::none();
+        for (const Tensor* t : {&q, &k_pages, &v_pages})
+            if (t->storage().data() == out->storage().data()) return py::none();  // paged.py looks closer
+    }
+    Tensor o;
+    {
+        py::gil_scoped_release free;
+        o = out ? *out : at::empty(q.sizes(), q.options().requires_grad(false));
+        size_t bytes = 0;
+        check(fa_paged_workspace_bytes(&c, &bytes), "fa_paged_workspace_bytes");
+        Tensor work = at::empty({int64_t(bytes)}, q.options().dtype(at::kByte));
+        const fa_rows rq = rows_view(q), ro = rows_view(o);
+        check(fa_paged_fwd(&c, int(q.size(0)), int(H), starts ? starts->const_data_ptr<int>() : nullptr, float(sm_scale), &s, &rq, &ro, out ? 0 : 1, work.data_ptr(),
+                           bytes, status.data_ptr<int>(), current_stream(q)),
+              "fa_paged_fwd");
+        n_launched += 2;
+    }
+    if (out) bump(*out);
+    return py::cast(o);
+}
+
 int64_t launched() { return n_launched; }
 
 // What `grad_fn` of a regular call shows to Python: what it shows of ops.FlashAttention (the reference's contract, flash_triton.py:558-562).
@@ -341,6 +542,9 @@ PYBIND11_MODULE(_host, m) {
     m.def("forward", &forward);
     m.def("backward", &backward);
     m.def("attend", &attend);
+    m.def("attend_scored", &attend_scored);
+    m.def("paged_append", &paged_append);
+    m.def("paged_attention", &paged_attention);
     m.def("launched", &launched);
     register_node();
 }

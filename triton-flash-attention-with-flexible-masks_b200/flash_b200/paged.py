@@ -6,7 +6,7 @@ import torch
 
 from . import _lib, ops
 from .ops import _count, _current, _same_device, _status_word, _stream, check_status
-from .scored import _checked_softcap, _checked_slopes, _scores
+from .scored import _checked_softcap, _checked_slopes, _native, _scores
 
 _TYPES = {torch.bfloat16: _lib.FA_BF16, torch.float16: _lib.FA_FP16}
 _workspace_bytes = {}  # (device, head dim) -> bytes
@@ -78,6 +78,9 @@ def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None):
 
     All lengths and tables are read on the device, so that a captured call follows them. A page number or a length that the cache does not have
     writes nothing and is reported by `check_status`."""
+    native = _native(k, v, k_pages, v_pages, page_table, kv_lens, q_starts)
+    if native is not None and native[0].paged_append(k, v, k_pages, v_pages, page_table, kv_lens, q_starts, native[1]):
+        return
     if v.shape != k.shape or k.shape[1:2] != k_pages.shape[2:3]:
         raise ValueError("flash_b200: k and v must be [T, Hk, D] with the heads of the cache")
     if v.dtype != k.dtype:
@@ -93,9 +96,14 @@ def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None):
     with _current(k.device):
         _lib.check(_lib.load().fa_paged_append(cache, T, starts, _rows(k), _rows(v), _status_word(k.device).data_ptr(), _stream()), "fa_paged_append")
     _count(1)
-    torch.autograd.graph.increment_version((k_pages, v_pages))
+    _bump(k_pages, v_pages)
     if ops._SYNC_STATUS:
         check_status(k.device)
+
+
+def _bump(*tensors):
+    """They have been written to in place, which autograd's version counters tell (tensors made in inference mode have none)."""
+    torch.autograd.graph.increment_version([x for x in tensors if not x.is_inference()])
 
 
 def _overlap(a, b):
@@ -116,6 +124,13 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_
     or the cache. What lies in the pages behind a sequence's length, or in pages that no sequence names, has no influence, also
     if it is not finite. How the work is cut goes by all lengths of the batch, so that the last bits of a sequence's rows can differ with what
     it is batched with."""
+    softcap = _checked_softcap(softcap)
+    if sm_scale is None or type(sm_scale) is float:
+        native = _native(q, k_pages, v_pages, page_table, kv_lens, q_starts, slopes, prefix, out)
+        if native is not None:
+            done = native[0].paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts, sm_scale, softcap, slopes, prefix, out, native[1])
+            if done is not None:
+                return done if out is None else out
     cache, starts, held = _checked(q, "q", k_pages, v_pages, page_table, kv_lens, q_starts)
     T, H, D = q.shape
     if cache.Hk == 0 or H == 0 or H % cache.Hk or H // cache.Hk > 128:
@@ -124,7 +139,7 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_
         sm_scale = 1. / math.sqrt(D)
     if not 0 < sm_scale < math.inf:
         raise NotImplementedError("flash_b200 needs sm_scale > 0")
-    softcap, slopes = _checked_softcap(softcap), _checked_slopes(slopes, H, q)
+    slopes = _checked_slopes(slopes, H, q)
     if prefix is not None:
         prefix = _int32(prefix, (cache.B,), "prefix", q)
     fill = out is None
@@ -153,7 +168,7 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_
             _lib.check(lib.fa_paged_fwd(cache, T, H, starts, sm_scale, _scores(softcap, slopes, prefix), _rows(q), _rows(out), fill, work.data_ptr(), size,
                                         _status_word(device).data_ptr(), _stream()), "fa_paged_fwd")
     if not fill:
-        torch.autograd.graph.increment_version(out)
+        _bump(out)
     if ops._SYNC_STATUS:
         check_status(device)
     return out

@@ -48,6 +48,15 @@ def _checked_prefix(prefix, B, N, q):
     return (prefix if prefix.dtype == torch.int32 else prefix.clamp(0, N).to(torch.int32)).contiguous()
 
 
+def _native(*tensors):
+    """The native host calls, where a call of these tensors may take them (see `attention`): the module and the device's status word; else None."""
+    first = tensors[0]
+    if (all(x is None or type(x) in ops._PLAIN for x in tensors) and ops.PROFILE is None and not ops._SYNC_STATUS and ops._transforms() is None
+            and ops._forward_ad._current_level < 0 and ops._tracing_state() is None and first.is_cuda):
+        return ops._HOST or ops._host(), _status_word(first.device)
+    return None
+
+
 def _scores(softcap, slopes, prefix):
     return _lib.Scores(softcap, None if slopes is None else slopes.data_ptr(), None if prefix is None else prefix.data_ptr())
 
@@ -134,6 +143,13 @@ def attention_scored(q, k, v, causal=False, sm_scale=None, eq=None, ek=None, sco
     softcap = _checked_softcap(softcap)
     if softcap == 0.0 and slopes is None and prefix is None:
         return attention(q, k, v, causal, sm_scale, eq, ek, score_func_mode)
+    grouped = ops.GROUP_QUERIES and eq is not None and not causal and slopes is None and q.dim() == 4 and 128 < q.shape[2] <= _lib.FA_GROUP_MAX_ROWS
+    if not grouped and type(score_func_mode) is int and abs(score_func_mode) < 8 and (sm_scale is None or type(sm_scale) is float):
+        native = _native(q, k, v, eq, ek, slopes, prefix)
+        if native is not None:
+            done = native[0].attend_scored(q, k, v, bool(causal), sm_scale, eq, ek, score_func_mode, softcap, slopes, prefix, native[1])
+            if done is not None:
+                return done
     D = q.shape[-1]
     assert k.shape[-1] == D and v.shape[-1] == D, "feature size of q, k, v should be equal"
     assert D in {16, 32, 64, 128}
@@ -159,8 +175,8 @@ def attention_scored(q, k, v, causal=False, sm_scale=None, eq=None, ek=None, sco
     slopes, prefix = _checked_slopes(slopes, H, q), _checked_prefix(prefix, B, N, q)
     args = float(sm_scale), softcap, slopes, prefix
     # queries of scattered documents side by side, as in `attention`; a bias goes by the queries' places, which have to stay
-    if ops.GROUP_QUERIES and eq is not None and not causal and slopes is None and 128 < M <= _lib.FA_GROUP_MAX_ROWS:
-        order, inverse, grouped, id_heads = group_rows(eq, B, H, M)
-        o = ScoredAttention.apply(_PermuteRows.apply(q, order, inverse, id_heads), k, v, False, args[0], grouped.expand(B, H, M), ek, score_func_mode, *args[1:])
+    if grouped:
+        order, inverse, ids, id_heads = group_rows(eq, B, H, M)
+        o = ScoredAttention.apply(_PermuteRows.apply(q, order, inverse, id_heads), k, v, False, args[0], ids.expand(B, H, M), ek, score_func_mode, *args[1:])
         return _PermuteRows.apply(o, inverse, order, id_heads)
     return ScoredAttention.apply(q, k, v, bool(causal), args[0], eq, ek, int(score_func_mode), *args[1:])
