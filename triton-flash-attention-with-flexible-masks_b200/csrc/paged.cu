@@ -81,8 +81,10 @@ int map4(CUtensorMap* out, int dtype, const void* ptr, int D, const int (&extent
     return r == CUDA_SUCCESS ? FA_OK : FA_ERR_TENSORMAP;
 }
 
-// fp32 rows and log-sum-exps of two pieces for each worker
-size_t workspace_bytes(int D, int workers) { return size_t(2) * workers * fa::kBlk * ((D > 64 ? 128 : 64) + 1) * sizeof(float); }
+// fp32 rows and log-sum-exps of two pieces for each worker, and what is merged from which
+size_t workspace_bytes(int D, int workers) {
+    return size_t(2) * workers * fa::kBlk * ((D > 64 ? 128 : 64) + 1) * sizeof(float) + workers * (sizeof(int4) + 2 * sizeof(int));
+}
 
 }  // namespace
 
@@ -133,6 +135,8 @@ int fa_paged_fwd(const fa_paged_cache* cache, int32_t T, int32_t H, const int32_
     p.out_h = o->stride[1];
     p.part_o = static_cast<float*>(workspace);
     p.part_lse = p.part_o + size_t(2) * sms * fa::kBlk * (cache->D > 64 ? 128 : 64);
+    p.merge = reinterpret_cast<int4*>(p.part_lse + size_t(2) * sms * fa::kBlk);
+    p.merge_slots = reinterpret_cast<int*>(p.merge + sms);
     p.H = H;
     p.G = G;
     p.tokens = fa::kBlk / G;
@@ -179,6 +183,7 @@ int fa_debug_paged_pieces(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t c
             if (s.tiles > 0 && s.len > longest) longest = s.len;
         });
     fa::paged_share_out(plan, weight, items, longest, most_workers);
+    if (plan.workers > 1023) return -1;
     plan.sums[0] = 0;
     for (int g = 0; g < fa::kPagedGroups; ++g) {
         plan.sums[g + 1] = plan.sums[g];
@@ -192,16 +197,21 @@ int fa_debug_paged_pieces(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t c
         ++n;
     };
     for (int w = 0; w < plan.workers; ++w) {
+        bool first = true;
         fa::paged_stretch(p, plan, w, [&](const fa::PagedWalk& k, int tiles, int lo, int hi, int part) {
             put(w, k.b, k.hk, k.tile, lo, hi, tiles, part);
+            if (first && fa::paged_first_cut(plan, w, k)) {
+                int slots[2048], pieces = 0;
+                bool last = false;
+                for (int i = 0; !last; ++i) {
+                    const int slot = fa::paged_piece(p, plan, w, k, i, last);
+                    if (slot >= 0) slots[pieces++] = slot;
+                }
+                for (int i = 0; pieces > 1 && i < pieces; ++i) put(-1, k.b, k.hk, k.tile, 0, 0, 0, slots[i]);
+            }
+            first = false;
             return true;
         });
-        fa::PagedWalk k;
-        if (fa::paged_first_cut(p, plan, w, k)) {
-            int pieces = 0;
-            fa::paged_pieces(p, plan, w, k, [&](int) { ++pieces; });
-            if (pieces > 1) fa::paged_pieces(p, plan, w, k, [&](int slot) { put(-1, k.b, k.hk, k.tile, 0, 0, 0, slot); });
-        }
     }
     return n;
 }

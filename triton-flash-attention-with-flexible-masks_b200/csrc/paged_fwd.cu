@@ -8,10 +8,10 @@
 //  - all heads of a kv head's group share a tile of queries, row = token * G + head of the group, so that K and V are read once for the group: one decoded
 //    token of 32 / 8 heads reads its keys once instead of four times;
 //  - a tile of 128 keys is 128 / page size boxes, one a page, which land one behind the other in the tile (a page of 8 rows is one
-//    swizzle atom); the producer's lanes read the page numbers of the next tile while this one is under way;
-//  - P of a masked entry is 0, but 0 times a NaN that an earlier user left in the page is not: rows of K and V behind the sequence's end are
-//    zeroed in shared memory by the warp that issues the product, before it does (of K, for what a masked score is must not tell the other rows
-//    which form of the cap to take);
+//    swizzle atom); the producers' lanes read the page numbers of the next tile while this one is under way;
+//  - P of a masked entry is 0, but 0 times a NaN that an earlier user left in the page is not: rows of V behind the sequence's end are
+//    zeroed in shared memory by the softmax group before it gives its P away (not by the warp that issues P V: its code has to stay free of loops by
+//    lanes, or the descriptors go through vector registers);
 //  - each block works on one stretch of a line of all items (paged_plan.cuh); a piece of an item that was cut leaves normalised fp32 rows and
 //    their log-sum-exp to paged_combine_kernel.
 #include <type_traits>
@@ -41,9 +41,9 @@ struct PagedSmem {
     static constexpr int off_info = off_ml + NQ * 4 * kBlk * 4;  // int32 [NQ][16]: see I_*
     static constexpr int off_plan = off_info + NQ * 64;
     static constexpr int off_bar = off_plan + int(sizeof(PagedPlan));
-    // item_full[NQ] item_empty[NQ] q_full[NQ] q_empty[NQ] ml_full[NQ] k_full[NS] k_empty[NS] v_full[NS] v_empty[NS]
+    // item_full[NQ] item_empty[NQ] q_full[NQ] ml_full[NQ] k_full[NS] k_empty[NS] v_full[NS] v_empty[NS]
     // s_full[4] s_free[2] p_full[NP] pv_done[NP] o_full[2] o_free[2]
-    static constexpr int n_bar = 5 * NQ + 4 * NS + 6 + 2 * NP + 4;
+    static constexpr int n_bar = 4 * NQ + 4 * NS + 6 + 2 * NP + 4;
     static constexpr int off_misc = off_bar + n_bar * 8;  // tmem slot, abort flag
     static constexpr int total = off_misc + 16;
     static_assert(off_plan % 8 == 0 && off_bar % 8 == 0, "alignment");
@@ -71,7 +71,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     PagedPlan& plan = *reinterpret_cast<PagedPlan*>(smem + S::off_plan);
     const uint32_t bar0 = sbase + S::off_bar;
     auto BAR = [&](int i) { return bar0 + 8u * uint32_t(i); };
-    constexpr int B_ITEMFULL = 0, B_ITEMEMPTY = NQ, B_QFULL = 2 * NQ, B_QEMPTY = 3 * NQ, B_MLFULL = 4 * NQ, B_KFULL = 5 * NQ,
+    constexpr int B_ITEMFULL = 0, B_ITEMEMPTY = NQ, B_QFULL = 2 * NQ, B_MLFULL = 3 * NQ, B_KFULL = 4 * NQ,
                   B_KEMPTY = B_KFULL + NS, B_VFULL = B_KEMPTY + NS, B_VEMPTY = B_VFULL + NS, B_SFULL = B_VEMPTY + NS,
                   B_SFREE = B_SFULL + 4, B_PFULL = B_SFREE + 2, B_PVDONE = B_PFULL + NP, B_OFULL = B_PVDONE + NP, B_OFREE = B_OFULL + 2;
     static_assert(B_OFREE + 2 == S::n_bar, "barriers");
@@ -80,9 +80,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (tid == 0) {
         for (int s = 0; s < NQ; ++s) {
             mbar_init(BAR(B_ITEMFULL + s), 1);
-            mbar_init(BAR(B_ITEMEMPTY + s), 15);  // producer, two MMA issuers, eight softmax warps, four epilogue warps
+            mbar_init(BAR(B_ITEMEMPTY + s), 15);  // V producer, two MMA issuers, eight softmax warps, four epilogue warps
             mbar_init(BAR(B_QFULL + s), 1);
-            mbar_init(BAR(B_QEMPTY + s), 1);
             mbar_init(BAR(B_MLFULL + s), 8);
         }
         for (int s = 0; s < NS; ++s) {
@@ -119,6 +118,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const bool aborted = misc[1] != 0;
     uint16_t* const out = static_cast<uint16_t*>(p.out);
     if (aborted) {
+        if (tid == 0) p.merge[blockIdx.x] = make_int4(0, 0, 0, 0);
         // an earlier launch ran into a time-out that the host has not yet cleared: the whole of the output becomes NaN, shared out by rows of a head
         for (int64_t i = blockIdx.x; i < int64_t(p.T) * p.H; i += gridDim.x)
             for (int d = tid; d < p.D; d += kFwdThreads) out[i / p.H * p.out_t + i % p.H * p.out_h + d] = 0xffffu;
@@ -133,36 +133,90 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     auto sV = [&](int s) { return sbase + S::off_v + uint32_t(s) * S::TILE; };
     if (warp >= 12) {
         setmaxnreg_dec<kFwdServiceRegs>();
+        // K and V are loaded by a warp each. (By one, 16 to 32 loads a tile with small pages, and the step from one tile's to the next, took longer than a
+        // tile: one chunk of 500 tokens behind 7500, 32 / 8 heads of 128, pages of 128 | 16: 105 | 116 us.)
+        const int rows = p.page < kBlk ? p.page : kBlk, log2_rows = p.page < kBlk ? p.log2_page : 7;  // of a box
+        const int boxes = kBlk >> log2_rows;                                                          // of a tile, 16 at most
+        // Lane i: the page that box i of a tile comes from. (Nothing is done with it here: the warp would wait for the load.)
+        auto pages_of = [&](const int32_t* row_of_table, int tile, int len) {
+            const int at = (tile << 7) + (lane << log2_rows);
+            return lane < boxes && at < len ? row_of_table[at >> p.log2_page] : 0;
+        };
+        auto load = [&](const CUtensorMap* m, uint32_t dst, uint32_t bar, int pages, int tile, int hk, int len) {
+            const int left = len - (tile << 7), n = left >= kBlk ? boxes : (left + rows - 1) >> log2_rows;
+            pages = int(min(uint32_t(pages), uint32_t(p.n_pages)));  // (a page that there is not reads as zeros; the epilogue group reports it)
+            mbar_expect_tx_elect(bar, uint32_t(n) << (log2_rows + 7) << (S::NBOX - 1));
+            const int row = (tile << 7) & (p.page - 1) & ~(rows - 1);
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) {
+                const int page = __shfl_sync(0xffffffffu, pages, i);
+#pragma unroll
+                for (int x = 0; x < S::NBOX; ++x) tma_load_4d_elect(dst + uint32_t(x) * S::BOX, m, bar, x * 64, hk, row, page);
+                dst += uint32_t(rows) * 128u;
+            }
+        };
+        static_assert(S::NBOX == 1 || S::NBOX == 2, "bytes of a tile");
         if (aborted) {
         } else if (warp == 14) {
-            // ------------------------------ item scheduler ------------------------------
-            bool ok = true;
-            int k = 0;
+            // ------------------------------ item scheduler, and loads of Q and K ------------------------------
+            tma_prefetch_desc(&tmQ);
+            tma_prefetch_desc(&tmK);
+            bool ok = true, first = true;
+            int k = 0, gk = 0, pieces = 0;
+            int4 merge = make_int4(0, 0, 0, 0);
             if (!idle) {
                 paged_stretch(p, plan, worker, [&](const PagedWalk& walk, int, int lo, int hi, int part) {
                     const int s = k % NQ, use = k / NQ;
+                    const int T = uniform(hi - lo), tile0 = uniform(lo), hk = uniform(walk.hk), len = uniform(walk.s.len), tok0 = uniform(walk.s.start + walk.tile * p.tokens);
+                    const int32_t* const row_of_table = p.table + walk.b * p.table_stride;
+                    int pages = T > 0 ? pages_of(row_of_table, tile0, len) : 0;
                     if (use > 0) ok = mbar_wait_warp(BAR(B_ITEMEMPTY + s), (use - 1) & 1, ab, ST_WAIT_TIMEOUT + 11);
                     if (!ok) return false;
                     if (lane == 0) {
                         volatile int* it = info + 16 * s;
-                        it[I_TILES] = hi - lo;
-                        it[I_LO] = lo;
+                        it[I_TILES] = T;
+                        it[I_LO] = tile0;
                         it[I_MORE] = 1;
-                        it[I_HEAD] = walk.hk;
-                        it[I_ROW] = walk.s.start + walk.tile * p.tokens;
+                        it[I_HEAD] = hk;
+                        it[I_ROW] = tok0;
                         it[I_TOKENS] = min(p.tokens, walk.s.n - walk.tile * p.tokens);
                         it[I_POS] = walk.s.base + walk.tile * p.tokens;
-                        it[I_LEN] = walk.s.len;
+                        it[I_LEN] = len;
                         it[I_FRONT] = walk.s.front;
                         it[I_SEQ] = walk.b;
                         it[I_PART] = part;
                         mbar_arrive(BAR(B_ITEMFULL + s));
                     }
                     __syncwarp();
+                    // (an item's slot is given away when its O has left, so that Q has been read, too)
+                    mbar_expect_tx_elect(BAR(B_QFULL + s), uint32_t(p.tokens * p.G) * 128u * S::NBOX);
+                    for (int x = 0; x < S::NBOX; ++x) tma_load_4d_elect(sQ(s) + x * S::BOX, &tmQ, BAR(B_QFULL + s), x * 64, 0, hk, tok0);
+                    for (int t = 0; t < T; ++t, ++gk) {
+                        const int st = gk % NS, ug = gk / NS, own = pages;
+                        if (t + 1 < T) pages = pages_of(row_of_table, tile0 + t + 1, len);
+                        if (ug > 0) ok = mbar_wait_warp(BAR(B_KEMPTY + st), (ug - 1) & 1, ab, ST_WAIT_TIMEOUT + 1);
+                        if (!ok) return false;
+                        load(&tmK, sK(st), BAR(B_KFULL + st), own, tile0 + t, hk, len);
+                    }
                     ++k;
+                    if (first && paged_first_cut(plan, worker, walk)) {
+                        // the item that this worker's stretch begins within is merged from its pieces by the second kernel
+                        for (int i0 = 0;; i0 += 32) {
+                            bool last;
+                            const int slot = paged_piece(p, plan, worker, walk, i0 + lane, last);
+                            const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
+                            // (a piece behind the last one has no tiles)
+                            if (slot >= 0) p.merge_slots[2 * worker + pieces + __popc(there & ((1u << lane) - 1u))] = slot;
+                            pieces += __popc(there);
+                            if (__any_sync(0xffffffffu, last)) break;
+                        }
+                        merge = make_int4(pieces, tok0, min(p.tokens, walk.s.n - walk.tile * p.tokens), hk);
+                    }
+                    first = false;
                     return true;
                 });
             }
+            if (lane == 0) p.merge[worker] = merge;
             if (ok) {  // end marker
                 const int s = k % NQ, use = k / NQ;
                 if (use > 0) ok = mbar_wait_warp(BAR(B_ITEMEMPTY + s), (use - 1) & 1, ab, ST_WAIT_TIMEOUT + 11);
@@ -172,102 +226,30 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 }
             }
         } else if (warp == 12) {
-            // ------------------------------ TMA producer ------------------------------
-            // Two walks over the block's tiles, as in the forward kernel: K (with its item's Q), up to kAhead tiles ahead of V.
-            tma_prefetch_desc(&tmQ);
-            tma_prefetch_desc(&tmK);
+            // ------------------------------ loads of V ------------------------------
             tma_prefetch_desc(&tmV);
-            constexpr int kAhead = 3;
-            const int rows = p.page < kBlk ? p.page : kBlk;  // of a box
-            const int boxes = kBlk / rows;                   // of a tile, 16 at most
-            bool ok = true, last = false;
-            int kk = -1, kt = 0, kT = 0, gk = 0, klo = 0, khk = 0, klen = 0, kseq = 0;
-            int vk = -1, vt = 0, vT = 0, gv = 0, vlo = 0, vhk = 0, vlen = 0, vseq = 0;
-            // Lane i: the page that box i of the tile comes from, or -1 behind the sequence's end.
-            auto pages_of = [&](int seq, int tile, int len) {
-                const int at = tile * kBlk + lane * rows;
-                if (lane >= boxes || at >= len) return -1;
-                const int page = p.table[int64_t(seq) * p.table_stride + (at >> p.log2_page)];
-                if (uint32_t(page) >= uint32_t(p.n_pages)) {
-                    atomicCAS(p.status, 0, ST_PAGED_PAGE);
-                    return p.n_pages;  // beyond the tensor: zeros
-                }
-                return page;
-            };
-            auto load = [&](const CUtensorMap* m, uint32_t dst, uint32_t bar, int pages, int tile, int hk, int len) {
-                const int left = len - tile * kBlk, n = left >= kBlk ? boxes : cdiv(left, rows);
-                mbar_expect_tx_elect(bar, uint32_t(n * rows) * 128u * S::NBOX);
-                const int row = p.page > kBlk ? tile * kBlk & (p.page - 1) : 0;
-                for (int i = 0; i < n; ++i) {
-                    const int page = __shfl_sync(0xffffffffu, pages, i);
-#pragma unroll
-                    for (int x = 0; x < S::NBOX; ++x)
-                        tma_load_4d_elect(dst + uint32_t(x) * S::BOX + uint32_t(i * rows) * 128u, m, bar, x * 64, hk, row, page);
-                }
-            };
-            int kpages = -1, vpages = -1;  // of the next tile of each walk
-            while (ok) {
-                while (vt == vT && vk < kk) {  // the V walk goes on to the next item
-                    if (vk >= 0 && lane == 0) mbar_arrive(BAR(B_ITEMEMPTY + vk % NQ));
-                    ++vk;
-                    volatile int* it = info + 16 * (vk % NQ);
-                    vt = 0;
-                    vT = uniform(it[I_TILES]);
-                    vlo = uniform(it[I_LO]);
-                    vhk = uniform(it[I_HEAD]);
-                    vlen = uniform(it[I_LEN]);
-                    vseq = uniform(it[I_SEQ]);
-                    if (vT > 0) vpages = pages_of(vseq, vlo, vlen);
-                }
-                if (last && gv == gk) break;
-                bool do_k = !last && gk - gv < kAhead;
-                if (do_k && kt == kT) {  // the next item: the rows of the one that had its slot must have left
-                    const int s = (kk + 1) % NQ, use = (kk + 1) / NQ;
-                    if (gv < gk && !(mbar_test_warp(BAR(B_ITEMFULL + s), use & 1) &&
-                                     (use == 0 || mbar_test_warp(BAR(B_QEMPTY + s), (use - 1) & 1)))) {
-                        do_k = false;
-                    } else {
-                        ok = mbar_wait_warp(BAR(B_ITEMFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 12);
-                        if (!ok) break;
-                        volatile int* it = info + 16 * s;
-                        if (uniform(it[I_MORE]) < 0) {
-                            last = true;
-                            continue;
-                        }
-                        if (use > 0) ok = mbar_wait_warp(BAR(B_QEMPTY + s), (use - 1) & 1, ab, ST_WAIT_TIMEOUT + 13);
-                        if (!ok) break;
-                        ++kk;
-                        kt = 0;
-                        kT = uniform(it[I_TILES]);
-                        klo = uniform(it[I_LO]);
-                        khk = uniform(it[I_HEAD]);
-                        klen = uniform(it[I_LEN]);
-                        kseq = uniform(it[I_SEQ]);
-                        const int row = uniform(it[I_ROW]);
-                        if (kT > 0) kpages = pages_of(kseq, klo, klen);
-                        mbar_expect_tx_elect(BAR(B_QFULL + s), uint32_t(p.tokens * p.G) * 128u * S::NBOX);
-                        for (int x = 0; x < S::NBOX; ++x)
-                            tma_load_4d_elect(sQ(s) + x * S::BOX, &tmQ, BAR(B_QFULL + s), x * 64, 0, khk, row);
-                        continue;  // (an item may have no tiles)
-                    }
-                }
-                if (do_k) {
-                    const int st = gk % NS, ug = gk / NS, pages = kpages;
-                    if (kt + 1 < kT) kpages = pages_of(kseq, klo + kt + 1, klen);
-                    if (ug > 0) ok = mbar_wait_warp(BAR(B_KEMPTY + st), (ug - 1) & 1, ab, ST_WAIT_TIMEOUT + 1);
-                    if (!ok) break;
-                    load(&tmK, sK(st), BAR(B_KFULL + st), pages, klo + kt, khk, klen);
-                    ++kt;
-                    ++gk;
-                } else {
-                    const int st = gv % NS, ug = gv / NS, pages = vpages;
-                    if (vt + 1 < vT) vpages = pages_of(vseq, vlo + vt + 1, vlen);
+            bool ok = true;
+            int gv = 0;
+            for (int k = 0; ok; ++k) {
+                const int s = k % NQ, use = k / NQ;
+                ok = mbar_wait_warp(BAR(B_ITEMFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 12);
+                if (!ok) break;
+                volatile int* it = info + 16 * s;
+                const int T = uniform(it[I_TILES]), lo = uniform(it[I_LO]), hk = uniform(it[I_HEAD]), len = uniform(it[I_LEN]), seq = uniform(it[I_SEQ]);
+                if (uniform(it[I_MORE]) < 0) break;
+                const int32_t* const row_of_table = p.table + seq * p.table_stride;
+                int pages = T > 0 ? pages_of(row_of_table, lo, len) : 0;
+                for (int t = 0; t < T; ++t, ++gv) {
+                    const int st = gv % NS, ug = gv / NS, own = pages;
+                    if (t + 1 < T) pages = pages_of(row_of_table, lo + t + 1, len);
                     if (ug > 0) ok = mbar_wait_warp(BAR(B_VEMPTY + st), (ug - 1) & 1, ab, ST_WAIT_TIMEOUT + 2);
                     if (!ok) break;
-                    load(&tmV, sV(st), BAR(B_VFULL + st), pages, vlo + vt, vhk, vlen);
-                    ++vt;
-                    ++gv;
+                    load(&tmV, sV(st), BAR(B_VFULL + st), own, lo + t, hk, len);
                 }
+                if (!ok) break;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(BAR(B_ITEMEMPTY + s));
+                __syncwarp();
             }
         } else {
             // ------------------------------ MMA issuers ------------------------------
@@ -276,15 +258,6 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             constexpr uint32_t idesc_s = make_idesc(BF16, 128, 128, false, false);
             constexpr uint32_t idesc_pv = make_idesc(BF16, 128, D, false, true);
             constexpr uint64_t desc_v = desc_mn_major(S::BOX);
-            // Rows behind the sequence's end hold what was in the page, or in the stage.
-            auto zero_behind = [&](int tile, int real) {
-                if (real >= kBlk) return;
-#pragma unroll
-                for (int x = 0; x < S::NBOX; ++x)
-                    for (int i = real * 8 + lane; i < kBlk * 8; i += 32) reinterpret_cast<uint4*>(smem + tile + x * S::BOX)[i] = make_uint4(0, 0, 0, 0);
-                fence_proxy_async();
-                __syncwarp();
-            };
             bool ok = true;
             int G = 0;           // tiles of all earlier items
             int n0 = 0, n1 = 0;  // items in which the chains had tiles
@@ -292,7 +265,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 const int s = k % NQ, use = k / NQ;
                 ok = mbar_wait_warp(BAR(B_ITEMFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 12);
                 if (!ok) break;
-                const int T = uniform(info[16 * s + I_TILES]), lo = uniform(info[16 * s + I_LO]), len = uniform(info[16 * s + I_LEN]);
+                const int T = uniform(info[16 * s + I_TILES]);
                 if (uniform(info[16 * s + I_MORE]) < 0) break;
                 if (warp == 15) {
                     if (T > 0) ok = mbar_wait_warp(BAR(B_QFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 3);
@@ -303,7 +276,6 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         if (S::POWN && ok && g > 0) ok = mbar_wait_warp(BAR(B_SFREE + ((g - 1) & 1)), ((g - 1) >> 1) & 1, ab, ST_WAIT_TIMEOUT + 15);
                         if (!S::POWN && ok && g >= NP) ok = mbar_wait_warp(BAR(B_PVDONE + g % NP), (g / NP - 1) & 1, ab, ST_WAIT_TIMEOUT + 15);
                         if (!ok) break;
-                        zero_behind(S::off_k + st * S::TILE, len - (lo + g - G) * kBlk);
                         tc_fence_after();
                         const uint32_t tS = utmem + uint32_t(S::tmem_s(g)), q_tile = sQ(s), k_tile = sK(st);
 #pragma unroll
@@ -319,7 +291,6 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         const int g = G + t, st = g % NS, w = g & 1;
                         const uint32_t tO = utmem + uint32_t(S::tmem_o + w * D), tP = utmem + uint32_t(S::tmem_p(g)), v_tile = sV(st);
                         ok = mbar_wait_warp(BAR(B_VFULL + st), (g / NS) & 1, ab, ST_WAIT_TIMEOUT + 5);
-                        if (ok) zero_behind(S::off_v + st * S::TILE, len - (lo + t) * kBlk);
                         // The first P*V of a chain in an item overwrites its O: the epilogue of the last item that used it must have
                         // read it. (o_full and o_free count the items in which the chain had tiles, on both sides.)
                         const int n = w ? n1 : n0;
@@ -373,6 +344,12 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             const int T = it[I_TILES], part = it[I_PART], hk = it[I_HEAD], row = it[I_ROW] + tok;
             if (it[I_MORE] < 0) break;
             const bool valid = tok < it[I_TOKENS];
+            {
+                const int64_t row_of_table = it[I_SEQ] * p.table_stride;
+                const int last = min((it[I_LO] + T) * kBlk, it[I_LEN]) - 1;
+                for (int i = (it[I_LO] * kBlk >> p.log2_page) + r; i <= last >> p.log2_page && T > 0; i += kBlk)
+                    if (uint32_t(p.table[row_of_table + i]) >= uint32_t(p.n_pages)) atomicCAS(p.status, 0, ST_PAGED_PAGE);
+            }
             // the only wait here that lasts as long as an item: it allows each of the tiles what another wait may last
             const Abort item{ab.flag, ab.status, ab.limit * (T + 1)};
             alive = mbar_wait_warp(BAR(B_MLFULL + s), use & 1, item, ST_WAIT_TIMEOUT + 16);
@@ -387,8 +364,6 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             const float* ml = reinterpret_cast<const float*>(smem + S::off_ml) + s * (4 * kBlk);  // [2 groups][m, l][128]
             const int even = we * (2 * kBlk), odd = 2 * kBlk - even;
             const float m0 = ml[even + r], l0 = ml[even + kBlk + r], m1 = ml[odd + r], l1 = ml[odd + kBlk + r];
-            // Q has been read (every S of the item is complete) and so have m and l
-            if (warp == 8 && lane == 0) mbar_arrive(BAR(B_QEMPTY + s));
             const float mt = fmaxf(m0, m1);
             const float a0 = (m0 == -INFINITY) ? 0.f : fast_exp2((m0 - mt) * c);
             const float a1 = (m1 == -INFINITY) ? 0.f : fast_exp2((m1 - mt) * c);
@@ -397,6 +372,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             const float f0 = a0 * inv, f1 = a1 * inv;
             // a chain in which the row had no key takes no part, whatever the values behind its mask are
             const bool use0 = (T > 0) && (f0 != 0.f), use1 = (T > 1) && (f1 != 0.f);
+            const bool both = __all_sync(0xffffffffu, !valid || (use0 && use1));
             const bool store = valid && misc[1] == 0;
             if (part >= 0 && store)  // (a piece that went NaN says so: -inf would pass for a piece without keys)
                 p.part_lse[int64_t(part) * kBlk + r] = lt > 0.f ? fmaf(mt, c, log2f(lt)) : lt == lt ? -INFINITY : lt;
@@ -415,12 +391,17 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     if (T > 0) mbar_arrive_warp(BAR(B_OFREE + we), lane);
                     if (T > 1) mbar_arrive_warp(BAR(B_OFREE + (we ^ 1)), lane);
                 }
+                if (both) {
 #pragma unroll
-                for (int y = 0; y < 16; ++y) {
-                    float v = 0.f;
-                    if (use0) v = __uint_as_float(x0[y]) * f0;
-                    if (use1) v = fmaf(__uint_as_float(x1[y]), f1, v);
-                    x0[y] = __float_as_uint(v);
+                    for (int y = 0; y < 16; ++y) x0[y] = __float_as_uint(fmaf(__uint_as_float(x1[y]), f1, __uint_as_float(x0[y]) * f0));
+                } else {
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) {
+                        float v = 0.f;
+                        if (use0) v = __uint_as_float(x0[y]) * f0;
+                        if (use1) v = fmaf(__uint_as_float(x1[y]), f1, v);
+                        x0[y] = __float_as_uint(v);
+                    }
                 }
                 if (store && 16 * q < p.D) {
                     if (part >= 0) {
@@ -451,6 +432,15 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const uint32_t tO = tmem + lane_base + uint32_t(S::tmem_o + w * D);
         const int tok = r / p.G, g_row = r - tok * p.G;
         bool alive = !aborted;
+        // Rows of V behind the sequence's end hold what was in the page, or in the stage: zeros, before P*V(g) is issued. A quarter of them a warp.
+        auto zero_behind = [&](int g, int real) {
+            const int st = g % NS;
+            if (!mbar_wait_warp(BAR(B_VFULL + st), (g / NS) & 1, ab, ST_WAIT_TIMEOUT + 19)) return false;
+            for (int x = 0; x < S::NBOX; ++x)
+                for (int i = real * 8 + r; i < kBlk * 8; i += kBlk) reinterpret_cast<uint4*>(smem + S::off_v + st * S::TILE + x * S::BOX)[i] = make_uint4(0, 0, 0, 0);
+            fence_proxy_async();
+            return true;
+        };
         int G = 0;  // tiles of all earlier items
         for (int k = 0; alive; ++k) {
             const int s = k % NQ, use = k / NQ;
@@ -487,6 +477,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         alive = pv_before();
                         if (!alive) break;
                     }
+                    if (len - k0 < kBlk) alive = zero_behind(g, len - k0);
+                    if (!alive) break;
                     mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
                     continue;
                 }
@@ -499,7 +491,13 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     mbar_arrive_warp(BAR(B_SFREE + w), lane);  // the next tile's scores may overwrite these
                 }
                 float* sc = reinterpret_cast<float*>(sr);
+                const int real = len - k0;  // keys of the tile that there are
                 if constexpr (SCORED) {
+                    // (what the others' scores are must not tell the warp which form of the cap to take)
+                    if (real < kBlk) {
+#pragma unroll
+                        for (int x = 0; x < kBlk; ++x) sc[x] = x < real ? sc[x] : 0.f;
+                    }
                     const Bias bias(slope, front == 0, pos0 - (k0 + kBlk - 1), pos0 + kBlk - 1 - k0);
                     score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, pos - k0, valid);
                 }
@@ -574,8 +572,10 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     tmem_st16(tP + uint32_t(q) * 16u, pk);
                 }
                 tc_wait_st();
+                if (real < kBlk) alive = zero_behind(g, real);
                 tc_fence_before();
                 mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
+                if (!alive) break;
                 {
                     float a0, a1, b0, b1;
                     unpack_f2(lacc0, a0, a1);
@@ -603,48 +603,111 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
 }
 
-// Merges the pieces of the items that a cut went through: O = sum_s w_s O_s with w_s = 2^(lse_s - lse). Block w looks after the item
-// that the cut before worker w goes through first. A piece whose lse is NaN or +inf makes the row its own, as in fwd_combine_kernel. All
-// sums in fp32, in the order of the pieces. One warp per row, lane l owns columns l, l + 32, ...
-template <bool BF16>
-__global__ void __launch_bounds__(256) paged_combine_kernel(const PagedParams p, int most_workers) {
-    __shared__ PagedPlan plan;
-    // The lengths were complete before the attention kernel let this one begin, so that the plan need not wait for that kernel.
-    paged_plan<256>(p, plan, most_workers);
-    wait_prerequisites();
-    launch_dependents();
+// Merges the pieces of the items that a cut went through: O = sum_s w_s O_s with w_s = 2^(lse_s - lse). The blocks (w, 0 .. 3) look after the item that
+// the cut before worker w goes through first, each after 32 of its rows; the attention kernel has left a list of its pieces. A piece whose lse is NaN or +inf makes the row its own, as in fwd_combine_kernel. All sums in fp32, in an order that the number of rows
+// and pieces gives. Bound by latency: a warp has four rows, whose loads are in flight together, and where there are few rows (a decoded token's
+// heads) several warps share the pieces.
+constexpr int kCombineThreads = 256, kCombineRows = 4;
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const PagedParams p) {
+    constexpr int kOwn = D / 32, kBatch = 4, kWarps = kCombineThreads / 32;  // columns of a lane; pieces in flight
+    __shared__ float sums[kWarps][kCombineRows][D + 1];
+    follow_stream();
     const int w = int(blockIdx.x), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    PagedWalk walk;
-    if (!paged_first_cut(p, plan, w, walk) || status_is_fatal(*reinterpret_cast<volatile int*>(p.status))) return;
-    int pieces = 0;
-    paged_pieces(p, plan, w, walk, [&](int) { ++pieces; });
-    if (pieces < 2) return;  // one piece that has all tiles has gone straight to the output
-    const int Dk = p.D > 64 ? 128 : 64;
-    const int tokens = min(p.tokens, walk.s.n - walk.tile * p.tokens);
-    for (int r = warp; r < tokens * p.G; r += 8) {
-        const int tok = r / p.G, g = r - tok * p.G;
-        float top = -INFINITY, total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-        bool spoilt = false;
-        paged_pieces(p, plan, w, walk, [&](int slot) {
-            const float lse = p.part_lse[int64_t(slot) * kBlk + r];
-            spoilt |= !(lse < INFINITY);
-            top = fmaxf(top, lse);
-        });
-        if (top != -INFINITY || spoilt)
-            paged_pieces(p, plan, w, walk, [&](int slot) {
-                const int64_t at = int64_t(slot) * kBlk + r;
-                const float lse = p.part_lse[at], wgt = !spoilt ? fast_exp2(lse - top) : lse < INFINITY ? 0.f : 1.f;
-                if (wgt == 0.f) return;
-                total += wgt;
+    const bool failed = status_is_fatal(*reinterpret_cast<volatile int*>(p.status));
+    const int4 merge = p.merge[w];
+    const int* const slots = p.merge_slots + 2 * w;
+    const int pieces = merge.x, rows = merge.z * p.G - int(blockIdx.y) * kWarps * kCombineRows, row0 = int(blockIdx.y) * kWarps * kCombineRows;
+    if (failed || pieces < 2 || rows <= 0) return;
+    const int groups = min(cdiv(rows, kCombineRows), kWarps), subs = kWarps / groups;
+    const int sub = warp / groups, r0 = (warp - sub * groups) * kCombineRows;  // (of this block's rows)
+    float top[kCombineRows], acc[kCombineRows][kOwn] = {}, total[kCombineRows] = {};
+    if (sub < subs) {
+        bool spoilt[kCombineRows] = {};
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (lane + 32 * i < p.D) acc[i] = fmaf(wgt, p.part_o[at * Dk + lane + 32 * i], acc[i]);
-            });
-        const float inv = total > 0.f ? 1.f / total : 0.f;
-        uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(walk.s.start + walk.tile * p.tokens + tok) * p.out_t + int64_t(walk.hk * p.G + g) * p.out_h;
+        for (int i = 0; i < kCombineRows; ++i) top[i] = -INFINITY;
+        for (int s = lane; s < pieces; s += 32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 32 * i < p.D) out[lane + 32 * i] = uint16_t(pack2<BF16>(acc[i] * inv, 0.f));
+            for (int i = 0; i < kCombineRows; ++i) {
+                const float lse = r0 + i < rows ? p.part_lse[int64_t(slots[s]) * kBlk + row0 + r0 + i] : -INFINITY;
+                spoilt[i] |= !(lse < INFINITY);
+                top[i] = fmaxf(top[i], lse);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kCombineRows; ++i) {
+            spoilt[i] = __any_sync(0xffffffffu, spoilt[i]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+        }
+#pragma unroll 1
+        for (int s0 = sub; s0 < pieces; s0 += subs * kBatch) {
+            float v[kBatch][kCombineRows][kOwn], lse[kBatch][kCombineRows];
+#pragma unroll
+            for (int s = 0; s < kBatch; ++s) {
+                const int64_t at = int64_t(slots[min(s0 + s * subs, pieces - 1)]) * kBlk;
+#pragma unroll
+                for (int i = 0; i < kCombineRows; ++i) {
+                    const int64_t row = at + row0 + min(r0 + i, rows - 1);
+                    lse[s][i] = p.part_lse[row];
+                    if constexpr (kOwn == 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(p.part_o + row * D + 4 * lane);
+                        v[s][i][0] = x.x; v[s][i][1] = x.y; v[s][i][2] = x.z; v[s][i][3] = x.w;
+                    } else {
+                        // (columns beyond a head dim of 16 or 32 have not been written, and go nowhere)
+                        const float2 x = *reinterpret_cast<const float2*>(p.part_o + row * D + 2 * lane);
+                        v[s][i][0] = x.x; v[s][i][1] = x.y;
+                    }
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < kBatch; ++s) {
+                if (s0 + s * subs >= pieces) break;
+#pragma unroll
+                for (int i = 0; i < kCombineRows; ++i) {
+                    const float x = lse[s][i], wgt = spoilt[i] ? (x < INFINITY ? 0.f : 1.f) : top[i] == -INFINITY ? 0.f : fast_exp2(x - top[i]);
+                    if (wgt == 0.f) continue;
+                    total[i] += wgt;
+#pragma unroll
+                    for (int c = 0; c < kOwn; ++c) acc[i][c] = fmaf(wgt, v[s][i][c], acc[i][c]);
+                }
+            }
+        }
+    }
+    if (subs > 1) {  // (the same for all threads)
+        float (*mine)[D + 1] = sums[warp];
+        if (sub > 0 && sub < subs) {
+#pragma unroll
+            for (int i = 0; i < kCombineRows; ++i) {
+#pragma unroll
+                for (int c = 0; c < kOwn; ++c) mine[i][lane * kOwn + c] = acc[i][c];
+                if (lane == 0) mine[i][D] = total[i];
+            }
+        }
+        __syncthreads();
+        if (sub == 0) {
+            for (int u = 1; u < subs; ++u) {
+#pragma unroll
+                for (int i = 0; i < kCombineRows; ++i) {
+#pragma unroll
+                    for (int c = 0; c < kOwn; ++c) acc[i][c] += sums[warp + u * groups][i][lane * kOwn + c];
+                    total[i] += sums[warp + u * groups][i][D];
+                }
+            }
+        }
+    }
+    if (sub > 0 || lane * kOwn >= p.D) return;
+#pragma unroll
+    for (int i = 0; i < kCombineRows; ++i) {
+        if (r0 + i >= rows) return;
+        const int r = row0 + r0 + i, tok = r / p.G, g = r - tok * p.G;
+        const float inv = total[i] > 0.f ? 1.f / total[i] : 0.f;
+        uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(merge.y + tok) * p.out_t + int64_t(merge.w * p.G + g) * p.out_h + lane * kOwn;
+        if constexpr (kOwn == 4)
+            *reinterpret_cast<uint2*>(out) = make_uint2(pack2<BF16>(acc[i][0] * inv, acc[i][1] * inv), pack2<BF16>(acc[i][2] * inv, acc[i][3] * inv));
+        else
+            *reinterpret_cast<uint32_t*>(out) = pack2<BF16>(acc[i][0] * inv, acc[i][1] * inv);
     }
 }
 
@@ -658,7 +721,7 @@ static cudaError_t launch_paged_t(const CUtensorMap& tq, const CUtensorMap& tk, 
     if (e != cudaSuccess) return e;
     e = launch_overlapping(kern, dim3(workers), kFwdThreads, smem, stream, tq, tk, tv, p);
     if (e != cudaSuccess) return e;
-    return launch_overlapping(paged_combine_kernel<BF16>, dim3(workers), 256, 0, stream, p, workers);
+    return launch_overlapping(paged_combine_kernel<D, BF16>, dim3(workers, kBlk / (kCombineThreads / 32 * kCombineRows)), kCombineThreads, 0, stream, p);
 }
 
 cudaError_t launch_paged_fwd(bool bf16, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {

@@ -3,8 +3,8 @@
 //
 // An item is a tile of queries (tokens_per_tile new tokens of a sequence, all heads of a kv head's group) of one kv head. Its weight is the
 // number of keys that its last token sees, and a constant for what an item costs besides its tiles. The items, in the order sequence, kv head,
-// tile, lie behind one another on a line of length `total`, and worker w of n gets the stretch [w total / n, (w + 1) total / n) of it: equal work
-// whatever the lengths, with at most n - 1 cuts. An item that a cut goes through is computed in pieces, whose fp32 rows the second kernel merges.
+// tile, lie behind one another on a line of length `total`, and each of n workers gets an equal stretch of it, whatever the lengths, with at most
+// n - 1 cuts. An item that a cut goes through is computed in pieces, whose fp32 rows the second kernel merges.
 // Where whole items, one a worker, are done as soon, nothing is cut (`keyed` false: all weights are 1).
 #pragma once
 #include "common.cuh"
@@ -14,11 +14,12 @@ namespace fa {
 
 constexpr int kPagedGroups = 1024;   // entries of the table of sums: a sequence each, or several
 constexpr int kPagedItemCost = 256;  // of an item, in keys
-constexpr int kPagedPieceKeys = 512; // a worker's stretch is at least this long
+constexpr int kPagedLog2Piece = 10;  // a worker's stretch is at least 2 to this long
 constexpr int kPagedMergeTiles = 6;  // of the second kernel, in tiles of 128 keys
 
 struct PagedPlan {
     long long total;
+    long long stretch;  // of a worker: no less than total / workers
     int workers;
     int keyed;
     int group;  // sequences an entry of `sums`
@@ -79,13 +80,20 @@ __host__ __device__ __forceinline__ long long paged_weight(const PagedParams& p,
     return m == s.tiles && m > 0 ? sum + s.len : sum;
 }
 
+// a / b for 0 <= a, 0 < b: the short division where it will do
+__host__ __device__ __forceinline__ long long paged_divide(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)(uint32_t(a) / uint32_t(b)) : a / b;
+}
+
 // Weights of all items together, their number and the longest sequence's length, to the plan's numbers.
 __host__ __device__ __forceinline__ void paged_share_out(PagedPlan& plan, long long weight, long long items, int longest, int most_workers) {
-    long long workers = weight / (kPagedPieceKeys + kPagedItemCost);
+    long long workers = weight >> kPagedLog2Piece;
     workers = workers < 1 ? 1 : workers > most_workers ? most_workers : workers;
-    plan.keyed = items > most_workers || cdiv(longest, kBlk) > weight / workers / kBlk + kPagedMergeTiles;
+    plan.keyed = items > most_workers || (long long)(cdiv(longest, kBlk) - kPagedMergeTiles) * kBlk * workers > weight;
     plan.workers = int(plan.keyed ? workers : items);
     plan.total = plan.keyed ? weight : items;
+    // (a hair more than total / workers: a division in fp32 takes a fraction of one of 64 bits)
+    plan.stretch = plan.keyed ? (long long)(float(weight) / float(workers) * 1.00001f) + 1 : 1;
 }
 
 // All threads of the block (a multiple of 32, at most 1024, that divides 2 * kPagedGroups). Ends with a barrier.
@@ -110,42 +118,42 @@ __device__ __forceinline__ void paged_plan(const PagedParams& p, PagedPlan& plan
         w += weight[o];
         n += items[o];
     }
+    // inclusive sums over the warp, then over the warps
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    long long w_before = w, n_before = n;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        w += __shfl_xor_sync(0xffffffffu, w, o);
-        n += __shfl_xor_sync(0xffffffffu, n, o);
-        longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, w_before, o), y = __shfl_up_sync(0xffffffffu, n_before, o);
+        if (lane >= o) {
+            w_before += x;
+            n_before += y;
+        }
     }
-    if (lane == 0) {
-        plan.warp_sums[warp] = w;
-        plan.warp_items[warp] = n;
+    if (lane == 31) {
+        plan.warp_sums[warp] = w_before;
+        plan.warp_items[warp] = n_before;
         plan.warp_max[warp] = longest;
     }
     __syncthreads();
+    w_before -= w;
+    n_before -= n;
     w = n = 0;
     longest = 0;
+#pragma unroll
     for (int i = 0; i < kWarps; ++i) {
-        w += plan.warp_sums[i];
-        n += plan.warp_items[i];
+        const long long x = plan.warp_sums[i], y = plan.warp_items[i];
+        w += x;
+        n += y;
+        if (i < warp) {
+            w_before += x;
+            n_before += y;
+        }
         longest = max(longest, plan.warp_max[i]);
     }
     PagedPlan own;
     paged_share_out(own, w, n, longest, most_workers);
     const bool keyed = own.keyed;
-    long long mine = 0;
-#pragma unroll
-    for (int o = 0; o < kOwn; ++o) mine += keyed ? weight[o] : items[o];
-    long long before = mine;  // an inclusive sum over the warp, then the warps before
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += x;
-    }
-    __syncthreads();  // (the sums above have been read)
-    if (lane == 31) plan.warp_sums[warp] = before;
-    __syncthreads();
-    before -= mine;
-    for (int i = 0; i < warp; ++i) before += plan.warp_sums[i];
+    long long before = keyed ? w_before : n_before;
 #pragma unroll
     for (int o = 0; o < kOwn; ++o) {
         plan.sums[first + o] = before;
@@ -153,6 +161,7 @@ __device__ __forceinline__ void paged_plan(const PagedParams& p, PagedPlan& plan
     }
     if (threadIdx.x == 0) {
         plan.total = plan.sums[kPagedGroups] = own.total;
+        plan.stretch = own.stretch;
         plan.workers = own.workers;
         plan.keyed = own.keyed;
         plan.group = group;
@@ -160,10 +169,10 @@ __device__ __forceinline__ void paged_plan(const PagedParams& p, PagedPlan& plan
     __syncthreads();
 }
 
-// Where worker w's stretch begins.
+// Where worker w's stretch begins; the last ones' may be empty.
 __host__ __device__ __forceinline__ long long paged_cut(const PagedPlan& plan, int w) {
-    // total < 2^49 (see api.cu) and w <= 2^14
-    return plan.total * w / plan.workers;
+    const long long x = plan.stretch * w;
+    return x < plan.total ? x : plan.total;
 }
 
 // A walk over the items from a point of the line on.
@@ -174,11 +183,14 @@ struct PagedWalk {
 
     // The item that covers x, 0 <= x < total.
     __host__ __device__ __forceinline__ void find(const PagedParams& p, const PagedPlan& plan, long long x) {
-        int lo = 0, hi = kPagedGroups;  // sums[lo] <= x < sums[hi]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (plan.sums[mid] <= x) lo = mid; else hi = mid;
-        }
+        int lo = 0;  // the last entry with sums[lo] <= x
+#ifdef __CUDA_ARCH__
+        static_assert(kPagedGroups == 32 * 32, "two steps of a warp");  // (whose lanes all ask for the same x)
+        lo = 32 * (31 - __clz(__ballot_sync(0xffffffffu, plan.sums[32 * (threadIdx.x & 31)] <= x)));
+        lo += 31 - __clz(__ballot_sync(0xffffffffu, plan.sums[lo + (threadIdx.x & 31)] <= x));
+#else
+        while (lo + 1 < kPagedGroups && plan.sums[lo + 1] <= x) ++lo;
+#endif
         long long rem = x - plan.sums[lo];
         b = lo * plan.group;
         long long head;
@@ -194,7 +206,7 @@ struct PagedWalk {
             if (rem < head * p.Hk) break;
             rem -= head * p.Hk;
         }
-        hk = int(rem / head);
+        hk = int(paged_divide(rem, head));
         rem -= hk * head;
         int t0 = 0, t1 = s.tiles;  // weight(t0) <= rem < weight(t1)
         while (t1 - t0 > 1) {
@@ -222,8 +234,9 @@ struct PagedWalk {
         const int n = key_tiles(p);
         if (x <= at) return 0;
         if (x >= end(p, plan)) return n;
-        const long long t = (x - at - kPagedItemCost) / kBlk;
-        return t < 0 ? 0 : t > n ? n : int(t);
+        const long long t = x - at - kPagedItemCost;
+        static_assert(kBlk == 1 << 7, "shift");
+        return t < 0 ? 0 : (t >> 7) > n ? n : int(t >> 7);
     }
 };
 
@@ -232,8 +245,9 @@ struct PagedWalk {
 // whose rows are zeros.
 template <class Emit>
 __host__ __device__ __forceinline__ void paged_stretch(const PagedParams& p, const PagedPlan& plan, int w, Emit emit) {
-    const long long x0 = paged_cut(plan, w), x1 = paged_cut(plan, w + 1);
     PagedWalk walk;
+    const long long x0 = paged_cut(plan, w), x1 = paged_cut(plan, w + 1);
+    if (x0 >= x1) return;
     walk.find(p, plan, x0);
     for (long long from = x0;;) {
         const int n = walk.key_tiles(p), lo = walk.key_tile_at(p, plan, from), hi = walk.key_tile_at(p, plan, x1);
@@ -244,23 +258,17 @@ __host__ __device__ __forceinline__ void paged_stretch(const PagedParams& p, con
     }
 }
 
-// Does the cut before worker w go through an item, as the first one that does? `walk` is at that item then.
-__host__ __device__ __forceinline__ bool paged_first_cut(const PagedParams& p, const PagedPlan& plan, int w, PagedWalk& walk) {
-    if (w <= 0 || w >= plan.workers) return false;
-    const long long x = paged_cut(plan, w);
-    walk.find(p, plan, x);
-    return walk.s.tiles > 0 && walk.at < x && (w == 1 || walk.at >= paged_cut(plan, w - 1));
+// Is the cut before worker w the first one through the item at `walk`, which it falls into?
+__host__ __device__ __forceinline__ bool paged_first_cut(const PagedPlan& plan, int w, const PagedWalk& walk) {
+    return w > 0 && walk.s.tiles > 0 && walk.at < paged_cut(plan, w) && (w == 1 || walk.at >= paged_cut(plan, w - 1));
 }
 
-// The pieces of the item at `walk`, which the cut before worker w goes through first: each(slot) in their order.
-template <class Each>
-__host__ __device__ __forceinline__ void paged_pieces(const PagedParams& p, const PagedPlan& plan, int w, const PagedWalk& walk, Each each) {
-    const int n = walk.key_tiles(p);
-    for (int v = w, lo = 0; lo < n; ++v) {
-        const int hi = v < plan.workers ? walk.key_tile_at(p, plan, paged_cut(plan, v)) : n;
-        if (hi > lo) each(2 * (v - 1) + (lo == 0 ? 1 : 0));
-        lo = hi;
-    }
+// Piece i of the item at `walk`, which the cut before worker w goes through first: worker w - 1 + i's. Its slot, or -1 if it has no tiles. There are none
+// behind the first i with `last`.
+__host__ __device__ __forceinline__ int paged_piece(const PagedParams& p, const PagedPlan& plan, int w, const PagedWalk& walk, int i, bool& last) {
+    const int lo = i == 0 ? 0 : walk.key_tile_at(p, plan, paged_cut(plan, w + i - 1)), hi = walk.key_tile_at(p, plan, paged_cut(plan, w + i));
+    last = hi >= walk.key_tiles(p);
+    return hi > lo ? 2 * (w - 1 + i) + (lo == 0 ? 1 : 0) : -1;
 }
 
 }  // namespace fa
