@@ -8,7 +8,7 @@
 
 namespace fa {
 cudaError_t launch_paged_append(const PagedParams&, const void*, const void*, void*, void*, const int64_t*, cudaStream_t);
-cudaError_t launch_paged_fwd(bool, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const PagedParams&, int, cudaStream_t);
+cudaError_t launch_paged_fwd(bool, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const PagedParams&, int, cudaStream_t);
 }  // namespace fa
 
 namespace {
@@ -83,7 +83,7 @@ int map4(CUtensorMap* out, int dtype, const void* ptr, int D, const int (&extent
 
 // fp32 rows and log-sum-exps of two pieces for each worker, and what is merged from which
 size_t workspace_bytes(int D, int workers) {
-    return size_t(2) * workers * fa::kBlk * ((D > 64 ? 128 : 64) + 1) * sizeof(float) + workers * (sizeof(int4) + 2 * sizeof(int));
+    return size_t(2) * workers * fa::kBlk * ((D > 64 ? 128 : 64) + 1) * sizeof(float) + workers * sizeof(int4);
 }
 
 }  // namespace
@@ -136,10 +136,10 @@ int fa_paged_fwd(const fa_paged_cache* cache, int32_t T, int32_t H, const int32_
     p.part_o = static_cast<float*>(workspace);
     p.part_lse = p.part_o + size_t(2) * sms * fa::kBlk * (cache->D > 64 ? 128 : 64);
     p.merge = reinterpret_cast<int4*>(p.part_lse + size_t(2) * sms * fa::kBlk);
-    p.merge_slots = reinterpret_cast<int*>(p.merge + sms);
     p.H = H;
     p.G = G;
     p.tokens = fa::kBlk / G;
+    p.narrow = 32 / G;
     p.fill = fill ? 1 : 0;
     p.scale_log2 = sm_scale * fa::kScoreLog2e;
     p.score = fa::make_score_args(sc->softcap, sc->slopes, sc->prefix != nullptr, sm_scale);
@@ -149,11 +149,13 @@ int fa_paged_fwd(const fa_paged_cache* cache, int32_t T, int32_t H, const int32_
     const int box_rows = cache->page_size < fa::kBlk ? cache->page_size : fa::kBlk;
     CUtensorMap tq, tk, tv;
     if ((rc = map4(&tq, cache->dtype, q->ptr, cache->D, {G, cache->Hk, T}, {q->stride[1], q->stride[1] * G, q->stride[0]}, {G, 1, p.tokens}))) return rc;
+    CUtensorMap tn;  // of the rows of 32 / G tokens
+    if ((rc = map4(&tn, cache->dtype, q->ptr, cache->D, {G, cache->Hk, T}, {q->stride[1], q->stride[1] * G, q->stride[0]}, {G, 1, p.narrow > 0 ? p.narrow : p.tokens}))) return rc;
     if ((rc = map4(&tk, cache->dtype, cache->k, cache->D, {cache->Hk, cache->page_size, cache->pages},
                    {cache->k_stride[2], cache->k_stride[1], cache->k_stride[0]}, {1, box_rows, 1}))) return rc;
     if ((rc = map4(&tv, cache->dtype, cache->v, cache->D, {cache->Hk, cache->page_size, cache->pages},
                    {cache->v_stride[2], cache->v_stride[1], cache->v_stride[0]}, {1, box_rows, 1}))) return rc;
-    return fa::launch_paged_fwd(cache->dtype == FA_BF16, tq, tk, tv, p, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+    return fa::launch_paged_fwd(cache->dtype == FA_BF16, tq, tn, tk, tv, p, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
 int fa_debug_paged_pieces(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t capacity, const int32_t* lens, const int32_t* starts, const int32_t* prefix,
@@ -201,13 +203,9 @@ int fa_debug_paged_pieces(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t c
         fa::paged_stretch(p, plan, w, [&](const fa::PagedWalk& k, int tiles, int lo, int hi, int part) {
             put(w, k.b, k.hk, k.tile, lo, hi, tiles, part);
             if (first && fa::paged_first_cut(plan, w, k)) {
-                int slots[2048], pieces = 0;
-                bool last = false;
-                for (int i = 0; !last; ++i) {
-                    const int slot = fa::paged_piece(p, plan, w, k, i, last);
-                    if (slot >= 0) slots[pieces++] = slot;
-                }
-                for (int i = 0; pieces > 1 && i < pieces; ++i) put(-1, k.b, k.hk, k.tile, 0, 0, 0, slots[i]);
+                int from;
+                const int pieces = fa::paged_pieces(p, plan, w, k, from);
+                for (int i = 0; pieces > 1 && i < pieces; ++i) put(-1, k.b, k.hk, k.tile, 0, 0, 0, 2 * (from + i) + (i == 0));
             }
             first = false;
             return true;

@@ -41,9 +41,9 @@ struct PagedSmem {
     static constexpr int off_info = off_ml + NQ * 4 * kBlk * 4;  // int32 [NQ][16]: see I_*
     static constexpr int off_plan = off_info + NQ * 64;
     static constexpr int off_bar = off_plan + int(sizeof(PagedPlan));
-    // item_full[NQ] item_empty[NQ] q_full[NQ] ml_full[NQ] k_full[NS] k_empty[NS] v_full[NS] v_empty[NS]
+    // item_full[NQ] item_empty[NQ] q_full[NQ] ml_full[NQ] staged k_full[NS] k_empty[NS] v_full[NS] v_empty[NS]
     // s_full[4] s_free[2] p_full[NP] pv_done[NP] o_full[2] o_free[2]
-    static constexpr int n_bar = 4 * NQ + 4 * NS + 6 + 2 * NP + 4;
+    static constexpr int n_bar = 4 * NQ + 1 + 4 * NS + 6 + 2 * NP + 4;
     static constexpr int off_misc = off_bar + n_bar * 8;  // tmem slot, abort flag
     static constexpr int total = off_misc + 16;
     static_assert(off_plan % 8 == 0 && off_bar % 8 == 0, "alignment");
@@ -57,8 +57,8 @@ enum : int { I_TILES = 0, I_LO, I_MORE, I_HEAD, I_ROW, I_TOKENS, I_POS, I_LEN, I
 
 template <int D, bool BF16, int KIND>
 __global__ void __launch_bounds__(kFwdThreads, 1)
-paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                 const PagedParams p) {
+paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmN, const __grid_constant__ CUtensorMap tmK,
+                 const __grid_constant__ CUtensorMap tmV, const PagedParams p) {
     using S = PagedSmem<D>;
     constexpr bool SCORED = KIND != SCORE_PLAIN;
     constexpr int NS = S::NS, NQ = S::NQ, NP = S::NP;
@@ -71,7 +71,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     PagedPlan& plan = *reinterpret_cast<PagedPlan*>(smem + S::off_plan);
     const uint32_t bar0 = sbase + S::off_bar;
     auto BAR = [&](int i) { return bar0 + 8u * uint32_t(i); };
-    constexpr int B_ITEMFULL = 0, B_ITEMEMPTY = NQ, B_QFULL = 2 * NQ, B_MLFULL = 3 * NQ, B_KFULL = 4 * NQ,
+    constexpr int B_ITEMFULL = 0, B_ITEMEMPTY = NQ, B_QFULL = 2 * NQ, B_MLFULL = 3 * NQ, B_STAGED = 4 * NQ, B_KFULL = 4 * NQ + 1,
                   B_KEMPTY = B_KFULL + NS, B_VFULL = B_KEMPTY + NS, B_VEMPTY = B_VFULL + NS, B_SFULL = B_VEMPTY + NS,
                   B_SFREE = B_SFULL + 4, B_PFULL = B_SFREE + 2, B_PVDONE = B_PFULL + NP, B_OFULL = B_PVDONE + NP, B_OFREE = B_OFULL + 2;
     static_assert(B_OFREE + 2 == S::n_bar, "barriers");
@@ -90,6 +90,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             mbar_init(BAR(B_VFULL + s), 1);
             mbar_init(BAR(B_VEMPTY + s), 1);
         }
+        mbar_init(BAR(B_STAGED), 4);
         for (int s = 0; s < 4; ++s) mbar_init(BAR(B_SFULL + s), 1);
         for (int s = 0; s < NP; ++s) {
             mbar_init(BAR(B_PFULL + s), 4);  // here and below: one arrival a warp
@@ -160,14 +161,16 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         } else if (warp == 14) {
             // ------------------------------ item scheduler, and loads of Q and K ------------------------------
             tma_prefetch_desc(&tmQ);
+            tma_prefetch_desc(&tmN);
             tma_prefetch_desc(&tmK);
             bool ok = true, first = true;
-            int k = 0, gk = 0, pieces = 0;
+            int k = 0, gk = 0;
             int4 merge = make_int4(0, 0, 0, 0);
             if (!idle) {
                 paged_stretch(p, plan, worker, [&](const PagedWalk& walk, int, int lo, int hi, int part) {
                     const int s = k % NQ, use = k / NQ;
                     const int T = uniform(hi - lo), tile0 = uniform(lo), hk = uniform(walk.hk), len = uniform(walk.s.len), tok0 = uniform(walk.s.start + walk.tile * p.tokens);
+                    const int tokens = uniform(min(p.tokens, walk.s.n - walk.tile * p.tokens));
                     const int32_t* const row_of_table = p.table + walk.b * p.table_stride;
                     int pages = T > 0 ? pages_of(row_of_table, tile0, len) : 0;
                     if (use > 0) ok = mbar_wait_warp(BAR(B_ITEMEMPTY + s), (use - 1) & 1, ab, ST_WAIT_TIMEOUT + 11);
@@ -179,7 +182,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         it[I_MORE] = 1;
                         it[I_HEAD] = hk;
                         it[I_ROW] = tok0;
-                        it[I_TOKENS] = min(p.tokens, walk.s.n - walk.tile * p.tokens);
+                        it[I_TOKENS] = tokens;
                         it[I_POS] = walk.s.base + walk.tile * p.tokens;
                         it[I_LEN] = len;
                         it[I_FRONT] = walk.s.front;
@@ -189,8 +192,14 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
                     __syncwarp();
                     // (an item's slot is given away when its O has left, so that Q has been read, too)
-                    mbar_expect_tx_elect(BAR(B_QFULL + s), uint32_t(p.tokens * p.G) * 128u * S::NBOX);
-                    for (int x = 0; x < S::NBOX; ++x) tma_load_4d_elect(sQ(s) + x * S::BOX, &tmQ, BAR(B_QFULL + s), x * 64, 0, hk, tok0);
+                    if (tokens <= p.narrow) {  // four times the same rows
+                        mbar_expect_tx_elect(BAR(B_QFULL + s), uint32_t(p.narrow * p.G) * 512u * S::NBOX);
+                        for (int i = 0; i < 4 * S::NBOX; ++i)
+                            tma_load_4d_elect(sQ(s) + (i >> 2) * S::BOX + (i & 3) * 4096, &tmN, BAR(B_QFULL + s), (i >> 2) * 64, 0, hk, tok0);
+                    } else {
+                        mbar_expect_tx_elect(BAR(B_QFULL + s), uint32_t(p.tokens * p.G) * 128u * S::NBOX);
+                        for (int x = 0; x < S::NBOX; ++x) tma_load_4d_elect(sQ(s) + x * S::BOX, &tmQ, BAR(B_QFULL + s), x * 64, 0, hk, tok0);
+                    }
                     for (int t = 0; t < T; ++t, ++gk) {
                         const int st = gk % NS, ug = gk / NS, own = pages;
                         if (t + 1 < T) pages = pages_of(row_of_table, tile0 + t + 1, len);
@@ -201,16 +210,9 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     ++k;
                     if (first && paged_first_cut(plan, worker, walk)) {
                         // the item that this worker's stretch begins within is merged from its pieces by the second kernel
-                        for (int i0 = 0;; i0 += 32) {
-                            bool last;
-                            const int slot = paged_piece(p, plan, worker, walk, i0 + lane, last);
-                            const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
-                            // (a piece behind the last one has no tiles)
-                            if (slot >= 0) p.merge_slots[2 * worker + pieces + __popc(there & ((1u << lane) - 1u))] = slot;
-                            pieces += __popc(there);
-                            if (__any_sync(0xffffffffu, last)) break;
-                        }
-                        merge = make_int4(pieces, tok0, min(p.tokens, walk.s.n - walk.tile * p.tokens), hk);
+                        int from;
+                        const int pieces = paged_pieces(p, plan, worker, walk, from);
+                        merge = make_int4(pieces, tok0, tokens | hk << 8, from);
                     }
                     first = false;
                     return true;
@@ -323,7 +325,10 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const int r = tid & 127;
         const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
         const float c = SCORED ? 1.f : p.scale_log2;
-        const int tok = r / p.G, g_row = r - tok * p.G;
+        const int tok_wide = r / p.G, tok_narrow = lane / p.G;
+        // of a narrow item's sums: this thread adds up four columns of row r / 4
+        const int row_sum = r >> 2, tok_sum = row_sum / p.G;
+        int staged = 0;  // passes through the staging barrier
         bool alive = !aborted;
         if (alive && p.fill && p.starts) {
             // rows in front of the first sequence and behind the last one
@@ -341,9 +346,11 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             alive = mbar_wait_warp(BAR(B_ITEMFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 12);
             if (!alive) break;
             volatile int* it = info + 16 * s;
-            const int T = it[I_TILES], part = it[I_PART], hk = it[I_HEAD], row = it[I_ROW] + tok;
+            const int T = it[I_TILES], part = it[I_PART], hk = it[I_HEAD], tokens = it[I_TOKENS];
             if (it[I_MORE] < 0) break;
-            const bool valid = tok < it[I_TOKENS];
+            const bool narrow = tokens <= p.narrow;
+            const int tok = narrow ? tok_narrow : tok_wide, g_row = narrow ? lane - tok * p.G : r - tok * p.G, row = it[I_ROW] + tok;
+            const bool valid = tok < tokens;
             {
                 const int64_t row_of_table = it[I_SEQ] * p.table_stride;
                 const int last = min((it[I_LO] + T) * kBlk, it[I_LEN]) - 1;
@@ -364,20 +371,34 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             const float* ml = reinterpret_cast<const float*>(smem + S::off_ml) + s * (4 * kBlk);  // [2 groups][m, l][128]
             const int even = we * (2 * kBlk), odd = 2 * kBlk - even;
             const float m0 = ml[even + r], l0 = ml[even + kBlk + r], m1 = ml[odd + r], l1 = ml[odd + kBlk + r];
-            const float mt = fmaxf(m0, m1);
+            float mt = fmaxf(m0, m1);
+            if (narrow) {  // over the four warps' chains of the row
+                for (int q = 0; q < 4; ++q) mt = fmaxf(mt, fmaxf(ml[even + 32 * q + lane], ml[odd + 32 * q + lane]));
+            }
             const float a0 = (m0 == -INFINITY) ? 0.f : fast_exp2((m0 - mt) * c);
             const float a1 = (m1 == -INFINITY) ? 0.f : fast_exp2((m1 - mt) * c);
-            const float lt = l0 * a0 + l1 * a1;
+            float lt = l0 * a0 + l1 * a1;
+            if (narrow) {
+                lt = 0.f;
+                for (int q = 0; q < 4; ++q) {
+                    const float me = ml[even + 32 * q + lane], mo = ml[odd + 32 * q + lane];
+                    lt += (me == -INFINITY ? 0.f : ml[even + kBlk + 32 * q + lane] * fast_exp2((me - mt) * c)) +
+                          (mo == -INFINITY ? 0.f : ml[odd + kBlk + 32 * q + lane] * fast_exp2((mo - mt) * c));
+                }
+            }
             const float inv = (lt > 0.f) ? 1.0f / lt : 0.f;
             const float f0 = a0 * inv, f1 = a1 * inv;
             // a chain in which the row had no key takes no part, whatever the values behind its mask are
             const bool use0 = (T > 0) && (f0 != 0.f), use1 = (T > 1) && (f1 != 0.f);
             const bool both = __all_sync(0xffffffffu, !valid || (use0 && use1));
             const bool store = valid && misc[1] == 0;
-            if (part >= 0 && store)  // (a piece that went NaN says so: -inf would pass for a piece without keys)
+            if (part >= 0 && store && (!narrow || warp == 8))  // (a piece that went NaN says so: -inf would pass for a piece without keys)
                 p.part_lse[int64_t(part) * kBlk + r] = lt > 0.f ? fmaf(mt, c, log2f(lt)) : lt == lt ? -INFINITY : lt;
-            float* const rows_of_part = p.part_o + (int64_t(part) * kBlk + r) * D;
-            uint16_t* const row_out = out + int64_t(row) * p.out_t + int64_t(hk * p.G + g_row) * p.out_h;
+            float* const rows_of_part = p.part_o + (int64_t(part) * kBlk + (narrow ? row_sum : r)) * D;
+            uint16_t* const row_out = narrow ? out + int64_t(it[I_ROW] + tok_sum) * p.out_t + int64_t(hk * p.G + row_sum - tok_sum * p.G) * p.out_h
+                                             : out + int64_t(row) * p.out_t + int64_t(hk * p.G + g_row) * p.out_h;
+            const bool store_sum = tok_sum < tokens && misc[1] == 0;
+            float* const stage = reinterpret_cast<float*>(smem + S::off_q + s * S::TILE);  // (Q has been read) [2][4 warps][32 rows][16]
             const uint32_t tO0 = tmem + lane_base + uint32_t(S::tmem_o + we * D), tO1 = tmem + lane_base + uint32_t(S::tmem_o + (we ^ 1) * D);
 #pragma unroll 1
             for (int q = 0; q < D / 16; ++q) {
@@ -403,7 +424,27 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         x0[y] = __float_as_uint(v);
                     }
                 }
-                if (store && 16 * q < p.D) {
+                if (narrow) {
+                    // the warps' sums of a row, 16 columns at a time, through one of two buffers
+                    float* const buf = stage + (q & 1) * 2048;
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        *reinterpret_cast<uint4*>(buf + (warp & 3) * 512 + lane * 16 + 4 * ((y + (lane >> 1)) & 3)) = make_uint4(x0[4 * y], x0[4 * y + 1], x0[4 * y + 2], x0[4 * y + 3]);
+                    mbar_arrive_warp(BAR(B_STAGED), lane);
+                    alive = mbar_wait_warp(BAR(B_STAGED), staged++ & 1, ab, ST_WAIT_TIMEOUT + 18);
+                    if (!alive) break;
+                    if (store_sum && 16 * q < p.D) {
+                        const int y = r & 3;
+                        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const float4 x = *reinterpret_cast<const float4*>(buf + u * 512 + row_sum * 16 + 4 * ((y + (row_sum >> 1)) & 3));
+                            v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+                        }
+                        if (part >= 0) *reinterpret_cast<float4*>(rows_of_part + 16 * q + 4 * y) = make_float4(v[0], v[1], v[2], v[3]);
+                        else *reinterpret_cast<uint2*>(row_out + 16 * q + 4 * y) = make_uint2(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]));
+                    }
+                } else if (store && 16 * q < p.D) {
                     if (part >= 0) {
 #pragma unroll
                         for (int y = 0; y < 4; ++y)
@@ -416,6 +457,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
                 }
             }
+            if (!alive) break;
+            if (narrow) fence_proxy_async();  // the slot may take another item's Q
             G += T;
             n0 += (we ? T > 1 : T > 0) ? 1 : 0;
             n1 += (we ? T > 0 : T > 1) ? 1 : 0;
@@ -430,7 +473,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
         const float c = SCORED ? 1.f : p.scale_log2;
         const uint32_t tO = tmem + lane_base + uint32_t(S::tmem_o + w * D);
-        const int tok = r / p.G, g_row = r - tok * p.G;
+        const int tok_wide = r / p.G, tok_narrow = lane / p.G;
         bool alive = !aborted;
         // Rows of V behind the sequence's end hold what was in the page, or in the stage: zeros, before P*V(g) is issued. A quarter of them a warp.
         auto zero_behind = [&](int g, int real) {
@@ -441,6 +484,18 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             fence_proxy_async();
             return true;
         };
+        auto rescale = [&](float alpha) {
+#pragma unroll 1
+            for (int q = 0; q < D / 16; ++q) {
+                uint32_t orr[16];
+                tmem_ld16(tO + uint32_t(q) * 16u, orr);
+                tc_wait_ld();
+#pragma unroll
+                for (int x = 0; x < 16; ++x) orr[x] = __float_as_uint(__uint_as_float(orr[x]) * alpha);
+                tmem_st16(tO + uint32_t(q) * 16u, orr);
+            }
+            tc_wait_st();
+        };
         int G = 0;  // tiles of all earlier items
         for (int k = 0; alive; ++k) {
             const int s = k % NQ, use = k / NQ;
@@ -450,7 +505,10 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             const int T = it[I_TILES], lo = it[I_LO];
             if (it[I_MORE] < 0) break;
             const int pos0 = it[I_POS], len = it[I_LEN], front = it[I_FRONT];
-            const bool valid = tok < it[I_TOKENS];
+            const int tokens = it[I_TOKENS];
+            const bool narrow = tokens <= p.narrow;
+            const int tok = narrow ? tok_narrow : tok_wide, g_row = narrow ? lane - tok * p.G : r - tok * p.G;
+            const bool valid = tok < tokens;
             const bool active = __any_sync(0xffffffffu, valid);  // does this warp hold a query at all?
             const int pos = pos0 + tok;
             const int last = min(max(pos, front - 1), len - 1);                // the last key that this row sees
@@ -480,6 +538,77 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     if (len - k0 < kBlk) alive = zero_behind(g, len - k0);
                     if (!alive) break;
                     mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
+                    continue;
+                }
+                if (narrow) {
+                    // The tile's rows are the same 32 four times over, and this warp has 32 keys of each (its P of the others is 0): a chain of its own,
+                    // which the epilogue merges with those of the other warps.
+                    const int quarter = warp & 3, kq = k0 + 32 * quarter;
+                    uint32_t sq[32];
+                    tmem_ld32(tS + uint32_t(quarter) * 32u, sq);
+                    tc_wait_ld();
+                    if (S::POWN) {
+                        tc_fence_before();
+                        mbar_arrive_warp(BAR(B_SFREE + w), lane);
+                    }
+                    float* v = reinterpret_cast<float*>(sq);
+                    if constexpr (SCORED) {
+                        if (len - kq < 32) {
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) v[x] = x < len - kq ? v[x] : 0.f;
+                        }
+                        const Bias bias(slope, front == 0, pos0 - (kq + 31), pos0 + 31 - kq);
+                        score_row<KIND, 32>(v, p.score, bias, p.scale_log2, pos - kq, valid);
+                    }
+                    if (kq + 31 > all_see) {
+                        const uint32_t keep = first_bits(last - kq + 1);
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) v[x] = (keep & (1u << x)) ? v[x] : -INFINITY;
+                    }
+                    float mx[4];
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) mx[a] = max3(v[a], v[4 + a], v[8 + a]);
+#pragma unroll
+                    for (int x = 12; x < 28; x += 8) {
+#pragma unroll
+                        for (int a = 0; a < 4; ++a) mx[a] = max3(mx[a], v[x + a], v[x + 4 + a]);
+                    }
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) mx[a] = fmaxf(mx[a], v[28 + a]);
+                    float m_new = fmaxf(m_run, fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]));
+                    const bool need = (m_new - m_run) * c > 8.0f;
+                    if (!need) m_new = m_run;
+                    const bool scale_o = __any_sync(0xffffffffu, need) && t > t0;
+                    if (S::POWN || scale_o) {  // P*V of the group's tile before has read its P and added to O
+                        alive = pv_before();
+                        if (!alive) break;
+                        tc_fence_after();
+                    }
+                    const float alpha = need ? fast_exp2((m_run - m_new) * c) : 1.0f;
+                    l_run *= alpha;
+                    if (scale_o) rescale(alpha);
+                    m_run = m_new;
+                    const float mneg = (m_run == -INFINITY) ? 0.f : -m_run * c;
+                    float l4[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int x = 0; x < 32; x += 2) {
+                        const float p0 = fast_exp2(fmaf(v[x], c, mneg)), p1 = fast_exp2(fmaf(v[x + 1], c, mneg));
+                        l4[x & 2] += p0;
+                        l4[(x & 2) + 1] += p1;
+                        pk[x / 2] = pack2<BF16>(p0, p1);
+                    }
+                    uint32_t zero[16] = {};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (q != quarter) tmem_st16(tP + uint32_t(q) * 16u, zero);
+                    tmem_st16(tP + uint32_t(quarter) * 16u, pk);
+                    tc_wait_st();
+                    if (len - k0 < kBlk) alive = zero_behind(g, len - k0);
+                    tc_fence_before();
+                    mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
+                    if (!alive) break;
+                    l_run += (l4[0] + l4[1]) + (l4[2] + l4[3]);
                     continue;
                 }
                 uint32_t sr[128];
@@ -540,16 +669,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                             if (!alive) break;
                             tc_fence_after();
                         }
-#pragma unroll 1
-                        for (int q = 0; q < D / 16; ++q) {
-                            uint32_t orr[16];
-                            tmem_ld16(tO + uint32_t(q) * 16u, orr);
-                            tc_wait_ld();
-#pragma unroll
-                            for (int x = 0; x < 16; ++x) orr[x] = __float_as_uint(__uint_as_float(orr[x]) * alpha);
-                            tmem_st16(tO + uint32_t(q) * 16u, orr);
-                        }
-                        tc_wait_st();
+                        rescale(alpha);
                     }
                 }
                 m_run = m_new;
@@ -604,7 +724,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 }
 
 // Merges the pieces of the items that a cut went through: O = sum_s w_s O_s with w_s = 2^(lse_s - lse). The blocks (w, 0 .. 3) look after the item that
-// the cut before worker w goes through first, each after 32 of its rows; the attention kernel has left a list of its pieces. A piece whose lse is NaN or +inf makes the row its own, as in fwd_combine_kernel. All sums in fp32, in an order that the number of rows
+// the cut before worker w goes through first, each after 32 of its rows; the attention kernel has left word of its pieces. A piece whose lse is NaN or +inf makes the row its own, as in fwd_combine_kernel. All sums in fp32, in an order that the number of rows
 // and pieces gives. Bound by latency: a warp has four rows, whose loads are in flight together, and where there are few rows (a decoded token's
 // heads) several warps share the pieces.
 constexpr int kCombineThreads = 256, kCombineRows = 4;
@@ -617,8 +737,8 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const Pa
     const int w = int(blockIdx.x), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool failed = status_is_fatal(*reinterpret_cast<volatile int*>(p.status));
     const int4 merge = p.merge[w];
-    const int* const slots = p.merge_slots + 2 * w;
-    const int pieces = merge.x, rows = merge.z * p.G - int(blockIdx.y) * kWarps * kCombineRows, row0 = int(blockIdx.y) * kWarps * kCombineRows;
+    const int row0 = int(blockIdx.y) * kWarps * kCombineRows, pieces = merge.x, rows = (merge.z & 255) * p.G - row0, hk = merge.z >> 8;
+    auto slot = [&](int s) { return 2 * (merge.w + s) + (s == 0 ? 1 : 0); };
     if (failed || pieces < 2 || rows <= 0) return;
     const int groups = min(cdiv(rows, kCombineRows), kWarps), subs = kWarps / groups;
     const int sub = warp / groups, r0 = (warp - sub * groups) * kCombineRows;  // (of this block's rows)
@@ -630,7 +750,7 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const Pa
         for (int s = lane; s < pieces; s += 32) {
 #pragma unroll
             for (int i = 0; i < kCombineRows; ++i) {
-                const float lse = r0 + i < rows ? p.part_lse[int64_t(slots[s]) * kBlk + row0 + r0 + i] : -INFINITY;
+                const float lse = r0 + i < rows ? p.part_lse[int64_t(slot(s)) * kBlk + row0 + r0 + i] : -INFINITY;
                 spoilt[i] |= !(lse < INFINITY);
                 top[i] = fmaxf(top[i], lse);
             }
@@ -646,7 +766,7 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const Pa
             float v[kBatch][kCombineRows][kOwn], lse[kBatch][kCombineRows];
 #pragma unroll
             for (int s = 0; s < kBatch; ++s) {
-                const int64_t at = int64_t(slots[min(s0 + s * subs, pieces - 1)]) * kBlk;
+                const int64_t at = int64_t(slot(min(s0 + s * subs, pieces - 1))) * kBlk;
 #pragma unroll
                 for (int i = 0; i < kCombineRows; ++i) {
                     const int64_t row = at + row0 + min(r0 + i, rows - 1);
@@ -703,7 +823,7 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const Pa
         if (r0 + i >= rows) return;
         const int r = row0 + r0 + i, tok = r / p.G, g = r - tok * p.G;
         const float inv = total[i] > 0.f ? 1.f / total[i] : 0.f;
-        uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(merge.y + tok) * p.out_t + int64_t(merge.w * p.G + g) * p.out_h + lane * kOwn;
+        uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(merge.y + tok) * p.out_t + int64_t(hk * p.G + g) * p.out_h + lane * kOwn;
         if constexpr (kOwn == 4)
             *reinterpret_cast<uint2*>(out) = make_uint2(pack2<BF16>(acc[i][0] * inv, acc[i][1] * inv), pack2<BF16>(acc[i][2] * inv, acc[i][3] * inv));
         else
@@ -713,21 +833,21 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const Pa
 
 // ---- host launchers (called from paged.cu) ----------------------------------------------
 template <int D, bool BF16, int KIND>
-static cudaError_t launch_paged_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {
+static cudaError_t launch_paged_t(const CUtensorMap& tq, const CUtensorMap& tn, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {
     auto kern = paged_fwd_kernel<D, BF16, KIND>;
     constexpr int smem = PagedSmem<D>::total;
     static SmemAllowed allowed;
     cudaError_t e = allow_smem(kern, smem, allowed);
     if (e != cudaSuccess) return e;
-    e = launch_overlapping(kern, dim3(workers), kFwdThreads, smem, stream, tq, tk, tv, p);
+    e = launch_overlapping(kern, dim3(workers), kFwdThreads, smem, stream, tq, tn, tk, tv, p);
     if (e != cudaSuccess) return e;
     return launch_overlapping(paged_combine_kernel<D, BF16>, dim3(workers, kBlk / (kCombineThreads / 32 * kCombineRows)), kCombineThreads, 0, stream, p);
 }
 
-cudaError_t launch_paged_fwd(bool bf16, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {
+cudaError_t launch_paged_fwd(bool bf16, const CUtensorMap& tq, const CUtensorMap& tn, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {
     auto pick = [&](auto d, auto kind) {
         constexpr int kD = decltype(d)::value, kKind = decltype(kind)::value;
-        return bf16 ? launch_paged_t<kD, true, kKind>(tq, tk, tv, p, workers, stream) : launch_paged_t<kD, false, kKind>(tq, tk, tv, p, workers, stream);
+        return bf16 ? launch_paged_t<kD, true, kKind>(tq, tn, tk, tv, p, workers, stream) : launch_paged_t<kD, false, kKind>(tq, tn, tk, tv, p, workers, stream);
     };
     using std::integral_constant;
     auto of = [&](auto d) {

@@ -263,12 +263,19 @@ __host__ __device__ __forceinline__ bool paged_first_cut(const PagedPlan& plan, 
     return w > 0 && walk.s.tiles > 0 && walk.at < paged_cut(plan, w) && (w == 1 || walk.at >= paged_cut(plan, w - 1));
 }
 
-// Piece i of the item at `walk`, which the cut before worker w goes through first: worker w - 1 + i's. Its slot, or -1 if it has no tiles. There are none
-// behind the first i with `last`.
-__host__ __device__ __forceinline__ int paged_piece(const PagedParams& p, const PagedPlan& plan, int w, const PagedWalk& walk, int i, bool& last) {
-    const int lo = i == 0 ? 0 : walk.key_tile_at(p, plan, paged_cut(plan, w + i - 1)), hi = walk.key_tile_at(p, plan, paged_cut(plan, w + i));
-    last = hi >= walk.key_tiles(p);
-    return hi > lo ? 2 * (w - 1 + i) + (lo == 0 ? 1 : 0) : -1;
+// The pieces of the item at `walk`, which the cut before worker w goes through first: those of `count` workers from `from` on. (The first one's is left out where
+// the cut falls into the item's fixed cost, the last one's where it falls into the last tile; a stretch that lies within the item has tiles, for it is
+// longer than the cost and a tile.) The first piece's slot is 2 * from + 1, the others' are 2 * (from + i).
+__host__ __device__ __forceinline__ int paged_pieces(const PagedParams& p, const PagedPlan& plan, int w, const PagedWalk& walk, int& from) {
+    static_assert((1 << kPagedLog2Piece) > kPagedItemCost + 2 * kBlk, "every stretch within an item has tiles");
+    const int n = walk.key_tiles(p);
+    from = walk.key_tile_at(p, plan, paged_cut(plan, w)) > 0 ? w - 1 : w;
+    int v = w;  // the last worker with tiles of it
+    // the cuts lie a stretch apart: the last one before the item's last tile ends
+    const long long end = walk.end(p, plan);
+    v += int(paged_divide(end - 1 - paged_cut(plan, w), plan.stretch));
+    if (walk.key_tile_at(p, plan, paged_cut(plan, v)) >= n) --v;
+    return v - from + 1;
 }
 
 }  // namespace fa

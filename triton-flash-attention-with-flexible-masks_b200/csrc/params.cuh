@@ -104,10 +104,11 @@ struct PagedParams {
     int64_t out_t, out_h;   // element strides
     float* part_o;          // [2 * workers, 128, 64 or 128] fp32 rows of the pieces
     float* part_lse;        // [2 * workers, 128]
-    int4* merge;            // [workers] {pieces of the item that the cut before a worker goes through first, or fewer than 2; its first row; tokens; kv head}
-    int* merge_slots;       // [2 * workers] the pieces' slots, from place 2 * worker on
+    int4* merge;            // [workers] {pieces of the item that the cut before a worker goes through first, or fewer than 2; its first row; tokens
+                            // and 256 * kv head; worker of the first piece}
     int B, T, H, Hk, G, D;
     int tokens;             // of a tile: 128 / G
+    int narrow;             // tokens that fit 32 rows of a tile: 32 / G
     int page, log2_page, n_pages;
     int capacity;           // tokens that the table has room for
     int fill;               // rows of no sequence are set to 0
