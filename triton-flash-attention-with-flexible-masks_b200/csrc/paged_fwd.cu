@@ -123,11 +123,10 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         // an earlier launch ran into a time-out that the host has not yet cleared: the whole of the output becomes NaN, shared out by rows of a head
         for (int64_t i = blockIdx.x; i < int64_t(p.T) * p.H; i += gridDim.x)
             for (int d = tid; d < p.D; d += kFwdThreads) out[i / p.H * p.out_t + i % p.H * p.out_h + d] = 0xffffu;
-    } else {
+    } else if (p.B > kPagedWarpPlan) {
         paged_plan<kFwdThreads>(p, plan, int(gridDim.x));
     }
     const int worker = int(blockIdx.x);
-    const bool idle = aborted || worker >= plan.workers;
 
     auto sQ = [&](int s) { return sbase + S::off_q + uint32_t(s) * S::TILE; };
     auto sK = [&](int s) { return sbase + S::off_k + uint32_t(s) * S::TILE; };
@@ -166,7 +165,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             bool ok = true, first = true;
             int k = 0, gk = 0;
             int4 merge = make_int4(0, 0, 0, 0);
-            if (!idle) {
+            if (p.B <= kPagedWarpPlan) paged_plan_warp(p, plan, int(gridDim.x));
+            if (worker < plan.workers) {
                 paged_stretch(p, plan, worker, [&](const PagedWalk& walk, int, int lo, int hi, int part) {
                     const int s = k % NQ, use = k / NQ;
                     const int T = uniform(hi - lo), tile0 = uniform(lo), hk = uniform(walk.hk), len = uniform(walk.s.len), tok0 = uniform(walk.s.start + walk.tile * p.tokens);
@@ -730,9 +730,9 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 constexpr int kCombineThreads = 256, kCombineRows = 4;
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const PagedParams p) {
+__global__ void __launch_bounds__(kCombineThreads, 2) paged_combine_kernel(const PagedParams p) {
     constexpr int kOwn = D / 32, kBatch = 4, kWarps = kCombineThreads / 32;  // columns of a lane; pieces in flight
-    __shared__ float sums[kWarps][kCombineRows][D + 1];
+    __shared__ float sums[kWarps][kCombineRows][D + 2];
     follow_stream();
     const int w = int(blockIdx.x), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool failed = status_is_fatal(*reinterpret_cast<volatile int*>(p.status));
@@ -742,25 +742,13 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const Pa
     if (failed || pieces < 2 || rows <= 0) return;
     const int groups = min(cdiv(rows, kCombineRows), kWarps), subs = kWarps / groups;
     const int sub = warp / groups, r0 = (warp - sub * groups) * kCombineRows;  // (of this block's rows)
+    // A warp's own pieces first: their greatest lse, and the sums relative to it. (An empty piece has an lse of -inf.)
     float top[kCombineRows], acc[kCombineRows][kOwn] = {}, total[kCombineRows] = {};
+#pragma unroll
+    for (int i = 0; i < kCombineRows; ++i) top[i] = -INFINITY;
+    // A spoilt row's "greatest" is +inf: of such pieces each counts once, and all others not at all.
+    auto weight = [](float lse, float most) { return lse < INFINITY ? (lse == -INFINITY ? 0.f : fast_exp2(lse - most)) : 1.f; };
     if (sub < subs) {
-        bool spoilt[kCombineRows] = {};
-#pragma unroll
-        for (int i = 0; i < kCombineRows; ++i) top[i] = -INFINITY;
-        for (int s = lane; s < pieces; s += 32) {
-#pragma unroll
-            for (int i = 0; i < kCombineRows; ++i) {
-                const float lse = r0 + i < rows ? p.part_lse[int64_t(slot(s)) * kBlk + row0 + r0 + i] : -INFINITY;
-                spoilt[i] |= !(lse < INFINITY);
-                top[i] = fmaxf(top[i], lse);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kCombineRows; ++i) {
-            spoilt[i] = __any_sync(0xffffffffu, spoilt[i]);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
-        }
 #pragma unroll 1
         for (int s0 = sub; s0 < pieces; s0 += subs * kBatch) {
             float v[kBatch][kCombineRows][kOwn], lse[kBatch][kCombineRows];
@@ -782,11 +770,21 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const Pa
                 }
             }
 #pragma unroll
-            for (int s = 0; s < kBatch; ++s) {
-                if (s0 + s * subs >= pieces) break;
+            for (int i = 0; i < kCombineRows; ++i) {
+                float most = top[i];
 #pragma unroll
-                for (int i = 0; i < kCombineRows; ++i) {
-                    const float x = lse[s][i], wgt = spoilt[i] ? (x < INFINITY ? 0.f : 1.f) : top[i] == -INFINITY ? 0.f : fast_exp2(x - top[i]);
+                for (int s = 0; s < kBatch; ++s) {
+                    if (s0 + s * subs >= pieces) lse[s][i] = -INFINITY;
+                    most = lse[s][i] < INFINITY ? fmaxf(most, lse[s][i]) : INFINITY;
+                }
+                const float keep = top[i] == most ? 1.f : weight(top[i], most);  // (0 if nothing was there, or the row is spoilt from here on)
+                total[i] *= keep;
+#pragma unroll
+                for (int c = 0; c < kOwn; ++c) acc[i][c] = keep == 0.f ? 0.f : acc[i][c] * keep;
+                top[i] = most;
+#pragma unroll
+                for (int s = 0; s < kBatch; ++s) {
+                    const float wgt = weight(lse[s][i], most);
                     if (wgt == 0.f) continue;
                     total[i] += wgt;
 #pragma unroll
@@ -796,23 +794,34 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const Pa
         }
     }
     if (subs > 1) {  // (the same for all threads)
-        float (*mine)[D + 1] = sums[warp];
+        float (*mine)[D + 2] = sums[warp];
         if (sub > 0 && sub < subs) {
 #pragma unroll
             for (int i = 0; i < kCombineRows; ++i) {
 #pragma unroll
                 for (int c = 0; c < kOwn; ++c) mine[i][lane * kOwn + c] = acc[i][c];
-                if (lane == 0) mine[i][D] = total[i];
+                if (lane == 0) {
+                    mine[i][D] = total[i];
+                    mine[i][D + 1] = top[i];
+                }
             }
         }
         __syncthreads();
         if (sub == 0) {
-            for (int u = 1; u < subs; ++u) {
 #pragma unroll
-                for (int i = 0; i < kCombineRows; ++i) {
+            for (int i = 0; i < kCombineRows; ++i) {
+                float most = top[i];
+                for (int u = 1; u < subs; ++u) most = fmaxf(most, sums[warp + u * groups][i][D + 1]);
+                for (int u = 0; u < subs; ++u) {
+                    const float* other = sums[warp + u * groups][i];
+                    const float t = u == 0 ? top[i] : other[D + 1], wgt = t == most && t != -INFINITY ? 1.f : t < INFINITY ? weight(t, most) : 0.f;
+                    const float tt = u == 0 ? total[i] : other[D];
+                    total[i] = (u == 0 ? 0.f : total[i]) + (wgt == 0.f ? 0.f : tt * wgt);
 #pragma unroll
-                    for (int c = 0; c < kOwn; ++c) acc[i][c] += sums[warp + u * groups][i][lane * kOwn + c];
-                    total[i] += sums[warp + u * groups][i][D];
+                    for (int c = 0; c < kOwn; ++c) {
+                        const float x = u == 0 ? acc[i][c] : other[lane * kOwn + c];
+                        acc[i][c] = (u == 0 ? 0.f : acc[i][c]) + (wgt == 0.f ? 0.f : x * wgt);
+                    }
                 }
             }
         }

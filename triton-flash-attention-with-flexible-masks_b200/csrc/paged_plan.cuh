@@ -13,6 +13,7 @@
 namespace fa {
 
 constexpr int kPagedGroups = 1024;   // entries of the table of sums: a sequence each, or several
+constexpr int kPagedWarpPlan = 128;  // sequences up to which one warp makes the plan
 constexpr int kPagedItemCost = 256;  // of an item, in keys
 constexpr int kPagedLog2Piece = 10;  // a worker's stretch is at least 2 to this long
 constexpr int kPagedMergeTiles = 6;  // of the second kernel, in tiles of 128 keys
@@ -94,6 +95,45 @@ __host__ __device__ __forceinline__ void paged_share_out(PagedPlan& plan, long l
     plan.total = plan.keyed ? weight : items;
     // (a hair more than total / workers: a division in fp32 takes a fraction of one of 64 bits)
     plan.stretch = plan.keyed ? (long long)(float(weight) / float(workers) * 1.00001f) + 1 : 1;
+}
+
+// The plan of up to kPagedWarpPlan sequences, by one warp, the one that needs it: 32 entries of `sums`. (By all warps it costs a microsecond more, of which with
+// many sequences nothing is left.)
+__device__ __forceinline__ void paged_plan_warp(const PagedParams& p, PagedPlan& plan, int most_workers) {
+    const int lane = threadIdx.x & 31, group = (p.B + 31) >> 5;
+    long long w = 0, n = 0;
+    int longest = 0;
+#pragma unroll 1
+    for (int b = lane * group; b < min(p.B, (lane + 1) * group); ++b) {
+        const int len = p.lens[b];
+        const PagedSeq s = paged_seq(p, b);
+        if (len > p.capacity || len < 0) atomicCAS(p.status, 0, ST_PAGED_LENGTH);
+        w += p.Hk * paged_weight(p, s, s.tiles, true);
+        n += (long long)p.Hk * s.tiles;
+        longest = max(longest, s.tiles > 0 ? s.len : 0);
+    }
+    __syncwarp();
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    long long w_sum = w, n_sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, w_sum, o), y = __shfl_up_sync(0xffffffffu, n_sum, o);
+        if (lane >= o) {
+            w_sum += x;
+            n_sum += y;
+        }
+    }
+    PagedPlan own;
+    paged_share_out(own, __shfl_sync(0xffffffffu, w_sum, 31), __shfl_sync(0xffffffffu, n_sum, 31), longest, most_workers);
+    plan.sums[lane] = own.keyed ? w_sum - w : n_sum - n;
+    if (lane == 0) {
+        plan.total = own.total;
+        plan.stretch = own.stretch;
+        plan.workers = own.workers;
+        plan.keyed = own.keyed;
+        plan.group = group;
+    }
+    __syncwarp();
 }
 
 // All threads of the block (a multiple of 32, at most 1024, that divides 2 * kPagedGroups). Ends with a barrier.
@@ -186,7 +226,7 @@ struct PagedWalk {
         int lo = 0;  // the last entry with sums[lo] <= x
 #ifdef __CUDA_ARCH__
         static_assert(kPagedGroups == 32 * 32, "two steps of a warp");  // (whose lanes all ask for the same x)
-        lo = 32 * (31 - __clz(__ballot_sync(0xffffffffu, plan.sums[32 * (threadIdx.x & 31)] <= x)));
+        if (p.B > kPagedWarpPlan) lo = 32 * (31 - __clz(__ballot_sync(0xffffffffu, plan.sums[32 * (threadIdx.x & 31)] <= x)));
         lo += 31 - __clz(__ballot_sync(0xffffffffu, plan.sums[lo + (threadIdx.x & 31)] <= x));
 #else
         while (lo + 1 < kPagedGroups && plan.sums[lo + 1] <= x) ++lo;
