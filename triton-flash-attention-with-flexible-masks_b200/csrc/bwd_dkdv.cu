@@ -562,54 +562,41 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 } else if constexpr (SCORED) {
                     const float slope = p.score.slopes ? p.score.slopes[hk * G + cg] * kScoreLog2e : 0.f;
                     const Bias bias(slope, mk.causal && front == 0, qb0 + mk.gap - (k0 + kBlk - 1), qb0 + kBlk - 1 + mk.gap - k0);
-                    const bool beyond = KIND == SCORE_CAPPED && any_beyond<32>(pr, p.score.most);
+                    constexpr bool kCapped = (KIND & SCORE_CAPPED) != 0, kBias = (KIND & SCORE_BIAS) != 0;
+                    if constexpr (kCapped) cap_scores<32>(pr, p.score);
                     const float d = float(q0 + 2 * (lane & 3) + mk.gap - (k0 + 32 * (warp & 3) + (lane >> 2)));
                     uint32_t bits[4];
 #pragma unroll
                     for (int y = 0; y < 4; ++y) bits[y] = __shfl_sync(0xffffffffu, keep, 8 * y + (lane >> 2)) >> (2 * (lane & 3));
-                    // y is exponent + lse from here on to the place where P is made
-                    auto walk = [&](auto capped) {
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            const float2 l2 = *reinterpret_cast<const float2*>(vlse + 8 * n);
-                            uint64_t b2 = pack_f2(fmaf(bias.line, d + float(8 * n), -l2.x), fmaf(bias.line, d + float(8 * n + 1), -l2.y));
+                    for (int n = 0; n < 4; ++n) {
+                        const float2 l2 = *reinterpret_cast<const float2*>(vlse + 8 * n);
+                        uint64_t b2 = pack_f2(-l2.x, -l2.y);
+                        if constexpr (kBias) b2 = pack_f2(fmaf(bias.line, d + float(8 * n), -l2.x), fmaf(bias.line, d + float(8 * n + 1), -l2.y));
 #pragma unroll
-                            for (int y = 0; y < 4; ++y) {
-                                float* x = pr + 16 * (y >> 1) + 4 * n + 2 * (y & 1);
-                                const uint64_t s2 = pack_f2(x[0], x[1]);
-                                uint64_t v, f = 0;
-                                if constexpr (KIND == SCORE_CAPPED) {
-                                    v = capped(s2);
-                                    f = cap_slope(v, p.score);
-                                    v = add_f2(v, b2);
-                                } else {
-                                    v = fma_f2(s2, pack_f2(c, c), b2);
-                                }
-                                if (y < 3) b2 = add_f2(b2, pack_f2(-8.f * bias.line, -8.f * bias.line));
-                                float x0, x1;
-                                unpack_f2(v, x0, x1);
-                                if (bias.both) {
-                                    x0 = fmaf(bias.s, fabsf(d + float(8 * n - 8 * y)), x0);
-                                    x1 = fmaf(bias.s, fabsf(d + float(8 * n - 8 * y + 1)), x1);
-                                }
-                                x0 = fast_exp2(x0);
-                                x1 = fast_exp2(x1);
-                                if (flagged) {
-                                    x0 = (bits[y] & (1u << (8 * n))) ? x0 : 0.f;
-                                    x1 = (bits[y] & (2u << (8 * n))) ? x1 : 0.f;
-                                }
-                                pk[8 * (y >> 1) + 2 * n + (y & 1)] = pack2<BF16>(x0, x1);
-                                if constexpr (KIND == SCORE_CAPPED) {
-                                    unpack_f2(mul_f2(pack_f2(x0, x1), f), x[0], x[1]);
-                                } else {
-                                    x[0] = x0;
-                                    x[1] = x1;
-                                }
+                        for (int y = 0; y < 4; ++y) {
+                            float* x = pr + 16 * (y >> 1) + 4 * n + 2 * (y & 1);
+                            const uint64_t s2 = pack_f2(x[0], x[1]);
+                            float x0, x1;
+                            if constexpr (kCapped) unpack_f2(add_f2(s2, b2), x0, x1);
+                            else unpack_f2(fma_f2(s2, pack_f2(c, c), b2), x0, x1);
+                            if (kBias && y < 3) b2 = add_f2(b2, pack_f2(-8.f * bias.line, -8.f * bias.line));
+                            if (kBias && bias.both) {
+                                x0 = fmaf(bias.s, fabsf(d + float(8 * n - 8 * y)), x0);
+                                x1 = fmaf(bias.s, fabsf(d + float(8 * n - 8 * y + 1)), x1);
                             }
+                            x0 = fast_exp2(x0);
+                            x1 = fast_exp2(x1);
+                            if (flagged) {
+                                x0 = (bits[y] & (1u << (8 * n))) ? x0 : 0.f;
+                                x1 = (bits[y] & (2u << (8 * n))) ? x1 : 0.f;
+                            }
+                            pk[8 * (y >> 1) + 2 * n + (y & 1)] = pack2<BF16>(x0, x1);
+                            if constexpr (kCapped) unpack_f2(mul_f2(pack_f2(x0, x1), cap_slope(s2, p.score)), x0, x1);
+                            x[0] = x0;
+                            x[1] = x1;
                         }
-                    };
-                    if (beyond) walk([&](uint64_t s2) { return cap_pair(s2, p.score, true); });
-                    else walk([&](uint64_t s2) { return cap_pair(s2, p.score, false); });
+                    }
                 } else {
                     const uint64_t c2 = pack_f2(c, c);
 #pragma unroll
@@ -787,6 +774,7 @@ cudaError_t launch_bwd_dkdv(int D, bool bf16, const CUtensorMap& tq, const CUten
     };
     using std::integral_constant;
     auto of = [&](auto d) {
+        if (p.score.kind == SCORE_CAPPED_BIAS) return pick(d, integral_constant<int, SCORE_CAPPED_BIAS>{});
         if (p.score.kind == SCORE_CAPPED) return pick(d, integral_constant<int, SCORE_CAPPED>{});
         if (p.score.kind == SCORE_BIAS) return pick(d, integral_constant<int, SCORE_BIAS>{});
         return pick(d, integral_constant<int, SCORE_PLAIN>{});

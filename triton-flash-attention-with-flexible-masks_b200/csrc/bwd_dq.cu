@@ -482,45 +482,33 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                     }
                     if constexpr (SCORED) {
                         const Bias bias(slope, mk.causal && front == 0, q0 + mk.gap - (kb0 + kBlk - 1), q0 + kBlk - 1 + mk.gap - kb0);
-                        const bool beyond = KIND == SCORE_CAPPED && any_beyond<32>(pr + 32 * q, p.score.most);
+                        constexpr bool kCapped = (KIND & SCORE_CAPPED) != 0, kBias = (KIND & SCORE_BIAS) != 0;
+                        if constexpr (kCapped) cap_scores<32>(pr + 32 * q, p.score);
                         const float d = float(row + mk.gap - k0 - 32 * q);
-                        auto walk = [&](auto capped) {
-                            uint64_t b2 = pack_f2(fmaf(bias.line, d, -lse), fmaf(bias.line, d - 1.f, -lse));
+                        uint64_t b2 = nl2;
+                        if constexpr (kBias) b2 = pack_f2(fmaf(bias.line, d, -lse), fmaf(bias.line, d - 1.f, -lse));
 #pragma unroll
-                            for (int x = 0; x < 32; x += 2) {
-                                float* y = pr + 32 * q + x;
-                                const uint64_t s2 = pack_f2(y[0], y[1]);
-                                uint64_t v, f = 0;
-                                if constexpr (KIND == SCORE_CAPPED) {
-                                    v = capped(s2);
-                                    f = cap_slope(v, p.score);
-                                    v = add_f2(v, b2);
-                                } else {
-                                    v = fma_f2(s2, c2, b2);
-                                }
-                                if (x < 30) b2 = add_f2(b2, pack_f2(-2.f * bias.line, -2.f * bias.line));
-                                float x0, x1;
-                                unpack_f2(v, x0, x1);
-                                if (bias.both) {
-                                    x0 = fmaf(bias.s, fabsf(d - float(x)), x0);
-                                    x1 = fmaf(bias.s, fabsf(d - float(x + 1)), x1);
-                                }
-                                x0 = fast_exp2(x0);
-                                x1 = fast_exp2(x1);
-                                if (flagged) {
-                                    x0 = (keep[q] & (1u << x)) ? x0 : 0.f;
-                                    x1 = (keep[q] & (2u << x)) ? x1 : 0.f;
-                                }
-                                if constexpr (KIND == SCORE_CAPPED) {
-                                    unpack_f2(mul_f2(pack_f2(x0, x1), f), y[0], y[1]);
-                                } else {
-                                    y[0] = x0;
-                                    y[1] = x1;
-                                }
+                        for (int x = 0; x < 32; x += 2) {
+                            float* y = pr + 32 * q + x;
+                            const uint64_t s2 = pack_f2(y[0], y[1]);
+                            float x0, x1;
+                            if constexpr (kCapped) unpack_f2(add_f2(s2, b2), x0, x1);
+                            else unpack_f2(fma_f2(s2, c2, b2), x0, x1);
+                            if (kBias && x < 30) b2 = add_f2(b2, pack_f2(-2.f * bias.line, -2.f * bias.line));
+                            if (kBias && bias.both) {
+                                x0 = fmaf(bias.s, fabsf(d - float(x)), x0);
+                                x1 = fmaf(bias.s, fabsf(d - float(x + 1)), x1);
                             }
-                        };
-                        if (beyond) walk([&](uint64_t s2) { return cap_pair(s2, p.score, true); });
-                        else walk([&](uint64_t s2) { return cap_pair(s2, p.score, false); });
+                            x0 = fast_exp2(x0);
+                            x1 = fast_exp2(x1);
+                            if (flagged) {
+                                x0 = (keep[q] & (1u << x)) ? x0 : 0.f;
+                                x1 = (keep[q] & (2u << x)) ? x1 : 0.f;
+                            }
+                            if constexpr (kCapped) unpack_f2(mul_f2(pack_f2(x0, x1), cap_slope(s2, p.score)), x0, x1);
+                            y[0] = x0;
+                            y[1] = x1;
+                        }
                         continue;
                     }
 #pragma unroll
@@ -669,6 +657,7 @@ cudaError_t launch_bwd_dq(int D, bool bf16, const CUtensorMap& tq, const CUtenso
                         : launch_dq_t<kD, kWarps, false, kKind>(tq, tk, tv, tdo, tdq, p, num_sms, overlap, stream);
         };
         using std::integral_constant;
+        if (p.score.kind == SCORE_CAPPED_BIAS) return of(integral_constant<int, SCORE_CAPPED_BIAS>{});
         if (p.score.kind == SCORE_CAPPED) return of(integral_constant<int, SCORE_CAPPED>{});
         if (p.score.kind == SCORE_BIAS) return of(integral_constant<int, SCORE_BIAS>{});
         return of(integral_constant<int, SCORE_PLAIN>{});

@@ -675,7 +675,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                 if constexpr (SCORED) {
                     const int first = SHORT ? 0 : qb * kBlk, last = SHORT ? mk.M - 1 : qb * kBlk + kBlk - 1;  // rows of the tile, and perhaps more
                     const Bias bias(slope, mk.causal && front == 0, first + mk.gap - (k0 + kBlk - 1), last + mk.gap - k0);
-                    score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, row + mk.gap - k0, valid);
+                    score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, row + mk.gap - k0, valid, m_run == -INFINITY ? 0.f : m_run);
                 }
 
                 if (fl & (TILE_BOUND | TILE_DOC)) {
@@ -727,7 +727,12 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                 const float mx = fmaxf(max3(mxa[0], mxa[1], mxa[2]), max3(max3(mxa[3], mxa[4], mxa[5]), mxa[6], mxa[7]));
                 float m_new = fmaxf(m_run, mx);
                 // lazy rescale: keep the old reference point while the new maximum is within 2^8 of it
-                const bool need = (m_new - m_run) * c > 8.0f;
+                bool need = (m_new - m_run) * c > 8.0f;
+                if constexpr (SCORED) {  // (the scores, and mx, are relative to the old reference point, or to 0 in front of a row's first key)
+                    const bool fresh = m_run == -INFINITY;
+                    need = fresh ? mx != -INFINITY : mx > 8.0f;
+                    m_new = (fresh ? 0.f : m_run) + mx;
+                }
                 if (!need) m_new = m_run;
                 if (S::POWN) {  // this tile's P overwrites that one's
                     alive = pv_before();
@@ -735,6 +740,11 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     tc_fence_after();
                 }
                 if (__any_sync(0xffffffffu, need)) {
+                    if constexpr (SCORED) {
+                        const float less = need ? -mx : 0.f;
+#pragma unroll
+                        for (int x = 0; x < 128; x += 2) unpack_f2(add_f2(pack_f2(sc[x], sc[x + 1]), pack_f2(less, less)), sc[x], sc[x + 1]);
+                    }
                     const float alpha = need ? fast_exp2((m_run - m_new) * c) : 1.0f;
                     l_run *= alpha;
                     if (t > t0) {
@@ -767,9 +777,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     uint32_t pk[16];
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
-                        const uint64_t x2 = fma_f2(pack_f2(sc[32 * q + 2 * x], sc[32 * q + 2 * x + 1]), c2, mneg2);
-                        float x0, x1;
-                        unpack_f2(x2, x0, x1);
+                        float x0 = sc[32 * q + 2 * x], x1 = sc[32 * q + 2 * x + 1];
+                        if constexpr (!SCORED) unpack_f2(fma_f2(pack_f2(x0, x1), c2, mneg2), x0, x1);
                         const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
                         if (x & 1) lacc1 = add_f2(lacc1, pack_f2(p0, p1)); else lacc0 = add_f2(lacc0, pack_f2(p0, p1));
                         pk[x] = pack2<BF16>(p0, p1);
@@ -917,6 +926,7 @@ cudaError_t launch_fwd(int D, bool bf16, const CUtensorMap& tq, const CUtensorMa
                         : launch_fwd_t<kD, false, kShort, kKind>(tq, tk, tv, to, p, num_sms, stream);
         };
         using std::integral_constant;
+        if (p.score.kind == SCORE_CAPPED_BIAS) return of(integral_constant<int, SCORE_CAPPED_BIAS>{});
         if (p.score.kind == SCORE_CAPPED) return of(integral_constant<int, SCORE_CAPPED>{});
         if (p.score.kind == SCORE_BIAS) return of(integral_constant<int, SCORE_BIAS>{});
         return of(integral_constant<int, SCORE_PLAIN>{});

@@ -558,7 +558,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                             for (int x = 0; x < 32; ++x) v[x] = x < len - kq ? v[x] : 0.f;
                         }
                         const Bias bias(slope, front == 0, pos0 - (kq + 31), pos0 + 31 - kq);
-                        score_row<KIND, 32>(v, p.score, bias, p.scale_log2, pos - kq, valid);
+                        score_row<KIND, 32>(v, p.score, bias, p.scale_log2, pos - kq, valid, m_run == -INFINITY ? 0.f : m_run);
                     }
                     if (kq + 31 > all_see) {
                         const uint32_t keep = first_bits(last - kq + 1);
@@ -575,8 +575,14 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
 #pragma unroll
                     for (int a = 0; a < 4; ++a) mx[a] = fmaxf(mx[a], v[28 + a]);
-                    float m_new = fmaxf(m_run, fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]));
-                    const bool need = (m_new - m_run) * c > 8.0f;
+                    const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+                    float m_new = fmaxf(m_run, top);
+                    bool need = (m_new - m_run) * c > 8.0f;
+                    if constexpr (SCORED) {
+                        const bool fresh = m_run == -INFINITY;
+                        need = fresh ? top != -INFINITY : top > 8.0f;
+                        m_new = (fresh ? 0.f : m_run) + top;
+                    }
                     if (!need) m_new = m_run;
                     const bool scale_o = __any_sync(0xffffffffu, need) && t > t0;
                     if (S::POWN || scale_o) {  // P*V of the group's tile before has read its P and added to O
@@ -588,7 +594,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     l_run *= alpha;
                     if (scale_o) rescale(alpha);
                     m_run = m_new;
-                    const float mneg = (m_run == -INFINITY) ? 0.f : -m_run * c;
+                    // (SCORED: what is left to be subtracted)
+                    const float mneg = SCORED ? (need ? -top : 0.f) : (m_run == -INFINITY) ? 0.f : -m_run * c;
                     float l4[4] = {0.f, 0.f, 0.f, 0.f};
                     uint32_t pk[16];
 #pragma unroll
@@ -628,7 +635,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         for (int x = 0; x < kBlk; ++x) sc[x] = x < real ? sc[x] : 0.f;
                     }
                     const Bias bias(slope, front == 0, pos0 - (k0 + kBlk - 1), pos0 + kBlk - 1 - k0);
-                    score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, pos - k0, valid);
+                    score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, pos - k0, valid, m_run == -INFINITY ? 0.f : m_run);
                 }
                 if (k0 + kBlk - 1 > all_see) {
 #pragma unroll
@@ -653,7 +660,12 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 const float mx = fmaxf(max3(mxa[0], mxa[1], mxa[2]), max3(max3(mxa[3], mxa[4], mxa[5]), mxa[6], mxa[7]));
                 float m_new = fmaxf(m_run, mx);
                 // lazy rescale: keep the old reference point while the new maximum is within 2^8 of it
-                const bool need = (m_new - m_run) * c > 8.0f;
+                bool need = (m_new - m_run) * c > 8.0f;
+                if constexpr (SCORED) {  // (the scores, and mx, are relative to the old reference point, or to 0 in front of a row's first key)
+                    const bool fresh = m_run == -INFINITY;
+                    need = fresh ? mx != -INFINITY : mx > 8.0f;
+                    m_new = (fresh ? 0.f : m_run) + mx;
+                }
                 if (!need) m_new = m_run;
                 if (S::POWN) {  // this tile's P overwrites that one's
                     alive = pv_before();
@@ -661,6 +673,11 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     tc_fence_after();
                 }
                 if (__any_sync(0xffffffffu, need)) {
+                    if constexpr (SCORED) {
+                        const float less = need ? -mx : 0.f;
+#pragma unroll
+                        for (int x = 0; x < 128; x += 2) unpack_f2(add_f2(pack_f2(sc[x], sc[x + 1]), pack_f2(less, less)), sc[x], sc[x + 1]);
+                    }
                     const float alpha = need ? fast_exp2((m_run - m_new) * c) : 1.0f;
                     l_run *= alpha;
                     if (t > t0) {
@@ -682,9 +699,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     uint32_t pk[16];
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
-                        const uint64_t x2 = fma_f2(pack_f2(sc[32 * q + 2 * x], sc[32 * q + 2 * x + 1]), c2, mneg2);
-                        float x0, x1;
-                        unpack_f2(x2, x0, x1);
+                        float x0 = sc[32 * q + 2 * x], x1 = sc[32 * q + 2 * x + 1];
+                        if constexpr (!SCORED) unpack_f2(fma_f2(pack_f2(x0, x1), c2, mneg2), x0, x1);
                         const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
                         if (x & 1) lacc1 = add_f2(lacc1, pack_f2(p0, p1)); else lacc0 = add_f2(lacc0, pack_f2(p0, p1));
                         pk[x] = pack2<BF16>(p0, p1);
@@ -860,8 +876,9 @@ cudaError_t launch_paged_fwd(bool bf16, const CUtensorMap& tq, const CUtensorMap
     };
     using std::integral_constant;
     auto of = [&](auto d) {
+        if (p.score.kind == SCORE_CAPPED_BIAS) return pick(d, integral_constant<int, SCORE_CAPPED_BIAS>{});
         if (p.score.kind == SCORE_CAPPED) return pick(d, integral_constant<int, SCORE_CAPPED>{});
-        if (p.score.kind == SCORE_BIAS && p.score.slopes) return pick(d, integral_constant<int, SCORE_BIAS>{});
+        if (p.score.slopes) return pick(d, integral_constant<int, SCORE_BIAS>{});
         return pick(d, integral_constant<int, SCORE_PLAIN>{});  // (a prefix alone is part of the mask)
     };
     return p.D == 128 ? of(integral_constant<int, 128>{}) : of(integral_constant<int, 64>{});

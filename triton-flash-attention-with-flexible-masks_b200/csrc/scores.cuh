@@ -15,8 +15,9 @@ namespace fa {
 // Instances of the attention kernels
 enum : int {
     SCORE_PLAIN = 0,   // attention
-    SCORE_BIAS = 1,    // a bias, a prefix, or both (a bias of 0 costs one packed addition for two scores)
-    SCORE_CAPPED = 2,  // the same and a cap
+    SCORE_BIAS = 1,    // a bias, a prefix, or both
+    SCORE_CAPPED = 2,  // a cap, and perhaps a prefix
+    SCORE_CAPPED_BIAS = SCORE_BIAS | SCORE_CAPPED,
 };
 
 constexpr int kTanhTerms = 5;
@@ -41,7 +42,7 @@ inline ScoreArgs make_score_args(float cap, const float* slopes, bool prefix, fl
     ScoreArgs s{};
     s.slopes = slopes;
     s.cap = cap;
-    s.kind = cap > 0.f ? SCORE_CAPPED : slopes || prefix ? SCORE_BIAS : SCORE_PLAIN;
+    s.kind = (cap > 0.f ? SCORE_CAPPED : SCORE_PLAIN) | (slopes || (prefix && !(cap > 0.f)) ? SCORE_BIAS : SCORE_PLAIN);
     if (cap > 0.f) {
         const double a = double(cap) * 1.4426950408889634, k = double(sm_scale) / cap;
         double power = a * k, most = 0.75;
@@ -90,12 +91,6 @@ __device__ __forceinline__ uint64_t cap_poly(uint64_t s2, const ScoreArgs& a) {
 __device__ __forceinline__ float cap_any(float s, const ScoreArgs& a) {
     return fmaf(-2.f * a.a, fast_rcp(1.f + fast_exp2(s * a.k2e)), a.a);
 }
-__device__ __forceinline__ uint64_t cap_pair(uint64_t s2, const ScoreArgs& a, bool beyond) {
-    if (!beyond) return mul_f2(s2, cap_poly(s2, a));
-    float s0, s1;
-    unpack_f2(s2, s0, s1);
-    return pack_f2(cap_any(s0, a), cap_any(s1, a));
-}
 // 1 - tanh^2 of two capped scores
 __device__ __forceinline__ uint64_t cap_slope(uint64_t y2, const ScoreArgs& a) {
     const uint64_t t2 = mul_f2(y2, pack_f2(a.inv_a, a.inv_a));
@@ -118,33 +113,70 @@ struct Bias {
     }
 };
 
-// N neighbouring scores of one row (a multiple of 32), in place, to the log2 domain; dist: distance of the first one. real: the row is a
+// v[x] = f(v[x], x) for the N values of a thread, 32 at a time, in a loop that moves them all on: for what is rarely done. Unrolled, it would be most of the
+// code of the softmax warps, which is fetched again and again.
+template <int N, class F>
+__device__ __forceinline__ void rolled(float* v, F f) {
+#pragma unroll 1
+    for (int x0 = 0; x0 < N; x0 += 32) {
+        float first[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) first[x] = f(v[x], x0 + x);
+#pragma unroll
+        for (int x = 0; x + 32 < N; ++x) v[x] = v[x + 32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) v[N - 32 + x] = first[x];
+    }
+}
+
+// N neighbouring scores of one row (a multiple of 32), in place, to the log2 domain, less `ref`; dist: distance of the first one. real: the row is a
 // query's (what lies in other rows of the tile must not tell the warp which form of the tanh to take, and so the last bits).
 template <int KIND, int N>
-__device__ __forceinline__ void score_row(float* v, const ScoreArgs& a, const Bias& bias, float c, int dist, bool real) {
-    const uint64_t step2 = pack_f2(-2.f * bias.line, -2.f * bias.line);
-    auto each = [&](auto score) {  // score(two scores, their bias)
+__device__ __forceinline__ void score_row(float* v, const ScoreArgs& a, const Bias& bias, float c, int dist, bool real, float ref) {
+    constexpr bool kCapped = (KIND & SCORE_CAPPED) != 0, kBias = (KIND & SCORE_BIAS) != 0;
+    const bool beyond = kCapped && any_beyond<N>(v, real ? a.most : INFINITY);
+    auto each = [&](auto score) {  // score(two scores, what is added to them)
 #pragma unroll
         for (int q = 0; q < N; q += 32) {
-            const float d = float(dist - q);
-            uint64_t b2 = pack_f2(bias.line * d, bias.line * (d - 1.f));
+            uint64_t b2 = pack_f2(-ref, -ref);
+            if constexpr (kBias) {
+                const float d = float(dist - q);
+                b2 = pack_f2(fmaf(bias.line, d, -ref), fmaf(bias.line, d - 1.f, -ref));
+            }
 #pragma unroll
             for (int x = q; x < q + 32; x += 2) {
                 unpack_f2(score(pack_f2(v[x], v[x + 1]), b2), v[x], v[x + 1]);
-                if (x + 2 < q + 32) b2 = add_f2(b2, step2);
+                if (kBias && x + 2 < q + 32) b2 = add_f2(b2, pack_f2(-2.f * bias.line, -2.f * bias.line));
             }
         }
     };
-    if constexpr (KIND == SCORE_CAPPED) {
-        if (!any_beyond<N>(v, real ? a.most : INFINITY)) each([&](uint64_t s2, uint64_t b2) { return fma_f2(s2, cap_poly(s2, a), b2); });
-        else each([&](uint64_t s2, uint64_t b2) { return add_f2(cap_pair(s2, a, true), b2); });
+    if constexpr (kCapped) {
+        if (beyond) {
+            const float d = float(dist);
+            rolled<N>(v, [&](float s, int x) { return cap_any(s, a) + (kBias ? fmaf(bias.line, d - float(x), -ref) : -ref); });
+        } else {
+            each([&](uint64_t s2, uint64_t b2) { return fma_f2(s2, cap_poly(s2, a), b2); });
+        }
     } else {
         each([&](uint64_t s2, uint64_t b2) { return fma_f2(s2, pack_f2(c, c), b2); });
     }
-    if (bias.both) {
+    if (kBias && bias.both) {
         const float d = float(dist);
+        rolled<N>(v, [&](float y, int x) { return fmaf(bias.s, fabsf(d - float(x)), y); });
+    }
+}
+
+// The same as above without bias and reference: scores to capped scores, for the backward kernels.
+template <int N>
+__device__ __forceinline__ void cap_scores(float* v, const ScoreArgs& a) {
+    if (any_beyond<N>(v, a.most)) {
+        rolled<N>(v, [&](float s, int) { return cap_any(s, a); });
+    } else {
 #pragma unroll
-        for (int x = 0; x < N; ++x) v[x] = fmaf(bias.s, fabsf(d - float(x)), v[x]);
+        for (int x = 0; x < N; x += 2) {
+            const uint64_t s2 = pack_f2(v[x], v[x + 1]);
+            unpack_f2(mul_f2(s2, cap_poly(s2, a)), v[x], v[x + 1]);
+        }
     }
 }
 
