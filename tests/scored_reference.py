@@ -60,9 +60,10 @@ def attention_64(q, k, v, do, causal, sm_scale, eq, ek, cap, slopes, prefix):
     dp_err = D * 2.0 ** -23 * (DO.abs() @ V.abs().mT)
     delta_err = (DO.abs() * (o_err + D * 2.0 ** -23 * o.abs())).sum(-1, keepdim=True)
     ds = p * (dp - delta) * f
-    # f = 1 - tanh^2 is off by some 2^-22 in absolute terms and by the score's error
+    # f = 1 - tanh^2 is off by some 2^-22 in absolute terms and by the score's error. (f + e)(d + g) - f d = f g + e d + e g: the last term is all there
+    # is where f is 0 (a score far beyond the cap) and so is d = dP - delta (a row of one key).
     f_err = (2.0 ** -21 + 2 * err / cap) if cap else 0.0
-    ds_err = sub * seen + (up + rel) * ds.abs() + p * (f * (dp_err + delta_err) + f_err * (dp - delta).abs())
+    ds_err = sub * seen + (up + rel) * ds.abs() + p * ((f + f_err) * (dp_err + delta_err) + f_err * (dp - delta).abs())
     dq, dk = ds @ K * scale, ds.mT @ Q * scale
     dq_err = scale * ((ds_err + acc * ds.abs()) @ K.abs())
     dk_err = scale * ((ds_err + accm * ds.abs()).mT @ Q.abs())

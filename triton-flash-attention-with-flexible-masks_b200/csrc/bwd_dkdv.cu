@@ -120,7 +120,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 const __grid_constant__ CUtensorMap tmdK, const __grid_constant__ CUtensorMap tmdV,
                 const DkdvParams p) {
     using S = DkdvSmem<D>;
-    constexpr bool SCORED = KIND != SCORE_PLAIN;
+    constexpr bool PREFIX = KIND != SCORE_PLAIN, SCORED = score_changed(KIND);  // perhaps a prefix; other scores
     constexpr int NQ = S::NQ, NDO = S::NDO;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -256,7 +256,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     const int ng = (mk.He == 1) ? 1 : G;
                     for (int g = 0; g < ng; ++g) {
                         int l, h2;
-                        q_range<SCORED>(mk, b, mk.He == 1 ? 0 : hk * G + g, kb, l, h2);
+                        q_range<PREFIX>(mk, b, mk.He == 1 ? 0 : hk * G + g, kb, l, h2);
                         if (h2 > l) { lo = min(lo, l); hi = max(hi, h2); }
                     }
                     if (hi == 0) lo = 0;
@@ -270,7 +270,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     for (int e = 0; e < 4; ++e) {
                         const int c = 4 * i + e;
                         if (c >= n) break;
-                        const uint32_t f = classify_group<SCORED>(mk, b, hk, G, lo + c, kb);
+                        const uint32_t f = classify_group<PREFIX>(mk, b, hk, G, lo + c, kb);
                         uint32_t code = KC_SKIP;
                         if (f & TILE_VISIT) code = !(f & TILE_DOC) ? KC_PLAIN : (f & TILE_QMANY) ? KC_DOCMANY : KC_DOC;
                         cnt += (code != KC_SKIP);
@@ -288,7 +288,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     info[s * 8 + 4] = kb;
                     info[s * 8 + 5] = hk;
                     info[s * 8 + 6] = b;
-                    if constexpr (SCORED) info[s * 8 + 7] = front_keys<true>(mk, b);
+                    if constexpr (PREFIX) info[s * 8 + 7] = front_keys<true>(mk, b);
                     mbar_arrive(BAR(B_ITEMFULL + s));
                 }
             }
@@ -506,13 +506,13 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             int cg = 0, cc = -1;
             uint32_t code = KC_SKIP;
             int kc = 0, kc_g = -1;  // this key's code for the current query head
-            const int front = SCORED ? info[s * 8 + 7] : 0;
+            const int front = PREFIX ? info[s * 8 + 7] : 0;
             const float* const delta0 = p.delta + (int64_t(b) * p.H + hk * G) * mk.L.Mpad + cbase + 2 * (lane & 3);
             for (int it = 0; it < NIT && ok; ++it) {
                 wk.next(cg, cc, code);
                 const bool fl_doc = code >= KC_DOC, many = code == KC_DOCMANY;
                 const int qb0 = (lo + cc) * kBlk;
-                const bool fl_range = (mk.causal && (k0 + kBlk > mk.N || (k1 - 1 > qb0 + mk.gap && (!SCORED || k1 > front)))) || (qb0 + kBlk > mk.M);
+                const bool fl_range = (mk.causal && (k0 + kBlk > mk.N || (k1 - 1 > qb0 + mk.gap && (!PREFIX || k1 > front)))) || (qb0 + kBlk > mk.M);
                 const int q0 = qb0 + cbase;  // first query row of this warp's columns
                 const int gi = gt + it;
                 // the rows' LSE came with Q, which S^T has been computed from; their delta is asked for here
@@ -535,7 +535,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         keep = codes_equal(qcs, qc, kc, many) | __ballot_sync(0xffffffffu, qc >= 0);
                     }
                     if (fl_range) {
-                        const int cmin = mk.causal && (!SCORED || j >= front) ? (j - mk.gap) - q0 : 0, cmax = mk.M - q0;
+                        const int cmin = mk.causal && (!PREFIX || j >= front) ? (j - mk.gap) - q0 : 0, cmax = mk.M - q0;
                         keep &= first_bits(cmax) & ~first_bits(cmin);
                     }
                 }
@@ -777,6 +777,7 @@ cudaError_t launch_bwd_dkdv(int D, bool bf16, const CUtensorMap& tq, const CUten
         if (p.score.kind == SCORE_CAPPED_BIAS) return pick(d, integral_constant<int, SCORE_CAPPED_BIAS>{});
         if (p.score.kind == SCORE_CAPPED) return pick(d, integral_constant<int, SCORE_CAPPED>{});
         if (p.score.kind == SCORE_BIAS) return pick(d, integral_constant<int, SCORE_BIAS>{});
+        if (p.score.kind == SCORE_PREFIX) return pick(d, integral_constant<int, SCORE_PREFIX>{});
         return pick(d, integral_constant<int, SCORE_PLAIN>{});
     };
     return D == 128 ? of(integral_constant<int, 128>{}) : of(integral_constant<int, 64>{});

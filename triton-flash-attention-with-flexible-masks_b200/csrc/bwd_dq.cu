@@ -71,7 +71,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
               const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
               const __grid_constant__ CUtensorMap tmdQ, const DqParams p) {
     using S = DqSmem<D, NW>;
-    constexpr bool SCORED = KIND != SCORE_PLAIN;
+    constexpr bool PREFIX = KIND != SCORE_PLAIN, SCORED = score_changed(KIND);  // perhaps a prefix; other scores
     constexpr int NSK = S::NSK, NC = S::COLS;
     constexpr bool kOne = D == 128;  // one warp issues all MMAs
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -186,7 +186,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                 decode(j, qb, h, b);
                 const int he = (mk.He == 1) ? 0 : h;
                 int lo, hi;
-                kv_range<SCORED>(mk, b, he, qb, lo, hi);
+                kv_range<PREFIX>(mk, b, he, qb, lo, hi);
                 int n = hi - lo;
                 if (n > kListCap) n = kListCap;  // the host refuses problems that could exceed the cap
                 uint8_t* fl = smem + S::off_flags + s * S::FLAGS;
@@ -196,7 +196,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                     for (int e = 0; e < 4; ++e) {
                         const int c = 4 * i + e;
                         if (c >= n) break;
-                        const uint32_t f = classify_from_plan<SCORED>(mk, b, he, qb, lo + c);
+                        const uint32_t f = classify_from_plan<PREFIX>(mk, b, he, qb, lo + c);
                         uint32_t code = QC_SKIP;
                         if (f & TILE_VISIT) code = !(f & TILE_DOC) ? QC_PLAIN : (f & TILE_KMANY) ? QC_DOCMANY : QC_DOC;
                         cnt += (code != QC_SKIP);
@@ -214,7 +214,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                     info[s * 8 + 4] = qb;
                     info[s * 8 + 5] = h;
                     info[s * 8 + 6] = b;
-                    if constexpr (SCORED) info[s * 8 + 7] = front_keys<true>(mk, b);
+                    if constexpr (PREFIX) info[s * 8 + 7] = front_keys<true>(mk, b);
                     mbar_arrive(BAR(B_ITEMFULL + s));
                 }
             }
@@ -414,7 +414,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             const int he = (mk.He == 1) ? 0 : h;
             const DqWalk wk = walk_of(s, n);
             const int row = qb * kBlk + r;
-            const int front = SCORED ? info[s * 8 + 7] : 0;
+            const int front = PREFIX ? info[s * 8 + 7] : 0;
             const float slope = SCORED && p.score.slopes ? p.score.slopes[h] * kScoreLog2e : 0.f;
             const int q0 = qb * kBlk;
             const int64_t bh_ids = int64_t(b) * mk.He + he;
@@ -435,7 +435,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                 const bool fl_doc = code >= QC_DOC, many = code == QC_DOCMANY;
                 const int kb0 = (lo + cc) * kBlk;
                 const int kb1 = min(kb0 + kBlk, mk.N);
-                const bool fl_bound = (kb0 + kBlk > mk.N) || (mk.causal && kb1 - 1 > q0 + mk.gap && (!SCORED || kb1 > front));
+                const bool fl_bound = (kb0 + kBlk > mk.N) || (mk.causal && kb1 - 1 > q0 + mk.gap && (!PREFIX || kb1 > front));
                 const int k0 = kb0 + cbase;  // first key column of this thread
                 const uint32_t tS = tmem + lane_base + uint32_t(gi & 1) * 128u + uint32_t(cbase);
                 // keep(x) = (x <= lim) & (qc >= 0 | kc[x] == qc) as 32-bit masks, worked out before the scores are there
@@ -457,7 +457,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                     }
                     if (fl_bound) {
                         int jmax = mk.N - 1;
-                        if (mk.causal) jmax = min(jmax, SCORED ? max(row + mk.gap, front - 1) : row + mk.gap);
+                        if (mk.causal) jmax = min(jmax, PREFIX ? max(row + mk.gap, front - 1) : row + mk.gap);
 #pragma unroll
                         for (int q = 0; q < NC / 32; ++q) keep[q] &= first_bits(jmax + 1 - k0 - 32 * q);
                     }
@@ -659,6 +659,7 @@ cudaError_t launch_bwd_dq(int D, bool bf16, const CUtensorMap& tq, const CUtenso
         using std::integral_constant;
         if (p.score.kind == SCORE_CAPPED_BIAS) return of(integral_constant<int, SCORE_CAPPED_BIAS>{});
         if (p.score.kind == SCORE_CAPPED) return of(integral_constant<int, SCORE_CAPPED>{});
+        if (p.score.kind == SCORE_PREFIX) return of(integral_constant<int, SCORE_PREFIX>{});
         if (p.score.kind == SCORE_BIAS) return of(integral_constant<int, SCORE_BIAS>{});
         return of(integral_constant<int, SCORE_PLAIN>{});
     };

@@ -98,13 +98,13 @@ static_assert(FwdSmem<128>::total > 116736 && FwdSmem<64>::total > 116736, "shar
 //    and their log-sum-exp go to the workspace, and fwd_combine_kernel merges them.
 // Such calls are bound by reading K and V (16 tokens of 32 / 8 heads of 128 against 4500 keys: 295 MB, 45 us at the
 // copy rate; 127 us with a tile per head, 55 us packed) or, with few heads, by the longest item's chain of tiles.
-// KIND: other than SCORE_PLAIN, the scores pass through score_row (scores.cuh) and are in the log2 domain from there on, and the causal mask may leave a prefix visible.
+// KIND (scores.cuh): with a cap or a bias the scores pass through score_row and are in the log2 domain from there on; the causal mask may leave a prefix visible.
 template <int D, bool BF16, bool SHORT, int KIND = SCORE_PLAIN>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
            const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const FwdParams p) {
     using S = FwdSmem<D>;
-    constexpr bool SCORED = KIND != SCORE_PLAIN;
+    constexpr bool PREFIX = KIND != SCORE_PLAIN, SCORED = score_changed(KIND);  // perhaps a prefix; other scores
     constexpr int NS = S::NS, NQ = S::NQ, NP = S::NP;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -150,7 +150,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         int4 qc;
     };
     auto classify = [&](const Item& it, int i) {
-        return i < it.n ? classify_from_plan<SCORED>(mk, it.b, (mk.He == 1) ? 0 : it.h, it.qb, it.lo + i) & (TILE_VISIT | TILE_BOUND | TILE_DOC | TILE_KMONO | TILE_KMANY) : 0u;
+        return i < it.n ? classify_from_plan<PREFIX>(mk, it.b, (mk.He == 1) ? 0 : it.h, it.qb, it.lo + i) & (TILE_VISIT | TILE_BOUND | TILE_DOC | TILE_KMONO | TILE_KMANY) : 0u;
     };
     auto prepare = [&](int j) {
         Item it;
@@ -158,7 +158,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         decode(SHORT ? j / ns : j, it.qb, it.h, it.b);
         const int he = (mk.He == 1) ? 0 : it.h;
         int lo, hi;
-        kv_range<SCORED>(mk, it.b, he, it.qb, lo, hi);
+        kv_range<PREFIX>(mk, it.b, he, it.qb, lo, hi);
         int n = hi - lo;
         if constexpr (SHORT) {  // no ids: every tile of the range is visited
             const int first = int(int64_t(n) * sp / ns);
@@ -307,7 +307,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     info[s * 8 + 4] = item.qb;
                     info[s * 8 + 5] = item.h;
                     info[s * 8 + 6] = item.b;
-                    if constexpr (SCORED) info[s * 8 + 7] = front_keys<true>(mk, item.b);
+                    if constexpr (PREFIX) info[s * 8 + 7] = front_keys<true>(mk, item.b);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(BAR(B_ITEMFULL + s));
@@ -634,10 +634,9 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
             const bool active = !SHORT || __any_sync(0xffffffffu, valid);  // does this warp hold a query at all?
             const int qc = reinterpret_cast<const int*>(smem + S::off_qc)[s * kBlk + r];
             const int t0 = (G ^ w) & 1;  // this group's first tile of the item
-            int front = 0;       // SCORED: of the item's sequence and this row's head
-            float slope = 0.f;
+            const int front = PREFIX ? info[s * 8 + 7] : 0;  // of the item's sequence
+            float slope = 0.f;                               // SCORED: of this row's head
             if constexpr (SCORED) {
-                front = info[s * 8 + 7];
                 const int h = info[s * 8 + 5], own = SHORT ? min((h % nG) * p.pack + g_row, p.G - 1) + h / nG * p.G : h;
                 if (p.score.slopes) slope = p.score.slopes[int64_t(own)] * kScoreLog2e;
             }
@@ -672,10 +671,14 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     mbar_arrive_warp(BAR(B_SFREE + w), lane);  // the next tile's scores may overwrite these
                 }
                 float* sc = reinterpret_cast<float*>(sr);
+                // A capped tile without a mask is not capped before its exponentials: the greatest score tells the greatest capped one, and the polynomial
+                // runs beside the special-function unit. (With a bias the greatest one has to be looked for behind it.)
+                bool late = false;
                 if constexpr (SCORED) {
                     const int first = SHORT ? 0 : qb * kBlk, last = SHORT ? mk.M - 1 : qb * kBlk + kBlk - 1;  // rows of the tile, and perhaps more
                     const Bias bias(slope, mk.causal && front == 0, first + mk.gap - (k0 + kBlk - 1), last + mk.gap - k0);
-                    score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, row + mk.gap - k0, valid, m_run == -INFINITY ? 0.f : m_run);
+                    if constexpr (KIND == SCORE_CAPPED) late = !(fl & (TILE_BOUND | TILE_DOC)) && !any_beyond<kBlk>(sc, valid ? p.score.most : INFINITY);
+                    if (!late) score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, row + mk.gap - k0, valid, m_run == -INFINITY ? 0.f : m_run);
                 }
 
                 if (fl & (TILE_BOUND | TILE_DOC)) {
@@ -687,7 +690,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     int lim = kBlk - 1;
                     if (fl & TILE_BOUND) {
                         int jmax = mk.N - 1;
-                        if (mk.causal) jmax = min(jmax, SCORED ? max(row + mk.gap, front - 1) : row + mk.gap);
+                        if (mk.causal) jmax = min(jmax, PREFIX ? max(row + mk.gap, front - 1) : row + mk.gap);
                         lim = jmax - k0;
                     }
                     // (the key codes completed on K's barrier, before the S MMA whose result was just read)
@@ -724,12 +727,13 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                 }
 #pragma unroll
                 for (int a = 0; a < 8; ++a) mxa[a] = fmaxf(mxa[a], sc[120 + a]);
-                const float mx = fmaxf(max3(mxa[0], mxa[1], mxa[2]), max3(max3(mxa[3], mxa[4], mxa[5]), mxa[6], mxa[7]));
+                float mx = fmaxf(max3(mxa[0], mxa[1], mxa[2]), max3(max3(mxa[3], mxa[4], mxa[5]), mxa[6], mxa[7]));
                 float m_new = fmaxf(m_run, mx);
                 // lazy rescale: keep the old reference point while the new maximum is within 2^8 of it
                 bool need = (m_new - m_run) * c > 8.0f;
                 if constexpr (SCORED) {  // (the scores, and mx, are relative to the old reference point, or to 0 in front of a row's first key)
                     const bool fresh = m_run == -INFINITY;
+                    if (late) mx = cap_one(mx, p.score) - (fresh ? 0.f : m_run);
                     need = fresh ? mx != -INFINITY : mx > 8.0f;
                     m_new = (fresh ? 0.f : m_run) + mx;
                 }
@@ -740,7 +744,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     tc_fence_after();
                 }
                 if (__any_sync(0xffffffffu, need)) {
-                    if constexpr (SCORED) {
+                    if (SCORED && !late) {
                         const float less = need ? -mx : 0.f;
 #pragma unroll
                         for (int x = 0; x < 128; x += 2) unpack_f2(add_f2(pack_f2(sc[x], sc[x + 1]), pack_f2(less, less)), sc[x], sc[x + 1]);
@@ -772,19 +776,24 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                 // exp2(s*c - m*c) on packed pairs
                 const uint64_t c2 = pack_f2(c, c), mneg2 = pack_f2(mneg, mneg);
                 uint64_t lacc0 = pack_f2(0.f, 0.f), lacc1 = lacc0;
+                auto exponentials = [&](auto exponent) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t pk[16];
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t pk[16];
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) {
-                        float x0 = sc[32 * q + 2 * x], x1 = sc[32 * q + 2 * x + 1];
-                        if constexpr (!SCORED) unpack_f2(fma_f2(pack_f2(x0, x1), c2, mneg2), x0, x1);
-                        const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-                        if (x & 1) lacc1 = add_f2(lacc1, pack_f2(p0, p1)); else lacc0 = add_f2(lacc0, pack_f2(p0, p1));
-                        pk[x] = pack2<BF16>(p0, p1);
+                        for (int x = 0; x < 16; ++x) {
+                            float x0, x1;
+                            unpack_f2(exponent(pack_f2(sc[32 * q + 2 * x], sc[32 * q + 2 * x + 1])), x0, x1);
+                            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+                            if (x & 1) lacc1 = add_f2(lacc1, pack_f2(p0, p1)); else lacc0 = add_f2(lacc0, pack_f2(p0, p1));
+                            pk[x] = pack2<BF16>(p0, p1);
+                        }
+                        tmem_st16(tP + uint32_t(q) * 16u, pk);
                     }
-                    tmem_st16(tP + uint32_t(q) * 16u, pk);
-                }
+                };
+                if constexpr (!SCORED) exponentials([&](uint64_t s2) { return fma_f2(s2, c2, mneg2); });
+                else if (KIND == SCORE_CAPPED && late) exponentials([&](uint64_t s2) { return fma_f2(s2, cap_poly(s2, p.score), mneg2); });
+                else exponentials([&](uint64_t s2) { return s2; });
                 tc_wait_st();
                 tc_fence_before();
                 mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
@@ -928,6 +937,7 @@ cudaError_t launch_fwd(int D, bool bf16, const CUtensorMap& tq, const CUtensorMa
         using std::integral_constant;
         if (p.score.kind == SCORE_CAPPED_BIAS) return of(integral_constant<int, SCORE_CAPPED_BIAS>{});
         if (p.score.kind == SCORE_CAPPED) return of(integral_constant<int, SCORE_CAPPED>{});
+        if (p.score.kind == SCORE_PREFIX) return of(integral_constant<int, SCORE_PREFIX>{});
         if (p.score.kind == SCORE_BIAS) return of(integral_constant<int, SCORE_BIAS>{});
         return of(integral_constant<int, SCORE_PLAIN>{});
     };

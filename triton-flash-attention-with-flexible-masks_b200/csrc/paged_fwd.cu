@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmN, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const PagedParams p) {
     using S = PagedSmem<D>;
-    constexpr bool SCORED = KIND != SCORE_PLAIN;
+    constexpr bool SCORED = score_changed(KIND);
     constexpr int NS = S::NS, NQ = S::NQ, NP = S::NP;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -628,6 +628,9 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 }
                 float* sc = reinterpret_cast<float*>(sr);
                 const int real = len - k0;  // keys of the tile that there are
+                // A capped tile without a mask is not capped before its exponentials: the greatest score tells the greatest capped one, and the polynomial
+                // runs beside the special-function unit. (With a bias the greatest one has to be looked for behind it.)
+                bool late = false;
                 if constexpr (SCORED) {
                     // (what the others' scores are must not tell the warp which form of the cap to take)
                     if (real < kBlk) {
@@ -635,7 +638,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         for (int x = 0; x < kBlk; ++x) sc[x] = x < real ? sc[x] : 0.f;
                     }
                     const Bias bias(slope, front == 0, pos0 - (k0 + kBlk - 1), pos0 + kBlk - 1 - k0);
-                    score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, pos - k0, valid, m_run == -INFINITY ? 0.f : m_run);
+                    if constexpr (KIND == SCORE_CAPPED) late = k0 + kBlk - 1 <= all_see && !any_beyond<kBlk>(sc, valid ? p.score.most : INFINITY);
+                    if (!late) score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, pos - k0, valid, m_run == -INFINITY ? 0.f : m_run);
                 }
                 if (k0 + kBlk - 1 > all_see) {
 #pragma unroll
@@ -657,12 +661,13 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 }
 #pragma unroll
                 for (int a = 0; a < 8; ++a) mxa[a] = fmaxf(mxa[a], sc[120 + a]);
-                const float mx = fmaxf(max3(mxa[0], mxa[1], mxa[2]), max3(max3(mxa[3], mxa[4], mxa[5]), mxa[6], mxa[7]));
+                float mx = fmaxf(max3(mxa[0], mxa[1], mxa[2]), max3(max3(mxa[3], mxa[4], mxa[5]), mxa[6], mxa[7]));
                 float m_new = fmaxf(m_run, mx);
                 // lazy rescale: keep the old reference point while the new maximum is within 2^8 of it
                 bool need = (m_new - m_run) * c > 8.0f;
                 if constexpr (SCORED) {  // (the scores, and mx, are relative to the old reference point, or to 0 in front of a row's first key)
                     const bool fresh = m_run == -INFINITY;
+                    if (late) mx = cap_one(mx, p.score) - (fresh ? 0.f : m_run);
                     need = fresh ? mx != -INFINITY : mx > 8.0f;
                     m_new = (fresh ? 0.f : m_run) + mx;
                 }
@@ -673,7 +678,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     tc_fence_after();
                 }
                 if (__any_sync(0xffffffffu, need)) {
-                    if constexpr (SCORED) {
+                    if (SCORED && !late) {
                         const float less = need ? -mx : 0.f;
 #pragma unroll
                         for (int x = 0; x < 128; x += 2) unpack_f2(add_f2(pack_f2(sc[x], sc[x + 1]), pack_f2(less, less)), sc[x], sc[x + 1]);
@@ -694,19 +699,24 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 // exp2(s*c - m*c) on packed pairs
                 const uint64_t c2 = pack_f2(c, c), mneg2 = pack_f2(mneg, mneg);
                 uint64_t lacc0 = pack_f2(0.f, 0.f), lacc1 = lacc0;
+                auto exponentials = [&](auto exponent) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t pk[16];
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t pk[16];
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) {
-                        float x0 = sc[32 * q + 2 * x], x1 = sc[32 * q + 2 * x + 1];
-                        if constexpr (!SCORED) unpack_f2(fma_f2(pack_f2(x0, x1), c2, mneg2), x0, x1);
-                        const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-                        if (x & 1) lacc1 = add_f2(lacc1, pack_f2(p0, p1)); else lacc0 = add_f2(lacc0, pack_f2(p0, p1));
-                        pk[x] = pack2<BF16>(p0, p1);
+                        for (int x = 0; x < 16; ++x) {
+                            float x0, x1;
+                            unpack_f2(exponent(pack_f2(sc[32 * q + 2 * x], sc[32 * q + 2 * x + 1])), x0, x1);
+                            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+                            if (x & 1) lacc1 = add_f2(lacc1, pack_f2(p0, p1)); else lacc0 = add_f2(lacc0, pack_f2(p0, p1));
+                            pk[x] = pack2<BF16>(p0, p1);
+                        }
+                        tmem_st16(tP + uint32_t(q) * 16u, pk);
                     }
-                    tmem_st16(tP + uint32_t(q) * 16u, pk);
-                }
+                };
+                if constexpr (!SCORED) exponentials([&](uint64_t s2) { return fma_f2(s2, c2, mneg2); });
+                else if (KIND == SCORE_CAPPED && late) exponentials([&](uint64_t s2) { return fma_f2(s2, cap_poly(s2, p.score), mneg2); });
+                else exponentials([&](uint64_t s2) { return s2; });
                 tc_wait_st();
                 if (real < kBlk) alive = zero_behind(g, real);
                 tc_fence_before();

@@ -15,10 +15,13 @@ namespace fa {
 // Instances of the attention kernels
 enum : int {
     SCORE_PLAIN = 0,   // attention
-    SCORE_BIAS = 1,    // a bias, a prefix, or both
+    SCORE_BIAS = 1,    // a bias, and perhaps a prefix
     SCORE_CAPPED = 2,  // a cap, and perhaps a prefix
     SCORE_CAPPED_BIAS = SCORE_BIAS | SCORE_CAPPED,
+    SCORE_PREFIX = 4,  // a prefix alone: the scores are attention's
 };
+// Does an instance change the scores?
+__host__ __device__ constexpr bool score_changed(int kind) { return (kind & SCORE_CAPPED_BIAS) != 0; }
 
 constexpr int kTanhTerms = 5;
 
@@ -30,7 +33,8 @@ struct ScoreArgs {
     float most;
     float k2e;            // 2 log2(e) sm_scale / cap
     float k;              // sm_scale / cap
-    float a, inv_a;       // cap log2(e)
+    float a;              // cap log2(e)
+    float minus_inv_a2;   // -1 / a^2
 };
 
 constexpr float kScoreLog2e = 1.4426950408889634f;
@@ -42,7 +46,8 @@ inline ScoreArgs make_score_args(float cap, const float* slopes, bool prefix, fl
     ScoreArgs s{};
     s.slopes = slopes;
     s.cap = cap;
-    s.kind = (cap > 0.f ? SCORE_CAPPED : SCORE_PLAIN) | (slopes || (prefix && !(cap > 0.f)) ? SCORE_BIAS : SCORE_PLAIN);
+    s.kind = (cap > 0.f ? SCORE_CAPPED : SCORE_PLAIN) | (slopes ? SCORE_BIAS : SCORE_PLAIN);
+    if (prefix && s.kind == SCORE_PLAIN) s.kind = SCORE_PREFIX;
     if (cap > 0.f) {
         const double a = double(cap) * 1.4426950408889634, k = double(sm_scale) / cap;
         double power = a * k, most = 0.75;
@@ -56,7 +61,7 @@ inline ScoreArgs make_score_args(float cap, const float* slopes, bool prefix, fl
         s.k = float(k < 1e37 ? k : 1e37);
         s.k2e = float(2.885390081777927 * k < 1e38 ? 2.885390081777927 * k : 1e38);
         s.a = float(a);
-        s.inv_a = float(1.0 / a);
+        s.minus_inv_a2 = float(-1.0 / (a * a));
     }
     return s;
 }
@@ -87,16 +92,21 @@ __device__ __forceinline__ uint64_t cap_poly(uint64_t s2, const ScoreArgs& a) {
     for (int i = kTanhTerms - 2; i >= 0; --i) t = fma_f2(t, u2, pack_f2(a.poly[i], a.poly[i]));
     return t;
 }
+// the capped score of one that the polynomial covers: the bits of its place in a pair
+__device__ __forceinline__ float cap_one(float s, const ScoreArgs& a) {
+    const float u = __fmul_rn(s, s);
+    float t = a.poly[kTanhTerms - 1];
+#pragma unroll
+    for (int i = kTanhTerms - 2; i >= 0; --i) t = fmaf(t, u, a.poly[i]);
+    return __fmul_rn(s, t);
+}
 // the capped score, whatever its size
 __device__ __forceinline__ float cap_any(float s, const ScoreArgs& a) {
     return fmaf(-2.f * a.a, fast_rcp(1.f + fast_exp2(s * a.k2e)), a.a);
 }
 // 1 - tanh^2 of two capped scores
 __device__ __forceinline__ uint64_t cap_slope(uint64_t y2, const ScoreArgs& a) {
-    const uint64_t t2 = mul_f2(y2, pack_f2(a.inv_a, a.inv_a));
-    float t0, t1;
-    unpack_f2(t2, t0, t1);
-    return fma_f2(t2, pack_f2(-t0, -t1), pack_f2(1.f, 1.f));
+    return fma_f2(mul_f2(y2, y2), pack_f2(a.minus_inv_a2, a.minus_inv_a2), pack_f2(1.f, 1.f));
 }
 
 // The bias of the entries of one tile. The distance i + gap - j of an entry that the masks keep has one sign over most tiles (with a causal
@@ -151,7 +161,9 @@ __device__ __forceinline__ void score_row(float* v, const ScoreArgs& a, const Bi
         }
     };
     if constexpr (kCapped) {
-        if (beyond) {
+        if (N == kBlk && !kBias && !beyond) {
+            rolled<N>(v, [&](float s, int) { return cap_one(s, a) - ref; });  // (a tile with a mask: the others are capped elsewhere)
+        } else if (beyond) {
             const float d = float(dist);
             rolled<N>(v, [&](float s, int x) { return cap_any(s, a) + (kBias ? fmaf(bias.line, d - float(x), -ref) : -ref); });
         } else {
