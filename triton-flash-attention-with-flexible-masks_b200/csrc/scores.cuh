@@ -123,19 +123,19 @@ struct Bias {
     }
 };
 
-// v[x] = f(v[x], x) for the N values of a thread, 32 at a time, in a loop that moves them all on: for what is rarely done. Unrolled, it would be most of the
+// v[x] = f(v[x], x) for the N values of a thread, kStep at a time, in a loop that moves them all on: for what is rarely done. Unrolled, it would be most of the
 // code of the softmax warps, which is fetched again and again.
-template <int N, class F>
+template <int N, int kStep, class F>
 __device__ __forceinline__ void rolled(float* v, F f) {
 #pragma unroll 1
-    for (int x0 = 0; x0 < N; x0 += 32) {
-        float first[32];
+    for (int x0 = 0; x0 < N; x0 += kStep) {
+        float first[kStep];
 #pragma unroll
-        for (int x = 0; x < 32; ++x) first[x] = f(v[x], x0 + x);
+        for (int x = 0; x < kStep; ++x) first[x] = f(v[x], x0 + x);
 #pragma unroll
-        for (int x = 0; x + 32 < N; ++x) v[x] = v[x + 32];
+        for (int x = 0; x + kStep < N; ++x) v[x] = v[x + kStep];
 #pragma unroll
-        for (int x = 0; x < 32; ++x) v[N - 32 + x] = first[x];
+        for (int x = 0; x < kStep; ++x) v[N - kStep + x] = first[x];
     }
 }
 
@@ -144,6 +144,7 @@ __device__ __forceinline__ void rolled(float* v, F f) {
 template <int KIND, int N>
 __device__ __forceinline__ void score_row(float* v, const ScoreArgs& a, const Bias& bias, float c, int dist, bool real, float ref) {
     constexpr bool kCapped = (KIND & SCORE_CAPPED) != 0, kBias = (KIND & SCORE_BIAS) != 0;
+    constexpr int kStep = kBias ? 16 : 32;  // (with a bias 32 do not fit the registers)
     const bool beyond = kCapped && any_beyond<N>(v, real ? a.most : INFINITY);
     auto each = [&](auto score) {  // score(two scores, what is added to them)
 #pragma unroll
@@ -162,10 +163,10 @@ __device__ __forceinline__ void score_row(float* v, const ScoreArgs& a, const Bi
     };
     if constexpr (kCapped) {
         if (N == kBlk && !kBias && !beyond) {
-            rolled<N>(v, [&](float s, int) { return cap_one(s, a) - ref; });  // (a tile with a mask: the others are capped elsewhere)
+            rolled<N, kStep>(v, [&](float s, int) { return cap_one(s, a) - ref; });  // (a tile with a mask: the others are capped elsewhere)
         } else if (beyond) {
             const float d = float(dist);
-            rolled<N>(v, [&](float s, int x) { return cap_any(s, a) + (kBias ? fmaf(bias.line, d - float(x), -ref) : -ref); });
+            rolled<N, kStep>(v, [&](float s, int x) { return cap_any(s, a) + (kBias ? fmaf(bias.line, d - float(x), -ref) : -ref); });
         } else {
             each([&](uint64_t s2, uint64_t b2) { return fma_f2(s2, cap_poly(s2, a), b2); });
         }
@@ -174,7 +175,7 @@ __device__ __forceinline__ void score_row(float* v, const ScoreArgs& a, const Bi
     }
     if (kBias && bias.both) {
         const float d = float(dist);
-        rolled<N>(v, [&](float y, int x) { return fmaf(bias.s, fabsf(d - float(x)), y); });
+        rolled<N, kStep>(v, [&](float y, int x) { return fmaf(bias.s, fabsf(d - float(x)), y); });
     }
 }
 
@@ -182,7 +183,7 @@ __device__ __forceinline__ void score_row(float* v, const ScoreArgs& a, const Bi
 template <int N>
 __device__ __forceinline__ void cap_scores(float* v, const ScoreArgs& a) {
     if (any_beyond<N>(v, a.most)) {
-        rolled<N>(v, [&](float s, int) { return cap_any(s, a); });
+        rolled<N, 16>(v, [&](float s, int) { return cap_any(s, a); });
     } else {
 #pragma unroll
         for (int x = 0; x < N; x += 2) {
