@@ -177,13 +177,16 @@ typedef struct fa_scores {
 
 /* fa_plan_build, fa_fwd_split (splits = 1: fa_fwd) and fa_bwd of a call with such scores: the same arguments and rules. The plan of a call
  * with ids must have been built with the same prefix; without ids fa_plan_build's will do. With M <= 64 and no ids the heads of a group share
- * tiles and fa_fwd_splits says into how many runs the keys are best cut, as for fa_fwd_split. */
+ * tiles and fa_fwd_splits says into how many runs the keys are best cut, as for fa_fwd_split.
+ * rest: NULL, or (16-bit types, some change of the scores, splits = 1) a contiguous [B, H, M, D] buffer of the type, 16-byte aligned, that the forward fills with
+ * what the rounding of o has left out and the backward adds to it: dq and dk are then as exact as their own rounding lets them also where a few
+ * keys carry a row. */
 int fa_plan_build_scored(const fa_problem* p, const fa_scores* scores, const fa_ids* eq, const fa_ids* ek, void* plan, size_t plan_bytes,
                          int32_t* status, void* stream);
-int fa_fwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
+int fa_fwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o, void* rest,
                   float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 int fa_bwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
-                  const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv,
+                  const void* rest, const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv,
                   const void* plan, int32_t* status, void* stream);
 
 /* A cache of keys and values in pages, for serving (no counterpart in the reference). k and v are [pages, page_size, Hk, D], 16-bit, with 16-byte

@@ -58,6 +58,7 @@ def attention_64(q, k, v, do, causal, sm_scale, eq, ek, cap, slopes, prefix):
     dv_err = (up + rel + accm) * (p.mT @ DO.abs()) + sub * (seen.mT @ DO.abs())
     dp, delta = DO @ V.mT, (DO * o).sum(-1, keepdim=True)
     dp_err = D * 2.0 ** -23 * (DO.abs() @ V.abs().mT)
+    # (delta takes what the rounding of o leaves out, too)
     delta_err = (DO.abs() * (o_err + D * 2.0 ** -23 * o.abs())).sum(-1, keepdim=True)
     ds = p * (dp - delta) * f
     # f = 1 - tanh^2 is off by some 2^-22 in absolute terms and by the score's error. (f + e)(d + g) - f d = f g + e d + e g: the last term is all there

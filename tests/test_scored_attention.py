@@ -17,8 +17,8 @@ def _problem(**kw):
 def _calls(prob, scores):
     lib = _lib.load()
     t = _lib.Tensor(256, (64 * 64 * 2, 64 * 64, 64, 1))
-    return (lib.fa_fwd_scored(prob, scores, t, t, t, t, 256, None, 1, None, 0, 256, None),
-            lib.fa_bwd_scored(prob, scores, t, t, t, t, t, 256, 256, t, t, t, None, 256, None),
+    return (lib.fa_fwd_scored(prob, scores, t, t, t, t, None, 256, None, 1, None, 0, 256, None),
+            lib.fa_bwd_scored(prob, scores, t, t, t, t, None, t, 256, 256, t, t, t, None, 256, None),
             lib.fa_plan_build_scored(prob, scores, None, None, 256, 512, 256, None))
 
 
@@ -41,7 +41,17 @@ def test_bad_problems_are_refused_as_elsewhere():
     assert _calls(_problem(M=128), s) == (1, 1, 1)
     prob = _problem(M=16, N=1024)
     t = _lib.Tensor(256, (64 * 64 * 2, 64 * 64, 64, 1))
-    assert _lib.load().fa_fwd_scored(prob, s, t, t, t, t, 256, None, 2, None, 0, 256, None) == 6  # no workspace
+    assert _lib.load().fa_fwd_scored(prob, s, t, t, t, t, None, 256, None, 2, None, 0, 256, None) == 6  # no workspace
+
+
+def test_what_a_rounding_leaves_out_is_for_16_bit_calls_with_changed_scores_in_one_run():
+    lib, s, t = _lib.load(), _lib.Scores(1.0, None, None), _lib.Tensor(256, (64 * 64 * 2, 64 * 64, 64, 1))
+    fwd = lambda prob, scores, rest, splits=1: lib.fa_fwd_scored(prob, scores, t, t, t, t, rest, 256, None, splits, 256, 1 << 30, 256, None)  # noqa: E731
+    assert fwd(_problem(dtype=2), s, 256) == 2
+    assert fwd(_problem(M=16, N=1024), s, 256, 2) == 2
+    assert fwd(_problem(), _lib.Scores(0.0, None, None), 256) == 2
+    assert fwd(_problem(), s, 264) == 3
+    assert lib.fa_bwd_scored(_problem(dtype=2), s, t, t, t, t, 256, t, 256, 256, t, t, t, None, 256, None) == 2
 
 
 def test_cpu_tensors_and_bad_arguments_raise():

@@ -337,12 +337,14 @@ int run_plan_build(const fa_problem* p, const fa_scores* sc, const fa_ids* eq, c
     return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
-int run_fwd(const fa_problem* p, const fa_scores* sc, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
+int run_fwd(const fa_problem* p, const fa_scores* sc, void* rest, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
             float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
     int rc = check_problem(p);
     if (rc) return rc;
     if ((rc = check_scores(p, sc))) return rc;
     if (!lse || !status || splits < 1) return FA_ERR_BAD_ARG;
+    if (rest && (p->dtype == FA_FP32 || splits > 1 || score_args(p, sc).kind == fa::SCORE_PLAIN)) return FA_ERR_UNSUPPORTED;
+    if (!aligned16(rest)) return FA_ERR_ALIGNMENT;
     if (!aligned16(lse)) return FA_ERR_ALIGNMENT;
     if (splits > 1) {
         if (p->mode != FA_MODE0_NOPE || p->dtype == FA_FP32 || splits > fa::cdiv(p->N, fa::kBlk)) return FA_ERR_UNSUPPORTED;
@@ -357,6 +359,8 @@ int run_fwd(const fa_problem* p, const fa_scores* sc, const fa_tensor* q, const 
     fa::FwdParams fp;
     if ((rc = make_mask(&fp.mask, p, plan, sc))) return rc;
     fp.score = score_args(p, sc);
+    fp.rest = static_cast<uint16_t*>(rest);
+    fp.rest_d = p->D;
     fp.G = p->H / p->Hk;
     fp.pack = fwd_pack(p);
     fp.ns = splits;
@@ -387,6 +391,29 @@ int run_fwd(const fa_problem* p, const fa_scores* sc, const fa_tensor* q, const 
         fa::CombineParams cp{fp.part_o, fp.part_lse, out_view(o), lse, p->B, p->H, p->M, p->D, dk, splits, fa::pad128(p->M), status};
         e = fa::launch_fwd_combine(p->dtype == FA_BF16, cp, static_cast<cudaStream_t>(stream));
     }
+    return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+int run_bwd_delta(const fa_problem* p, const void* rest, const fa_tensor* o, const fa_tensor* d_o, float* delta, void* stream) {
+    int rc = check_problem(p);
+    if (rc) return rc;
+    if (!delta) return FA_ERR_BAD_ARG;
+    if (!aligned16(delta)) return FA_ERR_ALIGNMENT;
+    if (rest && p->dtype == FA_FP32) return FA_ERR_UNSUPPORTED;
+    if (p->dtype == FA_FP32)
+        return run_f32(1, p, nullptr, nullptr, nullptr, o, d_o, nullptr, nullptr, nullptr, nullptr, delta, nullptr, stream, nullptr);
+    if ((rc = check_tensor(o, p->B, p->H, p->M))) return rc;
+    if ((rc = check_tensor(d_o, p->B, p->H, p->M))) return rc;
+    fa::DeltaParams dp;
+    if (!aligned16(rest)) return FA_ERR_ALIGNMENT;
+    dp.rest = static_cast<const uint16_t*>(rest);
+    dp.o = out_view(o);
+    dp.d_o = out_view(d_o);
+    dp.delta = delta;
+    dp.B = p->B; dp.H = p->H; dp.M = p->M; dp.D = p->D;
+    dp.Mpad = fa::pad128(p->M);
+    dp.bf16 = p->dtype == FA_BF16;
+    const cudaError_t e = fa::launch_bwd_delta(dp, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
@@ -588,32 +615,16 @@ int fa_fwd(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa
 int fa_fwd_split(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
                  float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status,
                  void* stream) {
-    return run_fwd(p, nullptr, q, k, v, o, lse, plan, splits, workspace, workspace_bytes, status, stream);
+    return run_fwd(p, nullptr, nullptr, q, k, v, o, lse, plan, splits, workspace, workspace_bytes, status, stream);
 }
 
-int fa_fwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
+int fa_fwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o, void* rest,
                   float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
-    return scores ? run_fwd(p, scores, q, k, v, o, lse, plan, splits, workspace, workspace_bytes, status, stream) : FA_ERR_BAD_ARG;
+    return scores ? run_fwd(p, scores, rest, q, k, v, o, lse, plan, splits, workspace, workspace_bytes, status, stream) : FA_ERR_BAD_ARG;
 }
 
 int fa_bwd_delta(const fa_problem* p, const fa_tensor* o, const fa_tensor* d_o, float* delta, void* stream) {
-    int rc = check_problem(p);
-    if (rc) return rc;
-    if (!delta) return FA_ERR_BAD_ARG;
-    if (!aligned16(delta)) return FA_ERR_ALIGNMENT;
-    if (p->dtype == FA_FP32)
-        return run_f32(1, p, nullptr, nullptr, nullptr, o, d_o, nullptr, nullptr, nullptr, nullptr, delta, nullptr, stream, nullptr);
-    if ((rc = check_tensor(o, p->B, p->H, p->M))) return rc;
-    if ((rc = check_tensor(d_o, p->B, p->H, p->M))) return rc;
-    fa::DeltaParams dp;
-    dp.o = out_view(o);
-    dp.d_o = out_view(d_o);
-    dp.delta = delta;
-    dp.B = p->B; dp.H = p->H; dp.M = p->M; dp.D = p->D;
-    dp.Mpad = fa::pad128(p->M);
-    dp.bf16 = p->dtype == FA_BF16;
-    const cudaError_t e = fa::launch_bwd_delta(dp, static_cast<cudaStream_t>(stream));
-    return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+    return run_bwd_delta(p, nullptr, o, d_o, delta, stream);
 }
 
 int fa_bwd_dkdv(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v,
@@ -638,12 +649,12 @@ int fa_bwd(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa
 }
 
 int fa_bwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
-                  const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv,
+                  const void* rest, const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv,
                   const void* plan, int32_t* status, void* stream) {
     if (!scores) return FA_ERR_BAD_ARG;
     int rc = check_problem(p);
     if (!rc) rc = check_scores(p, scores);
-    if (!rc) rc = fa_bwd_delta(p, o, d_o, delta, stream);
+    if (!rc) rc = run_bwd_delta(p, rest, o, d_o, delta, stream);
     if (!rc) rc = run_bwd_dkdv(p, scores, q, k, v, d_o, lse, delta, dk, dv, plan, status, stream);
     if (!rc) rc = run_bwd_dq(p, scores, q, k, v, d_o, lse, delta, dq, plan, status, true, stream);
     return rc;

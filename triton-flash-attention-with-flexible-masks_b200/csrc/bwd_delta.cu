@@ -20,7 +20,8 @@ struct DeltaShape {
     static constexpr int kBlockRows = kStep * kRows;
 };
 
-template <int D, bool BF16>
+// REST: what the rounding of O has left out is added to it.
+template <int D, bool BF16, bool REST = false>
 __global__ void __launch_bounds__(256) bwd_delta_kernel(const DeltaParams p) {
     using S = DeltaShape<D>;
     follow_stream();
@@ -29,7 +30,7 @@ __global__ void __launch_bounds__(256) bwd_delta_kernel(const DeltaParams p) {
     const int part = int(threadIdx.x) % S::kLanes;
     const uint16_t* po = static_cast<const uint16_t*>(p.o.ptr) + int64_t(b) * p.o.sb + int64_t(h) * p.o.sh + part * 8;
     const uint16_t* pd = static_cast<const uint16_t*>(p.d_o.ptr) + int64_t(b) * p.d_o.sb + int64_t(h) * p.d_o.sh + part * 8;
-    uint4 a[S::kRows], g[S::kRows];
+    uint4 a[S::kRows], g[S::kRows], e[S::kRows];
 #pragma unroll
     for (int r = 0; r < S::kRows; ++r) {
         const int row = row0 + r * S::kStep;
@@ -37,6 +38,9 @@ __global__ void __launch_bounds__(256) bwd_delta_kernel(const DeltaParams p) {
         if (row < p.M) {
             a[r] = *reinterpret_cast<const uint4*>(po + int64_t(row) * p.o.sl);
             g[r] = *reinterpret_cast<const uint4*>(pd + int64_t(row) * p.d_o.sl);
+            if constexpr (REST) e[r] = *reinterpret_cast<const uint4*>(p.rest + ((int64_t(b) * p.H + h) * p.M + row) * D + part * 8);
+        } else if constexpr (REST) {
+            e[r] = make_uint4(0, 0, 0, 0);
         }
     }
 #pragma unroll
@@ -56,6 +60,13 @@ __global__ void __launch_bounds__(256) bwd_delta_kernel(const DeltaParams p) {
                 a0 = __low2float(ah); a1 = __high2float(ah);
                 g0 = __low2float(gh); g1 = __high2float(gh);
             }
+            if constexpr (REST) {
+                const uint32_t ew[4] = {e[r].x, e[r].y, e[r].z, e[r].w};
+                float e0, e1;
+                unpack2<BF16>(ew[k], e0, e1);
+                a0 += e0;
+                a1 += e1;
+            }
             acc = fmaf(a0, g0, acc);
             acc = fmaf(a1, g1, acc);
         }
@@ -69,6 +80,7 @@ __global__ void __launch_bounds__(256) bwd_delta_kernel(const DeltaParams p) {
 template <int D>
 static cudaError_t launch_delta_t(const DeltaParams& p, cudaStream_t stream) {
     const dim3 grid(unsigned((p.Mpad + DeltaShape<D>::kBlockRows - 1) / DeltaShape<D>::kBlockRows), p.H, p.B);
+    if (p.rest) return launch_overlapping(p.bf16 ? bwd_delta_kernel<D, true, true> : bwd_delta_kernel<D, false, true>, grid, DeltaShape<D>::kThreads, 0, stream, p);
     return launch_overlapping(p.bf16 ? bwd_delta_kernel<D, true> : bwd_delta_kernel<D, false>, grid, DeltaShape<D>::kThreads, 0, stream, p);
 }
 

@@ -534,6 +534,11 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                 if (ns > 1 && valid && healthy)
                     part = p.part_o + ((int64_t(j % ns) * p.B * p.H + int64_t(b) * p.H + int64_t(h / nG) * p.G + g_own) * mk.M + row) * D;
             }
+            uint16_t* rest = nullptr;  // this thread's row of it
+            if constexpr (KIND != SCORE_PLAIN) {
+                if (p.rest && row < mk.M && valid && healthy)
+                    rest = p.rest + ((int64_t(b) * p.H + (SHORT ? int64_t(h / nG) * p.G + g_own : h)) * mk.M + row) * p.rest_d;
+            }
             // The O tile is staged in this item's Q slot (Q is dead: every S MMA of the item has completed) in the
             // 128-byte-swizzled layout of the tensor map.
             uint8_t* stage = smem + S::off_q + s * S::TILE;
@@ -566,6 +571,22 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     }
                 }
                 auto two = [&](int y) { return pack2<BF16>(__uint_as_float(x0[y]), __uint_as_float(x0[y + 1])); };
+                if constexpr (KIND != SCORE_PLAIN) {
+                    // What the rounding of O leaves out, for delta = rowsum(dO O): where a few keys carry a row, the error that a rounded O has there reaches dQ and dK
+                    // as large as their own rounding (scores of deviation 4, bf16, dQ off by 3.8e-3 of its size without this, 2.4e-3 with it).
+                    if (rest && 16 * q < p.rest_d) {
+                        uint32_t lo[8];
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) {
+                            float r0, r1;
+                            unpack2<BF16>(two(2 * y), r0, r1);
+                            lo[y] = pack2<BF16>(__uint_as_float(x0[2 * y]) - r0, __uint_as_float(x0[2 * y + 1]) - r1);
+                        }
+                        uint4* dst = reinterpret_cast<uint4*>(rest + 16 * q);
+                        dst[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        dst[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int cg = 2 * q + i;  // 16-byte chunk of the row

@@ -116,11 +116,12 @@ Tensor plan(uintptr_t problem, const std::optional<Tensor>& eq, const std::optio
 struct Outputs {
     Tensor o, lse;
     int splits;
+    Tensor rest;  // of a call of attention_scored that needs a gradient: what the rounding of o has left out
 };
 
 // The forward's allocations and launches for a problem that `regular` has filled.
 Outputs launch_forward(const fa_problem& p, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& plan, int key_runs,
-                       const Tensor& status, const std::optional<Tensor>& out, const fa_scores* scores = nullptr) {
+                       const Tensor& status, const std::optional<Tensor>& out, const fa_scores* scores = nullptr, bool backward = false) {
     Outputs r;
     r.o = out ? *out : at::empty_like(q);
     if (!taken_as_is(r.o)) r.o = at::empty(q.sizes(), q.options());
@@ -136,8 +137,9 @@ Outputs launch_forward(const fa_problem& p, const Tensor& q, const Tensor& k, co
     const fa_tensor tq = view(q), tk = view(k), tv = view(v), to = view(r.o);
     void* const plan_ptr = plan.defined() ? plan.data_ptr() : nullptr;
     void* const work_ptr = work.defined() ? work.data_ptr() : nullptr;
+    if (scores && backward && r.splits == 1 && p.dtype != FA_FP32) r.rest = at::empty({p.B, p.H, p.M, p.D}, q.options());
     if (scores)
-        check(fa_fwd_scored(&p, scores, &tq, &tk, &tv, &to, r.lse.data_ptr<float>(), plan_ptr, r.splits, work_ptr, bytes, status.data_ptr<int>(),
+        check(fa_fwd_scored(&p, scores, &tq, &tk, &tv, &to, r.rest.defined() ? r.rest.data_ptr() : nullptr, r.lse.data_ptr<float>(), plan_ptr, r.splits, work_ptr, bytes, status.data_ptr<int>(),
                             current_stream(q)),
               "fa_fwd_scored");
     else
@@ -149,14 +151,14 @@ Outputs launch_forward(const fa_problem& p, const Tensor& q, const Tensor& k, co
 // dq, dk, dv. q, k, v, o, lse and the problem are those of a forward, d_o is like q.
 std::array<Tensor, 3> launch_backward(const fa_problem& p, const Tensor& d_o, const Tensor& q, const Tensor& k, const Tensor& v,
                                       const Tensor& o, const Tensor& lse, const Tensor& plan, const Tensor& status,
-                                      const fa_scores* scores = nullptr) {
+                                      const fa_scores* scores = nullptr, const Tensor& rest = Tensor()) {
     Tensor delta = at::empty_like(lse);
     Tensor dk = at::empty({p.B, p.Hk, p.N, p.D}, k.options()), dv = at::empty({p.B, p.Hk, p.N, p.D}, v.options());
     Tensor dq = at::empty(q.sizes(), q.options());
     const fa_tensor tq = view(q), tk = view(k), tv = view(v), to = view(o), tdo = view(d_o), tdq = view(dq), tdk = view(dk), tdv = view(dv);
     void* const plan_ptr = plan.defined() ? plan.data_ptr() : nullptr;
     if (scores)
-        check(fa_bwd_scored(&p, scores, &tq, &tk, &tv, &to, &tdo, lse.data_ptr<float>(), delta.data_ptr<float>(), &tdq, &tdk, &tdv, plan_ptr,
+        check(fa_bwd_scored(&p, scores, &tq, &tk, &tv, &to, rest.defined() ? rest.data_ptr() : nullptr, &tdo, lse.data_ptr<float>(), delta.data_ptr<float>(), &tdq, &tdk, &tdv, plan_ptr,
                             status.data_ptr<int>(), current_stream(q)),
               "fa_bwd_scored");
     else
@@ -311,7 +313,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
     static Outputs launch(const Tensor& q, const Tensor& k, const Tensor& v, const Call& c, const fa_scores& s, Tensor& plan) {
         py::gil_scoped_release free;
         if (c.eq || !fa_plan_optional(&c.p, c.needs_grad)) plan = build_plan(c.p, c.eq, c.ek, c.status, &s);
-        Outputs r = launch_forward(c.p, q, k, v, plan, 0, c.status, std::nullopt, &s);
+        Outputs r = launch_forward(c.p, q, k, v, plan, 0, c.status, std::nullopt, &s, c.needs_grad);
         n_launched += (plan.defined() ? c.plan_kernels : 0) + (r.splits > 1 ? 2 : 1);
         return r;
     }
@@ -332,6 +334,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
         data["scale"] = c.sm_scale;
         data["softcap"] = double(sc.s.softcap);
         data["slopes"] = sc.slopes.has_value();
+        data["rest"] = r.rest;
         return r.o;
     }
 
@@ -354,7 +357,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
         d_o = d_o.resolve_neg();
         TORCH_CHECK(like_query(d_o, q), "flash_b200: the gradient is not a plain [bs, H, M, D] CUDA tensor");
         if (!taken_as_is(d_o)) d_o = d_o.contiguous();  // (ops.maybe_contiguous)
-        auto g = launch_backward(p, d_o, q, k, v, saved[3], saved[4], data["plan"].toTensor(), data["status"].toTensor(), &s);
+        auto g = launch_backward(p, d_o, q, k, v, saved[3], saved[4], data["plan"].toTensor(), data["status"].toTensor(), &s, data["rest"].toTensor());
         n_launched += 3;
         return {std::move(g[0]), std::move(g[1]), std::move(g[2]), Tensor(), Tensor()};
     }

@@ -27,6 +27,8 @@ struct FwdParams {
     float* part_o;    // [ns, B, H, M, 64 or 128] normalised rows of each run (ns > 1)
     float* part_lse;  // [B, H, M, ns]
     ScoreArgs score;  // the instances for attention_scored
+    uint16_t* rest;   // and there, or null: [B, H, M, rest_d] what the rounding of O has left out, rounded itself
+    int rest_d;       // head dim
 };
 
 struct CombineParams {
@@ -41,6 +43,7 @@ struct CombineParams {
 
 struct DeltaParams {
     OutTensor o, d_o;
+    const uint16_t* rest;  // of a forward of attention_scored, or null
     float* delta;  // [B, H, Mpad]
     int B, H, M, D;
     int64_t Mpad;

@@ -413,6 +413,16 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return r;
 }
 
+template <bool BF16>
+__device__ __forceinline__ void unpack2(uint32_t x, float& lo, float& hi) {
+    if constexpr (BF16) {
+        lo = __uint_as_float(x << 16);
+        hi = __uint_as_float(x & 0xffff0000u);
+    } else {
+        asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(lo), "=f"(hi) : "r"(x));
+    }
+}
+
 }  // namespace fa
 
 namespace fa {

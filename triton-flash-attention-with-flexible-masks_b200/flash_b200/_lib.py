@@ -99,9 +99,9 @@ def load():
     lib.fa_plan_build_scored.restype = i32
     lib.fa_plan_build_scored.argtypes = [P, S, I, I, vp, size, vp, vp]
     lib.fa_fwd_scored.restype = i32
-    lib.fa_fwd_scored.argtypes = [P, S, T, T, T, T, vp, vp, ctypes.c_int32, vp, size, vp, vp]
+    lib.fa_fwd_scored.argtypes = [P, S, T, T, T, T, vp, vp, vp, ctypes.c_int32, vp, size, vp, vp]
     lib.fa_bwd_scored.restype = i32
-    lib.fa_bwd_scored.argtypes = [P, S, T, T, T, T, T, vp, vp, T, T, T, vp, vp, vp]
+    lib.fa_bwd_scored.argtypes = [P, S, T, T, T, T, vp, T, vp, vp, T, T, T, vp, vp, vp]
     C, R = ctypes.POINTER(PagedCache), ctypes.POINTER(Rows)
     lib.fa_paged_append.restype = i32
     lib.fa_paged_append.argtypes = [C, ctypes.c_int32, vp, R, R, vp, vp]

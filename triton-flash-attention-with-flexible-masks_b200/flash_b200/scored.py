@@ -57,8 +57,12 @@ def _native(*tensors):
     return None
 
 
+def _pointer(x):
+    return None if x is None else x.data_ptr()
+
+
 def _scores(softcap, slopes, prefix):
-    return _lib.Scores(softcap, None if slopes is None else slopes.data_ptr(), None if prefix is None else prefix.data_ptr())
+    return _lib.Scores(softcap, _pointer(slopes), _pointer(prefix))
 
 
 class ScoredAttention(torch.autograd.Function):
@@ -95,16 +99,18 @@ class ScoredAttention(torch.autograd.Function):
             if splits > 1:
                 _lib.check(lib.fa_fwd_workspace_bytes(prob, splits, size), "fa_fwd_workspace_bytes")
                 work = torch.empty(size.value // 4, dtype=torch.float32, device=device)
+            # what the rounding of the output leaves out, for the gradients
+            rest = torch.empty((B, H, M, D), dtype=q.dtype, device=device) if needs_grad and splits == 1 and q.dtype != torch.float32 else None
             with ops._timed("fwd", 2 if splits > 1 else 1):
-                _lib.check(lib.fa_fwd_scored(prob, scores, _tensor(q), _tensor(k), _tensor(v), _tensor(out), lse.data_ptr(),
-                                             None if plan is None else plan.data_ptr(), splits, None if work is None else work.data_ptr(),
+                _lib.check(lib.fa_fwd_scored(prob, scores, _tensor(q), _tensor(k), _tensor(v), _tensor(out), _pointer(rest), lse.data_ptr(),
+                                             _pointer(plan), splits, _pointer(work),
                                              size.value, status.data_ptr(), stream), "fa_fwd_scored")
             if ops._SYNC_STATUS:
                 check_status(device)
         if needs_grad:
             ctx.save_for_backward(q, k, v, out, lse, *(x for x in (slopes, prefix) if x is not None))
             ctx.has = slopes is not None, prefix is not None
-            ctx.plan, ctx.prob, ctx.softcap = plan, prob, softcap
+            ctx.plan, ctx.prob, ctx.softcap, ctx.rest = plan, prob, softcap, rest
         return out
 
     @staticmethod
@@ -117,8 +123,8 @@ class ScoredAttention(torch.autograd.Function):
         with _current(device):
             delta = torch.empty_like(lse)
             dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
-            _lib.check(lib.fa_bwd_scored(ctx.prob, _scores(ctx.softcap, slopes, prefix), *map(_tensor, (q, k, v, out, do)), lse.data_ptr(), delta.data_ptr(),
-                                         *map(_tensor, (dq, dk, dv)), None if plan is None else plan.data_ptr(), _status_word(device).data_ptr(),
+            _lib.check(lib.fa_bwd_scored(ctx.prob, _scores(ctx.softcap, slopes, prefix), *map(_tensor, (q, k, v, out)), _pointer(ctx.rest), _tensor(do),
+                                         lse.data_ptr(), delta.data_ptr(), *map(_tensor, (dq, dk, dv)), _pointer(plan), _status_word(device).data_ptr(),
                                          _stream()), "fa_bwd_scored")
             _count(3)
             if ops._SYNC_STATUS:
