@@ -383,3 +383,39 @@ def test_inference_mode_and_both_ways_through_the_host(monkeypatch):
         for a, b in zip(*results):
             assert torch.equal(a.view(torch.int16), b.view(torch.int16))
         assert torch.equal(results[0][2], results[0][3])
+
+
+def test_after_a_time_out_results_are_nan_until_it_has_been_read():
+    import flash_b200 as fb
+    from flash_b200 import ops
+    cache = Cache([700, 40], 2, 64, 16, BF16, 21).fill()
+    q, new = torch.randn(8, 4, 64, device="cuda").to(BF16), [1, 5]
+    args = (cache.k_pages, cache.v_pages, cache.table, cache.kv_lens, _starts(new))
+    want = fb.paged_attention(q, *args)
+    ops._status_word(q.device).fill_(142)  # as a bounded wait that ran out leaves it
+    assert torch.isnan(fb.paged_attention(q, *args)).all()
+    rows = torch.randn(6, 2, 64, device="cuda").to(BF16)
+    fb.paged_append(rows, rows, *args)  # waits for nothing that can run out
+    place = cache.places(1, 35, 40)
+    assert torch.equal(cache.k_pages[place], rows[1:]) and torch.equal(cache.v_pages[place], rows[1:])
+    with pytest.raises(RuntimeError, match="role 42"):
+        fb.check_status()
+    cache.fill()
+    assert torch.equal(fb.paged_attention(q, *args), want)
+
+
+def test_neighbours_in_a_batch_do_not_reach_a_sequence():
+    """Rows of another sequence in the same tile of queries, NaN among them, and what an earlier call left in shared memory."""
+    import flash_b200 as fb
+    cache = Cache([130, 130, 130], 2, 64, 16, BF16, 22).fill()
+    new = [40, 3, 40]
+    q = torch.randn(83, 4, 64, device="cuda").to(BF16)
+    call = lambda: fb.paged_attention(q, cache.k_pages, cache.v_pages, cache.table, cache.kv_lens, _starts(new), softcap=3.0)  # noqa: E731
+    want = call()
+    q[:40] = float("nan")
+    q[43:] *= 1e4
+    for _ in range(3):
+        assert torch.equal(call()[40:43], want[40:43])
+    bad = cache.places(2, 0, 130)
+    cache.k_pages[bad], cache.v_pages[bad] = float("nan"), float("nan")
+    assert torch.equal(call()[40:43], want[40:43])

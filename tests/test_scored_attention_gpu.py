@@ -311,3 +311,38 @@ def test_saved_tensors_that_change_are_noticed():
         kw[victim].add_(1)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             o.backward(do)
+
+
+def _with_a_time_out_on_record():
+    """The status word as a bounded wait that ran out leaves it (nothing waits, faults or hangs here)."""
+    from flash_b200 import ops
+    ops._status_word(torch.device("cuda", torch.cuda.current_device())).fill_(142)
+
+
+def test_after_a_time_out_results_are_nan_until_it_has_been_read():
+    import flash_b200 as fb
+    q, k, v, do = _inputs(1, 4, 2, 300, 300, 64, BF16, 43)
+    for kw in (dict(softcap=9.0), dict(slopes=_slopes(4, "series")), dict(prefix=torch.tensor([70], dtype=torch.int32, device="cuda"))):
+        a, b, c = (x.detach().requires_grad_() for x in (q, k, v))
+        o = fb.attention_scored(a, b, c, True, **kw)
+        want = torch.autograd.grad(o, (a, b, c), do, retain_graph=True)
+        _with_a_time_out_on_record()
+        lost = fb.attention_scored(q, k, v, True, **kw)
+        grads = torch.autograd.grad(o, (a, b, c), do, retain_graph=True)
+        assert all(torch.isnan(x).all() for x in (lost, *grads))
+        with pytest.raises(RuntimeError, match="role 42"):
+            fb.check_status()
+        assert torch.equal(fb.attention_scored(q, k, v, True, **kw), o)
+        assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(o, (a, b, c), do), want))
+
+
+def test_gradients_where_a_few_keys_carry_a_row():
+    """Scores of deviation 9. Each of dQ's and dK's two roundings (of dS and of the result) is off by u / sqrt(3) at most in the mean square, u = 2^-8; delta adds what
+    the rounding of P puts into O, as much again at most: 1.75 u / sqrt(3) = 3.9e-3 of the whole, where a delta from the rounded O alone had 4.5e-3."""
+    import flash_b200 as fb
+    q, k, v, do = _inputs(1, 4, 4, 1024, 1024, 128, BF16, 44, std=3.0)
+    got = _run(fb, q, k, v, do, True, cap=50.0)
+    want = attention_64(q, k, v, do, True, None, None, None, 50.0, None, None)
+    for name in ("dq", "dk"):
+        value = want[name][0]
+        assert ((got[name].double() - value).norm() / value.norm()).item() < 3.9e-3, name

@@ -146,6 +146,10 @@ __device__ __forceinline__ void score_row(float* v, const ScoreArgs& a, const Bi
     constexpr bool kCapped = (KIND & SCORE_CAPPED) != 0, kBias = (KIND & SCORE_BIAS) != 0;
     constexpr int kStep = kBias ? 16 : 32;  // (with a bias 32 do not fit the registers)
     const bool beyond = kCapped && any_beyond<N>(v, real ? a.most : INFINITY);
+    if (KIND == SCORE_BIAS && bias.both) {  // (in front of what follows it costs the other tiles less)
+        const float d = float(dist), e = bias.s / c;
+        rolled<N, kStep>(v, [&](float y, int x) { return fmaf(e, fabsf(d - float(x)), y); });
+    }
     auto each = [&](auto score) {  // score(two scores, what is added to them)
 #pragma unroll
         for (int q = 0; q < N; q += 32) {
@@ -173,7 +177,7 @@ __device__ __forceinline__ void score_row(float* v, const ScoreArgs& a, const Bi
     } else {
         each([&](uint64_t s2, uint64_t b2) { return fma_f2(s2, pack_f2(c, c), b2); });
     }
-    if (kBias && bias.both) {
+    if (KIND == SCORE_CAPPED_BIAS && bias.both) {
         const float d = float(dist);
         rolled<N, kStep>(v, [&](float y, int x) { return fmaf(bias.s, fabsf(d - float(x)), y); });
     }
