@@ -1,4 +1,5 @@
 """attention_scored against the plain computation in 64 bits, element by element within bounds derived from the roundings (scored_reference.py)."""
+import contextlib
 import itertools
 
 import pytest
@@ -346,3 +347,19 @@ def test_gradients_where_a_few_keys_carry_a_row():
     for name in ("dq", "dk"):
         value = want[name][0]
         assert ((got[name].double() - value).norm() / value.norm()).item() < 3.9e-3, name
+
+
+def test_what_the_node_saves_is_freed_with_its_gradients():
+    """Between the call and the end of this test the output and the gradient of q stay; the LSE and what the rounding of the output has left out do not."""
+    import flash_b200 as fb
+    q, k, v, do = _inputs(1, 8, 8, 1024, 1024, 128, BF16, 61)
+    size = q.numel() * q.element_size()
+    for hooked in (False, True):  # the native node, and the one in Python
+        a = q.detach().requires_grad_()
+        before = torch.cuda.memory_allocated()
+        with (torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: x) if hooked else contextlib.nullcontext()):
+            o = fb.attention_scored(a, k, v, True, softcap=20.0)
+        o.backward(do)
+        torch.cuda.synchronize()
+        assert 2 * size <= torch.cuda.memory_allocated() - before < 2 * size + size // 2
+        del o, a

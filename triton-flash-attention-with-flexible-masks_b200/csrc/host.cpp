@@ -324,6 +324,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
         torch::autograd::variable_list saved{q, k, v, r.o, r.lse};
         if (sc.slopes) saved.push_back(*sc.slopes);
         if (sc.prefix) saved.push_back(*sc.prefix);
+        if (r.rest.defined()) saved.push_back(r.rest);
         ctx->save_for_backward(std::move(saved));
         auto& data = ctx->saved_data;
         data["plan"] = plan;
@@ -334,7 +335,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
         data["scale"] = c.sm_scale;
         data["softcap"] = double(sc.s.softcap);
         data["slopes"] = sc.slopes.has_value();
-        data["rest"] = r.rest;
+        data["prefix"] = sc.prefix.has_value();
         return r.o;
     }
 
@@ -348,16 +349,16 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
                             int(data["id_heads"].toInt()), p),
                     "flash_b200: the saved q, k, v are not plain [bs, H, L, D] CUDA tensors of matching shapes");
         size_t at = 5;
-        const bool slopes = data["slopes"].toBool();
         fa_scores s{float(data["softcap"].toDouble()), nullptr, nullptr};
-        if (slopes) s.slopes = saved[at++].const_data_ptr<float>();
-        if (saved.size() > at) s.prefix = saved[at].const_data_ptr<int>();
+        if (data["slopes"].toBool()) s.slopes = saved[at++].const_data_ptr<float>();
+        if (data["prefix"].toBool()) s.prefix = saved[at++].const_data_ptr<int>();
+        const Tensor rest = saved.size() > at ? saved[at] : Tensor();
         Tensor d_o = grads[0];
         if (d_o.scalar_type() != q.scalar_type()) d_o = d_o.to(q.scalar_type());
         d_o = d_o.resolve_neg();
         TORCH_CHECK(like_query(d_o, q), "flash_b200: the gradient is not a plain [bs, H, M, D] CUDA tensor");
         if (!taken_as_is(d_o)) d_o = d_o.contiguous();  // (ops.maybe_contiguous)
-        auto g = launch_backward(p, d_o, q, k, v, saved[3], saved[4], data["plan"].toTensor(), data["status"].toTensor(), &s, data["rest"].toTensor());
+        auto g = launch_backward(p, d_o, q, k, v, saved[3], saved[4], data["plan"].toTensor(), data["status"].toTensor(), &s, rest);
         n_launched += 3;
         return {std::move(g[0]), std::move(g[1]), std::move(g[2]), Tensor(), Tensor()};
     }

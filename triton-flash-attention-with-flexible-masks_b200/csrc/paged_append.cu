@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Page
     }
 }
 
-// strides[12]: k rows (token, head), v rows, k pages (page, slot, head), v pages, in 16 bytes (called from paged.cu)
+// strides[10]: k rows (token, head), v rows, k pages (page, slot, head), v pages, in 16 bytes (called from paged.cu)
 cudaError_t launch_paged_append(const PagedParams& p, const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* strides, cudaStream_t stream) {
     const AppendRows in{static_cast<const uint4*>(k), static_cast<const uint4*>(v), strides[0], strides[1], strides[2], strides[3]};
     const AppendPages to{static_cast<uint4*>(k_pages), static_cast<uint4*>(v_pages), strides[4], strides[5], strides[6], strides[7], strides[8], strides[9]};

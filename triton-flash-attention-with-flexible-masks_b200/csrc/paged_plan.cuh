@@ -314,6 +314,7 @@ __host__ __device__ __forceinline__ int paged_pieces(const PagedParams& p, const
     // the cuts lie a stretch apart: the last one before the item's last tile ends
     const long long end = walk.end(p, plan);
     v += int(paged_divide(end - 1 - paged_cut(plan, w), plan.stretch));
+    v = v < plan.workers ? v : plan.workers - 1;  // (somebody writes the lengths while the kernel reads them)
     if (walk.key_tile_at(p, plan, paged_cut(plan, v)) >= n) --v;
     return v - from + 1;
 }

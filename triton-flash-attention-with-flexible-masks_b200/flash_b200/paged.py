@@ -74,7 +74,8 @@ def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None):
     j % page size of page page_table[b, j // page size] (int32 [B, pages of a sequence]; entries behind a sequence's last page may hold anything).
     kv_lens: int32 [B], how many tokens each sequence has, the new ones among them. q_starts: int32 [B + 1], non-decreasing: the rows q_starts[b] to
     q_starts[b + 1] are sequence b's last tokens; None: one row a sequence. Rows of no sequence are left out, and so are new tokens in
-    front of a sequence's beginning (more rows than kv_lens).
+    front of a sequence's beginning (more rows than kv_lens). The places that are written share no memory with k and v, and where two rows go to one place either may
+    stay.
 
     All lengths and tables are read on the device, so that a captured call follows them. A page number or a length that the cache does not have
     writes nothing and is reported by `check_status`."""
@@ -122,7 +123,8 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_
 
     Returns [T, H, D], zeros in the rows of no sequence; or `out`, whose rows of no sequence are left as they were. `out` shares no memory with q
     or the cache. What lies in the pages behind a sequence's length, or in pages that no sequence names, has no influence, also
-    if it is not finite. How the work is cut goes by all lengths of the batch, so that the last bits of a sequence's rows can differ with what
+    if it is not finite; a value that some row of a block sees (a block is the heads of a group and up to 128 / G neighbouring tokens of a sequence) may spread in it if it is
+    not finite. How the work is cut goes by all lengths of the batch, so that the last bits of a sequence's rows can differ with what
     it is batched with."""
     softcap = _checked_softcap(softcap)
     if sm_scale is None or type(sm_scale) is float:

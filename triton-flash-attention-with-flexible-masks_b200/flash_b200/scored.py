@@ -66,7 +66,8 @@ def _scores(softcap, slopes, prefix):
 
 
 class ScoredAttention(torch.autograd.Function):
-    """The autograd node of `attention_scored`. Saves q, k, v, the output, its log-sum-exp, and the slopes and prefix that there are."""
+    """The autograd node of `attention_scored`. Saves q, k, v, the output, its log-sum-exp, the slopes and prefix that there are, and what the rounding
+    of the output has left out."""
 
     @staticmethod
     def forward(ctx, q, k, v, causal, sm_scale, eq, ek, score_func_mode, softcap, slopes, prefix):
@@ -108,22 +109,23 @@ class ScoredAttention(torch.autograd.Function):
             if ops._SYNC_STATUS:
                 check_status(device)
         if needs_grad:
-            ctx.save_for_backward(q, k, v, out, lse, *(x for x in (slopes, prefix) if x is not None))
-            ctx.has = slopes is not None, prefix is not None
-            ctx.plan, ctx.prob, ctx.softcap, ctx.rest = plan, prob, softcap, rest
+            extra = slopes, prefix, rest
+            ctx.save_for_backward(q, k, v, out, lse, *(x for x in extra if x is not None))
+            ctx.has = tuple(x is not None for x in extra)
+            ctx.plan, ctx.prob, ctx.softcap = plan, prob, softcap
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, out, lse, *rest = ctx.saved_tensors
-        slopes, prefix = (rest.pop(0) if has else None for has in ctx.has)
+        q, k, v, out, lse, *extra = ctx.saved_tensors
+        slopes, prefix, rest = (extra.pop(0) if has else None for has in ctx.has)
         lib, device, plan = _lib.load(), q.device, ctx.plan
         do = maybe_contiguous(do.to(q.dtype))
         with _current(device):
             delta = torch.empty_like(lse)
             dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
-            _lib.check(lib.fa_bwd_scored(ctx.prob, _scores(ctx.softcap, slopes, prefix), *map(_tensor, (q, k, v, out)), _pointer(ctx.rest), _tensor(do),
+            _lib.check(lib.fa_bwd_scored(ctx.prob, _scores(ctx.softcap, slopes, prefix), *map(_tensor, (q, k, v, out)), _pointer(rest), _tensor(do),
                                          lse.data_ptr(), delta.data_ptr(), *map(_tensor, (dq, dk, dv)), _pointer(plan), _status_word(device).data_ptr(),
                                          _stream()), "fa_bwd_scored")
             _count(3)
