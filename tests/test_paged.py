@@ -97,7 +97,8 @@ def test_work_is_even():
     loads = _check(lens, [1] * 64, 8, 4, 148)
     assert len(loads) == 148 and max(loads.values()) <= 1.15 * sum(loads.values()) / 148 + 2
     loads = _check([131072], [1], 8, 8, 148)
-    assert len(loads) == 148 and max(loads.values()) - min(loads.values()) <= 4
+    # stretches of equal length: a tile more or less at either end, and 640 / 128 = 5 tiles less where an item begins
+    assert len(loads) == 148 and max(loads.values()) - min(loads.values()) <= 2 + 5
 
 
 def test_lengths_beyond_everything_stay_inside():

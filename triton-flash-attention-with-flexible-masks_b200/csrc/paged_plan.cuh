@@ -5,7 +5,9 @@
 // number of keys that its last token sees, and a constant for what an item costs besides its tiles. The items, in the order sequence, kv head,
 // tile, lie behind one another on a line of length `total`, and each of n workers gets an equal stretch of it, whatever the lengths, with at most
 // n - 1 cuts. An item that a cut goes through is computed in pieces, whose fp32 rows the second kernel merges.
-// Where whole items, one a worker, are done as soon, nothing is cut (`keyed` false: all weights are 1).
+// Where there are no more items than workers and whole items, one a worker, are done as soon, nothing is cut (`keyed` false: all weights are 1):
+// merging costs what some tiles cost. Whole | cut, us, 32 / 8 heads of 128 but for the first: one token behind 699 of 8 heads of 64 15.9 | 20.7, eight behind 300
+// each 16.6 | 33.0, one behind 1500 22.6 | 25.7, one behind 3000 28.9 | 26.3, one behind 131071 879 | 99.
 #pragma once
 #include "common.cuh"
 #include "params.cuh"
@@ -13,10 +15,16 @@
 namespace fa {
 
 constexpr int kPagedGroups = 1024;   // entries of the table of sums: a sequence each, or several
-constexpr int kPagedWarpPlan = 128;  // sequences up to which one warp makes the plan
-constexpr int kPagedItemCost = 256;  // of an item, in keys
-constexpr int kPagedLog2Piece = 10;  // a worker's stretch is at least 2 to this long
-constexpr int kPagedMergeTiles = 6;  // of the second kernel, in tiles of 128 keys
+// Sequences up to which one warp makes the plan, beside which the others go on. One warp | all, us: single tokens of 1 sequence 15.9 | 16.6, of 128 101.0 | 102.0,
+// of 256 179.6 | 179.9, of 512 322 | 318.
+constexpr int kPagedWarpPlan = 128;
+// Of an item besides its tiles, in keys. With 64 | 256 | 640 | 1500, us: 256 single tokens behind up to 1000 189 | 177 | 165 | 167, two chunks of 500 behind 1500
+// 67 | 53 | 43 | 45, twelve sequences with four chunks of 1000 186 | 183 | 174 | 175, one token behind 3000 26.9 | 26.1 | 24.5 | 29.7 (pieces of 2048 there).
+constexpr int kPagedItemCost = 640;
+// A worker's stretch is at least 2 to this long. With 10 | 11 | 12, us: one token behind 3000 26.1 | 30.8 | 29.4, two chunks of 500 behind 1500 53 | 53 | 65.
+constexpr int kPagedLog2Piece = 10;
+// What the second kernel costs, in tiles of 128 keys. With 2 | 6 | 12, us: eight tokens behind 1500 each 30.9 | 24.5 | 24.8.
+constexpr int kPagedMergeTiles = 6;
 
 struct PagedPlan {
     long long total;
