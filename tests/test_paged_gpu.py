@@ -419,3 +419,22 @@ def test_neighbours_in_a_batch_do_not_reach_a_sequence():
     bad = cache.places(2, 0, 130)
     cache.k_pages[bad], cache.v_pages[bad] = float("nan"), float("nan")
     assert torch.equal(call()[40:43], want[40:43])
+
+
+@pytest.mark.parametrize("cap", [None, 3.0])
+@pytest.mark.parametrize("length, at, new", [(97, 96, 1), (97, 0, 1), (300, 130, 1), (20000, 7, 1), (20000, 19999, 1), (500, 400, 150), (20000, 19900, 200)])
+def test_a_row_that_sees_a_key_that_is_not_a_number(length, at, new, cap):
+    """It is NaN, whether the key is the only one of its warp, in a piece of an item, or in a tile of many rows; the rows in front of the key keep their bits."""
+    import flash_b200 as fb
+    cache = Cache([length, 140], 2, 64, 16, BF16, 23).fill()
+    q = torch.randn(new + 1, 4, 64, device="cuda").to(BF16)
+    place = cache.places(0, at, at + 1)
+    call = lambda: fb.paged_attention(q, cache.k_pages, cache.v_pages, cache.table, cache.kv_lens, _starts([new, 1]), softcap=cap)  # noqa: E731
+    cache.k_pages[place] = 0
+    want = call()
+    cache.k_pages[place] = float("nan")
+    got = call()
+    sees = torch.arange(length - new, length, device="cuda") >= at
+    assert torch.equal(got[:new][~sees], want[:new][~sees]) and torch.equal(got[new:], want[new:])
+    assert sees.any() and torch.isnan(got[:new][sees]).all()
+    fb.check_status()

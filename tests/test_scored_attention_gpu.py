@@ -363,3 +363,28 @@ def test_what_the_node_saves_is_freed_with_its_gradients():
         torch.cuda.synchronize()
         assert 2 * size <= torch.cuda.memory_allocated() - before < 2 * size + size // 2
         del o, a
+
+
+@pytest.mark.parametrize("slopes", [None, "series"])
+@pytest.mark.parametrize("times", [0.6, 1.5, 3.9, 12.0])
+@pytest.mark.parametrize("D, dtype", [(64, FP16), (128, BF16)])
+def test_scores_up_to_so_many_caps(times, slopes, D, dtype):
+    """Each form of the tanh by itself, in whole tiles and masked ones."""
+    q, k, v, do = _inputs(1, 2, 2, 300, 300, D, dtype, 62)
+    cap = (q.double() @ k.double().mT).abs().max().item() / D ** 0.5 / times
+    _compare(q, k, v, do, True, cap=cap, slopes=_slopes(2, slopes))
+
+
+@pytest.mark.parametrize("slopes", [None, "series"])
+@pytest.mark.parametrize("cap", [100.0, 3.0, 0.2])
+def test_a_key_that_is_not_a_number_behind_the_mask(cap, slopes):
+    """Rows in front of it have the bits that they have with a key of zeros there, also beside it in a pair of scores."""
+    import flash_b200 as fb
+    for N, at in ((300, 101), (300, 290), (40, 30)):
+        q, k, v, _ = _inputs(1, 2, 1, N, N, 64, BF16, 63)
+        k[:, :, at] = 0
+        with torch.no_grad():
+            want = fb.attention_scored(q, k, v, True, softcap=cap, slopes=_slopes(2, slopes))
+            k[:, :, at] = float("nan")
+            got = fb.attention_scored(q, k, v, True, softcap=cap, slopes=_slopes(2, slopes))
+        assert torch.equal(got[:, :, :at], want[:, :, :at]) and torch.isnan(got[:, :, at:]).all()

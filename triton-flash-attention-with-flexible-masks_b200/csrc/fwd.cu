@@ -507,13 +507,14 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
             const float a0 = (m0 == -INFINITY) ? 0.f : fast_exp2((m0 - mt) * c);
             const float a1 = (m1 == -INFINITY) ? 0.f : fast_exp2((m1 - mt) * c);
             const float lt = l0 * a0 + l1 * a1;
-            const float inv = (lt > 0.f) ? 1.0f / lt : 0.f;
+            // (attention_scored: a NaN among a row's scores makes it NaN; attention's result for such a row is zeros)
+            const float inv = (lt > 0.f) ? 1.0f / lt : KIND == SCORE_PLAIN || lt == lt ? 0.f : lt;
             const float f0 = a0 * inv, f1 = a1 * inv;
             // a chain in which the row had no key takes no part, whatever the values behind its mask are
             const bool use0 = (T > 0) && (f0 != 0.f), use1 = (T > 1) && (f1 != 0.f);
             const bool healthy = misc[1] == 0;
             if (healthy) {
-                const float lse = (lt > 0.f) ? fmaf(mt, c, log2f(lt)) : -INFINITY;
+                const float lse = (lt > 0.f) ? fmaf(mt, c, log2f(lt)) : KIND == SCORE_PLAIN || lt == lt ? -INFINITY : lt;
                 if constexpr (SHORT) {
                     const int64_t bh0 = int64_t(b) * p.H + int64_t(h / nG) * p.G;
                     if (ns > 1) {

@@ -382,11 +382,11 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 lt = 0.f;
                 for (int q = 0; q < 4; ++q) {
                     const float me = ml[even + 32 * q + lane], mo = ml[odd + 32 * q + lane];
-                    lt += (me == -INFINITY ? 0.f : ml[even + kBlk + 32 * q + lane] * fast_exp2((me - mt) * c)) +
-                          (mo == -INFINITY ? 0.f : ml[odd + kBlk + 32 * q + lane] * fast_exp2((mo - mt) * c));
+                    lt += ml[even + kBlk + 32 * q + lane] * (me == -INFINITY ? 0.f : fast_exp2((me - mt) * c)) +
+                          ml[odd + kBlk + 32 * q + lane] * (mo == -INFINITY ? 0.f : fast_exp2((mo - mt) * c));
                 }
             }
-            const float inv = (lt > 0.f) ? 1.0f / lt : 0.f;
+            const float inv = (lt > 0.f) ? 1.0f / lt : lt == lt ? 0.f : lt;  // a NaN among a row's scores makes it NaN
             const float f0 = a0 * inv, f1 = a1 * inv;
             // a chain in which the row had no key takes no part, whatever the values behind its mask are
             const bool use0 = (T > 0) && (f0 != 0.f), use1 = (T > 1) && (f1 != 0.f);
