@@ -28,7 +28,7 @@ def attention_64(q, k, v, do, causal, sm_scale, eq, ek, cap, slopes, prefix):
     if cap:
         t = torch.tanh(s / cap)
         x, f = cap * t, 1 - t * t
-        # the polynomial 7.3e-7 of the value, the other form a few 2^-23 of the cap where tanh > 0.76; arithmetic a few 2^-24 more
+        # the polynomial 3.0e-6 of the value, the other form a few 2^-23 of the cap where tanh > 0.71; arithmetic a few 2^-24 more
         err = err * f + 4e-6 * x.abs()
     if slopes is not None:
         bias = slopes.double()[:, None, None] * far.abs()

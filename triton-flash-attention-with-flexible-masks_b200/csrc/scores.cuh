@@ -3,8 +3,9 @@
 // without a cap y = log2(e) * (s * sm_scale - ...). The gradient through the cap is the factor 1 - tanh^2 = 1 - (y before the bias / a)^2,
 // a = cap * log2(e).
 //
-// The capped score is s * (an even polynomial of s) where all of a warp's are at most 0.75 cap: tanh(x) / x over x^2 in [0, 0.5625] by interpolation at
-// Chebyshev's points, relative error 7.1e-7, with a and sm_scale / cap multiplied into its coefficients. That is six packed FMAs for two
+// The capped score is s * (an even polynomial of s) where all of a warp's are at most 0.9 cap: tanh(x) / x over x^2 in [0, 0.81] by interpolation at
+// Chebyshev's points, relative error 3.0e-6 (up to 50 that is 1.4e-4 of an exponential, a quarter of the rounding of P to fp16), with a and sm_scale / cap
+// multiplied into its coefficients. That is six packed FMAs for two
 // scores and nothing of the special-function unit, which the exponentials keep busy. Elsewhere it is a - 2 a / (1 + 2^(2 log2(e) x)), whose absolute error
 // is some 2^-22 of a; close to 0 that form would lose the small scores of a large cap.
 #pragma once
@@ -40,9 +41,9 @@ struct ScoreArgs {
 constexpr float kScoreLog2e = 1.4426950408889634f;
 
 inline ScoreArgs make_score_args(float cap, const float* slopes, bool prefix, float sm_scale) {
-    constexpr double kTanh[kTanhTerms] = {0.999999424, -0.333281921, 0.132584621, -0.0500416086, 0.0129166518};
+    constexpr double kTanh[kTanhTerms] = {0.999997105, -0.333153478, 0.131495683, -0.0471230871, 0.010487992};
     // largest x at which the term of x^(2i) is below 2e-7 of the sum
-    constexpr double kWithout[kTanhTerms] = {0.0, 7.7e-4, 0.035, 0.126, 0.25};
+    constexpr double kWithout[kTanhTerms] = {0.0, 7.7e-4, 0.035, 0.127, 0.257};
     ScoreArgs s{};
     s.slopes = slopes;
     s.cap = cap;
@@ -50,7 +51,7 @@ inline ScoreArgs make_score_args(float cap, const float* slopes, bool prefix, fl
     if (prefix && s.kind == SCORE_PLAIN) s.kind = SCORE_PREFIX;
     if (cap > 0.f) {
         const double a = double(cap) * 1.4426950408889634, k = double(sm_scale) / cap;
-        double power = a * k, most = 0.75;
+        double power = a * k, most = 0.9;
         for (int i = 0; i < kTanhTerms; ++i, power *= k * k) {
             const double c = kTanh[i] * power, size = c < 0 ? -c : c;
             // a coefficient that fp32 cannot hold is left out, with the scores that need it
