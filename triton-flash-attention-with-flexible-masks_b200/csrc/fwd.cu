@@ -98,7 +98,8 @@ static_assert(FwdSmem<128>::total > 116736 && FwdSmem<64>::total > 116736, "shar
 //    and their log-sum-exp go to the workspace, and fwd_combine_kernel merges them.
 // Such calls are bound by reading K and V (16 tokens of 32 / 8 heads of 128 against 4500 keys: 295 MB, 45 us at the
 // copy rate; 127 us with a tile per head, 55 us packed) or, with few heads, by the longest item's chain of tiles.
-// KIND (scores.cuh): with a cap or a bias the scores pass through score_row and are in the log2 domain from there on; the causal mask may leave a prefix visible.
+// KIND (scores.cuh, with what each costs): with a cap or a bias the scores pass through score_row and are in the log2 domain from there on, relative to the row's reference
+// point; the causal mask may leave a prefix visible. Instances of their own, so that attention's keep their code.
 template <int D, bool BF16, bool SHORT, int KIND = SCORE_PLAIN>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,

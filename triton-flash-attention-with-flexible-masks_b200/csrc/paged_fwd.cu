@@ -12,8 +12,15 @@
 //  - P of a masked entry is 0, but 0 times a NaN that an earlier user left in the page is not: rows of V behind the sequence's end are
 //    zeroed in shared memory by the softmax group before it gives its P away (not by the warp that issues P V: its code has to stay free of loops by
 //    lanes, or the descriptors go through vector registers);
+//  - items of at most 32 rows (a decoded token's heads) take the tile four times over, so that each of a group's four warps has 32 keys of every row instead of 32 rows of
+//    which most are nobody's: the chain from the scores to P is a quarter as long. 64 single tokens, 32 / 8 heads of 128, capped, 251 -> 218 us;
 //  - each block works on one stretch of a line of all items (paged_plan.cuh); a piece of an item that was cut leaves normalised fp32 rows and
 //    their log-sum-exp to paged_combine_kernel.
+//
+// What bounds it. Single tokens: HBM. 64 tokens over 1288 MB of keys and values 207-215 us (6.0-6.2 TB/s; the copy rate is 6.56), one token over 537 MB 99 us, of which
+// the plan and the first item's place take 2.3, the last tile's drain 3, the second kernel up to 4 (the main loop streams at 7 TB/s); one token over 1.4 MB
+// 16 us, all of it latency: start, plan, a chain of tiles, epilogue, the second kernel's start. Chunks: the forward's chain of tiles, and twice as many loads. One chunk of 2000
+// tokens, pages of 128 | 16: 199 | 220 us (1150 | 1043 TFLOP/s); a chunk of 500 behind 7500 76 | 83 us, where dense keys take 55.
 #include <type_traits>
 #include "common.cuh"
 #include "paged_plan.cuh"
