@@ -73,8 +73,8 @@ struct FwdSmem {
     static constexpr int off_list = off_v + NS * TILE;           // uint16 [NQ][kListCap]
     static constexpr int off_qc = off_list + NQ * kListCap * 2;  // int32  [NQ][128] query codes
     static constexpr int off_kc = off_qc + NQ * kBlk * 4;        // int32  [NKC][128] key codes, loaded with K on K's barrier
-    static constexpr int off_ml = off_kc + NKC * kBlk * 4;       // float  [NQ][2 groups][m, l][128]
-    static constexpr int off_info = off_ml + NQ * 4 * kBlk * 4;  // int32 [NQ][8]: T, lo, item (-1: no more items), kv head, query block, head, batch
+    static constexpr int off_ml = off_kc + NKC * kBlk * 4;       // float  [NQ][2 groups][m, l, and l less what of it P has][128]
+    static constexpr int off_info = off_ml + NQ * 6 * kBlk * 4;  // int32 [NQ][8]: T, lo, item (-1: no more items), kv head, query block, head, batch
     static constexpr int off_bar = off_info + NQ * 32;
     // item_full[NQ] item_empty[NQ] q_full[NQ] q_empty[NQ] ml_full[NQ] staged[NQ] k_full[NS] k_empty[NS] v_full[NS] v_empty[NS]
     // s_full[4] s_free[2] p_full[NP] pv_done[NP] o_full[2] o_free[2]
@@ -501,15 +501,18 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
             if (alive && T > 1) alive = mbar_wait_warp(BAR(B_OFULL + (we ^ 1)), i1 & 1, ab, ST_WAIT_TIMEOUT + 9);
             if (!alive) break;
             tc_fence_after();
-            const float* ml = reinterpret_cast<const float*>(smem + S::off_ml) + s * (4 * kBlk);  // [2 groups][m, l][128]
-            const int even = we * (2 * kBlk), odd = 2 * kBlk - even;
+            const float* ml = reinterpret_cast<const float*>(smem + S::off_ml) + s * (6 * kBlk);  // [2 groups][m, l, lost][128]
+            const int even = we * (3 * kBlk), odd = 3 * kBlk - even;
             const float m0 = ml[even + r], l0 = ml[even + kBlk + r], m1 = ml[odd + r], l1 = ml[odd + kBlk + r];
             const float mt = fmaxf(m0, m1);
             const float a0 = (m0 == -INFINITY) ? 0.f : fast_exp2((m0 - mt) * c);
             const float a1 = (m1 == -INFINITY) ? 0.f : fast_exp2((m1 - mt) * c);
             const float lt = l0 * a0 + l1 * a1;
             // (attention_scored: a NaN among a row's scores makes it NaN; attention's result for such a row is zeros)
-            const float inv = (lt > 0.f) ? 1.0f / lt : KIND == SCORE_PLAIN || lt == lt ? 0.f : lt;
+            // What the rounding of a chain's greatest P has left out of P V is left out of the sum that P V is divided by as well: where that entry carries the row, its rounding
+            // would reach O, and by way of delta = rowsum(dO O) the gradients, several times as large. (The LSE is the sum's as it is.)
+            const float sum = KIND == SCORE_PLAIN ? lt : lt + (ml[even + 2 * kBlk + r] * a0 + ml[odd + 2 * kBlk + r] * a1);
+            const float inv = (lt > 0.f) ? 1.0f / sum : KIND == SCORE_PLAIN || lt == lt ? 0.f : lt;
             const float f0 = a0 * inv, f1 = a1 * inv;
             // a chain in which the row had no key takes no part, whatever the values behind its mask are
             const bool use0 = (T > 0) && (f0 != 0.f), use1 = (T > 1) && (f1 != 0.f);
@@ -664,6 +667,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                 if (p.score.slopes) slope = p.score.slopes[int64_t(own)] * kScoreLog2e;
             }
             float m_run = -INFINITY, l_run = 0.f;
+            float most = 0.f, lost = 0.f;  // KIND: the chain's greatest P, and what its rounding has added to it
 
             for (int t = t0; t < T && alive; t += 2) {
                 const uint32_t entry = list[t];
@@ -774,6 +778,10 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     }
                     const float alpha = need ? fast_exp2((m_run - m_new) * c) : 1.0f;
                     l_run *= alpha;
+                    if constexpr (KIND != SCORE_PLAIN) {
+                        most *= alpha;
+                        lost *= alpha;
+                    }
                     if (t > t0) {
                         if (!S::POWN) {
                             alive = pv_before();
@@ -796,6 +804,15 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                 }
                 m_run = m_new;
                 const float mneg = (m_run == -INFINITY) ? 0.f : -m_run * c;
+                if constexpr (KIND != SCORE_PLAIN) {
+                    const float greatest_p = fast_exp2(!SCORED ? fmaf(mx, c, mneg) : need ? 0.f : mx);
+                    if (greatest_p > most) {
+                        float rounded, none;
+                        unpack2<BF16>(pack2<BF16>(greatest_p, 0.f), rounded, none);
+                        most = greatest_p;
+                        lost = rounded - greatest_p;
+                    }
+                }
                 // exp2(s*c - m*c) on packed pairs
                 const uint64_t c2 = pack_f2(c, c), mneg2 = pack_f2(mneg, mneg);
                 uint64_t lacc0 = pack_f2(0.f, 0.f), lacc1 = lacc0;
@@ -828,9 +845,10 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                 }
             }
             if (!alive) break;
-            float* ml = reinterpret_cast<float*>(smem + S::off_ml) + s * (4 * kBlk) + w * (2 * kBlk) + r;
+            float* ml = reinterpret_cast<float*>(smem + S::off_ml) + s * (6 * kBlk) + w * (3 * kBlk) + r;
             ml[0] = m_run;
             ml[kBlk] = l_run;
+            if (KIND != SCORE_PLAIN) ml[2 * kBlk] = lost;
             mbar_arrive_warp(BAR(B_MLFULL + s), lane);
             G += T;
             __syncwarp();
