@@ -1,6 +1,8 @@
 """CPU tests of attention_scored: what the library and the Python call refuse before a device is touched, and the plain computation in 64 bits
 that the GPU tests go by, against autograd."""
 import ctypes
+import os
+import re
 
 import pytest
 import torch
@@ -85,3 +87,18 @@ def test_the_formulas_against_autograd(causal):
     got = attention_64(q, k, v, do, causal, None, ids[..., 3:], ids, 2.0, slopes, prefix)
     for name, want in (("o", o), ("dq", a.grad), ("dk", b.grad), ("dv", c.grad)):
         assert torch.allclose(got[name][0], want, rtol=1e-12, atol=1e-12), name
+
+
+def test_the_forward_reads_no_prefix_before_the_kernel_before_it_is_complete():
+    """Its first item's range of keys goes by the prefix, so that a call with one works that item out behind the wait. (In the sources, as the order in
+    test_launch_order.py: a wrong one shows only now and then.)"""
+    csrc = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "triton-flash-attention-with-flexible-masks_b200", "csrc")
+    with open(os.path.join(csrc, "fwd.cu")) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    kernel = code[code.index("fwd_kernel(const"):]
+    wait = kernel.index("wait_prerequisites();")
+    before = kernel[kernel.index("fence_mbar_init();"): wait]
+    assert re.search(r"early = mk\.mode == 0 && !\(PREFIX && mk\.prefix\);", before)
+    assert re.findall(r"if \([^\n]*\bprepare\(|\bprepare\(", before) == ["if (warp == 14 && early) item = prepare("]
+    assert not re.search(r"\b(front_keys|slopes|prefix\[)", before)
+    assert "if ((k > 0 || !early) && j < n_items) item = prepare(j);" in kernel[wait:]

@@ -388,3 +388,55 @@ def test_a_key_that_is_not_a_number_behind_the_mask(cap, slopes):
             k[:, :, at] = float("nan")
             got = fb.attention_scored(q, k, v, True, softcap=cap, slopes=_slopes(2, slopes))
         assert torch.equal(got[:, :, :at], want[:, :, :at]) and torch.isnan(got[:, :, at:]).all()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("M, N, slopes, splits", [(600, 600, None, 1), (600, 600, "series", 1), (40, 2500, None, 1), (16, 4000, "series", 5)])
+def test_a_prefix_that_the_kernel_directly_before_writes(M, N, slopes, splits, captured):
+    """The build of a plan lets its dependents begin before it has written anything: its first query's code (the largest int32 for an id that is not negative, else the
+    id) is the prefix of the forward behind it, all keys visible or the causal mask alone, in turn. The bits of forwards that the host has waited in front of."""
+    import ctypes
+    from flash_b200 import _lib, ops
+    lib, H, D, L, n = _lib.load(), 8, 64, 4096, 8
+    q, k, v, _ = _inputs(1, H, H, M, N, D, BF16, 64)
+    slopes = _slopes(H, slopes)
+    prob, build = ops._problem(1, H, H, M, N, D, BF16, True, 0, 1, D ** -0.5), ops._problem(1, 1, 1, L, L, D, BF16, True, 1, 1, 1.0)
+    status, size = torch.zeros(1, dtype=torch.int32, device="cuda"), ctypes.c_size_t()
+    _lib.check(lib.fa_plan_bytes(build, size), "fa_plan_bytes")
+    plan = torch.zeros(size.value // 4, dtype=torch.int32, device="cuda")
+    ids = [torch.full((1, 1, L), x, dtype=torch.int32, device="cuda") for x in (-1, 5)]
+    lse, work = torch.empty(1, H, lib.fa_padded_rows(M), device="cuda"), None
+    if splits > 1:
+        need = ctypes.c_size_t()
+        _lib.check(lib.fa_fwd_workspace_bytes(prob, splits, need), "fa_fwd_workspace_bytes")
+        work = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    scores = _lib.Scores(0.0, None if slopes is None else slopes.data_ptr(), plan.data_ptr())
+    t = [ops._tensor(x) for x in (q, k, v)]
+
+    def run(outs, wait):
+        s = ops._stream()
+        for i, o in enumerate(outs):
+            e = ops._ids(ids[i % 2])
+            _lib.check(lib.fa_plan_build(build, e, e, plan.data_ptr(), size.value, status.data_ptr(), s), "fa_plan_build")
+            if wait:
+                torch.cuda.synchronize()
+            _lib.check(lib.fa_fwd_scored(prob, scores, *t, ops._tensor(o), None, lse.data_ptr(), None, splits, None if work is None else work.data_ptr(),
+                                         0 if work is None else work.numel(), status.data_ptr(), s), "fa_fwd_scored")
+
+    want, got = ([torch.empty_like(q) for _ in range(n)] for _ in range(2))
+    run(want, True)
+    torch.cuda.synchronize()
+    assert not torch.equal(want[0], want[1])
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run(got, False)
+    for _ in range(5):
+        if captured:
+            graph.replay()
+        else:
+            torch.cuda._sleep(3_000_000)
+            run(got, False)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
+    assert int(status.item()) == 0

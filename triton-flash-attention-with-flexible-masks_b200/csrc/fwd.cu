@@ -208,9 +208,10 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         for (int i = tid; i < NQ * S::TILE / 16; i += kFwdThreads) reinterpret_cast<uint4*>(smem + S::off_q)[i] = make_uint4(0, 0, 0, 0);
         fence_proxy_async();
     }
-    // Without ids the scheduler knows its first item before the kernel may touch memory.
+    // Without ids the scheduler knows its first item before the kernel may touch memory. (Not so with a prefix, which is read from there.)
+    const bool early = mk.mode == 0 && !(PREFIX && mk.prefix);
     Item item;
-    if (warp == 14 && mk.mode == 0) item = prepare(int(blockIdx.x));
+    if (warp == 14 && early) item = prepare(int(blockIdx.x));
     wait_prerequisites();
     if (warp == 13) {
         tmem_alloc(sbase + S::off_misc, 512);
@@ -282,7 +283,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     }
                     j = __shfl_sync(0xffffffffu, j, 0);
                 }
-                if ((k > 0 || mk.mode != 0) && j < n_items) item = prepare(j);
+                if ((k > 0 || !early) && j < n_items) item = prepare(j);
                 if (j >= n_items) {  // end marker
                     if (lane == 0) {
                         info[s * 8 + 2] = -1;
