@@ -438,3 +438,33 @@ def test_a_row_that_sees_a_key_that_is_not_a_number(length, at, new, cap):
     assert torch.equal(got[:new][~sees], want[:new][~sees]) and torch.equal(got[new:], want[new:])
     assert sees.any() and torch.isnan(got[:new][sees]).all()
     fb.check_status()
+
+
+@pytest.mark.parametrize("cap", [3.0, 30.0, 1e4])
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("D, new", [(64, 3), (128, 3), (64, 40), (128, 90)])
+def test_a_key_beyond_the_cap_leaves_the_bits_of_rows_in_front_of_it(D, new, slopes, cap):
+    import flash_b200 as fb
+    cache = Cache([333, 200], 2, D, 16, BF16, 24).fill()
+    q = torch.randn(new + 1, 8, D, device="cuda").to(BF16)
+    call = lambda: fb.paged_attention(q, cache.k_pages, cache.v_pages, cache.table, cache.kv_lens, _starts([new, 1]), softcap=cap, slopes=_slopes(8, slopes))  # noqa: E731
+    want, place = call(), cache.places(0, 332, 333)
+    cache.k_pages[place] *= 40 * cap
+    got = call()
+    assert torch.equal(got[:new - 1], want[:new - 1]) and torch.equal(got[new:], want[new:]) and not torch.equal(got, want)
+
+
+@pytest.mark.parametrize("cap", [1e4, 1e6])
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("D, new", [(64, 3), (128, 3), (64, 40), (128, 90)])
+def test_a_query_beyond_a_large_cap_among_ordinary_ones(D, new, slopes, cap):
+    """Its neighbours are within their own bounds."""
+    import flash_b200 as fb
+    cache = Cache([333, 200], 2, D, 16, BF16, 25).fill()
+    q = (torch.randn(new + 1, 8, D, device="cuda") * 1.5).to(BF16)
+    args = (cache.k_pages, cache.v_pages, cache.table, cache.kv_lens, _starts([new, 1]))
+    big = q.clone()
+    big[1] *= 10 * cap
+    got = fb.paged_attention(big, *args, softcap=cap, slopes=_slopes(8, slopes))
+    got[1] = fb.paged_attention(q, *args, softcap=cap, slopes=_slopes(8, slopes))[1]
+    _check(got, cache, q, [new, 1], cap=cap, slopes=_slopes(8, slopes))

@@ -440,3 +440,57 @@ def test_a_prefix_that_the_kernel_directly_before_writes(M, N, slopes, splits, c
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
     assert int(status.item()) == 0
+
+
+def _outliers(M, N, D, dtype, seed, q_rows, key, times):
+    """Ordinary inputs, and the same with some queries and a key so many times as large; the last query and `q_rows` have no gradient."""
+    q, k, v, do = _inputs(1, 4, 2, M, N, D, dtype, seed)
+    do[:, :, [*q_rows, M - 1]] = 0
+    big_q, big_k = q.clone(), k.clone()
+    big_q[:, :, q_rows] *= times
+    big_k[:, :, key] *= times
+    return q, k, v, do, big_q, big_k
+
+
+@pytest.mark.parametrize("slopes", [None, "series"])
+@pytest.mark.parametrize("dtype, D, M, N, cap", [(FP16, 64, 300, 300, 1e4), (FP16, 128, 280, 400, 1e4), (FP16, 64, 20, 700, 1e4), (BF16, 128, 700, 700, 1e5), (BF16, 64, 300, 300, 1e6)])
+def test_a_score_beyond_a_large_cap_among_ordinary_ones(dtype, D, M, N, cap, slopes):
+    """Queries of which all scores, and a last key of which the last query's score, are beyond the cap: all other rows, and the gradients of all keys (those queries have
+    none), are those of ordinary inputs, within the bounds of these."""
+    import flash_b200 as fb
+    rows, slopes = [i for i in (5, 70, 150) if i < M - 1], _slopes(4, slopes)
+    q, k, v, do, big_q, big_k = _outliers(M, N, D, dtype, 65, rows, N - 1, 0.8 * cap if dtype == FP16 else 4 * cap)
+    want = attention_64(q, k, v, do, True, None, None, None, cap, slopes, None)
+    got = _run(fb, big_q, big_k, v, do, True, cap=cap, slopes=slopes)
+    plain = torch.ones(M, dtype=torch.bool, device="cuda")
+    plain[[*rows, M - 1]] = False
+    for name in ("o", "dq"):
+        _check(got[name][:, :, plain], tuple(x[:, :, plain] for x in want[name]), name)
+    for name in ("dk", "dv"):
+        _check(got[name], want[name], name)
+
+
+@pytest.mark.parametrize("cap", [3.0, 30.0, 1e4])
+@pytest.mark.parametrize("slopes", [None, "mixed"])
+@pytest.mark.parametrize("dtype, D, M, N", [(BF16, 64, 300, 300), (FP16, 128, 500, 500), (BF16, 128, 140, 333), (FP16, 64, 25, 700)])
+@pytest.mark.parametrize("hidden", ["ahead", "other document"])
+def test_a_hidden_key_beyond_the_cap_leaves_all_bits(hidden, dtype, D, M, N, slopes, cap):
+    """One that only the last query sees, which has no gradient, or one of a document that no query is of, in tiles with others."""
+    import flash_b200 as fb
+    key, kw = N - 1, dict(cap=cap, slopes=_slopes(4, slopes))
+    if hidden != "ahead":
+        key = N - 30
+        ids = torch.full((1, 1, N), -1, dtype=torch.int32, device="cuda")
+        ids[..., N // 2:] = -2
+        kw["eq"] = ids[..., N - M:].clone().expand(1, 4, M)
+        ids[..., key] = -9
+        kw["ek"] = ids.expand(1, 4, N)
+    q, k, v, do, _, big_k = _outliers(M, N, D, dtype, 66, [], key, 10 * cap)
+    if dtype == FP16:
+        big_k = big_k.clamp(-6e4, 6e4)
+    for causal in (True, False) if hidden != "ahead" else (True,):
+        want, got = (_run(fb, q, x, v, do, causal, **kw) for x in (k, big_k))
+        rows = M - 1 if hidden == "ahead" else M
+        for name in ("o", "dq", "dk", "dv"):
+            n = rows if name in ("o", "dq") else N
+            assert torch.equal(got[name][:, :, :n], want[name][:, :, :n]), (name, causal)

@@ -6,14 +6,14 @@
 // The capped score is s * (an even polynomial of s) where all of a warp's are at most 0.9 cap: tanh(x) / x over x^2 in [0, 0.81] by interpolation at
 // Chebyshev's points, relative error 3.0e-6 (up to 50 that is 1.4e-4 of an exponential, a quarter of the rounding of P to fp16), with a and sm_scale / cap
 // multiplied into its coefficients. That is six packed FMAs for two
-// scores and nothing of the special-function unit, which the exponentials keep busy. Elsewhere it is a - 2 a / (1 + 2^(2 log2(e) x)), whose absolute error
-// is some 2^-22 of a; close to 0 that form would lose the small scores of a large cap.
+// scores and nothing of the special-function unit, which the exponentials keep busy. Beyond, a score is a - 2 a / (1 + 2^(2 log2(e) x)), whose absolute error
+// is some 2^-22 of a: close to 0 that form would lose the small scores of a large cap, so that a warp with a score beyond the polynomial works out both forms and takes each score's own.
 //
 // What bounds it: what two softmax warps a scheduler get through of a tile's straight code (no unit is full: issue slots 46 %, MUFU 39, FMA 36, tensor pipe 38 with a cap), so that each
 // instruction shows. Forward of 2 x 16 x 4096 x 128 causal, unchanged, capped, biased, both: 49, 77, 75, 104 million
 // instructions in 206, 296, 259, 365 thousand clocks. Forward of 32 / 8 heads x 5801 x 128 causal 257, 325, 298, 395 us; kernels of a step of 16 x 8111 x 128 in documents, us,
 // forward 117, 167, 138, 195, dK/dV 193, 241, 210, 262, dQ 142, 192, 154, 210.
-// Tried and taken back (the same forward, cap 50 | cap 20, which at deviation 4 goes through the slow form now and then; now 327 | 460): five terms for 7.1e-7 up to 0.75 cap 325 | 682; six up
+// Tried and taken back (the same forward, cap 50 | cap 20, which at deviation 4 goes through both forms now and then; now 324 | 460): five terms for 7.1e-7 up to 0.75 cap 325 | 682; six up
 // to the cap 352 | 378; a quotient of polynomials of degree 2, up to 2.5 caps, with one reciprocal for two scores 426 | 418; eight terms up to 1.4 cap as a second unrolled
 // form 358 | 528 (registers); the cap of the next 16 scores in front of the exponentials of these, as the source goes, 328 | -. The bias as one more product of 16 columns on the tensor cores (slope and position in three 16-bit parts): the biased forward 277 for 298, but 8 ragged
 // sequences over a paged cache 222 for 218 and an encoder's step 136 for 134, for a quarter more code.
@@ -110,9 +110,16 @@ __device__ __forceinline__ float cap_one(float s, const ScoreArgs& a) {
     for (int i = kTanhTerms - 2; i >= 0; --i) t = fmaf(t, u, a.poly[i]);
     return __fmul_rn(s, t);
 }
-// the capped score, whatever its size
-__device__ __forceinline__ float cap_any(float s, const ScoreArgs& a) {
-    return fmaf(-2.f * a.a, fast_rcp(1.f + fast_exp2(s * a.k2e)), a.a);
+// two capped scores, whatever their size, with b2 added to them: each by the form that is exact for it (the other one's error goes by the cap), and one that the polynomial
+// covers to the bits that it has in a warp without any that it does not. So a score beyond it, perhaps one that a mask hides, is nothing to its neighbours.
+__device__ __forceinline__ uint64_t cap_any(uint64_t s2, uint64_t b2, const ScoreArgs& a) {
+    float s0, s1, x0, x1, p0, p1;
+    unpack_f2(s2, s0, s1);
+    unpack_f2(mul_f2(s2, pack_f2(a.k2e, a.k2e)), x0, x1);
+    unpack_f2(add_f2(pack_f2(fast_exp2(x0), fast_exp2(x1)), pack_f2(1.f, 1.f)), x0, x1);
+    unpack_f2(add_f2(fma_f2(pack_f2(fast_rcp(x0), fast_rcp(x1)), pack_f2(-2.f * a.a, -2.f * a.a), pack_f2(a.a, a.a)), b2), x0, x1);
+    unpack_f2(fma_f2(s2, cap_poly(s2, a), b2), p0, p1);
+    return pack_f2(fabsf(s0) <= a.most ? p0 : x0, fabsf(s1) <= a.most ? p1 : x1);
 }
 // 1 - tanh^2 of two capped scores
 __device__ __forceinline__ uint64_t cap_slope(uint64_t y2, const ScoreArgs& a) {
@@ -148,6 +155,20 @@ __device__ __forceinline__ void rolled(float* v, F f) {
         for (int x = 0; x < kStep; ++x) v[N - kStep + x] = first[x];
     }
 }
+// The same two at a time: f(values, x0, x) for those of x0 + x, x0 a multiple of kStep.
+template <int N, int kStep, class F>
+__device__ __forceinline__ void rolled_pairs(float* v, F f) {
+#pragma unroll 1
+    for (int x0 = 0; x0 < N; x0 += kStep) {
+        float first[kStep];
+#pragma unroll
+        for (int x = 0; x < kStep; x += 2) unpack_f2(f(pack_f2(v[x], v[x + 1]), x0, x), first[x], first[x + 1]);
+#pragma unroll
+        for (int x = 0; x + kStep < N; ++x) v[x] = v[x + kStep];
+#pragma unroll
+        for (int x = 0; x < kStep; ++x) v[N - kStep + x] = first[x];
+    }
+}
 
 // N neighbouring scores of one row (a multiple of 32), in place, to the log2 domain, less `ref`; dist: distance of the first one. real: the row is a
 // query's (what lies in other rows of the tile must not tell the warp which form of the tanh to take, and so the last bits).
@@ -177,10 +198,19 @@ __device__ __forceinline__ void score_row(float* v, const ScoreArgs& a, const Bi
     };
     if constexpr (kCapped) {
         if (N == kBlk && !kBias && !beyond) {
-            rolled<N, kStep>(v, [&](float s, int) { return cap_one(s, a) - ref; });  // (a tile with a mask: the others are capped elsewhere)
+            rolled_pairs<N, kStep>(v, [&](uint64_t s2, int, int) { return fma_f2(s2, cap_poly(s2, a), pack_f2(-ref, -ref)); });  // (a tile with a mask: the others are capped elsewhere)
         } else if (beyond) {
-            const float d = float(dist);
-            rolled<N, kStep>(v, [&](float s, int x) { return cap_any(s, a) + (kBias ? fmaf(bias.line, d - float(x), -ref) : -ref); });
+            // 16 at a time: with 32 the registers do not do, with 8 a call of 16 x 4096 x 128 most of whose tiles go this way takes 224 us for 179
+            uint64_t b2 = pack_f2(-ref, -ref);
+            rolled_pairs<N, 16>(v, [&](uint64_t s2, int x0, int x) {
+                if (kBias && x == 0 && x0 % 32 == 0) {  // (as in `each`)
+                    const float d = float(dist - x0);
+                    b2 = pack_f2(fmaf(bias.line, d, -ref), fmaf(bias.line, d - 1.f, -ref));
+                }
+                const uint64_t y2 = cap_any(s2, b2, a);
+                if constexpr (kBias) b2 = add_f2(b2, pack_f2(-2.f * bias.line, -2.f * bias.line));
+                return y2;
+            });
         } else {
             each([&](uint64_t s2, uint64_t b2) { return fma_f2(s2, cap_poly(s2, a), b2); });
         }
@@ -196,8 +226,10 @@ __device__ __forceinline__ void score_row(float* v, const ScoreArgs& a, const Bi
 // The same as above without bias and reference: scores to capped scores, for the backward kernels.
 template <int N>
 __device__ __forceinline__ void cap_scores(float* v, const ScoreArgs& a) {
+    // (both in straight code: with the rare one in a loop of 16 at a time dQ of 16 x 4096 x 128 causal, none of whose scores is beyond, takes 127 us for 120)
     if (any_beyond<N>(v, a.most)) {
-        rolled<N, 16>(v, [&](float s, int) { return cap_any(s, a); });
+#pragma unroll
+        for (int x = 0; x < N; x += 2) unpack_f2(cap_any(pack_f2(v[x], v[x + 1]), 0, a), v[x], v[x + 1]);
     } else {
 #pragma unroll
         for (int x = 0; x < N; x += 2) {
