@@ -1,6 +1,7 @@
 """attention_scored against the plain computation in 64 bits, element by element within bounds derived from the roundings (scored_reference.py)."""
 import contextlib
 import itertools
+import math
 
 import pytest
 import torch
@@ -494,3 +495,46 @@ def test_a_hidden_key_beyond_the_cap_leaves_all_bits(hidden, dtype, D, M, N, slo
         for name in ("o", "dq", "dk", "dv"):
             n = rows if name in ("o", "dq") else N
             assert torch.equal(got[name][:, :, :n], want[name][:, :, :n]), (name, causal)
+
+
+def _capped_scores(dtype, cap, s, N, slopes=None):
+    """What the kernels make of scores s (fp32, of up to 24 bits), one a row, each for N keys alike: the logarithm of the sum of N equal exponentials, less log N."""
+    from flash_b200 import _lib, ops
+    import ctypes
+    M, D = s.numel(), 16
+    q, rest = torch.zeros(1, 1, M, D, dtype=dtype, device="cuda"), s.clone()
+    for i in range(3):  # parts whose sum, in fp32, is the score
+        q[0, 0, :, i] = rest.to(dtype)
+        rest -= q[0, 0, :, i].float()
+    assert (rest == 0).all()
+    k = torch.zeros(1, 1, N, D, dtype=dtype, device="cuda")
+    k[..., :3] = 1
+    o, lib, status = torch.empty_like(q), _lib.load(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    prob = ops._problem(1, 1, 1, M, N, D, dtype, False, 0, 1, 1.0)
+    lse = torch.empty(1, 1, lib.fa_padded_rows(M), device="cuda")
+    t = [ops._tensor(x) for x in (q, k, k, o)]
+    scores = _lib.Scores(cap, None if slopes is None else slopes.data_ptr(), None)
+    _lib.check(lib.fa_fwd_scored(prob, scores, *t, None, lse.data_ptr(), None, 1, None, 0, status.data_ptr(), ops._stream()), "fa_fwd_scored")
+    assert int(status.item()) == 0
+    return lse[0, 0, :M].double() * math.log(2) - math.log(N)
+
+
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("N", [128, 1])  # without a mask, and with one
+@pytest.mark.parametrize("cap", [1e-3, 1.0, 30.0, 64.0, 65.0, 320.0, 330.0, 2000.0, 6000.0, 5e4, 1e6])
+def test_how_exact_a_capped_score_is(cap, N, slopes):
+    """Scores from 1e-4 to 3 caps of both signs, mixed over the rows, so that the warps have both forms of the tanh side by side.
+    The polynomial: its fit, 3.0e-6 up to a cap of 64, 6e-7 up to one of 320 and 8e-8 beyond, and 4e-7 for its coefficients' rounding and four FMAs. The other form, a - 2 a r with
+    r = 1 / (1 + e): an exp2 and a reciprocal to 2^-22 and 2^-23, the argument, the sum and the product to 2^-24, at most 5e-7 of the cap; it begins at 0.9 caps, 0.75, 0.6, or
+    (where a coefficient leaves fp32's range) 0.24 or 0.125. The sum's logarithm 2^-22 of its value and 2e-6."""
+    gen = torch.Generator(device="cuda").manual_seed(67)
+    t = torch.logspace(-4, 0.5, 1024, device="cuda", dtype=torch.float64)[torch.randperm(1024, generator=gen, device="cuda")]
+    s = (t * cap * (1 - 2 * torch.randint(0, 2, t.shape, generator=gen, device="cuda"))).float()
+    got = _capped_scores(BF16, cap, s, N, torch.zeros(1, device="cuda") if slopes else None)
+    want = cap * torch.tanh(s.double() / cap)
+    bound = (4e-6 if cap <= 64 else 1e-6 if cap <= 320 else 5e-7) * want.abs()
+    if cap > 64:
+        bound = torch.where(s.abs() > cap / 8, torch.full_like(bound, 5.5e-7 * cap), bound)
+    bound = bound + 2.0 ** -22 * want.abs() + 2e-6
+    off = (got - want).abs()
+    assert (off <= bound).all(), (off / bound).max().item()

@@ -4,8 +4,9 @@
 // a = cap * log2(e).
 //
 // The capped score is s * (an even polynomial of s) where all of a warp's are at most 0.9 cap: tanh(x) / x over x^2 in [0, 0.81] by interpolation at
-// Chebyshev's points, relative error 3.0e-6 (up to 50 that is 1.4e-4 of an exponential, a quarter of the rounding of P to fp16), with a and sm_scale / cap
-// multiplied into its coefficients. That is six packed FMAs for two
+// Chebyshev's points, with a and sm_scale / cap multiplied into its coefficients. Its relative error, 2.9e-6, is up to a cap of 64 1.4e-4 of an exponential, a quarter of the rounding of P to
+// fp16; for larger caps, whose scores may be hundreds or thousands, it is interpolated up to 0.75 cap (5.8e-7) or 0.6 cap (7.4e-8) instead, for scores beyond that take the other form: forward of
+// 16 x 4096 x 128 causal, greatest score 0.85 cap, interpolated up to 0.9 | 0.75 | 0.6 cap 90 | 93 | 136 us. That is six packed FMAs for two
 // scores and nothing of the special-function unit, which the exponentials keep busy. Beyond, a score is a - 2 a / (1 + 2^(2 log2(e) x)), whose absolute error
 // is some 2^-22 of a: close to 0 that form would lose the small scores of a large cap, so that a warp with a score beyond the polynomial works out both forms and takes each score's own.
 //
@@ -50,9 +51,14 @@ struct ScoreArgs {
 constexpr float kScoreLog2e = 1.4426950408889634f;
 
 inline ScoreArgs make_score_args(float cap, const float* slopes, bool prefix, float sm_scale) {
-    constexpr double kTanh[kTanhTerms] = {0.999997105, -0.333153478, 0.131495683, -0.0471230871, 0.010487992};
-    // largest x at which the term of x^(2i) is below 2e-7 of the sum
-    constexpr double kWithout[kTanhTerms] = {0.0, 7.7e-4, 0.035, 0.127, 0.257};
+    // tanh(x) / x up to x = kUpTo: the widest that is off by less than 1.5e-4 of an exponential at the greatest score
+    constexpr double kUpTo[3] = {0.9, 0.75, 0.6};
+    constexpr double kTanh[3][kTanhTerms] = {{0.999997105, -0.333153478, 0.131495683, -0.0471230871, 0.010487992},   // 2.9e-6 of the value
+                                             {0.999999424, -0.333281921, 0.132584621, -0.0500416086, 0.0129166518},  // 5.8e-7
+                                             {0.999999926, -0.33332302, 0.133100644, -0.0520966534, 0.0154687513}};  // 7.4e-8
+    // largest x at which the terms from x^(2i) on are below 2e-7 of the sum
+    constexpr double kWithout[kTanhTerms] = {0.0, 7.3e-4, 0.0349, 0.125, 0.241};
+    const int fit = cap <= 64.f ? 0 : cap <= 320.f ? 1 : 2;
     ScoreArgs s{};
     s.slopes = slopes;
     s.cap = cap;
@@ -60,9 +66,9 @@ inline ScoreArgs make_score_args(float cap, const float* slopes, bool prefix, fl
     if (prefix && s.kind == SCORE_PLAIN) s.kind = SCORE_PREFIX;
     if (cap > 0.f) {
         const double a = double(cap) * 1.4426950408889634, k = double(sm_scale) / cap;
-        double power = a * k, most = 0.9;
+        double power = a * k, most = kUpTo[fit];
         for (int i = 0; i < kTanhTerms; ++i, power *= k * k) {
-            const double c = kTanh[i] * power, size = c < 0 ? -c : c;
+            const double c = kTanh[fit][i] * power, size = c < 0 ? -c : c;
             // a coefficient that fp32 cannot hold is left out, with the scores that need it
             if (i > 0 && !(size > 1e-37 && size < 1e37)) most = most < kWithout[i] ? most : kWithout[i];
             else s.poly[i] = float(c);
