@@ -23,6 +23,11 @@ import torch
 SCORE_FUNC_MODE0_NOPE = 0  # flash_triton.py:20
 SCORE_FUNC_MODE1_DOC = 1   # flash_triton.py:22
 
+# torch's first exp of a process, if several threads take part in it, is now and then off by 1e-4 of its values (the math library behind it is then still
+# setting its accuracy up); every later one is exact. So the first one is made here, by one thread.
+for _dtype in (torch.float32, torch.float64):
+    torch.exp(torch.zeros(16, dtype=_dtype))
+
 
 def doc_mask(eq, ek):
     """[.., Lq, Lk] bool: (eq >= 0) | (eq == ek). README.md:16, flash_triton.py:114, testing.py:114."""
