@@ -125,11 +125,9 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const uint32_t tmem = uint32_t(misc[0]);
     const bool aborted = misc[1] != 0;
     uint16_t* const out = static_cast<uint16_t*>(p.out);
+    // (aborted: an earlier launch ran into a time-out that the host has not yet cleared. The second kernel fills the output.)
     if (aborted) {
         if (tid == 0) p.merge[blockIdx.x] = make_int4(0, 0, 0, 0);
-        // an earlier launch ran into a time-out that the host has not yet cleared: the whole of the output becomes NaN, shared out by rows of a head
-        for (int64_t i = blockIdx.x; i < int64_t(p.T) * p.H; i += gridDim.x)
-            for (int d = tid; d < p.D; d += kFwdThreads) out[i / p.H * p.out_t + i % p.H * p.out_h + d] = 0xffffu;
     } else if (p.B > kPagedWarpPlan) {
         paged_plan<kFwdThreads>(p, plan, int(gridDim.x));
     }
@@ -768,11 +766,20 @@ __global__ void __launch_bounds__(kCombineThreads, 2) paged_combine_kernel(const
     __shared__ float sums[kWarps][kCombineRows][D + 2];
     follow_stream();
     const int w = int(blockIdx.x), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool failed = status_is_fatal(*reinterpret_cast<volatile int*>(p.status));
+    if (status_is_fatal(*reinterpret_cast<volatile int*>(p.status))) {
+        // A time-out, of an earlier launch, of one on another stream meanwhile, or in the attention kernel: some of its blocks, or all, have left their rows as they
+        // were, and which is not known. All rows become NaN, or those of the sequences in an output of the caller's.
+        const bool all = p.fill || !p.starts;
+        const int front = all ? 0 : min(max(p.starts[0], 0), p.T), behind = all ? p.T : max(min(p.starts[p.B], p.T), front);
+        const int64_t first = int64_t(front) * p.H, end = int64_t(behind) * p.H;
+        for (int64_t i = first + (int64_t(blockIdx.y) * gridDim.x + w) * kWarps + warp; i < end; i += int64_t(gridDim.x) * gridDim.y * kWarps)
+            for (int d = lane; d < p.D; d += 32) static_cast<uint16_t*>(p.out)[i / p.H * p.out_t + i % p.H * p.out_h + d] = 0xffffu;
+        return;
+    }
     const int4 merge = p.merge[w];
     const int row0 = int(blockIdx.y) * kWarps * kCombineRows, pieces = merge.x, rows = (merge.z & 255) * p.G - row0, hk = merge.z >> 8;
     auto slot = [&](int s) { return 2 * (merge.w + s) + (s == 0 ? 1 : 0); };
-    if (failed || pieces < 2 || rows <= 0) return;
+    if (pieces < 2 || rows <= 0) return;
     const int groups = min(cdiv(rows, kCombineRows), kWarps), subs = kWarps / groups;
     const int sub = warp / groups, r0 = (warp - sub * groups) * kCombineRows;  // (of this block's rows)
     // A warp's own pieces first: their greatest lse, and the sums relative to it. (An empty piece has an lse of -inf.)
