@@ -186,10 +186,10 @@ int fa_debug_paged_pieces(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t c
         });
     fa::paged_share_out(plan, weight, items, longest, most_workers);
     if (plan.workers > 1023) return -1;
-    plan.sums[0] = 0;
+    long long before = 0;
     for (int g = 0; g < fa::kPagedGroups; ++g) {
-        plan.sums[g + 1] = plan.sums[g];
-        each(g, [&](const fa::PagedSeq& s) { plan.sums[g + 1] += Hk * fa::paged_weight(p, s, s.tiles, plan.keyed); });
+        plan.sums[g] = before;
+        each(g, [&](const fa::PagedSeq& s) { before += Hk * fa::paged_weight(p, s, s.tiles, plan.keyed); });
     }
     int n = 0;
     auto put = [&](int a, int b, int c, int d, int e, int f, int g, int h) {

@@ -35,7 +35,7 @@ struct PagedPlan {
     int pad;
     long long warp_sums[32], warp_items[32];
     int warp_max[32];
-    long long sums[kPagedGroups + 1];  // of what lies before an entry's sequences
+    long long sums[kPagedGroups];  // of what lies before an entry's sequences
 };
 
 __host__ __device__ __forceinline__ int paged_clamp(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
@@ -208,7 +208,7 @@ __device__ __forceinline__ void paged_plan(const PagedParams& p, PagedPlan& plan
         before += keyed ? weight[o] : items[o];
     }
     if (threadIdx.x == 0) {
-        plan.total = plan.sums[kPagedGroups] = own.total;
+        plan.total = own.total;
         plan.stretch = own.stretch;
         plan.workers = own.workers;
         plan.keyed = own.keyed;
@@ -311,20 +311,15 @@ __host__ __device__ __forceinline__ bool paged_first_cut(const PagedPlan& plan, 
     return w > 0 && walk.s.tiles > 0 && walk.at < paged_cut(plan, w) && (w == 1 || walk.at >= paged_cut(plan, w - 1));
 }
 
-// The pieces of the item at `walk`, which the cut before worker w goes through first: those of `count` workers from `from` on. (The first one's is left out where
-// the cut falls into the item's fixed cost, the last one's where it falls into the last tile; a stretch that lies within the item has tiles, for it is
-// longer than the cost and a tile.) The first piece's slot is 2 * from + 1, the others' are 2 * (from + i).
+// How many pieces the item at `walk` has, which the cut before worker w goes through first: one each of the workers from `from` on. (Where that cut falls into the item's fixed
+// cost or into its first tile, the worker in front of it has none: a cut inside a tile gives the tile to the worker behind the cut, who thus has the last one at least; and a stretch
+// that lies within the item has tiles, for it is longer than the cost and a tile.) The first piece's slot is 2 * from + 1, the others' are 2 * (from + i).
 __host__ __device__ __forceinline__ int paged_pieces(const PagedParams& p, const PagedPlan& plan, int w, const PagedWalk& walk, int& from) {
     static_assert((1 << kPagedLog2Piece) > kPagedItemCost + 2 * kBlk, "every stretch within an item has tiles");
-    const int n = walk.key_tiles(p);
     from = walk.key_tile_at(p, plan, paged_cut(plan, w)) > 0 ? w - 1 : w;
-    int v = w;  // the last worker with tiles of it
-    // the cuts lie a stretch apart: the last one before the item's last tile ends
-    const long long end = walk.end(p, plan);
-    v += int(paged_divide(end - 1 - paged_cut(plan, w), plan.stretch));
-    v = v < plan.workers ? v : plan.workers - 1;  // (somebody writes the lengths while the kernel reads them)
-    if (walk.key_tile_at(p, plan, paged_cut(plan, v)) >= n) --v;
-    return v - from + 1;
+    // the last worker: the cuts lie a stretch apart, and its own is the last one before the item's end
+    const int v = w + int(paged_divide(walk.end(p, plan) - 1 - paged_cut(plan, w), plan.stretch));
+    return (v < plan.workers ? v : plan.workers - 1) - from + 1;  // (somebody writes the lengths while the kernel reads them)
 }
 
 }  // namespace fa
