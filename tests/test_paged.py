@@ -113,6 +113,18 @@ def test_lengths_beyond_everything_stay_inside():
     assert 0 < n <= 100
 
 
+def test_a_wait_for_the_longest_item_fits_its_type():
+    """The longest limit that a wait may be given, times the tiles of an item of the longest sequence and one."""
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "triton-flash-attention-with-flexible-masks_b200", "csrc")
+    read = lambda name: open(os.path.join(csrc, name)).read()  # noqa: E731
+    most = int(re.search(r"kMost = 1LL << (\d+);", read("api.cu")).group(1))
+    tokens = int(re.search(r"kMostTokens = 1 << (\d+);", read("paged.cu")).group(1))
+    assert "ab.limit * (T + 1)" in read("paged_fwd.cu")
+    assert (1 << most) * ((1 << tokens) // 128 + 1) < 1 << 63
+
+
 def _cache(**kw):
     c = dict(B=2, Hk=2, D=64, dtype=0, pages=8, page_size=16, table_pages=4, table=256, table_stride=4, lens=256, k=256, v=256,
              k_stride=(16 * 2 * 64, 2 * 64, 64), v_stride=(16 * 2 * 64, 2 * 64, 64))

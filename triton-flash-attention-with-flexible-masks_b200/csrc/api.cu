@@ -43,7 +43,7 @@ EncodeFn encode_fn() {
 // Limit of one bounded wait inside the kernels, in SM clocks: FA_B200_WAIT_LIMIT_CLOCKS if set to a
 // number >= 10000 when the library is first used, else the built-in default.
 long long wait_limit_clocks() {
-    constexpr long long kMost = 1LL << 50;  // a week; a wait for a whole item multiplies it by the item's tiles
+    constexpr long long kMost = 1LL << 47;  // most of a day; a wait for a whole item multiplies it by the item's tiles and one, up to 2^22 / 128 + 1 over a paged cache
     static const long long v = [] {
         const char* e = getenv("FA_B200_WAIT_LIMIT_CLOCKS");
         if (e) {

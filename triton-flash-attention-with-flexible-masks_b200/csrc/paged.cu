@@ -14,6 +14,8 @@ cudaError_t launch_paged_fwd(bool, const CUtensorMap&, const CUtensorMap&, const
 namespace {
 
 constexpr int kMostTokens = 1 << 22;  // of a sequence, and of a call
+// The line of all items (paged_plan.cuh), whose points are 64-bit numbers: (kMostTokens + 65535) tiles of queries of 1024 heads, each weighing kMostTokens keys and its cost.
+static_assert(double(kMostTokens + 65535) * 1024 * (kMostTokens + fa::kPagedItemCost) < 9.2e18, "64 bits");
 
 bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
@@ -143,9 +145,6 @@ int fa_paged_fwd(const fa_paged_cache* cache, int32_t T, int32_t H, const int32_
     p.fill = fill ? 1 : 0;
     p.scale_log2 = sm_scale * fa::kScoreLog2e;
     p.score = fa::make_score_args(sc->softcap, sc->slopes, sc->prefix != nullptr, sm_scale);
-    // the line of all items stays below 2^53 (paged_plan.cuh)
-    const double line = (double(T) / p.tokens + cache->B) * cache->Hk * (double(p.capacity) + 256);
-    if (line > 9e15) return FA_ERR_PAGED;
     const int box_rows = cache->page_size < fa::kBlk ? cache->page_size : fa::kBlk;
     CUtensorMap tq, tk, tv;
     if ((rc = map4(&tq, cache->dtype, q->ptr, cache->D, {G, cache->Hk, T}, {q->stride[1], q->stride[1] * G, q->stride[0]}, {G, 1, p.tokens}))) return rc;
