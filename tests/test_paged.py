@@ -83,6 +83,19 @@ def test_cuts_of_random_batches():
         _check(lens, new, rng.choice((1, 2, 8)), rng.choice((1, 2, 3, 4, 7, 8, 64, 128)), rng.choice((1, 2, 13, 148)), prefix, rng.choice((1 << 20, 4096)))
 
 
+@pytest.mark.parametrize("B", [31, 32, 33, 63, 64, 65, 96, 97, 127, 128, 129, 200])
+def test_sequences_that_share_an_entry_of_the_table_of_sums(B):
+    """Up to 128 sequences the table has 32 entries, of one to four sequences each (the last ones perhaps of none), beyond it 1024."""
+    rng = random.Random(B)
+    for workers in (1, 7, 148):
+        _check([500] * B, [1] * B, 2, 4, workers)
+        for _ in range(6):
+            lens = [rng.choice((0, 1, 127, 128, 129, rng.randrange(1, 9000))) for _ in range(B)]
+            new = [rng.choice((0, 0, 1, 1, min(n, rng.randrange(0, 300)))) for n in lens]
+            prefix = None if rng.random() < 0.5 else [rng.randrange(-5, 3000) for _ in range(B)]
+            _check(lens, new, rng.choice((1, 2, 8)), rng.choice((1, 4, 7, 64)), workers, prefix)
+
+
 def test_more_sequences_than_entries_of_the_table_of_sums():
     rng = random.Random(1)
     for B in (1024, 1025, 5000):

@@ -171,13 +171,14 @@ int fa_debug_paged_pieces(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t c
     p.tokens = fa::kBlk / G;
     p.capacity = capacity;
     fa::PagedPlan plan;
-    plan.group = fa::cdiv(B, fa::kPagedGroups);
+    plan.group = fa::paged_group(B);
+    const int entries = fa::paged_entries(B);
     long long weight = 0, items = 0;
     int longest = 0;
     auto each = [&](int g, auto add) {
         for (int b = g * plan.group; b < B && b < (g + 1) * plan.group; ++b) add(fa::paged_seq(p, b));
     };
-    for (int g = 0; g < fa::kPagedGroups; ++g)
+    for (int g = 0; g < entries; ++g)
         each(g, [&](const fa::PagedSeq& s) {
             weight += Hk * fa::paged_weight(p, s, s.tiles, true);
             items += (long long)Hk * s.tiles;
@@ -186,7 +187,7 @@ int fa_debug_paged_pieces(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t c
     fa::paged_share_out(plan, weight, items, longest, most_workers);
     if (plan.workers > 1023) return -1;
     long long before = 0;
-    for (int g = 0; g < fa::kPagedGroups; ++g) {
+    for (int g = 0; g < entries; ++g) {
         plan.sums[g] = before;
         each(g, [&](const fa::PagedSeq& s) { before += Hk * fa::paged_weight(p, s, s.tiles, plan.keyed); });
     }

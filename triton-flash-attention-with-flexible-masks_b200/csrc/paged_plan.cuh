@@ -18,6 +18,9 @@ constexpr int kPagedGroups = 1024;   // entries of the table of sums: a sequence
 // Sequences up to which one warp makes the plan, beside which the others go on. One warp | all, us: single tokens of 1 sequence 15.9 | 16.6, of 128 101.0 | 102.0,
 // of 256 179.6 | 179.9, of 512 322 | 318.
 constexpr int kPagedWarpPlan = 128;
+// Entries of the table of a batch, and its sequences an entry.
+__host__ __device__ __forceinline__ int paged_entries(int B) { return B <= kPagedWarpPlan ? 32 : kPagedGroups; }
+__host__ __device__ __forceinline__ int paged_group(int B) { return cdiv(B, paged_entries(B)); }
 // Of an item besides its tiles, in keys. With 64 | 256 | 640 | 1500, us: 256 single tokens behind up to 1000 189 | 177 | 165 | 167, two chunks of 500 behind 1500
 // 67 | 53 | 43 | 45, twelve sequences with four chunks of 1000 186 | 183 | 174 | 175, one token behind 3000 26.9 | 26.1 | 24.5 | 29.7 (pieces of 2048 there).
 constexpr int kPagedItemCost = 640;
@@ -108,7 +111,7 @@ __host__ __device__ __forceinline__ void paged_share_out(PagedPlan& plan, long l
 // The plan of up to kPagedWarpPlan sequences, by one warp, the one that needs it: 32 entries of `sums`. (By all warps it costs a microsecond more, of which with
 // many sequences nothing is left.)
 __device__ __forceinline__ void paged_plan_warp(const PagedParams& p, PagedPlan& plan, int most_workers) {
-    const int lane = threadIdx.x & 31, group = (p.B + 31) >> 5;
+    const int lane = threadIdx.x & 31, group = paged_group(p.B);
     long long w = 0, n = 0;
     int longest = 0;
 #pragma unroll 1
@@ -150,7 +153,7 @@ __device__ __forceinline__ void paged_plan(const PagedParams& p, PagedPlan& plan
     constexpr int kOwn = kPagedGroups / kThreads, kWarps = kThreads / 32;
     static_assert(kOwn * kThreads == kPagedGroups && kOwn >= 1, "groups of a thread");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int group = cdiv(p.B, kPagedGroups), first = threadIdx.x * kOwn;
+    const int group = paged_group(p.B), first = threadIdx.x * kOwn;
     long long weight[kOwn], items[kOwn], w = 0, n = 0;
     int longest = 0;
 #pragma unroll
@@ -237,7 +240,7 @@ struct PagedWalk {
         if (p.B > kPagedWarpPlan) lo = 32 * (31 - __clz(__ballot_sync(0xffffffffu, plan.sums[32 * (threadIdx.x & 31)] <= x)));
         lo += 31 - __clz(__ballot_sync(0xffffffffu, plan.sums[lo + (threadIdx.x & 31)] <= x));
 #else
-        while (lo + 1 < kPagedGroups && plan.sums[lo + 1] <= x) ++lo;
+        while (lo + 1 < paged_entries(p.B) && plan.sums[lo + 1] <= x) ++lo;
 #endif
         long long rem = x - plan.sums[lo];
         b = lo * plan.group;
