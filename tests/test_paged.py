@@ -197,6 +197,24 @@ def test_python_calls_refuse_before_a_launch():
         paged_attention(rows[0], pages, pages, table, lens)
 
 
+def test_tangents_are_refused():
+    """In front of all that asks for a device, so that it shows here."""
+    import torch.autograd.forward_ad as fwad
+    pages = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+    rows, table, lens = torch.zeros(2, 2, 64, dtype=torch.bfloat16), torch.zeros(2, 2, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    slopes = torch.ones(2)
+    with fwad.dual_level():
+        dual = lambda x: fwad.make_dual(x, torch.ones_like(x))  # noqa: E731
+        for args in ((dual(rows), rows, pages, pages), (rows, dual(rows), pages, pages), (rows, rows, dual(pages), pages), (rows, rows, pages, dual(pages))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                paged_append(*args, table, lens)
+        for args, kw in (((dual(rows), pages, pages), {}), ((rows, dual(pages), pages), {}), ((rows, pages, dual(pages)), {}), ((rows, pages, pages), dict(slopes=dual(slopes)))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                paged_attention(*args, table, lens, **kw)
+        with pytest.raises(RuntimeError, match="CUDA"):  # within a level, and none of them dual
+            paged_append(rows, rows, pages, pages, table, lens)
+
+
 def test_tensor_memory_is_taken_between_the_wait_and_the_next_launch():
     """The order that test_launch_order.py asks of the other kernels that allocate tensor memory."""
     import os

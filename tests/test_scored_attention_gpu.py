@@ -538,3 +538,16 @@ def test_how_exact_a_capped_score_is(cap, N, slopes):
     bound = bound + 2.0 ** -22 * want.abs() + 2e-6
     off = (got - want).abs()
     assert (off <= bound).all(), (off / bound).max().item()
+
+
+def test_tangents_are_refused():
+    import flash_b200 as fb
+    import torch.autograd.forward_ad as fwad
+    q, k, v, _ = _inputs(1, 4, 2, 40, 40, 64, BF16, 68)
+    with fwad.dual_level():
+        dual = lambda x: fwad.make_dual(x, torch.ones_like(x))  # noqa: E731
+        for args, slopes in (((dual(q), k, v), None), ((q, k, dual(v)), None), ((q, k, v), dual(_slopes(4, "series")))):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                fb.attention_scored(*args, True, softcap=9.0, slopes=slopes)
+        plain = fb.attention_scored(q, k, v, True, softcap=9.0)
+    assert torch.equal(plain, fb.attention_scored(q, k, v, True, softcap=9.0))

@@ -29,6 +29,12 @@ def _rows(x):
     return _lib.Rows(x.data_ptr(), x.stride()[:2])
 
 
+def _no_tangents(*tensors):
+    """No derivative goes through a cache, forward-mode ones no more than gradients: they are refused, not lost."""
+    if ops._forward_ad._current_level >= 0 and any(isinstance(x, torch.Tensor) and ops._forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise RuntimeError("flash_b200: there is no forward-mode derivative through a paged cache; call it with the primals")
+
+
 def _checked(rows, name, k_pages, v_pages, page_table, kv_lens, q_starts):
     """The cache as the library takes it, its starts, and what has to live as long as they are used."""
     if rows.dim() != 3 or k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
@@ -77,11 +83,14 @@ def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None):
     front of a sequence's beginning (more rows than kv_lens). The places that are written share no memory with k and v, and where two rows go to one place either may
     stay.
 
+    There is no derivative through the cache: under autograd, tensors that ask for a gradient are refused, and so are dual tensors of forward mode.
+
     All lengths and tables are read on the device, so that a captured call follows them. A page number or a length that the cache does not have
     writes nothing and is reported by `check_status`."""
     native = _native(k, v, k_pages, v_pages, page_table, kv_lens, q_starts)
     if native is not None and native[0].paged_append(k, v, k_pages, v_pages, page_table, kv_lens, q_starts, native[1]):
         return
+    _no_tangents(k, v, k_pages, v_pages)
     if v.shape != k.shape or k.shape[1:2] != k_pages.shape[2:3]:
         raise ValueError("flash_b200: k and v must be [T, Hk, D] with the heads of the cache")
     if v.dtype != k.dtype:
@@ -119,7 +128,7 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_
 
     q: [T, H, D], bf16 or fp16, H a multiple of the cache's Hk and at most 128 times that; the rest as in `paged_append`. The new token at position p of its sequence sees the
     tokens 0 to p. sm_scale: 1 / sqrt(D) if None. softcap, slopes, prefix: as in `attention_scored`, the token's position in the place of
-    i + gap; prefix is int32 [B]. A row that sees no token (a length of 0, a position below 0) gives zeros. No gradient.
+    i + gap; prefix is int32 [B]. A row that sees no token (a length of 0, a position below 0) gives zeros. No derivative, as in `paged_append`.
 
     Returns [T, H, D], zeros in the rows of no sequence; or `out`, whose rows of no sequence are left as they were. `out` shares no memory with q
     or the cache. What lies in the pages behind a sequence's length, or in pages that no sequence names, has no influence, also
@@ -133,6 +142,7 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_
             done = native[0].paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts, sm_scale, softcap, slopes, prefix, out, native[1])
             if done is not None:
                 return done if out is None else out
+    _no_tangents(q, k_pages, v_pages, slopes, out)
     cache, starts, held = _checked(q, "q", k_pages, v_pages, page_table, kv_lens, q_starts)
     T, H, D = q.shape
     if cache.Hk == 0 or H == 0 or H % cache.Hk or H // cache.Hk > 128:
