@@ -551,3 +551,23 @@ def test_tangents_are_refused():
                 fb.attention_scored(*args, True, softcap=9.0, slopes=slopes)
         plain = fb.attention_scored(q, k, v, True, softcap=9.0)
     assert torch.equal(plain, fb.attention_scored(q, k, v, True, softcap=9.0))
+
+
+def test_slopes_that_are_a_parameter_without_grad_mode(monkeypatch):
+    """As other inputs that would ask for a gradient: refused under grad mode, taken without, by either way through the host."""
+    import flash_b200 as fb
+    from flash_b200 import ops
+    q, k, v, _ = _inputs(1, 4, 2, 40, 40, 64, BF16, 69)
+    slopes = torch.nn.Parameter(_slopes(4, "series"))
+    pages, table, lens = k.transpose(1, 2)[:, :32].reshape(2, 16, 2, 64).contiguous(), torch.tensor([[0, 1]], dtype=torch.int32, device="cuda"), torch.tensor([32], dtype=torch.int32, device="cuda")
+    calls = (lambda s: fb.attention_scored(q, k, v, True, slopes=s), lambda s: fb.paged_attention(q[0, :, :1].transpose(0, 1), pages, pages, table, lens, slopes=s))
+    for profile in (None, []):
+        monkeypatch.setattr(ops, "PROFILE", profile)
+        for call in calls:
+            with pytest.raises(ValueError, match="gradient"):
+                call(slopes)
+            want = call(slopes.detach())
+            for off in (torch.no_grad, torch.inference_mode):
+                with off():
+                    got = call(slopes)
+                assert torch.equal(got, want) and not got.requires_grad

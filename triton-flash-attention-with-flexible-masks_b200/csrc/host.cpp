@@ -296,7 +296,7 @@ bool scores_of(double softcap, const std::optional<Tensor>& slopes, const std::o
     if (!(softcap == 0.0 || (softcap >= 1e-6 && softcap <= 1e6))) return false;
     auto vector = [&](const Tensor& t, at::ScalarType type, int64_t n) {
         return t.is_cuda() && t.layout() == at::kStrided && t.dim() == 1 && t.size(0) == n && t.scalar_type() == type && t.is_contiguous() && !t.is_neg() &&
-               t.device() == q.device() && !t.requires_grad();
+               t.device() == q.device() && !(at::GradMode::is_enabled() && t.requires_grad());
     };
     if ((slopes && !vector(*slopes, at::kFloat, H)) || (prefix && !vector(*prefix, at::kInt, B))) return false;
     s = fa_scores{float(softcap), slopes ? slopes->const_data_ptr<float>() : nullptr, prefix ? prefix->const_data_ptr<int>() : nullptr};

@@ -32,7 +32,7 @@ def _checked_slopes(slopes, H, q):
         return None
     if not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32 or slopes.shape != (H,):
         raise ValueError(f"flash_b200: slopes must be a float32 tensor of shape [H] = [{H}]")
-    if slopes.requires_grad:
+    if slopes.requires_grad and torch.is_grad_enabled():
         raise ValueError("flash_b200: slopes are constants of the operator (there is no gradient for them); pass slopes.detach()")
     _same_device(q, slopes=slopes)
     return slopes.resolve_neg().contiguous()
@@ -146,7 +146,7 @@ def attention_scored(q, k, v, causal=False, sm_scale=None, eq=None, ek=None, sco
     softcap: None or 0 for none, else from 1e-6 to 1e6. slopes: float32 [H], None for none. prefix: int32 or int64 [bs], None for none; it
     needs causal=True, values are taken into [0, N]. All else is as in `attention`: types (bf16, fp16, fp32), head dims, grouped heads, strides, a row
     that the masks leave no key gives zeros and takes no part in the gradients. There are gradients for q, k and v, once; slopes and
-    prefix are constants, and slopes that ask for a gradient are refused. As in `attention`, masked entries are products with an exact 0: a
+    prefix are constants, and slopes that ask for a gradient are refused unless grad mode is off. As in `attention`, masked entries are products with an exact 0: a
     value that is not finite may spread from a key that some query of its block of 128 sees."""
     softcap = _checked_softcap(softcap)
     if softcap == 0.0 and slopes is None and prefix is None:
