@@ -267,13 +267,13 @@ __global__ void __launch_bounds__(threads(R), R == 32 && D <= 32 ? 4 : 0) f32_fw
     const int32_t* kcodes = mk.mode == 1 ? mk.plan + mk.L.off_kc + (int64_t(b) * mk.He + he) * mk.L.Npad : nullptr;
     const int front = front_keys<SCORED>(mk, b);
     const float slope = slope_of<SCORED>(p, h);
-    const int end = mk.causal ? min(mk.N, max(i0 + R + mk.gap, front)) : mk.N;  // keys beyond the last row's causal bound
+    const int end = mk.causal ? min(mk.N, SCORED ? max(i0 + R + mk.gap, front) : i0 + R + mk.gap) : mk.N;  // keys beyond the last row's causal bound
     // In a block of 32 rows those beyond the first half's: the values there stay out of its P V, for a product with a P of 0 may be NaN.
     // What a NaN or an infinity reaches then does not go by the size of the blocks, which goes by what a sequence is batched with. us, forward and
     // forward with backward, products over the whole tile | over what the half sees: 4 x 8 heads x 1024 x 64 causal 179, 726 | 177, 712, not causal
     // 324, 1342 | 324, 1329; 4 x 8 x 1024 x 128 causal 363, 1462 | 359, 1466; 8 x 16 x 512 x 32 causal 121, 496 | 119, 488, not causal 205, 855 | 208, 859
     // (four blocks of head dims up to 32 share an SM only while a thread has 64 registers: 211 with three).
-    const int end_half = mk.causal && r0 < 16 ? max(i0 + 16 + mk.gap, front) : mk.N + kC;
+    const int end_half = mk.causal && r0 < 16 ? (SCORED ? max(i0 + 16 + mk.gap, front) : i0 + 16 + mk.gap) : mk.N + kC;
     auto fetch = [&](int j0, int st) {
         load_tile<D, kC, R>(KVs + st * 2 * S::cols, kbase, p.k.sl, kvec, j0, end);
         load_tile<D, kC, R>(KVs + (st * 2 + 1) * S::cols, vbase, p.v.sl, vvec, j0, end);
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(threads(R), R == 32 && D <= 32 ? 4 : 0) f32_fw
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int j = j0 + x + 32 * c;
-                const bool keep = keep_entry(i, j, qc[r], kcodes ? codes[st * kC + x + 32 * c] : 0, mk.N, mk.gap, mk.causal, mk.mode, front);
+                const bool keep = keep_entry<SCORED>(i, j, qc[r], kcodes ? codes[st * kC + x + 32 * c] : 0, mk.N, mk.gap, mk.causal, mk.mode, front);
                 float factor;
                 s[r][c] = keep ? score_f32<SCORED>(p, s[r][c], slope, i, j, factor) : -INFINITY;
                 mx = fmaxf(mx, s[r][c]);
@@ -391,8 +391,8 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dq_kernel(const F32Params 
     const int32_t* kcodes = mk.mode == 1 ? mk.plan + mk.L.off_kc + (int64_t(b) * mk.He + he) * mk.L.Npad : nullptr;
     const int front = front_keys<SCORED>(mk, b);
     const float slope = slope_of<SCORED>(p, h);
-    const int end = mk.causal ? min(mk.N, max(i0 + R + mk.gap, front)) : mk.N;  // keys beyond the last row's causal bound
-    const int end_half = mk.causal && r0 < 16 ? max(i0 + 16 + mk.gap, front) : mk.N + kC;  // (see the forward)
+    const int end = mk.causal ? min(mk.N, SCORED ? max(i0 + R + mk.gap, front) : i0 + R + mk.gap) : mk.N;  // keys beyond the last row's causal bound
+    const int end_half = mk.causal && r0 < 16 ? (SCORED ? max(i0 + 16 + mk.gap, front) : i0 + 16 + mk.gap) : mk.N + kC;  // (see the forward)
     auto fetch = [&](int j0, int st) {
         load_tile<D, kC, R>(KVs + st * 2 * S::cols, kbase, p.k.sl, kvec, j0, end);
         load_tile<D, kC, R>(KVs + (st * 2 + 1) * S::cols, vbase, p.v.sl, vvec, j0, end);
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dq_kernel(const F32Params 
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int j = j0 + x + 32 * c;
-                const bool keep = (i < mk.M) && keep_entry(i, j, qc[r], kcodes ? codes[st * kC + x + 32 * c] : 0, mk.N, mk.gap, mk.causal, mk.mode, front);
+                const bool keep = (i < mk.M) && keep_entry<SCORED>(i, j, qc[r], kcodes ? codes[st * kC + x + 32 * c] : 0, mk.N, mk.gap, mk.causal, mk.mode, front);
                 float factor;
                 const float pe = keep ? expf(score_f32<SCORED>(p, s[r][c], slope, i, j, factor) - lse[r]) : 0.f;  // a kept entry has a finite lse
                 dp[r][c] = keep ? pe * (dp[r][c] - dl[r]) * factor : 0.f;  // dS (flash_triton.py:301)
@@ -486,8 +486,8 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
     dv.clear();
     // first query row that can see key j0 under the causal mask (flash_triton.py:214-218)
     const int front = front_keys<SCORED>(mk, b);
-    const int first = mk.causal && j0 >= front ? max(0, j0 - mk.gap) : 0;
-    const int first_half = mk.causal && r0 >= 16 && j0 + 16 >= front ? j0 + 16 - mk.gap : 0;  // the same for the second half of 32 keys (see the forward)
+    const int first = mk.causal && (!SCORED || j0 >= front) ? max(0, j0 - mk.gap) : 0;
+    const int first_half = mk.causal && r0 >= 16 && (!SCORED || j0 + 16 >= front) ? j0 + 16 - mk.gap : 0;  // the same for the second half of 32 keys (see the forward)
     for (int g = 0; g < p.G; ++g) {
         const int h = hk * p.G + g;
         const int he = (mk.He == 1) ? 0 : h;
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
                 const float lse = vec[kC + x + 32 * c], dl = vec[2 * kC + x + 32 * c];
 #pragma unroll
                 for (int r = 0; r < kRW; ++r) {
-                    const bool keep = (i < mk.M) && keep_entry(i, j0 + r0 + r, qc, kc[r], mk.N, mk.gap, mk.causal, mk.mode, front);
+                    const bool keep = (i < mk.M) && keep_entry<SCORED>(i, j0 + r0 + r, qc, kc[r], mk.N, mk.gap, mk.causal, mk.mode, front);
                     float factor;
                     const float pe = keep ? expf(score_f32<SCORED>(p, s[r][c], slope, i, j0 + r0 + r, factor) - lse) : 0.f;
                     s[r][c] = pe;

@@ -112,7 +112,7 @@ enum : uint32_t {
 
 // Classification of tile (qb, kb) from the block statistics. Conservative: a tile is skipped
 // only when every entry is masked, and declared free of a check only when every entry passes it.
-// front: leading keys that the causal mask does not hide.
+// front: leading keys that the causal mask does not hide; nothing is left of it where it is the constant 0.
 __host__ __device__ inline uint32_t classify_tile(int qb, int kb, int M, int N, int gap, int causal,
                                                   int mode, int qmin, int qmax, int kmin, int kmax, int front = 0) {
     const int q0 = qb * kBlk, k0 = kb * kBlk;
@@ -122,8 +122,8 @@ __host__ __device__ inline uint32_t classify_tile(int qb, int kb, int M, int N, 
     if (k0 + kBlk > N) f |= TILE_BOUND;
     if (q0 + kBlk > M) f |= TILE_QTAIL;
     if (causal) {
-        if (k0 > q1 - 1 + gap && k0 >= front) return 0;
-        if (k1 - 1 > q0 + gap && k1 > front) f |= TILE_BOUND;
+        if (k0 > q1 - 1 + gap && (front <= 0 || k0 >= front)) return 0;
+        if (k1 - 1 > q0 + gap && (front <= 0 || k1 > front)) f |= TILE_BOUND;
     }
     if (mode == 1) {
         if (qmax < 0 && (kmax < qmin || kmin > qmax)) return 0;
@@ -192,7 +192,7 @@ __device__ __forceinline__ void q_range(const MaskArgs& a, int b, int he, int kb
         hi = a.L.nQ;
         if (a.causal) {
             const int first = kb * kBlk - a.gap;  // first query row that sees key k0
-            lo = first > 0 && kb * kBlk >= front_keys<kPrefix>(a, b) ? first / kBlk : 0;
+            lo = first > 0 && (!kPrefix || kb * kBlk >= front_keys<kPrefix>(a, b)) ? first / kBlk : 0;
             if (lo > hi) lo = hi;
         }
     }
@@ -201,9 +201,10 @@ __device__ __forceinline__ void q_range(const MaskArgs& a, int b, int he, int kb
 // The per-entry predicate on codes. Identical to the reference's rule on the original ids:
 // qc >= 0 <=> eq >= 0; for eq < 0, qc == eq and kc == ek whenever ek is a negative int32,
 // and kc == 0 != qc otherwise.
+template <bool kPrefix = false>
 __device__ __forceinline__ bool keep_entry(int i, int j, int qc, int kc, int N, int gap, int causal, int mode, int front = 0) {
     bool keep = j < N;
-    if (causal) keep = keep && (gap + i >= j || j < front);
+    if (causal) keep = keep && (gap + i >= j || (kPrefix && j < front));
     if (mode == 1) keep = keep && ((qc >= 0) || (qc == kc));
     return keep;
 }
