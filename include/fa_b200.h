@@ -185,6 +185,8 @@ int fa_plan_build_scored(const fa_problem* p, const fa_scores* scores, const fa_
                          int32_t* status, void* stream);
 int fa_fwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o, void* rest,
                   float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* The same rest of a forward that fa_fwd_scored has cut into splits > 1 runs, from the workspace that it has left, by a kernel of its own. */
+int fa_fwd_rest(const fa_problem* p, int32_t splits, const void* workspace, size_t workspace_bytes, void* rest, int32_t* status, void* stream);
 int fa_bwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
                   const void* rest, const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv,
                   const void* plan, int32_t* status, void* stream);

@@ -102,3 +102,13 @@ def test_the_forward_reads_no_prefix_before_the_kernel_before_it_is_complete():
     assert re.findall(r"if \([^\n]*\bprepare\(|\bprepare\(", before) == ["if (warp == 14 && early) item = prepare("]
     assert not re.search(r"\b(front_keys|slopes|prefix\[)", before)
     assert "if ((k > 0 || !early) && j < n_items) item = prepare(j);" in kernel[wait:]
+
+
+def test_what_the_library_refuses_of_a_rest_of_runs():
+    lib = _lib.load()
+    prob = _problem(M=16, N=1024)
+    call = lambda p=prob, splits=2, work=256, size=1 << 30, rest=256, status=256: lib.fa_fwd_rest(p, splits, work, size, rest, status, None)  # noqa: E731
+    assert call(_problem(D=48)) == 2 and call(_problem(M=16, N=1024, dtype=2)) == 2 and call(_problem(M=16, N=1024, mode=1)) == 2 and call(splits=9) == 2
+    assert call(splits=1) == 1 and call(rest=None) == 1 and call(status=None) == 1
+    assert call(work=None) == 6 and call(size=100) == 6
+    assert call(work=264) == 3 and call(rest=264) == 3

@@ -14,7 +14,7 @@ cudaError_t launch_plan_clear(int32_t*, int, cudaStream_t);
 cudaError_t launch_debug_mask(const MaskArgs&, uint8_t*, uint8_t*, cudaStream_t);
 cudaError_t launch_fwd(int, bool, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
                        const FwdParams&, int, cudaStream_t);
-cudaError_t launch_fwd_combine(bool, const CombineParams&, cudaStream_t);
+cudaError_t launch_fwd_combine(bool, bool, const CombineParams&, cudaStream_t);
 cudaError_t launch_bwd_delta(const DeltaParams&, cudaStream_t);
 cudaError_t launch_bwd_dkdv(int, bool, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
                             const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const DkdvParams&, int,
@@ -389,7 +389,7 @@ int run_fwd(const fa_problem* p, const fa_scores* sc, void* rest, const fa_tenso
     cudaError_t e = fa::launch_fwd(p->D, p->dtype == FA_BF16, tq, tk, tv, to, fp, sms, static_cast<cudaStream_t>(stream));
     if (e == cudaSuccess && splits > 1) {
         fa::CombineParams cp{fp.part_o, fp.part_lse, out_view(o), lse, p->B, p->H, p->M, p->D, dk, splits, fa::pad128(p->M), status};
-        e = fa::launch_fwd_combine(p->dtype == FA_BF16, cp, static_cast<cudaStream_t>(stream));
+        e = fa::launch_fwd_combine(p->dtype == FA_BF16, false, cp, static_cast<cudaStream_t>(stream));
     }
     return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
@@ -621,6 +621,21 @@ int fa_fwd_split(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, co
 int fa_fwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o, void* rest,
                   float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
     return scores ? run_fwd(p, scores, rest, q, k, v, o, lse, plan, splits, workspace, workspace_bytes, status, stream) : FA_ERR_BAD_ARG;
+}
+
+int fa_fwd_rest(const fa_problem* p, int32_t splits, const void* workspace, size_t workspace_bytes, void* rest, int32_t* status, void* stream) {
+    const int rc = check_problem(p);
+    if (rc) return rc;
+    if (splits < 2 || !rest || !status) return FA_ERR_BAD_ARG;
+    if (p->mode != FA_MODE0_NOPE || p->dtype == FA_FP32 || splits > fa::cdiv(p->N, fa::kBlk)) return FA_ERR_UNSUPPORTED;
+    if (!workspace || workspace_bytes < fwd_workspace_bytes(p, splits)) return FA_ERR_PLAN_SIZE;
+    if (!aligned16(workspace) || !aligned16(rest)) return FA_ERR_ALIGNMENT;
+    const int64_t rows = int64_t(p->M) * p->H;
+    const int dk = p->D > 64 ? 128 : 64;
+    const float* part_o = static_cast<const float*>(workspace);
+    const fa_tensor r{rest, {rows * p->D, int64_t(p->M) * p->D, p->D, 1}};
+    const fa::CombineParams cp{part_o, part_o + rows * p->B * splits * dk, out_view(&r), nullptr, p->B, p->H, p->M, p->D, dk, splits, fa::pad128(p->M), status};
+    return fa::launch_fwd_combine(p->dtype == FA_BF16, true, cp, static_cast<cudaStream_t>(stream)) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
 int fa_bwd_delta(const fa_problem* p, const fa_tensor* o, const fa_tensor* d_o, float* delta, void* stream) {

@@ -880,7 +880,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
 // in fp32 in the order of the parts. Bound by latency: at most 20 MB are read (fwd_splits in api.cu), mostly from L2, so that eight parts' loads are in flight
 // together. A call of one token, 32 / 8 heads of 128, us, four parts behind their own weights | now: 4096 keys in 16 runs 16.1 | 12.7, 16384 in 16 20.7 |
 // 17.3; 2 x 64 / 8 heads, 3000 in 8 14.5 | 13.0.
-template <bool BF16>
+// REST: not the result, but what its rounding leaves out, rounded itself (see the forward), goes to `o`, and no LSE.
+template <bool BF16, bool REST = false>
 __global__ void __launch_bounds__(256) fwd_combine_kernel(const CombineParams p) {
     follow_stream();
     const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);  // of the [B, H, M] rows
@@ -890,7 +891,7 @@ __global__ void __launch_bounds__(256) fwd_combine_kernel(const CombineParams p)
     const int64_t bh = row / p.M;
     const int i = int(row - bh * p.M);
     float* lse = p.lse + bh * p.Mpad;
-    if (i == p.M - 1)  // the rows past M that pad the buffer
+    if (!REST && i == p.M - 1)  // the rows past M that pad the buffer
         for (int64_t x = p.M + lane; x < p.Mpad; x += 32) lse[x] = 0.f;
     const bool failed = status_is_fatal(*p.status);  // the forward left no parts: NaN, as the other kernels do
     float mx = -INFINITY;
@@ -940,13 +941,21 @@ __global__ void __launch_bounds__(256) fwd_combine_kernel(const CombineParams p)
     const int b = int(bh / p.H), h = int(bh - int64_t(b) * p.H);
     uint16_t* out = static_cast<uint16_t*>(p.o.ptr) + int64_t(b) * p.o.sb + int64_t(h) * p.o.sh + int64_t(i) * p.o.sl;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (lane + 32 * k < p.D) out[lane + 32 * k] = failed ? uint16_t(0xffff) : uint16_t(pack2<BF16>(acc[k] * inv, 0.f));
-    if (lane == 0) lse[i] = (total > 0.f && !spoilt) ? mx + log2f(total) : -INFINITY;
+    for (int k = 0; k < 4; ++k) {
+        float x = acc[k] * inv;
+        if constexpr (REST) {
+            float rounded, none;
+            unpack2<BF16>(pack2<BF16>(x, 0.f), rounded, none);
+            x -= rounded;
+        }
+        if (lane + 32 * k < p.D) out[lane + 32 * k] = failed ? uint16_t(0xffff) : uint16_t(pack2<BF16>(x, 0.f));
+    }
+    if (!REST && lane == 0) lse[i] = (total > 0.f && !spoilt) ? mx + log2f(total) : -INFINITY;
 }
 
-cudaError_t launch_fwd_combine(bool bf16, const CombineParams& p, cudaStream_t stream) {
+cudaError_t launch_fwd_combine(bool bf16, bool rest, const CombineParams& p, cudaStream_t stream) {
     const unsigned grid = unsigned((int64_t(p.B) * p.H * p.M + 7) / 8);
+    if (rest) return launch_overlapping(bf16 ? fwd_combine_kernel<true, true> : fwd_combine_kernel<false, true>, dim3(grid), 256, 0, stream, p);
     return launch_overlapping(bf16 ? fwd_combine_kernel<true> : fwd_combine_kernel<false>, dim3(grid), 256, 0, stream, p);
 }
 

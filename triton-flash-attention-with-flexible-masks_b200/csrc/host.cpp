@@ -137,14 +137,16 @@ Outputs launch_forward(const fa_problem& p, const Tensor& q, const Tensor& k, co
     const fa_tensor tq = view(q), tk = view(k), tv = view(v), to = view(r.o);
     void* const plan_ptr = plan.defined() ? plan.data_ptr() : nullptr;
     void* const work_ptr = work.defined() ? work.data_ptr() : nullptr;
-    if (scores && backward && r.splits == 1 && p.dtype != FA_FP32) r.rest = at::empty({p.B, p.H, p.M, p.D}, q.options());
+    if (scores && backward && p.dtype != FA_FP32) r.rest = at::empty({p.B, p.H, p.M, p.D}, q.options());
     if (scores)
-        check(fa_fwd_scored(&p, scores, &tq, &tk, &tv, &to, r.rest.defined() ? r.rest.data_ptr() : nullptr, r.lse.data_ptr<float>(), plan_ptr, r.splits, work_ptr, bytes, status.data_ptr<int>(),
+        check(fa_fwd_scored(&p, scores, &tq, &tk, &tv, &to, r.rest.defined() && r.splits == 1 ? r.rest.data_ptr() : nullptr, r.lse.data_ptr<float>(), plan_ptr, r.splits, work_ptr, bytes, status.data_ptr<int>(),
                             current_stream(q)),
               "fa_fwd_scored");
     else
         check(fa_fwd_split(&p, &tq, &tk, &tv, &to, r.lse.data_ptr<float>(), plan_ptr, r.splits, work_ptr, bytes, status.data_ptr<int>(), current_stream(q)),
               "fa_fwd_split");
+    if (r.rest.defined() && r.splits > 1)
+        check(fa_fwd_rest(&p, r.splits, work_ptr, bytes, r.rest.data_ptr(), status.data_ptr<int>(), current_stream(q)), "fa_fwd_rest");
     return r;
 }
 
@@ -314,7 +316,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
         py::gil_scoped_release free;
         if (c.eq || !fa_plan_optional(&c.p, c.needs_grad)) plan = build_plan(c.p, c.eq, c.ek, c.status, &s);
         Outputs r = launch_forward(c.p, q, k, v, plan, 0, c.status, std::nullopt, &s, c.needs_grad);
-        n_launched += (plan.defined() ? c.plan_kernels : 0) + (r.splits > 1 ? 2 : 1);
+        n_launched += (plan.defined() ? c.plan_kernels : 0) + (r.splits > 1 ? 2 + r.rest.defined() : 1);
         return r;
     }
 

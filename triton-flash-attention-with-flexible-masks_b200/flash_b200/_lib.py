@@ -17,7 +17,7 @@ EXPORTS = (
     "fa_version", "fa_error_string", "fa_padded_rows", "fa_plan_bytes", "fa_plan_build", "fa_fwd",
     "fa_bwd_delta", "fa_bwd_dkdv", "fa_bwd_dq", "fa_debug_mask", "fa_classify_tile", "fa_fwd_static_plan",
     "fa_debug_wait_timeout", "fa_group_rows", "fa_permute_rows", "fa_fwd_splits", "fa_fwd_workspace_bytes", "fa_fwd_split",
-    "fa_plan_optional", "fa_bwd", "fa_plan_build_scored", "fa_fwd_scored", "fa_bwd_scored", "fa_paged_append",
+    "fa_plan_optional", "fa_bwd", "fa_plan_build_scored", "fa_fwd_scored", "fa_fwd_rest", "fa_bwd_scored", "fa_paged_append",
     "fa_paged_workspace_bytes", "fa_paged_fwd", "fa_debug_paged_pieces",
 )
 
@@ -100,6 +100,8 @@ def load():
     lib.fa_plan_build_scored.argtypes = [P, S, I, I, vp, size, vp, vp]
     lib.fa_fwd_scored.restype = i32
     lib.fa_fwd_scored.argtypes = [P, S, T, T, T, T, vp, vp, vp, ctypes.c_int32, vp, size, vp, vp]
+    lib.fa_fwd_rest.restype = i32
+    lib.fa_fwd_rest.argtypes = [P, ctypes.c_int32, vp, size, vp, vp, vp]
     lib.fa_bwd_scored.restype = i32
     lib.fa_bwd_scored.argtypes = [P, S, T, T, T, T, vp, T, vp, vp, T, T, T, vp, vp, vp]
     C, R = ctypes.POINTER(PagedCache), ctypes.POINTER(Rows)

@@ -101,11 +101,13 @@ class ScoredAttention(torch.autograd.Function):
                 _lib.check(lib.fa_fwd_workspace_bytes(prob, splits, size), "fa_fwd_workspace_bytes")
                 work = torch.empty(size.value // 4, dtype=torch.float32, device=device)
             # what the rounding of the output leaves out, for the gradients
-            rest = torch.empty((B, H, M, D), dtype=q.dtype, device=device) if needs_grad and splits == 1 and q.dtype != torch.float32 else None
-            with ops._timed("fwd", 2 if splits > 1 else 1):
-                _lib.check(lib.fa_fwd_scored(prob, scores, _tensor(q), _tensor(k), _tensor(v), _tensor(out), _pointer(rest), lse.data_ptr(),
+            rest = torch.empty((B, H, M, D), dtype=q.dtype, device=device) if needs_grad and q.dtype != torch.float32 else None
+            with ops._timed("fwd", (2 if splits > 1 else 1) + (splits > 1 and rest is not None)):
+                _lib.check(lib.fa_fwd_scored(prob, scores, _tensor(q), _tensor(k), _tensor(v), _tensor(out), _pointer(rest) if splits == 1 else None, lse.data_ptr(),
                                              _pointer(plan), splits, _pointer(work),
                                              size.value, status.data_ptr(), stream), "fa_fwd_scored")
+                if splits > 1 and rest is not None:
+                    _lib.check(lib.fa_fwd_rest(prob, splits, work.data_ptr(), size.value, rest.data_ptr(), status.data_ptr(), stream), "fa_fwd_rest")
             if ops._SYNC_STATUS:
                 check_status(device)
         if needs_grad:
