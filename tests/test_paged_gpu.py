@@ -495,3 +495,21 @@ def test_a_time_out_on_record_while_the_call_runs(given):
     for x in (got[:front], got[front + sum(new):]):
         assert (x == 7.0).all() if given else torch.isnan(x).all()
     assert torch.equal(call(), want)
+
+
+@pytest.mark.parametrize("cap", [None, 3.0])
+@pytest.mark.parametrize("D, G, at", [(64, 4, 470), (128, 4, 470), (64, 1, 470), (128, 30, 425)])
+def test_a_later_token_of_a_chunk_that_is_not_finite(D, G, at, cap):
+    """100 tokens behind 400, keys and values from position `at` on NaN and infinite: they lie in the same 128 keys as what earlier blocks of 128 / G tokens see, none of whose
+    rows sees them."""
+    import flash_b200 as fb
+    cache = Cache([500, 77], 2, D, 16, BF16, 27).fill()
+    q = torch.randn(101, 2 * G, D, device="cuda").to(BF16)
+    call = lambda: fb.paged_attention(q, cache.k_pages, cache.v_pages, cache.table, cache.kv_lens, _starts([100, 1]), softcap=cap)  # noqa: E731
+    want, block = call(), 128 // G
+    place = cache.places(0, at, 500)
+    cache.k_pages[place], cache.v_pages[place] = float("nan"), float("inf")
+    got, clean = call(), (at - 400) // block * block  # rows of blocks that end in front of it
+    assert torch.equal(got[:clean], want[:clean]) and torch.equal(got[100:], want[100:])
+    assert not torch.isfinite(got[at - 400: 100]).any()
+    fb.check_status()

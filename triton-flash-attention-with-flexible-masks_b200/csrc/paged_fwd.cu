@@ -9,8 +9,8 @@
 //    token of 32 / 8 heads reads its keys once instead of four times;
 //  - a tile of 128 keys is 128 / page size boxes, one a page, which land one behind the other in the tile (a page of 8 rows is one
 //    swizzle atom); the producers' lanes read the page numbers of the next tile while this one is under way;
-//  - P of a masked entry is 0, but 0 times a NaN that an earlier user left in the page is not: rows of V behind the sequence's end are
-//    zeroed in shared memory by the softmax group before it gives its P away (not by the warp that issues P V: its code has to stay free of loops by
+//  - P of a masked entry is 0, but 0 times a NaN that an earlier user left in the page, or that a later token of the chunk has, is not: rows of V behind the last that the item
+//    sees are zeroed in shared memory by the softmax group before it gives its P away (not by the warp that issues P V: its code has to stay free of loops by
 //    lanes, or the descriptors go through vector registers);
 //  - items of at most 32 rows (a decoded token's heads) take the tile four times over, so that each of a group's four warps has 32 keys of every row instead of 32 rows of
 //    which most are nobody's: the chain from the scores to P is a quarter as long. 64 single tokens, 32 / 8 heads of 128, capped, 251 -> 218 us;
@@ -480,7 +480,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const uint32_t tO = tmem + lane_base + uint32_t(S::tmem_o + w * D);
         const int tok_wide = r / p.G, tok_narrow = lane / p.G;
         bool alive = !aborted;
-        // Rows of V behind the sequence's end hold what was in the page, or in the stage: zeros, before P*V(g) is issued. A quarter of them a warp.
+        // Rows of V behind the keys that the item sees hold what was in the page, or in the stage: zeros, before P*V(g) is issued. A quarter of them a warp.
         auto zero_behind = [&](int g, int real) {
             const int st = g % NS;
             if (!mbar_wait_warp(BAR(B_VFULL + st), (g / NS) & 1, ab, ST_WAIT_TIMEOUT + 19)) return false;
@@ -518,6 +518,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             const int pos = pos0 + tok;
             const int last = min(max(pos, front - 1), len - 1);                // the last key that this row sees
             const int all_see = min(max(pos0, front - 1), len - 1);            // and that all rows of the tile see
+            const int seen = min(max(pos0 + tokens, front), len);              // keys that any row sees
             float slope = 0.f;
             if constexpr (SCORED) {
                 if (p.score.slopes) slope = p.score.slopes[int64_t(it[I_HEAD]) * p.G + g_row] * kScoreLog2e;
@@ -540,7 +541,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         alive = pv_before();
                         if (!alive) break;
                     }
-                    if (len - k0 < kBlk) alive = zero_behind(g, len - k0);
+                    if (seen - k0 < kBlk) alive = zero_behind(g, seen - k0);
                     if (!alive) break;
                     mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
                     continue;
@@ -558,9 +559,9 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
                     float* v = reinterpret_cast<float*>(sq);
                     if constexpr (SCORED) {
-                        if (len - kq < 32) {
+                        if (seen - kq < 32) {
 #pragma unroll
-                            for (int x = 0; x < 32; ++x) v[x] = x < len - kq ? v[x] : 0.f;
+                            for (int x = 0; x < 32; ++x) v[x] = x < seen - kq ? v[x] : 0.f;
                         }
                         const Bias bias(slope, front == 0, pos0 - (kq + 31), pos0 + 31 - kq);
                         score_row<KIND, 32>(v, p.score, bias, p.scale_log2, pos - kq, valid, m_run == -INFINITY ? 0.f : m_run);
@@ -616,7 +617,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         if (q != quarter) tmem_st16(tP + uint32_t(q) * 16u, zero);
                     tmem_st16(tP + uint32_t(quarter) * 16u, pk);
                     tc_wait_st();
-                    if (len - k0 < kBlk) alive = zero_behind(g, len - k0);
+                    if (seen - k0 < kBlk) alive = zero_behind(g, seen - k0);
                     tc_fence_before();
                     mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
                     if (!alive) break;
@@ -632,7 +633,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     mbar_arrive_warp(BAR(B_SFREE + w), lane);  // the next tile's scores may overwrite these
                 }
                 float* sc = reinterpret_cast<float*>(sr);
-                const int real = len - k0;  // keys of the tile that there are
+                const int real = seen - k0;  // keys of the tile that some row sees
                 // A capped tile without a mask is not capped before its exponentials: the greatest score tells the greatest capped one, and the polynomial
                 // runs beside the special-function unit. (With a bias the greatest one has to be looked for behind it.)
                 bool late = false;
