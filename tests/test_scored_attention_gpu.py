@@ -611,3 +611,26 @@ def test_gradients_of_few_queries_where_a_few_keys_carry_a_row(hooked):
     for name in ("dq", "dk"):
         value = want[name][0]
         assert ((got[name].double() - value).norm() / value.norm()).item() < 3.9e-3, name
+
+
+@pytest.mark.parametrize("hooked", [False, True])  # the native node, and the one in Python
+def test_second_gradients_are_refused_beside_others(hooked):
+    """A penalty on the gradients, added to a loss that has gradients of its own, raises: nothing of it is lost. The first gradients are what they are without a graph."""
+    import flash_b200 as fb
+    q, k, v, do = _inputs(1, 4, 2, 40, 40, 64, BF16, 72)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+
+    def forward():
+        with (torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: x) if hooked else contextlib.nullcontext()):
+            return fb.attention_scored(*leaves, True, softcap=5.0)
+
+    want = torch.autograd.grad(forward(), leaves, do)
+    for asks in (False, True):
+        o = forward()
+        grads = torch.autograd.grad(o, leaves, do.detach().requires_grad_(asks), create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(grads, want))
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(o.sum() + grads[0].square().sum(), leaves)
+    o = forward()
+    o.backward(do, create_graph=True)
+    assert all(torch.equal(x.grad, g) for x, g in zip(leaves, want))

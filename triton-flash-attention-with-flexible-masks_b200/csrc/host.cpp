@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_cpp_function.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/types.h>
@@ -305,6 +306,16 @@ bool scores_of(double softcap, const std::optional<Tensor>& slopes, const std::o
     return true;
 }
 
+// Gradients that a graph is to be made of: an error waits between them and q, k and v, where there would be nothing (scored._once).
+void once(std::array<Tensor, 3>& g, const Tensor& q, const Tensor& k, const Tensor& v) {
+    if (!at::GradMode::is_enabled()) return;
+    torch::autograd::variable_list in{q, k, v};
+    for (int i = 0; i < 3; ++i) in.insert(in.begin() + i, g[i].detach().set_requires_grad(true));
+    torch::autograd::DelayedError error("flash_b200: attention_scored has gradients once; these cannot be differentiated", 6);
+    auto out = error.apply(std::move(in));
+    for (int i = 0; i < 3; ++i) g[i] = std::move(out[i]);
+}
+
 // The autograd node of a regular call of attention_scored, as scored.ScoredAttention.
 struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
     struct Scores {
@@ -362,6 +373,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
         if (!taken_as_is(d_o)) d_o = d_o.contiguous();  // (ops.maybe_contiguous)
         auto g = launch_backward(p, d_o, q, k, v, saved[3], saved[4], data["plan"].toTensor(), data["status"].toTensor(), &s, rest);
         n_launched += 3;
+        once(g, q, k, v);
         return {std::move(g[0]), std::move(g[1]), std::move(g[2]), Tensor(), Tensor()};
     }
 };

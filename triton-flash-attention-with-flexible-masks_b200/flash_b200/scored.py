@@ -7,8 +7,6 @@ import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
-
 from . import _lib, ops
 from .ops import (SCORE_FUNC_MODE0_NOPE, SCORE_FUNC_MODE1_DOC, _count, _current, _id_tensor, _ids, _plan_kernels, _PermuteRows, _problem,
                   _same_device, _status_word, _stream, _tensor, attention, check_status, group_rows, maybe_contiguous)
@@ -65,6 +63,14 @@ def _scores(softcap, slopes, prefix):
     return _lib.Scores(softcap, _pointer(slopes), _pointer(prefix))
 
 
+def _once(grads, inputs):
+    """Gradients that a graph is to be made of (create_graph=True): an error waits between them and the inputs, where there would be nothing."""
+    if not torch.is_grad_enabled():
+        return grads
+    error = torch._C._functions.DelayedError(b"flash_b200: attention_scored has gradients once; these cannot be differentiated", 6)
+    return error(*(g.detach().requires_grad_() for g in grads), *inputs)[:3]
+
+
 class ScoredAttention(torch.autograd.Function):
     """The autograd node of `attention_scored`. Saves q, k, v, the output, its log-sum-exp, the slopes and prefix that there are, and what the rounding
     of the output has left out."""
@@ -118,12 +124,11 @@ class ScoredAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, do):
         q, k, v, out, lse, *extra = ctx.saved_tensors
         slopes, prefix, rest = (extra.pop(0) if has else None for has in ctx.has)
         lib, device, plan = _lib.load(), q.device, ctx.plan
-        do = maybe_contiguous(do.to(q.dtype))
+        do = maybe_contiguous(do.detach().to(q.dtype))
         with _current(device):
             delta = torch.empty_like(lse)
             dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
@@ -133,7 +138,7 @@ class ScoredAttention(torch.autograd.Function):
             _count(3)
             if ops._SYNC_STATUS:
                 check_status(device)
-        return (dq, dk, dv) + (None,) * 8
+        return (*_once((dq, dk, dv), (q, k, v)), *(None,) * 8)
 
 
 def attention_scored(q, k, v, causal=False, sm_scale=None, eq=None, ek=None, score_func_mode=SCORE_FUNC_MODE0_NOPE, softcap=None, slopes=None,
@@ -147,7 +152,7 @@ def attention_scored(q, k, v, causal=False, sm_scale=None, eq=None, ek=None, sco
 
     softcap: None or 0 for none, else from 1e-6 to 1e6. slopes: float32 [H], None for none. prefix: int32 or int64 [bs], None for none; it
     needs causal=True, values are taken into [0, N]. All else is as in `attention`: types (bf16, fp16, fp32), head dims, grouped heads, strides, a row
-    that the masks leave no key gives zeros and takes no part in the gradients. There are gradients for q, k and v, once; slopes and
+    that the masks leave no key gives zeros and takes no part in the gradients. There are gradients for q, k and v, once (with create_graph=True, to differentiate them raises); slopes and
     prefix are constants, and slopes that ask for a gradient are refused unless grad mode is off. As in `attention`, masked entries are products with an exact 0: a
     value that is not finite may spread from a key that some query of its block of 128 sees."""
     softcap = _checked_softcap(softcap)
