@@ -16,12 +16,13 @@
  *  - every function enqueues on `stream` and returns without synchronising;
  *  - return value 0 = ok, otherwise an FA_ERR_* code (fa_error_string() describes it);
  *  - `status` is one int32 in device memory, zeroed by the caller. Kernels write a non-zero
- *    code there when a bounded wait ran out (100..199) or an id was out of range (200); the
- *    first code wins. A time-out code is sticky: while the word holds one, every later
- *    fa_fwd / fa_bwd_dkdv / fa_bwd_dq launch given that word computes nothing and fills its
+ *    code there when a bounded wait ran out (100..199), an id was out of range (200), or a page or
+ *    a length of a paged cache was (201, 202). The first code stays, but a time-out takes the place
+ *    of the others. A time-out code is sticky: while the word holds one, every later
+ *    fa_fwd / fa_bwd_dkdv / fa_bwd_dq / fa_paged_fwd launch given that word computes nothing and fills its
  *    outputs (o; dk, dv; dq) with NaN, until the host has read the word and set it back to 0.
- *    The outputs of the launch in which the wait ran out are undefined. Code 200 only concerns
- *    the call that passed the id (its result may mask that query wrongly); later calls run.
+ *    The outputs of the launch in which the wait ran out are undefined. Codes from 200 on only concern
+ *    the call that they come from (with 200, its result may mask that query wrongly); later calls run.
  *  - one bounded wait lasts at most 5e8 SM clocks (about 0.25 s); the environment variable
  *    FA_B200_WAIT_LIMIT_CLOCKS (>= 10000), read when the library is first used, replaces the limit,
  *    e.g. on hosts where several contexts time-share the GPU. The scheduler of a kernel waits for as

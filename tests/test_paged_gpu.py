@@ -524,3 +524,22 @@ def test_a_later_token_of_a_chunk_that_is_not_finite(D, G, at, cap):
     assert torch.equal(got[:clean], want[:clean]) and torch.equal(got[100:], want[100:])
     assert not torch.isfinite(got[at - 400: 100]).any()
     fb.check_status()
+
+
+@pytest.mark.parametrize("code", [200, 201, 202])
+def test_a_time_out_is_recorded_over_what_concerned_one_call(code):
+    """A report that nobody has read yet lets later calls run; a wait that runs out in one of them (the test hook's here) has to stop those behind it."""
+    import flash_b200 as fb
+    from flash_b200 import _lib, ops
+    cache = Cache([100, 30], 2, 64, 16, BF16, 28).fill()
+    q = torch.randn(2, 4, 64, device="cuda").to(BF16)
+    args = (q, cache.k_pages, cache.v_pages, cache.table, cache.kv_lens)
+    want, status = fb.paged_attention(*args), ops._status_word(q.device)
+    status.fill_(code)
+    assert torch.equal(fb.paged_attention(*args), want) and int(status.item()) == code
+    _lib.check(_lib.load().fa_debug_wait_timeout(status.data_ptr(), 20000, 42, ops._stream()), "fa_debug_wait_timeout")
+    assert torch.isnan(fb.paged_attention(*args)).all() and torch.isnan(fb.attention(q[None].transpose(1, 2), q[None].transpose(1, 2), q[None].transpose(1, 2))).all()
+    cache.kv_lens[0] = -1  # is reported, but not in the place of the time-out
+    fb.paged_append(q[:, :2].contiguous(), q[:, :2].contiguous(), *args[1:])
+    with pytest.raises(RuntimeError, match="role 42"):
+        fb.check_status()

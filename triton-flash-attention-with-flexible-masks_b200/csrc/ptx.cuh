@@ -11,7 +11,7 @@
 namespace fa {
 
 // ----------------------------------------------------------------------------------------
-// status codes written to the device status word (first error wins)
+// status codes written to the device status word (the first one stays until the host has read it, but a time-out takes the place of the others)
 // ----------------------------------------------------------------------------------------
 enum : int {
     ST_OK = 0,
@@ -100,7 +100,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const A
         if (*ab.flag) return false;
         if (clock64() - t0 > ab.limit) {
             *ab.flag = 1;
-            atomicCAS(ab.status, 0, code);
+            atomicExch(ab.status, code);  // (also over what concerned one call only, or nothing would stop the calls to come)
             return false;
         }
     }
