@@ -223,7 +223,7 @@ typedef struct fa_rows {
 int fa_paged_append(const fa_paged_cache* cache, int32_t T, const int32_t* starts, const fa_rows* k, const fa_rows* v, int32_t* status, void* stream);
 
 /* o[t] = softmax(scores of row t with the keys it sees) V, for new tokens q [T, H, D] whose own keys are in the cache already. A token at position p
- * sees the keys j <= p and, with scores->prefix, j < prefix[b], of its sequence (scores may be NULL; i + gap in fa_scores is the position). H / Hk at most 128. A row that sees no key gets zeros. Rows of no
+ * sees the keys j <= p and, with scores->prefix, j < prefix[b], of its sequence (scores may be NULL; i + gap in fa_scores is the position). H / Hk at most 128. A row that sees no key, or is at a position below 0, gets zeros. Rows of no
  * sequence are set to 0 where `fill` is not 0 and else left as they are. o may not overlap q or the cache. Two kernels; `workspace`: 16-byte
  * aligned, at least fa_paged_workspace_bytes, which goes by the head dim and the current device alone; free again when the launches are done.
  * How the work is cut depends on all lengths of the batch, so the last bits of a sequence's result can differ with what it is batched with. */

@@ -543,3 +543,12 @@ def test_a_time_out_is_recorded_over_what_concerned_one_call(code):
     fb.paged_append(q[:, :2].contiguous(), q[:, :2].contiguous(), *args[1:])
     with pytest.raises(RuntimeError, match="role 42"):
         fb.check_status()
+
+
+@pytest.mark.parametrize("cap, slopes", [(None, False), (5.0, False), (5.0, True)])
+@pytest.mark.parametrize("G", [1, 4, 33])
+def test_tokens_in_front_of_a_sequence_see_no_prefix(G, cap, slopes):
+    """More new tokens than the sequence has: those at positions below 0 are nobody's (`paged_append` leaves them out) and give zeros, whatever the prefix."""
+    lens, new = [1, 40, 0, 200], [24, 41, 3, 330]
+    prefix = torch.tensor([28, 17, 5, 150], dtype=torch.int32, device="cuda")
+    _attend(Cache(lens, 2, 64, 16, BF16, 29).fill(), 2 * G, new, BF16, prefix=prefix, cap=cap, slopes=_slopes(2 * G, slopes))

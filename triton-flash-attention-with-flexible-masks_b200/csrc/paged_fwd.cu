@@ -516,8 +516,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             const bool valid = tok < tokens;
             const bool active = __any_sync(0xffffffffu, valid);  // does this warp hold a query at all?
             const int pos = pos0 + tok;
-            const int last = min(max(pos, front - 1), len - 1);                // the last key that this row sees
-            const int all_see = min(max(pos0, front - 1), len - 1);            // and that all rows of the tile see
+            const int last = pos < 0 ? -1 : min(max(pos, front - 1), len - 1);  // the last key that this row sees (a token in front of the sequence sees no prefix, either)
+            const int all_see = pos0 < 0 ? -1 : min(max(pos0, front - 1), len - 1);  // and that all rows of the tile see
             const int seen = min(max(pos0 + tokens, front), len);              // keys that any row sees
             float slope = 0.f;
             if constexpr (SCORED) {
