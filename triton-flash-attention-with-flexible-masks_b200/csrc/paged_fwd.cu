@@ -127,7 +127,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     uint16_t* const out = static_cast<uint16_t*>(p.out);
     // (aborted: an earlier launch ran into a time-out that the host has not yet cleared. The second kernel fills the output.)
     if (aborted) {
-        if (tid == 0) p.merge[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if (tid == 0) p.merge[blockIdx.x] = make_int4(-1, 0, 0, 0);
     } else if (p.B > kPagedWarpPlan) {
         paged_plan<kFwdThreads>(p, plan, int(gridDim.x));
     }
@@ -767,7 +767,8 @@ __global__ void __launch_bounds__(kCombineThreads, 2) paged_combine_kernel(const
     __shared__ float sums[kWarps][kCombineRows][D + 2];
     follow_stream();
     const int w = int(blockIdx.x), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (status_is_fatal(*reinterpret_cast<volatile int*>(p.status))) {
+    const int4 merge = p.merge[w];
+    if (merge.x < 0 || status_is_fatal(*reinterpret_cast<volatile int*>(p.status))) {  // (the host may have cleared the word since)
         // A time-out, of an earlier launch, of one on another stream meanwhile, or in the attention kernel: some of its blocks, or all, have left their rows as they
         // were, and which is not known. All rows become NaN, or those of the sequences in an output of the caller's.
         const bool all = p.fill || !p.starts;
@@ -777,7 +778,6 @@ __global__ void __launch_bounds__(kCombineThreads, 2) paged_combine_kernel(const
             for (int d = lane; d < p.D; d += 32) static_cast<uint16_t*>(p.out)[i / p.H * p.out_t + i % p.H * p.out_h + d] = 0xffffu;
         return;
     }
-    const int4 merge = p.merge[w];
     const int row0 = int(blockIdx.y) * kWarps * kCombineRows, pieces = merge.x, rows = (merge.z & 255) * p.G - row0, hk = merge.z >> 8;
     auto slot = [&](int s) { return 2 * (merge.w + s) + (s == 0 ? 1 : 0); };
     if (pieces < 2 || rows <= 0) return;

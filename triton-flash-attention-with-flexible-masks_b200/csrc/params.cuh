@@ -107,7 +107,7 @@ struct PagedParams {
     int64_t out_t, out_h;   // element strides
     float* part_o;          // [2 * workers, 128, 64 or 128] fp32 rows of the pieces
     float* part_lse;        // [2 * workers, 128]
-    int4* merge;            // [workers] {pieces of the item that the cut before a worker goes through first, or fewer than 2; its first row; tokens
+    int4* merge;            // [workers] {pieces of the item that the cut before a worker goes through first, or fewer than 2 (-1: the worker has found a time-out on record); its first row; tokens
                             // and 256 * kv head; worker of the first piece}
     int B, T, H, Hk, G, D;
     int tokens;             // of a tile: 128 / G
