@@ -484,7 +484,10 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         auto zero_behind = [&](int g, int real) {
             const int st = g % NS;
             if (!mbar_wait_warp(BAR(B_VFULL + st), (g / NS) & 1, ab, ST_WAIT_TIMEOUT + 19)) return false;
+            // (not unrolled: it stands twice in the code of the softmax warps, a batch of chunks and tokens with a bias 224 us for 237)
+#pragma unroll 1
             for (int x = 0; x < S::NBOX; ++x)
+#pragma unroll 1
                 for (int i = real * 8 + r; i < kBlk * 8; i += kBlk) reinterpret_cast<uint4*>(smem + S::off_v + st * S::TILE + x * S::BOX)[i] = make_uint4(0, 0, 0, 0);
             fence_proxy_async();
             return true;
@@ -767,8 +770,14 @@ __global__ void __launch_bounds__(kCombineThreads, 2) paged_combine_kernel(const
     __shared__ float sums[kWarps][kCombineRows][D + 2];
     follow_stream();
     const int w = int(blockIdx.x), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (both loads in flight together: one behind the other cost a call of one token a microsecond)
+    const int status = *reinterpret_cast<volatile int*>(p.status);
     const int4 merge = p.merge[w];
-    if (merge.x < 0 || status_is_fatal(*reinterpret_cast<volatile int*>(p.status))) {  // (the host may have cleared the word since)
+    const bool failed = status_is_fatal(status) | (merge.x < 0);  // (the host may have cleared the word since)
+    const int row0 = int(blockIdx.y) * kWarps * kCombineRows, pieces = merge.x, rows = (merge.z & 255) * p.G - row0, hk = merge.z >> 8;
+    auto slot = [&](int s) { return 2 * (merge.w + s) + (s == 0 ? 1 : 0); };
+    if (!failed && (pieces < 2 || rows <= 0)) return;
+    if (failed) {
         // A time-out, of an earlier launch, of one on another stream meanwhile, or in the attention kernel: some of its blocks, or all, have left their rows as they
         // were, and which is not known. All rows become NaN, or those of the sequences in an output of the caller's.
         const bool all = p.fill || !p.starts;
@@ -778,9 +787,6 @@ __global__ void __launch_bounds__(kCombineThreads, 2) paged_combine_kernel(const
             for (int d = lane; d < p.D; d += 32) static_cast<uint16_t*>(p.out)[i / p.H * p.out_t + i % p.H * p.out_h + d] = 0xffffu;
         return;
     }
-    const int row0 = int(blockIdx.y) * kWarps * kCombineRows, pieces = merge.x, rows = (merge.z & 255) * p.G - row0, hk = merge.z >> 8;
-    auto slot = [&](int s) { return 2 * (merge.w + s) + (s == 0 ? 1 : 0); };
-    if (pieces < 2 || rows <= 0) return;
     const int groups = min(cdiv(rows, kCombineRows), kWarps), subs = kWarps / groups;
     const int sub = warp / groups, r0 = (warp - sub * groups) * kCombineRows;  // (of this block's rows)
     // A warp's own pieces first: their greatest lse, and the sums relative to it. (An empty piece has an lse of -inf.)
