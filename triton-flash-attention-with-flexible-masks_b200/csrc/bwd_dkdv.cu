@@ -112,7 +112,7 @@ struct Walk {
     }
 };
 
-// KIND: as in the forward; with a cap dS takes the factor 1 - tanh^2, which P is multiplied by once it has been packed for dV. 16 x 8111 x 128 in documents, us: unchanged 193, capped 241, biased 210, both 262.
+// KIND: as in the forward; with a cap dS takes the factor 1 - tanh^2, which P is multiplied by once it has been packed for dV. 16 x 8111 x 128 in documents, us: unchanged 178, capped 222, biased 194, both 242.
 template <int D, bool BF16, int KIND = SCORE_PLAIN>
 __global__ void __launch_bounds__(kDkdvThreads, 1)
 bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,

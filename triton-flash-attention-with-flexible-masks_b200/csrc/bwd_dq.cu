@@ -64,7 +64,7 @@ struct DqWalk {
     }
 };
 
-// KIND: as in the forward; with a cap dS takes the factor 1 - tanh^2. 16 x 8111 x 128 in documents, us: unchanged 142, capped 192, biased 154, both 210. (Sixteen compute
+// KIND: as in the forward; with a cap dS takes the factor 1 - tanh^2. 16 x 8111 x 128 in documents, us: unchanged 138, capped 177, biased 146, both 198. (Sixteen compute
 // warps for the capped instances, of 32 columns, as head dims up to 64 with ids have them: the step 650 for 638, head dim 64 2 % slower.)
 template <int D, int NW, bool BF16, int KIND = SCORE_PLAIN>
 __global__ void __launch_bounds__(DqSmem<D, NW>::THREADS, 1)

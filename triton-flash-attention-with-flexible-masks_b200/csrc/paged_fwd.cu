@@ -17,10 +17,11 @@
 //  - each block works on one stretch of a line of all items (paged_plan.cuh); a piece of an item that was cut leaves normalised fp32 rows and
 //    their log-sum-exp to paged_combine_kernel.
 //
-// What bounds it. Single tokens: HBM. 64 tokens over 1288 MB of keys and values 207-215 us (6.0-6.2 TB/s; the copy rate is 6.56), one token over 537 MB 99 us, of which
+// What bounds it. Single tokens: HBM. 64 tokens over 1288 MB of keys and values 212-215 us in replayed graphs (6.0-6.1 TB/s; the copy rate is 6.56) and up to 243 in long series of
+// calls under the power cap (5.3), one token over 537 MB 98-107 us, of which
 // the plan and the first item's place take 2.3, the last tile's drain 3, the second kernel up to 4 (the main loop streams at 7 TB/s); one token over 1.4 MB
 // 16 us, all of it latency: start, plan, a chain of tiles, epilogue, the second kernel's start. Chunks: the forward's chain of tiles, and twice as many loads. One chunk of 2000
-// tokens, pages of 128 | 16: 199 | 220 us (1150 | 1043 TFLOP/s); a chunk of 500 behind 7500 76 | 83 us, where dense keys take 55.
+// tokens, 32 / 8 heads, pages of 128 | 16: 64 | 64 us; a chunk of 500 behind 7500 67 | 76 us, where dense keys take 55.
 #include <type_traits>
 #include "common.cuh"
 #include "paged_plan.cuh"

@@ -10,11 +10,11 @@
 // scores and nothing of the special-function unit, which the exponentials keep busy. Beyond, a score is a - 2 a / (1 + 2^(2 log2(e) x)), whose absolute error
 // is some 2^-22 of a: close to 0 that form would lose the small scores of a large cap, so that a warp with a score beyond the polynomial works out both forms and takes each score's own.
 //
-// What bounds it: what two softmax warps a scheduler get through of a tile's straight code (no unit is full: issue slots 46 %, MUFU 39, FMA 36, tensor pipe 38 with a cap), so that each
-// instruction shows. Forward of 2 x 16 x 4096 x 128 causal, unchanged, capped, biased, both: 49, 77, 75, 104 million
-// instructions in 206, 296, 259, 365 thousand clocks. Forward of 32 / 8 heads x 5801 x 128 causal 257, 325, 298, 395 us; kernels of a step of 16 x 8111 x 128 in documents, us,
-// forward 117, 167, 138, 195, dK/dV 193, 241, 210, 262, dQ 142, 192, 154, 210.
-// Tried and taken back (the same forward, cap 50 | cap 20, which at deviation 4 goes through both forms now and then; now 324 | 460): five terms for 7.1e-7 up to 0.75 cap 325 | 682; six up
+// What bounds it: what two softmax warps a scheduler get through of a tile's straight code (no unit is full: issue slots 46 %, MUFU 40, tensor pipe 40 with a cap), so that each
+// instruction shows: 2 x 16 x 4096 x 128 causal, capped | biased, 80 | 71 million instructions, issue slots 46 | 47 %.
+// Forward of 32 / 8 heads x 5801 x 128 causal, unchanged, capped, biased, both: 259, 330, 298, 399 us; kernels of a step of 16 x 8111 x 128 in documents, us,
+// forward 112, 164, 130, 178, dK/dV 178, 222, 194, 242, dQ 138, 177, 146, 198.
+// Tried and taken back (the same forward, cap 50 | cap 20, which at deviation 4 goes through both forms now and then; now 330 | 463): five terms for 7.1e-7 up to 0.75 cap 325 | 682; six up
 // to the cap 352 | 378; a quotient of polynomials of degree 2, up to 2.5 caps, with one reciprocal for two scores 426 | 418; eight terms up to 1.4 cap as a second unrolled
 // form 358 | 528 (registers); the cap of the next 16 scores in front of the exponentials of these, as the source goes, 328 | -. The bias as one more product of 16 columns on the tensor cores (slope and position in three 16-bit parts): the biased forward 277 for 298, but 8 ragged
 // sequences over a paged cache 222 for 218 and an encoder's step 136 for 134, for a quarter more code.
