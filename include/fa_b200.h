@@ -61,7 +61,8 @@ enum fa_error {
     FA_ERR_PLAN_SIZE = 6,    /* plan buffer too small / missing for FA_MODE1_DOC, or workspace of a split forward */
     FA_ERR_NO_DRIVER = 7,    /* cuTensorMapEncodeTiled could not be resolved */
     FA_ERR_SCRATCH_LIMIT = 8, /* fa_fwd_static_plan: the plan does not fit in FA_STATIC_PLAN_BYTES */
-    FA_ERR_SCORES = 9,       /* fa_scores: softcap neither 0 nor within 1e-6 .. 1e6, or a prefix without a causal mask */
+    FA_ERR_SCORES = 9,       /* fa_scores: softcap neither 0 nor within 1e-6 .. 1e6, or a prefix or a window without a causal mask, or
+                              sinks without a window */
     FA_ERR_PAGED = 10        /* fa_paged_cache: page size not a power of two from 8 on, or sizes beyond what the kernels count */
 };
 
@@ -191,6 +192,25 @@ int fa_fwd_rest(const fa_problem* p, int32_t splits, const void* workspace, size
 int fa_bwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
                   const void* rest, const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv,
                   const void* plan, int32_t* status, void* stream);
+
+/* A sliding window, and the first tokens that it leaves visible: with a causal mask, query i sees the keys j <= i + gap with i + gap - j < keys or
+ * j < sinks, besides those that a prefix shows it; the ids' rule holds on top. keys 0: none. */
+typedef struct fa_window {
+    int32_t keys;
+    int32_t sinks;
+} fa_window;
+
+/* The four of a call with a window (scores may be NULL, window NULL or of 0 keys is a call without one). The plan of a call with ids must have been built with the
+ * same window; fa_fwd_splits_windowed says into how many runs the keys that are left are best cut; fa_fwd_rest serves these forwards, too. */
+int fa_plan_build_windowed(const fa_problem* p, const fa_scores* scores, const fa_window* window, const fa_ids* eq, const fa_ids* ek, void* plan,
+                           size_t plan_bytes, int32_t* status, void* stream);
+int fa_fwd_splits_windowed(const fa_problem* p, const fa_window* window);
+int fa_fwd_windowed(const fa_problem* p, const fa_scores* scores, const fa_window* window, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v,
+                    const fa_tensor* o, void* rest, float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status,
+                    void* stream);
+int fa_bwd_windowed(const fa_problem* p, const fa_scores* scores, const fa_window* window, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v,
+                    const fa_tensor* o, const void* rest, const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk,
+                    const fa_tensor* dv, const void* plan, int32_t* status, void* stream);
 
 /* A cache of keys and values in pages, for serving (no counterpart in the reference). k and v are [pages, page_size, Hk, D], 16-bit, with 16-byte
  * aligned bases, last stride 1 and other strides multiples of 8 elements. Sequence b's tokens lie, page_size at a time, in the pages

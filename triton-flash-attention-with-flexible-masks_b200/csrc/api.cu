@@ -1,5 +1,6 @@
 // extern "C" surface of the library (declared in include/fa_b200.h): argument checks, TMA
 // tensor-map encoding, parameter packing and launches. Nothing here allocates or synchronises.
+#include <algorithm>
 #include <cstdlib>
 #include <mutex>
 #include "../../include/fa_b200.h"
@@ -9,7 +10,7 @@
 
 namespace fa {
 cudaError_t launch_plan_build(const void*, const int64_t*, int, const void*, const int64_t*, int, int32_t*,
-                              const PlanLayout&, int, int, const int32_t*, int*, cudaStream_t);
+                              const PlanLayout&, int, int, const int32_t*, int, int, int*, cudaStream_t);
 cudaError_t launch_plan_clear(int32_t*, int, cudaStream_t);
 cudaError_t launch_debug_mask(const MaskArgs&, uint8_t*, uint8_t*, cudaStream_t);
 cudaError_t launch_fwd(int, bool, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
@@ -198,20 +199,27 @@ int debug_flags() {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// What a call of attention_scored changes.
+struct Changes : fa_scores {
+    fa_window window;  // keys 0: none
+    Changes(const fa_scores* s, const fa_window* w) : fa_scores(s ? *s : fa_scores{}), window(w ? *w : fa_window{}) {}
+};
+
 // null: a call of attention() itself
-int check_scores(const fa_problem* p, const fa_scores* sc) {
+int check_scores(const fa_problem* p, const Changes* sc) {
     if (!sc) return FA_OK;
     if (sc->softcap != 0.f && !(sc->softcap >= 1e-6f && sc->softcap <= 1e6f)) return FA_ERR_SCORES;
     if (sc->prefix && !p->causal) return FA_ERR_SCORES;
+    if (sc->window.keys < 0 || sc->window.sinks < 0 || (sc->window.keys > 0 && !p->causal) || (sc->window.keys == 0 && sc->window.sinks > 0)) return FA_ERR_SCORES;
     if (reinterpret_cast<uintptr_t>(sc->slopes) % 4 != 0 || reinterpret_cast<uintptr_t>(sc->prefix) % 4 != 0) return FA_ERR_ALIGNMENT;
     return FA_OK;
 }
 
-fa::ScoreArgs score_args(const fa_problem* p, const fa_scores* sc) {
-    return sc ? fa::make_score_args(sc->softcap, sc->slopes, sc->prefix != nullptr, p->sm_scale) : fa::ScoreArgs{};
+fa::ScoreArgs score_args(const fa_problem* p, const Changes* sc) {
+    return sc ? fa::make_score_args(sc->softcap, sc->slopes, sc->prefix != nullptr, p->sm_scale, sc->window.keys > 0) : fa::ScoreArgs{};
 }
 
-int make_mask(fa::MaskArgs* m, const fa_problem* p, const void* plan, const fa_scores* sc = nullptr) {
+int make_mask(fa::MaskArgs* m, const fa_problem* p, const void* plan, const Changes* sc = nullptr) {
     if (p->mode == FA_MODE1_DOC && !plan) return FA_ERR_PLAN_SIZE;
     if (!aligned16(plan)) return FA_ERR_ALIGNMENT;  // the kernels read it with 16-byte and bulk loads
     m->plan = (p->mode == FA_MODE1_DOC) ? static_cast<const int32_t*>(plan) : nullptr;
@@ -227,6 +235,8 @@ int make_mask(fa::MaskArgs* m, const fa_problem* p, const void* plan, const fa_s
     m->mode = p->mode;
     m->debug = debug_flags();
     m->prefix = sc ? sc->prefix : nullptr;
+    m->window = sc ? std::min(sc->window.keys, p->N) : 0;
+    m->sinks = sc ? std::min(sc->window.sinks, p->N) : 0;
     return FA_OK;
 }
 
@@ -288,7 +298,7 @@ size_t fwd_workspace_bytes(const fa_problem* p, int ns) {
 // fp32 inputs: which = 0 forward, 1 delta, 2 dK / dV, 3 dQ; absent tensors are null
 int run_f32(int which, const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
             const fa_tensor* d_o, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv, float* lse, float* delta,
-            const void* plan, void* stream, const fa_scores* sc, bool overlap = false) {
+            const void* plan, void* stream, const Changes* sc, bool overlap = false) {
     int rc;
     fa::F32Params fp{};
     const struct { const fa_tensor* t; fa::F32Tensor* dst; int H, L; } all[8] = {
@@ -312,7 +322,7 @@ int run_f32(int which, const fa_problem* p, const fa_tensor* q, const fa_tensor*
     return fa::launch_f32(which, p->D, fp, overlap, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
-int run_plan_build(const fa_problem* p, const fa_scores* sc, const fa_ids* eq, const fa_ids* ek, void* plan, size_t plan_bytes,
+int run_plan_build(const fa_problem* p, const Changes* sc, const fa_ids* eq, const fa_ids* ek, void* plan, size_t plan_bytes,
                    int32_t* status, void* stream) {
     int rc = check_problem(p);
     if (!rc) rc = check_scores(p, sc);
@@ -333,11 +343,12 @@ int run_plan_build(const fa_problem* p, const fa_scores* sc, const fa_ids* eq, c
     const int gap = p->N > p->M ? p->N - p->M : 0;
     const cudaError_t e = fa::launch_plan_build(eq->ptr, eq->stride, eq->dtype == FA_ID_INT64, ek->ptr, ek->stride,
                                                 ek->dtype == FA_ID_INT64, static_cast<int32_t*>(plan), L, gap,
-                                                p->causal ? 1 : 0, sc ? sc->prefix : nullptr, status, static_cast<cudaStream_t>(stream));
+                                                p->causal ? 1 : 0, sc ? sc->prefix : nullptr, sc ? std::min(sc->window.keys, p->N) : 0,
+                                                sc ? std::min(sc->window.sinks, p->N) : 0, status, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
-int run_fwd(const fa_problem* p, const fa_scores* sc, void* rest, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
+int run_fwd(const fa_problem* p, const Changes* sc, void* rest, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
             float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
     int rc = check_problem(p);
     if (rc) return rc;
@@ -417,7 +428,7 @@ int run_bwd_delta(const fa_problem* p, const void* rest, const fa_tensor* o, con
     return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
-int run_bwd_dkdv(const fa_problem* p, const fa_scores* sc, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v,
+int run_bwd_dkdv(const fa_problem* p, const Changes* sc, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v,
                 const fa_tensor* d_o, const float* lse, const float* delta, const fa_tensor* dk, const fa_tensor* dv,
                 const void* plan, int32_t* status, void* stream) {
     int rc = check_problem(p);
@@ -465,7 +476,7 @@ int run_bwd_dkdv(const fa_problem* p, const fa_scores* sc, const fa_tensor* q, c
     return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
-int run_bwd_dq(const fa_problem* p, const fa_scores* sc, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* d_o,
+int run_bwd_dq(const fa_problem* p, const Changes* sc, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* d_o,
               const float* lse, const float* delta, const fa_tensor* dq, const void* plan, int32_t* status,
                bool overlap, void* stream) {
     int rc = check_problem(p);
@@ -545,7 +556,7 @@ const char* fa_error_string(int code) {
         case FA_ERR_PLAN_SIZE: return "mask plan or workspace missing or too small";
         case FA_ERR_NO_DRIVER: return "CUDA driver entry point cuTensorMapEncodeTiled not available";
         case FA_ERR_SCRATCH_LIMIT: return "mask plan larger than the library's built-in FA_STATIC_PLAN_BYTES array";
-        case FA_ERR_SCORES: return "scores refused (softcap must be 0 or from 1e-6 to 1e6, a prefix needs a causal mask)";
+        case FA_ERR_SCORES: return "scores refused (softcap must be 0 or from 1e-6 to 1e6, a prefix or a window needs a causal mask, sinks a window)";
         case FA_ERR_PAGED:
             return "paged cache refused (page size a power of two from 8 on, at most 4194304 tokens per sequence and call, 65535 sequences, 1024 kv heads)";
         default: return "unknown error";
@@ -588,15 +599,32 @@ int fa_plan_build(const fa_problem* p, const fa_ids* eq, const fa_ids* ek, void*
     return run_plan_build(p, nullptr, eq, ek, plan, plan_bytes, status, stream);
 }
 
+int fa_plan_build_windowed(const fa_problem* p, const fa_scores* scores, const fa_window* window, const fa_ids* eq, const fa_ids* ek, void* plan,
+                           size_t plan_bytes, int32_t* status, void* stream) {
+    const Changes c(scores, window);
+    return run_plan_build(p, &c, eq, ek, plan, plan_bytes, status, stream);
+}
+
 int fa_plan_build_scored(const fa_problem* p, const fa_scores* scores, const fa_ids* eq, const fa_ids* ek, void* plan, size_t plan_bytes,
                          int32_t* status, void* stream) {
-    return scores ? run_plan_build(p, scores, eq, ek, plan, plan_bytes, status, stream) : FA_ERR_BAD_ARG;
+    return scores ? fa_plan_build_windowed(p, scores, nullptr, eq, ek, plan, plan_bytes, status, stream) : FA_ERR_BAD_ARG;
 }
 
 int fa_fwd_splits(const fa_problem* p) {
     if (check_problem(p)) return 1;
     const int sms = sm_count();
     return sms > 0 ? fwd_splits(p, sms) : 1;
+}
+
+// With a window a query's keys are at most the window's and the sinks, and those of a tile of queries so many more.
+int fa_fwd_splits_windowed(const fa_problem* p, const fa_window* window) {
+    if (check_problem(p)) return 1;
+    fa_problem seen = *p;
+    if (window && window->keys > 0 && p->causal) {
+        const int64_t keys = int64_t(window->keys) + std::max(0, window->sinks) + std::min(p->M, fa::kBlk);
+        seen.N = int(std::max(int64_t(p->M), std::min(int64_t(p->N), keys)));
+    }
+    return fa_fwd_splits(&seen);
 }
 
 int fa_fwd_workspace_bytes(const fa_problem* p, int32_t splits, size_t* bytes) {
@@ -618,9 +646,17 @@ int fa_fwd_split(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, co
     return run_fwd(p, nullptr, nullptr, q, k, v, o, lse, plan, splits, workspace, workspace_bytes, status, stream);
 }
 
+int fa_fwd_windowed(const fa_problem* p, const fa_scores* scores, const fa_window* window, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v,
+                    const fa_tensor* o, void* rest, float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status,
+                    void* stream) {
+    const Changes c(scores, window);
+    return run_fwd(p, &c, rest, q, k, v, o, lse, plan, splits, workspace, workspace_bytes, status, stream);
+}
+
 int fa_fwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o, void* rest,
                   float* lse, const void* plan, int32_t splits, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
-    return scores ? run_fwd(p, scores, rest, q, k, v, o, lse, plan, splits, workspace, workspace_bytes, status, stream) : FA_ERR_BAD_ARG;
+    if (!scores) return FA_ERR_BAD_ARG;
+    return fa_fwd_windowed(p, scores, nullptr, q, k, v, o, rest, lse, plan, splits, workspace, workspace_bytes, status, stream);
 }
 
 int fa_fwd_rest(const fa_problem* p, int32_t splits, const void* workspace, size_t workspace_bytes, void* rest, int32_t* status, void* stream) {
@@ -663,16 +699,23 @@ int fa_bwd(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa
     return rc;
 }
 
+int fa_bwd_windowed(const fa_problem* p, const fa_scores* scores, const fa_window* window, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v,
+                    const fa_tensor* o, const void* rest, const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk,
+                    const fa_tensor* dv, const void* plan, int32_t* status, void* stream) {
+    const Changes c(scores, window);
+    int rc = check_problem(p);
+    if (!rc) rc = check_scores(p, &c);
+    if (!rc) rc = run_bwd_delta(p, rest, o, d_o, delta, stream);
+    if (!rc) rc = run_bwd_dkdv(p, &c, q, k, v, d_o, lse, delta, dk, dv, plan, status, stream);
+    if (!rc) rc = run_bwd_dq(p, &c, q, k, v, d_o, lse, delta, dq, plan, status, true, stream);
+    return rc;
+}
+
 int fa_bwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
                   const void* rest, const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv,
                   const void* plan, int32_t* status, void* stream) {
     if (!scores) return FA_ERR_BAD_ARG;
-    int rc = check_problem(p);
-    if (!rc) rc = check_scores(p, scores);
-    if (!rc) rc = run_bwd_delta(p, rest, o, d_o, delta, stream);
-    if (!rc) rc = run_bwd_dkdv(p, scores, q, k, v, d_o, lse, delta, dk, dv, plan, status, stream);
-    if (!rc) rc = run_bwd_dq(p, scores, q, k, v, d_o, lse, delta, dq, plan, status, true, stream);
-    return rc;
+    return fa_bwd_windowed(p, scores, nullptr, q, k, v, o, rest, d_o, lse, delta, dq, dk, dv, plan, status, stream);
 }
 
 uint32_t fa_classify_tile(int32_t M, int32_t N, int32_t causal, int32_t mode, int32_t qb, int32_t kb, int32_t qmin,

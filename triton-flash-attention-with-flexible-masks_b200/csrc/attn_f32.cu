@@ -223,11 +223,11 @@ __device__ __forceinline__ float warp_sum(float x) {
 }
 
 // visited[o] for every 128-block o of the other side; the caller synchronises
-template <int R, bool SCORED>
+template <int R, bool SCORED, bool WINDOW>
 __device__ __forceinline__ void find_visited(uint8_t* visited, const MaskArgs& mk, int b, int he, bool rows_are_queries, int own) {
     const int n = rows_are_queries ? mk.L.nK : mk.L.nQ;
     for (int o = threadIdx.x; o < n; o += threads(R))
-        visited[o] = (classify_from_plan<SCORED>(mk, b, he, rows_are_queries ? own : o, rows_are_queries ? o : own) & TILE_VISIT) != 0;
+        visited[o] = (classify_from_plan<SCORED, WINDOW>(mk, b, he, rows_are_queries ? own : o, rows_are_queries ? o : own) & TILE_VISIT) != 0;
 }
 // first column >= c (a multiple of kC) of a visited block, or end
 __device__ __forceinline__ int next_tile(const uint8_t* visited, int c, int end) {
@@ -245,7 +245,7 @@ __device__ __forceinline__ int code_k(const MaskArgs& mk, int b, int he, int j) 
 // ---------------------------------------------------------------------------------------------
 // forward: grid (H, B, ceil(M / R))
 // ---------------------------------------------------------------------------------------------
-template <int D, int R, bool SCORED>
+template <int D, int R, bool SCORED, bool WINDOW>
 __global__ void __launch_bounds__(threads(R), R == 32 && D <= 32 ? 4 : 0) f32_fwd_kernel(const F32Params p) {
     using S = F32Smem<D, R>;
     extern __shared__ __align__(16) float sm[];
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(threads(R), R == 32 && D <= 32 ? 4 : 0) f32_fw
         if (kcodes && threadIdx.x < kC) cp_async4(smem_u32(codes + st * kC + threadIdx.x), kcodes + j0 + threadIdx.x, true);
     };
     load_tile<D, R, R>(Qs, qbase, p.q.sl, rows_aligned(qbase, p.q.sl), i0, mk.M);
-    find_visited<R, SCORED>(visited, mk, b, he, true, i0 / kBlk);
+    find_visited<R, SCORED, WINDOW>(visited, mk, b, he, true, i0 / kBlk);
     float m[kRW], l[kRW];
     F32Acc<D> acc;
     acc.clear();
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(threads(R), R == 32 && D <= 32 ? 4 : 0) f32_fw
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int j = j0 + x + 32 * c;
-                const bool keep = keep_entry<SCORED>(i, j, qc[r], kcodes ? codes[st * kC + x + 32 * c] : 0, mk.N, mk.gap, mk.causal, mk.mode, front);
+                const bool keep = keep_entry<SCORED, WINDOW>(i, j, qc[r], kcodes ? codes[st * kC + x + 32 * c] : 0, mk.N, mk.gap, mk.causal, mk.mode, front, mk.window, mk.sinks);
                 float factor;
                 s[r][c] = keep ? score_f32<SCORED>(p, s[r][c], slope, i, j, factor) : -INFINITY;
                 mx = fmaxf(mx, s[r][c]);
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(128) f32_delta_kernel(const F32Params p) {
 // ---------------------------------------------------------------------------------------------
 // dQ: grid (H, B, ceil(M / R)). rows = queries, columns = keys
 // ---------------------------------------------------------------------------------------------
-template <int D, int R, bool SCORED>
+template <int D, int R, bool SCORED, bool WINDOW>
 __global__ void __launch_bounds__(threads(R)) f32_bwd_dq_kernel(const F32Params p) {
     using S = F32Smem<D, R>;
     extern __shared__ __align__(16) float sm[];
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dq_kernel(const F32Params 
     };
     load_tile<D, R, R>(Qs, qbase, p.q.sl, rows_aligned(qbase, p.q.sl), i0, mk.M);
     load_tile<D, R, R>(dOs, dobase, p.d_o.sl, rows_aligned(dobase, p.d_o.sl), i0, mk.M);
-    find_visited<R, SCORED>(visited, mk, b, he, true, i0 / kBlk);
+    find_visited<R, SCORED, WINDOW>(visited, mk, b, he, true, i0 / kBlk);
     F32Acc<D> acc;
     acc.clear();
     float lse[kRW], dl[kRW];
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dq_kernel(const F32Params 
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int j = j0 + x + 32 * c;
-                const bool keep = (i < mk.M) && keep_entry<SCORED>(i, j, qc[r], kcodes ? codes[st * kC + x + 32 * c] : 0, mk.N, mk.gap, mk.causal, mk.mode, front);
+                const bool keep = (i < mk.M) && keep_entry<SCORED, WINDOW>(i, j, qc[r], kcodes ? codes[st * kC + x + 32 * c] : 0, mk.N, mk.gap, mk.causal, mk.mode, front, mk.window, mk.sinks);
                 float factor;
                 const float pe = keep ? expf(score_f32<SCORED>(p, s[r][c], slope, i, j, factor) - lse[r]) : 0.f;  // a kept entry has a finite lse
                 dp[r][c] = keep ? pe * (dp[r][c] - dl[r]) * factor : 0.f;  // dS (flash_triton.py:301)
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dq_kernel(const F32Params 
 // dK, dV: grid (Hk, B, ceil(N / R)). rows = keys, columns = queries; the query heads of the group
 // are walked one after the other, so the group sum (flash_triton.py:635-637) needs no second pass
 // ---------------------------------------------------------------------------------------------
-template <int D, int R, bool SCORED>
+template <int D, int R, bool SCORED, bool WINDOW>
 __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Params p) {
     using S = F32Smem<D, R>;
     extern __shared__ __align__(16) float sm[];
@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
             // A head without a visible tile has passed no barrier since its next_tile: without this one a fast warp
             // would rewrite the table while a slow one reads it, and the two would take different numbers of tiles.
             if (g > 0) __syncthreads();
-            find_visited<R, SCORED>(visited, mk, b, he, false, j0 / kBlk);
+            find_visited<R, SCORED, WINDOW>(visited, mk, b, he, false, j0 / kBlk);
         }
         int kc[kRW];
 #pragma unroll
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
                 const float lse = vec[kC + x + 32 * c], dl = vec[2 * kC + x + 32 * c];
 #pragma unroll
                 for (int r = 0; r < kRW; ++r) {
-                    const bool keep = (i < mk.M) && keep_entry<SCORED>(i, j0 + r0 + r, qc, kc[r], mk.N, mk.gap, mk.causal, mk.mode, front);
+                    const bool keep = (i < mk.M) && keep_entry<SCORED, WINDOW>(i, j0 + r0 + r, qc, kc[r], mk.N, mk.gap, mk.causal, mk.mode, front, mk.window, mk.sinks);
                     float factor;
                     const float pe = keep ? expf(score_f32<SCORED>(p, s[r][c], slope, i, j0 + r0 + r, factor) - lse) : 0.f;
                     s[r][c] = pe;
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
 }
 
 // ---------------------------------------------------------------------------------------------
-template <int D, int R, bool SCORED>
+template <int D, int R, bool SCORED, bool WINDOW>
 static cudaError_t launch_f32_t(int which, const F32Params& p, bool overlap, cudaStream_t stream) {
     using S = F32Smem<D, R>;
     const MaskArgs& mk = p.mask;
@@ -588,9 +588,9 @@ static cudaError_t launch_f32_t(int which, const F32Params& p, bool overlap, cud
         kern<<<grid, threads(R), smem, stream>>>(p);
         return cudaGetLastError();
     };
-    if (which == 0) return run(f32_fwd_kernel<D, R, SCORED>, S::fwd_bytes, mk.M, p.H);
-    if (which == 2) return run(f32_bwd_dkdv_kernel<D, R, SCORED>, S::bwd_bytes, mk.N, p.Hk);
-    return run(f32_bwd_dq_kernel<D, R, SCORED>, S::bwd_bytes, mk.M, p.H);
+    if (which == 0) return run(f32_fwd_kernel<D, R, SCORED, WINDOW>, S::fwd_bytes, mk.M, p.H);
+    if (which == 2) return run(f32_bwd_dkdv_kernel<D, R, SCORED, WINDOW>, S::bwd_bytes, mk.N, p.Hk);
+    return run(f32_bwd_dq_kernel<D, R, SCORED, WINDOW>, S::bwd_bytes, mk.M, p.H);
 }
 
 // Blocks of 16 rows while those of 32 fit on the GPU all at once (`slots`): they have a chain of as many tiles but half the work, and the
@@ -607,8 +607,9 @@ static cudaError_t launch_f32_rows(int which, const F32Params& p, bool overlap, 
     constexpr int room = 232448 / ((S::fwd_bytes) + kStatic), per_sm = room < 4 ? room : 4;
     const int64_t rows = int64_t(cdiv(mk.M, 32)) * p.H * p.B, cols = int64_t(cdiv(mk.N, 32)) * p.Hk * p.B, slots = int64_t(per_sm) * sms;
     const bool small = which == 0 ? rows <= slots : 10 * (rows + cols) <= 13 * slots;
-    if (p.score.kind != SCORE_PLAIN) return small ? launch_f32_t<D, 16, true>(which, p, overlap, stream) : launch_f32_t<D, 32, true>(which, p, overlap, stream);
-    return small ? launch_f32_t<D, 16, false>(which, p, overlap, stream) : launch_f32_t<D, 32, false>(which, p, overlap, stream);
+    if (p.score.kind & SCORE_WINDOW) return small ? launch_f32_t<D, 16, true, true>(which, p, overlap, stream) : launch_f32_t<D, 32, true, true>(which, p, overlap, stream);
+    if (p.score.kind != SCORE_PLAIN) return small ? launch_f32_t<D, 16, true, false>(which, p, overlap, stream) : launch_f32_t<D, 32, true, false>(which, p, overlap, stream);
+    return small ? launch_f32_t<D, 16, false, false>(which, p, overlap, stream) : launch_f32_t<D, 32, false, false>(which, p, overlap, stream);
 }
 
 // which: 0 forward, 1 delta, 2 dK / dV, 3 dQ. overlap: the launch directly before this one in the stream is the dK/dV

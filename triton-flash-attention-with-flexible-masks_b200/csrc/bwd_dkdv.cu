@@ -72,13 +72,13 @@ enum : uint32_t { KC_SKIP = 0u, KC_PLAIN = 1u, KC_DOC = 2u, KC_DOCMANY = 3u };
 
 // Flags of tile (qb, kb) for all query heads of one kv head at once. When the heads disagree
 // (ids given per head) the id check is forced, entry by entry, which is always exact.
-template <bool SCORED>
+template <bool PREFIX, bool WINDOW>
 __device__ __forceinline__ uint32_t classify_group(const MaskArgs& mk, int b, int hk, int G, int qb, int kb) {
-    if (mk.He == 1 || G == 1) return classify_from_plan<SCORED>(mk, b, mk.He == 1 ? 0 : hk * G, qb, kb);
+    if (mk.He == 1 || G == 1) return classify_from_plan<PREFIX, WINDOW>(mk, b, mk.He == 1 ? 0 : hk * G, qb, kb);
     uint32_t f = 0;
     bool all = true;
     for (int g = 0; g < G; ++g) {
-        const uint32_t fg = classify_from_plan<SCORED>(mk, b, hk * G + g, qb, kb);
+        const uint32_t fg = classify_from_plan<PREFIX, WINDOW>(mk, b, hk * G + g, qb, kb);
         if (fg & TILE_VISIT) f |= fg; else all = false;
     }
     if (f && !all) f |= TILE_DOC;
@@ -120,7 +120,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 const __grid_constant__ CUtensorMap tmdK, const __grid_constant__ CUtensorMap tmdV,
                 const DkdvParams p) {
     using S = DkdvSmem<D>;
-    constexpr bool PREFIX = KIND != SCORE_PLAIN, SCORED = score_changed(KIND);  // perhaps a prefix; other scores
+    constexpr bool PREFIX = KIND != SCORE_PLAIN, SCORED = score_changed(KIND), WINDOW = (KIND & SCORE_WINDOW) != 0;  // perhaps a prefix; other scores
     constexpr int NQ = S::NQ, NDO = S::NDO;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -256,7 +256,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     const int ng = (mk.He == 1) ? 1 : G;
                     for (int g = 0; g < ng; ++g) {
                         int l, h2;
-                        q_range<PREFIX>(mk, b, mk.He == 1 ? 0 : hk * G + g, kb, l, h2);
+                        q_range<PREFIX, WINDOW>(mk, b, mk.He == 1 ? 0 : hk * G + g, kb, l, h2);
                         if (h2 > l) { lo = min(lo, l); hi = max(hi, h2); }
                     }
                     if (hi == 0) lo = 0;
@@ -270,7 +270,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     for (int e = 0; e < 4; ++e) {
                         const int c = 4 * i + e;
                         if (c >= n) break;
-                        const uint32_t f = classify_group<PREFIX>(mk, b, hk, G, lo + c, kb);
+                        const uint32_t f = classify_group<PREFIX, WINDOW>(mk, b, hk, G, lo + c, kb);
                         uint32_t code = KC_SKIP;
                         if (f & TILE_VISIT) code = !(f & TILE_DOC) ? KC_PLAIN : (f & TILE_QMANY) ? KC_DOCMANY : KC_DOC;
                         cnt += (code != KC_SKIP);
@@ -512,7 +512,8 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 wk.next(cg, cc, code);
                 const bool fl_doc = code >= KC_DOC, many = code == KC_DOCMANY;
                 const int qb0 = (lo + cc) * kBlk;
-                const bool fl_range = (mk.causal && (k0 + kBlk > mk.N || (k1 - 1 > qb0 + mk.gap && (!PREFIX || k1 > front)))) || (qb0 + kBlk > mk.M);
+                const bool fl_range = (mk.causal && (k0 + kBlk > mk.N || (k1 - 1 > qb0 + mk.gap && (!PREFIX || k1 > front)))) || (qb0 + kBlk > mk.M) ||
+                                      (WINDOW && k0 < qb0 + kBlk + mk.gap - mk.window && k1 > early_keys<true>(front, mk.sinks));
                 const int q0 = qb0 + cbase;  // first query row of this warp's columns
                 const int gi = gt + it;
                 // the rows' LSE came with Q, which S^T has been computed from; their delta is asked for here
@@ -535,7 +536,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         keep = codes_equal(qcs, qc, kc, many) | __ballot_sync(0xffffffffu, qc >= 0);
                     }
                     if (fl_range) {
-                        const int cmin = mk.causal && (!PREFIX || j >= front) ? (j - mk.gap) - q0 : 0, cmax = mk.M - q0;
+                        const int cmin = mk.causal && (!PREFIX || j >= front) ? (j - mk.gap) - q0 : 0, cmax = WINDOW && j >= early_keys<true>(front, mk.sinks) ? min(mk.M, j - mk.gap + mk.window) - q0 : mk.M - q0;
                         keep &= first_bits(cmax) & ~first_bits(cmin);
                     }
                 }
@@ -778,6 +779,10 @@ cudaError_t launch_bwd_dkdv(int D, bool bf16, const CUtensorMap& tq, const CUten
         if (p.score.kind == SCORE_CAPPED) return pick(d, integral_constant<int, SCORE_CAPPED>{});
         if (p.score.kind == SCORE_BIAS) return pick(d, integral_constant<int, SCORE_BIAS>{});
         if (p.score.kind == SCORE_PREFIX) return pick(d, integral_constant<int, SCORE_PREFIX>{});
+        if (p.score.kind == (SCORE_WINDOW | SCORE_CAPPED_BIAS)) return pick(d, integral_constant<int, SCORE_WINDOW | SCORE_CAPPED_BIAS>{});
+        if (p.score.kind == (SCORE_WINDOW | SCORE_CAPPED)) return pick(d, integral_constant<int, SCORE_WINDOW | SCORE_CAPPED>{});
+        if (p.score.kind == (SCORE_WINDOW | SCORE_BIAS)) return pick(d, integral_constant<int, SCORE_WINDOW | SCORE_BIAS>{});
+        if (p.score.kind == SCORE_WINDOW) return pick(d, integral_constant<int, SCORE_WINDOW>{});
         return pick(d, integral_constant<int, SCORE_PLAIN>{});
     };
     return D == 128 ? of(integral_constant<int, 128>{}) : of(integral_constant<int, 64>{});

@@ -72,7 +72,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
               const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
               const __grid_constant__ CUtensorMap tmdQ, const DqParams p) {
     using S = DqSmem<D, NW>;
-    constexpr bool PREFIX = KIND != SCORE_PLAIN, SCORED = score_changed(KIND);  // perhaps a prefix; other scores
+    constexpr bool PREFIX = KIND != SCORE_PLAIN, SCORED = score_changed(KIND), WINDOW = (KIND & SCORE_WINDOW) != 0;  // perhaps a prefix; other scores
     constexpr int NSK = S::NSK, NC = S::COLS;
     constexpr bool kOne = D == 128;  // one warp issues all MMAs
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -112,6 +112,12 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     const uint32_t sdO = sbase + S::off_do, sV = sbase + S::off_v;
     auto sK = [&](int s) { return sbase + S::off_k + uint32_t(s) * S::TILE; };
     auto sVec = [&](int s) { return sbase + S::off_vec + uint32_t(s) * S::VEC; };
+    // candidate c of an item, as the scheduler has left word of its walk
+    auto block_of = [](int lo, int walked, int c) {
+        const int block = lo + c;
+        return WINDOW && block >= (walked >> 11 & 2047) ? block + int(uint32_t(walked) >> 22) : block;
+    };
+    static_assert(kListCap < 2048, "bits of a walk");
     auto walk_of = [&](int s, int n) { return DqWalk{smem + S::off_flags + s * S::FLAGS, n}; };
 
     if (tid == 0) {
@@ -186,9 +192,17 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                 int qb, h, b;
                 decode(j, qb, h, b);
                 const int he = (mk.He == 1) ? 0 : h;
-                int lo, hi;
-                kv_range<PREFIX>(mk, b, he, qb, lo, hi);
-                int n = hi - lo;
+                KeyWalk walk;  // WINDOW
+                int lo, n;
+                if constexpr (WINDOW) {
+                    walk = kv_walk<PREFIX, true>(mk, b, he, qb);
+                    lo = walk.lo;
+                    n = walk.n;
+                } else {
+                    int hi;
+                    kv_range<PREFIX>(mk, b, he, qb, lo, hi);
+                    n = hi - lo;
+                }
                 if (n > kListCap) n = kListCap;  // the host refuses problems that could exceed the cap
                 uint8_t* fl = smem + S::off_flags + s * S::FLAGS;
                 int cnt = 0;
@@ -197,7 +211,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                     for (int e = 0; e < 4; ++e) {
                         const int c = 4 * i + e;
                         if (c >= n) break;
-                        const uint32_t f = classify_from_plan<PREFIX>(mk, b, he, qb, lo + c);
+                        const uint32_t f = classify_from_plan<PREFIX, WINDOW>(mk, b, he, qb, WINDOW ? walk.block(c) : lo + c);
                         uint32_t code = QC_SKIP;
                         if (f & TILE_VISIT) code = !(f & TILE_DOC) ? QC_PLAIN : (f & TILE_KMANY) ? QC_DOCMANY : QC_DOC;
                         cnt += (code != QC_SKIP);
@@ -209,7 +223,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                 __syncwarp();
                 if (lane == 0) {
                     info[s * 8 + 0] = lo;
-                    info[s * 8 + 1] = n;
+                    info[s * 8 + 1] = WINDOW ? n | walk.border << 11 | walk.skip << 22 : n;  // (as block_of takes it apart)
                     info[s * 8 + 2] = cnt;
                     info[s * 8 + 3] = j;
                     info[s * 8 + 4] = qb;
@@ -244,7 +258,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                     const int s = k & 1;
                     ok = mbar_wait(BAR(B_ITEMFULL + s), (k >> 1) & 1, ab, ST_WAIT_TIMEOUT + 33);
                     if (!ok) break;
-                    const int lo = info[s * 8 + 0], n = info[s * 8 + 1], T = info[s * 8 + 2], j = info[s * 8 + 3];
+                    const int lo = info[s * 8 + 0], walked = info[s * 8 + 1], n = WINDOW ? walked & 2047 : walked, T = info[s * 8 + 2], j = info[s * 8 + 3];
                     if (j < 0) break;
                     const int qb = info[s * 8 + 4], h = info[s * 8 + 5], b = info[s * 8 + 6];
                     const int hk = h / p.G;
@@ -269,7 +283,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                                 if (!ok) break;
                                 mbar_expect_tx(BAR(B_KFULL + st), S::TILE);
                                 for (int x = 0; x < S::NBOX; ++x)
-                                    tma_load_4d(sK(st) + x * S::BOX, &tmK, BAR(B_KFULL + st), x * 64, (lo + ck) * kBlk, hk, b);
+                                    tma_load_4d(sK(st) + x * S::BOX, &tmK, BAR(B_KFULL + st), x * 64, block_of(lo, walked, ck) * kBlk, hk, b);
                                 ck = wk.first_from(ck + 1);
                             }
                             if (t == 0) {
@@ -285,7 +299,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                                 if (!ok) break;
                                 mbar_expect_tx(BAR(B_VFULL), S::TILE);
                                 for (int x = 0; x < S::NBOX; ++x)
-                                    tma_load_4d(sV + x * S::BOX, &tmV, BAR(B_VFULL), x * 64, (lo + cv) * kBlk, hk, b);
+                                    tma_load_4d(sV + x * S::BOX, &tmV, BAR(B_VFULL), x * 64, block_of(lo, walked, cv) * kBlk, hk, b);
                                 cv = wk.first_from(cv + 1);
                             }
                         }
@@ -409,7 +423,7 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             ok = mbar_wait(BAR(B_ITEMFULL + s), (k >> 1) & 1, ab, ST_WAIT_TIMEOUT + 33);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const int lo = info[s * 8 + 0], n = info[s * 8 + 1], T = info[s * 8 + 2], j = info[s * 8 + 3];
+            const int lo = info[s * 8 + 0], walked = info[s * 8 + 1], n = WINDOW ? walked & 2047 : walked, T = info[s * 8 + 2], j = info[s * 8 + 3];
             if (j < 0) break;
             const int qb = info[s * 8 + 4], h = info[s * 8 + 5], b = info[s * 8 + 6];
             const int he = (mk.He == 1) ? 0 : h;
@@ -434,9 +448,10 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 #pragma unroll 1
                 do code = wk.code(++cc); while (code == QC_SKIP);
                 const bool fl_doc = code >= QC_DOC, many = code == QC_DOCMANY;
-                const int kb0 = (lo + cc) * kBlk;
+                const int kb0 = block_of(lo, walked, cc) * kBlk;
                 const int kb1 = min(kb0 + kBlk, mk.N);
-                const bool fl_bound = (kb0 + kBlk > mk.N) || (mk.causal && kb1 - 1 > q0 + mk.gap && (!PREFIX || kb1 > front));
+                const bool fl_bound = (kb0 + kBlk > mk.N) || (mk.causal && kb1 - 1 > q0 + mk.gap && (!PREFIX || kb1 > front)) ||
+                                      (WINDOW && kb0 < q0 + kBlk + mk.gap - mk.window && kb1 > early_keys<true>(front, mk.sinks));
                 const int k0 = kb0 + cbase;  // first key column of this thread
                 const uint32_t tS = tmem + lane_base + uint32_t(gi & 1) * 128u + uint32_t(cbase);
                 // keep(x) = (x <= lim) & (qc >= 0 | kc[x] == qc) as 32-bit masks, worked out before the scores are there
@@ -461,6 +476,11 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
                         if (mk.causal) jmax = min(jmax, PREFIX ? max(row + mk.gap, front - 1) : row + mk.gap);
 #pragma unroll
                         for (int q = 0; q < NC / 32; ++q) keep[q] &= first_bits(jmax + 1 - k0 - 32 * q);
+                        if constexpr (WINDOW) {
+#pragma unroll
+                            for (int q = 0; q < NC / 32; ++q)
+                                keep[q] &= ~hidden_bits(row + mk.gap - mk.window + 1 - k0 - 32 * q, early_keys<true>(front, mk.sinks) - k0 - 32 * q);
+                        }
                     }
                 }
                 ok = mbar_wait(BAR(B_SFULL + (gi & 1)), (gi >> 1) & 1, ab, ST_WAIT_TIMEOUT + 27);
@@ -661,6 +681,12 @@ cudaError_t launch_bwd_dq(int D, bool bf16, const CUtensorMap& tq, const CUtenso
         if (p.score.kind == SCORE_CAPPED_BIAS) return of(integral_constant<int, SCORE_CAPPED_BIAS>{});
         if (p.score.kind == SCORE_CAPPED) return of(integral_constant<int, SCORE_CAPPED>{});
         if (p.score.kind == SCORE_PREFIX) return of(integral_constant<int, SCORE_PREFIX>{});
+        if constexpr (kWarps == 8) {  // (a window needs a causal mask)
+            if (p.score.kind == (SCORE_WINDOW | SCORE_CAPPED_BIAS)) return of(integral_constant<int, SCORE_WINDOW | SCORE_CAPPED_BIAS>{});
+            if (p.score.kind == (SCORE_WINDOW | SCORE_CAPPED)) return of(integral_constant<int, SCORE_WINDOW | SCORE_CAPPED>{});
+            if (p.score.kind == (SCORE_WINDOW | SCORE_BIAS)) return of(integral_constant<int, SCORE_WINDOW | SCORE_BIAS>{});
+            if (p.score.kind == SCORE_WINDOW) return of(integral_constant<int, SCORE_WINDOW>{});
+        }
         if (p.score.kind == SCORE_BIAS) return of(integral_constant<int, SCORE_BIAS>{});
         return of(integral_constant<int, SCORE_PLAIN>{});
     };

@@ -77,6 +77,8 @@ struct MaskArgs {
     int debug;            // DBG_* bits (0 in normal use)
     const int32_t* prefix;  // [B], or null: with a causal mask, so many leading keys are visible to every query (the ids' rule holds for them too).
                             // Looked at by the instances for attention_scored alone (kPrefix below)
+    int window, sinks;      // with a causal mask: a query at position i + gap sees the last `window` keys up to there and, of those before, the first `sinks`.
+                            // Looked at by the instances with a window alone (kWindow below)
 };
 
 // Leading keys that the causal mask leaves visible to every query of sequence b.
@@ -86,6 +88,9 @@ __device__ __forceinline__ int front_keys(const MaskArgs& a, int b) {
     const int n = a.prefix[b];
     return n < 0 ? 0 : n > a.N ? a.N : n;
 }
+// Leading keys that the window hides from no query.
+template <bool kWindow>
+__host__ __device__ __forceinline__ int early_keys(int front, int sinks) { return kWindow && sinks > front ? sinks : front; }
 
 // Debug switches that change which tiles are visited and how they are evaluated, never the result:
 // they exist to show that skipping tiles and the per-chunk shortcuts are exact.
@@ -112,9 +117,10 @@ enum : uint32_t {
 
 // Classification of tile (qb, kb) from the block statistics. Conservative: a tile is skipped
 // only when every entry is masked, and declared free of a check only when every entry passes it.
-// front: leading keys that the causal mask does not hide; nothing is left of it where it is the constant 0.
+// front: leading keys that the causal mask does not hide; nothing is left of it where it is the constant 0. window: 0 for none, else with `early`, the
+// leading keys that it does not hide.
 __host__ __device__ inline uint32_t classify_tile(int qb, int kb, int M, int N, int gap, int causal,
-                                                  int mode, int qmin, int qmax, int kmin, int kmax, int front = 0) {
+                                                  int mode, int qmin, int qmax, int kmin, int kmax, int front = 0, int window = 0, int early = 0) {
     const int q0 = qb * kBlk, k0 = kb * kBlk;
     const int q1 = (q0 + kBlk < M) ? q0 + kBlk : M;  // exclusive
     const int k1 = (k0 + kBlk < N) ? k0 + kBlk : N;
@@ -124,6 +130,10 @@ __host__ __device__ inline uint32_t classify_tile(int qb, int kb, int M, int N, 
     if (causal) {
         if (k0 > q1 - 1 + gap && (front <= 0 || k0 >= front)) return 0;
         if (k1 - 1 > q0 + gap && (front <= 0 || k1 > front)) f |= TILE_BOUND;
+        if (window > 0) {
+            if (k1 <= q0 + gap - window + 1 && k0 >= early) return 0;
+            if (k0 < q1 - 1 + gap - window + 1 && k1 > early) f |= TILE_BOUND;
+        }
     }
     if (mode == 1) {
         if (qmax < 0 && (kmax < qmin || kmin > qmax)) return 0;
@@ -135,9 +145,9 @@ __host__ __device__ inline uint32_t classify_tile(int qb, int kb, int M, int N, 
 }
 
 // All loads are issued together: they are on the way of a kernel's first tile. Bits that a caller does not look at cost none.
-template <bool kPrefix = false>
+template <bool kPrefix = false, bool kWindow = false>
 __device__ __forceinline__ uint32_t classify_from_plan(const MaskArgs& a, int b, int he, int qb, int kb) {
-    const int front = front_keys<kPrefix>(a, b);
+    const int front = front_keys<kPrefix>(a, b), window = kWindow ? a.window : 0, early = kWindow ? early_keys<true>(front, a.sinks) : 0;
     int qmin = 0, qmax = 0, kmin = 0, kmax = 0, qf = 0, kf = 0;
     if (a.mode == 1) {
         const int64_t bh = int64_t(b) * a.He + he;
@@ -148,10 +158,10 @@ __device__ __forceinline__ uint32_t classify_from_plan(const MaskArgs& a, int b,
         qf = a.plan[a.L.off_qflags + bh * a.L.nQ + qb];
         kf = a.plan[a.L.off_kflags + bh * a.L.nK + kb];
     }
-    uint32_t f = classify_tile(qb, kb, a.M, a.N, a.gap, a.causal, a.mode, qmin, qmax, kmin, kmax, front);
+    uint32_t f = classify_tile(qb, kb, a.M, a.N, a.gap, a.causal, a.mode, qmin, qmax, kmin, kmax, front, window, early);
     if (a.debug) {
         if ((a.debug & DBG_NO_SKIP) && f == 0 && a.mode == 1) {
-            f = classify_tile(qb, kb, a.M, a.N, a.gap, a.causal, 0, 0, 0, 0, 0, front);  // the bounds alone
+            f = classify_tile(qb, kb, a.M, a.N, a.gap, a.causal, 0, 0, 0, 0, 0, front, window, early);  // the bounds alone
             if (f) f |= TILE_DOC;                                                // the ids mask every entry
         }
         if ((a.debug & DBG_ALL_PARTIAL) && f) return f | TILE_BOUND | (a.mode == 1 ? TILE_DOC : 0u);
@@ -164,7 +174,7 @@ __device__ __forceinline__ uint32_t classify_from_plan(const MaskArgs& a, int b,
 }
 
 // Key-block range [lo, hi) a query block has to walk.
-template <bool kPrefix = false>
+template <bool kPrefix = false, bool kWindow = false>
 __device__ __forceinline__ void kv_range(const MaskArgs& a, int b, int he, int qb, int& lo, int& hi) {
     if (a.mode == 1 && !(a.debug & DBG_NO_SKIP)) {
         const int64_t bh = int64_t(b) * a.He + he;
@@ -180,8 +190,37 @@ __device__ __forceinline__ void kv_range(const MaskArgs& a, int b, int he, int q
         }
     }
 }
+// The same as a walk over candidates 0 .. n - 1: with a window those between the first keys and the window's are left out.
+struct KeyWalk {
+    int lo, n;
+    int border, skip;  // from this key block on, so many blocks lie in between
+    __device__ __forceinline__ int block(int c) const { return lo + c + (lo + c >= border ? skip : 0); }
+};
+template <bool kPrefix, bool kWindow>
+__device__ __forceinline__ KeyWalk kv_walk(const MaskArgs& a, int b, int he, int qb) {
+    KeyWalk w;
+    int hi;
+    kv_range<kPrefix, kWindow>(a, b, he, qb, w.lo, hi);
+    w.border = hi;
+    w.skip = 0;
+    w.n = hi - w.lo;
+    if (kWindow && !(a.debug & DBG_NO_SKIP)) {
+        const int early = cdiv(early_keys<true>(front_keys<kPrefix>(a, b), min(a.sinks, a.N)), kBlk), first = min(max(0, qb * kBlk + a.gap - a.window + 1) / kBlk, hi);
+        if (w.lo < early) {
+            if (first > early) {
+                w.border = early;
+                w.skip = first - early;
+                w.n -= w.skip;
+            }
+        } else if (w.lo < first) {
+            w.lo = first;
+            w.n = hi - first;
+        }
+    }
+    return w;
+}
 // Query-block range [lo, hi) a key block has to walk.
-template <bool kPrefix = false>
+template <bool kPrefix = false, bool kWindow = false>
 __device__ __forceinline__ void q_range(const MaskArgs& a, int b, int he, int kb, int& lo, int& hi) {
     if (a.mode == 1 && !(a.debug & DBG_NO_SKIP)) {
         const int64_t bh = int64_t(b) * a.He + he;
@@ -193,6 +232,10 @@ __device__ __forceinline__ void q_range(const MaskArgs& a, int b, int he, int kb
         if (a.causal) {
             const int first = kb * kBlk - a.gap;  // first query row that sees key k0
             lo = first > 0 && (!kPrefix || kb * kBlk >= front_keys<kPrefix>(a, b)) ? first / kBlk : 0;
+            if (kWindow && kb * kBlk >= early_keys<true>(front_keys<kPrefix>(a, b), a.sinks)) {
+                const int last = min(kb * kBlk + kBlk, a.N) - 2 + a.window - a.gap;  // the last row that sees the block's last key
+                hi = last < 0 ? 0 : min(hi, last / kBlk + 1);
+            }
             if (lo > hi) lo = hi;
         }
     }
@@ -201,10 +244,10 @@ __device__ __forceinline__ void q_range(const MaskArgs& a, int b, int he, int kb
 // The per-entry predicate on codes. Identical to the reference's rule on the original ids:
 // qc >= 0 <=> eq >= 0; for eq < 0, qc == eq and kc == ek whenever ek is a negative int32,
 // and kc == 0 != qc otherwise.
-template <bool kPrefix = false>
-__device__ __forceinline__ bool keep_entry(int i, int j, int qc, int kc, int N, int gap, int causal, int mode, int front = 0) {
+template <bool kPrefix = false, bool kWindow = false>
+__device__ __forceinline__ bool keep_entry(int i, int j, int qc, int kc, int N, int gap, int causal, int mode, int front = 0, int window = 0, int sinks = 0) {
     bool keep = j < N;
-    if (causal) keep = keep && (gap + i >= j || (kPrefix && j < front));
+    if (causal) keep = keep && ((gap + i >= j && (!kWindow || gap + i - j < window || j < sinks)) || (kPrefix && j < front));
     if (mode == 1) keep = keep && ((qc >= 0) || (qc == kc));
     return keep;
 }
@@ -216,6 +259,8 @@ __device__ __forceinline__ bool keep_entry(int i, int j, int qc, int kc, int N, 
 // 118 -> 111 us with 8 x 8 heads of 1024 queries, 8192 keys in 8 documents; 250 -> 242 and 168 -> 163 us with 4 x 16 heads x 4096 in
 // up to 16 documents.
 __device__ __forceinline__ uint32_t first_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+// Those that a window hides: from `early` on and below `low`.
+__device__ __forceinline__ uint32_t hidden_bits(int low, int early) { return first_bits(low) & ~first_bits(early); }
 
 // Bit x of the result: codes[x] (32 of them, 16-byte aligned; `code` is the lane's own) equals this thread's `own`. All
 // lanes of the warp take part. A walk over the distinct codes of the chunk costs a shuffle and a vote for each (one to

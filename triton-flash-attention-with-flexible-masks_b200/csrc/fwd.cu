@@ -105,7 +105,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
            const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const FwdParams p) {
     using S = FwdSmem<D>;
-    constexpr bool PREFIX = KIND != SCORE_PLAIN, SCORED = score_changed(KIND);  // perhaps a prefix; other scores
+    constexpr bool PREFIX = KIND != SCORE_PLAIN, SCORED = score_changed(KIND), WINDOW = (KIND & SCORE_WINDOW) != 0;  // perhaps a prefix; other scores
+    constexpr int SCORES = KIND & SCORE_CAPPED_BIAS;
     constexpr int NS = S::NS, NQ = S::NQ, NP = S::NP;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -149,9 +150,10 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         int qb, h, b, lo, n;
         uint32_t flags;
         int4 qc;
+        KeyWalk walk;  // WINDOW: of all runs' tiles
     };
     auto classify = [&](const Item& it, int i) {
-        return i < it.n ? classify_from_plan<PREFIX>(mk, it.b, (mk.He == 1) ? 0 : it.h, it.qb, it.lo + i) & (TILE_VISIT | TILE_BOUND | TILE_DOC | TILE_KMONO | TILE_KMANY) : 0u;
+        return i < it.n ? classify_from_plan<PREFIX, WINDOW>(mk, it.b, (mk.He == 1) ? 0 : it.h, it.qb, WINDOW ? it.walk.block(it.lo + i) : it.lo + i) & (TILE_VISIT | TILE_BOUND | TILE_DOC | TILE_KMONO | TILE_KMANY) : 0u;
     };
     auto prepare = [&](int j) {
         Item it;
@@ -159,7 +161,13 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
         decode(SHORT ? j / ns : j, it.qb, it.h, it.b);
         const int he = (mk.He == 1) ? 0 : it.h;
         int lo, hi;
-        kv_range<PREFIX>(mk, it.b, he, it.qb, lo, hi);
+        if constexpr (WINDOW) {  // candidates by their place in the walk; the list has the blocks themselves
+            it.walk = kv_walk<PREFIX, true>(mk, it.b, he, it.qb);
+            lo = 0;
+            hi = it.walk.n;
+        } else {
+            kv_range<PREFIX>(mk, it.b, he, it.qb, lo, hi);
+        }
         int n = hi - lo;
         if constexpr (SHORT) {  // no ids: every tile of the range is visited
             const int first = int(int64_t(n) * sp / ns);
@@ -297,13 +305,13 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     const int i = base + lane;
                     const uint32_t f = base == 0 ? item.flags : classify(item, i);
                     const uint32_t m = __ballot_sync(0xffffffffu, (f & TILE_VISIT) != 0);
-                    if (f & TILE_VISIT) list[T + __popc(m & ((1u << lane) - 1u))] = uint16_t(uint32_t(i) | ((f & ~TILE_KMANY) | ((f & TILE_KMANY) ? LIST_KMANY : 0u)) << 10);
+                    if (f & TILE_VISIT) list[T + __popc(m & ((1u << lane) - 1u))] = uint16_t(uint32_t(WINDOW ? item.walk.block(item.lo + i) : i) | ((f & ~TILE_KMANY) | ((f & TILE_KMANY) ? LIST_KMANY : 0u)) << 10);
                     T += __popc(m);
                 }
                 reinterpret_cast<int4*>(smem + S::off_qc)[s * 32 + lane] = item.qc;
                 if (lane == 0) {
                     info[s * 8 + 0] = T;
-                    info[s * 8 + 1] = item.lo;
+                    info[s * 8 + 1] = WINDOW ? 0 : item.lo;
                     info[s * 8 + 2] = j;
                     info[s * 8 + 3] = SHORT ? item.h / nG : item.h / p.G;
                     info[s * 8 + 4] = item.qb;
@@ -705,8 +713,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                 if constexpr (SCORED) {
                     const int first = SHORT ? 0 : qb * kBlk, last = SHORT ? mk.M - 1 : qb * kBlk + kBlk - 1;  // rows of the tile, and perhaps more
                     const Bias bias(slope, mk.causal && front == 0, first + mk.gap - (k0 + kBlk - 1), last + mk.gap - k0);
-                    if constexpr (KIND == SCORE_CAPPED) late = !(fl & (TILE_BOUND | TILE_DOC)) && !any_beyond<kBlk>(sc, valid ? p.score.most : INFINITY);
-                    if (!late) score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, row + mk.gap - k0, valid, m_run == -INFINITY ? 0.f : m_run);
+                    if constexpr (SCORES == SCORE_CAPPED) late = !(fl & (TILE_BOUND | TILE_DOC)) && !any_beyond<kBlk>(sc, valid ? p.score.most : INFINITY);
+                    if (!late) score_row<SCORES, kBlk>(sc, p.score, bias, p.scale_log2, row + mk.gap - k0, valid, m_run == -INFINITY ? 0.f : m_run);
                 }
 
                 if (fl & (TILE_BOUND | TILE_DOC)) {
@@ -738,7 +746,10 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     }
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const uint32_t keep = first_bits(lim + 1 - 32 * q) & same[q];
+                        uint32_t keep = first_bits(lim + 1 - 32 * q) & same[q];
+                        if constexpr (WINDOW) {
+                            if (fl & TILE_BOUND) keep &= ~hidden_bits(row + mk.gap - mk.window + 1 - k0 - 32 * q, early_keys<true>(front, mk.sinks) - k0 - 32 * q);
+                        }
                         if (__any_sync(0xffffffffu, keep != ~0u)) {
 #pragma unroll
                             for (int x = 0; x < 32; ++x) sc[32 * q + x] = (keep & (1u << x)) ? sc[32 * q + x] : -INFINITY;
@@ -833,7 +844,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     }
                 };
                 if constexpr (!SCORED) exponentials([&](uint64_t s2) { return fma_f2(s2, c2, mneg2); });
-                else if (KIND == SCORE_CAPPED && late) exponentials([&](uint64_t s2) { return fma_f2(s2, cap_poly(s2, p.score), mneg2); });
+                else if (SCORES == SCORE_CAPPED && late) exponentials([&](uint64_t s2) { return fma_f2(s2, cap_poly(s2, p.score), mneg2); });
                 else exponentials([&](uint64_t s2) { return s2; });
                 tc_wait_st();
                 tc_fence_before();
@@ -989,6 +1000,10 @@ cudaError_t launch_fwd(int D, bool bf16, const CUtensorMap& tq, const CUtensorMa
         if (p.score.kind == SCORE_CAPPED_BIAS) return of(integral_constant<int, SCORE_CAPPED_BIAS>{});
         if (p.score.kind == SCORE_CAPPED) return of(integral_constant<int, SCORE_CAPPED>{});
         if (p.score.kind == SCORE_PREFIX) return of(integral_constant<int, SCORE_PREFIX>{});
+        if (p.score.kind == (SCORE_WINDOW | SCORE_CAPPED_BIAS)) return of(integral_constant<int, SCORE_WINDOW | SCORE_CAPPED_BIAS>{});
+        if (p.score.kind == (SCORE_WINDOW | SCORE_CAPPED)) return of(integral_constant<int, SCORE_WINDOW | SCORE_CAPPED>{});
+        if (p.score.kind == (SCORE_WINDOW | SCORE_BIAS)) return of(integral_constant<int, SCORE_WINDOW | SCORE_BIAS>{});
+        if (p.score.kind == SCORE_WINDOW) return of(integral_constant<int, SCORE_WINDOW>{});
         if (p.score.kind == SCORE_BIAS) return of(integral_constant<int, SCORE_BIAS>{});
         return of(integral_constant<int, SCORE_PLAIN>{});
     };

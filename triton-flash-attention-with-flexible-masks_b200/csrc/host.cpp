@@ -94,14 +94,14 @@ fa_ids id_view(const Tensor& t) {
 
 // The plan of a call: its memory and the launches that fill it. eq and ek, if any, are int32 or int64 tensors [B, H, M] and [B, H, N].
 // scores: of attention_scored, else null (here and below).
-Tensor build_plan(const fa_problem& p, const Tensor* eq, const Tensor* ek, const Tensor& status, const fa_scores* scores = nullptr) {
+Tensor build_plan(const fa_problem& p, const Tensor* eq, const Tensor* ek, const Tensor& status, const fa_scores* scores = nullptr, const fa_window* window = nullptr) {
     size_t bytes = 0;
     check(fa_plan_bytes(&p, &bytes), "fa_plan_bytes");
     Tensor plan = at::empty({int64_t(bytes / 4)}, status.options());
     const fa_ids q = eq ? id_view(*eq) : fa_ids{}, k = ek ? id_view(*ek) : fa_ids{};
     if (scores)
-        check(fa_plan_build_scored(&p, scores, eq ? &q : nullptr, ek ? &k : nullptr, plan.data_ptr(), bytes, status.data_ptr<int>(), current_stream(status)),
-              "fa_plan_build_scored");
+        check(fa_plan_build_windowed(&p, scores, window, eq ? &q : nullptr, ek ? &k : nullptr, plan.data_ptr(), bytes, status.data_ptr<int>(), current_stream(status)),
+              "fa_plan_build_windowed");
     else
         check(fa_plan_build(&p, eq ? &q : nullptr, ek ? &k : nullptr, plan.data_ptr(), bytes, status.data_ptr<int>(), current_stream(status)),
               "fa_plan_build");
@@ -122,13 +122,13 @@ struct Outputs {
 
 // The forward's allocations and launches for a problem that `regular` has filled.
 Outputs launch_forward(const fa_problem& p, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& plan, int key_runs,
-                       const Tensor& status, const std::optional<Tensor>& out, const fa_scores* scores = nullptr, bool backward = false) {
+                       const Tensor& status, const std::optional<Tensor>& out, const fa_scores* scores = nullptr, bool backward = false, const fa_window* window = nullptr) {
     Outputs r;
     r.o = out ? *out : at::empty_like(q);
     if (!taken_as_is(r.o)) r.o = at::empty(q.sizes(), q.options());
     const auto f32 = q.options().dtype(at::kFloat);
     r.lse = at::empty({p.B, p.H, fa_padded_rows(p.M)}, f32);
-    r.splits = key_runs != 0 ? key_runs : fa_fwd_splits(&p);  // (a number below 1 is the library's to refuse)
+    r.splits = key_runs != 0 ? key_runs : fa_fwd_splits_windowed(&p, window);  // (a number below 1 is the library's to refuse)
     Tensor work;
     size_t bytes = 0;
     if (r.splits > 1) {
@@ -140,9 +140,9 @@ Outputs launch_forward(const fa_problem& p, const Tensor& q, const Tensor& k, co
     void* const work_ptr = work.defined() ? work.data_ptr() : nullptr;
     if (scores && backward && p.dtype != FA_FP32) r.rest = at::empty({p.B, p.H, p.M, p.D}, q.options());
     if (scores)
-        check(fa_fwd_scored(&p, scores, &tq, &tk, &tv, &to, r.rest.defined() && r.splits == 1 ? r.rest.data_ptr() : nullptr, r.lse.data_ptr<float>(), plan_ptr, r.splits, work_ptr, bytes, status.data_ptr<int>(),
+        check(fa_fwd_windowed(&p, scores, window, &tq, &tk, &tv, &to, r.rest.defined() && r.splits == 1 ? r.rest.data_ptr() : nullptr, r.lse.data_ptr<float>(), plan_ptr, r.splits, work_ptr, bytes, status.data_ptr<int>(),
                             current_stream(q)),
-              "fa_fwd_scored");
+              "fa_fwd_windowed");
     else
         check(fa_fwd_split(&p, &tq, &tk, &tv, &to, r.lse.data_ptr<float>(), plan_ptr, r.splits, work_ptr, bytes, status.data_ptr<int>(), current_stream(q)),
               "fa_fwd_split");
@@ -154,16 +154,16 @@ Outputs launch_forward(const fa_problem& p, const Tensor& q, const Tensor& k, co
 // dq, dk, dv. q, k, v, o, lse and the problem are those of a forward, d_o is like q.
 std::array<Tensor, 3> launch_backward(const fa_problem& p, const Tensor& d_o, const Tensor& q, const Tensor& k, const Tensor& v,
                                       const Tensor& o, const Tensor& lse, const Tensor& plan, const Tensor& status,
-                                      const fa_scores* scores = nullptr, const Tensor& rest = Tensor()) {
+                                      const fa_scores* scores = nullptr, const Tensor& rest = Tensor(), const fa_window* window = nullptr) {
     Tensor delta = at::empty_like(lse);
     Tensor dk = at::empty({p.B, p.Hk, p.N, p.D}, k.options()), dv = at::empty({p.B, p.Hk, p.N, p.D}, v.options());
     Tensor dq = at::empty(q.sizes(), q.options());
     const fa_tensor tq = view(q), tk = view(k), tv = view(v), to = view(o), tdo = view(d_o), tdq = view(dq), tdk = view(dk), tdv = view(dv);
     void* const plan_ptr = plan.defined() ? plan.data_ptr() : nullptr;
     if (scores)
-        check(fa_bwd_scored(&p, scores, &tq, &tk, &tv, &to, rest.defined() ? rest.data_ptr() : nullptr, &tdo, lse.data_ptr<float>(), delta.data_ptr<float>(), &tdq, &tdk, &tdv, plan_ptr,
+        check(fa_bwd_windowed(&p, scores, window, &tq, &tk, &tv, &to, rest.defined() ? rest.data_ptr() : nullptr, &tdo, lse.data_ptr<float>(), delta.data_ptr<float>(), &tdq, &tdk, &tdv, plan_ptr,
                             status.data_ptr<int>(), current_stream(q)),
-              "fa_bwd_scored");
+              "fa_bwd_windowed");
     else
         check(fa_bwd(&p, &tq, &tk, &tv, &to, &tdo, lse.data_ptr<float>(), delta.data_ptr<float>(), &tdq, &tdk, &tdv, plan_ptr, status.data_ptr<int>(),
                      current_stream(q)),
@@ -320,20 +320,21 @@ void once(std::array<Tensor, 3>& g, const Tensor& q, const Tensor& k, const Tens
 struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
     struct Scores {
         fa_scores s;
+        fa_window window;
         const std::optional<Tensor>&slopes, &prefix;
     };
 
-    static Outputs launch(const Tensor& q, const Tensor& k, const Tensor& v, const Call& c, const fa_scores& s, Tensor& plan) {
+    static Outputs launch(const Tensor& q, const Tensor& k, const Tensor& v, const Call& c, const fa_scores& s, const fa_window& w, Tensor& plan) {
         py::gil_scoped_release free;
-        if (c.eq || !fa_plan_optional(&c.p, c.needs_grad)) plan = build_plan(c.p, c.eq, c.ek, c.status, &s);
-        Outputs r = launch_forward(c.p, q, k, v, plan, 0, c.status, std::nullopt, &s, c.needs_grad);
+        if (c.eq || !fa_plan_optional(&c.p, c.needs_grad)) plan = build_plan(c.p, c.eq, c.ek, c.status, &s, &w);
+        Outputs r = launch_forward(c.p, q, k, v, plan, 0, c.status, std::nullopt, &s, c.needs_grad, &w);
         n_launched += (plan.defined() ? c.plan_kernels : 0) + (r.splits > 1 ? 2 + r.rest.defined() : 1);
         return r;
     }
 
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Call& c, const Scores& sc) {
         Tensor plan;
-        Outputs r = launch(q, k, v, c, sc.s, plan);
+        Outputs r = launch(q, k, v, c, sc.s, sc.window, plan);
         torch::autograd::variable_list saved{q, k, v, r.o, r.lse};
         if (sc.slopes) saved.push_back(*sc.slopes);
         if (sc.prefix) saved.push_back(*sc.prefix);
@@ -347,6 +348,8 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
         data["id_heads"] = int64_t(c.p.id_heads);
         data["scale"] = c.sm_scale;
         data["softcap"] = double(sc.s.softcap);
+        data["window"] = int64_t(sc.window.keys);
+        data["sinks"] = int64_t(sc.window.sinks);
         data["slopes"] = sc.slopes.has_value();
         data["prefix"] = sc.prefix.has_value();
         return r.o;
@@ -363,6 +366,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
                     "flash_b200: the saved q, k, v are not plain [bs, H, L, D] CUDA tensors of matching shapes");
         size_t at = 5;
         fa_scores s{float(data["softcap"].toDouble()), nullptr, nullptr};
+        const fa_window w{int(data["window"].toInt()), int(data["sinks"].toInt())};
         if (data["slopes"].toBool()) s.slopes = saved[at++].const_data_ptr<float>();
         if (data["prefix"].toBool()) s.prefix = saved[at++].const_data_ptr<int>();
         const Tensor rest = saved.size() > at ? saved[at] : Tensor();
@@ -371,7 +375,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
         d_o = d_o.resolve_neg();
         TORCH_CHECK(like_query(d_o, q), "flash_b200: the gradient is not a plain [bs, H, M, D] CUDA tensor");
         if (!taken_as_is(d_o)) d_o = d_o.contiguous();  // (ops.maybe_contiguous)
-        auto g = launch_backward(p, d_o, q, k, v, saved[3], saved[4], data["plan"].toTensor(), data["status"].toTensor(), &s, rest);
+        auto g = launch_backward(p, d_o, q, k, v, saved[3], saved[4], data["plan"].toTensor(), data["status"].toTensor(), &s, rest, &w);
         n_launched += 3;
         once(g, q, k, v);
         return {std::move(g[0]), std::move(g[1]), std::move(g[2]), Tensor(), Tensor()};
@@ -381,10 +385,10 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
 // The whole of a regular call of attention_scored, its gradients included; None: scored.py takes it another way.
 py::object attend_scored(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, std::optional<double> scale, const std::optional<Tensor>& eq,
                          const std::optional<Tensor>& ek, int64_t mode, double softcap, const std::optional<Tensor>& slopes,
-                         const std::optional<Tensor>& prefix, const Tensor& status) {
+                         const std::optional<Tensor>& prefix, int64_t window, int64_t sinks, const Tensor& status) {
     fa_problem p;
     const double sm_scale = scale ? *scale : 1.0 / std::sqrt(double(q.dim() == 4 ? q.size(3) : 1));
-    if (eq.has_value() != ek.has_value() || mode != (eq ? FA_MODE1_DOC : FA_MODE0_NOPE) || (prefix && !causal)) return py::none();
+    if (eq.has_value() != ek.has_value() || mode != (eq ? FA_MODE1_DOC : FA_MODE0_NOPE) || ((prefix || window) && !causal)) return py::none();
     if (!regular(q, k, v, false, causal, sm_scale, int(mode), 1, p)) return py::none();
     if (eq) {
         if (eq->device() != q.device() || ek->device() != q.device()) return py::none();
@@ -393,13 +397,14 @@ py::object attend_scored(const Tensor& q, const Tensor& k, const Tensor& v, bool
     }
     fa_scores s;
     if (!scores_of(softcap, slopes, prefix, q, p.H, p.B, s)) return py::none();
+    const fa_window w{int(window), int(sinks)};  // (as scored.py has checked it)
     const bool needs_grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
     if (needs_grad && at::SavedTensorDefaultHooks::get_hooks()) return py::none();
     const int plan_kernels = !eq || (p.M + 127) / 128 + (p.N + 127) / 128 <= FA_PLAN_ONE_KERNEL_BLOCKS ? 1 : 3;
     const Call call{p, sm_scale, eq ? &*eq : nullptr, ek ? &*ek : nullptr, status, needs_grad, plan_kernels};
-    if (needs_grad) return py::cast(ScoredAttention::apply(q, k, v, call, ScoredAttention::Scores{s, slopes, prefix}));
+    if (needs_grad) return py::cast(ScoredAttention::apply(q, k, v, call, ScoredAttention::Scores{s, w, slopes, prefix}));
     Tensor plan;
-    return py::cast(ScoredAttention::launch(q, k, v, call, s, plan).o);
+    return py::cast(ScoredAttention::launch(q, k, v, call, s, w, plan).o);
 }
 
 // ---- paged cache (paged.py). A call that is not a regular one on the current device is declined, and paged.py copies, raises or does nothing.

@@ -30,6 +30,7 @@ enum : int {
     SCORE_CAPPED = 2,  // a cap, and perhaps a prefix
     SCORE_CAPPED_BIAS = SCORE_BIAS | SCORE_CAPPED,
     SCORE_PREFIX = 4,  // a prefix alone: the scores are attention's
+    SCORE_WINDOW = 8,  // a window, and perhaps a prefix, with or without the changes above
 };
 // Does an instance change the scores?
 __host__ __device__ constexpr bool score_changed(int kind) { return (kind & SCORE_CAPPED_BIAS) != 0; }
@@ -50,7 +51,7 @@ struct ScoreArgs {
 
 constexpr float kScoreLog2e = 1.4426950408889634f;
 
-inline ScoreArgs make_score_args(float cap, const float* slopes, bool prefix, float sm_scale) {
+inline ScoreArgs make_score_args(float cap, const float* slopes, bool prefix, float sm_scale, bool window = false) {
     // tanh(x) / x up to x = kUpTo: the widest that is off by less than 1.5e-4 of an exponential at the greatest score
     constexpr double kUpTo[3] = {0.9, 0.75, 0.6};
     constexpr double kTanh[3][kTanhTerms] = {{0.999997105, -0.333153478, 0.131495683, -0.0471230871, 0.010487992},   // 2.9e-6 of the value
@@ -63,6 +64,7 @@ inline ScoreArgs make_score_args(float cap, const float* slopes, bool prefix, fl
     s.slopes = slopes;
     s.cap = cap;
     s.kind = (cap > 0.f ? SCORE_CAPPED : SCORE_PLAIN) | (slopes ? SCORE_BIAS : SCORE_PLAIN);
+    if (window) s.kind |= SCORE_WINDOW;
     if (prefix && s.kind == SCORE_PLAIN) s.kind = SCORE_PREFIX;
     if (cap > 0.f) {
         const double a = double(cap) * 1.4426950408889634, k = double(sm_scale) / cap;

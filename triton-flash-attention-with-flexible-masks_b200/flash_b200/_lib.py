@@ -19,6 +19,7 @@ EXPORTS = (
     "fa_debug_wait_timeout", "fa_group_rows", "fa_permute_rows", "fa_fwd_splits", "fa_fwd_workspace_bytes", "fa_fwd_split",
     "fa_plan_optional", "fa_bwd", "fa_plan_build_scored", "fa_fwd_scored", "fa_fwd_rest", "fa_bwd_scored", "fa_paged_append",
     "fa_paged_workspace_bytes", "fa_paged_fwd", "fa_debug_paged_pieces",
+    "fa_plan_build_windowed", "fa_fwd_splits_windowed", "fa_fwd_windowed", "fa_bwd_windowed",
 )
 
 
@@ -41,6 +42,10 @@ class Ids(ctypes.Structure):
 
 class Scores(ctypes.Structure):
     _fields_ = [("softcap", ctypes.c_float), ("slopes", ctypes.c_void_p), ("prefix", ctypes.c_void_p)]
+
+
+class Window(ctypes.Structure):
+    _fields_ = [("keys", ctypes.c_int32), ("sinks", ctypes.c_int32)]
 
 
 class PagedCache(ctypes.Structure):
@@ -104,6 +109,15 @@ def load():
     lib.fa_fwd_rest.argtypes = [P, ctypes.c_int32, vp, size, vp, vp, vp]
     lib.fa_bwd_scored.restype = i32
     lib.fa_bwd_scored.argtypes = [P, S, T, T, T, T, vp, T, vp, vp, T, T, T, vp, vp, vp]
+    W = ctypes.POINTER(Window)
+    lib.fa_plan_build_windowed.restype = i32
+    lib.fa_plan_build_windowed.argtypes = [P, S, W, I, I, vp, size, vp, vp]
+    lib.fa_fwd_splits_windowed.restype = i32
+    lib.fa_fwd_splits_windowed.argtypes = [P, W]
+    lib.fa_fwd_windowed.restype = i32
+    lib.fa_fwd_windowed.argtypes = [P, S, W, T, T, T, T, vp, vp, vp, ctypes.c_int32, vp, size, vp, vp]
+    lib.fa_bwd_windowed.restype = i32
+    lib.fa_bwd_windowed.argtypes = [P, S, W, T, T, T, T, vp, T, vp, vp, T, T, T, vp, vp, vp]
     C, R = ctypes.POINTER(PagedCache), ctypes.POINTER(Rows)
     lib.fa_paged_append.restype = i32
     lib.fa_paged_append.argtypes = [C, ctypes.c_int32, vp, R, R, vp, vp]
