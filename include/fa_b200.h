@@ -17,7 +17,7 @@
  *  - return value 0 = ok, otherwise an FA_ERR_* code (fa_error_string() describes it);
  *  - `status` is one int32 in device memory, zeroed by the caller. Kernels write a non-zero
  *    code there when a bounded wait ran out (100..199), an id was out of range (200), or a page or
- *    a length of a paged cache was (201, 202). The first code stays, but a time-out takes the place
+ *    a length of a paged cache or the parent of a drafted token was (201, 202, 203). The first code stays, but a time-out takes the place
  *    of the others. A time-out code is sticky: while the word holds one, every later
  *    fa_fwd / fa_bwd_dkdv / fa_bwd_dq / fa_paged_fwd launch given that word computes nothing and fills its
  *    outputs (o; dk, dv; dq) with NaN, until the host has read the word and set it back to 0.
@@ -251,6 +251,20 @@ int fa_paged_workspace_bytes(const fa_paged_cache* cache, size_t* bytes);
 int fa_paged_fwd(const fa_paged_cache* cache, int32_t T, int32_t H, const int32_t* starts, float sm_scale, const fa_scores* scores, const fa_rows* q,
                  const fa_rows* o, int32_t fill, void* workspace, size_t bytes, int32_t* status, void* stream);
 
+/* What attention over a paged cache, and an append, may have besides; NULL, or all zeros: nothing.
+ * window: a token at position p sees, of the keys j <= p, those with p - j < window.keys or j < window.sinks. Entries of the table whose pages no token of the call
+ *   sees may hold anything.
+ * parents [T], device: sequences of up to 256 new tokens have them drafted as a tree. parents[t] is the place, among its sequence's new tokens, of the one that token t
+ *   continues, which lies before it, or -1: it continues the cached text. A token then sees the cached text, itself and those on its branch; its position is
+ *   that of the text's end and its depth on the branch. Sequences of more new tokens are chunks, whose parents are not read. A parent that does not lie before its
+ *   token sets status 203 and counts as -1. Not with slopes or a prefix (FA_ERR_SCORES). */
+typedef struct fa_paged_more {
+    fa_window window;
+    const int32_t* parents;
+} fa_paged_more;
+int fa_paged_fwd_more(const fa_paged_cache* cache, const fa_paged_more* more, int32_t T, int32_t H, const int32_t* starts, float sm_scale,
+                      const fa_scores* scores, const fa_rows* q, const fa_rows* o, int32_t fill, void* workspace, size_t bytes, int32_t* status, void* stream);
+
 /* Debug: materialise the kernels' decisions. keep is [B, id_heads, M, N] bytes (1 = unmasked),
  * produced by the same device predicate the attention kernels use; tile_class is
  * [B, id_heads, ceil(M/128), ceil(N/128)] bytes: bit0 visited, bit1 bound/causal check,
@@ -319,6 +333,9 @@ uint32_t fa_classify_tile(int32_t M, int32_t N, int32_t causal, int32_t mode, in
  * piece that the second kernel merges. Exposed so that the cutting can be tested on a CPU. */
 int fa_debug_paged_pieces(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t capacity, const int32_t* lens, const int32_t* starts, const int32_t* prefix,
                           int32_t most_workers, int32_t* rows, int32_t most_rows);
+/* The same of fa_paged_fwd_more (parents: host memory that is not read, NULL for none); key tiles are counted without those that lie between the first keys and the window. */
+int fa_debug_paged_pieces_more(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t capacity, const int32_t* lens, const int32_t* starts, const int32_t* prefix,
+                               const fa_window* window, const int32_t* parents, int32_t most_workers, int32_t* rows, int32_t most_rows);
 
 #ifdef __cplusplus
 }

@@ -78,3 +78,26 @@ def check(got, want, what):
     off = (got.double() - value).abs()
     worst = (off / bound).max().item() if off.numel() else 0.0
     assert worst <= 1, f"{what}: {worst:.2f} times its bound, at most {off.max().item():.3g} off"
+
+
+def paged_keep(length, n, window=None, sinks=0, parents=None, prefix=0, device="cuda"):
+    """[n, length]: which places of a sequence's cache each of its last n tokens sees; `parents` of drafted ones, a list."""
+    base = length - n
+    keep = torch.zeros(n, length, dtype=torch.bool)
+    j = torch.arange(length)
+    for t in range(n):
+        if base + t < 0:
+            continue
+        if parents is None:
+            row = (j <= base + t) & ((base + t - j < window) | (j < sinks)) if window else j <= base + t
+            keep[t] = row | (j < prefix)
+            continue
+        branch = [t]
+        while parents[branch[-1]] >= 0:
+            branch.append(parents[branch[-1]])
+        depth = len(branch) - 1
+        keep[t] = (j < base) & ((base + depth - j < window) | (j < sinks)) if window else j < base
+        for up, a in enumerate(branch):
+            if base + a >= 0 and (not window or up < window or base + depth - up < sinks):
+                keep[t, base + a] = True
+    return keep.to(device)

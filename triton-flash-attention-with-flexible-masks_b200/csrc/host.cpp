@@ -439,6 +439,12 @@ bool cache_of(const Tensor& rows, const Tensor& k_pages, const Tensor& v_pages, 
     return true;
 }
 
+// n contiguous int32 numbers on the device of `like`
+bool int_vector(const Tensor& t, const Tensor& like, int64_t n) {
+    return t.is_cuda() && t.layout() == at::kStrided && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous() && !t.is_neg() &&
+           t.device() == like.device();
+}
+
 fa_rows rows_view(const Tensor& t) { return fa_rows{t.data_ptr(), {t.stride(0), t.stride(1)}}; }
 
 void bump(const Tensor& t) {
@@ -465,13 +471,16 @@ bool paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const
 
 py::object paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens,
                            const std::optional<Tensor>& starts, std::optional<double> scale, double softcap, const std::optional<Tensor>& slopes,
-                           const std::optional<Tensor>& prefix, const std::optional<Tensor>& out, const Tensor& status) {
+                           const std::optional<Tensor>& prefix, const std::optional<Tensor>& out, int64_t window, int64_t sinks, const std::optional<Tensor>& parents,
+                           const Tensor& status) {
     fa_paged_cache c;
     fa_scores s;
     if (!cache_of(q, k_pages, v_pages, table, lens, starts, c)) return py::none();
     const int64_t H = q.size(1);
     const double sm_scale = scale ? *scale : 1.0 / std::sqrt(double(c.D));
     if (H % c.Hk != 0 || H / c.Hk > 128 || !(sm_scale > 0) || !std::isfinite(sm_scale) || !scores_of(softcap, slopes, prefix, q, H, c.B, s)) return py::none();
+    if (parents && !int_vector(*parents, q, q.size(0))) return py::none();
+    const fa_paged_more more{{int(window), int(sinks)}, parents ? parents->const_data_ptr<int>() : nullptr};  // (as paged.py has checked them)
     if (out) {
         if (!rows_as_is(*out, 3) || out->sizes() != q.sizes() || out->scalar_type() != q.scalar_type() || out->device() != q.device() || out->requires_grad())
             return py::none();
@@ -486,9 +495,9 @@ py::object paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor&
         check(fa_paged_workspace_bytes(&c, &bytes), "fa_paged_workspace_bytes");
         Tensor work = at::empty({int64_t(bytes)}, q.options().dtype(at::kByte));
         const fa_rows rq = rows_view(q), ro = rows_view(o);
-        check(fa_paged_fwd(&c, int(q.size(0)), int(H), starts ? starts->const_data_ptr<int>() : nullptr, float(sm_scale), &s, &rq, &ro, out ? 0 : 1, work.data_ptr(),
+        check(fa_paged_fwd_more(&c, &more, int(q.size(0)), int(H), starts ? starts->const_data_ptr<int>() : nullptr, float(sm_scale), &s, &rq, &ro, out ? 0 : 1, work.data_ptr(),
                            bytes, status.data_ptr<int>(), current_stream(q)),
-              "fa_paged_fwd");
+              "fa_paged_fwd_more");
         n_launched += 2;
     }
     if (out) bump(*out);

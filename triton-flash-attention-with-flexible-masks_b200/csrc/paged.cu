@@ -1,5 +1,6 @@
 // extern "C" surface of the paged cache (declared in include/fa_b200.h): argument checks, tensor maps, launches. Nothing here allocates,
 // synchronises or throws.
+#include <algorithm>
 #include "../../include/fa_b200.h"
 #include "common.cuh"
 #include "host_shared.cuh"
@@ -88,6 +89,68 @@ size_t workspace_bytes(int D, int workers) {
     return size_t(2) * workers * fa::kBlk * ((D > 64 ? 128 : 64) + 1) * sizeof(float) + workers * sizeof(int4);
 }
 
+// fa_debug_paged_pieces and fa_debug_paged_pieces_more
+template <bool MASKED>
+int debug_pieces(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t capacity, const int32_t* lens, const int32_t* starts, const int32_t* prefix,
+                 fa_window window, const int32_t* parents, int32_t most_workers, int32_t* rows, int32_t most_rows) {
+    if (B <= 0 || T < 0 || Hk <= 0 || G <= 0 || G > fa::kBlk || capacity <= 0 || !lens || most_workers <= 0 || !rows) return -1;
+    fa::PagedParams p{};
+    p.lens = lens;
+    p.starts = starts;
+    p.prefix = prefix;
+    p.B = B;
+    p.T = T;
+    p.Hk = Hk;
+    p.G = G;
+    p.tokens = fa::kBlk / G;
+    p.capacity = capacity;
+    p.window = window.keys;
+    p.sinks = window.sinks;
+    p.parents = parents;
+    fa::PagedPlan plan;
+    plan.group = fa::paged_group(B);
+    const int entries = fa::paged_entries(B);
+    long long weight = 0, items = 0;
+    int longest = 0;
+    auto each = [&](int g, auto add) {
+        for (int b = g * plan.group; b < B && b < (g + 1) * plan.group; ++b) add(fa::paged_seq<MASKED>(p, b));
+    };
+    for (int g = 0; g < entries; ++g)
+        each(g, [&](const fa::PagedSeq& s) {
+            weight += Hk * fa::paged_weight<MASKED>(p, s, s.tiles, true);
+            items += (long long)Hk * s.tiles;
+            if (s.tiles > 0) longest = std::max(longest, MASKED ? fa::paged_keys<MASKED>(p, s, s.tiles - 1) : s.len);
+        });
+    fa::paged_share_out(plan, weight, items, longest, most_workers);
+    if (plan.workers > 1023) return -1;
+    long long before = 0;
+    for (int g = 0; g < entries; ++g) {
+        plan.sums[g] = before;
+        each(g, [&](const fa::PagedSeq& s) { before += Hk * fa::paged_weight<MASKED>(p, s, s.tiles, plan.keyed); });
+    }
+    int n = 0;
+    auto put = [&](int a, int b, int c, int d, int e, int f, int g, int h) {
+        const int32_t row[8] = {a, b, c, d, e, f, g, h};
+        if (n < most_rows)
+            for (int i = 0; i < 8; ++i) rows[8 * n + i] = row[i];
+        ++n;
+    };
+    for (int w = 0; w < plan.workers; ++w) {
+        bool first = true;
+        fa::paged_stretch<MASKED>(p, plan, w, [&](const fa::PagedWalk<MASKED>& k, int tiles, int lo, int hi, int part) {
+            put(w, k.b, k.hk, k.tile, lo, hi, tiles, part);
+            if (first && fa::paged_first_cut(plan, w, k)) {
+                int from;
+                const int pieces = fa::paged_pieces(p, plan, w, k, from);
+                for (int i = 0; pieces > 1 && i < pieces; ++i) put(-1, k.b, k.hk, k.tile, 0, 0, 0, 2 * (from + i) + (i == 0));
+            }
+            first = false;
+            return true;
+        });
+    }
+    return n;
+}
+
 }  // namespace
 
 extern "C" {
@@ -114,8 +177,8 @@ int fa_paged_workspace_bytes(const fa_paged_cache* cache, size_t* bytes) {
     return FA_OK;
 }
 
-int fa_paged_fwd(const fa_paged_cache* cache, int32_t T, int32_t H, const int32_t* starts, float sm_scale, const fa_scores* scores, const fa_rows* q,
-                 const fa_rows* o, int32_t fill, void* workspace, size_t bytes, int32_t* status, void* stream) {
+int fa_paged_fwd_more(const fa_paged_cache* cache, const fa_paged_more* more, int32_t T, int32_t H, const int32_t* starts, float sm_scale,
+                      const fa_scores* scores, const fa_rows* q, const fa_rows* o, int32_t fill, void* workspace, size_t bytes, int32_t* status, void* stream) {
     int rc = check_cache(cache);
     if (rc) return rc;
     if (H <= 0 || H % cache->Hk != 0) return FA_ERR_BAD_ARG;
@@ -125,6 +188,11 @@ int fa_paged_fwd(const fa_paged_cache* cache, int32_t T, int32_t H, const int32_
     const fa_scores none{};
     const fa_scores* sc = scores ? scores : &none;
     if (sc->softcap != 0.f && !(sc->softcap >= 1e-6f && sc->softcap <= 1e6f)) return FA_ERR_SCORES;
+    const fa_paged_more nothing{};
+    if (!more) more = &nothing;
+    const fa_window window = more->window;
+    if (window.keys < 0 || window.sinks < 0 || (window.keys == 0 && window.sinks > 0) || (more->parents && (sc->slopes || sc->prefix))) return FA_ERR_SCORES;
+    if (!aligned(more->parents, 4)) return FA_ERR_ALIGNMENT;
     if (!aligned(sc->slopes, 4) || !aligned(sc->prefix, 4) || !aligned(workspace, 16)) return FA_ERR_ALIGNMENT;
     fa::PagedParams p{};
     if ((rc = fill_params(&p, cache, T, starts, status))) return rc;
@@ -132,6 +200,9 @@ int fa_paged_fwd(const fa_paged_cache* cache, int32_t T, int32_t H, const int32_
     if (sms <= 0) return FA_ERR_LAUNCH;
     if (!workspace || bytes < workspace_bytes(cache->D, sms)) return FA_ERR_PLAN_SIZE;
     p.prefix = sc->prefix;
+    p.window = std::min(window.keys, kMostTokens + 1);  // (no token is further away)
+    p.sinks = std::min(window.sinks, kMostTokens + 1);
+    p.parents = more->parents;
     p.out = o->ptr;
     p.out_t = o->stride[0];
     p.out_h = o->stride[1];
@@ -157,61 +228,19 @@ int fa_paged_fwd(const fa_paged_cache* cache, int32_t T, int32_t H, const int32_
     return fa::launch_paged_fwd(cache->dtype == FA_BF16, tq, tn, tk, tv, p, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
+int fa_paged_fwd(const fa_paged_cache* cache, int32_t T, int32_t H, const int32_t* starts, float sm_scale, const fa_scores* scores, const fa_rows* q,
+                 const fa_rows* o, int32_t fill, void* workspace, size_t bytes, int32_t* status, void* stream) {
+    return fa_paged_fwd_more(cache, nullptr, T, H, starts, sm_scale, scores, q, o, fill, workspace, bytes, status, stream);
+}
+
 int fa_debug_paged_pieces(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t capacity, const int32_t* lens, const int32_t* starts, const int32_t* prefix,
                           int32_t most_workers, int32_t* rows, int32_t most_rows) {
-    if (B <= 0 || T < 0 || Hk <= 0 || G <= 0 || G > fa::kBlk || capacity <= 0 || !lens || most_workers <= 0 || !rows) return -1;
-    fa::PagedParams p{};
-    p.lens = lens;
-    p.starts = starts;
-    p.prefix = prefix;
-    p.B = B;
-    p.T = T;
-    p.Hk = Hk;
-    p.G = G;
-    p.tokens = fa::kBlk / G;
-    p.capacity = capacity;
-    fa::PagedPlan plan;
-    plan.group = fa::paged_group(B);
-    const int entries = fa::paged_entries(B);
-    long long weight = 0, items = 0;
-    int longest = 0;
-    auto each = [&](int g, auto add) {
-        for (int b = g * plan.group; b < B && b < (g + 1) * plan.group; ++b) add(fa::paged_seq(p, b));
-    };
-    for (int g = 0; g < entries; ++g)
-        each(g, [&](const fa::PagedSeq& s) {
-            weight += Hk * fa::paged_weight(p, s, s.tiles, true);
-            items += (long long)Hk * s.tiles;
-            if (s.tiles > 0 && s.len > longest) longest = s.len;
-        });
-    fa::paged_share_out(plan, weight, items, longest, most_workers);
-    if (plan.workers > 1023) return -1;
-    long long before = 0;
-    for (int g = 0; g < entries; ++g) {
-        plan.sums[g] = before;
-        each(g, [&](const fa::PagedSeq& s) { before += Hk * fa::paged_weight(p, s, s.tiles, plan.keyed); });
-    }
-    int n = 0;
-    auto put = [&](int a, int b, int c, int d, int e, int f, int g, int h) {
-        const int32_t row[8] = {a, b, c, d, e, f, g, h};
-        if (n < most_rows)
-            for (int i = 0; i < 8; ++i) rows[8 * n + i] = row[i];
-        ++n;
-    };
-    for (int w = 0; w < plan.workers; ++w) {
-        bool first = true;
-        fa::paged_stretch(p, plan, w, [&](const fa::PagedWalk& k, int tiles, int lo, int hi, int part) {
-            put(w, k.b, k.hk, k.tile, lo, hi, tiles, part);
-            if (first && fa::paged_first_cut(plan, w, k)) {
-                int from;
-                const int pieces = fa::paged_pieces(p, plan, w, k, from);
-                for (int i = 0; pieces > 1 && i < pieces; ++i) put(-1, k.b, k.hk, k.tile, 0, 0, 0, 2 * (from + i) + (i == 0));
-            }
-            first = false;
-            return true;
-        });
-    }
-    return n;
+    return debug_pieces<false>(B, T, Hk, G, capacity, lens, starts, prefix, fa_window{}, nullptr, most_workers, rows, most_rows);
+}
+
+int fa_debug_paged_pieces_more(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t capacity, const int32_t* lens, const int32_t* starts, const int32_t* prefix,
+                               const fa_window* window, const int32_t* parents, int32_t most_workers, int32_t* rows, int32_t most_rows) {
+    return debug_pieces<true>(B, T, Hk, G, capacity, lens, starts, prefix, window ? *window : fa_window{}, parents, most_workers, rows, most_rows);
 }
 
 }  // extern "C"

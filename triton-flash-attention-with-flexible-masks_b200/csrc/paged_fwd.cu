@@ -22,6 +22,7 @@
 // the plan and the first item's place take 2.3, the last tile's drain 3, the second kernel up to 4 (the main loop streams at 7 TB/s); one token over 1.4 MB
 // 16 us, all of it latency: start, plan, a chain of tiles, epilogue, the second kernel's start. Chunks: the forward's chain of tiles, and twice as many loads. One chunk of 2000
 // tokens, 32 / 8 heads, pages of 128 | 16: 64 | 64 us; a chunk of 500 behind 7500 67 | 76 us, where dense keys take 55.
+#include <cstddef>
 #include <type_traits>
 #include "common.cuh"
 #include "paged_plan.cuh"
@@ -55,20 +56,31 @@ struct PagedSmem {
     static constexpr int off_misc = off_bar + n_bar * 8;  // tmem slot, abort flag
     static constexpr int total = off_misc + 16;
     static_assert(off_plan % 8 == 0 && off_bar % 8 == 0, "alignment");
+    // FORM_MASKED: bits [2 groups][kPagedTree / 32][128 rows] of the new tokens that a drafted one sees, in the place of the plan's sums, which nobody needs when the
+    // first item is there
+    static constexpr int off_masks = off_plan + int(offsetof(PagedPlan, sums)), kMaskWords = kPagedTree / 32;
+    static_assert(2 * kMaskWords * kBlk * 4 <= int(sizeof(PagedPlan::sums)), "room for the masks");
 };
 static_assert(PagedSmem<128>::total <= 232448 && PagedSmem<64>::total <= 232448, "shared memory budget");
 static_assert(PagedSmem<128>::total > 116736 && PagedSmem<64>::total > 116736, "shares an SM");
 
 // What an item's slot says: number of its key tiles, the first one, whether there is an item (1, or -1: no more), kv head, first row of its tokens in
 // q and out, how many of them, position of the first one, the sequence's length, its prefix, the sequence, slot of the workspace (-1: straight to out)
-enum : int { I_TILES = 0, I_LO, I_MORE, I_HEAD, I_ROW, I_TOKENS, I_POS, I_LEN, I_FRONT, I_SEQ, I_PART };
+// FORM_MASKED: key blocks from I_BORDER on lie I_SKIP further (I_TILES and I_LO count without those in between); place of a tree's first new token (else the
+// length); first row of the sequence
+enum : int { I_TILES = 0, I_LO, I_MORE, I_HEAD, I_ROW, I_TOKENS, I_POS, I_LEN, I_FRONT, I_SEQ, I_PART, I_BORDER, I_SKIP, I_BASE, I_FIRST };
 
-template <int D, bool BF16, int KIND>
+// Instances. FORM_MASKED: perhaps a window, perhaps drafted tokens whose parents are given. A tile of keys that the window hides from all of an item's tokens is not among its
+// tiles, and what lies in such keys of the others is as far from the results as what lies behind the sequence: V's rows are zeroed, scores masked. A drafted token's branch is
+// walked once an item, by the thread of each of its rows, while the first keys are on their way, and left as bits in shared memory.
+enum : int { FORM_PLAIN = 0, FORM_MASKED = 1 };
+
+template <int D, bool BF16, int KIND, int FORM>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmN, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const PagedParams p) {
     using S = PagedSmem<D>;
-    constexpr bool SCORED = score_changed(KIND);
+    constexpr bool SCORED = score_changed(KIND), MASKED = (FORM & FORM_MASKED) != 0;
     constexpr int NS = S::NS, NQ = S::NQ, NP = S::NP;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -130,9 +142,11 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (aborted) {
         if (tid == 0) p.merge[blockIdx.x] = make_int4(-1, 0, 0, 0);
     } else if (p.B > kPagedWarpPlan) {
-        paged_plan<kFwdThreads>(p, plan, int(gridDim.x));
+        paged_plan<kFwdThreads, MASKED>(p, plan, int(gridDim.x));
     }
     const int worker = int(blockIdx.x);
+    // the key block that is an item's x-th
+    auto key_block = [](int x, int border, int skip) { return MASKED && x >= border ? x + skip : x; };
 
     auto sQ = [&](int s) { return sbase + S::off_q + uint32_t(s) * S::TILE; };
     auto sK = [&](int s) { return sbase + S::off_k + uint32_t(s) * S::TILE; };
@@ -171,14 +185,15 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             bool ok = true, first = true;
             int k = 0, gk = 0;
             int4 merge = make_int4(0, 0, 0, 0);
-            if (p.B <= kPagedWarpPlan) paged_plan_warp(p, plan, int(gridDim.x));
+            if (p.B <= kPagedWarpPlan) paged_plan_warp<MASKED>(p, plan, int(gridDim.x));
             if (worker < plan.workers) {
-                paged_stretch(p, plan, worker, [&](const PagedWalk& walk, int, int lo, int hi, int part) {
+                paged_stretch<MASKED>(p, plan, worker, [&](const PagedWalk<MASKED>& walk, int, int lo, int hi, int part) {
                     const int s = k % NQ, use = k / NQ;
                     const int T = uniform(hi - lo), tile0 = uniform(lo), hk = uniform(walk.hk), len = uniform(walk.s.len), tok0 = uniform(walk.s.start + walk.tile * p.tokens);
                     const int tokens = uniform(min(p.tokens, walk.s.n - walk.tile * p.tokens));
                     const int32_t* const row_of_table = p.table + walk.b * p.table_stride;
-                    int pages = T > 0 ? pages_of(row_of_table, tile0, len) : 0;
+                    const int border = MASKED ? uniform(cdiv(walk.s.early, kBlk)) : 0, skip = MASKED ? uniform(paged_skip(p, walk.s, walk.tile)) : 0;
+                    int pages = T > 0 ? pages_of(row_of_table, key_block(tile0, border, skip), len) : 0;
                     if (use > 0) ok = mbar_wait_warp(BAR(B_ITEMEMPTY + s), (use - 1) & 1, ab, ST_WAIT_TIMEOUT + 11);
                     if (!ok) return false;
                     if (lane == 0) {
@@ -194,6 +209,12 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         it[I_FRONT] = walk.s.front;
                         it[I_SEQ] = walk.b;
                         it[I_PART] = part;
+                        if constexpr (MASKED) {
+                            it[I_BORDER] = border;
+                            it[I_SKIP] = skip;
+                            it[I_BASE] = walk.s.tree ? walk.s.base : len;
+                            it[I_FIRST] = walk.s.start;
+                        }
                         mbar_arrive(BAR(B_ITEMFULL + s));
                     }
                     __syncwarp();
@@ -208,10 +229,10 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
                     for (int t = 0; t < T; ++t, ++gk) {
                         const int st = gk % NS, ug = gk / NS, own = pages;
-                        if (t + 1 < T) pages = pages_of(row_of_table, tile0 + t + 1, len);
+                        if (t + 1 < T) pages = pages_of(row_of_table, key_block(tile0 + t + 1, border, skip), len);
                         if (ug > 0) ok = mbar_wait_warp(BAR(B_KEMPTY + st), (ug - 1) & 1, ab, ST_WAIT_TIMEOUT + 1);
                         if (!ok) return false;
-                        load(&tmK, sK(st), BAR(B_KFULL + st), own, tile0 + t, hk, len);
+                        load(&tmK, sK(st), BAR(B_KFULL + st), own, key_block(tile0 + t, border, skip), hk, len);
                     }
                     ++k;
                     if (first && paged_first_cut(plan, worker, walk)) {
@@ -245,14 +266,15 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 volatile int* it = info + 16 * s;
                 const int T = uniform(it[I_TILES]), lo = uniform(it[I_LO]), hk = uniform(it[I_HEAD]), len = uniform(it[I_LEN]), seq = uniform(it[I_SEQ]);
                 if (uniform(it[I_MORE]) < 0) break;
+                const int border = MASKED ? uniform(it[I_BORDER]) : 0, skip = MASKED ? uniform(it[I_SKIP]) : 0;
                 const int32_t* const row_of_table = p.table + seq * p.table_stride;
-                int pages = T > 0 ? pages_of(row_of_table, lo, len) : 0;
+                int pages = T > 0 ? pages_of(row_of_table, key_block(lo, border, skip), len) : 0;
                 for (int t = 0; t < T; ++t, ++gv) {
                     const int st = gv % NS, ug = gv / NS, own = pages;
-                    if (t + 1 < T) pages = pages_of(row_of_table, lo + t + 1, len);
+                    if (t + 1 < T) pages = pages_of(row_of_table, key_block(lo + t + 1, border, skip), len);
                     if (ug > 0) ok = mbar_wait_warp(BAR(B_VEMPTY + st), (ug - 1) & 1, ab, ST_WAIT_TIMEOUT + 2);
                     if (!ok) break;
-                    load(&tmV, sV(st), BAR(B_VFULL + st), own, lo + t, hk, len);
+                    load(&tmV, sV(st), BAR(B_VFULL + st), own, key_block(lo + t, border, skip), hk, len);
                 }
                 if (!ok) break;
                 __syncwarp();
@@ -359,9 +381,20 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             const bool valid = tok < tokens;
             {
                 const int64_t row_of_table = it[I_SEQ] * p.table_stride;
-                const int last = min((it[I_LO] + T) * kBlk, it[I_LEN]) - 1;
-                for (int i = (it[I_LO] * kBlk >> p.log2_page) + r; i <= last >> p.log2_page && T > 0; i += kBlk)
-                    if (uint32_t(p.table[row_of_table + i]) >= uint32_t(p.n_pages)) atomicCAS(p.status, 0, ST_PAGED_PAGE);
+                auto check_pages = [&](int from, int end) {  // of the keys in between
+                    for (int i = (from >> p.log2_page) + r; i <= (end - 1) >> p.log2_page && end > from; i += kBlk)
+                        if (uint32_t(p.table[row_of_table + i]) >= uint32_t(p.n_pages)) atomicCAS(p.status, 0, ST_PAGED_PAGE);
+                };
+                if constexpr (MASKED) {
+                    // (a window's server may have given the pages behind it away: nothing is asked of their entries)
+                    const int lo = it[I_LO], border = it[I_BORDER], skip = it[I_SKIP], len = it[I_LEN], tree = it[I_BASE] < len;
+                    const int early = p.window > 0 ? max(it[I_FRONT], p.sinks) : len, low = p.window > 0 ? (tree ? it[I_BASE] : it[I_POS]) - p.window + 1 : 0;
+                    const int from = key_block(lo, border, skip) * kBlk, end = T > 0 ? min((key_block(lo + T - 1, border, skip) + 1) * kBlk, len) : 0;
+                    check_pages(from, min(end, early));
+                    if (p.window > 0) check_pages(max(from, low), end);
+                } else {
+                    check_pages(it[I_LO] * kBlk, T > 0 ? min((it[I_LO] + T) * kBlk, it[I_LEN]) : 0);
+                }
             }
             // the only wait here that lasts as long as an item: it allows each of the tiles what another wait may last
             const Abort item{ab.flag, ab.status, ab.limit * (T + 1)};
@@ -481,8 +514,9 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const uint32_t tO = tmem + lane_base + uint32_t(S::tmem_o + w * D);
         const int tok_wide = r / p.G, tok_narrow = lane / p.G;
         bool alive = !aborted;
-        // Rows of V behind the keys that the item sees hold what was in the page, or in the stage: zeros, before P*V(g) is issued. A quarter of them a warp.
-        auto zero_behind = [&](int g, int real) {
+        // Rows of V behind the keys that the item sees hold what was in the page, or in the stage: zeros, before P*V(g) is issued. A quarter of them a warp. (MASKED: and the
+        // rows from `from` to `end`, between the early keys and the window.)
+        auto zero_behind = [&](int g, int real, int from, int end) {
             const int st = g % NS;
             if (!mbar_wait_warp(BAR(B_VFULL + st), (g / NS) & 1, ab, ST_WAIT_TIMEOUT + 19)) return false;
             // (not unrolled: it stands twice in the code of the softmax warps, a batch of chunks and tokens with a bias 224 us for 237)
@@ -490,6 +524,12 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             for (int x = 0; x < S::NBOX; ++x)
 #pragma unroll 1
                 for (int i = real * 8 + r; i < kBlk * 8; i += kBlk) reinterpret_cast<uint4*>(smem + S::off_v + st * S::TILE + x * S::BOX)[i] = make_uint4(0, 0, 0, 0);
+            if constexpr (MASKED) {
+#pragma unroll 1
+                for (int x = 0; x < S::NBOX; ++x)
+#pragma unroll 1
+                    for (int i = from * 8 + r; i < end * 8; i += kBlk) reinterpret_cast<uint4*>(smem + S::off_v + st * S::TILE + x * S::BOX)[i] = make_uint4(0, 0, 0, 0);
+            }
             fence_proxy_async();
             return true;
         };
@@ -521,8 +561,63 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             const bool active = __any_sync(0xffffffffu, valid);  // does this warp hold a query at all?
             const int pos = pos0 + tok;
             const int last = pos < 0 ? -1 : min(max(pos, front - 1), len - 1);  // the last key that this row sees (a token in front of the sequence sees no prefix, either)
-            const int all_see = pos0 < 0 ? -1 : min(max(pos0, front - 1), len - 1);  // and that all rows of the tile see
+            int all_see = pos0 < 0 ? -1 : min(max(pos0, front - 1), len - 1);  // and that all rows of the tile see
             const int seen = min(max(pos0 + tokens, front), len);              // keys that any row sees
+            // MASKED: keys below `low` are not in the row's window (below low_first in none's, low_last in some row's) and hidden but for the first `early`; of those
+            // from `base` on, a tree's, the row sees those that its mask says
+            const int border = MASKED ? it[I_BORDER] : 0, skip = MASKED ? it[I_SKIP] : 0, base = MASKED ? it[I_BASE] : 0;
+            int low = 0, low_first = 0, low_last = 0, early = 0;
+            bool tree = false;
+            uint32_t* const masks = reinterpret_cast<uint32_t*>(smem + S::off_masks) + w * (S::kMaskWords * kBlk) + r;
+            if constexpr (MASKED) {
+                tree = base < len;
+                int depth = 0;  // of the row's token in its tree, or its place behind the tile's first token
+                if (tree) {
+                    all_see = min(all_see, base - 1);
+#pragma unroll
+                    for (int i = 0; i < S::kMaskWords; ++i) masks[i * kBlk] = 0u;
+                    if (valid && pos >= 0) {
+                        const int32_t* const parents = p.parents + it[I_FIRST];
+                        const int own = it[I_ROW] - it[I_FIRST] + tok;
+                        auto parent = [&](int a) {  // one that does not lie before its token would be no tree's: the token continues the cached text
+                            const int x = parents[a];
+                            return x < a ? max(x, -1) : -1;
+                        };
+                        if (parents[own] < -1 || parents[own] >= own) atomicCAS(p.status, 0, ST_PAGED_PARENT);
+                        if (p.window > 0) {
+#pragma unroll 1
+                            for (int a = own; (a = parent(a)) >= 0;) ++depth;
+                        }
+                        int up = 0;  // steps above the token
+#pragma unroll 1
+                        for (int a = own; a >= 0; a = parent(a), ++up)
+                            if (p.window == 0 || up < p.window || base + depth - up < p.sinks) masks[(a >> 5) * kBlk] |= 1u << (a & 31);
+                    }
+                } else {
+                    depth = tok;
+                }
+                if (p.window > 0) {
+                    early = max(front, p.sinks);
+                    low_first = (tree ? base : pos0) - p.window + 1;
+                    low = low_first + depth;
+                    low_last = pos0 + tokens - p.window;
+                }
+            }
+            // Which of the 32 keys from x0 on the row sees.
+            auto sees = [&](int x0) {
+                uint32_t keep = first_bits(last - x0 + 1);
+                if constexpr (MASKED) {
+                    if (p.window > 0) keep &= ~hidden_bits(low - x0, early - x0);
+                    if (tree && x0 + 31 >= base) {
+                        const int i = x0 - base, word = i >> 5;  // (below 0 where the cached text ends among the 32)
+                        const uint32_t lo_bits = word >= 0 && word < S::kMaskWords ? masks[word * kBlk] : 0u;
+                        const uint32_t hi_bits = word + 1 >= 0 && word + 1 < S::kMaskWords ? masks[(word + 1) * kBlk] : 0u;
+                        const uint32_t text = first_bits(base - x0);
+                        keep = (keep & text) | (__funnelshift_r(lo_bits, hi_bits, i) & ~text);
+                    }
+                }
+                return keep;
+            };
             float slope = 0.f;
             if constexpr (SCORED) {
                 if (p.score.slopes) slope = p.score.slopes[int64_t(it[I_HEAD]) * p.G + g_row] * kScoreLog2e;
@@ -531,7 +626,12 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             float m_run = -INFINITY, l_run = 0.f;
 
             for (int t = t0; t < T && alive; t += 2) {
-                const int k0 = (lo + t) * kBlk;
+                const int k0 = key_block(lo + t, border, skip) * kBlk;
+                // MASKED: rows of the tile that no row of the item sees although they lie before its last key
+                const int none_from = MASKED ? max(early - k0, 0) : 0, none_end = MASKED ? min(low_first - k0, kBlk) : 0;
+                const bool none = MASKED && none_end > none_from;
+                // does some row not see all of the tile?
+                const bool masked = k0 + kBlk - 1 > all_see || (MASKED && p.window > 0 && k0 < low_last && k0 + kBlk > early);
                 const int g = G + t;
                 const uint32_t tS = tmem + lane_base + uint32_t(S::tmem_s(g)), tP = tmem + lane_base + uint32_t(S::tmem_p(g));
                 // P*V of the group's tile before: it has read its P and added to O
@@ -545,7 +645,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         alive = pv_before();
                         if (!alive) break;
                     }
-                    if (seen - k0 < kBlk) alive = zero_behind(g, seen - k0);
+                    if (seen - k0 < kBlk || none) alive = zero_behind(g, min(seen - k0, kBlk), none_from, none_end);
                     if (!alive) break;
                     mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
                     continue;
@@ -567,11 +667,15 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
                             for (int x = 0; x < 32; ++x) v[x] = x < seen - kq ? v[x] : 0.f;
                         }
+                        if (none) {
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) v[x] = x + 32 * quarter >= none_from && x + 32 * quarter < none_end ? 0.f : v[x];
+                        }
                         const Bias bias(slope, front == 0, pos0 - (kq + 31), pos0 + 31 - kq);
                         score_row<KIND, 32>(v, p.score, bias, p.scale_log2, pos - kq, valid, m_run == -INFINITY ? 0.f : m_run);
                     }
-                    if (kq + 31 > all_see) {
-                        const uint32_t keep = first_bits(last - kq + 1);
+                    if (MASKED ? masked : kq + 31 > all_see) {
+                        const uint32_t keep = sees(kq);
 #pragma unroll
                         for (int x = 0; x < 32; ++x) v[x] = (keep & (1u << x)) ? v[x] : -INFINITY;
                     }
@@ -621,7 +725,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         if (q != quarter) tmem_st16(tP + uint32_t(q) * 16u, zero);
                     tmem_st16(tP + uint32_t(quarter) * 16u, pk);
                     tc_wait_st();
-                    if (seen - k0 < kBlk) alive = zero_behind(g, seen - k0);
+                    if (seen - k0 < kBlk || none) alive = zero_behind(g, min(seen - k0, kBlk), none_from, none_end);
                     tc_fence_before();
                     mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
                     if (!alive) break;
@@ -647,14 +751,18 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
                         for (int x = 0; x < kBlk; ++x) sc[x] = x < real ? sc[x] : 0.f;
                     }
+                    if (none) {
+#pragma unroll
+                        for (int x = 0; x < kBlk; ++x) sc[x] = x >= none_from && x < none_end ? 0.f : sc[x];
+                    }
                     const Bias bias(slope, front == 0, pos0 - (k0 + kBlk - 1), pos0 + kBlk - 1 - k0);
-                    if constexpr (KIND == SCORE_CAPPED) late = k0 + kBlk - 1 <= all_see && !any_beyond<kBlk>(sc, valid ? p.score.most : INFINITY);
+                    if constexpr (KIND == SCORE_CAPPED) late = !masked && !any_beyond<kBlk>(sc, valid ? p.score.most : INFINITY);
                     if (!late) score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, pos - k0, valid, m_run == -INFINITY ? 0.f : m_run);
                 }
-                if (k0 + kBlk - 1 > all_see) {
+                if (masked) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const uint32_t keep = first_bits(last - k0 + 1 - 32 * q);
+                        const uint32_t keep = sees(k0 + 32 * q);
                         if (__any_sync(0xffffffffu, keep != ~0u)) {
 #pragma unroll
                             for (int x = 0; x < 32; ++x) sc[32 * q + x] = (keep & (1u << x)) ? sc[32 * q + x] : -INFINITY;
@@ -728,7 +836,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 else if (KIND == SCORE_CAPPED && late) exponentials([&](uint64_t s2) { return fma_f2(s2, cap_poly(s2, p.score), mneg2); });
                 else exponentials([&](uint64_t s2) { return s2; });
                 tc_wait_st();
-                if (real < kBlk) alive = zero_behind(g, real);
+                if (real < kBlk || none) alive = zero_behind(g, min(real, kBlk), none_from, none_end);
                 tc_fence_before();
                 mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
                 if (!alive) break;
@@ -889,9 +997,9 @@ __global__ void __launch_bounds__(kCombineThreads, 2) paged_combine_kernel(const
 }
 
 // ---- host launchers (called from paged.cu) ----------------------------------------------
-template <int D, bool BF16, int KIND>
+template <int D, bool BF16, int KIND, int FORM>
 static cudaError_t launch_paged_t(const CUtensorMap& tq, const CUtensorMap& tn, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {
-    auto kern = paged_fwd_kernel<D, BF16, KIND>;
+    auto kern = paged_fwd_kernel<D, BF16, KIND, FORM>;
     constexpr int smem = PagedSmem<D>::total;
     static SmemAllowed allowed;
     cudaError_t e = allow_smem(kern, smem, allowed);
@@ -904,7 +1012,11 @@ static cudaError_t launch_paged_t(const CUtensorMap& tq, const CUtensorMap& tn, 
 cudaError_t launch_paged_fwd(bool bf16, const CUtensorMap& tq, const CUtensorMap& tn, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {
     auto pick = [&](auto d, auto kind) {
         constexpr int kD = decltype(d)::value, kKind = decltype(kind)::value;
-        return bf16 ? launch_paged_t<kD, true, kKind>(tq, tn, tk, tv, p, workers, stream) : launch_paged_t<kD, false, kKind>(tq, tn, tk, tv, p, workers, stream);
+        if (p.window > 0 || p.parents)
+            return bf16 ? launch_paged_t<kD, true, kKind, FORM_MASKED>(tq, tn, tk, tv, p, workers, stream)
+                        : launch_paged_t<kD, false, kKind, FORM_MASKED>(tq, tn, tk, tv, p, workers, stream);
+        return bf16 ? launch_paged_t<kD, true, kKind, FORM_PLAIN>(tq, tn, tk, tv, p, workers, stream)
+                    : launch_paged_t<kD, false, kKind, FORM_PLAIN>(tq, tn, tk, tv, p, workers, stream);
     };
     using std::integral_constant;
     auto of = [&](auto d) {

@@ -2,7 +2,7 @@
 // know them, and a captured call has to follow them).
 //
 // An item is a tile of queries (tokens_per_tile new tokens of a sequence, all heads of a kv head's group) of one kv head. Its weight is the
-// number of keys that its last token sees, and a constant for what an item costs besides its tiles. The items, in the order sequence, kv head,
+// number of keys that its last token sees (with a window, less those that lie between the first keys and it), and a constant for what an item costs besides its tiles. The items, in the order sequence, kv head,
 // tile, lie behind one another on a line of length `total`, and each of n workers gets an equal stretch of it, whatever the lengths, with at most
 // n - 1 cuts. An item that a cut goes through is computed in pieces, whose fp32 rows the second kernel merges.
 // Where there are no more items than workers and whole items, one a worker, are done as soon, nothing is cut (`keyed` false: all weights are 1):
@@ -14,6 +14,8 @@
 
 namespace fa {
 
+// New tokens of a sequence up to which its parents are looked at; more are a chunk, each behind the one before it.
+constexpr int kPagedTree = 256;
 constexpr int kPagedGroups = 1024;   // entries of the table of sums: a sequence each, or several
 // Sequences up to which one warp makes the plan, beside which the others go on. One warp | all, us: single tokens of 1 sequence 15.9 | 16.6, of 128 101.0 | 102.0,
 // of 256 179.6 | 179.9, of 512 322 | 318.
@@ -50,8 +52,12 @@ struct PagedSeq {
     int base;      // position of the first new one (below 0: those see nothing)
     int front;     // leading keys that all see
     int tiles;     // of queries
+    // MASKED (a call with a window or with parents, or of an 8-bit cache)
+    int early;     // leading keys that the window hides from none
+    int tree;      // the tokens' parents count
 };
 
+template <bool MASKED>
 __host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int b) {
     PagedSeq s;
     int end;
@@ -67,17 +73,43 @@ __host__ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int
     s.base = s.len - s.n;
     s.front = p.prefix ? paged_clamp(p.prefix[b], 0, s.len) : 0;
     s.tiles = cdiv(s.n, p.tokens);
+    if constexpr (MASKED) {
+        s.early = s.front > p.sinks ? s.front : p.sinks;
+        s.tree = p.parents && s.n <= kPagedTree;
+    }
     return s;
 }
 
-// Keys that tile i's last token sees.
-__host__ __device__ __forceinline__ int paged_keys(const PagedParams& p, const PagedSeq& s, int i) {
+// The end of the keys that tile i's last token sees.
+__host__ __device__ __forceinline__ int paged_seen(const PagedParams& p, const PagedSeq& s, int i) {
     const long long end = s.base + (long long)(i + 1) * p.tokens;
     const int seen = end < s.len ? int(end) : s.len;
     return seen > s.front ? seen : s.front;
 }
+// With a window: the first key that is in the window of a token of tile i (a tree's tokens may all continue the cached text).
+__host__ __device__ __forceinline__ int paged_low(const PagedParams& p, const PagedSeq& s, int i) {
+    const long long low = s.base + (s.tree ? 0 : (long long)i * p.tokens) - p.window + 1;
+    return low > 0 ? int(low) : 0;
+}
+// Key blocks that lie between tile i's early keys and its window.
+__host__ __device__ __forceinline__ int paged_skip(const PagedParams& p, const PagedSeq& s, int i) {
+    if (p.window == 0) return 0;
+    const int skip = paged_low(p, s, i) / kBlk - cdiv(s.early, kBlk);
+    return skip > 0 ? skip : 0;
+}
+// What tile i counts for: the keys that its last token sees, less those between the early ones and the window (so no more than its blocks hold).
+template <bool MASKED>
+__host__ __device__ __forceinline__ int paged_keys(const PagedParams& p, const PagedSeq& s, int i) {
+    int keys = paged_seen(p, s, i);
+    if constexpr (MASKED) {
+        const int hidden = p.window > 0 ? paged_low(p, s, i) - s.early : 0;
+        if (hidden > 0) keys -= hidden;
+    }
+    return keys;
+}
 
 // The weights of the first m tiles of one head together.
+template <bool MASKED>
 __host__ __device__ __forceinline__ long long paged_weight(const PagedParams& p, const PagedSeq& s, int m, bool keyed) {
     if (!keyed) return m;
     // the tiles but the last end at base + (i + 1) tokens < len; those below `front` see that many keys
@@ -88,6 +120,17 @@ __host__ __device__ __forceinline__ long long paged_weight(const PagedParams& p,
         const long long fewer = ahead > 0 ? (ahead + p.tokens - 1) / p.tokens - 1 : 0, below = fewer < inner ? fewer : inner;
         const long long rest = inner - below;
         sum += below * s.front + rest * s.base + (long long)p.tokens * (rest * (below + 1) + rest * (rest - 1) / 2);
+    }
+    if constexpr (MASKED) {
+        if (p.window > 0) {  // the hidden keys of tile i: first + i tokens of them where that is above 0; of a tree's tiles all the same
+            const long long first = (long long)s.base - p.window + 1 - s.early;
+            if (s.tree) {
+                if (first > 0) sum -= m * first;
+            } else {
+                const long long none = first >= 0 ? 0 : (-first + p.tokens - 1) / p.tokens, some = m > none ? m - none : 0;
+                sum -= some * first + (long long)p.tokens * (some * none + some * (some - 1) / 2);
+            }
+        }
     }
     return m == s.tiles && m > 0 ? sum + s.len : sum;
 }
@@ -110,6 +153,7 @@ __host__ __device__ __forceinline__ void paged_share_out(PagedPlan& plan, long l
 
 // The plan of up to kPagedWarpPlan sequences, by one warp, the one that needs it: 32 entries of `sums`. (By all warps it costs a microsecond more, of which with
 // many sequences nothing is left.)
+template <bool MASKED>
 __device__ __forceinline__ void paged_plan_warp(const PagedParams& p, PagedPlan& plan, int most_workers) {
     const int lane = threadIdx.x & 31, group = paged_group(p.B);
     long long w = 0, n = 0;
@@ -117,11 +161,11 @@ __device__ __forceinline__ void paged_plan_warp(const PagedParams& p, PagedPlan&
 #pragma unroll 1
     for (int b = lane * group; b < min(p.B, (lane + 1) * group); ++b) {
         const int len = p.lens[b];
-        const PagedSeq s = paged_seq(p, b);
+        const PagedSeq s = paged_seq<MASKED>(p, b);
         if (len > p.capacity || len < 0) atomicCAS(p.status, 0, ST_PAGED_LENGTH);
-        w += p.Hk * paged_weight(p, s, s.tiles, true);
+        w += p.Hk * paged_weight<MASKED>(p, s, s.tiles, true);
         n += (long long)p.Hk * s.tiles;
-        longest = max(longest, s.tiles > 0 ? s.len : 0);
+        longest = max(longest, s.tiles > 0 ? MASKED ? paged_keys<MASKED>(p, s, s.tiles - 1) : s.len : 0);
     }
     __syncwarp();
     longest = __reduce_max_sync(0xffffffffu, longest);
@@ -148,7 +192,7 @@ __device__ __forceinline__ void paged_plan_warp(const PagedParams& p, PagedPlan&
 }
 
 // All threads of the block (a multiple of 32, at most 1024, that divides 2 * kPagedGroups). Ends with a barrier.
-template <int kThreads>
+template <int kThreads, bool MASKED>
 __device__ __forceinline__ void paged_plan(const PagedParams& p, PagedPlan& plan, int most_workers) {
     constexpr int kOwn = kPagedGroups / kThreads, kWarps = kThreads / 32;
     static_assert(kOwn * kThreads == kPagedGroups && kOwn >= 1, "groups of a thread");
@@ -160,11 +204,11 @@ __device__ __forceinline__ void paged_plan(const PagedParams& p, PagedPlan& plan
     for (int o = 0; o < kOwn; ++o) {
         weight[o] = items[o] = 0;
         for (int b = (first + o) * group; b < min(p.B, (first + o + 1) * group); ++b) {
-            const PagedSeq s = paged_seq(p, b);
+            const PagedSeq s = paged_seq<MASKED>(p, b);
             if (p.lens[b] > p.capacity || p.lens[b] < 0) atomicCAS(p.status, 0, ST_PAGED_LENGTH);
-            weight[o] += p.Hk * paged_weight(p, s, s.tiles, true);
+            weight[o] += p.Hk * paged_weight<MASKED>(p, s, s.tiles, true);
             items[o] += (long long)p.Hk * s.tiles;
-            if (s.tiles > 0) longest = max(longest, s.len);
+            if (s.tiles > 0) longest = max(longest, MASKED ? paged_keys<MASKED>(p, s, s.tiles - 1) : s.len);
         }
         w += weight[o];
         n += items[o];
@@ -227,6 +271,7 @@ __host__ __device__ __forceinline__ long long paged_cut(const PagedPlan& plan, i
 }
 
 // A walk over the items from a point of the line on.
+template <bool MASKED>
 struct PagedWalk {
     PagedSeq s;
     int b, hk, tile;
@@ -252,8 +297,8 @@ struct PagedWalk {
                 at = x;
                 return;
             }
-            s = paged_seq(p, b);
-            head = paged_weight(p, s, s.tiles, plan.keyed);
+            s = paged_seq<MASKED>(p, b);
+            head = paged_weight<MASKED>(p, s, s.tiles, plan.keyed);
             if (rem < head * p.Hk) break;
             rem -= head * p.Hk;
         }
@@ -262,13 +307,13 @@ struct PagedWalk {
         int t0 = 0, t1 = s.tiles;  // weight(t0) <= rem < weight(t1)
         while (t1 - t0 > 1) {
             const int mid = (t0 + t1) >> 1;
-            if (paged_weight(p, s, mid, plan.keyed) <= rem) t0 = mid; else t1 = mid;
+            if (paged_weight<MASKED>(p, s, mid, plan.keyed) <= rem) t0 = mid; else t1 = mid;
         }
         tile = t0;
-        at = x - rem + paged_weight(p, s, t0, plan.keyed);
+        at = x - rem + paged_weight<MASKED>(p, s, t0, plan.keyed);
     }
     __host__ __device__ __forceinline__ long long end(const PagedParams& p, const PagedPlan& plan) const {
-        return at + (plan.keyed ? paged_keys(p, s, tile) + kPagedItemCost : 1);
+        return at + (plan.keyed ? paged_keys<MASKED>(p, s, tile) + kPagedItemCost : 1);
     }
     // The next item; there is one.
     __host__ __device__ __forceinline__ void next(const PagedParams& p, const PagedPlan& plan) {
@@ -277,9 +322,9 @@ struct PagedWalk {
         tile = 0;
         if (++hk < p.Hk) return;
         hk = 0;
-        do s = ++b < p.B ? paged_seq(p, b) : PagedSeq{}; while (s.tiles == 0 && b < p.B);
+        do s = ++b < p.B ? paged_seq<MASKED>(p, b) : PagedSeq{}; while (s.tiles == 0 && b < p.B);
     }
-    __host__ __device__ __forceinline__ int key_tiles(const PagedParams& p) const { return cdiv(paged_keys(p, s, tile), kBlk); }
+    __host__ __device__ __forceinline__ int key_tiles(const PagedParams& p) const { return cdiv(paged_seen(p, s, tile), kBlk) - (MASKED ? paged_skip(p, s, tile) : 0); }
     // The item's key tile at point x of the line: the pieces on both sides of a cut at x meet there.
     __host__ __device__ __forceinline__ int key_tile_at(const PagedParams& p, const PagedPlan& plan, long long x) const {
         const int n = key_tiles(p);
@@ -294,9 +339,9 @@ struct PagedWalk {
 // The pieces of worker w's stretch, in their order: emit(walk, key tiles of the item, first and last + 1 of the piece, slot of the workspace or -1 for a
 // piece that is the whole item) until one says false. A piece without tiles is left out, but for the one that begins an item without any,
 // whose rows are zeros.
-template <class Emit>
+template <bool MASKED, class Emit>
 __host__ __device__ __forceinline__ void paged_stretch(const PagedParams& p, const PagedPlan& plan, int w, Emit emit) {
-    PagedWalk walk;
+    PagedWalk<MASKED> walk;
     const long long x0 = paged_cut(plan, w), x1 = paged_cut(plan, w + 1);
     if (x0 >= x1) return;
     walk.find(p, plan, x0);
@@ -310,14 +355,16 @@ __host__ __device__ __forceinline__ void paged_stretch(const PagedParams& p, con
 }
 
 // Is the cut before worker w the first one through the item at `walk`, which it falls into?
-__host__ __device__ __forceinline__ bool paged_first_cut(const PagedPlan& plan, int w, const PagedWalk& walk) {
+template <bool MASKED>
+__host__ __device__ __forceinline__ bool paged_first_cut(const PagedPlan& plan, int w, const PagedWalk<MASKED>& walk) {
     return w > 0 && walk.s.tiles > 0 && walk.at < paged_cut(plan, w) && (w == 1 || walk.at >= paged_cut(plan, w - 1));
 }
 
 // How many pieces the item at `walk` has, which the cut before worker w goes through first: one each of the workers from `from` on. (Where that cut falls into the item's fixed
 // cost or into its first tile, the worker in front of it has none: a cut inside a tile gives the tile to the worker behind the cut, who thus has the last one at least; and a stretch
 // that lies within the item has tiles, for it is longer than the cost and a tile.) The first piece's slot is 2 * from + 1, the others' are 2 * (from + i).
-__host__ __device__ __forceinline__ int paged_pieces(const PagedParams& p, const PagedPlan& plan, int w, const PagedWalk& walk, int& from) {
+template <bool MASKED>
+__host__ __device__ __forceinline__ int paged_pieces(const PagedParams& p, const PagedPlan& plan, int w, const PagedWalk<MASKED>& walk, int& from) {
     static_assert((1 << kPagedLog2Piece) > kPagedItemCost + 2 * kBlk, "every stretch within an item has tiles");
     from = walk.key_tile_at(p, plan, paged_cut(plan, w)) > 0 ? w - 1 : w;
     // the last worker: the cuts lie a stretch apart, and its own is the last one before the item's end

@@ -119,6 +119,12 @@ struct PagedParams {
     int* status;
     long long wait_limit;
     ScoreArgs score;
+    // The instances of other forms (paged_fwd.cu)
+    int window, sinks;       // 0: no window
+    const int32_t* parents;  // [T] each new token's place among the sequence's new ones that it continues, -1: the cached text; null: each the one before it
+    const uint8_t* k_scales; // [pages, Hk, page size] exponents of an 8-bit cache's rows, biased by 127; null: a 16-bit cache
+    const uint8_t* v_scales;
+    int64_t k_scale_p, k_scale_h, v_scale_p, v_scale_h;  // strides in bytes
 };
 
 // A number for the current CUDA context that no other context of the process ever has, or 0 (api.cu).

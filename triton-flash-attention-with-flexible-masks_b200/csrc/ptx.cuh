@@ -19,6 +19,7 @@ enum : int {
     ST_ID_RANGE = 200,         // a negative query id does not fit in int32
     ST_PAGED_PAGE = 201,       // a page number of a paged cache is not one
     ST_PAGED_LENGTH = 202,     // a sequence's length is negative or beyond its row of the page table
+    ST_PAGED_PARENT = 203,     // a drafted token's parent does not lie before it
 };
 // A time-out leaves the device in an unknown state: every later launch refuses to compute until the
 // host has read and cleared the word. An id out of range only concerns the call that passed it.

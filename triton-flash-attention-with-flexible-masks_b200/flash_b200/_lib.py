@@ -19,7 +19,7 @@ EXPORTS = (
     "fa_debug_wait_timeout", "fa_group_rows", "fa_permute_rows", "fa_fwd_splits", "fa_fwd_workspace_bytes", "fa_fwd_split",
     "fa_plan_optional", "fa_bwd", "fa_plan_build_scored", "fa_fwd_scored", "fa_fwd_rest", "fa_bwd_scored", "fa_paged_append",
     "fa_paged_workspace_bytes", "fa_paged_fwd", "fa_debug_paged_pieces",
-    "fa_plan_build_windowed", "fa_fwd_splits_windowed", "fa_fwd_windowed", "fa_bwd_windowed",
+    "fa_plan_build_windowed", "fa_fwd_splits_windowed", "fa_fwd_windowed", "fa_bwd_windowed", "fa_paged_fwd_more", "fa_debug_paged_pieces_more",
 )
 
 
@@ -52,6 +52,10 @@ class PagedCache(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("B", "Hk", "D", "dtype", "pages", "page_size", "table_pages")] + [
         ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("lens", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
         ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3)]
+
+
+class PagedMore(ctypes.Structure):
+    _fields_ = [("window", Window), ("parents", ctypes.c_void_p)]
 
 
 class Rows(ctypes.Structure):
@@ -125,6 +129,10 @@ def load():
     lib.fa_paged_workspace_bytes.argtypes = [C, ctypes.POINTER(size)]
     lib.fa_paged_fwd.restype = i32
     lib.fa_paged_fwd.argtypes = [C, ctypes.c_int32, ctypes.c_int32, vp, ctypes.c_float, S, R, R, ctypes.c_int32, vp, size, vp, vp]
+    lib.fa_paged_fwd_more.restype = i32
+    lib.fa_paged_fwd_more.argtypes = [C, ctypes.POINTER(PagedMore), *lib.fa_paged_fwd.argtypes[1:]]
+    lib.fa_debug_paged_pieces_more.restype = i32
+    lib.fa_debug_paged_pieces_more.argtypes = [ctypes.c_int32] * 5 + [vp] * 3 + [W, vp, ctypes.c_int32, vp, ctypes.c_int32]
     lib.fa_debug_paged_pieces.restype = i32
     lib.fa_debug_paged_pieces.argtypes = [ctypes.c_int32] * 5 + [vp] * 3 + [ctypes.c_int32, vp, ctypes.c_int32]
     lib.fa_debug_mask.restype = i32

@@ -114,6 +114,8 @@ def check_status(device=None):
                 raise RuntimeError("flash_b200: a page table names a page that the cache does not have")
             if code == 202:
                 raise RuntimeError("flash_b200: a length of a paged cache is negative or beyond its row of the page table")
+            if code == 203:
+                raise RuntimeError("flash_b200: a drafted token's parent does not lie before it among its sequence's new tokens")
             raise RuntimeError(f"flash_b200: kernel status {code}")
 
 

@@ -6,7 +6,7 @@ import torch
 
 from . import _lib, ops
 from .ops import _count, _current, _same_device, _status_word, _stream, check_status
-from .scored import _checked_softcap, _checked_slopes, _native, _scores
+from .scored import _checked_softcap, _checked_slopes, _checked_window, _native, _pointer, _scores
 
 _TYPES = {torch.bfloat16: _lib.FA_BF16, torch.float16: _lib.FA_FP16}
 _workspace_bytes = {}  # (device, head dim) -> bytes
@@ -122,24 +122,33 @@ def _overlap(a, b):
     return ends[0][0] < ends[1][1] and ends[1][0] < ends[0][1]
 
 
-def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_scale=None, softcap=None, slopes=None, prefix=None, out=None):
+def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_scale=None, softcap=None, slopes=None, prefix=None, out=None, window=None, sinks=0, parents=None):
     """Attention of new tokens over a cache of pages that holds their keys and values already (`paged_append`): chunks of prompts and single
     tokens in one ragged batch.
 
     q: [T, H, D], bf16 or fp16, H a multiple of the cache's Hk and at most 128 times that; the rest as in `paged_append`. The new token at position p of its sequence sees the
     tokens 0 to p. sm_scale: 1 / sqrt(D) if None. softcap, slopes, prefix: as in `attention_scored`, the token's position in the place of
-    i + gap; prefix is int32 [B]. A row that sees no token (a length of 0, a position below 0) gives zeros. No derivative, as in `paged_append`.
+    i + gap; prefix is int32 [B]. window, sinks: as in `attention_scored`; entries of page_table whose pages no token of the call sees may then hold anything.
+
+    parents: int32 [T]; sequences of up to 256 new tokens then have them drafted as a tree. parents[t] is the place, among its sequence's new tokens, of the one that
+    token t continues, which lies before it, or -1: t continues the cached text. t sees the text in front of the new tokens, itself and the tokens on its
+    branch; its position, by which a window goes, is the text's length plus its depth on the branch (0 where it continues the text), theirs likewise. Sequences of more new tokens
+    are chunks, whose parents are not read. A parent that does not lie before its token counts as -1 and is reported by `check_status`. Not together with slopes or a prefix.
+
+    A row that sees no token (a length of 0, a position below 0) gives zeros. No derivative, as in `paged_append`.
 
     Returns [T, H, D], zeros in the rows of no sequence; or `out`, whose rows of no sequence are left as they were. `out` shares no memory with q
     or the cache. What lies in the pages behind a sequence's length, or in pages that no sequence names, has no influence, also
     if it is not finite; a value that some row of a block sees (a block is the heads of a group and up to 128 / G neighbouring tokens of a sequence) may spread in it if it is
-    not finite. How the work is cut goes by all lengths of the batch, so that the last bits of a sequence's rows can differ with what
+    not finite (a drafted token's in those that are drafted behind it, too). How the work is cut goes by all lengths of the batch, so that the last bits of a sequence's rows can differ with what
     it is batched with."""
-    softcap = _checked_softcap(softcap)
+    softcap, window = _checked_softcap(softcap), _checked_window(window, sinks)
+    if parents is not None and (slopes is not None or prefix is not None):
+        raise ValueError("flash_b200: drafted tokens have no bias by distance and no prefix: parents go without slopes and prefix")
     if sm_scale is None or type(sm_scale) is float:
-        native = _native(q, k_pages, v_pages, page_table, kv_lens, q_starts, slopes, prefix, out)
+        native = _native(q, k_pages, v_pages, page_table, kv_lens, q_starts, slopes, prefix, out, parents)
         if native is not None:
-            done = native[0].paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts, sm_scale, softcap, slopes, prefix, out, native[1])
+            done = native[0].paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts, sm_scale, softcap, slopes, prefix, out, *window, parents, native[1])
             if done is not None:
                 return done if out is None else out
     _no_tangents(q, k_pages, v_pages, slopes, out)
@@ -154,6 +163,8 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_
     slopes = _checked_slopes(slopes, H, q)
     if prefix is not None:
         prefix = _int32(prefix, (cache.B,), "prefix", q)
+    if parents is not None:
+        parents = _int32(parents, (T,), "parents", q)
     fill = out is None
     if fill:
         out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
@@ -177,8 +188,8 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_
             size = _workspace_bytes[device.index, D] = size.value
         work = torch.empty(size // 4, dtype=torch.float32, device=device)
         with ops._timed("paged", 2):
-            _lib.check(lib.fa_paged_fwd(cache, T, H, starts, sm_scale, _scores(softcap, slopes, prefix), _rows(q), _rows(out), fill, work.data_ptr(), size,
-                                        _status_word(device).data_ptr(), _stream()), "fa_paged_fwd")
+            _lib.check(lib.fa_paged_fwd_more(cache, _lib.PagedMore(_lib.Window(*window), _pointer(parents)), T, H, starts, sm_scale, _scores(softcap, slopes, prefix),
+                                             _rows(q), _rows(out), fill, work.data_ptr(), size, _status_word(device).data_ptr(), _stream()), "fa_paged_fwd_more")
     if not fill:
         _bump(out)
     if ops._SYNC_STATUS:
