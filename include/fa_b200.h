@@ -257,11 +257,21 @@ int fa_paged_fwd(const fa_paged_cache* cache, int32_t T, int32_t H, const int32_
  * parents [T], device: sequences of up to 256 new tokens have them drafted as a tree. parents[t] is the place, among its sequence's new tokens, of the one that token t
  *   continues, which lies before it, or -1: it continues the cached text. A token then sees the cached text, itself and those on its branch; its position is
  *   that of the text's end and its depth on the branch. Sequences of more new tokens are chunks, whose parents are not read. A parent that does not lie before its
- *   token sets status 203 and counts as -1. Not with slopes or a prefix (FA_ERR_SCORES). */
+ *   token sets status 203 and counts as -1. Not with slopes or a prefix (FA_ERR_SCORES).
+ * k_scales, v_scales [pages, Hk, page_size], device: the cache's k and v are e4m3, a byte each, with strides that are multiples of 16 and a page size of 16 at least; a head's row of a token stands for
+ *   its numbers times 2^(byte - 127), bytes from 112 to 134 (others are taken into that range by the attention). Rows and q are of cache->dtype, which the
+ *   cache itself does not depend on. An append stores, of a row x, the nearest of e4m3's numbers to x 2^-e (ties to even, 448 at most) with the least e from -15 to 7
+ *   for which the largest finite |x| is at most 448 2^e, and a NaN for what is not finite. Where two tokens go to one place their parts may mix.
+ *   Scales: 16-byte aligned, last stride 1, other strides multiples of 16. An append takes nothing else from this struct. */
 typedef struct fa_paged_more {
     fa_window window;
     const int32_t* parents;
+    uint8_t* k_scales; /* an 8-bit cache's (below), or both NULL */
+    uint8_t* v_scales;
+    int64_t k_scale_stride[2], v_scale_stride[2]; /* bytes: page, head */
 } fa_paged_more;
+int fa_paged_append_more(const fa_paged_cache* cache, const fa_paged_more* more, int32_t T, const int32_t* starts, const fa_rows* k, const fa_rows* v, int32_t* status,
+                         void* stream);
 int fa_paged_fwd_more(const fa_paged_cache* cache, const fa_paged_more* more, int32_t T, int32_t H, const int32_t* starts, float sm_scale,
                       const fa_scores* scores, const fa_rows* q, const fa_rows* o, int32_t fill, void* workspace, size_t bytes, int32_t* status, void* stream);
 

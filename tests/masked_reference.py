@@ -12,8 +12,9 @@ def windowed(M, N, window, sinks, prefix=None, device="cuda"):
     return keep if prefix is None else keep | (j < prefix.long()[:, None, None, None])
 
 
-def attention_64(q, k, v, do, keep, sm_scale=None, cap=None, slopes=None):
-    """{"o", "dq", "dk", "dv"}: (value, bound) of each; the gradients where there is a `do`."""
+def attention_64(q, k, v, do, keep, sm_scale=None, cap=None, slopes=None, sub=None):
+    """{"o", "dq", "dk", "dv"}: (value, bound) of each; the gradients where there is a `do`. `sub`: what an entry of P may lack absolutely, of a row whose sum is at
+    least 1, where that is not the type's (below)."""
     B, H, M, D = q.shape
     Hk, N = k.shape[1:3]
     G, gap, dev, dtype = H // Hk, max(0, N - M), q.device, q.dtype
@@ -44,7 +45,8 @@ def attention_64(q, k, v, do, keep, sm_scale=None, cap=None, slopes=None):
     up = u if half else 0.0
     # An entry below the type's least normal number is off by up to half the step there; and the 16-bit kernels' exponentials are 0 below fp32's least normal number,
     # 2^-126, which is bf16's as well: an entry of bf16 may lack that much, 2^8 half steps. (A key at a distance of 450 with a slope of 0.2 has exp(-90) = 2^-130.)
-    sub = max(torch.finfo(dtype).smallest_normal * u, 2.0 ** -126) if half else 0.0
+    if sub is None:
+        sub = max(torch.finfo(dtype).smallest_normal * u, 2.0 ** -126) if half else 0.0
     seen = keep.double()
     tiny = torch.finfo(dtype).tiny if dtype != torch.float16 else 2.0 ** -24
     o = p @ V

@@ -408,20 +408,23 @@ py::object attend_scored(const Tensor& q, const Tensor& k, const Tensor& v, bool
 }
 
 // ---- paged cache (paged.py). A call that is not a regular one on the current device is declined, and paged.py copies, raises or does nothing.
-bool rows_as_is(const Tensor& t, int dim) {
+bool rows_as_is(const Tensor& t, int dim, int multiple = 8) {
     if (!t.is_cuda() || t.layout() != at::kStrided || t.dim() != dim || t.is_neg() || t.stride(dim - 1) != 1 || t.numel() == 0 ||
         reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 != 0)
         return false;
     for (int i = 0; i < dim - 1; ++i)
-        if (t.size(i) > 1 && (t.stride(i) <= 0 || t.stride(i) % 8 != 0)) return false;
+        if (t.size(i) > 1 && (t.stride(i) <= 0 || t.stride(i) % multiple != 0)) return false;
     return !(at::GradMode::is_enabled() && t.requires_grad());
 }
 
 bool cache_of(const Tensor& rows, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens, const std::optional<Tensor>& starts,
-              fa_paged_cache& c) {
-    if (!rows_as_is(rows, 3) || !rows_as_is(k_pages, 4) || !rows_as_is(v_pages, 4) || rows.get_device() != c10::cuda::current_device()) return false;
+              const std::optional<Tensor>& k_scales, const std::optional<Tensor>& v_scales, fa_paged_cache& c, fa_paged_more& more) {
+    if (k_scales.has_value() != v_scales.has_value()) return false;
+    const int multiple = k_scales ? 16 : 8;
+    if (!rows_as_is(rows, 3) || !rows_as_is(k_pages, 4, multiple) || !rows_as_is(v_pages, 4, multiple) || rows.get_device() != c10::cuda::current_device()) return false;
     const int dt = dtype_of(rows);
-    if ((dt != FA_BF16 && dt != FA_FP16) || k_pages.scalar_type() != rows.scalar_type() || v_pages.scalar_type() != rows.scalar_type()) return false;
+    const auto cached = k_scales ? at::kFloat8_e4m3fn : rows.scalar_type();
+    if ((dt != FA_BF16 && dt != FA_FP16) || k_pages.scalar_type() != cached || v_pages.scalar_type() != cached) return false;
     auto ints = [&](const Tensor& t, int dim) {
         return t.is_cuda() && t.layout() == at::kStrided && t.scalar_type() == at::kInt && t.dim() == dim && t.device() == rows.device() && !t.is_neg();
     };
@@ -436,6 +439,19 @@ bool cache_of(const Tensor& rows, const Tensor& k_pages, const Tensor& v_pages, 
     c = fa_paged_cache{int(B), int(k_pages.size(2)), int(D), dt, int(k_pages.size(0)), int(page), int(table.size(1)), table.const_data_ptr<int>(), table.stride(0),
                        lens.const_data_ptr<int>(), k_pages.data_ptr(), v_pages.data_ptr(), {k_pages.stride(0), k_pages.stride(1), k_pages.stride(2)},
                        {v_pages.stride(0), v_pages.stride(1), v_pages.stride(2)}};
+    if (k_scales) {
+        for (const Tensor* t : {&*k_scales, &*v_scales})
+            if (!rows_as_is(*t, 3, 16) || t->scalar_type() != at::kFloat8_e8m0fnu || t->device() != rows.device() || t->size(0) != k_pages.size(0) ||
+                t->size(1) != k_pages.size(2) || t->size(2) != page)
+                return false;
+        if (page < 16) return false;
+        more.k_scales = static_cast<uint8_t*>(k_scales->data_ptr());
+        more.v_scales = static_cast<uint8_t*>(v_scales->data_ptr());
+        for (int i = 0; i < 2; ++i) {
+            more.k_scale_stride[i] = k_scales->stride(i);
+            more.v_scale_stride[i] = v_scales->stride(i);
+        }
+    }
     return true;
 }
 
@@ -452,39 +468,46 @@ void bump(const Tensor& t) {
 }
 
 bool paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens,
-                  const std::optional<Tensor>& starts, const Tensor& status) {
+                  const std::optional<Tensor>& starts, const std::optional<Tensor>& k_scales, const std::optional<Tensor>& v_scales, const Tensor& status) {
     fa_paged_cache c;
-    if (!cache_of(k, k_pages, v_pages, table, lens, starts, c) || !rows_as_is(v, 3) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() ||
+    fa_paged_more more{};
+    if (!cache_of(k, k_pages, v_pages, table, lens, starts, k_scales, v_scales, c, more) || !rows_as_is(v, 3) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() ||
         v.device() != k.device() || k.size(1) != c.Hk)
         return false;
     {
         py::gil_scoped_release free;
         const fa_rows rk = rows_view(k), rv = rows_view(v);
-        check(fa_paged_append(&c, int(k.size(0)), starts ? starts->const_data_ptr<int>() : nullptr, &rk, &rv, status.data_ptr<int>(), current_stream(k)),
-              "fa_paged_append");
+        check(fa_paged_append_more(&c, &more, int(k.size(0)), starts ? starts->const_data_ptr<int>() : nullptr, &rk, &rv, status.data_ptr<int>(), current_stream(k)),
+              "fa_paged_append_more");
         ++n_launched;
     }
     bump(k_pages);
     bump(v_pages);
+    if (k_scales) {
+        bump(*k_scales);
+        bump(*v_scales);
+    }
     return true;
 }
 
 py::object paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens,
                            const std::optional<Tensor>& starts, std::optional<double> scale, double softcap, const std::optional<Tensor>& slopes,
                            const std::optional<Tensor>& prefix, const std::optional<Tensor>& out, int64_t window, int64_t sinks, const std::optional<Tensor>& parents,
-                           const Tensor& status) {
+                           const std::optional<Tensor>& k_scales, const std::optional<Tensor>& v_scales, const Tensor& status) {
     fa_paged_cache c;
     fa_scores s;
-    if (!cache_of(q, k_pages, v_pages, table, lens, starts, c)) return py::none();
+    fa_paged_more more{};
+    if (!cache_of(q, k_pages, v_pages, table, lens, starts, k_scales, v_scales, c, more)) return py::none();
     const int64_t H = q.size(1);
     const double sm_scale = scale ? *scale : 1.0 / std::sqrt(double(c.D));
     if (H % c.Hk != 0 || H / c.Hk > 128 || !(sm_scale > 0) || !std::isfinite(sm_scale) || !scores_of(softcap, slopes, prefix, q, H, c.B, s)) return py::none();
     if (parents && !int_vector(*parents, q, q.size(0))) return py::none();
-    const fa_paged_more more{{int(window), int(sinks)}, parents ? parents->const_data_ptr<int>() : nullptr};  // (as paged.py has checked them)
+    more.window = {int(window), int(sinks)};  // (as paged.py has checked them)
+    more.parents = parents ? parents->const_data_ptr<int>() : nullptr;
     if (out) {
         if (!rows_as_is(*out, 3) || out->sizes() != q.sizes() || out->scalar_type() != q.scalar_type() || out->device() != q.device() || out->requires_grad())
             return py::none();
-        for (const Tensor* t : {&q, &k_pages, &v_pages})
+        for (const Tensor* t : {&q, &k_pages, &v_pages, k_scales ? &*k_scales : &q, v_scales ? &*v_scales : &q})
             if (t->storage().data() == out->storage().data()) return py::none();  // paged.py looks closer
     }
     Tensor o;

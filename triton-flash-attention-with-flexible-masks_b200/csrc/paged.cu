@@ -1,6 +1,7 @@
 // extern "C" surface of the paged cache (declared in include/fa_b200.h): argument checks, tensor maps, launches. Nothing here allocates,
 // synchronises or throws.
 #include <algorithm>
+#include <cmath>
 #include "../../include/fa_b200.h"
 #include "common.cuh"
 #include "host_shared.cuh"
@@ -9,6 +10,7 @@
 
 namespace fa {
 cudaError_t launch_paged_append(const PagedParams&, const void*, const void*, void*, void*, const int64_t*, cudaStream_t);
+cudaError_t launch_paged_append_e4m3(bool, const PagedParams&, const void*, const void*, void*, void*, uint8_t*, uint8_t*, const int64_t*, cudaStream_t);
 cudaError_t launch_paged_fwd(bool, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const PagedParams&, int, cudaStream_t);
 }  // namespace fa
 
@@ -42,6 +44,29 @@ int check_cache(const fa_paged_cache* c) {
     const int extent[3] = {c->pages, c->page_size, c->Hk};
     int rc = check_strides(c->k, c->k_stride, extent, 3);
     return rc ? rc : check_strides(c->v, c->v_stride, extent, 3);
+}
+
+// The scales of a cache of 8 bits, and what such a cache asks for besides; without any, nothing.
+int check_scales(const fa_paged_cache* c, const fa_paged_more* more) {
+    if (!more->k_scales && !more->v_scales) return FA_OK;
+    if (!more->k_scales || !more->v_scales) return FA_ERR_BAD_ARG;
+    if (c->page_size < 16) return FA_ERR_PAGED;
+    const int extent[3] = {c->pages, c->page_size, c->Hk};
+    for (int i = 0; i < 3; ++i)
+        if (extent[i] > 1 && (c->k_stride[i] % 16 != 0 || c->v_stride[i] % 16 != 0)) return FA_ERR_ALIGNMENT;
+    const int64_t strides[4] = {more->k_scale_stride[0], more->k_scale_stride[1], more->v_scale_stride[0], more->v_scale_stride[1]};
+    for (int i = 0; i < 4; ++i)
+        if ((i % 2 ? c->Hk : c->pages) > 1 && (strides[i] <= 0 || strides[i] % 16 != 0)) return FA_ERR_ALIGNMENT;
+    return aligned(more->k_scales, 16) && aligned(more->v_scales, 16) ? FA_OK : FA_ERR_ALIGNMENT;
+}
+
+void fill_scales(fa::PagedParams* p, const fa_paged_cache* c, const fa_paged_more* more) {
+    p->k_scales = more->k_scales;
+    p->v_scales = more->v_scales;
+    p->k_scale_p = c->pages > 1 ? more->k_scale_stride[0] : 0;
+    p->k_scale_h = c->Hk > 1 ? more->k_scale_stride[1] : 0;
+    p->v_scale_p = c->pages > 1 ? more->v_scale_stride[0] : 0;
+    p->v_scale_h = c->Hk > 1 ? more->v_scale_stride[1] : 0;
 }
 
 int check_rows(const fa_rows* r, int T, int H) {
@@ -81,6 +106,19 @@ int map4(CUtensorMap* out, int dtype, const void* ptr, int D, const int (&extent
     const CUresult r = fn(out, dtype == FA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(ptr), dims, bytes,
                           b, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? FA_OK : FA_ERR_TENSORMAP;
+}
+
+// The same over a cache of 8 bits: whole rows of 64 or 128 bytes as they lie, behind one another
+int map_bytes(CUtensorMap* out, const void* ptr, int D, const int (&extent)[3], const int64_t (&stride)[3], int rows) {
+    const fa::EncodeFn fn = fa::encode_fn();
+    if (!fn) return FA_ERR_NO_DRIVER;
+    const cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(extent[0]), cuuint64_t(extent[1]), cuuint64_t(extent[2])};
+    cuuint64_t bytes[3];
+    for (int i = 0; i < 3; ++i) bytes[i] = cuuint64_t(extent[i] > 1 ? stride[i] : D);  // an extent of 1 may carry any stride
+    const cuuint32_t b[4] = {D > 64 ? 128u : 64u, 1, cuuint32_t(rows), 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, bytes, b, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? FA_OK : FA_ERR_TENSORMAP;
 }
 
@@ -156,11 +194,24 @@ int debug_pieces(int32_t B, int32_t T, int32_t Hk, int32_t G, int32_t capacity, 
 extern "C" {
 
 int fa_paged_append(const fa_paged_cache* cache, int32_t T, const int32_t* starts, const fa_rows* k, const fa_rows* v, int32_t* status, void* stream) {
+    return fa_paged_append_more(cache, nullptr, T, starts, k, v, status, stream);
+}
+
+int fa_paged_append_more(const fa_paged_cache* cache, const fa_paged_more* more, int32_t T, const int32_t* starts, const fa_rows* k, const fa_rows* v, int32_t* status,
+                         void* stream) {
     int rc = check_cache(cache);
+    if (!rc && more) rc = check_scales(cache, more);
     if (rc) return rc;
     if ((rc = check_rows(k, T, cache->Hk)) || (rc = check_rows(v, T, cache->Hk))) return rc;
     fa::PagedParams p{};
     if ((rc = fill_params(&p, cache, T, starts, status))) return rc;
+    if (more && more->k_scales) {
+        fill_scales(&p, cache, more);
+        const int64_t strides[10] = {k->stride[0] / 8, k->stride[1] / 8, v->stride[0] / 8, v->stride[1] / 8, cache->k_stride[0], cache->k_stride[1], cache->k_stride[2],
+                                     cache->v_stride[0], cache->v_stride[1], cache->v_stride[2]};
+        return fa::launch_paged_append_e4m3(cache->dtype == FA_BF16, p, k->ptr, v->ptr, cache->k, cache->v, more->k_scales, more->v_scales, strides,
+                                            static_cast<cudaStream_t>(stream)) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+    }
     const int64_t strides[10] = {k->stride[0] / 8, k->stride[1] / 8, v->stride[0] / 8, v->stride[1] / 8,
                                  cache->k_stride[0] / 8, cache->k_stride[1] / 8, cache->k_stride[2] / 8,
                                  cache->v_stride[0] / 8, cache->v_stride[1] / 8, cache->v_stride[2] / 8};
@@ -193,6 +244,7 @@ int fa_paged_fwd_more(const fa_paged_cache* cache, const fa_paged_more* more, in
     const fa_window window = more->window;
     if (window.keys < 0 || window.sinks < 0 || (window.keys == 0 && window.sinks > 0) || (more->parents && (sc->slopes || sc->prefix))) return FA_ERR_SCORES;
     if (!aligned(more->parents, 4)) return FA_ERR_ALIGNMENT;
+    if ((rc = check_scales(cache, more))) return rc;
     if (!aligned(sc->slopes, 4) || !aligned(sc->prefix, 4) || !aligned(workspace, 16)) return FA_ERR_ALIGNMENT;
     fa::PagedParams p{};
     if ((rc = fill_params(&p, cache, T, starts, status))) return rc;
@@ -203,6 +255,7 @@ int fa_paged_fwd_more(const fa_paged_cache* cache, const fa_paged_more* more, in
     p.window = std::min(window.keys, kMostTokens + 1);  // (no token is further away)
     p.sinks = std::min(window.sinks, kMostTokens + 1);
     p.parents = more->parents;
+    fill_scales(&p, cache, more);
     p.out = o->ptr;
     p.out_t = o->stride[0];
     p.out_h = o->stride[1];
@@ -214,6 +267,14 @@ int fa_paged_fwd_more(const fa_paged_cache* cache, const fa_paged_more* more, in
     p.tokens = fa::kBlk / G;
     p.narrow = 32 / G;
     p.fill = fill ? 1 : 0;
+    p.lift = 1.f;
+    if (p.k_scales && cache->dtype == FA_BF16) {  // (the squares of the scores that a cap takes stay in fp32's range, however large q and small the scale)
+        int n = 0;
+        frexpf(sm_scale, &n);
+        n = n > 120 ? 120 : n < -120 ? -120 : n < 20 && n > -20 ? 0 : n;
+        p.lift = ldexpf(1.f, n);
+        sm_scale = ldexpf(sm_scale, -n);
+    }
     p.scale_log2 = sm_scale * fa::kScoreLog2e;
     p.score = fa::make_score_args(sc->softcap, sc->slopes, sc->prefix != nullptr, sm_scale);
     const int box_rows = cache->page_size < fa::kBlk ? cache->page_size : fa::kBlk;
@@ -221,6 +282,11 @@ int fa_paged_fwd_more(const fa_paged_cache* cache, const fa_paged_more* more, in
     if ((rc = map4(&tq, cache->dtype, q->ptr, cache->D, {G, cache->Hk, T}, {q->stride[1], q->stride[1] * G, q->stride[0]}, {G, 1, p.tokens}))) return rc;
     CUtensorMap tn;  // of the rows of 32 / G tokens
     if ((rc = map4(&tn, cache->dtype, q->ptr, cache->D, {G, cache->Hk, T}, {q->stride[1], q->stride[1] * G, q->stride[0]}, {G, 1, p.narrow > 0 ? p.narrow : p.tokens}))) return rc;
+    if (p.k_scales) {
+        if ((rc = map_bytes(&tk, cache->k, cache->D, {cache->Hk, cache->page_size, cache->pages}, {cache->k_stride[2], cache->k_stride[1], cache->k_stride[0]}, box_rows))) return rc;
+        if ((rc = map_bytes(&tv, cache->v, cache->D, {cache->Hk, cache->page_size, cache->pages}, {cache->v_stride[2], cache->v_stride[1], cache->v_stride[0]}, box_rows))) return rc;
+        return fa::launch_paged_fwd(cache->dtype == FA_BF16, tq, tn, tk, tv, p, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+    }
     if ((rc = map4(&tk, cache->dtype, cache->k, cache->D, {cache->Hk, cache->page_size, cache->pages},
                    {cache->k_stride[2], cache->k_stride[1], cache->k_stride[0]}, {1, box_rows, 1}))) return rc;
     if ((rc = map4(&tv, cache->dtype, cache->v, cache->D, {cache->Hk, cache->page_size, cache->pages},

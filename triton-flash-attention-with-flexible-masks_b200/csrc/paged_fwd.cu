@@ -30,9 +30,19 @@
 
 namespace fa {
 
-template <int D>
+// Instances. FORM_MASKED: perhaps a window, perhaps drafted tokens whose parents are given. A tile of keys that the window hides from all of an item's tokens is not among its
+// tiles, and what lies in such keys of the others is as far from the results as what lies behind the sequence: V's rows are zeroed, scores masked. A drafted token's branch is
+// walked once an item, by the thread of each of its rows, while the first keys are on their way, and left as bits in shared memory.
+// FORM_E4M3: the cache is of 8 bits. The rows of K and V land as they are in rings of their own, with their scales; the epilogue group, which has nothing to do while an item lasts, turns
+// each tile into the fp16 tile that the products read (a row is e4m3 times a power of two from 2^-15 to 2^7, all of whose numbers are fp16's: nothing is rounded), K a tile ahead of V, and hidden
+// rows into zeros. The products are fp16's also where q is bf16: q's rows are brought to fp16, by a power of two where their greatest entry asks for it (their scores take it back in fp32),
+// and P is 2^7 times as large as elsewhere, which brings what fp16 cannot tell from 0 from 2^-25 down to 2^-32 of a row's reference (l and O have the factor alike).
+enum : int { FORM_PLAIN = 0, FORM_MASKED = 1, FORM_E4M3 = 2 };
+
+template <int D, int FORM>
 struct PagedSmem {
-    static constexpr int NS = (D == 128) ? 2 : 4;  // depth of the K ring and of the V ring
+    static constexpr bool E4M3 = (FORM & FORM_E4M3) != 0;
+    static constexpr int NS = E4M3 ? (D == 128 ? 1 : 2) : (D == 128) ? 2 : 4;  // depth of the K ring and of the V ring
     static constexpr int NQ = 2;                   // item slots
     // TMEM columns as in the forward kernel
     static constexpr bool POWN = D == 128;
@@ -46,13 +56,19 @@ struct PagedSmem {
     static constexpr int off_q = 0;  // NQ Q tiles
     static constexpr int off_k = NQ * TILE;
     static constexpr int off_v = off_k + NS * TILE;
-    static constexpr int off_ml = off_v + NS * TILE;             // float [NQ][2 groups][m, l][128]
+    // E4M3: rings of rows as they are, and of their scales; the factor of each row's scores
+    static constexpr int RAW = E4M3 ? kBlk * D : 0;
+    static constexpr int NRK = !E4M3 ? 0 : D == 128 ? 3 : 5, NRV = !E4M3 ? 0 : D == 128 ? 2 : 5;
+    static constexpr int off_raw_k = off_v + NS * TILE, off_raw_v = off_raw_k + NRK * RAW;
+    static constexpr int off_ml = off_raw_v + NRV * RAW;         // float [NQ][2 groups][m, l][128]
     static constexpr int off_info = off_ml + NQ * 4 * kBlk * 4;  // int32 [NQ][16]: see I_*
-    static constexpr int off_plan = off_info + NQ * 64;
+    static constexpr int off_scale_k = off_info + NQ * 64, off_scale_v = off_scale_k + NRK * kBlk;
+    static constexpr int off_factor = off_scale_v + NRV * kBlk;  // float [NQ][128]
+    static constexpr int off_plan = off_factor + (E4M3 ? NQ * kBlk * 4 : 0);
     static constexpr int off_bar = off_plan + int(sizeof(PagedPlan));
     // item_full[NQ] item_empty[NQ] q_full[NQ] ml_full[NQ] staged k_full[NS] k_empty[NS] v_full[NS] v_empty[NS]
-    // s_full[4] s_free[2] p_full[NP] pv_done[NP] o_full[2] o_free[2]
-    static constexpr int n_bar = 4 * NQ + 1 + 4 * NS + 6 + 2 * NP + 4;
+    // s_full[4] s_free[2] p_full[NP] pv_done[NP] o_full[2] o_free[2]; E4M3: raw_k_full[NRK] raw_k_empty[NRK] raw_v_full[NRV] raw_v_empty[NRV] q_ready[NQ]
+    static constexpr int n_common = 4 * NQ + 1 + 4 * NS + 6 + 2 * NP + 4, n_bar = n_common + 2 * NRK + 2 * NRV + (E4M3 ? NQ : 0);
     static constexpr int off_misc = off_bar + n_bar * 8;  // tmem slot, abort flag
     static constexpr int total = off_misc + 16;
     static_assert(off_plan % 8 == 0 && off_bar % 8 == 0, "alignment");
@@ -61,8 +77,9 @@ struct PagedSmem {
     static constexpr int off_masks = off_plan + int(offsetof(PagedPlan, sums)), kMaskWords = kPagedTree / 32;
     static_assert(2 * kMaskWords * kBlk * 4 <= int(sizeof(PagedPlan::sums)), "room for the masks");
 };
-static_assert(PagedSmem<128>::total <= 232448 && PagedSmem<64>::total <= 232448, "shared memory budget");
-static_assert(PagedSmem<128>::total > 116736 && PagedSmem<64>::total > 116736, "shares an SM");
+template <int D, int FORM>
+constexpr bool kPagedFits = PagedSmem<D, FORM>::total <= 232448 && PagedSmem<D, FORM>::total > 116736;  // the budget, and no other block beside it on the SM
+static_assert(kPagedFits<128, FORM_PLAIN> && kPagedFits<64, FORM_PLAIN> && kPagedFits<128, FORM_E4M3> && kPagedFits<64, FORM_E4M3>, "shared memory");
 
 // What an item's slot says: number of its key tiles, the first one, whether there is an item (1, or -1: no more), kv head, first row of its tokens in
 // q and out, how many of them, position of the first one, the sequence's length, its prefix, the sequence, slot of the workspace (-1: straight to out)
@@ -70,17 +87,14 @@ static_assert(PagedSmem<128>::total > 116736 && PagedSmem<64>::total > 116736, "
 // length); first row of the sequence
 enum : int { I_TILES = 0, I_LO, I_MORE, I_HEAD, I_ROW, I_TOKENS, I_POS, I_LEN, I_FRONT, I_SEQ, I_PART, I_BORDER, I_SKIP, I_BASE, I_FIRST };
 
-// Instances. FORM_MASKED: perhaps a window, perhaps drafted tokens whose parents are given. A tile of keys that the window hides from all of an item's tokens is not among its
-// tiles, and what lies in such keys of the others is as far from the results as what lies behind the sequence: V's rows are zeroed, scores masked. A drafted token's branch is
-// walked once an item, by the thread of each of its rows, while the first keys are on their way, and left as bits in shared memory.
-enum : int { FORM_PLAIN = 0, FORM_MASKED = 1 };
-
 template <int D, bool BF16, int KIND, int FORM>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmN, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const PagedParams p) {
-    using S = PagedSmem<D>;
-    constexpr bool SCORED = score_changed(KIND), MASKED = (FORM & FORM_MASKED) != 0;
+    using S = PagedSmem<D, FORM>;
+    constexpr bool SCORED = score_changed(KIND), MASKED = (FORM & FORM_MASKED) != 0, E4M3 = S::E4M3;
+    constexpr bool PBF16 = BF16 && !E4M3;           // the products' type
+    constexpr float kRaised = E4M3 ? 7.f : 0.f;     // log2 of what P is multiplied by
     constexpr int NS = S::NS, NQ = S::NQ, NP = S::NP;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -94,7 +108,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     constexpr int B_ITEMFULL = 0, B_ITEMEMPTY = NQ, B_QFULL = 2 * NQ, B_MLFULL = 3 * NQ, B_STAGED = 4 * NQ, B_KFULL = 4 * NQ + 1,
                   B_KEMPTY = B_KFULL + NS, B_VFULL = B_KEMPTY + NS, B_VEMPTY = B_VFULL + NS, B_SFULL = B_VEMPTY + NS,
                   B_SFREE = B_SFULL + 4, B_PFULL = B_SFREE + 2, B_PVDONE = B_PFULL + NP, B_OFULL = B_PVDONE + NP, B_OFREE = B_OFULL + 2;
-    static_assert(B_OFREE + 2 == S::n_bar, "barriers");
+    static_assert(B_OFREE + 2 == S::n_common, "barriers");
+    constexpr int B_RAWK = S::n_common, B_RAWKEMPTY = B_RAWK + S::NRK, B_RAWV = B_RAWKEMPTY + S::NRK, B_RAWVEMPTY = B_RAWV + S::NRV, B_QREADY = B_RAWVEMPTY + S::NRV;
     Abort ab{misc + 1, p.status, p.wait_limit};
 
     if (tid == 0) {
@@ -105,10 +120,21 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             mbar_init(BAR(B_MLFULL + s), 8);
         }
         for (int s = 0; s < NS; ++s) {
-            mbar_init(BAR(B_KFULL + s), 1);
+            mbar_init(BAR(B_KFULL + s), E4M3 ? 4 : 1);  // (the warps that make the tile)
             mbar_init(BAR(B_KEMPTY + s), 1);
-            mbar_init(BAR(B_VFULL + s), 1);
+            mbar_init(BAR(B_VFULL + s), E4M3 ? 4 : 1);
             mbar_init(BAR(B_VEMPTY + s), 1);
+        }
+        if constexpr (E4M3) {
+            for (int s = 0; s < S::NRK; ++s) {
+                mbar_init(BAR(B_RAWK + s), 1);
+                mbar_init(BAR(B_RAWKEMPTY + s), 4);
+            }
+            for (int s = 0; s < S::NRV; ++s) {
+                mbar_init(BAR(B_RAWV + s), 1);
+                mbar_init(BAR(B_RAWVEMPTY + s), 4);
+            }
+            for (int s = 0; s < NQ; ++s) mbar_init(BAR(B_QREADY + s), 4);
         }
         mbar_init(BAR(B_STAGED), 4);
         for (int s = 0; s < 4; ++s) mbar_init(BAR(B_SFULL + s), 1);
@@ -145,6 +171,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         paged_plan<kFwdThreads, MASKED>(p, plan, int(gridDim.x));
     }
     const int worker = int(blockIdx.x);
+    // what a row's scores are multiplied by (a factor must bring it neither to 0 nor beyond fp32: a maximum of minus infinity is multiplied, too)
+    auto scale_of = [&](float factor) { return SCORED ? 1.f : E4M3 && BF16 ? fminf(fmaxf(p.scale_log2 * factor, 1.2e-38f), 3e38f) : p.scale_log2; };
     // the key block that is an item's x-th
     auto key_block = [](int x, int border, int skip) { return MASKED && x >= border ? x + skip : x; };
 
@@ -176,6 +204,20 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
         };
         static_assert(S::NBOX == 1 || S::NBOX == 2, "bytes of a tile");
+        // E4M3: rows of D bytes, and a byte for each
+        auto load_raw = [&](const CUtensorMap* m, uint32_t dst, const uint8_t* scales, int64_t scale_p, uint32_t dst_scale, uint32_t bar, int pages, int tile, int hk, int len) {
+            const int left = len - (tile << 7), n = left >= kBlk ? boxes : (left + rows - 1) >> log2_rows;
+            mbar_expect_tx_elect(bar, (uint32_t(n) << log2_rows) * uint32_t(D + 1));
+            const int row = (tile << 7) & (p.page - 1) & ~(rows - 1);
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) {
+                const uint32_t page = uint32_t(__shfl_sync(0xffffffffu, pages, i));
+                tma_load_4d_elect(dst, m, bar, 0, hk, row, int(min(page, uint32_t(p.n_pages))));
+                bulk_load_1d_elect(dst_scale, scales + min(page, uint32_t(p.n_pages - 1)) * scale_p + row, uint32_t(rows), bar);
+                dst += uint32_t(rows) * D;
+                dst_scale += uint32_t(rows);
+            }
+        };
         if (aborted) {
         } else if (warp == 14) {
             // ------------------------------ item scheduler, and loads of Q and K ------------------------------
@@ -228,11 +270,16 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         for (int x = 0; x < S::NBOX; ++x) tma_load_4d_elect(sQ(s) + x * S::BOX, &tmQ, BAR(B_QFULL + s), x * 64, 0, hk, tok0);
                     }
                     for (int t = 0; t < T; ++t, ++gk) {
-                        const int st = gk % NS, ug = gk / NS, own = pages;
+                        constexpr int R = E4M3 ? S::NRK : NS;
+                        const int st = gk % R, ug = gk / R, own = pages;
                         if (t + 1 < T) pages = pages_of(row_of_table, key_block(tile0 + t + 1, border, skip), len);
-                        if (ug > 0) ok = mbar_wait_warp(BAR(B_KEMPTY + st), (ug - 1) & 1, ab, ST_WAIT_TIMEOUT + 1);
+                        if (ug > 0) ok = mbar_wait_warp(BAR((E4M3 ? B_RAWKEMPTY : B_KEMPTY) + st), (ug - 1) & 1, ab, ST_WAIT_TIMEOUT + 1);
                         if (!ok) return false;
-                        load(&tmK, sK(st), BAR(B_KFULL + st), own, key_block(tile0 + t, border, skip), hk, len);
+                        if constexpr (E4M3)
+                            load_raw(&tmK, sbase + S::off_raw_k + uint32_t(st) * S::RAW, p.k_scales + hk * p.k_scale_h, p.k_scale_p, sbase + S::off_scale_k + uint32_t(st) * kBlk,
+                                     BAR(B_RAWK + st), own, key_block(tile0 + t, border, skip), hk, len);
+                        else
+                            load(&tmK, sK(st), BAR(B_KFULL + st), own, key_block(tile0 + t, border, skip), hk, len);
                     }
                     ++k;
                     if (first && paged_first_cut(plan, worker, walk)) {
@@ -270,11 +317,16 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 const int32_t* const row_of_table = p.table + seq * p.table_stride;
                 int pages = T > 0 ? pages_of(row_of_table, key_block(lo, border, skip), len) : 0;
                 for (int t = 0; t < T; ++t, ++gv) {
-                    const int st = gv % NS, ug = gv / NS, own = pages;
+                    constexpr int R = E4M3 ? S::NRV : NS;
+                    const int st = gv % R, ug = gv / R, own = pages;
                     if (t + 1 < T) pages = pages_of(row_of_table, key_block(lo + t + 1, border, skip), len);
-                    if (ug > 0) ok = mbar_wait_warp(BAR(B_VEMPTY + st), (ug - 1) & 1, ab, ST_WAIT_TIMEOUT + 2);
+                    if (ug > 0) ok = mbar_wait_warp(BAR((E4M3 ? B_RAWVEMPTY : B_VEMPTY) + st), (ug - 1) & 1, ab, ST_WAIT_TIMEOUT + 2);
                     if (!ok) break;
-                    load(&tmV, sV(st), BAR(B_VFULL + st), own, key_block(lo + t, border, skip), hk, len);
+                    if constexpr (E4M3)
+                        load_raw(&tmV, sbase + S::off_raw_v + uint32_t(st) * S::RAW, p.v_scales + hk * p.v_scale_h, p.v_scale_p, sbase + S::off_scale_v + uint32_t(st) * kBlk,
+                                 BAR(B_RAWV + st), own, key_block(lo + t, border, skip), hk, len);
+                    else
+                        load(&tmV, sV(st), BAR(B_VFULL + st), own, key_block(lo + t, border, skip), hk, len);
                 }
                 if (!ok) break;
                 __syncwarp();
@@ -285,8 +337,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             // ------------------------------ MMA issuers ------------------------------
             //   warp 13: P*V(g) when P(g) is there; warp 15: S(g) when its buffer is free
             const uint32_t utmem = uniform(int(tmem));
-            constexpr uint32_t idesc_s = make_idesc(BF16, 128, 128, false, false);
-            constexpr uint32_t idesc_pv = make_idesc(BF16, 128, D, false, true);
+            constexpr uint32_t idesc_s = make_idesc(PBF16, 128, 128, false, false);
+            constexpr uint32_t idesc_pv = make_idesc(PBF16, 128, D, false, true);
             constexpr uint64_t desc_v = desc_mn_major(S::BOX);
             bool ok = true;
             int G = 0;           // tiles of all earlier items
@@ -298,7 +350,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 const int T = uniform(info[16 * s + I_TILES]);
                 if (uniform(info[16 * s + I_MORE]) < 0) break;
                 if (warp == 15) {
-                    if (T > 0) ok = mbar_wait_warp(BAR(B_QFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 3);
+                    if (T > 0) ok = mbar_wait_warp(BAR((E4M3 && BF16 ? B_QREADY : B_QFULL) + s), use & 1, ab, ST_WAIT_TIMEOUT + 3);
                     for (int g = G; g < G + T && ok; ++g) {
                         const int st = g % NS;
                         ok = mbar_wait_warp(BAR(B_KFULL + st), (g / NS) & 1, ab, ST_WAIT_TIMEOUT + 4);
@@ -352,8 +404,69 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         setmaxnreg_dec<kFwdEpilogueRegs>();
         const int r = tid & 127;
         const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
-        const float c = SCORED ? 1.f : p.scale_log2;
         const int tok_wide = r / p.G, tok_narrow = lane / p.G;
+        // E4M3: the g-th tile of K or V, rows of D numbers in e4m3 to 64-column boxes of fp16 with the swizzle that the products read. A thread takes 16 numbers at a time; those
+        // that write together have eight different 16-byte places of the 128 bytes.
+        auto unpack_tile = [&](auto values, int g, int k0, int seen, int early, int low) {
+            constexpr bool V = decltype(values)::value;
+            constexpr int R = V ? S::NRV : S::NRK, kThreadsARow = D / 16, kRows = kBlk / kThreadsARow;  // rows that the group takes together
+            const int raw = g % R, st = g % NS;
+            if (!mbar_wait_warp(BAR((V ? B_RAWV : B_RAWK) + raw), (g / R) & 1, ab, ST_WAIT_TIMEOUT + 20)) return false;
+            if (g >= NS && !mbar_wait_warp(BAR((V ? B_VEMPTY : B_KEMPTY) + st), (g / NS - 1) & 1, ab, ST_WAIT_TIMEOUT + 21)) return false;
+            const uint8_t* const from = smem + (V ? S::off_raw_v : S::off_raw_k) + raw * S::RAW;
+            const uint8_t* const scales = smem + (V ? S::off_scale_v : S::off_scale_k) + raw * kBlk;
+            uint8_t* const to = smem + (V ? S::off_v : S::off_k) + st * S::TILE;
+            const int part = r % kThreadsARow, row0 = r / kThreadsARow, box = part >> 2, swap = box & 1;
+            const bool all = k0 + kBlk <= seen && (k0 + kBlk <= early || k0 >= low);
+#pragma unroll 4
+            for (int i = 0; i < kBlk / kRows; ++i) {
+                const int row = row0 + i * kRows, key = k0 + row;
+                const uint4 x = *reinterpret_cast<const uint4*>(from + row * D + part * 16);
+                const int e = min(max(int(scales[row]), kScaleLeast), kScaleMost) - kScaleLeast;
+                const uint32_t one = e > 0 ? uint32_t(e) << 10 : 0x200u, scale = one | one << 16;  // 2^(e - 15) in fp16
+                uint32_t y[8];
+                unpack_e4m3x4(x.x, y[0], y[1]);
+                unpack_e4m3x4(x.y, y[2], y[3]);
+                unpack_e4m3x4(x.z, y[4], y[5]);
+                unpack_e4m3x4(x.w, y[6], y[7]);
+                const bool real = all || (key < seen && (key < early || key >= low));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = real ? mul_h2(y[j], scale) : 0u;
+                uint8_t* const line = to + box * S::BOX + row * 128;
+                const int c0 = 2 * (part & 3) + swap, c1 = c0 ^ 1;
+                *reinterpret_cast<uint4*>(line + ((c0 ^ (row & 7)) << 4)) = swap ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(line + ((c1 ^ (row & 7)) << 4)) = swap ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
+            }
+            fence_proxy_async();
+            mbar_arrive_warp(BAR((V ? B_RAWVEMPTY : B_RAWKEMPTY) + raw), lane);
+            if (lane == 0) mbar_arrive(BAR((V ? B_VFULL : B_KFULL) + st));
+            return true;
+        };
+        // E4M3 of bf16: this thread's row of Q to fp16 in place, times a power of two where its greatest entry is beyond fp16 or so small that the others would lose bits; what the
+        // row's scores are to be multiplied by.
+        auto query_to_fp16 = [&](int s) {
+            uint8_t* const row = smem + S::off_q + s * S::TILE + r * 128;
+            auto at = [&](int i) { return reinterpret_cast<uint4*>(row + (i >> 3) * S::BOX + (((i + r) & 7) << 4)); };  // (any order will do: eight lanes at eight places)
+            uint32_t most = 0;  // bf16 numbers without their sign go by size
+#pragma unroll 4
+            for (int i = 0; i < D / 8; ++i) {
+                const uint4 x = *at(i);
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) most = max(most, max(w[j] & 0x7fffu, w[j] >> 16 & 0x7fffu));
+            }
+            // (0, infinities and NaN go as they are)
+            const int exponent = int(most >> 7) - 127, shift = most == 0 || most >= 0x7f80u || (exponent >= -8 && exponent < 15) ? 0 : min(max(exponent, -120), 120);
+            const float back = __uint_as_float(uint32_t(127 + shift) << 23), there = __uint_as_float(uint32_t(127 - shift) << 23);
+#pragma unroll 4
+            for (int i = 0; i < D / 8; ++i) {
+                uint4* const x = at(i);
+                const uint4 v = *x;
+                auto two = [&](uint32_t y) { return pack2<false>(__uint_as_float(y << 16) * there, __uint_as_float(y & 0xffff0000u) * there); };
+                *x = make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
+            }
+            return back;
+        };
         // of a narrow item's sums: this thread adds up four columns of row r / 4
         const int row_sum = r >> 2, tok_sum = row_sum / p.G;
         int staged = 0;  // passes through the staging barrier
@@ -396,6 +509,25 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     check_pages(it[I_LO] * kBlk, T > 0 ? min((it[I_LO] + T) * kBlk, it[I_LEN]) : 0);
                 }
             }
+            float factor = 1.f;  // E4M3 of bf16: of this row's scores
+            if constexpr (E4M3) {
+                if constexpr (BF16) {
+                    alive = mbar_wait_warp(BAR(B_QFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 17);
+                    if (!alive) break;
+                    factor = fminf(query_to_fp16(s) * p.lift, 3e38f);
+                    reinterpret_cast<float*>(smem + S::off_factor)[s * kBlk + r] = factor;
+                    fence_proxy_async();
+                    mbar_arrive_warp(BAR(B_QREADY + s), lane);
+                }
+                const int pos0 = it[I_POS], len = it[I_LEN], front = it[I_FRONT], lo = it[I_LO], border = it[I_BORDER], skip = it[I_SKIP];
+                const int seen = min(max(pos0 + tokens, front), len), early = p.window > 0 ? max(front, p.sinks) : len;
+                const int low = p.window > 0 ? (it[I_BASE] < len ? it[I_BASE] : pos0) - p.window + 1 : 0;
+                for (int t = 0; t <= T && alive; ++t) {
+                    if (t < T) alive = unpack_tile(std::false_type{}, G + t, key_block(lo + t, border, skip) * kBlk, seen, early, low);
+                    if (t > 0 && alive) alive = unpack_tile(std::true_type{}, G + t - 1, key_block(lo + t - 1, border, skip) * kBlk, seen, early, low);
+                }
+                if (!alive) break;
+            }
             // the only wait here that lasts as long as an item: it allows each of the tiles what another wait may last
             const Abort item{ab.flag, ab.status, ab.limit * (T + 1)};
             alive = mbar_wait_warp(BAR(B_MLFULL + s), use & 1, item, ST_WAIT_TIMEOUT + 16);
@@ -414,6 +546,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (narrow) {  // over the four warps' chains of the row
                 for (int q = 0; q < 4; ++q) mt = fmaxf(mt, fmaxf(ml[even + 32 * q + lane], ml[odd + 32 * q + lane]));
             }
+            const float c = scale_of(factor);
             const float a0 = (m0 == -INFINITY) ? 0.f : fast_exp2((m0 - mt) * c);
             const float a1 = (m1 == -INFINITY) ? 0.f : fast_exp2((m1 - mt) * c);
             float lt = l0 * a0 + l1 * a1;
@@ -510,7 +643,6 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const int w = warp >> 2;  // group
         const int r = tid & 127;  // row inside the tile
         const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
-        const float c = SCORED ? 1.f : p.scale_log2;
         const uint32_t tO = tmem + lane_base + uint32_t(S::tmem_o + w * D);
         const int tok_wide = r / p.G, tok_narrow = lane / p.G;
         bool alive = !aborted;
@@ -624,6 +756,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
             const int t0 = (G ^ w) & 1;  // this group's first tile of the item
             float m_run = -INFINITY, l_run = 0.f;
+            float factor = 1.f;  // E4M3 of bf16: of the row's scores
 
             for (int t = t0; t < T && alive; t += 2) {
                 const int k0 = key_block(lo + t, border, skip) * kBlk;
@@ -639,13 +772,15 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 alive = mbar_wait_warp(BAR(B_SFULL + (g & 3)), (g >> 2) & 1, ab, ST_WAIT_TIMEOUT + 7);
                 if (!alive) break;
                 tc_fence_after();
+                if constexpr (E4M3 && BF16) factor = reinterpret_cast<volatile float*>(smem + S::off_factor)[s * kBlk + r];  // (written before Q was given to the product)
+                const float c = scale_of(factor);
                 if (!active) {  // no row of this warp is a query: its lanes of P and O are never stored
                     if (S::POWN) {
                         mbar_arrive_warp(BAR(B_SFREE + w), lane);
                         alive = pv_before();
                         if (!alive) break;
                     }
-                    if (seen - k0 < kBlk || none) alive = zero_behind(g, min(seen - k0, kBlk), none_from, none_end);
+                    if (!E4M3 && (seen - k0 < kBlk || none)) alive = zero_behind(g, min(seen - k0, kBlk), none_from, none_end);
                     if (!alive) break;
                     mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
                     continue;
@@ -663,16 +798,20 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
                     float* v = reinterpret_cast<float*>(sq);
                     if constexpr (SCORED) {
-                        if (seen - kq < 32) {
+                        if (E4M3 && BF16 && __any_sync(0xffffffffu, factor != 1.f)) {
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) v[x] *= factor;
+                        }
+                        if (!E4M3 && seen - kq < 32) {
 #pragma unroll
                             for (int x = 0; x < 32; ++x) v[x] = x < seen - kq ? v[x] : 0.f;
                         }
-                        if (none) {
+                        if (!E4M3 && none) {
 #pragma unroll
                             for (int x = 0; x < 32; ++x) v[x] = x + 32 * quarter >= none_from && x + 32 * quarter < none_end ? 0.f : v[x];
                         }
                         const Bias bias(slope, front == 0, pos0 - (kq + 31), pos0 + 31 - kq);
-                        score_row<KIND, 32>(v, p.score, bias, p.scale_log2, pos - kq, valid, m_run == -INFINITY ? 0.f : m_run);
+                        score_row<KIND, 32>(v, p.score, bias, p.scale_log2, pos - kq, valid, (m_run == -INFINITY ? 0.f : m_run) - kRaised);
                     }
                     if (MASKED ? masked : kq + 31 > all_see) {
                         const uint32_t keep = sees(kq);
@@ -689,7 +828,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
 #pragma unroll
                     for (int a = 0; a < 4; ++a) mx[a] = fmaxf(mx[a], v[28 + a]);
-                    const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+                    const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) - (SCORED ? kRaised : 0.f);
                     float m_new = fmaxf(m_run, top);
                     bool need = (m_new - m_run) * c > 8.0f;
                     if constexpr (SCORED) {
@@ -709,7 +848,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     if (scale_o) rescale(alpha);
                     m_run = m_new;
                     // (SCORED: what is left to be subtracted)
-                    const float mneg = SCORED ? (need ? -top : 0.f) : (m_run == -INFINITY) ? 0.f : -m_run * c;
+                    const float mneg = SCORED ? (need ? -top : 0.f) : (m_run == -INFINITY) ? 0.f : kRaised - m_run * c;
                     float l4[4] = {0.f, 0.f, 0.f, 0.f};
                     uint32_t pk[16];
 #pragma unroll
@@ -717,7 +856,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         const float p0 = fast_exp2(fmaf(v[x], c, mneg)), p1 = fast_exp2(fmaf(v[x + 1], c, mneg));
                         l4[x & 2] += p0;
                         l4[(x & 2) + 1] += p1;
-                        pk[x / 2] = pack2<BF16>(p0, p1);
+                        pk[x / 2] = pack2<PBF16>(p0, p1);
                     }
                     uint32_t zero[16] = {};
 #pragma unroll
@@ -725,7 +864,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         if (q != quarter) tmem_st16(tP + uint32_t(q) * 16u, zero);
                     tmem_st16(tP + uint32_t(quarter) * 16u, pk);
                     tc_wait_st();
-                    if (seen - k0 < kBlk || none) alive = zero_behind(g, min(seen - k0, kBlk), none_from, none_end);
+                    if (!E4M3 && (seen - k0 < kBlk || none)) alive = zero_behind(g, min(seen - k0, kBlk), none_from, none_end);
                     tc_fence_before();
                     mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
                     if (!alive) break;
@@ -746,18 +885,22 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 // runs beside the special-function unit. (With a bias the greatest one has to be looked for behind it.)
                 bool late = false;
                 if constexpr (SCORED) {
-                    // (what the others' scores are must not tell the warp which form of the cap to take)
-                    if (real < kBlk) {
+                    if (E4M3 && BF16 && __any_sync(0xffffffffu, factor != 1.f)) {
+#pragma unroll
+                        for (int x = 0; x < kBlk; ++x) sc[x] *= factor;
+                    }
+                    // (what the others' scores are must not tell the warp which form of the cap to take. E4M3: they are 0)
+                    if (!E4M3 && real < kBlk) {
 #pragma unroll
                         for (int x = 0; x < kBlk; ++x) sc[x] = x < real ? sc[x] : 0.f;
                     }
-                    if (none) {
+                    if (!E4M3 && none) {
 #pragma unroll
                         for (int x = 0; x < kBlk; ++x) sc[x] = x >= none_from && x < none_end ? 0.f : sc[x];
                     }
                     const Bias bias(slope, front == 0, pos0 - (k0 + kBlk - 1), pos0 + kBlk - 1 - k0);
                     if constexpr (KIND == SCORE_CAPPED) late = !masked && !any_beyond<kBlk>(sc, valid ? p.score.most : INFINITY);
-                    if (!late) score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, pos - k0, valid, m_run == -INFINITY ? 0.f : m_run);
+                    if (!late) score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, pos - k0, valid, (m_run == -INFINITY ? 0.f : m_run) - kRaised);
                 }
                 if (masked) {
 #pragma unroll
@@ -785,7 +928,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 bool need = (m_new - m_run) * c > 8.0f;
                 if constexpr (SCORED) {  // (the scores, and mx, are relative to the old reference point, or to 0 in front of a row's first key)
                     const bool fresh = m_run == -INFINITY;
-                    if (late) mx = cap_one(mx, p.score) - (fresh ? 0.f : m_run);
+                    mx = late ? cap_one(mx, p.score) - (fresh ? 0.f : m_run) : mx - kRaised;
                     need = fresh ? mx != -INFINITY : mx > 8.0f;
                     m_new = (fresh ? 0.f : m_run) + mx;
                 }
@@ -813,7 +956,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
                 }
                 m_run = m_new;
-                const float mneg = (m_run == -INFINITY) ? 0.f : -m_run * c;
+                const float mneg = (m_run == -INFINITY) ? 0.f : kRaised - m_run * c;
                 // exp2(s*c - m*c) on packed pairs
                 const uint64_t c2 = pack_f2(c, c), mneg2 = pack_f2(mneg, mneg);
                 uint64_t lacc0 = pack_f2(0.f, 0.f), lacc1 = lacc0;
@@ -827,7 +970,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                             unpack_f2(exponent(pack_f2(sc[32 * q + 2 * x], sc[32 * q + 2 * x + 1])), x0, x1);
                             const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
                             if (x & 1) lacc1 = add_f2(lacc1, pack_f2(p0, p1)); else lacc0 = add_f2(lacc0, pack_f2(p0, p1));
-                            pk[x] = pack2<BF16>(p0, p1);
+                            pk[x] = pack2<PBF16>(p0, p1);
                         }
                         tmem_st16(tP + uint32_t(q) * 16u, pk);
                     }
@@ -836,7 +979,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 else if (KIND == SCORE_CAPPED && late) exponentials([&](uint64_t s2) { return fma_f2(s2, cap_poly(s2, p.score), mneg2); });
                 else exponentials([&](uint64_t s2) { return s2; });
                 tc_wait_st();
-                if (real < kBlk || none) alive = zero_behind(g, min(real, kBlk), none_from, none_end);
+                if (!E4M3 && (real < kBlk || none)) alive = zero_behind(g, min(real, kBlk), none_from, none_end);
                 tc_fence_before();
                 mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
                 if (!alive) break;
@@ -1000,7 +1143,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) paged_combine_kernel(const
 template <int D, bool BF16, int KIND, int FORM>
 static cudaError_t launch_paged_t(const CUtensorMap& tq, const CUtensorMap& tn, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {
     auto kern = paged_fwd_kernel<D, BF16, KIND, FORM>;
-    constexpr int smem = PagedSmem<D>::total;
+    constexpr int smem = PagedSmem<D, FORM>::total;
     static SmemAllowed allowed;
     cudaError_t e = allow_smem(kern, smem, allowed);
     if (e != cudaSuccess) return e;
@@ -1012,6 +1155,9 @@ static cudaError_t launch_paged_t(const CUtensorMap& tq, const CUtensorMap& tn, 
 cudaError_t launch_paged_fwd(bool bf16, const CUtensorMap& tq, const CUtensorMap& tn, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {
     auto pick = [&](auto d, auto kind) {
         constexpr int kD = decltype(d)::value, kKind = decltype(kind)::value;
+        if (p.k_scales)
+            return bf16 ? launch_paged_t<kD, true, kKind, FORM_MASKED | FORM_E4M3>(tq, tn, tk, tv, p, workers, stream)
+                        : launch_paged_t<kD, false, kKind, FORM_MASKED | FORM_E4M3>(tq, tn, tk, tv, p, workers, stream);
         if (p.window > 0 || p.parents)
             return bf16 ? launch_paged_t<kD, true, kKind, FORM_MASKED>(tq, tn, tk, tv, p, workers, stream)
                         : launch_paged_t<kD, false, kKind, FORM_MASKED>(tq, tn, tk, tv, p, workers, stream);

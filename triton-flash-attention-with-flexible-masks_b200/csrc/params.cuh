@@ -125,7 +125,12 @@ struct PagedParams {
     const uint8_t* k_scales; // [pages, Hk, page size] exponents of an 8-bit cache's rows, biased by 127; null: a 16-bit cache
     const uint8_t* v_scales;
     int64_t k_scale_p, k_scale_h, v_scale_p, v_scale_h;  // strides in bytes
+    float lift;  // 8-bit cache and bf16 queries: a power of two that scores are multiplied by and `score` and scale_log2 lack, 1 for any usual scale
 };
+
+// The scale of a row of an 8-bit cache is a power of two from 2^-15 to 2^7, stored as its exponent biased by 127: every number that the row then stands for is one of fp16's,
+// and of bf16's.
+constexpr int kScaleLeast = 112, kScaleMost = 134;
 
 // A number for the current CUDA context that no other context of the process ever has, or 0 (api.cu).
 uint64_t context_number();

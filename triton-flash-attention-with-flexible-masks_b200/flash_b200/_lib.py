@@ -19,7 +19,7 @@ EXPORTS = (
     "fa_debug_wait_timeout", "fa_group_rows", "fa_permute_rows", "fa_fwd_splits", "fa_fwd_workspace_bytes", "fa_fwd_split",
     "fa_plan_optional", "fa_bwd", "fa_plan_build_scored", "fa_fwd_scored", "fa_fwd_rest", "fa_bwd_scored", "fa_paged_append",
     "fa_paged_workspace_bytes", "fa_paged_fwd", "fa_debug_paged_pieces",
-    "fa_plan_build_windowed", "fa_fwd_splits_windowed", "fa_fwd_windowed", "fa_bwd_windowed", "fa_paged_fwd_more", "fa_debug_paged_pieces_more",
+    "fa_plan_build_windowed", "fa_fwd_splits_windowed", "fa_fwd_windowed", "fa_bwd_windowed", "fa_paged_append_more", "fa_paged_fwd_more", "fa_debug_paged_pieces_more",
 )
 
 
@@ -55,7 +55,8 @@ class PagedCache(ctypes.Structure):
 
 
 class PagedMore(ctypes.Structure):
-    _fields_ = [("window", Window), ("parents", ctypes.c_void_p)]
+    _fields_ = [("window", Window), ("parents", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
+                ("k_scale_stride", ctypes.c_int64 * 2), ("v_scale_stride", ctypes.c_int64 * 2)]
 
 
 class Rows(ctypes.Structure):
@@ -129,6 +130,8 @@ def load():
     lib.fa_paged_workspace_bytes.argtypes = [C, ctypes.POINTER(size)]
     lib.fa_paged_fwd.restype = i32
     lib.fa_paged_fwd.argtypes = [C, ctypes.c_int32, ctypes.c_int32, vp, ctypes.c_float, S, R, R, ctypes.c_int32, vp, size, vp, vp]
+    lib.fa_paged_append_more.restype = i32
+    lib.fa_paged_append_more.argtypes = [C, ctypes.POINTER(PagedMore), *lib.fa_paged_append.argtypes[1:]]
     lib.fa_paged_fwd_more.restype = i32
     lib.fa_paged_fwd_more.argtypes = [C, ctypes.POINTER(PagedMore), *lib.fa_paged_fwd.argtypes[1:]]
     lib.fa_debug_paged_pieces_more.restype = i32

@@ -12,10 +12,10 @@ _TYPES = {torch.bfloat16: _lib.FA_BF16, torch.float16: _lib.FA_FP16}
 _workspace_bytes = {}  # (device, head dim) -> bytes
 
 
-def _regular(x):
+def _regular(x, multiple=8):
     """Does the library take the tensor as it is?"""
     return x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and not x.is_neg() and all(
-        n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(x.shape[:-1], x.stride()[:-1]))
+        n == 1 or (s > 0 and s % multiple == 0) for n, s in zip(x.shape[:-1], x.stride()[:-1]))
 
 
 def _int32(x, shape, name, like):
@@ -35,8 +35,8 @@ def _no_tangents(*tensors):
         raise RuntimeError("flash_b200: there is no forward-mode derivative through a paged cache; call it with the primals")
 
 
-def _checked(rows, name, k_pages, v_pages, page_table, kv_lens, q_starts):
-    """The cache as the library takes it, its starts, and what has to live as long as they are used."""
+def _checked(rows, name, k_pages, v_pages, page_table, kv_lens, q_starts, k_scales, v_scales):
+    """The cache as the library takes it, what it has besides, its starts, and what has to live as long as they are used."""
     if rows.dim() != 3 or k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
         raise ValueError(f"flash_b200: {name} must be [T, heads, D], k_pages and v_pages [pages, page size, Hk, D]")
     if not rows.is_cuda:
@@ -46,12 +46,25 @@ def _checked(rows, name, k_pages, v_pages, page_table, kv_lens, q_starts):
     pages, page_size, Hk, D = k_pages.shape
     if rows.shape[2] != D or D not in (16, 32, 64, 128):
         raise ValueError(f"flash_b200: the head dim must be 16, 32, 64 or 128 and the cache's, got {rows.shape[2]} and {D}")
-    if rows.dtype not in _TYPES or k_pages.dtype != rows.dtype or v_pages.dtype != rows.dtype:
-        raise ValueError(f"flash_b200: a paged cache and its rows are all bf16 or all fp16, got {rows.dtype}, {k_pages.dtype}, {v_pages.dtype}")
+    eight, more = k_scales is not None or v_scales is not None, _lib.PagedMore()
+    if rows.dtype not in _TYPES or (not eight and (k_pages.dtype != rows.dtype or v_pages.dtype != rows.dtype)):
+        raise ValueError(f"flash_b200: a paged cache and its rows are all bf16 or all fp16 (or the cache has scales and is float8_e4m3fn), got {rows.dtype}, {k_pages.dtype}, {v_pages.dtype}")
     _same_device(rows, k_pages=k_pages, v_pages=v_pages)
     for x, n in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if not _regular(x):
-            raise ValueError(f"flash_b200: {n} needs a 16-byte aligned base, last stride 1 and other strides that are multiples of 8")
+        if not _regular(x, 16 if eight else 8):
+            raise ValueError(f"flash_b200: {n} needs a 16-byte aligned base, last stride 1 and other strides that are multiples of {16 if eight else 8}")
+    if eight:
+        if k_pages.dtype != torch.float8_e4m3fn or v_pages.dtype != torch.float8_e4m3fn:
+            raise ValueError(f"flash_b200: a paged cache with scales is float8_e4m3fn, got {k_pages.dtype}, {v_pages.dtype}")
+        if page_size < 16:
+            raise ValueError(f"flash_b200: the page size of a cache with scales must be 16 at least, got {page_size}")
+        for x, n in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+            if not isinstance(x, torch.Tensor) or x.dtype != torch.float8_e8m0fnu or tuple(x.shape) != (pages, Hk, page_size):
+                raise ValueError(f"flash_b200: {n} must be a float8_e8m0fnu tensor of shape [pages, Hk, page size] = {[pages, Hk, page_size]}; k_scales and v_scales go together")
+            if not _regular(x, 16):
+                raise ValueError(f"flash_b200: {n} needs a 16-byte aligned base, last stride 1 and other strides that are multiples of 16")
+        _same_device(rows, k_scales=k_scales, v_scales=v_scales)
+        more = _lib.PagedMore(_lib.Window(), None, k_scales.data_ptr(), v_scales.data_ptr(), k_scales.stride()[:2], v_scales.stride()[:2])
     if page_size < 8 or page_size & (page_size - 1):
         raise ValueError(f"flash_b200: the page size must be a power of two from 8 on, got {page_size}")
     if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2 or page_table.shape[1] == 0:
@@ -70,10 +83,10 @@ def _checked(rows, name, k_pages, v_pages, page_table, kv_lens, q_starts):
         q_starts = _int32(q_starts, (B + 1,), "q_starts", rows)
     cache = _lib.PagedCache(B, Hk, D, _TYPES[rows.dtype], pages, page_size, page_table.shape[1], page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(),
                             k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride()[:3], v_pages.stride()[:3])
-    return cache, None if q_starts is None else q_starts.data_ptr(), (page_table, kv_lens, q_starts)
+    return cache, more, None if q_starts is None else q_starts.data_ptr(), (page_table, kv_lens, q_starts)
 
 
-def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None):
+def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None, k_scales=None, v_scales=None):
     """Writes the keys and values of new tokens to their places in a cache of pages, in place.
 
     k, v: [T, Hk, D], bf16 or fp16. k_pages, v_pages: [pages, page size, Hk, D], page size a power of two from 8 on; token j of sequence b lies in slot
@@ -83,12 +96,16 @@ def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None):
     front of a sequence's beginning (more rows than kv_lens). The places that are written share no memory with k and v, and where two rows go to one place either may
     stay.
 
+    k_scales, v_scales: float8_e8m0fnu [pages, Hk, page size]; k_pages and v_pages are then float8_e4m3fn, with pages of 16 tokens at least, and a head's row x of a token is quantised as it
+    is written: to the numbers of e4m3 nearest to x / s (ties to even, 448 at most), and the scale s = 2^e with the least e from -15 to 7 for which the largest finite |x| is at most
+    448 s. A row stands for its numbers times its scale. What is not finite becomes a NaN. Where two rows go to one place their parts may mix.
+
     There is no derivative through the cache: under autograd, tensors that ask for a gradient are refused, and so are dual tensors of forward mode.
 
     All lengths and tables are read on the device, so that a captured call follows them. A page number or a length that the cache does not have
     writes nothing and is reported by `check_status`."""
-    native = _native(k, v, k_pages, v_pages, page_table, kv_lens, q_starts)
-    if native is not None and native[0].paged_append(k, v, k_pages, v_pages, page_table, kv_lens, q_starts, native[1]):
+    native = _native(k, v, k_pages, v_pages, page_table, kv_lens, q_starts, k_scales, v_scales)
+    if native is not None and native[0].paged_append(k, v, k_pages, v_pages, page_table, kv_lens, q_starts, k_scales, v_scales, native[1]):
         return
     _no_tangents(k, v, k_pages, v_pages)
     if v.shape != k.shape or k.shape[1:2] != k_pages.shape[2:3]:
@@ -97,16 +114,16 @@ def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None):
         raise ValueError(f"flash_b200: k and v must share one dtype, got {k.dtype}, {v.dtype}")
     if torch.is_grad_enabled() and v.requires_grad:
         raise RuntimeError("flash_b200: there is no gradient through a paged cache; call it under torch.no_grad()")
-    cache, starts, held = _checked(k, "k", k_pages, v_pages, page_table, kv_lens, q_starts)
+    cache, more, starts, held = _checked(k, "k", k_pages, v_pages, page_table, kv_lens, q_starts, k_scales, v_scales)
     _same_device(k, v=v)
     T = k.shape[0]
     if T == 0 or cache.B == 0 or cache.pages == 0:
         return
     k, v = (x if _regular(x) else x.resolve_neg().clone(memory_format=torch.contiguous_format) for x in (k, v))
     with _current(k.device):
-        _lib.check(_lib.load().fa_paged_append(cache, T, starts, _rows(k), _rows(v), _status_word(k.device).data_ptr(), _stream()), "fa_paged_append")
+        _lib.check(_lib.load().fa_paged_append_more(cache, more, T, starts, _rows(k), _rows(v), _status_word(k.device).data_ptr(), _stream()), "fa_paged_append_more")
     _count(1)
-    _bump(k_pages, v_pages)
+    _bump(k_pages, v_pages, *(x for x in (k_scales, v_scales) if x is not None))
     if ops._SYNC_STATUS:
         check_status(k.device)
 
@@ -122,7 +139,8 @@ def _overlap(a, b):
     return ends[0][0] < ends[1][1] and ends[1][0] < ends[0][1]
 
 
-def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_scale=None, softcap=None, slopes=None, prefix=None, out=None, window=None, sinks=0, parents=None):
+def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_scale=None, softcap=None, slopes=None, prefix=None, out=None, window=None, sinks=0, parents=None,
+                    k_scales=None, v_scales=None):
     """Attention of new tokens over a cache of pages that holds their keys and values already (`paged_append`): chunks of prompts and single
     tokens in one ragged batch.
 
@@ -135,6 +153,8 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_
     branch; its position, by which a window goes, is the text's length plus its depth on the branch (0 where it continues the text), theirs likewise. Sequences of more new tokens
     are chunks, whose parents are not read. A parent that does not lie before its token counts as -1 and is reported by `check_status`. Not together with slopes or a prefix.
 
+    k_scales, v_scales: of a cache of 8 bits, as `paged_append` leaves them (scales outside 2^-15 to 2^7 are taken into that range). Its rows are read as the numbers that they stand for, exactly.
+
     A row that sees no token (a length of 0, a position below 0) gives zeros. No derivative, as in `paged_append`.
 
     Returns [T, H, D], zeros in the rows of no sequence; or `out`, whose rows of no sequence are left as they were. `out` shares no memory with q
@@ -146,13 +166,13 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_
     if parents is not None and (slopes is not None or prefix is not None):
         raise ValueError("flash_b200: drafted tokens have no bias by distance and no prefix: parents go without slopes and prefix")
     if sm_scale is None or type(sm_scale) is float:
-        native = _native(q, k_pages, v_pages, page_table, kv_lens, q_starts, slopes, prefix, out, parents)
+        native = _native(q, k_pages, v_pages, page_table, kv_lens, q_starts, slopes, prefix, out, parents, k_scales, v_scales)
         if native is not None:
-            done = native[0].paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts, sm_scale, softcap, slopes, prefix, out, *window, parents, native[1])
+            done = native[0].paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts, sm_scale, softcap, slopes, prefix, out, *window, parents, k_scales, v_scales, native[1])
             if done is not None:
                 return done if out is None else out
     _no_tangents(q, k_pages, v_pages, slopes, out)
-    cache, starts, held = _checked(q, "q", k_pages, v_pages, page_table, kv_lens, q_starts)
+    cache, more, starts, held = _checked(q, "q", k_pages, v_pages, page_table, kv_lens, q_starts, k_scales, v_scales)
     T, H, D = q.shape
     if cache.Hk == 0 or H == 0 or H % cache.Hk or H // cache.Hk > 128:
         raise ValueError(f"flash_b200: the number of heads in q must be a multiple of that in the cache, at most 128 times it, got {H} and {cache.Hk}")
@@ -165,6 +185,7 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_
         prefix = _int32(prefix, (cache.B,), "prefix", q)
     if parents is not None:
         parents = _int32(parents, (T,), "parents", q)
+    more.window, more.parents = _lib.Window(*window), _pointer(parents)
     fill = out is None
     if fill:
         out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
@@ -172,8 +193,8 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_
         if out.shape != q.shape or out.dtype != q.dtype or out.requires_grad or not _regular(out):
             raise ValueError("flash_b200: out must be like q, with a 16-byte aligned base, last stride 1 and other strides that are multiples of 8")
         _same_device(q, out=out)
-        for x, name in ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages")):
-            if _overlap(out, x):
+        for x, name in ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (k_scales, "k_scales"), (v_scales, "v_scales")):
+            if x is not None and _overlap(out, x):
                 raise ValueError(f"flash_b200: out and {name} share memory")
     if T == 0 or cache.B == 0 or cache.pages == 0:
         return out.zero_() if fill else out
@@ -188,7 +209,7 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, q_starts=None, sm_
             size = _workspace_bytes[device.index, D] = size.value
         work = torch.empty(size // 4, dtype=torch.float32, device=device)
         with ops._timed("paged", 2):
-            _lib.check(lib.fa_paged_fwd_more(cache, _lib.PagedMore(_lib.Window(*window), _pointer(parents)), T, H, starts, sm_scale, _scores(softcap, slopes, prefix),
+            _lib.check(lib.fa_paged_fwd_more(cache, more, T, H, starts, sm_scale, _scores(softcap, slopes, prefix),
                                              _rows(q), _rows(out), fill, work.data_ptr(), size, _status_word(device).data_ptr(), _stream()), "fa_paged_fwd_more")
     if not fill:
         _bump(out)
