@@ -264,3 +264,51 @@ def test_the_general_way_through_the_host_gives_the_same(monkeypatch):
     fb.paged_attention(q, *other.args(), _starts(new), window=100, sinks=2, parents=_parents([_tree(40, 5), _tree(5, 6)]), out=out, **other.scales())
     monkeypatch.undo()
     assert torch.equal(out, fb.paged_attention(q, *cache.args(), _starts(new), window=100, sinks=2, parents=_parents([_tree(40, 5), _tree(5, 6)]), **cache.scales()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("changes", [{}, dict(softcap=4.0), dict(slopes=True), dict(softcap=10.0, slopes=True)], ids=["plain", "cap", "bias", "both"])
+@pytest.mark.parametrize("Hk,G,D,page", [(2, 4, 128, 16), (1, 1, 64, 64), (2, 8, 64, 32), (1, 12, 128, 128), (2, 16, 32, 16), (1, 17, 64, 16), (3, 9, 16, 32), (1, 48, 128, 16)])
+def test_single_tokens(Hk, G, D, page, changes, dtype):
+    """Without starts; up to 16 heads a group an instance of its own."""
+    import flash_b200 as fb
+    lens = [1, 700, 0, 128, 129, 5000, 31, 16, 2500]
+    cache = Cache8(lens, Hk, D, page, dtype, 20).fill()
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    q = (torch.randn(len(lens), Hk * G, D, generator=gen, device="cuda") * 1.5).to(dtype)
+    slopes = _slopes(Hk * G) if changes.get("slopes") else None
+    for window, sinks, prefix in ((None, 0, None), (100, 3, None), (1, 0, None), (40, 200, None), (300, 2, (0, 50, 9, 300, 100, 4000, 1, 0, 1000))):
+        keeps = [paged_keep(n, 1, window, sinks, prefix=0 if prefix is None else prefix[b]) for b, n in enumerate(lens)]
+        p = None if prefix is None else torch.tensor(prefix, dtype=torch.int32, device="cuda")
+        got = fb.paged_attention(q, *cache.args(), window=window, sinks=sinks, prefix=p, softcap=changes.get("softcap"), slopes=slopes, **cache.scales())
+        fb.check_status()
+        compare(got, cache, q, [1] * len(lens), keeps, changes.get("softcap"), slopes)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_single_tokens_of_many_sequences_and_as_trees(tree):
+    import flash_b200 as fb
+    lens = [(37 * i) % 900 for i in range(300)]
+    cache = Cache8(lens, 2, 64, 16, BF16, 22).fill()
+    q = torch.randn(300, 8, 64, device="cuda").to(BF16)
+    got = fb.paged_attention(q, *cache.args(), parents=torch.full((300,), -1, dtype=torch.int32, device="cuda") if tree else None, **cache.scales())
+    fb.check_status()
+    compare(got, cache, q, [1] * 300, [paged_keep(n, 1) for n in lens])
+
+
+def test_single_tokens_of_all_sizes_and_not_finite():
+    """Rows of bf16 at their own factors in the instance of single tokens, too; a row that sees a key that is not a number is NaN, and its neighbours are not."""
+    import flash_b200 as fb
+    cache = Cache8([300, 200], 1, 128, 16, BF16, 23, std=0.25)
+    size = torch.tensor([1.0, 3e4, 1e6, 1e-6, 1e30, 1e-30, 0.0, 2e-3], device="cuda").reshape(1, 8, 1)
+    gen = torch.Generator(device="cuda").manual_seed(24)
+    q = torch.randn(2, 8, 128, generator=gen, device="cuda")
+    for scale, most in ((1.0, 1), (1e-6, 1e6), (1e-30, 1e30)):
+        x = (q * torch.where(size <= most, size, 0.0)).to(BF16)
+        for cap in (None, 50.0):
+            got = fb.paged_attention(x, *cache.fill().args(), sm_scale=scale, softcap=cap, **cache.scales())
+            compare(got, cache, x, [1, 1], [paged_keep(300, 1), paged_keep(200, 1)], cap, sm_scale=scale)
+    page, slot = cache.places(0, 100, 101)
+    cache.k_pages.view(torch.uint8)[page, slot, 0, 5] = 127
+    got = fb.paged_attention(x, *cache.args(), **cache.scales())
+    assert got[0].isnan().all() and got[1].isfinite().all()

@@ -109,7 +109,7 @@ int map4(CUtensorMap* out, int dtype, const void* ptr, int D, const int (&extent
     return r == CUDA_SUCCESS ? FA_OK : FA_ERR_TENSORMAP;
 }
 
-// The same over a cache of 8 bits: whole rows of 64 or 128 bytes as they lie, behind one another
+// The same over a cache of 8 bits: whole rows of 64 or 128 bytes, with that swizzle
 int map_bytes(CUtensorMap* out, const void* ptr, int D, const int (&extent)[3], const int64_t (&stride)[3], int rows) {
     const fa::EncodeFn fn = fa::encode_fn();
     if (!fn) return FA_ERR_NO_DRIVER;
@@ -118,7 +118,7 @@ int map_bytes(CUtensorMap* out, const void* ptr, int D, const int (&extent)[3], 
     for (int i = 0; i < 3; ++i) bytes[i] = cuuint64_t(extent[i] > 1 ? stride[i] : D);  // an extent of 1 may carry any stride
     const cuuint32_t b[4] = {D > 64 ? 128u : 64u, 1, cuuint32_t(rows), 1}, step[4] = {1, 1, 1, 1};
     const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, bytes, b, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                          D > 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? FA_OK : FA_ERR_TENSORMAP;
 }
 

@@ -37,12 +37,16 @@ namespace fa {
 // each tile into the fp16 tile that the products read (a row is e4m3 times a power of two from 2^-15 to 2^7, all of whose numbers are fp16's: nothing is rounded), K a tile ahead of V, and hidden
 // rows into zeros. The products are fp16's also where q is bf16: q's rows are brought to fp16, by a power of two where their greatest entry asks for it (their scores take it back in fp32),
 // and P is 2^7 times as large as elsewhere, which brings what fp16 cannot tell from 0 from 2^-25 down to 2^-32 of a row's reference (l and O have the factor alike).
-enum : int { FORM_PLAIN = 0, FORM_MASKED = 1, FORM_E4M3 = 2 };
+// FORM_DIRECT: of 8 bits and single tokens of few heads, as the host can tell: all items are multiplied by warps from the rings, and these have nearly all of shared memory. (Of 64 tokens over 650 MB
+// 150 us with 3 and 2 places of 16 KB, which are all that the tiles of the tensor cores leave.)
+enum : int { FORM_PLAIN = 0, FORM_MASKED = 1, FORM_E4M3 = 2, FORM_DIRECT = 4 };
+
+constexpr int kDirectRows = 16;  // E4M3: of an item, up to which warps multiply it directly
 
 template <int D, int FORM>
 struct PagedSmem {
-    static constexpr bool E4M3 = (FORM & FORM_E4M3) != 0;
-    static constexpr int NS = E4M3 ? (D == 128 ? 1 : 2) : (D == 128) ? 2 : 4;  // depth of the K ring and of the V ring
+    static constexpr bool E4M3 = (FORM & FORM_E4M3) != 0, DIRECT = (FORM & FORM_DIRECT) != 0;
+    static constexpr int NS = DIRECT ? 0 : E4M3 ? (D == 128 ? 1 : 2) : (D == 128) ? 2 : 4;  // depth of the K ring and of the V ring
     static constexpr int NQ = 2;                   // item slots
     // TMEM columns as in the forward kernel
     static constexpr bool POWN = D == 128;
@@ -53,13 +57,16 @@ struct PagedSmem {
     static constexpr int TILE = kBlk * D * 2;
     static constexpr int BOX = kBlk * 64 * 2;
     static constexpr int NBOX = D / 64;
+    static constexpr int QBOX = DIRECT ? 32 * 128 : BOX, QTILE = QBOX * NBOX;
     static constexpr int off_q = 0;  // NQ Q tiles
-    static constexpr int off_k = NQ * TILE;
+    static constexpr int off_k = NQ * QTILE;
     static constexpr int off_v = off_k + NS * TILE;
     // E4M3: rings of rows as they are, and of their scales; the factor of each row's scores
     static constexpr int RAW = E4M3 ? kBlk * D : 0;
-    static constexpr int NRK = !E4M3 ? 0 : D == 128 ? 3 : 5, NRV = !E4M3 ? 0 : D == 128 ? 2 : 5;
-    static constexpr int off_raw_k = off_v + NS * TILE, off_raw_v = off_raw_k + NRK * RAW;
+    static constexpr int NRK = !E4M3 ? 0 : DIRECT ? (D == 128 ? 4 : 8) : D == 128 ? 3 : 5, NRV = !E4M3 ? 0 : DIRECT ? NRK : D == 128 ? 2 : 5;
+    static constexpr int SUMS = 8 * kDirectRows * D * 4, off_sums = off_k;  // E4M3: what the warps leave of O; K's and V's tiles have the place, or nobody else
+    static_assert(DIRECT || !E4M3 || SUMS <= 2 * NS * TILE, "room for the sums");
+    static constexpr int off_raw_k = DIRECT ? off_sums + SUMS : off_v + NS * TILE, off_raw_v = off_raw_k + NRK * RAW;
     static constexpr int off_ml = off_raw_v + NRV * RAW;         // float [NQ][2 groups][m, l][128]
     static constexpr int off_info = off_ml + NQ * 4 * kBlk * 4;  // int32 [NQ][16]: see I_*
     static constexpr int off_scale_k = off_info + NQ * 64, off_scale_v = off_scale_k + NRK * kBlk;
@@ -67,8 +74,8 @@ struct PagedSmem {
     static constexpr int off_plan = off_factor + (E4M3 ? NQ * kBlk * 4 : 0);
     static constexpr int off_bar = off_plan + int(sizeof(PagedPlan));
     // item_full[NQ] item_empty[NQ] q_full[NQ] ml_full[NQ] staged k_full[NS] k_empty[NS] v_full[NS] v_empty[NS]
-    // s_full[4] s_free[2] p_full[NP] pv_done[NP] o_full[2] o_free[2]; E4M3: raw_k_full[NRK] raw_k_empty[NRK] raw_v_full[NRV] raw_v_empty[NRV] q_ready[NQ]
-    static constexpr int n_common = 4 * NQ + 1 + 4 * NS + 6 + 2 * NP + 4, n_bar = n_common + 2 * NRK + 2 * NRV + (E4M3 ? NQ : 0);
+    // s_full[4] s_free[2] p_full[NP] pv_done[NP] o_full[2] o_free[2]; E4M3: raw_k_full[NRK] raw_k_empty[NRK] raw_v_full[NRV] raw_v_empty[NRV] q_ready[NQ] sums_free
+    static constexpr int n_common = 4 * NQ + 1 + 4 * NS + 6 + 2 * NP + 4, n_bar = n_common + 2 * NRK + 2 * NRV + (E4M3 ? NQ + 1 : 0);
     static constexpr int off_misc = off_bar + n_bar * 8;  // tmem slot, abort flag
     static constexpr int total = off_misc + 16;
     static_assert(off_plan % 8 == 0 && off_bar % 8 == 0, "alignment");
@@ -79,7 +86,8 @@ struct PagedSmem {
 };
 template <int D, int FORM>
 constexpr bool kPagedFits = PagedSmem<D, FORM>::total <= 232448 && PagedSmem<D, FORM>::total > 116736;  // the budget, and no other block beside it on the SM
-static_assert(kPagedFits<128, FORM_PLAIN> && kPagedFits<64, FORM_PLAIN> && kPagedFits<128, FORM_E4M3> && kPagedFits<64, FORM_E4M3>, "shared memory");
+static_assert(kPagedFits<128, FORM_PLAIN> && kPagedFits<64, FORM_PLAIN> && kPagedFits<128, FORM_E4M3> && kPagedFits<64, FORM_E4M3> &&
+              kPagedFits<128, FORM_E4M3 | FORM_DIRECT> && kPagedFits<64, FORM_E4M3 | FORM_DIRECT>, "shared memory");
 
 // What an item's slot says: number of its key tiles, the first one, whether there is an item (1, or -1: no more), kv head, first row of its tokens in
 // q and out, how many of them, position of the first one, the sequence's length, its prefix, the sequence, slot of the workspace (-1: straight to out)
@@ -87,13 +95,35 @@ static_assert(kPagedFits<128, FORM_PLAIN> && kPagedFits<64, FORM_PLAIN> && kPage
 // length); first row of the sequence
 enum : int { I_TILES = 0, I_LO, I_MORE, I_HEAD, I_ROW, I_TOKENS, I_POS, I_LEN, I_FRONT, I_SEQ, I_PART, I_BORDER, I_SKIP, I_BASE, I_FIRST };
 
+// E4M3: where 16 numbers of a row lie in a tile of a ring (the 128- or 64-byte swizzle of the copy: lanes of neighbouring rows and of every other row find different banks)
+template <int D>
+__device__ __forceinline__ int raw_place(int row, int part) { return row * D + ((part ^ (D == 128 ? row & 7 : row >> 1 & 3)) << 4); }
+// Where four columns of a row of a warp's O lie, so that those who write together, and who read together, have eight different 16-byte places
+template <int D>
+__device__ __forceinline__ int sums_place(int row, int four) { return four ^ (D == 128 ? row >> 1 & 3 : (row >> 1 & 1) | (row >> 2 & 1) << 2); }
+// A row's scale, from its exponent biased by 127, as two numbers of fp16 and in fp32
+__device__ __forceinline__ uint32_t scale_to_h2(uint32_t biased) {
+    const int e = min(max(int(biased), kScaleLeast), kScaleMost) - kScaleLeast;
+    const uint32_t one = e > 0 ? uint32_t(e) << 10 : 0x200u;  // 2^(e - 15)
+    return one | one << 16;
+}
+__device__ __forceinline__ float scale_to_float(uint32_t biased) { return __uint_as_float(uint32_t(min(max(int(biased), kScaleLeast), kScaleMost)) << 23); }
+// The power of two that a row of bf16 is divided by on its way to fp16; `most`: the bits of its greatest entry without the sign. (0, infinities and NaN go as they are.)
+__device__ __forceinline__ int query_shift(uint32_t most) {
+    const int exponent = int(most >> 7) - 127;
+    return most == 0 || most >= 0x7f80u || (exponent >= -8 && exponent < 15) ? 0 : min(max(exponent, -120), 120);
+}
+
 template <int D, bool BF16, int KIND, int FORM>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmN, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const PagedParams p) {
     using S = PagedSmem<D, FORM>;
-    constexpr bool SCORED = score_changed(KIND), MASKED = (FORM & FORM_MASKED) != 0, E4M3 = S::E4M3;
+    constexpr bool SCORED = score_changed(KIND), MASKED = (FORM & FORM_MASKED) != 0, E4M3 = S::E4M3, DIRECT = S::DIRECT;
     constexpr bool PBF16 = BF16 && !E4M3;           // the products' type
+    // (spilled registers come back from L2 here: shared memory leaves L1 nothing)
+    constexpr int kSoftmaxRegs = DIRECT ? 192 : E4M3 ? 176 : kFwdSoftmaxRegs, kEpilogueRegs = DIRECT ? 64 : E4M3 ? 104 : kFwdEpilogueRegs, kServiceRegs = DIRECT ? 64 : E4M3 ? 56 : kFwdServiceRegs;
+    static_assert(256 * kSoftmaxRegs + 128 * (kEpilogueRegs + kServiceRegs) <= kFwdThreads * 128, "registers at launch");
     constexpr float kRaised = E4M3 ? 7.f : 0.f;     // log2 of what P is multiplied by
     constexpr int NS = S::NS, NQ = S::NQ, NP = S::NP;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -109,13 +139,13 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                   B_KEMPTY = B_KFULL + NS, B_VFULL = B_KEMPTY + NS, B_VEMPTY = B_VFULL + NS, B_SFULL = B_VEMPTY + NS,
                   B_SFREE = B_SFULL + 4, B_PFULL = B_SFREE + 2, B_PVDONE = B_PFULL + NP, B_OFULL = B_PVDONE + NP, B_OFREE = B_OFULL + 2;
     static_assert(B_OFREE + 2 == S::n_common, "barriers");
-    constexpr int B_RAWK = S::n_common, B_RAWKEMPTY = B_RAWK + S::NRK, B_RAWV = B_RAWKEMPTY + S::NRK, B_RAWVEMPTY = B_RAWV + S::NRV, B_QREADY = B_RAWVEMPTY + S::NRV;
+    constexpr int B_RAWK = S::n_common, B_RAWKEMPTY = B_RAWK + S::NRK, B_RAWV = B_RAWKEMPTY + S::NRK, B_RAWVEMPTY = B_RAWV + S::NRV, B_QREADY = B_RAWVEMPTY + S::NRV, B_SUMSFREE = B_QREADY + NQ;
     Abort ab{misc + 1, p.status, p.wait_limit};
 
     if (tid == 0) {
         for (int s = 0; s < NQ; ++s) {
             mbar_init(BAR(B_ITEMFULL + s), 1);
-            mbar_init(BAR(B_ITEMEMPTY + s), 15);  // V producer, two MMA issuers, eight softmax warps, four epilogue warps
+            mbar_init(BAR(B_ITEMEMPTY + s), DIRECT ? 13 : 15);  // V producer, two MMA issuers (where there are), eight softmax warps, four epilogue warps
             mbar_init(BAR(B_QFULL + s), 1);
             mbar_init(BAR(B_MLFULL + s), 8);
         }
@@ -135,6 +165,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 mbar_init(BAR(B_RAWVEMPTY + s), 4);
             }
             for (int s = 0; s < NQ; ++s) mbar_init(BAR(B_QREADY + s), 4);
+            mbar_init(BAR(B_SUMSFREE), 4);
         }
         mbar_init(BAR(B_STAGED), 4);
         for (int s = 0; s < 4; ++s) mbar_init(BAR(B_SFULL + s), 1);
@@ -150,10 +181,10 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         fence_mbar_init();
     }
     // Rows without a query are multiplied all the same: as zeros, until another item's rows have been there
-    for (int i = tid; i < NQ * S::TILE / 16; i += kFwdThreads) reinterpret_cast<uint4*>(smem + S::off_q)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < NQ * S::QTILE / 16; i += kFwdThreads) reinterpret_cast<uint4*>(smem + S::off_q)[i] = make_uint4(0, 0, 0, 0);
     fence_proxy_async();
     wait_prerequisites();
-    if (warp == 13) {
+    if (!DIRECT && warp == 13) {
         take_tensor_memory(sbase + S::off_misc);
     }
     if (tid == 0) misc[1] = (status_is_fatal(*reinterpret_cast<volatile int*>(p.status)) || (sbase & 1023u) != 0) ? 1 : 0;
@@ -161,7 +192,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     __syncthreads();
     tc_fence_after();
     launch_dependents();
-    const uint32_t tmem = uint32_t(misc[0]);
+    const uint32_t tmem = DIRECT ? 0u : uint32_t(misc[0]);
     const bool aborted = misc[1] != 0;
     uint16_t* const out = static_cast<uint16_t*>(p.out);
     // (aborted: an earlier launch ran into a time-out that the host has not yet cleared. The second kernel fills the output.)
@@ -171,16 +202,74 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         paged_plan<kFwdThreads, MASKED>(p, plan, int(gridDim.x));
     }
     const int worker = int(blockIdx.x);
+    // E4M3: items of so few rows that warps multiply them with what they read of the rings
+    auto is_direct = [&](int tokens) { return DIRECT || (E4M3 && tokens * p.G <= kDirectRows); };
     // what a row's scores are multiplied by (a factor must bring it neither to 0 nor beyond fp32: a maximum of minus infinity is multiplied, too)
     auto scale_of = [&](float factor) { return SCORED ? 1.f : E4M3 && BF16 ? fminf(fmaxf(p.scale_log2 * factor, 1.2e-38f), 3e38f) : p.scale_log2; };
     // the key block that is an item's x-th
     auto key_block = [](int x, int border, int skip) { return MASKED && x >= border ? x + skip : x; };
 
-    auto sQ = [&](int s) { return sbase + S::off_q + uint32_t(s) * S::TILE; };
+    auto sQ = [&](int s) { return sbase + S::off_q + uint32_t(s) * S::QTILE; };
     auto sK = [&](int s) { return sbase + S::off_k + uint32_t(s) * S::TILE; };
     auto sV = [&](int s) { return sbase + S::off_v + uint32_t(s) * S::TILE; };
+    // E4M3: the g-th tile of K or V (the rings' raw_g-th), rows of D numbers in e4m3 to 64-column boxes of fp16 with the swizzle that the products read, by four warps. A thread takes 16
+    // numbers at a time. In a loop, and in one place of the code for K and one for V: with the loop unrolled and V's in three places, whose code the softmax groups fetch beside their own, warps
+    // stood without an instruction more than anything else (five chunks and tokens over 131 MB 525 us).
+    auto unpack_tile = [&](auto values, int g, int raw_g, int k0, int seen, int early, int low) {
+        constexpr bool V = decltype(values)::value;
+        const int r = tid & 127;
+        constexpr int R = V ? S::NRV : S::NRK, kThreadsARow = D / 16, kRows = kBlk / kThreadsARow;  // kRows: that the group takes together
+        const int raw = raw_g % R, st = g % NS;
+        if (!mbar_wait_warp(BAR((V ? B_RAWV : B_RAWK) + raw), (raw_g / R) & 1, ab, ST_WAIT_TIMEOUT + 20)) return false;
+        if (g >= NS && !mbar_wait_warp(BAR((V ? B_VEMPTY : B_KEMPTY) + st), (g / NS - 1) & 1, ab, ST_WAIT_TIMEOUT + 21)) return false;
+        const int part = r % kThreadsARow, row0 = r / kThreadsARow;
+        const uint8_t* from = smem + (V ? S::off_raw_v : S::off_raw_k) + raw * S::RAW + raw_place<D>(row0, part);  // (the rows that a thread takes have one swizzle)
+        const uint8_t* scales = smem + (V ? S::off_scale_v : S::off_scale_k) + raw * kBlk + row0;
+        uint8_t* to = smem + (V ? S::off_v : S::off_k) + st * S::TILE + (part >> 2) * S::BOX + row0 * 128;
+        const int c0 = ((2 * (part & 3)) ^ (row0 & 7)) << 4, c1 = c0 ^ 16;
+        static_assert(kRows % 8 == 0, "one swizzle");
+        const bool all = k0 + kBlk <= seen && (k0 + kBlk <= early || k0 >= low);
+        int key = k0 + row0;
+#pragma unroll 1
+        for (int i = 0; i < kBlk / (2 * kRows); ++i) {
+            uint4 x[2];
+            uint32_t scale[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                x[j] = *reinterpret_cast<const uint4*>(from + j * kRows * D);
+                scale[j] = scales[j * kRows];
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t two = scale_to_h2(scale[j]);
+                uint32_t y[8];
+                unpack_e4m3x4(x[j].x, y[0], y[1]);
+                unpack_e4m3x4(x[j].y, y[2], y[3]);
+                unpack_e4m3x4(x[j].z, y[4], y[5]);
+                unpack_e4m3x4(x[j].w, y[6], y[7]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = mul_h2(y[e], two);
+                if (!all) {
+                    const int at = key + j * kRows;
+                    const uint32_t real = at < seen && (at < early || at >= low) ? ~0u : 0u;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] &= real;
+                }
+                *reinterpret_cast<uint4*>(to + j * kRows * 128 + c0) = make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(to + j * kRows * 128 + c1) = make_uint4(y[4], y[5], y[6], y[7]);
+            }
+            from += 2 * kRows * D;
+            scales += 2 * kRows;
+            to += 2 * kRows * 128;
+            key += 2 * kRows;
+        }
+        mbar_arrive_warp(BAR((V ? B_RAWVEMPTY : B_RAWKEMPTY) + raw), lane);
+        fence_proxy_async();
+        mbar_arrive_warp(BAR((V ? B_VFULL : B_KFULL) + st), lane);
+        return true;
+    };
     if (warp >= 12) {
-        setmaxnreg_dec<kFwdServiceRegs>();
+        setmaxnreg_dec<kServiceRegs>();
         // K and V are loaded by a warp each. (By one, 16 to 32 loads a tile with small pages, and the step from one tile's to the next, took longer than a
         // tile: one chunk of 500 tokens behind 7500, 32 / 8 heads of 128, pages of 128 | 16: 105 | 116 us.)
         const int rows = p.page < kBlk ? p.page : kBlk, log2_rows = p.page < kBlk ? p.log2_page : 7;  // of a box
@@ -261,7 +350,10 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
                     __syncwarp();
                     // (an item's slot is given away when its O has left, so that Q has been read, too)
-                    if (tokens <= p.narrow) {  // four times the same rows
+                    if (is_direct(tokens)) {
+                        mbar_expect_tx_elect(BAR(B_QFULL + s), uint32_t(p.narrow * p.G) * 128u * S::NBOX);
+                        for (int x = 0; x < S::NBOX; ++x) tma_load_4d_elect(sQ(s) + x * S::QBOX, &tmN, BAR(B_QFULL + s), x * 64, 0, hk, tok0);
+                    } else if (tokens <= p.narrow) {  // four times the same rows
                         mbar_expect_tx_elect(BAR(B_QFULL + s), uint32_t(p.narrow * p.G) * 512u * S::NBOX);
                         for (int i = 0; i < 4 * S::NBOX; ++i)
                             tma_load_4d_elect(sQ(s) + (i >> 2) * S::BOX + (i & 3) * 4096, &tmN, BAR(B_QFULL + s), (i >> 2) * 64, 0, hk, tok0);
@@ -333,7 +425,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 if (lane == 0) mbar_arrive(BAR(B_ITEMEMPTY + s));
                 __syncwarp();
             }
-        } else {
+        } else if constexpr (!DIRECT) {
             // ------------------------------ MMA issuers ------------------------------
             //   warp 13: P*V(g) when P(g) is there; warp 15: S(g) when its buffer is free
             const uint32_t utmem = uniform(int(tmem));
@@ -347,7 +439,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 const int s = k % NQ, use = k / NQ;
                 ok = mbar_wait_warp(BAR(B_ITEMFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 12);
                 if (!ok) break;
-                const int T = uniform(info[16 * s + I_TILES]);
+                const int T = is_direct(uniform(info[16 * s + I_TOKENS])) ? 0 : uniform(info[16 * s + I_TILES]);
                 if (uniform(info[16 * s + I_MORE]) < 0) break;
                 if (warp == 15) {
                     if (T > 0) ok = mbar_wait_warp(BAR((E4M3 && BF16 ? B_QREADY : B_QFULL) + s), use & 1, ab, ST_WAIT_TIMEOUT + 3);
@@ -401,51 +493,14 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         __syncwarp();
     } else if (warp >= 8) {
         // ------------------------------ epilogue group ------------------------------
-        setmaxnreg_dec<kFwdEpilogueRegs>();
+        setmaxnreg_dec<kEpilogueRegs>();
         const int r = tid & 127;
         const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
         const int tok_wide = r / p.G, tok_narrow = lane / p.G;
-        // E4M3: the g-th tile of K or V, rows of D numbers in e4m3 to 64-column boxes of fp16 with the swizzle that the products read. A thread takes 16 numbers at a time; those
-        // that write together have eight different 16-byte places of the 128 bytes.
-        auto unpack_tile = [&](auto values, int g, int k0, int seen, int early, int low) {
-            constexpr bool V = decltype(values)::value;
-            constexpr int R = V ? S::NRV : S::NRK, kThreadsARow = D / 16, kRows = kBlk / kThreadsARow;  // rows that the group takes together
-            const int raw = g % R, st = g % NS;
-            if (!mbar_wait_warp(BAR((V ? B_RAWV : B_RAWK) + raw), (g / R) & 1, ab, ST_WAIT_TIMEOUT + 20)) return false;
-            if (g >= NS && !mbar_wait_warp(BAR((V ? B_VEMPTY : B_KEMPTY) + st), (g / NS - 1) & 1, ab, ST_WAIT_TIMEOUT + 21)) return false;
-            const uint8_t* const from = smem + (V ? S::off_raw_v : S::off_raw_k) + raw * S::RAW;
-            const uint8_t* const scales = smem + (V ? S::off_scale_v : S::off_scale_k) + raw * kBlk;
-            uint8_t* const to = smem + (V ? S::off_v : S::off_k) + st * S::TILE;
-            const int part = r % kThreadsARow, row0 = r / kThreadsARow, box = part >> 2, swap = box & 1;
-            const bool all = k0 + kBlk <= seen && (k0 + kBlk <= early || k0 >= low);
-#pragma unroll 4
-            for (int i = 0; i < kBlk / kRows; ++i) {
-                const int row = row0 + i * kRows, key = k0 + row;
-                const uint4 x = *reinterpret_cast<const uint4*>(from + row * D + part * 16);
-                const int e = min(max(int(scales[row]), kScaleLeast), kScaleMost) - kScaleLeast;
-                const uint32_t one = e > 0 ? uint32_t(e) << 10 : 0x200u, scale = one | one << 16;  // 2^(e - 15) in fp16
-                uint32_t y[8];
-                unpack_e4m3x4(x.x, y[0], y[1]);
-                unpack_e4m3x4(x.y, y[2], y[3]);
-                unpack_e4m3x4(x.z, y[4], y[5]);
-                unpack_e4m3x4(x.w, y[6], y[7]);
-                const bool real = all || (key < seen && (key < early || key >= low));
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = real ? mul_h2(y[j], scale) : 0u;
-                uint8_t* const line = to + box * S::BOX + row * 128;
-                const int c0 = 2 * (part & 3) + swap, c1 = c0 ^ 1;
-                *reinterpret_cast<uint4*>(line + ((c0 ^ (row & 7)) << 4)) = swap ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
-                *reinterpret_cast<uint4*>(line + ((c1 ^ (row & 7)) << 4)) = swap ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
-            }
-            fence_proxy_async();
-            mbar_arrive_warp(BAR((V ? B_RAWVEMPTY : B_RAWKEMPTY) + raw), lane);
-            if (lane == 0) mbar_arrive(BAR((V ? B_VFULL : B_KFULL) + st));
-            return true;
-        };
         // E4M3 of bf16: this thread's row of Q to fp16 in place, times a power of two where its greatest entry is beyond fp16 or so small that the others would lose bits; what the
         // row's scores are to be multiplied by.
         auto query_to_fp16 = [&](int s) {
-            uint8_t* const row = smem + S::off_q + s * S::TILE + r * 128;
+            uint8_t* const row = smem + S::off_q + s * S::QTILE + r * 128;
             auto at = [&](int i) { return reinterpret_cast<uint4*>(row + (i >> 3) * S::BOX + (((i + r) & 7) << 4)); };  // (any order will do: eight lanes at eight places)
             uint32_t most = 0;  // bf16 numbers without their sign go by size
 #pragma unroll 4
@@ -455,8 +510,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
                 for (int j = 0; j < 4; ++j) most = max(most, max(w[j] & 0x7fffu, w[j] >> 16 & 0x7fffu));
             }
-            // (0, infinities and NaN go as they are)
-            const int exponent = int(most >> 7) - 127, shift = most == 0 || most >= 0x7f80u || (exponent >= -8 && exponent < 15) ? 0 : min(max(exponent, -120), 120);
+            const int shift = query_shift(most);
             const float back = __uint_as_float(uint32_t(127 + shift) << 23), there = __uint_as_float(uint32_t(127 - shift) << 23);
 #pragma unroll 4
             for (int i = 0; i < D / 8; ++i) {
@@ -466,6 +520,46 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 *x = make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
             }
             return back;
+        };
+        // E4M3: the output of an item that eight warps have multiplied directly, or a piece of it. Each has left its maximum and sum of the rows in `ml` and its O, [16 rows][D] in fp32; this
+        // thread has D / 8 neighbouring columns of one row.
+        auto sum_warps = [&](int s, int T, int part, int row0, int hk, int tokens) {
+            constexpr int kTiles = D / 8;
+            const int row = 2 * (r >> 1 & 3) + (r >> 5 & 1) + 8 * (r >> 6), n = 2 * (r >> 3 & 3) + (r & 1), tok = row / p.G;
+            if (row >= tokens * p.G || misc[1] != 0) return;
+            const float* const ml = reinterpret_cast<const float*>(smem + S::off_ml) + s * (4 * kBlk) + row;
+            auto at = [](int q) { return (q >> 2) * (2 * kBlk) + (q & 3) * 32; };
+            float mt = -INFINITY, lt = 0.f, acc[kTiles] = {};
+#pragma unroll
+            for (int q = 0; q < 8; ++q) mt = fmaxf(mt, ml[at(q)]);
+#pragma unroll 1
+            for (int q = 0; q < 8; ++q) {
+                const float m = ml[at(q)], a = m == -INFINITY ? 0.f : fast_exp2(m - mt);
+                lt += ml[at(q) + kBlk] * (m == -INFINITY ? 1.f : a);  // (a NaN that a row without a maximum has is not lost)
+                if (a == 0.f) continue;
+                const float4* const o = reinterpret_cast<const float4*>(smem + S::off_sums) + (q * kDirectRows + row) * (D / 4);
+#pragma unroll
+                for (int j = 0; j < kTiles; j += 4) {
+                    const float4 x = o[sums_place<D>(row, (n * kTiles + j) / 4)];
+                    acc[j] = fmaf(a, x.x, acc[j]);
+                    acc[j + 1] = fmaf(a, x.y, acc[j + 1]);
+                    acc[j + 2] = fmaf(a, x.z, acc[j + 2]);
+                    acc[j + 3] = fmaf(a, x.w, acc[j + 3]);
+                }
+            }
+            const float inv = lt > 0.f ? 1.0f / lt : lt == lt ? 0.f : lt;
+            if (part >= 0) {
+                if (n == 0) p.part_lse[int64_t(part) * kBlk + row] = lt > 0.f ? mt + log2f(lt) : lt == lt ? -INFINITY : lt;
+                float4* const to = reinterpret_cast<float4*>(p.part_o + (int64_t(part) * kBlk + row) * D + n * kTiles);
+#pragma unroll
+                for (int j = 0; j < kTiles; j += 4) to[j / 4] = make_float4(acc[j] * inv, acc[j + 1] * inv, acc[j + 2] * inv, acc[j + 3] * inv);
+            } else if (n * kTiles < p.D) {
+                uint4* const to = reinterpret_cast<uint4*>(out + int64_t(row0 + tok) * p.out_t + int64_t(hk * p.G + row - tok * p.G) * p.out_h + n * kTiles);
+#pragma unroll
+                for (int j = 0; j < kTiles; j += 8)
+                    to[j / 8] = make_uint4(pack2<BF16>(acc[j] * inv, acc[j + 1] * inv), pack2<BF16>(acc[j + 2] * inv, acc[j + 3] * inv),
+                                           pack2<BF16>(acc[j + 4] * inv, acc[j + 5] * inv), pack2<BF16>(acc[j + 6] * inv, acc[j + 7] * inv));
+            }
         };
         // of a narrow item's sums: this thread adds up four columns of row r / 4
         const int row_sum = r >> 2, tok_sum = row_sum / p.G;
@@ -482,6 +576,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
         int G = 0;           // tiles of all earlier items
         int n0 = 0, n1 = 0;  // items in which the chains of group 0 and 1 had tiles
+        int raw_g = 0;       // E4M3: tiles of all earlier items, those counted that are multiplied directly
         for (int k = 0; alive; ++k) {
             const int s = k % NQ, use = k / NQ;
             alive = mbar_wait_warp(BAR(B_ITEMFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 12);
@@ -511,6 +606,22 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
             float factor = 1.f;  // E4M3 of bf16: of this row's scores
             if constexpr (E4M3) {
+                if (is_direct(tokens)) {
+                    // the products are none of this group's: it adds up what the eight warps have (sum_warps)
+                    if constexpr (BF16) mbar_arrive_warp(BAR(B_QREADY + s), lane);
+                    mbar_arrive_warp(BAR(B_SUMSFREE), lane);  // (what K's and V's tiles are made in serves for that, and this group is done with the item before)
+                    const Abort item{ab.flag, ab.status, ab.limit * (T + 1)};
+                    alive = mbar_wait_warp(BAR(B_MLFULL + s), use & 1, item, ST_WAIT_TIMEOUT + 16);
+                    if (!alive) break;
+                    sum_warps(s, T, part, it[I_ROW], hk, tokens);
+                    raw_g += T;
+                    // (all of the group before any of it may make a tile there)
+                    mbar_arrive_warp(BAR(B_STAGED), lane);
+                    alive = mbar_wait_warp(BAR(B_STAGED), staged++ & 1, ab, ST_WAIT_TIMEOUT + 18);
+                    if (!alive) break;
+                    if (lane == 0) mbar_arrive(BAR(B_ITEMEMPTY + s));
+                    continue;
+                }
                 if constexpr (BF16) {
                     alive = mbar_wait_warp(BAR(B_QFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 17);
                     if (!alive) break;
@@ -522,10 +633,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 const int pos0 = it[I_POS], len = it[I_LEN], front = it[I_FRONT], lo = it[I_LO], border = it[I_BORDER], skip = it[I_SKIP];
                 const int seen = min(max(pos0 + tokens, front), len), early = p.window > 0 ? max(front, p.sinks) : len;
                 const int low = p.window > 0 ? (it[I_BASE] < len ? it[I_BASE] : pos0) - p.window + 1 : 0;
-                for (int t = 0; t <= T && alive; ++t) {
-                    if (t < T) alive = unpack_tile(std::false_type{}, G + t, key_block(lo + t, border, skip) * kBlk, seen, early, low);
-                    if (t > 0 && alive) alive = unpack_tile(std::true_type{}, G + t - 1, key_block(lo + t - 1, border, skip) * kBlk, seen, early, low);
-                }
+                for (int t = 0; t < T && alive; ++t) alive = unpack_tile(std::false_type{}, G + t, raw_g + t, key_block(lo + t, border, skip) * kBlk, seen, early, low);
+                raw_g += T;
                 if (!alive) break;
             }
             // the only wait here that lasts as long as an item: it allows each of the tiles what another wait may last
@@ -570,7 +679,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             uint16_t* const row_out = narrow ? out + int64_t(it[I_ROW] + tok_sum) * p.out_t + int64_t(hk * p.G + row_sum - tok_sum * p.G) * p.out_h
                                              : out + int64_t(row) * p.out_t + int64_t(hk * p.G + g_row) * p.out_h;
             const bool store_sum = tok_sum < tokens && misc[1] == 0;
-            float* const stage = reinterpret_cast<float*>(smem + S::off_q + s * S::TILE);  // (Q has been read) [2][4 warps][32 rows][16]
+            float* const stage = reinterpret_cast<float*>(smem + S::off_q + s * S::QTILE);  // (Q has been read) [2][4 warps][32 rows][16]
             const uint32_t tO0 = tmem + lane_base + uint32_t(S::tmem_o + we * D), tO1 = tmem + lane_base + uint32_t(S::tmem_o + (we ^ 1) * D);
 #pragma unroll 1
             for (int q = 0; q < D / 16; ++q) {
@@ -638,7 +747,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (lane == 0) mbar_arrive(BAR(B_ITEMEMPTY + s));
         }
     } else {
-        setmaxnreg_inc<kFwdSoftmaxRegs>();
+        setmaxnreg_inc<kSoftmaxRegs>();
         // ------------------------------ softmax groups ------------------------------
         const int w = warp >> 2;  // group
         const int r = tid & 127;  // row inside the tile
@@ -665,6 +774,21 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             fence_proxy_async();
             return true;
         };
+        // Which of the 32 keys from x0 on a row sees.
+        auto keys_seen = [&](int x0, int last, int low, int early, int base, bool tree, const uint32_t* masks) {
+            uint32_t keep = first_bits(last - x0 + 1);
+            if constexpr (MASKED) {
+                if (p.window > 0) keep &= ~hidden_bits(low - x0, early - x0);
+                if (tree && x0 + 31 >= base) {
+                    const int i = x0 - base, word = i >> 5;  // (below 0 where the cached text ends among the 32)
+                    const uint32_t lo_bits = word >= 0 && word < S::kMaskWords ? masks[word * kBlk] : 0u;
+                    const uint32_t hi_bits = word + 1 >= 0 && word + 1 < S::kMaskWords ? masks[(word + 1) * kBlk] : 0u;
+                    const uint32_t text = first_bits(base - x0);
+                    keep = (keep & text) | (__funnelshift_r(lo_bits, hi_bits, i) & ~text);
+                }
+            }
+            return keep;
+        };
         auto rescale = [&](float alpha) {
 #pragma unroll 1
             for (int q = 0; q < D / 16; ++q) {
@@ -677,7 +801,9 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
             tc_wait_st();
         };
-        int G = 0;  // tiles of all earlier items
+        int G = 0;      // tiles of all earlier items
+        int raw_g = 0;  // E4M3: those counted that are multiplied directly
+        int direct = 0; // E4M3: items of that kind
         for (int k = 0; alive; ++k) {
             const int s = k % NQ, use = k / NQ;
             alive = mbar_wait_warp(BAR(B_ITEMFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 12);
@@ -735,30 +861,297 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     low_last = pos0 + tokens - p.window;
                 }
             }
-            // Which of the 32 keys from x0 on the row sees.
-            auto sees = [&](int x0) {
-                uint32_t keep = first_bits(last - x0 + 1);
-                if constexpr (MASKED) {
-                    if (p.window > 0) keep &= ~hidden_bits(low - x0, early - x0);
-                    if (tree && x0 + 31 >= base) {
-                        const int i = x0 - base, word = i >> 5;  // (below 0 where the cached text ends among the 32)
-                        const uint32_t lo_bits = word >= 0 && word < S::kMaskWords ? masks[word * kBlk] : 0u;
-                        const uint32_t hi_bits = word + 1 >= 0 && word + 1 < S::kMaskWords ? masks[(word + 1) * kBlk] : 0u;
-                        const uint32_t text = first_bits(base - x0);
-                        keep = (keep & text) | (__funnelshift_r(lo_bits, hi_bits, i) & ~text);
-                    }
-                }
-                return keep;
-            };
+            auto sees = [&](int x0) { return keys_seen(x0, last, low, early, base, tree, masks); };
             float slope = 0.f;
             if constexpr (SCORED) {
                 if (p.score.slopes) slope = p.score.slopes[int64_t(it[I_HEAD]) * p.G + g_row] * kScoreLog2e;
+            }
+            const int item_raw = raw_g;
+            raw_g += T;
+            // E4M3: V's tile of a group's own tile of keys
+            auto unpack_values = [&](int t) {
+                if constexpr (E4M3 && !DIRECT)
+                    return unpack_tile(std::true_type{}, G + t, item_raw + t, key_block(lo + t, border, skip) * kBlk, seen, p.window > 0 ? early : len, low_first);
+                return true;
+            };
+            if constexpr (E4M3) {
+                if (is_direct(tokens)) {
+                    // ------------------------------ few rows: by warps, from the rings ------------------------------
+                    // A tile belongs to one group, and each of its four warps has 32 of the keys, with a maximum, sums and an O of its own. mma.sync, with what there is much of as M: S^T = K Q^T, 16
+                    // keys by 8 rows, and O^T = V^T P^T, 16 columns by 8 rows. What a thread multiplies in a step along the head dim, and which columns of V its tiles have, is a matter of order
+                    // alone, so that it takes neighbouring bytes: of K's rows 4 a step, of V's the D / 8 of each of its keys. K's scales go to the scores, V's to the numbers, which fp16 holds exactly.
+                    // A warp has a tile's bytes in registers before it begins, and has given the rings' places back; nothing else waits. Clocks a tile of 128 keys of 128: HBM's share of an SM 1400,
+                    // conversions 450 of the ALU, products 256. 64 tokens, 32 / 8 heads of 128, over 650 MB, us: by the tensor memory's way 345; rows as M, 16 keys a warp of every tile 187; rows as
+                    // N 154.
+                    alive = mbar_wait_warp(BAR(B_QFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 3);
+                    if (!alive) break;
+                    __syncwarp();  // (a row's mask is its lane's)
+                    const int row0 = valid ? last : -1;
+                    auto multiply = [&](auto tiles) {
+                        constexpr int NT = decltype(tiles)::value;          // of 8 rows
+                        constexpr int U = NT == 1 ? 2 : 1;                  // times 16 keys at once (the registers do not do for two of both)
+                        constexpr int kSteps = D / 16, kCols = D / 16;      // along the head dim for S^T; of 16 columns of O
+                        const int g8 = lane >> 2, c4 = lane & 3, own_keys = 32 * (warp & 3);  // own_keys: the first of the warp's in a tile
+                        uint32_t qb[NT][kSteps][2];
+                        float scale[NT][2], back[NT][2];  // of the scores of rows 8 n + 2 c4, + 1: to the log2 domain, and to what they are
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            float most = 0.f, own = 1.f;
+                            const int row = g8 + 8 * n;
+#pragma unroll
+                            for (int i = 0; i < kSteps; ++i) {
+                                const int d0 = c4 * (D / 4) + 4 * i;
+                                const uint2 x = *reinterpret_cast<const uint2*>(smem + S::off_q + s * S::QTILE + (d0 >> 6) * S::QBOX + row * 128 + ((((d0 & 63) >> 3) ^ (row & 7)) << 4) + (d0 & 7) * 2);
+                                qb[n][i][0] = x.x;
+                                qb[n][i][1] = x.y;
+                                if constexpr (BF16) {
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e)
+                                        most = fmaxf(most, fmaxf(fabsf(__uint_as_float(qb[n][i][e] << 16)), fabsf(__uint_as_float(qb[n][i][e] & 0xffff0000u))));
+                                }
+                            }
+                            if constexpr (BF16) {
+                                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                                const int shift = query_shift(__float_as_uint(most) >> 16);
+                                const float there = __uint_as_float(uint32_t(127 - shift) << 23);
+                                own = fminf(__uint_as_float(uint32_t(127 + shift) << 23) * p.lift, 3e38f);
+#pragma unroll
+                                for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e)
+                                        qb[n][i][e] = pack2<false>(__uint_as_float(qb[n][i][e] << 16) * there, __uint_as_float(qb[n][i][e] & 0xffff0000u) * there);
+                                }
+                            }
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                back[n][e] = __shfl_sync(0xffffffffu, own, 4 * (2 * c4 + e));
+                                scale[n][e] = scale_of(back[n][e]);
+                            }
+                        }
+                        // (what an item's rows are lies one a lane)
+                        int row_pos[NT][2];
+                        float row_slope[NT][2];
+                        if constexpr ((KIND & SCORE_BIAS) != 0) {
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    row_pos[n][e] = __shfl_sync(0xffffffffu, pos, 8 * n + 2 * c4 + e);
+                                    row_slope[n][e] = __shfl_sync(0xffffffffu, slope, 8 * n + 2 * c4 + e);
+                                }
+                            }
+                        }
+                        const uint32_t* const warp_masks = reinterpret_cast<const uint32_t*>(smem + S::off_masks) + w * (S::kMaskWords * kBlk) + (warp & 3) * 32;
+                        float o[kCols][NT][4] = {}, m[NT][2], l[NT][2];
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            m[n][0] = m[n][1] = -INFINITY;
+                            l[n][0] = l[n][1] = 0.f;
+                        }
+#pragma unroll 1
+                        for (int step = ((item_raw ^ w) & 1) * (2 / U); step < T * (2 / U); step += U == 2 || (step & 1) ? 1 + 2 / U : 1) {
+                            const int t = step / (2 / U), half = U == 2 ? 0 : step & 1, mine = own_keys + 16 * half;
+                            const int k0 = key_block(lo + t, border, skip) * kBlk + mine, gr = item_raw + t;
+                            const int rk = gr % S::NRK, rv = gr % S::NRV;
+                            const bool give_back = U == 2 || half == 1;
+                            // does some row not see all of these keys?
+                            const bool masked = k0 + 16 * U - 1 > all_see || (p.window > 0 && k0 < low_last && k0 + 16 * U > early);
+                            uint4 xk[U][2][D / 64];  // keys 16 u + 8 j + g8
+                            float k_scale[U][2];
+                            uint32_t xv[U][4][D / 32], v_scale[U][2];  // keys 16 u + 2 c4, + 1, + 8, + 9; columns from g8 * D / 8 on
+                            auto take_values = [&] {
+                                if (!mbar_wait_warp(BAR(B_RAWV + rv), (gr / S::NRV) & 1, ab, ST_WAIT_TIMEOUT + 20)) return false;
+                                const uint8_t* const from = smem + S::off_raw_v + rv * S::RAW;
+#pragma unroll
+                                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        const int row = mine + 16 * u + 2 * c4 + (i & 1) + 8 * (i >> 1);
+                                        if constexpr (D == 128) {
+                                            const uint4 y = *reinterpret_cast<const uint4*>(from + raw_place<D>(row, g8));
+                                            xv[u][i][0] = y.x; xv[u][i][1] = y.y; xv[u][i][2] = y.z; xv[u][i][3] = y.w;
+                                        } else {
+                                            const uint2 y = *reinterpret_cast<const uint2*>(from + raw_place<D>(row, g8 >> 1) + (g8 & 1) * 8);
+                                            xv[u][i][0] = y.x; xv[u][i][1] = y.y;
+                                        }
+                                    }
+#pragma unroll
+                                    for (int i = 0; i < 2; ++i) v_scale[u][i] = *reinterpret_cast<const uint16_t*>(smem + S::off_scale_v + rv * kBlk + mine + 16 * u + 2 * c4 + 8 * i);
+                                }
+                                if (give_back) mbar_arrive_warp(BAR(B_RAWVEMPTY + rv), lane);
+                                return true;
+                            };
+                            if (!mbar_wait_warp(BAR(B_RAWK + rk), (gr / S::NRK) & 1, ab, ST_WAIT_TIMEOUT + 20)) return false;
+                            {
+                                const uint8_t* const from = smem + S::off_raw_k + rk * S::RAW;
+#pragma unroll
+                                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                                    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                                        for (int i = 0; i < D / 64; ++i)
+                                            xk[u][j][i] = *reinterpret_cast<const uint4*>(from + raw_place<D>(mine + 16 * u + 8 * j + g8, c4 * (D / 64) + i));
+                                        k_scale[u][j] = scale_to_float(smem[S::off_scale_k + rk * kBlk + mine + 16 * u + 8 * j + g8]);
+                                    }
+                                }
+                                if (give_back) mbar_arrive_warp(BAR(B_RAWKEMPTY + rk), lane);
+                            }
+                            if (NT == 1 && !take_values()) return false;
+                            float sc[NT][U][4] = {};
+#pragma unroll
+                            for (int i = 0; i < kSteps; ++i) {
+                                auto word = [&](const uint4& y) { return (i & 3) == 0 ? y.x : (i & 3) == 1 ? y.y : (i & 3) == 2 ? y.z : y.w; };
+#pragma unroll
+                                for (int u = 0; u < U; ++u) {
+                                    uint32_t ka[4];
+                                    unpack_e4m3x4(word(xk[u][0][i >> 2]), ka[0], ka[2]);
+                                    unpack_e4m3x4(word(xk[u][1][i >> 2]), ka[1], ka[3]);
+#pragma unroll
+                                    for (int n = 0; n < NT; ++n) mma_16816(sc[n][u], ka, qb[n][i][0], qb[n][i][1]);
+                                }
+                            }
+                            uint32_t pb[NT][U][2];
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                float y[U][4];  // keys 16 u + g8, + 8 by rows 2 c4, 2 c4 + 1, in the log2 domain
+#pragma unroll
+                                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                                    for (int j = 0; j < 2; ++j) {
+                                        const float* const f = SCORED ? back[n] : scale[n];
+                                        uint64_t y2 = mul_f2(pack_f2(sc[n][u][2 * j], sc[n][u][2 * j + 1]), pack_f2(k_scale[u][j] * f[0], k_scale[u][j] * f[1]));
+                                        if constexpr (SCORED) {
+                                            uint64_t b2 = 0;
+                                            if constexpr ((KIND & SCORE_BIAS) != 0) {
+                                                const int key = k0 + 16 * u + 8 * j + g8;
+                                                b2 = pack_f2(-row_slope[n][0] * fabsf(float(row_pos[n][0] - key)), -row_slope[n][1] * fabsf(float(row_pos[n][1] - key)));
+                                            }
+                                            if constexpr ((KIND & SCORE_CAPPED) != 0) y2 = cap_any(y2, b2, p.score);
+                                            else y2 = fma_f2(y2, pack_f2(p.scale_log2, p.scale_log2), b2);
+                                        }
+                                        unpack_f2(y2, y[u][2 * j], y[u][2 * j + 1]);
+                                    }
+                                }
+                                if (masked) {
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) {
+                                        const int row = 8 * n + 2 * c4 + e;
+                                        const uint32_t keep = keys_seen(k0, __shfl_sync(0xffffffffu, row0, row), __shfl_sync(0xffffffffu, low, row), early, base, tree, warp_masks + row) >> g8;
+#pragma unroll
+                                        for (int u = 0; u < U; ++u) {
+                                            y[u][e] = (keep >> (16 * u) & 1u) ? y[u][e] : -INFINITY;
+                                            y[u][2 + e] = (keep >> (16 * u) & 256u) ? y[u][2 + e] : -INFINITY;
+                                        }
+                                    }
+                                }
+                                float top[2];
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    top[e] = fmaxf(y[0][e], y[0][2 + e]);
+                                    if constexpr (U == 2) top[e] = fmaxf(top[e], fmaxf(y[U - 1][e], y[U - 1][2 + e]));
+                                    top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 4));
+                                    top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 8));
+                                    top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 16));
+                                }
+                                // lazy: the old reference point stays while the new maximum is within 2^8 of it
+                                const bool need0 = top[0] - m[n][0] > 8.f, need1 = top[1] - m[n][1] > 8.f;
+                                if (__any_sync(0xffffffffu, need0 || need1)) {
+                                    const float a0 = need0 ? fast_exp2(m[n][0] - top[0]) : 1.f, a1 = need1 ? fast_exp2(m[n][1] - top[1]) : 1.f;
+                                    if (need0) m[n][0] = top[0];
+                                    if (need1) m[n][1] = top[1];
+                                    l[n][0] *= a0;
+                                    l[n][1] *= a1;
+#pragma unroll
+                                    for (int i = 0; i < kCols; ++i) {
+                                        o[i][n][0] *= a0;
+                                        o[i][n][1] *= a1;
+                                        o[i][n][2] *= a0;
+                                        o[i][n][3] *= a1;
+                                    }
+                                }
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const float ref = (m[n][e] == -INFINITY ? 0.f : m[n][e]) - kRaised;
+#pragma unroll
+                                    for (int u = 0; u < U; ++u) {
+                                        y[u][e] = fast_exp2(y[u][e] - ref);
+                                        y[u][2 + e] = fast_exp2(y[u][2 + e] - ref);
+                                    }
+                                    l[n][e] += U == 2 ? (y[0][e] + y[0][2 + e]) + (y[U - 1][e] + y[U - 1][2 + e]) : y[0][e] + y[0][2 + e];
+                                }
+#pragma unroll
+                                for (int u = 0; u < U; ++u) {
+                                    pb[n][u][0] = transpose_8x8(pack2<false>(y[u][0], y[u][1]));
+                                    pb[n][u][1] = transpose_8x8(pack2<false>(y[u][2], y[u][3]));
+                                }
+                            }
+                            if (NT != 1 && !take_values()) return false;
+                            if (k0 + 16 * U > seen || (p.window > 0 && k0 + 16 * U > early && k0 < low_first)) {  // keys that no row sees
+#pragma unroll
+                                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        const int key = k0 + 16 * u + 2 * c4 + (i & 1) + 8 * (i >> 1);
+                                        const bool real = key < seen && !(p.window > 0 && key >= early && key < low_first);
+#pragma unroll
+                                        for (int j = 0; j < D / 32; ++j) xv[u][i][j] = real ? xv[u][i][j] : 0u;
+                                    }
+                                }
+                            }
+#pragma unroll
+                            for (int u = 0; u < U; ++u) {
+                                uint32_t two[2];
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) two[i] = (scale_to_h2(v_scale[u][i] & 255u) & 0xffffu) | (scale_to_h2(v_scale[u][i] >> 8) & 0xffff0000u);
+#pragma unroll
+                                for (int i = 0; i < kCols; ++i) {
+                                    // bytes 2 i and 2 i + 1 of the first key, each beside the second one's
+                                    const uint32_t pick = (i & 1) ? 0x7362u : 0x5140u;
+                                    uint32_t va[4];
+                                    unpack_e4m3x4(__byte_perm(xv[u][0][i >> 1], xv[u][1][i >> 1], pick), va[0], va[1]);
+                                    unpack_e4m3x4(__byte_perm(xv[u][2][i >> 1], xv[u][3][i >> 1], pick), va[2], va[3]);
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) va[e] = mul_h2(va[e], two[e >> 1]);
+#pragma unroll
+                                    for (int n = 0; n < NT; ++n) mma_16816(o[i][n], va, pb[n][u][0], pb[n][u][1]);
+                                }
+                            }
+                        }
+                        if (!mbar_wait_warp(BAR(B_SUMSFREE), direct & 1, ab, ST_WAIT_TIMEOUT + 22)) return false;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int row = 8 * n + 2 * c4 + e;
+#pragma unroll
+                                for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+                                if (g8 == 0) {
+                                    float* const ml = reinterpret_cast<float*>(smem + S::off_ml) + s * (4 * kBlk) + w * (2 * kBlk) + (warp & 3) * 32 + row;
+                                    ml[0] = m[n][e];
+                                    ml[kBlk] = l[n][e];
+                                }
+                                float4* const to = reinterpret_cast<float4*>(smem + S::off_sums) + (warp * kDirectRows + row) * (D / 4);
+#pragma unroll
+                                for (int i = 0; i < kCols; i += 2)
+                                    to[sums_place<D>(row, g8 * (D / 32) + i / 2)] = make_float4(o[i][n][e], o[i][n][2 + e], o[i + 1][n][e], o[i + 1][n][2 + e]);
+                            }
+                        }
+                        return true;
+                    };
+                    alive = tokens * p.G <= 8 ? multiply(std::integral_constant<int, 1>{}) : multiply(std::integral_constant<int, 2>{});
+                    ++direct;
+                    if (!alive) break;
+                    mbar_arrive_warp(BAR(B_MLFULL + s), lane);
+                    if (lane == 0) mbar_arrive(BAR(B_ITEMEMPTY + s));
+                    continue;
+                }
             }
             const int t0 = (G ^ w) & 1;  // this group's first tile of the item
             float m_run = -INFINITY, l_run = 0.f;
             float factor = 1.f;  // E4M3 of bf16: of the row's scores
 
-            for (int t = t0; t < T && alive; t += 2) {
+            for (int t = t0; t < T && alive; alive = alive && unpack_values(t), t += 2) {
                 const int k0 = key_block(lo + t, border, skip) * kBlk;
                 // MASKED: rows of the tile that no row of the item sees although they lie before its last key
                 const int none_from = MASKED ? max(early - k0, 0) : 0, none_end = MASKED ? min(low_first - k0, kBlk) : 0;
@@ -1004,7 +1397,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     // ------------------------------ tear-down ------------------------------
     tc_fence_before();
     __syncthreads();
-    if (warp == 13) {
+    if (!DIRECT && warp == 13) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -1155,6 +1548,9 @@ static cudaError_t launch_paged_t(const CUtensorMap& tq, const CUtensorMap& tn, 
 cudaError_t launch_paged_fwd(bool bf16, const CUtensorMap& tq, const CUtensorMap& tn, const CUtensorMap& tk, const CUtensorMap& tv, const PagedParams& p, int workers, cudaStream_t stream) {
     auto pick = [&](auto d, auto kind) {
         constexpr int kD = decltype(d)::value, kKind = decltype(kind)::value;
+        if (p.k_scales && !p.starts && p.G <= kDirectRows)
+            return bf16 ? launch_paged_t<kD, true, kKind, FORM_MASKED | FORM_E4M3 | FORM_DIRECT>(tq, tn, tk, tv, p, workers, stream)
+                        : launch_paged_t<kD, false, kKind, FORM_MASKED | FORM_E4M3 | FORM_DIRECT>(tq, tn, tk, tv, p, workers, stream);
         if (p.k_scales)
             return bf16 ? launch_paged_t<kD, true, kKind, FORM_MASKED | FORM_E4M3>(tq, tn, tk, tv, p, workers, stream)
                         : launch_paged_t<kD, false, kKind, FORM_MASKED | FORM_E4M3>(tq, tn, tk, tv, p, workers, stream);
