@@ -210,7 +210,9 @@ int fa_fwd_windowed(const fa_problem* p, const fa_scores* scores, const fa_windo
                     void* stream);
 int fa_bwd_windowed(const fa_problem* p, const fa_scores* scores, const fa_window* window, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v,
                     const fa_tensor* o, const void* rest, const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk,
-                    const fa_tensor* dv, const void* plan, int32_t* status, void* stream);
+                    const fa_tensor* dv, const void* plan, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* What fa_bwd_windowed needs as its workspace (16-byte aligned; 0: none, and NULL will do): with first keys that all queries see, fp32 sums of runs of queries. */
+int fa_bwd_workspace_bytes(const fa_problem* p, const fa_window* window, size_t* bytes);
 
 /* A cache of keys and values in pages, for serving (no counterpart in the reference). k and v are [pages, page_size, Hk, D], 16-bit, with 16-byte
  * aligned bases, last stride 1 and other strides multiples of 8 elements. Sequence b's tokens lie, page_size at a time, in the pages

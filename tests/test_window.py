@@ -40,7 +40,7 @@ def _codes(problem, window, scores=None):
     w = None if window is None else _lib.Window(*window)
     plan = lib.fa_plan_build_windowed(problem, scores, w, None, None, 256, 512, 256, None)
     fwd = lib.fa_fwd_windowed(problem, scores, w, t, t, t, t, None, None, None, 1, None, 0, 256, None)
-    bwd = lib.fa_bwd_windowed(problem, scores, w, t, t, t, t, None, t, None, None, t, t, t, None, 256, None)
+    bwd = lib.fa_bwd_windowed(problem, scores, w, t, t, t, t, None, t, None, None, t, t, t, None, None, 0, 256, None)
     return plan, fwd, bwd
 
 

@@ -20,6 +20,7 @@ cudaError_t launch_bwd_delta(const DeltaParams&, cudaStream_t);
 cudaError_t launch_bwd_dkdv(int, bool, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
                             const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const DkdvParams&, int,
                             cudaStream_t);
+cudaError_t launch_sum_parts(bool, const SumPartsParams&, cudaStream_t);
 cudaError_t launch_bwd_dq(int, bool, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&,
                           const CUtensorMap&, const CUtensorMap&, const DqParams&, int, bool, cudaStream_t);
 
@@ -428,9 +429,25 @@ int run_bwd_delta(const fa_problem* p, const void* rest, const fa_tensor* o, con
     return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
+// Into how many runs of queries dK / dV of the blocks with a window's first keys are cut, which every query sees something of: their items are as long as the others' then. With
+// `early` such blocks, and one run where nothing is gained, because the window is nearly as long or because there is so much other work that it hides them. us, 2 x 16 / 4 heads x 4000 x 128,
+// window 1024, 4 first keys, forward and backward, whole | cut 416 | - (without first keys 283).
+int query_runs(const fa_problem* p, const fa_window& w, int sms, int& early) {
+    early = 0;
+    if (w.keys <= 0 || w.sinks <= 0 || !p->causal || p->dtype == FA_FP32) return 1;
+    const int nq = fa::cdiv(p->M, fa::kBlk), nk = fa::cdiv(p->N, fa::kBlk);
+    early = std::min(nk, fa::cdiv(std::min(w.sinks, p->N), fa::kBlk));
+    const int64_t blocks = fa::cdiv(std::min(w.keys, p->N), fa::kBlk) + 1, share = int64_t(nk) * p->Hk * p->B * blocks / (2 * sms);
+    const int64_t runs = (nq + std::max(blocks, share) - 1) / std::max(blocks, share);
+    return int(std::max(int64_t(1), std::min(runs, int64_t(32))));
+}
+size_t runs_bytes(const fa_problem* p, int early, int runs) {
+    return runs > 1 ? size_t(runs) * early * p->B * p->Hk * 2 * fa::kBlk * (p->D > 64 ? 128 : 64) * sizeof(float) : 0;
+}
+
 int run_bwd_dkdv(const fa_problem* p, const Changes* sc, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v,
                 const fa_tensor* d_o, const float* lse, const float* delta, const fa_tensor* dk, const fa_tensor* dv,
-                const void* plan, int32_t* status, void* stream) {
+                const void* plan, int32_t* status, void* stream, float* sums = nullptr, int early = 0, int runs = 1) {
     int rc = check_problem(p);
     if (rc) return rc;
     if ((rc = check_scores(p, sc))) return rc;
@@ -447,6 +464,9 @@ int run_bwd_dkdv(const fa_problem* p, const Changes* sc, const fa_tensor* q, con
     fa::DkdvParams kp;
     if ((rc = make_mask(&kp.mask, p, plan, sc))) return rc;
     kp.score = score_args(p, sc);
+    kp.sums = sums;
+    kp.early = early;
+    kp.parts = runs;
     CUtensorMap tq, tk, tv, tdo;
     if ((rc = make_map(&tq, q, p->dtype, p->B, p->H, p->M, p->D))) return rc;
     if ((rc = make_map(&tdo, d_o, p->dtype, p->B, p->H, p->M, p->D))) return rc;
@@ -701,21 +721,45 @@ int fa_bwd(const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa
 
 int fa_bwd_windowed(const fa_problem* p, const fa_scores* scores, const fa_window* window, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v,
                     const fa_tensor* o, const void* rest, const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk,
-                    const fa_tensor* dv, const void* plan, int32_t* status, void* stream) {
+                    const fa_tensor* dv, const void* plan, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
     const Changes c(scores, window);
     int rc = check_problem(p);
     if (!rc) rc = check_scores(p, &c);
-    if (!rc) rc = run_bwd_delta(p, rest, o, d_o, delta, stream);
-    if (!rc) rc = run_bwd_dkdv(p, &c, q, k, v, d_o, lse, delta, dk, dv, plan, status, stream);
+    if (rc) return rc;
+    const int sms = c.window.keys > 0 && c.window.sinks > 0 ? sm_count() : 1;
+    if (sms <= 0) return FA_ERR_LAUNCH;
+    int early;
+    const int runs = query_runs(p, c.window, sms, early);
+    if (workspace_bytes < runs_bytes(p, early, runs) || (runs > 1 && !workspace)) return FA_ERR_PLAN_SIZE;
+    if (!aligned16(workspace)) return FA_ERR_ALIGNMENT;
+    float* const sums = static_cast<float*>(workspace);
+    rc = run_bwd_delta(p, rest, o, d_o, delta, stream);
+    if (!rc) rc = run_bwd_dkdv(p, &c, q, k, v, d_o, lse, delta, dk, dv, plan, status, stream, sums, early, runs);
     if (!rc) rc = run_bwd_dq(p, &c, q, k, v, d_o, lse, delta, dq, plan, status, true, stream);
-    return rc;
+    if (rc || runs < 2) return rc;
+    const fa::SumPartsParams sp{sums, out_view(dk), out_view(dv), early, runs, p->B, p->Hk, p->N, p->D, p->D > 64 ? 128 : 64, p->sm_scale, status};
+    return fa::launch_sum_parts(p->dtype == FA_BF16, sp, static_cast<cudaStream_t>(stream)) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+int fa_bwd_workspace_bytes(const fa_problem* p, const fa_window* window, size_t* bytes) {
+    if (!bytes) return FA_ERR_BAD_ARG;
+    const int rc = check_problem(p);
+    if (rc) return rc;
+    *bytes = 0;
+    if (!window || window->keys <= 0 || window->sinks <= 0 || !p->causal || p->dtype == FA_FP32) return FA_OK;
+    const int sms = sm_count();
+    if (sms <= 0) return FA_ERR_LAUNCH;
+    int early;
+    const int runs = query_runs(p, *window, sms, early);
+    *bytes = runs_bytes(p, early, runs);
+    return FA_OK;
 }
 
 int fa_bwd_scored(const fa_problem* p, const fa_scores* scores, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
                   const void* rest, const fa_tensor* d_o, const float* lse, float* delta, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv,
                   const void* plan, int32_t* status, void* stream) {
     if (!scores) return FA_ERR_BAD_ARG;
-    return fa_bwd_windowed(p, scores, nullptr, q, k, v, o, rest, d_o, lse, delta, dq, dk, dv, plan, status, stream);
+    return fa_bwd_windowed(p, scores, nullptr, q, k, v, o, rest, d_o, lse, delta, dq, dk, dv, plan, nullptr, 0, status, stream);
 }
 
 uint32_t fa_classify_tile(int32_t M, int32_t N, int32_t causal, int32_t mode, int32_t qb, int32_t kb, int32_t qmin,

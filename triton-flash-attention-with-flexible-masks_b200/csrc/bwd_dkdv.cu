@@ -129,7 +129,9 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const MaskArgs& mk = p.mask;
     const int G = p.G;
     const int nK = mk.L.nK;
-    const int n_items = nK * p.Hk * p.B;
+    const int n_blocks = nK * p.Hk * p.B;
+    const int n_parts = WINDOW && p.parts > 1 ? p.parts * p.early * p.Hk * p.B : 0;  // in front of the others; their key blocks' own items have nothing to do
+    const int n_items = n_blocks + n_parts;
     unsigned int* ctr = mk.ctr ? mk.ctr + CTR_DKDV : nullptr;
     // item -> (key block, kv head, batch). Heads are taken in groups of p.gh; inside a group the key
     // blocks go in order (with a causal mask: long ones first) and the heads of the group vary
@@ -208,7 +210,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         int gh = p.gh, nk = nK, heads = p.Hk, batches = p.B;
         asm volatile("" : "+r"(gh), "+r"(nk), "+r"(heads), "+r"(batches));
         if (tid == 0) {
-            for (int k = 0, j; (j = item_in_order(k)) < n_items; ++k) {
+            for (int k = 0, j; (j = item_in_order(k)) < n_blocks; ++k) {
                 int kb, hk, b;
                 decode(j, kb, hk, b, gh, nk, heads, batches);
                 for (int x = 0; x < S::NBOX; ++x) {
@@ -249,8 +251,16 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     }
                     break;
                 }
-                int kb, hk, b;
-                decode(j, kb, hk, b, p.gh, nK, p.Hk, p.B);
+                int kb, hk, b, part = 0;  // part: 1 .. p.parts of a block that is cut
+                if (WINDOW && j < n_parts) {
+                    const int rest = j / (p.Hk * p.B), bh = j - rest * (p.Hk * p.B);
+                    b = bh / p.Hk;
+                    hk = bh - b * p.Hk;
+                    kb = rest / p.parts;
+                    part = rest - kb * p.parts + 1;
+                } else {
+                    decode(j - n_parts, kb, hk, b, p.gh, nK, p.Hk, p.B);
+                }
                 int lo = 0x7fffffff, hi = 0;
                 {
                     const int ng = (mk.He == 1) ? 1 : G;
@@ -262,6 +272,11 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     if (hi == 0) lo = 0;
                 }
                 int n = hi - lo;
+                if (WINDOW && n_parts > 0 && kb < p.early) {
+                    const int first = part ? n * (part - 1) / p.parts : 0;
+                    n = part ? n * part / p.parts - first : 0;
+                    lo += first;
+                }
                 if (n > kListCap) n = kListCap;
                 uint8_t* fl = smem + S::off_flags + s * S::FLAGS;
                 int cnt = 0;
@@ -285,7 +300,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     info[s * 8 + 1] = n;
                     info[s * 8 + 2] = cnt * G;  // tiles of all query heads of the group, head-major
                     info[s * 8 + 3] = j;
-                    info[s * 8 + 4] = kb;
+                    info[s * 8 + 4] = WINDOW ? kb | part << 16 : kb;
                     info[s * 8 + 5] = hk;
                     info[s * 8 + 6] = b;
                     if constexpr (PREFIX) info[s * 8 + 7] = front_keys<true>(mk, b);
@@ -305,7 +320,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             auto finish_store = [&](int i, int kb, int hk, int b, int last) {
                 if (!mbar_wait_warp(BAR(B_STAGED), i & 1, ab, ST_WAIT_TIMEOUT + 55)) return false;
                 if (lane == 0) {
-                    if (misc[1] == 0) {
+                    if (misc[1] == 0 && !(WINDOW && kb >> 16)) {  // (a part's sums are stored by who has them)
                         for (int x = 0; x < S::NBOX; ++x) {
                             tma_store_4d(&tmdV, sdO(last % NDO) + x * S::BOX, x * 64, kb * kBlk, hk, b);
                             tma_store_4d(&tmdK, sQ(last % NQ) + x * S::BOX, x * 64, kb * kBlk, hk, b);
@@ -359,11 +374,11 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     if (kk > 0) ok = mbar_wait_warp(BAR(B_KEMPTY), (kk - 1) & 1, ab, ST_WAIT_TIMEOUT + 57);
                     if (!ok) break;
                     mbar_expect_tx_elect(BAR(B_KFULL), S::TILE);
-                    for (int x = 0; x < S::NBOX; ++x) tma_load_4d_elect(sK + x * S::BOX, &tmK, BAR(B_KFULL), x * 64, kb * kBlk, hk, b);
+                    for (int x = 0; x < S::NBOX; ++x) tma_load_4d_elect(sK + x * S::BOX, &tmK, BAR(B_KFULL), x * 64, (WINDOW ? kb & 0xffff : kb) * kBlk, hk, b);
                     if (kk > 0) ok = mbar_wait_warp(BAR(B_VEMPTY), (kk - 1) & 1, ab, ST_WAIT_TIMEOUT + 60);
                     if (!ok) break;
                     mbar_expect_tx_elect(BAR(B_VFULL), S::TILE);
-                    for (int x = 0; x < S::NBOX; ++x) tma_load_4d_elect(sV + x * S::BOX, &tmV, BAR(B_VFULL), x * 64, kb * kBlk, hk, b);
+                    for (int x = 0; x < S::NBOX; ++x) tma_load_4d_elect(sV + x * S::BOX, &tmV, BAR(B_VFULL), x * 64, (WINDOW ? kb & 0xffff : kb) * kBlk, hk, b);
                     for (int it = 0; it < nq && ok; ++it) {
                         ok = load_q(it);
                         if (ok && it < ndo) ok = load_do(it);
@@ -498,7 +513,7 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             if (!ok) break;
             const int lo = info[s * 8 + 0], n = info[s * 8 + 1], NIT = info[s * 8 + 2], jt = info[s * 8 + 3];
             if (jt < 0) break;
-            const int kb = info[s * 8 + 4], hk = info[s * 8 + 5], b = info[s * 8 + 6];
+            const int item_kb = info[s * 8 + 4], kb = WINDOW ? item_kb & 0xffff : item_kb, part = WINDOW ? item_kb >> 16 : 0, hk = info[s * 8 + 5], b = info[s * 8 + 6];
             const Walk wk = walk_of(s, n);
             const int j = kb * kBlk + r;  // this thread's key
             const int k0 = kb * kBlk, k1 = min(k0 + kBlk, mk.N);
@@ -701,6 +716,13 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         // tcgen05.ld is warp-collective: always executed, the values are ignored for an item without tiles
                         tmem_ld16(tmem + lane_base + 256u + uint32_t(which * D) + c0 + uint32_t(q) * 16u, x);
                         tc_wait_ld();
+                        if (WINDOW && part) {  // sums of a run of queries, which are added up later
+                            float* const to = p.sums + (((int64_t(part - 1) * p.early + kb) * p.B + b) * p.Hk + hk) * (2 * kBlk * D) + (which * kBlk + r) * D + c0 + 16 * q;
+#pragma unroll
+                            for (int y = 0; y < 16; y += 4)
+                                *reinterpret_cast<uint4*>(to + y) = NIT > 0 ? make_uint4(x[y], x[y + 1], x[y + 2], x[y + 3]) : make_uint4(0, 0, 0, 0);
+                            continue;
+                        }
                         uint32_t o16[8];
 #pragma unroll
                         for (int y = 0; y < 8; ++y) {
@@ -750,6 +772,38 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     }
 }
 
+// dK and dV of key blocks that were cut into runs of queries: the runs' fp32 sums, in their order, rounded once. A warp a row of dV or dK.
+template <bool BF16>
+__global__ void __launch_bounds__(256) sum_parts_kernel(const SumPartsParams p) {
+    follow_stream();
+    const int lane = threadIdx.x & 31;
+    const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5), rows = int64_t(p.early) * p.B * p.Hk * 2 * kBlk;  // as in the workspace
+    if (row >= rows) return;
+    const int r = int(row % kBlk), which = int(row / kBlk & 1);
+    const int64_t block = row / (2 * kBlk);
+    const int hk = int(block % p.Hk), b = int(block / p.Hk % p.B), kb = int(block / p.Hk / p.B), j = kb * kBlk + r;
+    if (j >= p.N) return;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    const float* from = p.sums + row * p.Dk + lane;
+#pragma unroll 4
+    for (int s = 0; s < p.parts; ++s, from += rows * p.Dk) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (32 * i < p.Dk) acc[i] += from[32 * i];
+    }
+    const bool failed = status_is_fatal(*p.status);  // there are no sums: NaN, as the other kernels do
+    const OutTensor& t = which ? p.dk : p.dv;
+    uint16_t* const to = static_cast<uint16_t*>(t.ptr) + int64_t(b) * t.sb + int64_t(hk) * t.sh + int64_t(j) * t.sl;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (lane + 32 * i < p.D) to[lane + 32 * i] = failed ? 0xffffu : uint16_t(pack2<BF16>(acc[i] * (which ? p.sm_scale : 1.f), 0.f) & 0xffffu);
+}
+
+cudaError_t launch_sum_parts(bool bf16, const SumPartsParams& p, cudaStream_t stream) {
+    const int64_t rows = int64_t(p.early) * p.B * p.Hk * 2 * kBlk;
+    return launch_overlapping(bf16 ? sum_parts_kernel<true> : sum_parts_kernel<false>, dim3(unsigned((rows + 7) / 8)), 256, 0, stream, p);
+}
+
 template <int D, bool BF16, int KIND>
 static cudaError_t launch_dkdv_t(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                                  const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
@@ -759,7 +813,7 @@ static cudaError_t launch_dkdv_t(const CUtensorMap& tq, const CUtensorMap& tk, c
     static SmemAllowed allowed;
     cudaError_t e = allow_smem(kern, smem, allowed);
     if (e != cudaSuccess) return e;
-    const int n_items = p.mask.L.nK * p.Hk * p.B;
+    const int n_items = (p.mask.L.nK + ((KIND & SCORE_WINDOW) && p.parts > 1 ? p.parts * p.early : 0)) * p.Hk * p.B;
     const int grid = n_items < num_sms ? n_items : num_sms;
     return launch_overlapping(kern, dim3(grid), kDkdvThreads, smem, stream, tq, tk, tv, tdo, tdk, tdv, p);
 }

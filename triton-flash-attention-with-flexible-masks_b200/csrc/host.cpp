@@ -114,6 +114,9 @@ Tensor plan(uintptr_t problem, const std::optional<Tensor>& eq, const std::optio
     return build_plan(*reinterpret_cast<const fa_problem*>(problem), eq ? &*eq : nullptr, ek ? &*ek : nullptr, status);
 }
 
+// Kernels launched by `attend` and its gradients (ops.LAUNCHES).
+std::atomic<int64_t> n_launched{0};
+
 struct Outputs {
     Tensor o, lse;
     int splits;
@@ -160,8 +163,15 @@ std::array<Tensor, 3> launch_backward(const fa_problem& p, const Tensor& d_o, co
     Tensor dq = at::empty(q.sizes(), q.options());
     const fa_tensor tq = view(q), tk = view(k), tv = view(v), to = view(o), tdo = view(d_o), tdq = view(dq), tdk = view(dk), tdv = view(dv);
     void* const plan_ptr = plan.defined() ? plan.data_ptr() : nullptr;
+    Tensor work;
+    size_t bytes = 0;
+    if (window && window->keys > 0) check(fa_bwd_workspace_bytes(&p, window, &bytes), "fa_bwd_workspace_bytes");
+    if (bytes > 0) {
+        work = at::empty({int64_t(bytes / 4)}, q.options().dtype(at::kFloat));
+        ++n_launched;
+    }
     if (scores)
-        check(fa_bwd_windowed(&p, scores, window, &tq, &tk, &tv, &to, rest.defined() ? rest.data_ptr() : nullptr, &tdo, lse.data_ptr<float>(), delta.data_ptr<float>(), &tdq, &tdk, &tdv, plan_ptr,
+        check(fa_bwd_windowed(&p, scores, window, &tq, &tk, &tv, &to, rest.defined() ? rest.data_ptr() : nullptr, &tdo, lse.data_ptr<float>(), delta.data_ptr<float>(), &tdq, &tdk, &tdv, plan_ptr, work.defined() ? work.data_ptr() : nullptr, bytes,
                             status.data_ptr<int>(), current_stream(q)),
               "fa_bwd_windowed");
     else
@@ -206,9 +216,6 @@ py::object backward(const Tensor& d_o, const Tensor& q, const Tensor& k, const T
     }
     return py::make_tuple(std::move(g[0]), std::move(g[1]), std::move(g[2]));
 }
-
-// Kernels launched by `attend` and its gradients (ops.LAUNCHES).
-std::atomic<int64_t> n_launched{0};
 
 // What a regular call is, besides q, k and v.
 struct Call {

@@ -64,6 +64,19 @@ struct DkdvParams {
     int* status;
     long long wait_limit;  // SM clocks a bounded wait may last
     ScoreArgs score;       // the instances for attention_scored
+    // With a window: the first `early` key blocks, which all queries see something of, are cut into `parts` runs of queries (1: they are not), whose fp32 sums go to
+    // [parts, early, B, Hk, dV and dK, 128, 64 or 128]
+    int early, parts;
+    float* sums;
+};
+
+// Adds such runs up.
+struct SumPartsParams {
+    const float* sums;
+    OutTensor dk, dv;
+    int early, parts, B, Hk, N, D, Dk;  // Dk: columns of a row of `sums`
+    float sm_scale;
+    const int* status;
 };
 
 struct DqParams {

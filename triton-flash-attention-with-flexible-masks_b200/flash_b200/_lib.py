@@ -19,7 +19,7 @@ EXPORTS = (
     "fa_debug_wait_timeout", "fa_group_rows", "fa_permute_rows", "fa_fwd_splits", "fa_fwd_workspace_bytes", "fa_fwd_split",
     "fa_plan_optional", "fa_bwd", "fa_plan_build_scored", "fa_fwd_scored", "fa_fwd_rest", "fa_bwd_scored", "fa_paged_append",
     "fa_paged_workspace_bytes", "fa_paged_fwd", "fa_debug_paged_pieces",
-    "fa_plan_build_windowed", "fa_fwd_splits_windowed", "fa_fwd_windowed", "fa_bwd_windowed", "fa_paged_append_more", "fa_paged_fwd_more", "fa_debug_paged_pieces_more",
+    "fa_plan_build_windowed", "fa_fwd_splits_windowed", "fa_fwd_windowed", "fa_bwd_windowed", "fa_bwd_workspace_bytes", "fa_paged_append_more", "fa_paged_fwd_more", "fa_debug_paged_pieces_more",
 )
 
 
@@ -122,7 +122,9 @@ def load():
     lib.fa_fwd_windowed.restype = i32
     lib.fa_fwd_windowed.argtypes = [P, S, W, T, T, T, T, vp, vp, vp, ctypes.c_int32, vp, size, vp, vp]
     lib.fa_bwd_windowed.restype = i32
-    lib.fa_bwd_windowed.argtypes = [P, S, W, T, T, T, T, vp, T, vp, vp, T, T, T, vp, vp, vp]
+    lib.fa_bwd_windowed.argtypes = [P, S, W, T, T, T, T, vp, T, vp, vp, T, T, T, vp, vp, size, vp, vp]
+    lib.fa_bwd_workspace_bytes.restype = i32
+    lib.fa_bwd_workspace_bytes.argtypes = [P, W, ctypes.POINTER(size)]
     C, R = ctypes.POINTER(PagedCache), ctypes.POINTER(Rows)
     lib.fa_paged_append.restype = i32
     lib.fa_paged_append.argtypes = [C, ctypes.c_int32, vp, R, R, vp, vp]

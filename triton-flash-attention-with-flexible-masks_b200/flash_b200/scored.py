@@ -154,10 +154,13 @@ class ScoredAttention(torch.autograd.Function):
         with _current(device):
             delta = torch.empty_like(lse)
             dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
+            size = ctypes.c_size_t(0)
+            _lib.check(lib.fa_bwd_workspace_bytes(ctx.prob, ctx.window, size), "fa_bwd_workspace_bytes")
+            work = torch.empty(size.value // 4, dtype=torch.float32, device=device) if size.value else None
             _lib.check(lib.fa_bwd_windowed(ctx.prob, _scores(ctx.softcap, slopes, prefix), ctx.window, *map(_tensor, (q, k, v, out)), _pointer(rest), _tensor(do),
-                                         lse.data_ptr(), delta.data_ptr(), *map(_tensor, (dq, dk, dv)), _pointer(plan), _status_word(device).data_ptr(),
+                                         lse.data_ptr(), delta.data_ptr(), *map(_tensor, (dq, dk, dv)), _pointer(plan), _pointer(work), size.value, _status_word(device).data_ptr(),
                                          _stream()), "fa_bwd_windowed")
-            _count(3)
+            _count(3 if work is None else 4)
             if ops._SYNC_STATUS:
                 check_status(device)
         return (*_once((dq, dk, dv), (q, k, v)), *(None,) * 9)
