@@ -312,3 +312,58 @@ def test_single_tokens_of_all_sizes_and_not_finite():
     cache.k_pages.view(torch.uint8)[page, slot, 0, 5] = 127
     got = fb.paged_attention(x, *cache.args(), **cache.scales())
     assert got[0].isnan().all() and got[1].isfinite().all()
+
+
+@pytest.mark.parametrize("single", [False, True])
+def test_after_a_time_out_results_are_nan_until_it_has_been_read(single):
+    import flash_b200 as fb
+    from flash_b200 import ops
+    cache = Cache8([700, 400], 2, 64, 16, BF16, 25).fill()
+    new = [1, 1] if single else [90, 5]
+    q = torch.randn(sum(new), 4, 64, device="cuda").to(BF16)
+    call = lambda: fb.paged_attention(q, *cache.args(), None if single else _starts(new), window=300, sinks=1, **cache.scales())  # noqa: E731
+    want = call()
+    ops._status_word(q.device).fill_(142)  # as a bounded wait that ran out leaves it
+    assert call().isnan().all()
+    with pytest.raises(RuntimeError, match="role 42"):
+        fb.check_status()
+    assert torch.equal(call(), want)
+
+
+def test_pages_and_lengths_that_there_are_not():
+    import flash_b200 as fb
+    cache = Cache8([300, 200], 2, 64, 16, BF16, 26).fill()
+    q = torch.randn(2, 8, 64, device="cuda").to(BF16)
+    want = fb.paged_attention(q, *cache.args(), **cache.scales())
+    table = cache.table.clone()
+    for bad in (-1, 1 << 29, cache.k_pages.shape[0]):
+        cache.table[1, 2] = bad
+        for starts in (None, _starts([1, 1])):
+            got = fb.paged_attention(q, *cache.args(), starts, **cache.scales())
+            with pytest.raises(RuntimeError, match="page"):
+                fb.check_status()
+            assert torch.equal(got[0], want[0])
+    cache.table.copy_(table)
+    cache.kv_lens[1] = 1 << 28
+    got = fb.paged_attention(q, *cache.args(), **cache.scales())
+    with pytest.raises(RuntimeError, match="length|page"):
+        fb.check_status()
+    assert torch.equal(got[0], want[0])
+
+
+def test_two_streams_at_once():
+    import flash_b200 as fb
+    caches = [Cache8([3000, 5000, 20], 2, 128, 64, BF16, 27 + i).fill() for i in range(2)]
+    q = [torch.randn(203, 8, 128, device="cuda").to(BF16) for _ in range(2)]
+    starts, streams = _starts([200, 1, 2]), [torch.cuda.Stream() for _ in range(2)]
+    call = lambda i: fb.paged_attention(q[i], *caches[i].args(), starts, window=1000, sinks=2, **caches[i].scales())  # noqa: E731
+    want = [call(i) for i in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    fb.check_status()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])

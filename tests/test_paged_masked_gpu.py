@@ -195,3 +195,33 @@ def test_captured_calls_follow_lengths_and_parents(monkeypatch):
         monkeypatch.setattr(paged, "_native", lambda *tensors: None)  # the general way through the host gives the same
         assert torch.equal(call(), got)
         monkeypatch.undo()
+
+
+def test_after_a_time_out_results_are_nan_until_it_has_been_read():
+    import flash_b200 as fb
+    from flash_b200 import ops
+    cache = Cache([700, 400], 2, 64, 16, BF16, 16).fill()
+    q, parents = torch.randn(25, 4, 64, device="cuda").to(BF16), _parents([_tree(20, 1), _tree(5, 2)])
+    call = lambda: fb.paged_attention(q, cache.k_pages, cache.v_pages, cache.table, cache.kv_lens, _starts([20, 5]), window=300, sinks=1, parents=parents)  # noqa: E731
+    want = call()
+    ops._status_word(q.device).fill_(142)  # as a bounded wait that ran out leaves it
+    assert call().isnan().all()
+    with pytest.raises(RuntimeError, match="role 42"):
+        fb.check_status()
+    assert torch.equal(call(), want)
+
+
+@pytest.mark.parametrize("cap", [None, 3.0])
+def test_a_drafted_token_that_is_not_finite_reaches_those_that_see_it(cap):
+    """A key that is not a number makes the tokens on its branch NaN and leaves the others' scores as they were; a value behind all tokens of a tile stays out."""
+    import flash_b200 as fb
+    n, length = 40, 300
+    tree = [-1] + [0] * 19 + [19] * 20  # two levels: 1 .. 19 continue 0, 20 .. 39 continue 19
+    cache = Cache([length], 1, 64, 16, BF16, 17).fill()
+    q = torch.randn(n, 2, 64, device="cuda").to(BF16)
+    call = lambda: fb.paged_attention(q, cache.k_pages, cache.v_pages, cache.table, cache.kv_lens, _starts([n]), parents=_parents([tree]), softcap=cap)  # noqa: E731
+    want = call()
+    page, slot = cache.places(0, length - n + 5, length - n + 6)
+    cache.k_pages[page, slot] = float("nan")
+    got = call()
+    assert got[5].isnan().all() and torch.equal(got[:5], want[:5]) and torch.equal(got[6:], want[6:])

@@ -246,3 +246,36 @@ def test_one_gradient_only_and_twice_refused():
     check(dk.detach(), attention_64(q, k.detach(), v, do, windowed(200, 200, 20, 0))["dk"], "dk")
     with pytest.raises(RuntimeError, match="once"):
         dk.sum().backward()
+
+
+def test_after_a_time_out_results_are_nan_until_it_has_been_read():
+    """The kernel that adds up the runs of queries of the first keys' blocks among the others."""
+    import flash_b200 as fb
+    from flash_b200 import ops
+    q, k, v, do = _inputs(1, 4, 2, 1000, 1000, 64, BF16, 26)
+    want = _run(q, k, v, do, 100, 4)
+    a, b, c = (x.detach().requires_grad_() for x in (q, k, v))
+    o = fb.attention_scored(a, b, c, True, window=100, sinks=4)
+    ops._status_word(q.device).fill_(142)  # as a bounded wait that ran out leaves it
+    for g in torch.autograd.grad(o, (a, b, c), do):
+        assert g.isnan().all()
+    assert fb.attention_scored(q, k, v, True, window=100, sinks=4).isnan().all()
+    with pytest.raises(RuntimeError, match="role 42"):
+        fb.check_status()
+    got = _run(q, k, v, do, 100, 4)
+    assert all(torch.equal(got[n], want[n]) for n in NAMES)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("B,H,Hk,L,D,window,sinks", [(1, 4, 1, 3000, 64, 128, 1), (2, 2, 2, 1300, 128, 200, 200), (1, 8, 2, 2000, 32, 64, 128), (1, 2, 1, 5000, 128, 1, 3)])
+def test_first_keys_that_all_queries_see(B, H, Hk, L, D, window, sinks, dtype):
+    """Their dK and dV come from many runs of queries."""
+    _compare(*_inputs(B, H, Hk, L, L, D, dtype, 27), window, sinks)
+
+
+def test_the_same_bits_again():
+    q, k, v, do = _inputs(1, 8, 2, 3000, 3000, 64, BF16, 28)
+    want = _run(q, k, v, do, 200, 4)
+    for _ in range(3):
+        got = _run(q, k, v, do, 200, 4)
+        assert all(torch.equal(got[n], want[n]) for n in NAMES)

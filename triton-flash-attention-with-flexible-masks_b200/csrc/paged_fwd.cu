@@ -601,7 +601,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     check_pages(from, min(end, early));
                     if (p.window > 0) check_pages(max(from, low), end);
                 } else {
-                    check_pages(it[I_LO] * kBlk, T > 0 ? min((it[I_LO] + T) * kBlk, it[I_LEN]) : 0);
+                    if (T > 0) check_pages(it[I_LO] * kBlk, min((it[I_LO] + T) * kBlk, it[I_LEN]));
                 }
             }
             float factor = 1.f;  // E4M3 of bf16: of this row's scores
@@ -1157,7 +1157,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 const int none_from = MASKED ? max(early - k0, 0) : 0, none_end = MASKED ? min(low_first - k0, kBlk) : 0;
                 const bool none = MASKED && none_end > none_from;
                 // does some row not see all of the tile?
-                const bool masked = k0 + kBlk - 1 > all_see || (MASKED && p.window > 0 && k0 < low_last && k0 + kBlk > early);
+                auto masked = [&] { return k0 + kBlk - 1 > all_see || (MASKED && p.window > 0 && k0 < low_last && k0 + kBlk > early); };
                 const int g = G + t;
                 const uint32_t tS = tmem + lane_base + uint32_t(S::tmem_s(g)), tP = tmem + lane_base + uint32_t(S::tmem_p(g));
                 // P*V of the group's tile before: it has read its P and added to O
@@ -1173,7 +1173,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         alive = pv_before();
                         if (!alive) break;
                     }
-                    if (!E4M3 && (seen - k0 < kBlk || none)) alive = zero_behind(g, min(seen - k0, kBlk), none_from, none_end);
+                    if (!E4M3 && (seen - k0 < kBlk || none)) alive = zero_behind(g, MASKED ? min(seen - k0, kBlk) : seen - k0, none_from, none_end);
                     if (!alive) break;
                     mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
                     continue;
@@ -1206,7 +1206,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         const Bias bias(slope, front == 0, pos0 - (kq + 31), pos0 + 31 - kq);
                         score_row<KIND, 32>(v, p.score, bias, p.scale_log2, pos - kq, valid, (m_run == -INFINITY ? 0.f : m_run) - kRaised);
                     }
-                    if (MASKED ? masked : kq + 31 > all_see) {
+                    if (MASKED ? masked() : kq + 31 > all_see) {
                         const uint32_t keep = sees(kq);
 #pragma unroll
                         for (int x = 0; x < 32; ++x) v[x] = (keep & (1u << x)) ? v[x] : -INFINITY;
@@ -1221,7 +1221,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
 #pragma unroll
                     for (int a = 0; a < 4; ++a) mx[a] = fmaxf(mx[a], v[28 + a]);
-                    const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) - (SCORED ? kRaised : 0.f);
+                    float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+                    if constexpr (E4M3 && SCORED) top -= kRaised;
                     float m_new = fmaxf(m_run, top);
                     bool need = (m_new - m_run) * c > 8.0f;
                     if constexpr (SCORED) {
@@ -1241,7 +1242,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     if (scale_o) rescale(alpha);
                     m_run = m_new;
                     // (SCORED: what is left to be subtracted)
-                    const float mneg = SCORED ? (need ? -top : 0.f) : (m_run == -INFINITY) ? 0.f : kRaised - m_run * c;
+                    const float mneg = SCORED ? (need ? -top : 0.f) : (m_run == -INFINITY) ? 0.f : E4M3 ? kRaised - m_run * c : -m_run * c;
                     float l4[4] = {0.f, 0.f, 0.f, 0.f};
                     uint32_t pk[16];
 #pragma unroll
@@ -1257,7 +1258,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         if (q != quarter) tmem_st16(tP + uint32_t(q) * 16u, zero);
                     tmem_st16(tP + uint32_t(quarter) * 16u, pk);
                     tc_wait_st();
-                    if (!E4M3 && (seen - k0 < kBlk || none)) alive = zero_behind(g, min(seen - k0, kBlk), none_from, none_end);
+                    if (!E4M3 && (seen - k0 < kBlk || none)) alive = zero_behind(g, MASKED ? min(seen - k0, kBlk) : seen - k0, none_from, none_end);
                     tc_fence_before();
                     mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
                     if (!alive) break;
@@ -1292,10 +1293,10 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         for (int x = 0; x < kBlk; ++x) sc[x] = x >= none_from && x < none_end ? 0.f : sc[x];
                     }
                     const Bias bias(slope, front == 0, pos0 - (k0 + kBlk - 1), pos0 + kBlk - 1 - k0);
-                    if constexpr (KIND == SCORE_CAPPED) late = !masked && !any_beyond<kBlk>(sc, valid ? p.score.most : INFINITY);
+                    if constexpr (KIND == SCORE_CAPPED) late = !masked() && !any_beyond<kBlk>(sc, valid ? p.score.most : INFINITY);
                     if (!late) score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, pos - k0, valid, (m_run == -INFINITY ? 0.f : m_run) - kRaised);
                 }
-                if (masked) {
+                if (masked()) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const uint32_t keep = sees(k0 + 32 * q);
@@ -1321,7 +1322,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 bool need = (m_new - m_run) * c > 8.0f;
                 if constexpr (SCORED) {  // (the scores, and mx, are relative to the old reference point, or to 0 in front of a row's first key)
                     const bool fresh = m_run == -INFINITY;
-                    mx = late ? cap_one(mx, p.score) - (fresh ? 0.f : m_run) : mx - kRaised;
+                    if (late) mx = cap_one(mx, p.score) - (fresh ? 0.f : m_run);
+                    else if constexpr (E4M3) mx -= kRaised;
                     need = fresh ? mx != -INFINITY : mx > 8.0f;
                     m_new = (fresh ? 0.f : m_run) + mx;
                 }
@@ -1349,7 +1351,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
                 }
                 m_run = m_new;
-                const float mneg = (m_run == -INFINITY) ? 0.f : kRaised - m_run * c;
+                const float mneg = (m_run == -INFINITY) ? 0.f : E4M3 ? kRaised - m_run * c : -m_run * c;
                 // exp2(s*c - m*c) on packed pairs
                 const uint64_t c2 = pack_f2(c, c), mneg2 = pack_f2(mneg, mneg);
                 uint64_t lacc0 = pack_f2(0.f, 0.f), lacc1 = lacc0;
@@ -1372,7 +1374,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 else if (KIND == SCORE_CAPPED && late) exponentials([&](uint64_t s2) { return fma_f2(s2, cap_poly(s2, p.score), mneg2); });
                 else exponentials([&](uint64_t s2) { return s2; });
                 tc_wait_st();
-                if (!E4M3 && (real < kBlk || none)) alive = zero_behind(g, min(real, kBlk), none_from, none_end);
+                if (!E4M3 && (real < kBlk || none)) alive = zero_behind(g, MASKED ? min(real, kBlk) : real, none_from, none_end);
                 tc_fence_before();
                 mbar_arrive_warp(BAR(B_PFULL + g % NP), lane);
                 if (!alive) break;

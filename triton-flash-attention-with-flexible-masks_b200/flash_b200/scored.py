@@ -50,6 +50,9 @@ def _checked_prefix(prefix, B, N, q):
 
 def _checked_window(window, sinks):
     """Keys of the window, 0 for none, and the first tokens that it leaves visible."""
+    if window is None and type(sinks) is int and sinks == 0:
+        return 0, 0
+
     def number(x, name):
         try:
             return operator.index(x)
