@@ -279,3 +279,10 @@ def test_the_same_bits_again():
     for _ in range(3):
         got = _run(q, k, v, do, 200, 4)
         assert all(torch.equal(got[n], want[n]) for n in NAMES)
+
+
+@pytest.mark.parametrize("B,H,Hk,L,D,window,sinks", [(1, 4, 1, 1500, 64, 60, 1), (2, 2, 2, 700, 128, 100, 200), (1, 8, 2, 900, 32, 64, 33), (3, 2, 1, 1000, 16, 1, 3), (8, 8, 8, 400, 32, 20, 40)])
+def test_first_keys_that_all_queries_see_in_fp32(B, H, Hk, L, D, window, sinks):
+    """Blocks of 16 and of 32 keys."""
+    _compare(*_inputs(B, H, Hk, L, L, D, FP32, 29), window, sinks)
+    _compare(*_inputs(B, H, Hk, L - 90, L, D, FP32, 30), window, sinks, softcap=7.0, slopes=_slopes(H))

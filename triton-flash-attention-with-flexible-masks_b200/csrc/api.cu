@@ -299,9 +299,12 @@ size_t fwd_workspace_bytes(const fa_problem* p, int ns) {
 // fp32 inputs: which = 0 forward, 1 delta, 2 dK / dV, 3 dQ; absent tensors are null
 int run_f32(int which, const fa_problem* p, const fa_tensor* q, const fa_tensor* k, const fa_tensor* v, const fa_tensor* o,
             const fa_tensor* d_o, const fa_tensor* dq, const fa_tensor* dk, const fa_tensor* dv, float* lse, float* delta,
-            const void* plan, void* stream, const Changes* sc, bool overlap = false) {
+            const void* plan, void* stream, const Changes* sc, bool overlap = false, float* sums = nullptr, int runs = 1) {
     int rc;
     fa::F32Params fp{};
+    fp.sums = sums;
+    fp.parts = runs;
+    fp.split = sc ? std::min(sc->window.sinks, p->N) : 0;
     const struct { const fa_tensor* t; fa::F32Tensor* dst; int H, L; } all[8] = {
         {q, &fp.q, p->H, p->M}, {k, &fp.k, p->Hk, p->N}, {v, &fp.v, p->Hk, p->N}, {o, &fp.o, p->H, p->M},
         {d_o, &fp.d_o, p->H, p->M}, {dq, &fp.dq, p->H, p->M}, {dk, &fp.dk, p->Hk, p->N}, {dv, &fp.dv, p->Hk, p->N}};
@@ -434,9 +437,13 @@ int run_bwd_delta(const fa_problem* p, const void* rest, const fa_tensor* o, con
 // window 1024, 4 first keys, forward and backward, whole | cut 416 | - (without first keys 283).
 int query_runs(const fa_problem* p, const fa_window& w, int sms, int& early) {
     early = 0;
-    if (w.keys <= 0 || w.sinks <= 0 || !p->causal || p->dtype == FA_FP32) return 1;
+    if (w.keys <= 0 || w.sinks <= 0 || !p->causal) return 1;
     const int nq = fa::cdiv(p->M, fa::kBlk), nk = fa::cdiv(p->N, fa::kBlk);
     early = std::min(nk, fa::cdiv(std::min(w.sinks, p->N), fa::kBlk));
+    if (p->dtype == FA_FP32) {  // (64 queries at a time; there is one such block more for every 16 or 32 of the first keys)
+        const int tiles = fa::cdiv(p->M, 64), own = fa::cdiv(std::min(w.keys, p->N) + 32, 64) + 1;
+        return std::max(1, std::min(fa::cdiv(tiles, own), 32));
+    }
     const int64_t blocks = fa::cdiv(std::min(w.keys, p->N), fa::kBlk) + 1, share = int64_t(nk) * p->Hk * p->B * blocks / (2 * sms);
     const int64_t runs = (nq + std::max(blocks, share) - 1) / std::max(blocks, share);
     return int(std::max(int64_t(1), std::min(runs, int64_t(32))));
@@ -454,7 +461,7 @@ int run_bwd_dkdv(const fa_problem* p, const Changes* sc, const fa_tensor* q, con
     if (!lse || !delta || !status) return FA_ERR_BAD_ARG;
     if (!aligned16(lse) || !aligned16(delta)) return FA_ERR_ALIGNMENT;  // read with bulk copies
     if (p->dtype == FA_FP32)
-        return run_f32(2, p, q, k, v, nullptr, d_o, nullptr, dk, dv, const_cast<float*>(lse), const_cast<float*>(delta), plan, stream, sc);
+        return run_f32(2, p, q, k, v, nullptr, d_o, nullptr, dk, dv, const_cast<float*>(lse), const_cast<float*>(delta), plan, stream, sc, false, sums, runs);
     if ((rc = check_tensor(q, p->B, p->H, p->M))) return rc;
     if ((rc = check_tensor(d_o, p->B, p->H, p->M))) return rc;
     if ((rc = check_tensor(k, p->B, p->Hk, p->N))) return rc;
@@ -737,6 +744,7 @@ int fa_bwd_windowed(const fa_problem* p, const fa_scores* scores, const fa_windo
     if (!rc) rc = run_bwd_dkdv(p, &c, q, k, v, d_o, lse, delta, dk, dv, plan, status, stream, sums, early, runs);
     if (!rc) rc = run_bwd_dq(p, &c, q, k, v, d_o, lse, delta, dq, plan, status, true, stream);
     if (rc || runs < 2) return rc;
+    if (p->dtype == FA_FP32) return run_f32(4, p, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, dk, dv, nullptr, delta, plan, stream, &c, false, sums, runs);
     const fa::SumPartsParams sp{sums, out_view(dk), out_view(dv), early, runs, p->B, p->Hk, p->N, p->D, p->D > 64 ? 128 : 64, p->sm_scale, status};
     return fa::launch_sum_parts(p->dtype == FA_BF16, sp, static_cast<cudaStream_t>(stream)) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
@@ -746,7 +754,7 @@ int fa_bwd_workspace_bytes(const fa_problem* p, const fa_window* window, size_t*
     const int rc = check_problem(p);
     if (rc) return rc;
     *bytes = 0;
-    if (!window || window->keys <= 0 || window->sinks <= 0 || !p->causal || p->dtype == FA_FP32) return FA_OK;
+    if (!window || window->keys <= 0 || window->sinks <= 0 || !p->causal) return FA_OK;
     const int sms = sm_count();
     if (sms <= 0) return FA_ERR_LAUNCH;
     int early;

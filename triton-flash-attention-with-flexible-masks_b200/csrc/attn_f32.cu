@@ -235,6 +235,17 @@ __device__ __forceinline__ int next_tile(const uint8_t* visited, int c, int end)
     return c;
 }
 
+// The same for a block of queries from i0 on; with a window columns that lie whole between the first keys and the window are passed over, too.
+template <bool WINDOW>
+__device__ __forceinline__ int next_keys(const uint8_t* visited, const MaskArgs& mk, int c, int end, int i0, int front) {
+    c = next_tile(visited, c, end);
+    if constexpr (WINDOW) {
+        const int low = i0 + mk.gap - mk.window + 1, early = early_keys<true>(front, mk.sinks);
+        while (c < end && c + kC <= low && c >= early) c = next_tile(visited, c + kC, end);
+    }
+    return c;
+}
+
 __device__ __forceinline__ int code_q(const MaskArgs& mk, int b, int he, int i) {
     return (mk.mode == 1 && i < mk.M) ? mk.plan[mk.L.off_qc + (int64_t(b) * mk.He + he) * mk.L.Mpad + i] : 0;
 }
@@ -292,11 +303,12 @@ __global__ void __launch_bounds__(threads(R), R == 32 && D <= 32 ? 4 : 0) f32_fw
         qc[r] = code_q(mk, b, he, i0 + r0 + r);
     }
     __syncthreads();
-    int j0 = next_tile(visited, 0, end);
+    auto next = [&](int c) { return next_keys<WINDOW>(visited, mk, c, end, i0, front); };
+    int j0 = next(0);
     if (j0 < end) fetch(j0, 0);
     cp_async_commit();
     for (int st = 0; j0 < end; st ^= 1) {
-        const int jn = next_tile(visited, j0 + kC, end);
+        const int jn = next(j0 + kC);
         if (jn < end) fetch(jn, st ^ 1);
         cp_async_commit();
         cp_async_wait<1>();
@@ -414,11 +426,12 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dq_kernel(const F32Params 
         qc[r] = code_q(mk, b, he, i);
     }
     __syncthreads();
-    int j0 = next_tile(visited, 0, end);
+    auto next = [&](int c) { return next_keys<WINDOW>(visited, mk, c, end, i0, front); };
+    int j0 = next(0);
     if (j0 < end) fetch(j0, 0);
     cp_async_commit();
     for (int st = 0; j0 < end; st ^= 1) {
-        const int jn = next_tile(visited, j0 + kC, end);
+        const int jn = next(j0 + kC);
         if (jn < end) fetch(jn, st ^ 1);
         cp_async_commit();
         cp_async_wait<1>();
@@ -475,7 +488,9 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
     float* vecs = Pall + S::p;              // two stages of id code, lse, delta per query
     __shared__ uint8_t visited[kListCap];
     const MaskArgs& mk = p.mask;
-    const int j0 = blockIdx.z * R, hk = blockIdx.x, b = blockIdx.y;
+    const int n_split = WINDOW && p.parts > 1 ? cdiv(p.split, R) : 0, kb = int(blockIdx.z) < n_split * p.parts ? int(blockIdx.z) / p.parts : int(blockIdx.z) - n_split * (p.parts - 1);
+    const int part = int(blockIdx.z) < n_split * p.parts ? int(blockIdx.z) - kb * p.parts : -1;  // the cut blocks first
+    const int j0 = (WINDOW ? kb : int(blockIdx.z)) * R, hk = blockIdx.x, b = blockIdx.y;
     const int x = threadIdx.x & 31, r0 = (threadIdx.x >> 5) * kRW;
     const float* kbase = p.k.ptr + int64_t(b) * p.k.sb + int64_t(hk) * p.k.sh;
     const float* vbase = p.v.ptr + int64_t(b) * p.v.sb + int64_t(hk) * p.v.sh;
@@ -488,6 +503,16 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
     const int front = front_keys<SCORED>(mk, b);
     const int first = mk.causal && (!SCORED || j0 >= front) ? max(0, j0 - mk.gap) : 0;
     const int first_half = mk.causal && r0 >= 16 && (!SCORED || j0 + 16 >= front) ? j0 + 16 - mk.gap : 0;  // the same for the second half of 32 keys (see the forward)
+    int begin = first / kC * kC, stop = mk.M;  // rows that the block has to do with
+    if constexpr (WINDOW) {
+        if (part >= 0) {
+            const int t0 = begin / kC, n = cdiv(mk.M, kC) - t0;
+            begin = (t0 + n * part / p.parts) * kC;
+            stop = min(mk.M, (t0 + n * (part + 1) / p.parts) * kC);
+        } else if (j0 >= early_keys<true>(front, mk.sinks)) {
+            stop = min(mk.M, j0 + R - 1 + mk.window - mk.gap);
+        }
+    }
     for (int g = 0; g < p.G; ++g) {
         const int h = hk * p.G + g;
         const int he = (mk.He == 1) ? 0 : h;
@@ -516,12 +541,12 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
 #pragma unroll
         for (int r = 0; r < kRW; ++r) kc[r] = code_k(mk, b, he, j0 + r0 + r);
         __syncthreads();
-        int i0 = next_tile(visited, first / kC * kC, mk.M);
-        if (i0 < mk.M) fetch(i0, 0);
+        int i0 = next_tile(visited, begin, stop);
+        if (i0 < stop) fetch(i0, 0);
         cp_async_commit();
-        for (int st = 0; i0 < mk.M; st ^= 1) {
-            const int in = next_tile(visited, i0 + kC, mk.M);
-            if (in < mk.M) fetch(in, st ^ 1);
+        for (int st = 0; i0 < stop; st ^= 1) {
+            const int in = next_tile(visited, i0 + kC, stop);
+            if (in < stop) fetch(in, st ^ 1);
             cp_async_commit();
             cp_async_wait<1>();
             __syncthreads();
@@ -565,6 +590,14 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
         const int j = j0 + r0 + r;
         if (j >= mk.N) continue;
         float own[Own<D>::N];
+        if (WINDOW && part >= 0) {  // sums of a run of queries, which are added up later
+            float* const to = p.sums + ((((int64_t(part) * n_split + kb) * p.B + b) * p.Hk + hk) * (2 * R) + r0 + r) * D;
+            dv.row(r, own);
+            Own<D>::store(to, x, true, own, 1.f);
+            dk.row(r, own);
+            Own<D>::store(to + R * D, x, true, own, p.scale);
+            continue;
+        }
         dk.row(r, own);
         Own<D>::store(dkbase + int64_t(j) * p.dk.sl, x, dkvec, own, p.scale);  // flash_triton.py:313
         dv.row(r, own);
@@ -572,22 +605,43 @@ __global__ void __launch_bounds__(threads(R)) f32_bwd_dkdv_kernel(const F32Param
     }
 }
 
+// dK and dV of blocks that were cut into runs of queries: the runs' sums, in their order. A thread a number.
+template <int D, int R>
+__global__ void __launch_bounds__(256) f32_sum_parts_kernel(const F32Params p) {
+    follow_stream();
+    const int blocks = cdiv(p.split, R);
+    const int64_t n = int64_t(blocks) * p.B * p.Hk * (2 * R * D), at = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (at >= n) return;
+    const int d = int(at % D), r = int(at / D % R), which = int(at / (R * D) & 1);
+    const int64_t block = at / (2 * R * D);
+    const int hk = int(block % p.Hk), b = int(block / p.Hk % p.B), j = int(block / p.Hk / p.B) * R + r;
+    if (j >= p.mask.N) return;
+    float sum = 0.f;
+    for (int s = 0; s < p.parts; ++s) sum += p.sums[at + s * n];
+    const F32Tensor& t = which ? p.dk : p.dv;
+    t.ptr[int64_t(b) * t.sb + int64_t(hk) * t.sh + int64_t(j) * t.sl + d] = sum;
+}
+
 // ---------------------------------------------------------------------------------------------
 template <int D, int R, bool SCORED, bool WINDOW>
 static cudaError_t launch_f32_t(int which, const F32Params& p, bool overlap, cudaStream_t stream) {
     using S = F32Smem<D, R>;
     const MaskArgs& mk = p.mask;
-    static SmemAllowed allowed[4];
+    static SmemAllowed allowed[4];  // (which 4 asks for none)
     auto run = [&](auto kern, int smem, int rows, int heads) {
         const cudaError_t e = allow_smem(kern, smem, allowed[which]);
         if (e != cudaSuccess) return e;
         // the blocks of all heads with many tiles first: with those of one head behind each other the last long ones started late (4 x 8
         // heads x 1024 x 64, forward and backward 851 -> 729 us)
-        const dim3 grid(heads, p.B, cdiv(rows, R));
+        const dim3 grid(heads, p.B, cdiv(rows, R) + (WINDOW && which == 2 && p.parts > 1 ? cdiv(p.split, R) * (p.parts - 1) : 0));
         if (which != 3 || overlap) return launch_overlapping(kern, grid, threads(R), smem, stream, p);
         kern<<<grid, threads(R), smem, stream>>>(p);
         return cudaGetLastError();
     };
+    if (which == 4) {
+        const int64_t n = int64_t(cdiv(p.split, R)) * p.B * p.Hk * (2 * R * D);
+        return launch_overlapping(f32_sum_parts_kernel<D, R>, dim3(unsigned((n + 255) / 256)), 256, 0, stream, p);
+    }
     if (which == 0) return run(f32_fwd_kernel<D, R, SCORED, WINDOW>, S::fwd_bytes, mk.M, p.H);
     if (which == 2) return run(f32_bwd_dkdv_kernel<D, R, SCORED, WINDOW>, S::bwd_bytes, mk.N, p.Hk);
     return run(f32_bwd_dq_kernel<D, R, SCORED, WINDOW>, S::bwd_bytes, mk.M, p.H);
@@ -612,7 +666,7 @@ static cudaError_t launch_f32_rows(int which, const F32Params& p, bool overlap, 
     return small ? launch_f32_t<D, 16, false, false>(which, p, overlap, stream) : launch_f32_t<D, 32, false, false>(which, p, overlap, stream);
 }
 
-// which: 0 forward, 1 delta, 2 dK / dV, 3 dQ. overlap: the launch directly before this one in the stream is the dK/dV
+// which: 0 forward, 1 delta, 2 dK / dV, 3 dQ, 4 what adds up the runs of dK / dV. overlap: the launch directly before this one in the stream is the dK/dV
 // kernel of the same backward, and the blocks of this one (dQ) may run beside its: two of 32 rows fit on an SM up to D = 64, and
 // one alone leaves its FMA pipes idle most of the time. Whole backward, us, one behind the other and side by side (blocks of 32 rows): 8 heads x 512 x 64 causal 104,
 // 82; 8 heads x 1024 283, 223; 32 heads x 1024 694, 634; 2 heads x 100 36, 22; D = 128, 8 heads x 512, 160, 136 (there dQ only

@@ -107,6 +107,9 @@ struct F32Params {
     int B, H, Hk, G;
     float scale;
     ScoreArgs score;  // the instances for attention_scored: cap and slopes
+    // With a window: dK / dV of the blocks with its first `split` keys are cut into `parts` runs of queries (1: they are not), whose sums go to [parts, blocks, B, Hk, dV and dK, R, D]
+    int split, parts;
+    float* sums;
 };
 
 // Attention over a paged cache (paged_fwd.cu), and the tokens' way into it (paged_append.cu)
