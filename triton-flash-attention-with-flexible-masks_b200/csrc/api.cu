@@ -434,7 +434,7 @@ int run_bwd_delta(const fa_problem* p, const void* rest, const fa_tensor* o, con
 
 // Into how many runs of queries dK / dV of the blocks with a window's first keys are cut, which every query sees something of: their items are as long as the others' then. With
 // `early` such blocks, and one run where nothing is gained, because the window is nearly as long or because there is so much other work that it hides them. us, 2 x 16 / 4 heads x 4000 x 128,
-// window 1024, 4 first keys, forward and backward, whole | cut 416 | - (without first keys 283).
+// window 1024, 4 first keys, forward and backward, whole | cut 416 | 317 (without first keys 283).
 int query_runs(const fa_problem* p, const fa_window& w, int sms, int& early) {
     early = 0;
     if (w.keys <= 0 || w.sinks <= 0 || !p->causal) return 1;

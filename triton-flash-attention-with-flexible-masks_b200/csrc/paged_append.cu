@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Page
 // numbers beyond 448 * 2^7 = 57344 become that.
 //
 // Moves 6 bytes for each element of K (2 read and 1 written, of K and of V each) and a byte for each row. The lanes that hold a head's row (16 at a head dim of 128) find its largest
-// number among them by shuffles, in registers.
+// number among them by shuffles, in registers. Bound by HBM, nearly by the ALU: each number in fp32 by itself, with its own look at whether it is finite, 115 instructions for 8 numbers and 66 % of
+// the ALU, 8 prompts of 3500 tokens, 8 heads of 128, pages of 16, 32.0 us.
 template <int kLog2Row, bool BF16>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_e4m3_kernel(const PagedParams p, const AppendRows in, const AppendPages8 to) {
     follow_stream();
@@ -132,27 +133,38 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_e4m3_kernel(const
     fetch(0);
     int page, slot;
     if (!place_of(p, t, lane, page, slot)) return;
-    auto put = [&](const uint4& row, uint8_t* data, uint8_t* scale, bool real, bool first) {
-        float x[8], most = 0.f;
-        unpack2<BF16>(row.x, x[0], x[1]);
-        unpack2<BF16>(row.y, x[2], x[3]);
-        unpack2<BF16>(row.z, x[4], x[5]);
-        unpack2<BF16>(row.w, x[6], x[7]);
+    constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
+    auto put = [&](uint4 row, uint8_t* data, uint8_t* scale, bool real, bool first) {
+        uint32_t w[4] = {row.x, row.y, row.z, row.w}, most = 0;
+        // (numbers of 16 bits without their sign go by size)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (!(fabsf(x[i]) < INFINITY)) x[i] = __int_as_float(0x7fffffff);
-            most = fmaxf(most, fabsf(x[i]));  // (a NaN is no maximum)
+        for (int i = 0; i < 4; ++i) most = __vmaxu2(most, w[i] & 0x7fff7fffu);
+        most = max(most & 0xffffu, most >> 16);
+        if (__any_sync(0xffffffffu, most >= kInf)) {  // not finite: NaN, which have no say
+            most = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t lo = w[i] & 0x7fffu, hi = w[i] >> 16 & 0x7fffu;
+                if (lo >= kInf) w[i] |= 0x7fffu; else most = max(most, lo);
+                if (hi >= kInf) w[i] |= 0x7fff0000u; else most = max(most, hi);
+            }
         }
 #pragma unroll
-        for (int o = 1; o <= kMask; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        const uint32_t bits = __float_as_uint(most);  // 448 = 1.75 * 2^8
+        for (int o = 1; o <= kMask; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        float largest, none;
+        unpack2<BF16>(most, largest, none);
+        const uint32_t bits = __float_as_uint(largest);  // 448 = 1.75 * 2^8
         const int biased = min(max(int(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), kScaleLeast), kScaleMost);
-        const float inverse = __uint_as_float(uint32_t(254 - biased) << 23);
         if (!real) return;
-        uint2 e;
-        e.x = pack_e4m3x2(x[0] * inverse, x[1] * inverse) | pack_e4m3x2(x[2] * inverse, x[3] * inverse) << 16;
-        e.y = pack_e4m3x2(x[4] * inverse, x[5] * inverse) | pack_e4m3x2(x[6] * inverse, x[7] * inverse) << 16;
-        *reinterpret_cast<uint2*>(data) = e;
+        const float inverse = __uint_as_float(uint32_t(254 - biased) << 23);
+        uint32_t e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float lo, hi;
+            unpack2<BF16>(w[i], lo, hi);
+            e[i] = pack_e4m3x2(lo * inverse, hi * inverse);
+        }
+        *reinterpret_cast<uint2*>(data) = make_uint2(__byte_perm(e[0], e[1], 0x5410), __byte_perm(e[2], e[3], 0x5410));
         if (first) *scale = uint8_t(biased);
     };
     uint8_t* const k_to = to.k + page * to.k_p + slot * to.k_s;

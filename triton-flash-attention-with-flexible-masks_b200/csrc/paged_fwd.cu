@@ -37,8 +37,8 @@ namespace fa {
 // each tile into the fp16 tile that the products read (a row is e4m3 times a power of two from 2^-15 to 2^7, all of whose numbers are fp16's: nothing is rounded), K a tile ahead of V, and hidden
 // rows into zeros. The products are fp16's also where q is bf16: q's rows are brought to fp16, by a power of two where their greatest entry asks for it (their scores take it back in fp32),
 // and P is 2^7 times as large as elsewhere, which brings what fp16 cannot tell from 0 from 2^-25 down to 2^-32 of a row's reference (l and O have the factor alike).
-// FORM_DIRECT: of 8 bits and single tokens of few heads, as the host can tell: all items are multiplied by warps from the rings, and these have nearly all of shared memory. (Of 64 tokens over 650 MB
-// 150 us with 3 and 2 places of 16 KB, which are all that the tiles of the tensor cores leave.)
+// FORM_DIRECT: of 8 bits and single tokens of few heads, as the host can tell: all items are multiplied by warps from the rings, and these have nearly all of shared memory. (The tiles of the tensor cores leave 3 and
+// 2 places of 16 KB.)
 enum : int { FORM_PLAIN = 0, FORM_MASKED = 1, FORM_E4M3 = 2, FORM_DIRECT = 4 };
 
 constexpr int kDirectRows = 16;  // E4M3: of an item, up to which warps multiply it directly
@@ -214,7 +214,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     auto sV = [&](int s) { return sbase + S::off_v + uint32_t(s) * S::TILE; };
     // E4M3: the g-th tile of K or V (the rings' raw_g-th), rows of D numbers in e4m3 to 64-column boxes of fp16 with the swizzle that the products read, by four warps. A thread takes 16
     // numbers at a time. In a loop, and in one place of the code for K and one for V: with the loop unrolled and V's in three places, whose code the softmax groups fetch beside their own, warps
-    // stood without an instruction more than anything else (five chunks and tokens over 131 MB 525 us).
+    // stood without an instruction more than anything else (three chunks of up to 500 and five tokens over 131 MB, 32 / 8 heads of 128, 525 us for 318).
     auto unpack_tile = [&](auto values, int g, int raw_g, int k0, int seen, int early, int low) {
         constexpr bool V = decltype(values)::value;
         const int r = tid & 127;
@@ -882,7 +882,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     // alone, so that it takes neighbouring bytes: of K's rows 4 a step, of V's the D / 8 of each of its keys. K's scales go to the scores, V's to the numbers, which fp16 holds exactly.
                     // A warp has a tile's bytes in registers before it begins, and has given the rings' places back; nothing else waits. Clocks a tile of 128 keys of 128: HBM's share of an SM 1400,
                     // conversions 450 of the ALU, products 256. 64 tokens, 32 / 8 heads of 128, over 650 MB, us: by the tensor memory's way 345; rows as M, 16 keys a warp of every tile 187; rows as
-                    // N 154.
+                    // N 154; 32 keys of every other tile 150; rings of 128 KB, and no spilled registers, 136.
                     alive = mbar_wait_warp(BAR(B_QFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 3);
                     if (!alive) break;
                     __syncwarp();  // (a row's mask is its lane's)
