@@ -286,3 +286,30 @@ def test_first_keys_that_all_queries_see_in_fp32(B, H, Hk, L, D, window, sinks):
     """Blocks of 16 and of 32 keys."""
     _compare(*_inputs(B, H, Hk, L, L, D, FP32, 29), window, sinks)
     _compare(*_inputs(B, H, Hk, L - 90, L, D, FP32, 30), window, sinks, softcap=7.0, slopes=_slopes(H))
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("B,Hk,L,D,window,sinks", [(1, 1, 131072, 128, 1, 131072), (1, 1, 131072, 128, 1000, 60000), (4, 8, 20000, 64, 64, 5000), (1, 1, 8000, 128, 1, 300), (64, 32, 4000, 128, 4, 4)])
+def test_runs_of_queries_stay_few(B, Hk, L, D, window, sinks, dtype):
+    """Where there are many first keys they are work enough by themselves: the workspace holds some blocks' sums for each SM, not 32 times all of dK and dV."""
+    import ctypes
+    from flash_b200 import _lib
+    problem, size = _lib.Problem(), ctypes.c_size_t(0)
+    for name, value in dict(B=B, H=Hk, Hk=Hk, M=L, N=L, D=D, dtype=dtype, causal=1, mode=0, id_heads=1, sm_scale=0.1).items():
+        setattr(problem, name, value)
+    _lib.check(_lib.load().fa_bwd_workspace_bytes(problem, _lib.Window(window, sinks), size), "fa_bwd_workspace_bytes")
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    # S = 2 SMs (fp32: 8, of blocks of 32 keys). All the work is W >= blocks * walk, a run is at least floor(W / S), which is at least W / 2S if it is 1, and walk / run + 1 bounds the runs: those of
+    # all blocks are at most 2 S + blocks; where there are two runs floor(W / S) < walk, so that blocks < S. (fp32 gives a block of 32 keys at most the room of 128.)
+    most = (3 * 8 if dtype == 2 else 3 * 2) * sms
+    assert size.value <= most * 2 * 128 * max(D, 64) * 4
+
+
+
+def test_many_first_keys_in_fp32():
+    """As many blocks, times 32 runs of queries, would be more than a launch can have. A window of one key with all keys first ones, and one of all keys, see the same."""
+    L = 70000
+    q, k, v, do = _inputs(1, 1, 1, L, L, 16, FP32, 33)
+    a, b = _run(q, k, v, do, 1, L), _run(q, k, v, do, L, 0)
+    for n in NAMES:
+        assert torch.equal(a[n], b[n]), n

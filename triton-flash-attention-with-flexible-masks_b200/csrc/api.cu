@@ -432,21 +432,21 @@ int run_bwd_delta(const fa_problem* p, const void* rest, const fa_tensor* o, con
     return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
-// Into how many runs of queries dK / dV of the blocks with a window's first keys are cut, which every query sees something of: their items are as long as the others' then. With
-// `early` such blocks, and one run where nothing is gained, because the window is nearly as long or because there is so much other work that it hides them. us, 2 x 16 / 4 heads x 4000 x 128,
-// window 1024, 4 first keys, forward and backward, whole | cut 416 | 317 (without first keys 283).
+// Into how many runs of queries dK / dV of the blocks with a window's first keys are cut, which every query sees something of: a run is as long as the others' walks, or as half of an SM's
+// share of all the work, whichever is more. (Without the share many first keys, which make work enough by themselves, would ask for a workspace of gigabytes; with it a GPU's SMs have
+// about four blocks of sums each.) With `early` such blocks. us, 2 x 16 / 4 heads x 4000 x 128, window 1024, 4 first keys, forward and backward, whole | cut 416 | 317 (without first
+// keys 283).
 int query_runs(const fa_problem* p, const fa_window& w, int sms, int& early) {
     early = 0;
     if (w.keys <= 0 || w.sinks <= 0 || !p->causal) return 1;
-    const int nq = fa::cdiv(p->M, fa::kBlk), nk = fa::cdiv(p->N, fa::kBlk);
-    early = std::min(nk, fa::cdiv(std::min(w.sinks, p->N), fa::kBlk));
-    if (p->dtype == FA_FP32) {  // (64 queries at a time; there is one such block more for every 16 or 32 of the first keys)
-        const int tiles = fa::cdiv(p->M, 64), own = fa::cdiv(std::min(w.keys, p->N) + 32, 64) + 1;
-        return std::max(1, std::min(fa::cdiv(tiles, own), 32));
-    }
-    const int64_t blocks = fa::cdiv(std::min(w.keys, p->N), fa::kBlk) + 1, share = int64_t(nk) * p->Hk * p->B * blocks / (2 * sms);
-    const int64_t runs = (nq + std::max(blocks, share) - 1) / std::max(blocks, share);
-    return int(std::max(int64_t(1), std::min(runs, int64_t(32))));
+    const int keys = std::min(w.keys, p->N), sinks = std::min(w.sinks, p->N);
+    const bool f32 = p->dtype == FA_FP32;
+    early = fa::cdiv(sinks, fa::kBlk);
+    // fp32: 64 queries at a time for 16 or 32 keys, and four blocks on an SM
+    const int64_t walk = f32 ? fa::cdiv(p->M, 64) : fa::cdiv(p->M, fa::kBlk), own = f32 ? fa::cdiv(keys + 32, 64) + 1 : fa::cdiv(keys, fa::kBlk) + 1;
+    const int64_t others = fa::cdiv(p->N, f32 ? 32 : fa::kBlk), first = f32 ? fa::cdiv(sinks, 32) : early;
+    const int64_t share = (others * own + first * walk) * p->Hk * p->B / ((f32 ? 8 : 2) * sms), run = std::max(own, share);
+    return int(std::max(int64_t(1), std::min((walk + run - 1) / run, int64_t(32))));
 }
 size_t runs_bytes(const fa_problem* p, int early, int runs) {
     return runs > 1 ? size_t(runs) * early * p->B * p->Hk * 2 * fa::kBlk * (p->D > 64 ? 128 : 64) * sizeof(float) : 0;
