@@ -367,3 +367,22 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     fb.check_status()
     assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D,page", [(128, 16), (64, 16), (128, 64), (64, 256)])
+def test_items_of_both_kinds_in_turn(D, page, dtype):
+    """Single tokens, which warps multiply as they read the rings, between chunks, which the tensor cores do, with odd and even numbers of tiles; the rings' places go to both groups of
+    warps then, and loads of small pages land in any order. The same bits each time."""
+    import flash_b200 as fb
+    lens = [1 + (977 * b * b + 613 * b) % 2500 for b in range(36)]
+    new = [1 if b % 3 else min(lens[b], 40 + 5 * b) for b in range(36)]
+    cache = Cache8(lens, 2, D, page, dtype, 41).fill()
+    q, first = _attend(cache, 8, new, dtype)
+    for _ in range(40):
+        assert torch.equal(fb.paged_attention(q, *cache.args(), _starts(new), **cache.scales()), first)
+    single = q[:36].contiguous()
+    once = fb.paged_attention(single, *cache.args(), torch.arange(37, dtype=torch.int32, device="cuda"), **cache.scales())
+    for _ in range(20):
+        assert torch.equal(fb.paged_attention(single, *cache.args(), torch.arange(37, dtype=torch.int32, device="cuda"), **cache.scales()), once)
+    fb.check_status()

@@ -33,15 +33,17 @@ namespace fa {
 // Instances. FORM_MASKED: perhaps a window, perhaps drafted tokens whose parents are given. A tile of keys that the window hides from all of an item's tokens is not among its
 // tiles, and what lies in such keys of the others is as far from the results as what lies behind the sequence: V's rows are zeroed, scores masked. A drafted token's branch is
 // walked once an item, by the thread of each of its rows, while the first keys are on their way, and left as bits in shared memory.
-// FORM_E4M3: the cache is of 8 bits. The rows of K and V land as they are in rings of their own, with their scales; the epilogue group, which has nothing to do while an item lasts, turns
-// each tile into the fp16 tile that the products read (a row is e4m3 times a power of two from 2^-15 to 2^7, all of whose numbers are fp16's: nothing is rounded), K a tile ahead of V, and hidden
-// rows into zeros. The products are fp16's also where q is bf16: q's rows are brought to fp16, by a power of two where their greatest entry asks for it (their scores take it back in fp32),
+// FORM_E4M3: the cache is of 8 bits. The rows of K and V land as they are in rings of their own, with their scales; each tile is turned
+// into the fp16 tile that the products read (a row is e4m3 times a power of two from 2^-15 to 2^7, all of whose numbers are fp16's: nothing is rounded), with hidden rows as zeros: K's by the epilogue
+// group, which has nothing to do while an item lasts, V's by the softmax group that owns the tile. The products are fp16's also where q is bf16: q's rows are brought to fp16, by a power of two where their greatest entry asks for it (their scores take it back in fp32),
 // and P is 2^7 times as large as elsewhere, which brings what fp16 cannot tell from 0 from 2^-25 down to 2^-32 of a row's reference (l and O have the factor alike).
 // FORM_DIRECT: of 8 bits and single tokens of few heads, as the host can tell: all items are multiplied by warps from the rings, and these have nearly all of shared memory. (The tiles of the tensor cores leave 3 and
 // 2 places of 16 KB.)
 enum : int { FORM_PLAIN = 0, FORM_MASKED = 1, FORM_E4M3 = 2, FORM_DIRECT = 4 };
 
-constexpr int kDirectRows = 16;  // E4M3: of an item, up to which warps multiply it directly
+// E4M3: rows of an item up to which warps multiply it directly. us, 32 single tokens over 349 MB, 8 kv heads of 128, 8 | 16 heads a kv head: by the tensor cores - | 148, directly 88 | 114, in
+// the instance of single tokens 79 | 117.
+constexpr int kDirectRows = 16;
 
 template <int D, int FORM>
 struct PagedSmem {
@@ -64,6 +66,10 @@ struct PagedSmem {
     // E4M3: rings of rows as they are, and of their scales; the factor of each row's scores
     static constexpr int RAW = E4M3 ? kBlk * D : 0;
     static constexpr int NRK = !E4M3 ? 0 : DIRECT ? (D == 128 ? 4 : 8) : D == 128 ? 3 : 5, NRV = !E4M3 ? 0 : DIRECT ? NRK : D == 128 ? 2 : 5;
+    // Barriers of those rings, and of V's places that have been read. A wait goes by a phase's parity, so that whoever waits must have seen the phase before: the groups take tiles in turn, and with
+    // an odd number of places, which both groups come to, there are two barriers a place, one for each group's tiles. (A tile that lands before the one in front of it would let a group through a phase early.)
+    static constexpr int NBK = NRK % 2 ? 2 * NRK : NRK, NBV = NRV % 2 ? 2 * NRV : NRV, NVE = E4M3 && NS % 2 ? 2 * NS : NS;
+    static_assert(!E4M3 || (NBK % 2 == 0 && NBV % 2 == 0 && NVE % 2 == 0), "a group comes to the same barriers again");
     static constexpr int SUMS = 8 * kDirectRows * D * 4, off_sums = off_k;  // E4M3: what the warps leave of O; K's and V's tiles have the place, or nobody else
     static_assert(DIRECT || !E4M3 || SUMS <= 2 * NS * TILE, "room for the sums");
     static constexpr int off_raw_k = DIRECT ? off_sums + SUMS : off_v + NS * TILE, off_raw_v = off_raw_k + NRK * RAW;
@@ -73,9 +79,9 @@ struct PagedSmem {
     static constexpr int off_factor = off_scale_v + NRV * kBlk;  // float [NQ][128]
     static constexpr int off_plan = off_factor + (E4M3 ? NQ * kBlk * 4 : 0);
     static constexpr int off_bar = off_plan + int(sizeof(PagedPlan));
-    // item_full[NQ] item_empty[NQ] q_full[NQ] ml_full[NQ] staged k_full[NS] k_empty[NS] v_full[NS] v_empty[NS]
-    // s_full[4] s_free[2] p_full[NP] pv_done[NP] o_full[2] o_free[2]; E4M3: raw_k_full[NRK] raw_k_empty[NRK] raw_v_full[NRV] raw_v_empty[NRV] q_ready[NQ] sums_free
-    static constexpr int n_common = 4 * NQ + 1 + 4 * NS + 6 + 2 * NP + 4, n_bar = n_common + 2 * NRK + 2 * NRV + (E4M3 ? NQ + 1 : 0);
+    // item_full[NQ] item_empty[NQ] q_full[NQ] ml_full[NQ] staged k_full[NS] k_empty[NS] v_full[NS] v_empty[NVE]
+    // s_full[4] s_free[2] p_full[NP] pv_done[NP] o_full[2] o_free[2]; E4M3: raw_k_full[NBK] raw_k_empty[NBK] raw_v_full[NBV] raw_v_empty[NBV] q_ready[NQ] sums_free
+    static constexpr int n_common = 4 * NQ + 1 + 3 * NS + NVE + 6 + 2 * NP + 4, n_bar = n_common + 2 * NBK + 2 * NBV + (E4M3 ? NQ + 1 : 0);
     static constexpr int off_misc = off_bar + n_bar * 8;  // tmem slot, abort flag
     static constexpr int total = off_misc + 16;
     static_assert(off_plan % 8 == 0 && off_bar % 8 == 0, "alignment");
@@ -136,10 +142,10 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const uint32_t bar0 = sbase + S::off_bar;
     auto BAR = [&](int i) { return bar0 + 8u * uint32_t(i); };
     constexpr int B_ITEMFULL = 0, B_ITEMEMPTY = NQ, B_QFULL = 2 * NQ, B_MLFULL = 3 * NQ, B_STAGED = 4 * NQ, B_KFULL = 4 * NQ + 1,
-                  B_KEMPTY = B_KFULL + NS, B_VFULL = B_KEMPTY + NS, B_VEMPTY = B_VFULL + NS, B_SFULL = B_VEMPTY + NS,
+                  B_KEMPTY = B_KFULL + NS, B_VFULL = B_KEMPTY + NS, B_VEMPTY = B_VFULL + NS, B_SFULL = B_VEMPTY + S::NVE,
                   B_SFREE = B_SFULL + 4, B_PFULL = B_SFREE + 2, B_PVDONE = B_PFULL + NP, B_OFULL = B_PVDONE + NP, B_OFREE = B_OFULL + 2;
     static_assert(B_OFREE + 2 == S::n_common, "barriers");
-    constexpr int B_RAWK = S::n_common, B_RAWKEMPTY = B_RAWK + S::NRK, B_RAWV = B_RAWKEMPTY + S::NRK, B_RAWVEMPTY = B_RAWV + S::NRV, B_QREADY = B_RAWVEMPTY + S::NRV, B_SUMSFREE = B_QREADY + NQ;
+    constexpr int B_RAWK = S::n_common, B_RAWKEMPTY = B_RAWK + S::NBK, B_RAWV = B_RAWKEMPTY + S::NBK, B_RAWVEMPTY = B_RAWV + S::NBV, B_QREADY = B_RAWVEMPTY + S::NBV, B_SUMSFREE = B_QREADY + NQ;
     Abort ab{misc + 1, p.status, p.wait_limit};
 
     if (tid == 0) {
@@ -153,14 +159,14 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             mbar_init(BAR(B_KFULL + s), E4M3 ? 4 : 1);  // (the warps that make the tile)
             mbar_init(BAR(B_KEMPTY + s), 1);
             mbar_init(BAR(B_VFULL + s), E4M3 ? 4 : 1);
-            mbar_init(BAR(B_VEMPTY + s), 1);
         }
+        for (int s = 0; s < S::NVE; ++s) mbar_init(BAR(B_VEMPTY + s), 1);
         if constexpr (E4M3) {
-            for (int s = 0; s < S::NRK; ++s) {
+            for (int s = 0; s < S::NBK; ++s) {
                 mbar_init(BAR(B_RAWK + s), 1);
                 mbar_init(BAR(B_RAWKEMPTY + s), 4);
             }
-            for (int s = 0; s < S::NRV; ++s) {
+            for (int s = 0; s < S::NBV; ++s) {
                 mbar_init(BAR(B_RAWV + s), 1);
                 mbar_init(BAR(B_RAWVEMPTY + s), 4);
             }
@@ -218,10 +224,10 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     auto unpack_tile = [&](auto values, int g, int raw_g, int k0, int seen, int early, int low) {
         constexpr bool V = decltype(values)::value;
         const int r = tid & 127;
-        constexpr int R = V ? S::NRV : S::NRK, kThreadsARow = D / 16, kRows = kBlk / kThreadsARow;  // kRows: that the group takes together
+        constexpr int R = V ? S::NRV : S::NRK, RB = V ? S::NBV : S::NBK, NE = V ? S::NVE : NS, kThreadsARow = D / 16, kRows = kBlk / kThreadsARow;  // kRows: that the group takes together
         const int raw = raw_g % R, st = g % NS;
-        if (!mbar_wait_warp(BAR((V ? B_RAWV : B_RAWK) + raw), (raw_g / R) & 1, ab, ST_WAIT_TIMEOUT + 20)) return false;
-        if (g >= NS && !mbar_wait_warp(BAR((V ? B_VEMPTY : B_KEMPTY) + st), (g / NS - 1) & 1, ab, ST_WAIT_TIMEOUT + 21)) return false;
+        if (!mbar_wait_warp(BAR((V ? B_RAWV : B_RAWK) + raw_g % RB), (raw_g / RB) & 1, ab, ST_WAIT_TIMEOUT + 20)) return false;
+        if (g >= NS && !mbar_wait_warp(BAR((V ? B_VEMPTY : B_KEMPTY) + (g - NS) % NE), ((g - NS) / NE) & 1, ab, ST_WAIT_TIMEOUT + 21)) return false;
         const int part = r % kThreadsARow, row0 = r / kThreadsARow;
         const uint8_t* from = smem + (V ? S::off_raw_v : S::off_raw_k) + raw * S::RAW + raw_place<D>(row0, part);  // (the rows that a thread takes have one swizzle)
         const uint8_t* scales = smem + (V ? S::off_scale_v : S::off_scale_k) + raw * kBlk + row0;
@@ -263,7 +269,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             to += 2 * kRows * 128;
             key += 2 * kRows;
         }
-        mbar_arrive_warp(BAR((V ? B_RAWVEMPTY : B_RAWKEMPTY) + raw), lane);
+        mbar_arrive_warp(BAR((V ? B_RAWVEMPTY : B_RAWKEMPTY) + raw_g % RB), lane);
         fence_proxy_async();
         mbar_arrive_warp(BAR((V ? B_VFULL : B_KFULL) + st), lane);
         return true;
@@ -362,14 +368,14 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         for (int x = 0; x < S::NBOX; ++x) tma_load_4d_elect(sQ(s) + x * S::BOX, &tmQ, BAR(B_QFULL + s), x * 64, 0, hk, tok0);
                     }
                     for (int t = 0; t < T; ++t, ++gk) {
-                        constexpr int R = E4M3 ? S::NRK : NS;
-                        const int st = gk % R, ug = gk / R, own = pages;
+                        constexpr int R = E4M3 ? S::NRK : NS, RB = E4M3 ? S::NBK : NS;
+                        const int st = gk % R, own = pages;
                         if (t + 1 < T) pages = pages_of(row_of_table, key_block(tile0 + t + 1, border, skip), len);
-                        if (ug > 0) ok = mbar_wait_warp(BAR((E4M3 ? B_RAWKEMPTY : B_KEMPTY) + st), (ug - 1) & 1, ab, ST_WAIT_TIMEOUT + 1);
+                        if (gk >= R) ok = mbar_wait_warp(BAR((E4M3 ? B_RAWKEMPTY : B_KEMPTY) + (gk - R) % RB), ((gk - R) / RB) & 1, ab, ST_WAIT_TIMEOUT + 1);
                         if (!ok) return false;
                         if constexpr (E4M3)
                             load_raw(&tmK, sbase + S::off_raw_k + uint32_t(st) * S::RAW, p.k_scales + hk * p.k_scale_h, p.k_scale_p, sbase + S::off_scale_k + uint32_t(st) * kBlk,
-                                     BAR(B_RAWK + st), own, key_block(tile0 + t, border, skip), hk, len);
+                                     BAR(B_RAWK + gk % RB), own, key_block(tile0 + t, border, skip), hk, len);
                         else
                             load(&tmK, sK(st), BAR(B_KFULL + st), own, key_block(tile0 + t, border, skip), hk, len);
                     }
@@ -409,14 +415,14 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 const int32_t* const row_of_table = p.table + seq * p.table_stride;
                 int pages = T > 0 ? pages_of(row_of_table, key_block(lo, border, skip), len) : 0;
                 for (int t = 0; t < T; ++t, ++gv) {
-                    constexpr int R = E4M3 ? S::NRV : NS;
-                    const int st = gv % R, ug = gv / R, own = pages;
+                    constexpr int R = E4M3 ? S::NRV : NS, RB = E4M3 ? S::NBV : NS;
+                    const int st = gv % R, own = pages;
                     if (t + 1 < T) pages = pages_of(row_of_table, key_block(lo + t + 1, border, skip), len);
-                    if (ug > 0) ok = mbar_wait_warp(BAR((E4M3 ? B_RAWVEMPTY : B_VEMPTY) + st), (ug - 1) & 1, ab, ST_WAIT_TIMEOUT + 2);
+                    if (gv >= R) ok = mbar_wait_warp(BAR((E4M3 ? B_RAWVEMPTY : B_VEMPTY) + (gv - R) % RB), ((gv - R) / RB) & 1, ab, ST_WAIT_TIMEOUT + 2);
                     if (!ok) break;
                     if constexpr (E4M3)
                         load_raw(&tmV, sbase + S::off_raw_v + uint32_t(st) * S::RAW, p.v_scales + hk * p.v_scale_h, p.v_scale_p, sbase + S::off_scale_v + uint32_t(st) * kBlk,
-                                 BAR(B_RAWV + st), own, key_block(lo + t, border, skip), hk, len);
+                                 BAR(B_RAWV + gv % RB), own, key_block(lo + t, border, skip), hk, len);
                     else
                         load(&tmV, sV(st), BAR(B_VFULL + st), own, key_block(lo + t, border, skip), hk, len);
                 }
@@ -476,7 +482,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         for (int kk = 0; kk < 8; ++kk)
                             umma_ts(tO, tP + uint32_t(kk) * 8u, smem_desc_at(desc_v, v_tile + uint32_t(kk) * 2048u), idesc_pv,
                                     (t > 1 || kk > 0) ? 1u : 0u);
-                        umma_commit(BAR(B_VEMPTY + st));
+                        umma_commit(BAR(B_VEMPTY + g % S::NVE));
                         umma_commit(BAR(B_PVDONE + g % NP));
                         if (t + 2 >= T) {  // the chain's last tile
                             umma_commit(BAR(B_OFULL + w));
@@ -804,6 +810,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         int G = 0;      // tiles of all earlier items
         int raw_g = 0;  // E4M3: those counted that are multiplied directly
         int direct = 0; // E4M3: items of that kind
+        bool was_direct = false;  // the item before
         for (int k = 0; alive; ++k) {
             const int s = k % NQ, use = k / NQ;
             alive = mbar_wait_warp(BAR(B_ITEMFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 12);
@@ -865,6 +872,12 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             float slope = 0.f;
             if constexpr (SCORED) {
                 if (p.score.slopes) slope = p.score.slopes[int64_t(it[I_HEAD]) * p.G + g_row] * kScoreLog2e;
+            }
+            if constexpr (E4M3 && !DIRECT) {
+                // Which group has a ring's even tiles can change with the kind of the items: all of the tiles before have to be done with.
+                if (k > 0 && is_direct(tokens) != was_direct) alive = mbar_wait_warp(BAR(B_MLFULL + (k - 1) % NQ), ((k - 1) / NQ) & 1, ab, ST_WAIT_TIMEOUT + 23);
+                if (!alive) break;
+                was_direct = is_direct(tokens);
             }
             const int item_raw = raw_g;
             raw_g += T;
@@ -961,7 +974,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                             float k_scale[U][2];
                             uint32_t xv[U][4][D / 32], v_scale[U][2];  // keys 16 u + 2 c4, + 1, + 8, + 9; columns from g8 * D / 8 on
                             auto take_values = [&] {
-                                if (!mbar_wait_warp(BAR(B_RAWV + rv), (gr / S::NRV) & 1, ab, ST_WAIT_TIMEOUT + 20)) return false;
+                                if (!mbar_wait_warp(BAR(B_RAWV + gr % S::NBV), (gr / S::NBV) & 1, ab, ST_WAIT_TIMEOUT + 20)) return false;
                                 const uint8_t* const from = smem + S::off_raw_v + rv * S::RAW;
 #pragma unroll
                                 for (int u = 0; u < U; ++u) {
@@ -979,10 +992,10 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
                                     for (int i = 0; i < 2; ++i) v_scale[u][i] = *reinterpret_cast<const uint16_t*>(smem + S::off_scale_v + rv * kBlk + mine + 16 * u + 2 * c4 + 8 * i);
                                 }
-                                if (give_back) mbar_arrive_warp(BAR(B_RAWVEMPTY + rv), lane);
+                                if (give_back) mbar_arrive_warp(BAR(B_RAWVEMPTY + gr % S::NBV), lane);
                                 return true;
                             };
-                            if (!mbar_wait_warp(BAR(B_RAWK + rk), (gr / S::NRK) & 1, ab, ST_WAIT_TIMEOUT + 20)) return false;
+                            if (!mbar_wait_warp(BAR(B_RAWK + gr % S::NBK), (gr / S::NBK) & 1, ab, ST_WAIT_TIMEOUT + 20)) return false;
                             {
                                 const uint8_t* const from = smem + S::off_raw_k + rk * S::RAW;
 #pragma unroll
@@ -995,7 +1008,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                                         k_scale[u][j] = scale_to_float(smem[S::off_scale_k + rk * kBlk + mine + 16 * u + 8 * j + g8]);
                                     }
                                 }
-                                if (give_back) mbar_arrive_warp(BAR(B_RAWKEMPTY + rk), lane);
+                                if (give_back) mbar_arrive_warp(BAR(B_RAWKEMPTY + gr % S::NBK), lane);
                             }
                             if (NT == 1 && !take_values()) return false;
                             float sc[NT][U][4] = {};
