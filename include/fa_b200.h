@@ -201,7 +201,8 @@ typedef struct fa_window {
 } fa_window;
 
 /* The four of a call with a window (scores may be NULL, window NULL or of 0 keys is a call without one). The plan of a call with ids must have been built with the
- * same window; fa_fwd_splits_windowed says into how many runs the keys that are left are best cut; fa_fwd_rest serves these forwards, too. */
+ * same window; fa_fwd_splits_windowed says into how many runs the keys that are left are best cut (in a call with a prefix, which may
+ * show any of the others, ask it with window NULL); fa_fwd_rest serves these forwards, too. */
 int fa_plan_build_windowed(const fa_problem* p, const fa_scores* scores, const fa_window* window, const fa_ids* eq, const fa_ids* ek, void* plan,
                            size_t plan_bytes, int32_t* status, void* stream);
 int fa_fwd_splits_windowed(const fa_problem* p, const fa_window* window);

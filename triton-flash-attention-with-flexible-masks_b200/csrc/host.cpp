@@ -131,7 +131,8 @@ Outputs launch_forward(const fa_problem& p, const Tensor& q, const Tensor& k, co
     if (!taken_as_is(r.o)) r.o = at::empty(q.sizes(), q.options());
     const auto f32 = q.options().dtype(at::kFloat);
     r.lse = at::empty({p.B, p.H, fa_padded_rows(p.M)}, f32);
-    r.splits = key_runs != 0 ? key_runs : fa_fwd_splits_windowed(&p, window);  // (a number below 1 is the library's to refuse)
+    // (a number below 1 is the library's to refuse; a prefix may show keys that the window would hide)
+    r.splits = key_runs != 0 ? key_runs : fa_fwd_splits_windowed(&p, scores && scores->prefix ? nullptr : window);
     Tensor work;
     size_t bytes = 0;
     if (r.splits > 1) {

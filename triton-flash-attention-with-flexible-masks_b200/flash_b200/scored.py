@@ -127,7 +127,8 @@ class ScoredAttention(torch.autograd.Function):
             if maybe_contiguous(out) is not out:
                 out = torch.empty((B, H, M, D), dtype=q.dtype, device=device)
             lse = torch.empty((B, H, lib.fa_padded_rows(M)), dtype=torch.float32, device=device)
-            splits, work, size = lib.fa_fwd_splits_windowed(prob, window), None, ctypes.c_size_t(0)
+            # (a prefix may show keys that the window would hide)
+            splits, work, size = lib.fa_fwd_splits_windowed(prob, window if prefix is None else None), None, ctypes.c_size_t(0)
             if splits > 1:
                 _lib.check(lib.fa_fwd_workspace_bytes(prob, splits, size), "fa_fwd_workspace_bytes")
                 work = torch.empty(size.value // 4, dtype=torch.float32, device=device)
