@@ -107,6 +107,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
     using S = FwdSmem<D>;
     constexpr bool PREFIX = KIND != SCORE_PLAIN, SCORED = score_changed(KIND), WINDOW = (KIND & SCORE_WINDOW) != 0;  // perhaps a prefix; other scores
     constexpr int SCORES = KIND & SCORE_CAPPED_BIAS;
+    constexpr bool BIASED = (SCORES & SCORE_BIAS) != 0;  // a window or scattered ids may leave tiles out, so that a tile's biases are far from those before (tile_reference)
     constexpr int NS = S::NS, NQ = S::NQ, NP = S::NP;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem);
@@ -710,11 +711,13 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                 // A capped tile without a mask is not capped before its exponentials: the greatest score tells the greatest capped one, and the polynomial
                 // runs beside the special-function unit. (With a bias the greatest one has to be looked for behind it.)
                 bool late = false;
+                float ref = m_run == -INFINITY ? 0.f : m_run;  // SCORED: what the scores are relative to
                 if constexpr (SCORED) {
                     const int first = SHORT ? 0 : qb * kBlk, last = SHORT ? mk.M - 1 : qb * kBlk + kBlk - 1;  // rows of the tile, and perhaps more
                     const Bias bias(slope, mk.causal && front == 0, first + mk.gap - (k0 + kBlk - 1), last + mk.gap - k0);
                     if constexpr (SCORES == SCORE_CAPPED) late = !(fl & (TILE_BOUND | TILE_DOC)) && !any_beyond<kBlk>(sc, valid ? p.score.most : INFINITY);
-                    if (!late) score_row<SCORES, kBlk>(sc, p.score, bias, p.scale_log2, row + mk.gap - k0, valid, m_run == -INFINITY ? 0.f : m_run);
+                    if constexpr (BIASED) ref = tile_reference(bias, ref, row + mk.gap - k0 - kBlk / 2);
+                    if (!late) score_row<SCORES, kBlk>(sc, p.score, bias, p.scale_log2, row + mk.gap - k0, valid, ref);
                 }
 
                 if (fl & (TILE_BOUND | TILE_DOC)) {
@@ -770,11 +773,14 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                 float m_new = fmaxf(m_run, mx);
                 // lazy rescale: keep the old reference point while the new maximum is within 2^8 of it
                 bool need = (m_new - m_run) * c > 8.0f;
-                if constexpr (SCORED) {  // (the scores, and mx, are relative to the old reference point, or to 0 in front of a row's first key)
+                float move = 0.f;  // SCORED: from `ref` to the reference point
+                if constexpr (SCORED) {  // (the scores, and mx, are relative to `ref`: the old reference point, or 0 in front of a row's first key, or BIASED perhaps the tile's own)
                     const bool fresh = m_run == -INFINITY;
-                    if (late) mx = cap_one(mx, p.score) - (fresh ? 0.f : m_run);
-                    need = fresh ? mx != -INFINITY : mx > 8.0f;
-                    m_new = (fresh ? 0.f : m_run) + mx;
+                    if (late) mx = cap_one(mx, p.score) - ref;
+                    if (BIASED && !fresh) move = ref - m_run;
+                    need = fresh ? mx != -INFINITY : mx + move > 8.0f;
+                    m_new = ref + mx;
+                    if (need) move = BIASED ? ref - m_new : -mx;
                 }
                 if (!need) m_new = m_run;
                 if (S::POWN) {  // this tile's P overwrites that one's
@@ -782,11 +788,10 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                     if (!alive) break;
                     tc_fence_after();
                 }
-                if (__any_sync(0xffffffffu, need)) {
+                if (__any_sync(0xffffffffu, need || (BIASED && move != 0.f))) {
                     if (SCORED && !late) {
-                        const float less = need ? -mx : 0.f;
 #pragma unroll
-                        for (int x = 0; x < 128; x += 2) unpack_f2(add_f2(pack_f2(sc[x], sc[x + 1]), pack_f2(less, less)), sc[x], sc[x + 1]);
+                        for (int x = 0; x < 128; x += 2) unpack_f2(add_f2(pack_f2(sc[x], sc[x + 1]), pack_f2(move, move)), sc[x], sc[x + 1]);
                     }
                     const float alpha = need ? fast_exp2((m_run - m_new) * c) : 1.0f;
                     l_run *= alpha;
@@ -794,7 +799,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                         most *= alpha;
                         lost *= alpha;
                     }
-                    if (t > t0) {
+                    if (t > t0 && (!BIASED || __any_sync(0xffffffffu, need))) {
                         if (!S::POWN) {
                             alive = pv_before();
                             if (!alive) break;
@@ -817,7 +822,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUte
                 m_run = m_new;
                 const float mneg = (m_run == -INFINITY) ? 0.f : -m_run * c;
                 if constexpr (KIND != SCORE_PLAIN) {
-                    const float greatest_p = fast_exp2(!SCORED ? fmaf(mx, c, mneg) : need ? 0.f : mx);
+                    const float greatest_p = fast_exp2(!SCORED ? fmaf(mx, c, mneg) : BIASED ? mx + move : need ? 0.f : mx);
                     if (greatest_p > most) {
                         float rounded, none;
                         unpack2<BF16>(pack2<BF16>(greatest_p, 0.f), rounded, none);

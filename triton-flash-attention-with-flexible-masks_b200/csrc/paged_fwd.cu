@@ -127,6 +127,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     using S = PagedSmem<D, FORM>;
     constexpr bool SCORED = score_changed(KIND), MASKED = (FORM & FORM_MASKED) != 0, E4M3 = S::E4M3, DIRECT = S::DIRECT;
     constexpr bool PBF16 = BF16 && !E4M3;           // the products' type
+    constexpr bool BIASED = MASKED && (KIND & SCORE_BIAS) != 0;  // a tile's biases may be far from those before (tile_reference); without a window the keys of a piece lie side by side
     // (spilled registers come back from L2 here: shared memory leaves L1 nothing)
     constexpr int kSoftmaxRegs = DIRECT ? 192 : E4M3 ? 176 : kFwdSoftmaxRegs, kEpilogueRegs = DIRECT ? 64 : E4M3 ? 104 : kFwdEpilogueRegs, kServiceRegs = DIRECT ? 64 : E4M3 ? 56 : kFwdServiceRegs;
     static_assert(256 * kSoftmaxRegs + 128 * (kEpilogueRegs + kServiceRegs) <= kFwdThreads * 128, "registers at launch");
@@ -1203,6 +1204,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         mbar_arrive_warp(BAR(B_SFREE + w), lane);
                     }
                     float* v = reinterpret_cast<float*>(sq);
+                    float ref = m_run == -INFINITY ? 0.f : m_run;  // SCORED: as below
                     if constexpr (SCORED) {
                         if (E4M3 && BF16 && __any_sync(0xffffffffu, factor != 1.f)) {
 #pragma unroll
@@ -1217,7 +1219,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                             for (int x = 0; x < 32; ++x) v[x] = x + 32 * quarter >= none_from && x + 32 * quarter < none_end ? 0.f : v[x];
                         }
                         const Bias bias(slope, front == 0, pos0 - (kq + 31), pos0 + 31 - kq);
-                        score_row<KIND, 32>(v, p.score, bias, p.scale_log2, pos - kq, valid, (m_run == -INFINITY ? 0.f : m_run) - kRaised);
+                        if constexpr (BIASED) ref = tile_reference(bias, ref, pos - kq - 16);
+                        score_row<KIND, 32>(v, p.score, bias, p.scale_log2, pos - kq, valid, ref - kRaised);
                     }
                     if (MASKED ? masked() : kq + 31 > all_see) {
                         const uint32_t keep = sees(kq);
@@ -1238,10 +1241,13 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     if constexpr (E4M3 && SCORED) top -= kRaised;
                     float m_new = fmaxf(m_run, top);
                     bool need = (m_new - m_run) * c > 8.0f;
+                    float move = 0.f;
                     if constexpr (SCORED) {
                         const bool fresh = m_run == -INFINITY;
-                        need = fresh ? top != -INFINITY : top > 8.0f;
-                        m_new = (fresh ? 0.f : m_run) + top;
+                        if (BIASED && !fresh) move = ref - m_run;
+                        need = fresh ? top != -INFINITY : top + move > 8.0f;
+                        m_new = ref + top;
+                        if (need) move = BIASED ? ref - m_new : -top;
                     }
                     if (!need) m_new = m_run;
                     const bool scale_o = __any_sync(0xffffffffu, need) && t > t0;
@@ -1254,8 +1260,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     l_run *= alpha;
                     if (scale_o) rescale(alpha);
                     m_run = m_new;
-                    // (SCORED: what is left to be subtracted)
-                    const float mneg = SCORED ? (need ? -top : 0.f) : (m_run == -INFINITY) ? 0.f : E4M3 ? kRaised - m_run * c : -m_run * c;
+                    // (SCORED: what is left to be added)
+                    const float mneg = SCORED ? move : (m_run == -INFINITY) ? 0.f : E4M3 ? kRaised - m_run * c : -m_run * c;
                     float l4[4] = {0.f, 0.f, 0.f, 0.f};
                     uint32_t pk[16];
 #pragma unroll
@@ -1291,6 +1297,7 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 // A capped tile without a mask is not capped before its exponentials: the greatest score tells the greatest capped one, and the polynomial
                 // runs beside the special-function unit. (With a bias the greatest one has to be looked for behind it.)
                 bool late = false;
+                float ref = m_run == -INFINITY ? 0.f : m_run;  // SCORED: what the scores are relative to
                 if constexpr (SCORED) {
                     if (E4M3 && BF16 && __any_sync(0xffffffffu, factor != 1.f)) {
 #pragma unroll
@@ -1307,7 +1314,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
                     const Bias bias(slope, front == 0, pos0 - (k0 + kBlk - 1), pos0 + kBlk - 1 - k0);
                     if constexpr (KIND == SCORE_CAPPED) late = !masked() && !any_beyond<kBlk>(sc, valid ? p.score.most : INFINITY);
-                    if (!late) score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, pos - k0, valid, (m_run == -INFINITY ? 0.f : m_run) - kRaised);
+                    if constexpr (BIASED) ref = tile_reference(bias, ref, pos - k0 - kBlk / 2);
+                    if (!late) score_row<KIND, kBlk>(sc, p.score, bias, p.scale_log2, pos - k0, valid, ref - kRaised);
                 }
                 if (masked()) {
 #pragma unroll
@@ -1333,12 +1341,15 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 float m_new = fmaxf(m_run, mx);
                 // lazy rescale: keep the old reference point while the new maximum is within 2^8 of it
                 bool need = (m_new - m_run) * c > 8.0f;
-                if constexpr (SCORED) {  // (the scores, and mx, are relative to the old reference point, or to 0 in front of a row's first key)
+                float move = 0.f;  // SCORED: from `ref` to the reference point
+                if constexpr (SCORED) {  // (the scores, and mx, are relative to `ref`: the old reference point, or 0 in front of a row's first key, or BIASED perhaps the tile's own)
                     const bool fresh = m_run == -INFINITY;
-                    if (late) mx = cap_one(mx, p.score) - (fresh ? 0.f : m_run);
+                    if (late) mx = cap_one(mx, p.score) - ref;
                     else if constexpr (E4M3) mx -= kRaised;
-                    need = fresh ? mx != -INFINITY : mx > 8.0f;
-                    m_new = (fresh ? 0.f : m_run) + mx;
+                    if (BIASED && !fresh) move = ref - m_run;
+                    need = fresh ? mx != -INFINITY : mx + move > 8.0f;
+                    m_new = ref + mx;
+                    if (need) move = BIASED ? ref - m_new : -mx;
                 }
                 if (!need) m_new = m_run;
                 if (S::POWN) {  // this tile's P overwrites that one's
@@ -1346,15 +1357,14 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     if (!alive) break;
                     tc_fence_after();
                 }
-                if (__any_sync(0xffffffffu, need)) {
+                if (__any_sync(0xffffffffu, need || (BIASED && move != 0.f))) {
                     if (SCORED && !late) {
-                        const float less = need ? -mx : 0.f;
 #pragma unroll
-                        for (int x = 0; x < 128; x += 2) unpack_f2(add_f2(pack_f2(sc[x], sc[x + 1]), pack_f2(less, less)), sc[x], sc[x + 1]);
+                        for (int x = 0; x < 128; x += 2) unpack_f2(add_f2(pack_f2(sc[x], sc[x + 1]), pack_f2(move, move)), sc[x], sc[x + 1]);
                     }
                     const float alpha = need ? fast_exp2((m_run - m_new) * c) : 1.0f;
                     l_run *= alpha;
-                    if (t > t0) {
+                    if (t > t0 && (!BIASED || __any_sync(0xffffffffu, need))) {
                         if (!S::POWN) {
                             alive = pv_before();
                             if (!alive) break;

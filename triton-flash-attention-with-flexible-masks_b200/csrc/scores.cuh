@@ -151,6 +151,16 @@ struct Bias {
     }
 };
 
+// What a tile's biased scores are computed relative to: the row's running reference point, `run`, but where the bias of the tile's middle, at distance `mid`, is far from it, that bias. (After
+// a sequence's first keys, or the beginning of a scattered document, come keys whose biases are thousands away: relative to the old point each step along the row would round at that size.
+// bf16, 30000 keys, window 100, slopes up to 0.84: rows off by 3.6 times what P's rounding allows.) The caller moves the scores by the two points' distance when it knows their maximum. What it
+// costs where no tile is far: steps of 16 x 8 heads x 577 x 32 without a causal mask 130.0 -> 130.9 us, of 16 heads x 8111 x 128 in documents, capped, 702 -> 708.
+constexpr float kFarReference = 256.f;
+__device__ __forceinline__ float tile_reference(const Bias& bias, float run, int mid) {
+    const float own = bias.line * float(mid);
+    return bias.s != 0.f && fabsf(own - run) > kFarReference && fabsf(own) < INFINITY ? own : run;
+}
+
 // v[x] = f(v[x], x) for the N values of a thread, kStep at a time, in a loop that moves them all on: for what is rarely done. Unrolled, it would be most of the
 // code of the softmax warps, which is fetched again and again.
 template <int N, int kStep, class F>
