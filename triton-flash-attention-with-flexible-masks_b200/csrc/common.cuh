@@ -174,7 +174,7 @@ __device__ __forceinline__ uint32_t classify_from_plan(const MaskArgs& a, int b,
 }
 
 // Key-block range [lo, hi) a query block has to walk.
-template <bool kPrefix = false, bool kWindow = false>
+template <bool kPrefix = false>
 __device__ __forceinline__ void kv_range(const MaskArgs& a, int b, int he, int qb, int& lo, int& hi) {
     if (a.mode == 1 && !(a.debug & DBG_NO_SKIP)) {
         const int64_t bh = int64_t(b) * a.He + he;
@@ -200,7 +200,7 @@ template <bool kPrefix, bool kWindow>
 __device__ __forceinline__ KeyWalk kv_walk(const MaskArgs& a, int b, int he, int qb) {
     KeyWalk w;
     int hi;
-    kv_range<kPrefix, kWindow>(a, b, he, qb, w.lo, hi);
+    kv_range<kPrefix>(a, b, he, qb, w.lo, hi);
     w.border = hi;
     w.skip = 0;
     w.n = hi - w.lo;
