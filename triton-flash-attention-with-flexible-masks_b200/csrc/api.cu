@@ -434,8 +434,9 @@ int run_bwd_delta(const fa_problem* p, const void* rest, const fa_tensor* o, con
 
 // Into how many runs of queries dK / dV of the blocks with a window's first keys are cut, which every query sees something of: a run is as long as the others' walks, or as half of an SM's
 // share of all the work, whichever is more. (Without the share many first keys, which make work enough by themselves, would ask for a workspace of gigabytes; with it a GPU's SMs have
-// about four blocks of sums each.) With `early` such blocks. us, 2 x 16 / 4 heads x 4000 x 128, window 1024, 4 first keys, forward and backward, whole | cut 416 | 317 (without first
-// keys 283).
+// about four blocks of sums each.) With `early` such blocks. us, 2 x 16 / 4 heads x 4000 x 128, window 1024, 4 first keys, forward and backward, long series, whole | cut 435 | 368 (without
+// first keys 337). The blocks of a prefix, which all queries see as well, are not among them: its length is on the device. A prefix of 4 | 128 | 500 keys there 426 | 413 | 464, as many first
+// keys 362 | 360 | 429.
 int query_runs(const fa_problem* p, const fa_window& w, int sms, int& early) {
     early = 0;
     if (w.keys <= 0 || w.sinks <= 0 || !p->causal) return 1;

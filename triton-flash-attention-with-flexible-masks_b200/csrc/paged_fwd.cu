@@ -32,7 +32,9 @@ namespace fa {
 
 // Instances. FORM_MASKED: perhaps a window, perhaps drafted tokens whose parents are given. A tile of keys that the window hides from all of an item's tokens is not among its
 // tiles, and what lies in such keys of the others is as far from the results as what lies behind the sequence: V's rows are zeroed, scores masked. A drafted token's branch is
-// walked once an item, by the thread of each of its rows, while the first keys are on their way, and left as bits in shared memory.
+// walked once an item, by the thread of each of its rows, and left as bits in shared memory: a load for each step, each behind the one before (with a window twice, first for the depth), which
+// the first keys' way here hides of shallow trees alone. 16 sequences, 32 / 8 heads of 128, 60 new tokens behind 4000, us, a star | a chain 123 | 125; 256 new tokens 344 | 422, with a window of 512
+// 168 | 284; one sequence, 256 behind 1200, 28 | 39 and 27 | 56.
 // FORM_E4M3: the cache is of 8 bits. The rows of K and V land as they are in rings of their own, with their scales; each tile is turned
 // into the fp16 tile that the products read (a row is e4m3 times a power of two from 2^-15 to 2^7, all of whose numbers are fp16's: nothing is rounded), with hidden rows as zeros: K's by the epilogue
 // group, which has nothing to do while an item lasts, V's by the softmax group that owns the tile. The products are fp16's also where q is bf16: q's rows are brought to fp16, by a power of two where their greatest entry asks for it (their scores take it back in fp32),
@@ -221,7 +223,8 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     auto sV = [&](int s) { return sbase + S::off_v + uint32_t(s) * S::TILE; };
     // E4M3: the g-th tile of K or V (the rings' raw_g-th), rows of D numbers in e4m3 to 64-column boxes of fp16 with the swizzle that the products read, by four warps. A thread takes 16
     // numbers at a time. In a loop, and in one place of the code for K and one for V: with the loop unrolled and V's in three places, whose code the softmax groups fetch beside their own, warps
-    // stood without an instruction more than anything else (three chunks of up to 500 and five tokens over 131 MB, 32 / 8 heads of 128, 525 us for 318).
+    // stood without an instruction more than anything else. Three chunks of up to 500 and five tokens over 131 MB, 32 / 8 heads of 128: 333 us, capped 466, where 16 bits take 211 and 294: each item
+    // converts all its keys for itself, a chunk of 500 tokens with four heads a kv head 16 times.
     auto unpack_tile = [&](auto values, int g, int raw_g, int k0, int seen, int early, int low) {
         constexpr bool V = decltype(values)::value;
         const int r = tid & 127;

@@ -31,8 +31,9 @@ enum : int {
     SCORE_CAPPED_BIAS = SCORE_BIAS | SCORE_CAPPED,
     SCORE_PREFIX = 4,  // a prefix alone: the scores are attention's
     // A window, and perhaps a prefix, with or without the changes above. What it costs is that tiles at both ends
-    // of a window are masked: 2 x 16 / 4 heads x 4000 x 128, bf16, forward | forward and backward, us, causal
-    // 114 | 483; window 1024 70 | 284, with 4 first keys 77 | 317; window 2048 with 4 first keys 99 | 423.
+    // of a window, and those of the first keys, take as long as whole ones: 2 x 16 / 4 heads x 4000 x 128, bf16, forward |
+    // forward and backward, us, long series of calls under the power cap, causal 138 | 580; window 1024 81 | 337, with 4
+    // first keys 87 | 368; window 2048 with 4 first keys 123 | 513.
     SCORE_WINDOW = 8,
 };
 // Does an instance change the scores?

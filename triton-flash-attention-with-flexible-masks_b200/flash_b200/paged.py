@@ -98,7 +98,7 @@ def paged_append(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None, k_s
 
     k_scales, v_scales: float8_e8m0fnu [pages, Hk, page size]; k_pages and v_pages are then float8_e4m3fn, with pages of 16 tokens at least, and a head's row x of a token is quantised as it
     is written: to the numbers of e4m3 nearest to x / s (ties to even, 448 at most), and the scale s = 2^e with the least e from -15 to 7 for which the largest finite |x| is at most
-    448 s. A row stands for its numbers times its scale. What is not finite becomes a NaN. Where two rows go to one place their parts may mix.
+    448 s. A row stands for its numbers times its scale. What is not finite becomes a NaN, a number beyond 448 * 2^7 = 57344 becomes that. Where two rows go to one place their parts may mix.
 
     There is no derivative through the cache: under autograd, tensors that ask for a gradient are refused, and so are dual tensors of forward mode.
 

@@ -178,7 +178,7 @@ def attention_scored(q, k, v, causal=False, sm_scale=None, eq=None, ek=None, sco
 
     takes the place of s before the softmax, and a key j < prefix[b] is visible to every query of sequence b whatever the causal mask says (the
     ids' rule holds for it as for the others). With a window a query sees, of the keys that the causal mask shows it, the last `window` (its own among them:
-    i + gap - j < window) and the first `sinks` of the sequence (j < sinks); a prefix and the ids' rule hold as they do without one. Blocks of keys that the window
+    i + gap - j < window) and the first `sinks` of the sequence (j < sinks; of a row of packed documents these are the first document's, which the ids hide from the others); a prefix and the ids' rule hold as they do without one. Blocks of keys that the window
     hides from a block of queries cost nothing, forward and backward.
 
     softcap: None or 0 for none, else from 1e-6 to 1e6. slopes: float32 [H], None for none. prefix: int32 or int64 [bs], None for none; it
