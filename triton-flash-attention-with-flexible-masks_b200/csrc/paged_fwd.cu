@@ -633,11 +633,14 @@ paged_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     continue;
                 }
                 if constexpr (BF16) {
-                    alive = mbar_wait_warp(BAR(B_QFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 17);
-                    if (!alive) break;
-                    factor = fminf(query_to_fp16(s) * p.lift, 3e38f);
-                    reinterpret_cast<float*>(smem + S::off_factor)[s * kBlk + r] = factor;
-                    fence_proxy_async();
+                    // (not of an item without tiles: there no product waits until all four warps have done so, and the first of them would stage its zeros where the others' rows of Q are)
+                    if (T > 0) {
+                        alive = mbar_wait_warp(BAR(B_QFULL + s), use & 1, ab, ST_WAIT_TIMEOUT + 17);
+                        if (!alive) break;
+                        factor = fminf(query_to_fp16(s) * p.lift, 3e38f);
+                        reinterpret_cast<float*>(smem + S::off_factor)[s * kBlk + r] = factor;
+                        fence_proxy_async();
+                    }
                     mbar_arrive_warp(BAR(B_QREADY + s), lane);
                 }
                 const int pos0 = it[I_POS], len = it[I_LEN], front = it[I_FRONT], lo = it[I_LO], border = it[I_BORDER], skip = it[I_SKIP];
